@@ -233,6 +233,175 @@ CASCADE_API int cascade_suffix_decode_noalloc(const cascade_paged_attn_t *p, voi
 CASCADE_API int cascade_probe_hbm_read(const void *src, size_t bytes, int32_t mode, int64_t row_bytes, uint32_t *sink,
                                        size_t sink_words, cascade_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Paged latent cache: attention whose keys and values of all heads come from
+ * one latent vector per token, the pages of such a cache, and the
+ * verification of drafted tokens against the target model's probabilities.
+ * (No counterpart in the reference.)
+ * ------------------------------------------------------------------------ */
+
+/* Latent attention, absorbed form. A token's cache row holds latent_dim = 512
+ * latent values followed by rope_dim = 64 rotary key values; a query row holds
+ * the head's query already multiplied by its key up-projection (512 values)
+ * and its rotary part (64). For query token i of a request with q_len query
+ * tokens and kv_len cached tokens (its own included), head h:
+ *   s_t = scale * <query[i,h], cache[t]>,  t < kv_len, and with causal != 0
+ *         t <= kv_len - q_len + i
+ *   out[i,h] = sum_t softmax(s)_t cache[t][0:512],  lse[i,h] = ln sum_t exp(s_t)
+ * Rows that see no token (kv_len 0, or causal with kv_len < q_len - i) give
+ * out = 0 and lse = -inf. What the pages hold past kv_len is never used, NaN
+ * or infinities included.
+ *   query  [num_tokens, num_heads, 576], contiguous, 16-byte aligned
+ *   cache  [num_blocks, block_size, 576], contiguous, 16-byte aligned
+ *   block_table int32 [batch, block_cols]; kv lengths are cut to
+ *          block_cols * block_size
+ *   actual_q_seqlens / actual_kv_seqlens int64 [batch], device memory;
+ *          q_seqlen_value > 0: every request has that many query tokens
+ *          (actual_q_seqlens may be NULL); 0: read from actual_q_seqlens on
+ *          the device. Their sum must be num_tokens: this is not checked, but
+ *          nothing outside the tensors is read or written if it is not.
+ * Neither path reads back to the host, so both can be captured in a graph.
+ * A block id outside [0, num_blocks) reads as zeros and sets (word & 2) of
+ * cascade_device_error(). */
+typedef struct cascade_latent_attn {
+  const void *query;
+  const void *cache;
+  const int32_t *block_table;
+  const int64_t *actual_q_seqlens;
+  const int64_t *actual_kv_seqlens;
+  int64_t num_tokens;
+  int64_t num_heads;
+  int64_t latent_dim; /* 512 */
+  int64_t rope_dim;   /* 64 */
+  int64_t num_blocks;
+  int64_t block_size; /* 16, 32, 64, 128, 256 or 512 */
+  int64_t batch;
+  int64_t block_cols;
+  int64_t q_seqlen_value;
+  float scale;
+  int32_t causal;
+  int32_t dtype; /* CASCADE_BF16 or CASCADE_FP16: query, cache and out */
+  int32_t flags; /* 0 or CASCADE_FLAG_DEBUG_STALL */
+} cascade_latent_attn_t;
+
+/* out: [num_tokens, num_heads, 512] in p->dtype; lse: fp32 [num_tokens * num_heads]
+ * (natural log, the compact layout cascade_lse_merge takes with stride 1). */
+CASCADE_API size_t cascade_latent_decode_workspace_size(const cascade_latent_attn_t *p);
+CASCADE_API int cascade_latent_decode(const cascade_latent_attn_t *p, void *out, float *lse, void *workspace,
+                                      size_t workspace_bytes, cascade_stream_t stream);
+
+/* Latent attention, expanded form, for prompts and chunks of prompts: every
+ * head's key (128 values) and value (128) have been expanded from the latents,
+ * the 64 rotary key values are shared by all heads. Sequence b owns query
+ * tokens [cu_q[b], cu_q[b+1]) and key tokens [cu_kv[b], cu_kv[b+1]);
+ * with n query and m key tokens, query i sees keys t < m, and with causal != 0
+ * t <= m - n + i (the last query sees every key).
+ *   s_t = scale * (<query[i,h,0:128], key[t,h]> + <query[i,h,128:192], key_rope[t]>)
+ * Rows that see no key give out = 0 and lse = -inf.
+ *   query     [num_tokens, num_heads, 192], contiguous
+ *   key       [num_kv, num_heads, 128], strides in elements, last dim contiguous
+ *   key_rope  [num_kv, 64], token stride in elements, last dim contiguous
+ *   value     [num_kv, num_heads, 128], strides in elements, last dim contiguous
+ *   cu_q_seqlens / cu_kv_seqlens  int64 [batch + 1], device memory, ascending
+ *   max_q_seqlen  at least the longest sequence's query tokens
+ * All pointers 16-byte aligned, all strides multiples of 8 elements. */
+typedef struct cascade_latent_prefill {
+  const void *query;
+  const void *key;
+  const void *key_rope;
+  const void *value;
+  const int64_t *cu_q_seqlens;
+  const int64_t *cu_kv_seqlens;
+  int64_t num_tokens;
+  int64_t num_kv;
+  int64_t num_heads;
+  int64_t batch;
+  int64_t max_q_seqlen;
+  int64_t key_token_stride;
+  int64_t key_head_stride;
+  int64_t rope_token_stride;
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  float scale;
+  int32_t causal;
+  int32_t dtype; /* CASCADE_BF16 or CASCADE_FP16: all four inputs and out */
+  int32_t flags; /* 0 or CASCADE_FLAG_DEBUG_STALL */
+} cascade_latent_prefill_t;
+
+/* out: [num_tokens, num_heads, 128] in p->dtype; lse: fp32 [num_tokens * num_heads]. */
+CASCADE_API int cascade_latent_prefill(const cascade_latent_prefill_t *p, void *out, float *lse,
+                                       cascade_stream_t stream);
+
+/* Pages of a cache. The state is a block table int32 [rows, cols] (-1 where a
+ * row has no page), the rows' lengths int64 [rows] and the pages' reference
+ * counts int32 [num_blocks] (0 = free): row r owns one reference to each of
+ * its first ceil(kv_lens[r] / block_size) pages. The calls read that state and
+ * write the new one beside it (table_out, ...), so a caller keeps two copies
+ * and swaps; only the pools' pages are written in place. A pool is one cache
+ * tensor [num_blocks, block_size, row_bytes] (one per layer, or two for
+ * separate keys and values); `pools` is a HOST array of num_pools device
+ * pointers, 16-byte aligned, with row_bytes a multiple of 16. All other
+ * pointers are device memory. Ids outside [0, num_blocks) are skipped and set
+ * (word & 2) of cascade_device_error(). */
+
+/* pools[*][dst[i]] = pools[*][src[i]], whole pages; a dst may appear once and
+ * must not be a src. */
+CASCADE_API int cascade_page_copy(void *const *pools, int64_t num_pools, int64_t num_blocks, int64_t page_bytes,
+                                  const int64_t *src, const int64_t *dst, int64_t count, cascade_stream_t stream);
+
+/* Child i becomes a copy of row parents[i]: it shares the parent's full pages
+ * (their counts rise by one) and gets a fresh page holding a copy of the
+ * filled rows of a partly filled last page. Fresh pages are the free pages in
+ * ascending order, given to the children in order. A child whose parent is
+ * outside [0, rows), or that finds no free page left, gets a row of -1 and
+ * length -1. child_table: int32 [count, cols]; child_lens: int64 [count];
+ * refs_out: int32 [num_blocks]. */
+CASCADE_API size_t cascade_page_fork_workspace_size(int64_t num_blocks, int64_t count);
+CASCADE_API int cascade_page_fork(void *const *pools, int64_t num_pools, int64_t num_blocks, int64_t block_size,
+                                  int64_t row_bytes, const int32_t *block_table, int64_t rows, int64_t cols,
+                                  const int64_t *kv_lens, const int32_t *page_refs, const int64_t *parents,
+                                  int64_t count, int32_t *child_table, int64_t *child_lens, int32_t *refs_out,
+                                  void *workspace, size_t workspace_bytes, cascade_stream_t stream);
+
+/* Cuts row r to keep_lens[r] tokens (clamped to [0, kv_lens[r]]; 0 frees the
+ * row) and drops its reference to each page it no longer needs. */
+CASCADE_API int cascade_page_free(const int32_t *block_table, int64_t rows, int64_t cols, const int64_t *kv_lens,
+                                  const int32_t *page_refs, int64_t num_blocks, const int64_t *keep_lens,
+                                  int64_t block_size, int32_t *table_out, int64_t *lens_out, int32_t *refs_out,
+                                  cascade_stream_t stream);
+
+/* Moves the live pages (count > 0) to the ids [0, live): the live pages with
+ * ids >= live go, in ascending order, to the free ids below live in ascending
+ * order. The pools' pages are moved, the table and the counts renamed; entries
+ * past a row's pages become -1. live_out: int32 [1]. */
+CASCADE_API size_t cascade_page_compact_workspace_size(int64_t num_blocks);
+CASCADE_API int cascade_page_compact(void *const *pools, int64_t num_pools, int64_t num_blocks, int64_t block_size,
+                                     int64_t row_bytes, const int32_t *block_table, int64_t rows, int64_t cols,
+                                     const int64_t *kv_lens, const int32_t *page_refs, int32_t *table_out,
+                                     int32_t *refs_out, int32_t *live_out, void *workspace, size_t workspace_bytes,
+                                     cascade_stream_t stream);
+
+/* Verification of drafted tokens. Request b drafted draft_lens[b] (0..K)
+ * tokens; target_probs[b][i] is the target's distribution at the place of
+ * draft i (row draft_lens[b]: of the token after the last draft),
+ * draft_probs[b][i] the one draft i was taken from. Draft i is accepted while
+ *   uniform[b][i] * draft_probs[b][i][x] < target_probs[b][i][x],  x = tokens[b][i]
+ * (products in fp32; without draft_probs the factor is 1). The request's last token
+ * is argmax_v left[v] / noise[b][v], lowest index on ties, which samples from
+ * `left` when noise holds independent exponential variates: left =
+ * max(target - draft, 0) of the first refused place (without draft_probs: the
+ * target with the refused token left out), or the target's row draft_lens[b]
+ * if none was refused. If left is 0 everywhere the target's own row stands in.
+ *   tokens int64 [B, K]; draft_lens int64 [B]; draft_probs [B, K, V] or NULL,
+ *   target_probs [B, K+1, V] in `dtype` (any of the three); uniform fp32
+ *   [B, K]; noise fp32 [B, V], positive; out_tokens int64 [B, K+1]: the
+ *   accepted drafts, the last token, then -1; accepted int64 [B].
+ * A drafted token outside [0, V) is refused, and nothing is left out for it. */
+CASCADE_API int cascade_verify_drafts(const int64_t *tokens, const int64_t *draft_lens, const void *draft_probs,
+                                      const void *target_probs, const float *uniform, const float *noise,
+                                      int32_t dtype, int64_t batch, int64_t max_drafts, int64_t vocab,
+                                      int64_t *out_tokens, int64_t *accepted, cascade_stream_t stream);
+
 /* Last error message of this thread ("" if none). */
 CASCADE_API const char *cascade_last_error(void);
 

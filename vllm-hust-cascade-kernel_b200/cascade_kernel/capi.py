@@ -30,6 +30,16 @@ EXPORTED = [
     "cascade_plan_paged_attn",
     "cascade_check_block_table",
     "cascade_probe_hbm_read",
+    "cascade_latent_decode_workspace_size",
+    "cascade_latent_decode",
+    "cascade_latent_prefill",
+    "cascade_page_copy",
+    "cascade_page_fork_workspace_size",
+    "cascade_page_fork",
+    "cascade_page_free",
+    "cascade_page_compact_workspace_size",
+    "cascade_page_compact",
+    "cascade_verify_drafts",
 ]
 
 
@@ -63,6 +73,24 @@ class AttnPlan(ctypes.Structure):
         ("num_splits", ctypes.c_int64),
         ("workspace_bytes", ctypes.c_size_t),
     ]
+
+
+class LatentAttn(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "query", "cache", "block_table", "actual_q_seqlens", "actual_kv_seqlens")] + [
+        (n, ctypes.c_int64) for n in (
+            "num_tokens", "num_heads", "latent_dim", "rope_dim", "num_blocks", "block_size", "batch", "block_cols",
+            "q_seqlen_value")] + [
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32)]
+
+
+class LatentPrefill(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "query", "key", "key_rope", "value", "cu_q_seqlens", "cu_kv_seqlens")] + [
+        (n, ctypes.c_int64) for n in (
+            "num_tokens", "num_kv", "num_heads", "batch", "max_q_seqlen", "key_token_stride", "key_head_stride",
+            "rope_token_stride", "value_token_stride", "value_head_stride")] + [
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32)]
 
 
 _lib = None
@@ -109,6 +137,26 @@ def load():
     lib.cascade_check_block_table.restype = ctypes.c_int
     lib.cascade_probe_hbm_read.argtypes = [vp, sz, i32, i64, vp, sz, vp]
     lib.cascade_probe_hbm_read.restype = ctypes.c_int
+    lib.cascade_latent_decode_workspace_size.argtypes = [ctypes.POINTER(LatentAttn)]
+    lib.cascade_latent_decode_workspace_size.restype = sz
+    lib.cascade_latent_decode.argtypes = [ctypes.POINTER(LatentAttn), vp, vp, vp, sz, vp]
+    lib.cascade_latent_decode.restype = ctypes.c_int
+    lib.cascade_latent_prefill.argtypes = [ctypes.POINTER(LatentPrefill), vp, vp, vp]
+    lib.cascade_latent_prefill.restype = ctypes.c_int
+    lib.cascade_page_copy.argtypes = [vp, i64, i64, i64, vp, vp, i64, vp]
+    lib.cascade_page_copy.restype = ctypes.c_int
+    lib.cascade_page_fork_workspace_size.argtypes = [i64, i64]
+    lib.cascade_page_fork_workspace_size.restype = sz
+    lib.cascade_page_fork.argtypes = [vp, i64, i64, i64, i64, vp, i64, i64, vp, vp, vp, i64, vp, vp, vp, vp, sz, vp]
+    lib.cascade_page_fork.restype = ctypes.c_int
+    lib.cascade_page_free.argtypes = [vp, i64, i64, vp, vp, i64, vp, i64, vp, vp, vp, vp]
+    lib.cascade_page_free.restype = ctypes.c_int
+    lib.cascade_page_compact_workspace_size.argtypes = [i64]
+    lib.cascade_page_compact_workspace_size.restype = sz
+    lib.cascade_page_compact.argtypes = [vp, i64, i64, i64, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.cascade_page_compact.restype = ctypes.c_int
+    lib.cascade_verify_drafts.argtypes = [vp, vp, vp, vp, vp, vp, i32, i64, i64, i64, vp, vp, vp]
+    lib.cascade_verify_drafts.restype = ctypes.c_int
     _lib = lib
     return lib
 
@@ -270,3 +318,43 @@ def add_rms_norm_stats(x1, x2, gamma, beta, x_out, rstd, y, M, K, mode, eps, str
     return check(load().cascade_add_rms_norm_stats(
         _ptr(x1), _ptr(x2), _ptr(gamma), _ptr(beta), _ptr(x_out), _ptr(rstd), _ptr(y), M, K,
         dtype_code(x1.dtype), mode, eps, stream_ptr(stream)))
+
+
+def latent_desc(query, cache, block_table, q_seqlens, kv_seqlens, q_seqlen_value, scale, causal=True, *,
+                shape=None, dtype=None, flags=0):
+    """The C descriptor of latent attention, from device tensors or from
+    explicit sizes (``shape`` = dict, tensors None)."""
+    d = LatentAttn()
+    if shape is None:
+        d.query, d.cache, d.block_table = query.data_ptr(), cache.data_ptr(), block_table.data_ptr()
+        d.actual_q_seqlens = None if q_seqlens is None else q_seqlens.data_ptr()
+        d.actual_kv_seqlens = kv_seqlens.data_ptr()
+        d.num_tokens, d.num_heads = query.shape[0], query.shape[1]
+        d.latent_dim, d.rope_dim = query.shape[2] - 64, 64
+        d.num_blocks, d.block_size = cache.shape[0], cache.shape[1]
+        d.batch, d.block_cols = kv_seqlens.numel(), block_table.shape[1]
+        d.dtype = dtype_code(query.dtype)
+    else:
+        for k, v in shape.items():
+            setattr(d, k, v)
+        d.dtype = BF16 if dtype is None else dtype
+    d.q_seqlen_value, d.scale, d.causal, d.flags = q_seqlen_value, scale, int(causal), flags
+    return d
+
+
+def latent_decode_workspace_size(desc):
+    return load().cascade_latent_decode_workspace_size(ctypes.byref(desc))
+
+
+def latent_decode(desc, out, lse, workspace=None, stream=None):
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    return check(load().cascade_latent_decode(ctypes.byref(desc), _ptr(out), _ptr(lse), _ptr(workspace), ws_bytes,
+                                              stream_ptr(stream)))
+
+
+def page_copy(pools, src, dst, stream=None):
+    """cascade_page_copy over device pools of equal shape [num_blocks, ...]."""
+    ptrs = (ctypes.c_void_p * len(pools))(*[t.data_ptr() for t in pools])
+    page = pools[0][0].numel() * pools[0].element_size()
+    return check(load().cascade_page_copy(ptrs, len(pools), pools[0].shape[0], page, _ptr(src), _ptr(dst),
+                                          src.numel(), stream_ptr(stream)))

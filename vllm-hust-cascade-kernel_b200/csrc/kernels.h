@@ -194,6 +194,93 @@ struct RmsNormLaunch {
 
 cudaError_t launch_add_rms_norm_stats(const RmsNormLaunch& p, bool fp16, cudaStream_t stream);
 
+// ----------------------------------------------------------------------------
+// Latent attention
+// ----------------------------------------------------------------------------
+constexpr int kLatentDim = 512;               // latent values of a cache row
+constexpr int kLatentRow = kLatentDim + 64;   // with the rotary key values
+constexpr int kPrefillDk = 192;               // expanded key: 128 per head + 64 shared
+constexpr int kPrefillDv = 128;
+
+struct LatentDecodeLaunch {
+  const void* query;
+  const void* cache;
+  const int32_t* block_table;
+  const int64_t* q_lens;   // null when q_len > 0
+  const int64_t* kv_lens;
+  void* out;               // [num_tokens, num_heads, 512]
+  float* lse;              // [num_tokens * num_heads]
+  int64_t num_tokens;
+  int32_t num_heads, num_blocks, block_size, batch, block_cols;
+  int32_t q_len;           // 0 = per request
+  int32_t causal;
+  float scale;
+  uint32_t wait_limit_us;
+  int32_t debug_stall;
+};
+cudaError_t launch_latent_decode(const LatentDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream);
+size_t latent_decode_workspace(const LatentDecodeLaunch& p);
+
+struct LatentPrefillLaunch {
+  const void* query;
+  const void* key;
+  const void* key_rope;
+  const void* value;
+  const int64_t* cu_q;
+  const int64_t* cu_kv;
+  void* out;
+  float* lse;
+  int64_t num_tokens, num_kv;
+  int64_t key_ts, key_hs, rope_ts, value_ts, value_hs;  // strides in elements
+  int32_t num_heads, batch, max_q;
+  int32_t causal;
+  float scale;
+  uint32_t wait_limit_us;
+  int32_t debug_stall;
+};
+cudaError_t launch_latent_prefill(const LatentPrefillLaunch& p, bool fp16, cudaStream_t stream);
+
+// ----------------------------------------------------------------------------
+// Pages of a cache
+// ----------------------------------------------------------------------------
+constexpr int kMaxPoolsPerLaunch = 128;  // pool pointers that travel as kernel arguments
+
+struct PageState {
+  const int32_t* table;
+  const int64_t* kv_lens;
+  const int32_t* refs;
+  int32_t* table_out;
+  int64_t* lens_out;
+  int32_t* refs_out;
+  int64_t rows, cols, num_blocks, block_size;
+};
+cudaError_t launch_page_copy(void* const* pools, int64_t num_pools, int64_t num_blocks, int64_t page_bytes,
+                             const int64_t* src, const int64_t* dst, int64_t count, cudaStream_t stream);
+size_t page_fork_workspace(int64_t num_blocks, int64_t count);
+cudaError_t launch_page_fork(const PageState& s, void* const* pools, int64_t num_pools, int64_t row_bytes,
+                             const int64_t* parents, int64_t count, void* workspace, cudaStream_t stream);
+cudaError_t launch_page_free(const PageState& s, const int64_t* keep_lens, cudaStream_t stream);
+size_t page_compact_workspace(int64_t num_blocks);
+cudaError_t launch_page_compact(const PageState& s, void* const* pools, int64_t num_pools, int64_t row_bytes,
+                                int32_t* live_out, void* workspace, cudaStream_t stream);
+
+// ----------------------------------------------------------------------------
+// Verification of drafted tokens
+// ----------------------------------------------------------------------------
+struct VerifyLaunch {
+  const int64_t* tokens;
+  const int64_t* draft_lens;
+  const void* draft;   // [B, K, V] or null
+  const void* target;  // [B, K + 1, V]
+  const float* uniform;
+  const float* noise;
+  int64_t* out_tokens;
+  int64_t* accepted;
+  int64_t batch, drafts, vocab;
+  int32_t dtype;       // 0 bf16, 1 fp16, 2 fp32
+};
+cudaError_t launch_verify_drafts(const VerifyLaunch& p, cudaStream_t stream);
+
 // Host: raise a kernel's dynamic shared memory limit once per (kernel,
 // device) instead of on every launch.
 cudaError_t ensure_smem_limit(const void* kernel, int bytes);

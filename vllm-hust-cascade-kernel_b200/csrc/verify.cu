@@ -1,0 +1,161 @@
+// Verification of drafted tokens (cascade_verify_drafts).
+//
+// Draft i of a request is accepted while u_i q_i(x_i) < p_i(x_i); the token
+// after the accepted ones is argmax_v r(v) / e(v) with r = max(p - q, 0) at the
+// first refused place (p of the row after the last draft if none was), e
+// independent exponential variates: P[argmax = v] = r(v) / sum r.
+//
+// Only one row of p, q and e is read per request, once: HBM-bound for large
+// batches, and for small ones bound by the chain draft token -> its two
+// probabilities -> the row. A cluster of CTAs shares a request's row; every CTA
+// repeats the acceptance (a few gathered loads) instead of waiting for another's,
+// and the CTAs' best entries meet in shared memory of rank 0.
+//
+// Each value is one rounded product, difference and quotient in fp32, and the
+// best entry is the largest (quotient, lowest index), so the answer does not
+// depend on how the row was split.
+#include <cooperative_groups.h>
+
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace cascade {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 512;
+constexpr int kUnroll = 8;
+constexpr int kMaxCtas = 8;  // CTAs per request
+
+template <int kType>
+__device__ __forceinline__ float load(const void* base, int64_t i) {
+  if constexpr (kType == 2) return __ldg(static_cast<const float*>(base) + i);
+  const uint16_t b = __ldg(static_cast<const uint16_t*>(base) + i);
+  if constexpr (kType == 1) return __half2float(__ushort_as_half(b));
+  return __uint_as_float(static_cast<uint32_t>(b) << 16);
+}
+
+// (quotient, index) as one ordered key: larger quotient first, then lower
+// index. Quotients are >= 0, so their bits order as integers. 0 = no entry.
+__device__ __forceinline__ uint64_t make_key(float quotient, uint32_t v) {
+  return (static_cast<uint64_t>(__float_as_uint(quotient)) << 32) | (0xffffffffu - v);
+}
+
+__device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+template <int kType>
+__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyLaunch p) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int64_t b = blockIdx.x / ctas;
+  const int64_t K = p.drafts, V = p.vocab;
+  const int64_t n = min(max(p.draft_lens[b], static_cast<int64_t>(0)), K);
+  __shared__ int64_t s_taken;
+  __shared__ uint64_t s_best[kThreads / 32], s_all[kMaxCtas];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  cluster.barrier_arrive();  // waited for before the first write to another CTA: all have started by then
+
+  if (warp == 0) {
+    int64_t taken = n;  // the first refused draft
+    for (int64_t i0 = 0; i0 < n; i0 += 32) {
+      const int64_t i = i0 + lane;
+      bool refused = false;
+      if (i < n) {
+        const int64_t x = p.tokens[b * K + i];
+        refused = true;
+        if (x >= 0 && x < V) {
+          const float q = p.draft ? load<kType>(p.draft, (b * K + i) * V + x) : 1.f;
+          const float t = load<kType>(p.target, (b * (K + 1) + i) * V + x);
+          refused = !(__fmul_rn(p.uniform[b * K + i], q) < t);
+        }
+      }
+      const uint32_t any = __ballot_sync(0xffffffffu, refused);
+      if (any) {
+        taken = i0 + __ffs(any) - 1;
+        break;
+      }
+    }
+    if (lane == 0) s_taken = taken;
+  }
+  __syncthreads();
+  const int64_t taken = s_taken;
+  const bool refused = taken < n;
+  const int64_t prow = (b * (K + 1) + taken) * V, qrow = (b * K + taken) * V, erow = b * V;
+  const int64_t out = refused && !p.draft ? p.tokens[b * K + taken] : -1;  // the token left out
+
+  // the best entry of this cluster's row: pass 0 over `left`; pass 1, only
+  // when left is 0 everywhere, over the target's row
+  uint64_t best = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool minus = pass == 0 && refused && p.draft;
+    const int64_t stride = static_cast<int64_t>(ctas) * kThreads;
+    for (int64_t v0 = static_cast<int64_t>(rank) * kThreads + threadIdx.x; v0 < V; v0 += stride * kUnroll) {
+      float t[kUnroll], q[kUnroll], e[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t v = v0 + u * stride;
+        const bool in = v < V;
+        t[u] = in ? load<kType>(p.target, prow + v) : 0.f;
+        q[u] = in && minus ? load<kType>(p.draft, qrow + v) : 0.f;
+        e[u] = in ? __ldg(p.noise + erow + v) : 1.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t v = v0 + u * stride;
+        const float left = __fsub_rn(t[u], q[u]);
+        if (left > 0.f && !(pass == 0 && v == out))
+          best = max_u64(best, make_key(__fdiv_rn(left, e[u]), static_cast<uint32_t>(v)));
+      }
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, d));
+    if (lane == 0) s_best[warp] = best;
+    __syncthreads();
+    if (pass == 0) cluster.barrier_wait();
+    if (warp == 0) {
+      best = lane < kThreads / 32 ? s_best[lane] : 0;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, d));
+      if (lane < ctas) cluster.map_shared_rank(s_all, lane)[rank] = best;
+    }
+    cluster.sync();
+    best = 0;
+    for (int r = 0; r < ctas; ++r) best = max_u64(best, s_all[r]);
+    if (best != 0) break;
+    cluster.sync();  // s_all is written again
+  }
+  if (rank == 0) {
+    // nothing positive in the whole row: index 0, as an argmax over zeros
+    const int64_t last = best ? static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(best)) : 0;
+    for (int64_t i = threadIdx.x; i <= K; i += kThreads)
+      p.out_tokens[b * (K + 1) + i] = i < taken ? p.tokens[b * K + i] : i == taken ? last : -1;
+    if (threadIdx.x == 0) p.accepted[b] = taken;
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_verify_drafts(const VerifyLaunch& p, cudaStream_t stream) {
+  // as many CTAs per request as give the GPU two waves of two per SM, at
+  // least one unrolled round of the row each
+  int ctas = 1;
+  while (ctas < kMaxCtas && p.batch * ctas < 4 * kNumSMs && p.vocab > static_cast<int64_t>(ctas) * kThreads * kUnroll)
+    ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.batch * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto kern = p.dtype == 2 ? verify_kernel<2> : p.dtype == 1 ? verify_kernel<1> : verify_kernel<0>;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+}  // namespace cascade
