@@ -56,7 +56,7 @@ int check_decode(const cascade_latent_attn_t* p, const char* op) {
                 op, static_cast<long long>(p->q_seqlen_value));
   if (p->num_heads > kI32 || p->num_tokens > kI32 || p->num_tokens * p->num_heads > kI32 ||
       p->batch > kI32 || p->block_cols > kI32 || p->num_blocks > kI32 || p->num_blocks * bs > kI32 ||
-      p->block_cols * bs > kI32)
+      p->block_cols * bs > kI32 / 2)
     return fail(CASCADE_ERR_UNSUPPORTED, "%s: problem too large for 32-bit row indices", op);
   if (!(p->scale > 0.f) || p->scale > 3e38f) return fail(CASCADE_ERR_INVALID, "%s: scale must be positive", op);
   if (p->flags & ~CASCADE_FLAG_DEBUG_STALL) return fail(CASCADE_ERR_INVALID, "%s: unknown flags", op);

@@ -1,111 +1,824 @@
-// Latent attention, absorbed form (cascade_latent_decode).
+// Latent attention, absorbed form (cascade_latent_decode), on the tensor cores.
 //
 // For a query row x (576 values) of a request: s_t = scale <x, c_t> over the
-// request's cache rows c_t, out = sum_t softmax(s)_t c_t[0:512] with the
-// running maximum m and sum l of exp(s - m) in fp32. One warp per query row:
-// the lanes hold 18 query and 16 output values each, a dot product is one
-// warp reduction per cache row.
+// request's cache rows c_t (576 values), out = sum_t softmax(s)_t c_t[0:512].
+// A cache row of 1,152 bytes meets 2 x 1,088 flops per query row, so 128 rows
+// (one token x 128 heads) sit where the tensor cores and HBM take equally
+// long (0.168 against 0.179 ns per cache row and GPU), and fewer rows are
+// bound by HBM: the kernel has to keep both busy at once.
+//
+// A cluster of two CTAs computes one tile of 128 query rows (the request's
+// [token x head] rows in memory order) against 64 cache rows at a time:
+//   * the output of 128 x 512 fp32 would fill a CTA's tensor memory, so each CTA
+//     owns 256 of the 512 output columns (256 TMEM columns);
+//   * each CTA computes the scores of its own 32 of the 64 cache rows for all
+//     128 query rows, so no score is computed twice;
+//   * P (128 x 64, 16-bit) is written to both CTAs' shared memory, each thread
+//     storing its row's 32 values locally and to the other CTA; the row
+//     maxima are exchanged the same way, so both scale by the same maximum.
+// Per 64 cache rows a CTA loads its own 32 rows in full (keys, and its columns
+// of V) and its columns of the other 32: 52 KB for 36 KB from HBM.
+// The query tile lives two thirds in TMEM (384 of 576 dims, 192 columns)
+// and one third in shared memory: 147 KB of shared memory would leave no room
+// for loads in flight, and the products with A in TMEM do not re-read it from
+// shared memory.
+//
+// Softmax: running maximum m in the log2 domain that moves only when a score
+// exceeds it by more than 2^8 (the exponentials stay below 256, exact in
+// relative terms in both types), so the accumulator is rescaled rarely. P is
+// rounded to the inputs' type, which the second product needs. Two row sums in
+// fp32: of the exponentials, for the log-sum-exp, and of the rounded P, by
+// which the output is divided: what rounding adds to all weights of a row
+// alike then cancels (a row that sees one token returns it exactly).
+//
+// Work: the 64-row tiles of all (request, row tile) units, concatenated, are
+// cut into one equal run per cluster, computed on the device from the lengths.
+// A unit cut by a run boundary leaves fp32 partials that a second, dependent
+// launch merges in run order; all others are written directly.
+//
+// Warps: 0-3 softmax (thread = row = TMEM lane), 4-7 query loads and
+// epilogue, 8 keys (TMA), 9 MMA issue, 10 the other CTA's rows (TMA).
+#include <algorithm>
+
 #include "kernels.h"
 #include "ptx.cuh"
 
 namespace cascade {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kRows = 128;     // query rows per tile
+constexpr int kTok = 64;       // cache rows per tile
+constexpr int kHalfTok = 32;   // per CTA
+constexpr int kThreads = 11 * 32;
+constexpr int kMaxClusters = kNumSMs / 2;
+
+constexpr int kStages = 3;
+constexpr int kGroup = kHalfTok * 128;    // 32 cache rows x 64 dims
+constexpr int kBytesA = 5 * kGroup;       // keys outside the CTA's own columns
+constexpr int kBytesV = 4 * kGroup;       // the CTA's own columns
+constexpr int kQGroup = kRows * 128;      // 128 query rows x 64 dims
+constexpr int kQTmem = 6;                 // groups of 64 dims in TMEM, the last three in shared memory
+constexpr int kOffQ = 0;
+constexpr int kOffP = kOffQ + 3 * kQGroup;
+constexpr int kOffA = kOffP + kRows * kTok * 2;
+constexpr int kOffB = kOffA + kStages * kBytesA;
+constexpr int kOffC = kOffB + kStages * kBytesV;
+constexpr int kOffAux = kOffC + kStages * kBytesV;
+
+constexpr uint32_t kColO = 0, kColQ = 256, kColS = 448;  // TMEM columns: O 256, Q 192, S 2 x 32
+
+struct Sched {
+  int64_t tiles, begin;  // all tiles; this cluster's first
+  int64_t tok;           // first query token of request b
+  int b, mt, t0, left;
+};
+
+struct __align__(16) Aux {
+  float peer_max[2][kRows];  // written by the other CTA
+  float peer_sum[2][kRows];  // exponentials, rounded P
+  float inv[2][kRows];       // 1 / sum, per unit parity
+  float lse[2][kRows];
+  uint64_t a_full[kStages], a_empty[kStages], b_full[kStages], b_empty[kStages], c_full[kStages], c_empty[kStages];
+  uint64_t q_full, q_empty, s_full[2], s_empty[2], x_full[2], p_full, pv_done, o_full, o_empty, stat_full, l_full;
+  uint64_t stall, drain;
+  uint32_t tmem_base;
+  Sched sched;
+  int64_t scan[2][kThreads / 32];
+};
+constexpr int kSmemBytes = kOffAux + static_cast<int>(sizeof(Aux)) + 1024;
+static_assert(kSmemBytes + 16 <= 227 * 1024, "shared memory per CTA");
+
+struct Params {
+  LatentDecodeLaunch L;
+  CUtensorMap map4, map1;  // boxes of 64 dims x kR cache rows x 4 groups (1 group)
+  int32_t* row_info;       // [tokens x heads]: how the row's partials are found, 0 = none
+  float* part_o;           // [2 clusters][128][512]
+  float* part_lse;         // [2 clusters][128]
+};
 
 template <bool kFp16>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if constexpr (kFp16) {
     return __half22float2(*reinterpret_cast<__half2*>(&v));
   } else {
-    return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
 }
 
-// Request and query token of flat token `tok`; returns false past the last.
-__device__ bool find_request(const LatentDecodeLaunch& p, int64_t tok, int* b, int64_t* i, int64_t* q_len) {
-  if (p.q_len > 0) {
-    *b = static_cast<int>(tok / p.q_len);
-    *i = tok % p.q_len;
-    *q_len = p.q_len;
-    return *b < p.batch;
+// row_info of a unit cut into `count` >= 2 pieces, the first in run `c`: row r
+// of the slots 2c + 1 (first piece), 2 (c + 1), 2 (c + 2), ...
+__device__ __forceinline__ int32_t pack_info(int c, int count, int r) { return (count << 17) | (c << 7) | r; }
+
+// The (request, row tile) units' geometry, and the walk over a cluster's run.
+struct Unit {
+  const LatentDecodeLaunch& p;
+  int cap;
+  __device__ explicit Unit(const LatentDecodeLaunch& l) : p(l), cap(l.block_cols * l.block_size) {}
+  __device__ __forceinline__ int q_len(int b) const {
+    return p.q_len > 0 ? p.q_len
+                       : static_cast<int>(min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens));
   }
-  for (int r = 0; r < p.batch; ++r) {
-    const int64_t n = max(p.q_lens[r], static_cast<int64_t>(0));
-    if (tok < n) {
-      *b = r;
-      *i = tok;
-      *q_len = n;
-      return true;
+  __device__ __forceinline__ int kv_len(int b) const {
+    return static_cast<int>(min(max(p.kv_lens[b], static_cast<int64_t>(0)), static_cast<int64_t>(1 << 30)));
+  }
+  __device__ __forceinline__ int row_tiles(int q) const {
+    return static_cast<int>((static_cast<int64_t>(q) * p.num_heads + kRows - 1) / kRows);
+  }
+  // cache rows that query token i of a request sees
+  __device__ __forceinline__ int limit(int q, int kv, int i) const {
+    return max(0, p.causal ? min(cap, kv - q + i + 1) : min(cap, kv));
+  }
+  // tiles of a unit: up to what its last row sees, at least one
+  __device__ __forceinline__ int tiles(int q, int kv, int mt) const {
+    const int last = static_cast<int>(min(static_cast<int64_t>(q) * p.num_heads, static_cast<int64_t>(mt + 1) * kRows) - 1) /
+                     p.num_heads;
+    return max(1, (limit(q, kv, last) + kTok - 1) / kTok);
+  }
+};
+
+struct Walk {
+  Unit u;
+  // the current piece
+  int b, mt, t0, n, q, kv;
+  int64_t tok;
+  bool starts, ends;
+  int unit_tiles;
+
+  int next_b, next_mt, next_t0, left, nq, nkv;
+  int64_t next_tok;
+
+  __device__ Walk(const LatentDecodeLaunch& l, const Sched& s)
+      : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), left(s.left), next_tok(s.tok) {
+    if (left > 0) load();
+  }
+  __device__ __forceinline__ void load() {
+    nq = u.q_len(next_b);
+    nkv = u.kv_len(next_b);
+  }
+  __device__ __forceinline__ bool next() {
+    if (left <= 0) return false;
+    b = next_b, mt = next_mt, t0 = next_t0, q = nq, kv = nkv, tok = next_tok;
+    unit_tiles = u.tiles(q, kv, mt);
+    n = min(left, unit_tiles - t0);
+    starts = t0 == 0;
+    ends = t0 + n == unit_tiles;
+    left -= n;
+    if (left > 0) {  // the next unit's lengths, loaded a piece ahead
+      next_t0 = 0;
+      if (++next_mt == u.row_tiles(q)) {
+        next_mt = 0;
+        do {
+          next_tok += nq;
+          ++next_b;
+          if (next_b >= u.p.batch) {
+            left = 0;
+            break;
+          }
+          load();
+        } while (nq == 0);
+      }
     }
-    tok -= n;
+    return true;
   }
-  return false;
+};
+
+// Finds this cluster's run: the block sums the units' tiles (and the query
+// tokens) per contiguous chunk of requests, then the thread whose chunk holds
+// the run's first tile walks to it.
+__device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluster, int clusters, Aux* aux) {
+  const Unit u(p);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+  int64_t tiles = 0, toks = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
+    for (int mt = 0; mt < m; ++mt) tiles += u.tiles(q, kv, mt);
+    toks += q;
+  }
+  int64_t st = tiles, sq = toks;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t a = __shfl_up_sync(0xffffffffu, st, d), c = __shfl_up_sync(0xffffffffu, sq, d);
+    if (lane >= d) st += a, sq += c;
+  }
+  if (lane == 31) aux->scan[0][warp] = st, aux->scan[1][warp] = sq;
+  if (tid == 0) aux->sched.left = 0;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) st += aux->scan[0][w], sq += aux->scan[1][w];
+    total += aux->scan[0][w];
+  }
+  const int64_t runs = min(static_cast<int64_t>(clusters), total);
+  if (cluster < runs) {
+    const int64_t begin = cluster * total / runs, end = (cluster + 1) * total / runs;
+    int64_t at = st - tiles;
+    if (begin >= at && begin < st) {
+      int64_t tok = sq - toks;
+      for (int b = b0; b < b1; ++b) {
+        const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
+        for (int mt = 0; mt < m; ++mt) {
+          const int t = u.tiles(q, kv, mt);
+          if (begin < at + t) {
+            aux->sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin)};
+            b = b1;
+            break;
+          }
+          at += t;
+        }
+        tok += q;
+      }
+    }
+  }
+  __syncthreads();
 }
 
+// Loads one box column of a tile: kR cache rows x groups per load, for the 32
+// rows that start at cache row `first`. The warp's lanes hold the pool rows of
+// the next loads (`rows`, refilled every 32 loads).
+template <int kR>
+struct PageRows {
+  static constexpr int kPer = kHalfTok / kR;  // loads (pages at most) per tile
+  const LatentDecodeLaunch& p;
+  const int32_t* bt;
+  int base, pages, half, row;
+
+  __device__ PageRows(const LatentDecodeLaunch& l, int half_) : p(l), half(half_) {}
+  // tiles [t, ...) of request b with kv valid cache rows
+  __device__ __forceinline__ void start(int b, int kv) {
+    bt = p.block_table + static_cast<int64_t>(b) * p.block_cols;
+    pages = (min(kv, p.block_cols * p.block_size) + p.block_size - 1) / p.block_size;
+    base = -(1 << 30);
+  }
+  // pool row of load i of tile t (called by the whole warp)
+  __device__ __forceinline__ int get(int t, int i, int lane) {
+    constexpr int kTiles = 32 / kPer;
+    if (t >= base + kTiles || t < base) {
+      base = t;
+      const int tok = (t + lane / kPer) * kTok + half * kHalfTok + (lane % kPer) * kR;
+      const int page = tok / p.block_size, oob = max(1, p.num_blocks * p.block_size);
+      row = page < pages ? paged_row(bt[page], tok, p.block_size, p.num_blocks, oob) : oob;
+    }
+    return __shfl_sync(0xffffffffu, row, (t - base) * kPer + i);
+  }
+};
+
+template <bool kFp16, int kR>
+__global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid_constant__ Params P) {
+  pdl_launch_dependents();
+  const LatentDecodeLaunch& p = P.L;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Aux* aux = reinterpret_cast<Aux*>(smem + kOffAux);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int c = static_cast<int>(cluster_cta_rank());
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+
+  if (tid == 0) {
+    cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&aux->a_full[s], 1);
+      mbar_init(&aux->a_empty[s], 1);
+      mbar_init(&aux->b_full[s], 1);
+      mbar_init(&aux->b_empty[s], 1);
+      mbar_init(&aux->c_full[s], 1);
+      mbar_init(&aux->c_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&aux->s_full[s], 1);
+      mbar_init(&aux->s_empty[s], 4);
+      mbar_init(&aux->x_full[s], 4);
+    }
+    mbar_init(&aux->q_full, 128);
+    mbar_init(&aux->q_empty, 1);
+    mbar_init(&aux->p_full, 8);
+    mbar_init(&aux->pv_done, 2);
+    mbar_init(&aux->o_full, 1);
+    mbar_init(&aux->o_empty, 128);
+    mbar_init(&aux->stat_full, 128);
+    mbar_init(&aux->l_full, 4);
+    mbar_init(&aux->stall, 1);
+    mbar_init(&aux->drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(&aux->tmem_base, 512);
+    tmem_relinquish();
+  }
+  find_run(p, cluster, clusters, aux);
+  tc_fence_before();
+  cluster_sync_all();  // both CTAs' barriers are initialised
+  tc_fence_after();
+  const uint32_t tbase = aux->tmem_base;
+  Walk w(p, aux->sched);
+
+  if (warp == 8 || warp == 10) {
+    // ------------------------------------------------------------ producers
+    // 8: this CTA's 32 rows, first the groups outside its own columns, then
+    // its own; 10: the other CTA's 32 rows, own columns
+    const bool keys = warp == 8;
+    PageRows<kR> rows(p, keys ? c : 1 - c);
+    int it = 0, issued_a = 0, issued_v = 0;
+    while (w.next()) {
+      rows.start(w.b, w.kv);
+      for (int t = w.t0; t < w.t0 + w.n && !cta_aborted(); ++t, ++it) {
+        const int st = it % kStages, ph = (it / kStages - 1) & 1;
+        int y[PageRows<kR>::kPer];
+#pragma unroll
+        for (int i = 0; i < PageRows<kR>::kPer; ++i) y[i] = rows.get(t, i, lane);
+        if (keys) {
+          if (it >= kStages) mbar_wait(&aux->a_empty[st], ph);
+          if (lane == 0 && !cta_aborted()) {
+            uint8_t* dst = smem + kOffA + st * kBytesA;
+            mbar_arrive_expect_tx(&aux->a_full[st], kBytesA);
+#pragma unroll
+            for (int i = 0; i < PageRows<kR>::kPer; ++i) {
+              tma_load_3d(dst + i * kR * 512, &P.map4, &aux->a_full[st], 0, y[i], 4 * (1 - c));
+              tma_load_3d(dst + 4 * kGroup + i * kR * 128, &P.map1, &aux->a_full[st], 0, y[i], 8);
+            }
+            ++issued_a;
+          }
+          __syncwarp();
+        }
+        uint64_t* full = keys ? &aux->b_full[st] : &aux->c_full[st];
+        if (it >= kStages) mbar_wait(keys ? &aux->b_empty[st] : &aux->c_empty[st], ph);
+        if (lane == 0 && !cta_aborted()) {
+          uint8_t* dst = smem + (keys ? kOffB : kOffC) + st * kBytesV;
+          mbar_arrive_expect_tx(full, kBytesV);
+#pragma unroll
+          for (int i = 0; i < PageRows<kR>::kPer; ++i)
+            tma_load_3d(dst + i * kR * 512, &P.map4, full, 0, y[i], 4 * c);
+          ++issued_v;
+        }
+        __syncwarp();
+      }
+    }
+    // aborting: every load issued has landed before the CTA leaves
+    if (cta_aborted() && lane == 0) {
+      for (int j = max(0, issued_a - kStages); j < issued_a; ++j)
+        mbar_wait_drain(&aux->a_full[j % kStages], (j / kStages) & 1);
+      for (int j = max(0, issued_v - kStages); j < issued_v; ++j)
+        mbar_wait_drain(keys ? &aux->b_full[j % kStages] : &aux->c_full[j % kStages], (j / kStages) & 1);
+    }
+  } else if (warp == 9) {
+    // ----------------------------------------------------------- MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t fmt = kFp16 ? 0u : 1u;
+      constexpr int kPer = kHalfTok / kR;
+      const uint32_t idesc_s = make_idesc_f16(kRows, kR, fmt, 0, 0);
+      const uint32_t idesc_pv = make_idesc_f16(kRows, 256, fmt, 0, 1);
+      const uint32_t sQ = smem_u32(smem + kOffQ), sP = smem_u32(smem + kOffP);
+      int pieces = 0;
+      auto scores = [&](int it, bool first, bool last) {
+        const int st = it % kStages, sb = it & 1;
+        if (first) mbar_wait(&aux->q_full, pieces & 1);
+        mbar_wait(&aux->b_full[st], (it / kStages) & 1);
+        mbar_wait(&aux->a_full[st], (it / kStages) & 1);
+        if (it >= 2) mbar_wait(&aux->s_empty[sb], (it / 2 - 1) & 1);
+        if (cta_aborted()) return;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + kOffA + st * kBytesA), b = smem_u32(smem + kOffB + st * kBytesV);
+#pragma unroll
+        for (int g = 0; g < 9; ++g) {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const uint32_t k0 = g < 4   ? b + (i * 4 + g) * kR * 128
+                                : g < 8 ? a + (i * 4 + g - 4) * kR * 128
+                                        : a + 4 * kGroup + i * kR * 128;
+            const uint32_t d = tbase + kColS + sb * 32 + i * kR;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t bd = make_smem_desc(k0 + k * 32, 16, 1024, 2);
+              if (g < kQTmem)
+                umma_f16_ts(d, tbase + kColQ + g * 32 + k * 8, bd, idesc_s, g + k > 0);
+              else
+                umma_f16_ss(d, make_smem_desc(sQ + (g - kQTmem) * kQGroup + k * 32, 16, 1024, 2), bd, idesc_s, 1u);
+            }
+          }
+        }
+        umma_commit(&aux->a_empty[st]);
+        umma_commit(&aux->s_full[sb]);
+        if (last) umma_commit(&aux->q_empty);
+      };
+      auto values = [&](int it, bool first, bool last) {
+        const int st = it % kStages;
+        mbar_wait(&aux->c_full[st], (it / kStages) & 1);
+        mbar_wait_cluster(&aux->p_full, it & 1);
+        if (first && pieces > 0) mbar_wait(&aux->o_empty, (pieces - 1) & 1);
+        if (cta_aborted()) return;
+        tc_fence_after();
+        const uint32_t own = smem_u32(smem + kOffB + st * kBytesV), other = smem_u32(smem + kOffC + st * kBytesV);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t v = h == c ? own : other;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            // 16 cache rows: the second 16 follow at once (32-row boxes) or as the next box
+            const uint32_t v0 = v + (kR == 32 ? k * 2048 : k * 4 * kR * 128);
+            umma_f16_ss(tbase + kColO, make_smem_desc(sP + (h * 2 + k) * 32, 16, 1024, 2),
+                        make_smem_desc(v0, kR * 128, 1024, 2), idesc_pv, !first || h + k > 0);
+          }
+        }
+        umma_commit(&aux->b_empty[st]);
+        umma_commit(&aux->c_empty[st]);
+        umma_commit_cluster(&aux->pv_done, 3);
+        if (last) umma_commit(&aux->o_full);
+      };
+      int it = 0;
+      while (w.next() && !cta_aborted()) {
+        // scores run one tile ahead of values, within a piece
+        scores(it, true, w.n == 1);
+        for (int j = 0; j < w.n && !cta_aborted(); ++j, ++it) {
+          if (j + 1 < w.n) scores(it + 1, false, j + 2 == w.n);
+          values(it, j == 0, j + 1 == w.n);
+        }
+        ++pieces;
+      }
+      if (cta_aborted()) {
+        umma_commit(&aux->drain);
+        mbar_wait_drain(&aux->drain, 0);
+      }
+    }
+  } else if (warp < 4) {
+    // -------------------------------------------------------------- softmax
+    const int r = tid;
+    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
+    const float sl2 = p.scale * 1.4426950408889634f;
+    const uint32_t peer = static_cast<uint32_t>(1 - c);
+    uint8_t* prow = smem + kOffP;
+    const uint32_t peer_p = mapa_shared(smem_u32(prow), peer);
+    const uint32_t peer_bar_x = mapa_shared(smem_u32(&aux->x_full[0]), peer);
+    const uint32_t peer_bar_p = mapa_shared(smem_u32(&aux->p_full), peer);
+    const uint32_t peer_bar_l = mapa_shared(smem_u32(&aux->l_full), peer);
+    const uint32_t peer_max = mapa_shared(smem_u32(&aux->peer_max[0][r]), peer);
+    const uint32_t peer_sum = mapa_shared(smem_u32(&aux->peer_sum[0][r]), peer);
+    if (p.debug_stall) mbar_wait(&aux->stall, 0);  // test hook: runs into the wait limit
+    int it = 0, pieces = 0;
+    while (!cta_aborted() && w.next()) {
+      const int row = w.mt * kRows + r;
+      const int valid = min(w.kv, w.u.cap);  // cache rows that hold anything
+      const int lim = w.u.limit(w.q, w.kv, min(row / p.num_heads, w.q - 1));
+      // tiles below this one are seen in full by every row (the first row sees the least)
+      const int clean = w.u.limit(w.q, w.kv, w.mt * kRows / p.num_heads) / kTok;
+      float m = -INFINITY, l = 0.f, lp = 0.f;
+      for (int j = 0; j < w.n; ++j, ++it) {
+        const int t = w.t0 + j, sb = it & 1;
+        mbar_wait(&aux->s_full[sb], (it >> 1) & 1);
+        if (cta_aborted()) break;
+        tc_fence_after();
+        uint32_t sv[32];
+        tmem_ld_32x32b_x32(tbase + lane_off + kColS + sb * 32, sv);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&aux->s_empty[sb]);
+        float s[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e] = __uint_as_float(sv[e]);
+        if (t >= clean) {
+          const int seen = lim - t * kTok - c * kHalfTok;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = e < seen ? s[e] : -INFINITY;
+        }
+        float mx = fmax3f(s[0], s[1], s[2]), my = fmax3f(s[3], s[4], s[5]);
+#pragma unroll
+        for (int e = 6; e < 30; e += 4) {
+          mx = fmax3f(mx, s[e], s[e + 1]);
+          my = fmax3f(my, s[e + 2], s[e + 3]);
+        }
+        mx = fmax3f(mx, my, fmaxf(s[30], s[31]));
+        st_cluster_f32(peer_max + sb * kRows * 4, mx);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(peer_bar_x + sb * 8);
+        mbar_wait_cluster(&aux->x_full[sb], (it >> 1) & 1);
+        if (cta_aborted()) break;
+        mx = fmaxf(mx, aux->peer_max[sb][r]) * sl2;
+        // both CTAs take the same decision from the same two maxima
+        const bool move = mx > m + 8.f;
+        const float dm = move ? ex2(m - mx) : 1.f;  // 0 while nothing has been seen
+        if (move) m = mx;
+        const float neg = m == -INFINITY ? 0.f : -m;
+        float r0 = 0.f, r1 = 0.f, p0 = 0.f, p1 = 0.f;
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          float y0, y1;
+          ffma2_bcast(y0, y1, s[e], s[e + 1], sl2, neg);
+          y0 = ex2(y0), y1 = ex2(y1);
+          fadd2(r0, r1, y0, y1);
+          pk[e >> 1] = pack2<kFp16>(y0, y1);
+          const float2 rounded = unpack2<kFp16>(pk[e >> 1]);
+          fadd2(p0, p1, rounded.x, rounded.y);
+        }
+        l = l * dm + (r0 + r1);
+        lp = lp * dm + (p0 + p1);
+        // P of the tile before has been read by both CTAs, and O holds it
+        if (it > 0) mbar_wait_cluster(&aux->pv_done, (it - 1) & 1);
+        if (cta_aborted()) break;
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int g = 0; g < 8; ++g) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(tbase + lane_off + kColO + g * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * dm);
+            tmem_st_32x32b_x32(tbase + lane_off + kColO + g * 32, o);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t at = sw128(r, c * 4 + q);
+          *reinterpret_cast<uint4*>(prow + at) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+          st_cluster_v4(peer_p + at, pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+        }
+        if ((t + 1) * kTok > valid) {
+          // rows past the request's length may hold NaN: weight 0 does not hide
+          // them from the product, so they are cleared
+          const int st = it % kStages;
+          mbar_wait(&aux->c_full[st], (it / kStages) & 1);
+          const int g = tid >> 5, i = lane;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (t * kTok + h * kHalfTok + i < valid) continue;
+            uint4* v = reinterpret_cast<uint4*>(smem + (h == c ? kOffB : kOffC) + st * kBytesV +
+                                                ((i / kR) * 4 + g) * kR * 128 + (i % kR) * 128);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        fence_proxy_async_all();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&aux->p_full);
+          mbar_arrive_remote(peer_bar_p);
+        }
+      }
+      if (cta_aborted()) break;
+      // the row's sums over both CTAs' cache rows (a sum of two: the same in both CTAs)
+      st_cluster_f32(peer_sum, l);
+      st_cluster_f32(peer_sum + kRows * 4, lp);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(peer_bar_l);
+      mbar_wait_cluster(&aux->l_full, pieces & 1);
+      l += aux->peer_sum[0][r];
+      lp += aux->peer_sum[1][r];
+      aux->inv[pieces & 1][r] = lp > 0.f ? 1.f / lp : 0.f;
+      aux->lse[pieces & 1][r] = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+      mbar_arrive(&aux->stat_full);
+      ++pieces;
+    }
+    // the other CTA's last commit has arrived here before this CTA may leave
+    if (it > 0) mbar_wait_cluster(&aux->pv_done, (it - 1) & 1);
+  } else {
+    // ------------------------------------------------ query loads, epilogue
+    const int r = tid - 128;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int64_t all_rows = p.num_tokens * p.num_heads;
+    auto load_q = [&](const Walk& x) {
+      const int row = x.mt * kRows + r;
+      const int64_t grow = x.tok * p.num_heads + row;
+      const bool ok = row < x.q * p.num_heads && grow < all_rows;
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) + (ok ? grow : 0) * kLatentRow);
+#pragma unroll 1
+      for (int g = 0; g < 9; ++g) {
+        // group order: the CTA's own columns, the other latent ones, the rotary part
+        const int col = g < 4 ? 4 * c + g : g < 8 ? 4 * (1 - c) + g - 4 : 8;
+        uint4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = ok ? __ldg(src + col * 8 + k) : make_uint4(0u, 0u, 0u, 0u);
+        if (g < kQTmem) {
+          uint32_t x32[32];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            x32[4 * k] = v[k].x;
+            x32[4 * k + 1] = v[k].y;
+            x32[4 * k + 2] = v[k].z;
+            x32[4 * k + 3] = v[k].w;
+          }
+          tmem_st_32x32b_x32(tbase + lane_off + kColQ + g * 32, x32);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            *reinterpret_cast<uint4*>(smem + kOffQ + (g - kQTmem) * kQGroup + sw128(r, k)) = v[k];
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      fence_proxy_async_smem();
+      mbar_arrive(&aux->q_full);
+    };
+    auto store_o = [&](const Walk& x, int piece, int first_tile) {
+      mbar_wait(&aux->stat_full, piece & 1);
+      mbar_wait(&aux->o_full, piece & 1);
+      if (cta_aborted()) return;
+      tc_fence_after();
+      const float inv = aux->inv[piece & 1][r], lse = aux->lse[piece & 1][r];
+      const int row = x.mt * kRows + r;
+      const int64_t grow = x.tok * p.num_heads + row;
+      const bool ok = row < x.q * p.num_heads && grow < all_rows;
+      const bool whole = x.starts && x.ends;
+      const int64_t slot = 2 * cluster + (x.starts ? 1 : 0);
+#pragma unroll 1
+      for (int g = 0; g < 8; ++g) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tbase + lane_off + kColO + g * 32, o);
+        tmem_wait_ld();
+        if (g == 7) {
+          tc_fence_before();
+          mbar_arrive(&aux->o_empty);
+        }
+        float f[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) f[e] = inv > 0.f ? __uint_as_float(o[e]) * inv : 0.f;
+        if (ok && whole) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + grow * kLatentDim + 256 * c + g * 32);
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            dst[q] = make_uint4(pack2<kFp16>(f[8 * q], f[8 * q + 1]), pack2<kFp16>(f[8 * q + 2], f[8 * q + 3]),
+                                pack2<kFp16>(f[8 * q + 4], f[8 * q + 5]), pack2<kFp16>(f[8 * q + 6], f[8 * q + 7]));
+        } else if (ok) {
+          float4* dst = reinterpret_cast<float4*>(P.part_o + (slot * kRows + r) * kLatentDim + 256 * c + g * 32);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) dst[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+        }
+      }
+      if (ok && c == 0) {
+        if (whole)
+          p.lse[grow] = lse;
+        else
+          P.part_lse[slot * kRows + r] = lse;
+        if (x.starts) {
+          int32_t info = 0;
+          if (!x.ends) {
+            // the run that holds the unit's last tile
+            const Sched& s = aux->sched;
+            const int64_t runs = min(static_cast<int64_t>(clusters), s.tiles);
+            const int64_t last = s.begin + first_tile + x.unit_tiles - 1;
+            const int64_t hi = ((last + 1) * runs + s.tiles - 1) / s.tiles - 1;
+            info = pack_info(cluster, static_cast<int>(hi) - cluster + 1, r);
+          }
+          P.row_info[grow] = info;
+        }
+      }
+    };
+    // the next piece's query goes in as soon as the last scores of this one are
+    // computed, before this one's epilogue
+    bool more = w.next();
+    if (more) load_q(w);
+    int piece = 0, tiles_before = 0;
+    while (more && !cta_aborted()) {
+      const Walk now = w;
+      more = w.next();
+      if (more) {
+        mbar_wait(&aux->q_empty, piece & 1);
+        if (cta_aborted()) break;
+        tc_fence_after();
+        load_q(w);
+      }
+      store_o(now, piece, tiles_before);
+      tiles_before += now.n;
+      ++piece;
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync_all();  // no more stores or arrivals to the other CTA
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+// Merges the partials of the rows whose unit was cut: one warp per row, in run
+// order, weights exp(lse_i - max).
 template <bool kFp16>
-__global__ void __launch_bounds__(kWarps * 32) latent_decode_kernel(const LatentDecodeLaunch p) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_constant__ Params P, int clusters) {
+  pdl_wait();
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (row >= p.num_tokens * p.num_heads) return;
-  int b = 0;
-  int64_t i = 0, q_len = 0, n = 0;
-  if (find_request(p, row / p.num_heads, &b, &i, &q_len)) {
-    n = min(p.kv_lens[b], static_cast<int64_t>(p.block_cols) * p.block_size);
-    if (p.causal) n = min(n, p.kv_lens[b] - q_len + i + 1);
-  }
-  // pairs of values: lane holds pairs lane + 32 j, j < 9 (the last 32 pairs are the rotary part)
-  const uint32_t* q = static_cast<const uint32_t*>(p.query) + row * (kLatentRow / 2);
-  float2 x[9], o[8];
+  if (row >= P.L.num_tokens * P.L.num_heads) return;
+  const int32_t info = P.row_info[row];
+  const int count = info >> 17, c0 = (info >> 7) & 1023, r = info & 127;
+  // rows of a call whose query lengths do not add up hold no info: nothing past the slots is read for them
+  if (count < 2 || c0 + count > clusters) return;
+  auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRows + r; };
+  float top = -INFINITY;
+  for (int i = lane; i < count; i += 32) top = fmaxf(top, P.part_lse[slot(i)]);
 #pragma unroll
-  for (int j = 0; j < 9; ++j) x[j] = unpack2<kFp16>(q[lane + 32 * j]);
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float4 acc[4] = {};
+  float sum = 0.f;
+  for (int i = 0; i < count; ++i) {
+    const float lse = P.part_lse[slot(i)];
+    const float wgt = top == -INFINITY ? 0.f : __expf(lse - top);
+    const float4* src = reinterpret_cast<const float4*>(P.part_o + slot(i) * kLatentDim);
+    sum += wgt;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = make_float2(0.f, 0.f);
-  float m = -INFINITY, l = 0.f;
-  const int32_t* bt = p.block_table + static_cast<int64_t>(b) * p.block_cols;
-  for (int64_t t = 0; t < n; ++t) {
-    const int32_t id = bt[t / p.block_size];
-    const bool ok = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks);
-    if (!ok && lane == 0) atomicOr(&g_cascade_device_error, kErrBadBlockId);
-    const uint32_t* c = static_cast<const uint32_t*>(p.cache) +
-                        (static_cast<int64_t>(ok ? id : 0) * p.block_size + t % p.block_size) * (kLatentRow / 2);
-    float2 v[9];
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 9; ++j) {
-      v[j] = unpack2<kFp16>(ok ? c[lane + 32 * j] : 0u);
-      s = fmaf(x[j].x, v[j].x, fmaf(x[j].y, v[j].y, s));
+    for (int k = 0; k < 4; ++k) {
+      const float4 v = src[lane + 32 * k];
+      acc[k].x = fmaf(wgt, v.x, acc[k].x);
+      acc[k].y = fmaf(wgt, v.y, acc[k].y);
+      acc[k].z = fmaf(wgt, v.z, acc[k].z);
+      acc[k].w = fmaf(wgt, v.w, acc[k].w);
     }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-    s *= p.scale;
-    const float m_new = fmaxf(m, s);
-    const float dm = m == m_new ? 1.f : expf(m - m_new);
-    const float e = m_new == -INFINITY ? 0.f : expf(s - m_new);
-    l = l * dm + e;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      o[j].x = fmaf(e, v[j].x, o[j].x * dm);
-      o[j].y = fmaf(e, v[j].y, o[j].y * dm);
-    }
-    m = m_new;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint32_t* out = static_cast<uint32_t*>(p.out) + row * (kLatentDim / 2);
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.L.out) + row * kLatentDim);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) out[lane + 32 * j] = pack2<kFp16>(o[j].x * inv, o[j].y * inv);
-  if (lane == 0) p.lse[row] = l > 0.f ? m + logf(l) : -INFINITY;
+  for (int k = 0; k < 4; ++k)
+    dst[lane + 32 * k] = make_uint2(pack2<kFp16>(acc[k].x * inv, acc[k].y * inv), pack2<kFp16>(acc[k].z * inv, acc[k].w * inv));
+  if (lane == 0) P.L.lse[row] = sum > 0.f ? top + __logf(sum) : -INFINITY;
+}
+
+// More clusters than tiles would stay idle, whatever the lengths.
+int cluster_bound(const LatentDecodeLaunch& p) {
+  const int64_t rows = p.num_tokens * p.num_heads;
+  const int64_t units = p.batch + rows / kRows;
+  const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(p.block_cols) * p.block_size + kTok - 1) / kTok);
+  return static_cast<int>(std::min<int64_t>(kMaxClusters, std::min<int64_t>(units, 1 << 20) * tiles));
+}
+
+size_t info_bytes(const LatentDecodeLaunch& p) {
+  return (static_cast<size_t>(p.num_tokens) * p.num_heads * sizeof(int32_t) + 255) / 256 * 256;
+}
+
+template <bool kFp16, int kR>
+cudaError_t launch(Params& P, cudaStream_t stream) {
+  auto kern = latent_decode_kernel<kFp16, kR>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), kSmemBytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // as many clusters as run at once: their runs are equal, a second wave would double the time
+  static int resident[64] = {};
+  int dev = 0;
+  e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int& n = resident[dev & 63];
+  if (n == 0) {
+    int found = 0;
+    cfg.gridDim = dim3(2 * kMaxClusters);
+    if (cudaOccupancyMaxActiveClusters(&found, reinterpret_cast<const void*>(kern), &cfg) != cudaSuccess || found <= 0) {
+      cudaGetLastError();
+      found = kMaxClusters;
+    }
+    n = std::min(found, kMaxClusters);
+  }
+  const int clusters = std::min(n, cluster_bound(P.L));
+  cfg.gridDim = dim3(2 * clusters);
+  e = cudaLaunchKernelEx(&cfg, kern, P);
+  if (e != cudaSuccess || clusters == 1) return e;
+  cudaLaunchConfig_t cc = {};
+  cc.gridDim = dim3(static_cast<unsigned>((P.L.num_tokens * P.L.num_heads + 7) / 8));
+  cc.blockDim = dim3(256);
+  cc.stream = stream;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cc.attrs = pdl;
+  cc.numAttrs = 1;
+  return cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16>, P, clusters);
 }
 
 }  // namespace
 
-size_t latent_decode_workspace(const LatentDecodeLaunch&) { return 0; }
+size_t latent_decode_workspace(const LatentDecodeLaunch& p) {
+  return info_bytes(p) + static_cast<size_t>(cluster_bound(p)) * 2 * kRows * (kLatentDim + 1) * sizeof(float);
+}
 
-cudaError_t launch_latent_decode(const LatentDecodeLaunch& p, bool fp16, void*, cudaStream_t stream) {
-  const int64_t rows = p.num_tokens * p.num_heads;
-  auto kern = fp16 ? latent_decode_kernel<true> : latent_decode_kernel<false>;
-  kern<<<static_cast<unsigned>((rows + kWarps - 1) / kWarps), kWarps * 32, 0, stream>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_latent_decode(const LatentDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
+  Params P;
+  P.L = p;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  P.row_info = reinterpret_cast<int32_t*>(ws);
+  P.part_o = reinterpret_cast<float*>(ws + info_bytes(p));
+  P.part_lse = P.part_o + static_cast<size_t>(cluster_bound(p)) * 2 * kRows * kLatentDim;
+  // cache rows as 9 groups of 64 dims; a load is the rows of one page (at most 32) x 4 groups (or 1).
+  // A cache without pages: a map over one row that nothing in bounds reads.
+  const uint32_t rows = p.block_size < kHalfTok ? 16 : 32;
+  const uint64_t pool_rows = std::max<uint64_t>(1, static_cast<uint64_t>(p.num_blocks) * p.block_size);
+  const void* base = p.num_blocks > 0 ? p.cache : p.query;
+  const uint64_t extent[3] = {64, pool_rows, 9}, stride[2] = {kLatentRow * 2, 128};
+  if (!encode_tmap_3d(&P.map4, base, extent, stride, {64, rows, 4}) ||
+      !encode_tmap_3d(&P.map1, base, extent, stride, {64, rows, 1}))
+    return cudaErrorInvalidValue;
+  if (rows == 16) return fp16 ? launch<true, 16>(P, stream) : launch<false, 16>(P, stream);
+  return fp16 ? launch<true, 32>(P, stream) : launch<false, 32>(P, stream);
 }
 
 }  // namespace cascade
