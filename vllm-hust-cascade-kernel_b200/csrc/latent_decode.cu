@@ -13,15 +13,17 @@
 //     owns 256 of the 512 output columns (256 TMEM columns);
 //   * each CTA computes the scores of its own 32 of the 64 cache rows for all
 //     128 query rows, so no score is computed twice;
-//   * P (128 x 64, 16-bit) is written to both CTAs' shared memory, each thread
-//     storing its row's 32 values locally and to the other CTA; the row
-//     maxima are exchanged the same way, so both scale by the same maximum.
+//   * the row maxima of a tile are exchanged (st.async), so both CTAs scale by
+//     the same maximum, and each CTA's half of P (128 x 32, 16-bit) is copied
+//     to the other by the bulk-copy engine; both take several hundred cycles,
+//     so three tiles are in flight: scores of tile n + 2, maxima of n + 1,
+//     exponentials and P of n (remote stores with a release instead held the
+//     softmax warps for about 4,000 cycles a tile).
 // Per 64 cache rows a CTA loads its own 32 rows in full (keys, and its columns
 // of V) and its columns of the other 32: 52 KB for 36 KB from HBM.
-// The query tile lives two thirds in TMEM (384 of 576 dims, 192 columns)
-// and one third in shared memory: 147 KB of shared memory would leave no room
-// for loads in flight, and the products with A in TMEM do not re-read it from
-// shared memory.
+// Seven of the query tile's nine groups of 64 dims live in TMEM (224 columns),
+// two in shared memory: with A in shared memory a 128 x 32 x 16 MMA takes 43
+// cycles (A's 4 KB), in TMEM 19.
 //
 // Softmax: running maximum m in the log2 domain that moves only when a score
 // exceeds it by more than 2^8 (the exponentials stay below 256, exact in
@@ -52,20 +54,22 @@ constexpr int kHalfTok = 32;   // per CTA
 constexpr int kThreads = 11 * 32;
 constexpr int kMaxClusters = kNumSMs / 2;
 
-constexpr int kStages = 3;
+constexpr int kStagesA = 2, kStagesB = 4, kStagesC = 3;  // keys outside the own columns; own columns; the other rows
+constexpr int kPBuf = 2, kXBuf = 4;
 constexpr int kGroup = kHalfTok * 128;    // 32 cache rows x 64 dims
 constexpr int kBytesA = 5 * kGroup;       // keys outside the CTA's own columns
 constexpr int kBytesV = 4 * kGroup;       // the CTA's own columns
 constexpr int kQGroup = kRows * 128;      // 128 query rows x 64 dims
-constexpr int kQTmem = 6;                 // groups of 64 dims in TMEM, the last three in shared memory
+constexpr int kQTmem = 7;                 // groups of 64 dims in TMEM, the last two in shared memory
+constexpr int kPHalf = kRows * kHalfTok * 2;  // P of one CTA's cache rows
 constexpr int kOffQ = 0;
-constexpr int kOffP = kOffQ + 3 * kQGroup;
-constexpr int kOffA = kOffP + kRows * kTok * 2;
-constexpr int kOffB = kOffA + kStages * kBytesA;
-constexpr int kOffC = kOffB + kStages * kBytesV;
-constexpr int kOffAux = kOffC + kStages * kBytesV;
+constexpr int kOffP = kOffQ + (9 - kQTmem) * kQGroup;
+constexpr int kOffA = kOffP + kPBuf * 2 * kPHalf;
+constexpr int kOffB = kOffA + kStagesA * kBytesA;
+constexpr int kOffC = kOffB + kStagesB * kBytesV;
+constexpr int kOffAux = kOffC + kStagesC * kBytesV;
 
-constexpr uint32_t kColO = 0, kColQ = 256, kColS = 448;  // TMEM columns: O 256, Q 192, S 2 x 32
+constexpr uint32_t kColO = 0, kColQ = 256, kColS = 480;  // TMEM columns: O 256, Q 224, S 32
 
 struct Sched {
   int64_t tiles, begin;  // all tiles; this cluster's first
@@ -74,12 +78,13 @@ struct Sched {
 };
 
 struct __align__(16) Aux {
-  float peer_max[2][kRows];  // written by the other CTA
+  float peer_max[kXBuf][kRows];  // written by the other CTA
   float peer_sum[2][kRows];  // exponentials, rounded P
   float inv[2][kRows];       // 1 / sum, per unit parity
   float lse[2][kRows];
-  uint64_t a_full[kStages], a_empty[kStages], b_full[kStages], b_empty[kStages], c_full[kStages], c_empty[kStages];
-  uint64_t q_full, q_empty, s_full[2], s_empty[2], x_full[2], p_full, pv_done, o_full, o_empty, stat_full, l_full;
+  uint64_t a_full[kStagesA], a_empty[kStagesA], b_full[kStagesB], b_empty[kStagesB], c_full[kStagesC], c_empty[kStagesC];
+  uint64_t q_full, q_empty, s_full, s_empty, x_full[kXBuf], p_full[kPBuf], pv_done[kPBuf], o_full, o_empty, stat_full;
+  uint64_t l_full;
   uint64_t stall, drain;
   uint32_t tmem_base;
   Sched sched;
@@ -277,23 +282,15 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 
   if (tid == 0) {
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&aux->a_full[s], 1);
-      mbar_init(&aux->a_empty[s], 1);
-      mbar_init(&aux->b_full[s], 1);
-      mbar_init(&aux->b_empty[s], 1);
-      mbar_init(&aux->c_full[s], 1);
-      mbar_init(&aux->c_empty[s], 1);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&aux->s_full[s], 1);
-      mbar_init(&aux->s_empty[s], 4);
-      mbar_init(&aux->x_full[s], 4);
-    }
+    for (int s = 0; s < kStagesA; ++s) mbar_init(&aux->a_full[s], 1), mbar_init(&aux->a_empty[s], 1);
+    for (int s = 0; s < kStagesB; ++s) mbar_init(&aux->b_full[s], 1), mbar_init(&aux->b_empty[s], 1);
+    for (int s = 0; s < kStagesC; ++s) mbar_init(&aux->c_full[s], 1), mbar_init(&aux->c_empty[s], 1);
+    for (int s = 0; s < kXBuf; ++s) mbar_init(&aux->x_full[s], 1);
+    for (int s = 0; s < kPBuf; ++s) mbar_init(&aux->p_full[s], 4), mbar_init(&aux->pv_done[s], 2);
+    mbar_init(&aux->s_full, 1);
+    mbar_init(&aux->s_empty, 4);
     mbar_init(&aux->q_full, 128);
     mbar_init(&aux->q_empty, 1);
-    mbar_init(&aux->p_full, 8);
-    mbar_init(&aux->pv_done, 2);
     mbar_init(&aux->o_full, 1);
     mbar_init(&aux->o_empty, 128);
     mbar_init(&aux->stat_full, 128);
@@ -320,16 +317,18 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     const bool keys = warp == 8;
     PageRows<kR> rows(p, keys ? c : 1 - c);
     int it = 0, issued_a = 0, issued_v = 0;
-    while (w.next()) {
+    bool live = true;
+    while (live && w.next()) {
       rows.start(w.b, w.kv);
-      for (int t = w.t0; t < w.t0 + w.n && !cta_aborted(); ++t, ++it) {
-        const int st = it % kStages, ph = (it / kStages - 1) & 1;
+      for (int t = w.t0; t < w.t0 + w.n; ++t, ++it) {
         int y[PageRows<kR>::kPer];
 #pragma unroll
         for (int i = 0; i < PageRows<kR>::kPer; ++i) y[i] = rows.get(t, i, lane);
         if (keys) {
-          if (it >= kStages) mbar_wait(&aux->a_empty[st], ph);
-          if (lane == 0 && !cta_aborted()) {
+          const int st = it % kStagesA;
+          live = it < kStagesA || mbar_wait_warp(&aux->a_empty[st], (it / kStagesA - 1) & 1);
+          if (!live) break;
+          if (lane == 0) {
             uint8_t* dst = smem + kOffA + st * kBytesA;
             mbar_arrive_expect_tx(&aux->a_full[st], kBytesA);
 #pragma unroll
@@ -337,108 +336,120 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
               tma_load_3d(dst + i * kR * 512, &P.map4, &aux->a_full[st], 0, y[i], 4 * (1 - c));
               tma_load_3d(dst + 4 * kGroup + i * kR * 128, &P.map1, &aux->a_full[st], 0, y[i], 8);
             }
-            ++issued_a;
           }
+          ++issued_a;
           __syncwarp();
         }
+        const int stages = keys ? kStagesB : kStagesC, st = it % stages;
         uint64_t* full = keys ? &aux->b_full[st] : &aux->c_full[st];
-        if (it >= kStages) mbar_wait(keys ? &aux->b_empty[st] : &aux->c_empty[st], ph);
-        if (lane == 0 && !cta_aborted()) {
+        live = it < stages || mbar_wait_warp(keys ? &aux->b_empty[st] : &aux->c_empty[st], (it / stages - 1) & 1);
+        if (!live) break;
+        if (lane == 0) {
           uint8_t* dst = smem + (keys ? kOffB : kOffC) + st * kBytesV;
           mbar_arrive_expect_tx(full, kBytesV);
 #pragma unroll
           for (int i = 0; i < PageRows<kR>::kPer; ++i)
             tma_load_3d(dst + i * kR * 512, &P.map4, full, 0, y[i], 4 * c);
-          ++issued_v;
         }
+        ++issued_v;
         __syncwarp();
       }
     }
     // aborting: every load issued has landed before the CTA leaves
-    if (cta_aborted() && lane == 0) {
-      for (int j = max(0, issued_a - kStages); j < issued_a; ++j)
-        mbar_wait_drain(&aux->a_full[j % kStages], (j / kStages) & 1);
-      for (int j = max(0, issued_v - kStages); j < issued_v; ++j)
-        mbar_wait_drain(keys ? &aux->b_full[j % kStages] : &aux->c_full[j % kStages], (j / kStages) & 1);
+    if (!live && lane == 0) {
+      for (int j = max(0, issued_a - kStagesA); j < issued_a; ++j)
+        mbar_wait_drain(&aux->a_full[j % kStagesA], (j / kStagesA) & 1);
+      const int stages = keys ? kStagesB : kStagesC;
+      for (int j = max(0, issued_v - stages); j < issued_v; ++j)
+        mbar_wait_drain(keys ? &aux->b_full[j % stages] : &aux->c_full[j % stages], (j / stages) & 1);
     }
   } else if (warp == 9) {
     // ----------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t fmt = kFp16 ? 0u : 1u;
-      constexpr int kPer = kHalfTok / kR;
-      const uint32_t idesc_s = make_idesc_f16(kRows, kR, fmt, 0, 0);
-      const uint32_t idesc_pv = make_idesc_f16(kRows, 256, fmt, 0, 1);
-      const uint32_t sQ = smem_u32(smem + kOffQ), sP = smem_u32(smem + kOffP);
-      int pieces = 0;
-      auto scores = [&](int it, bool first, bool last) {
-        const int st = it % kStages, sb = it & 1;
-        if (first) mbar_wait(&aux->q_full, pieces & 1);
-        mbar_wait(&aux->b_full[st], (it / kStages) & 1);
-        mbar_wait(&aux->a_full[st], (it / kStages) & 1);
-        if (it >= 2) mbar_wait(&aux->s_empty[sb], (it / 2 - 1) & 1);
-        if (cta_aborted()) return;
-        tc_fence_after();
-        const uint32_t a = smem_u32(smem + kOffA + st * kBytesA), b = smem_u32(smem + kOffB + st * kBytesV);
+    // the whole warp walks; one elected lane issues
+    constexpr uint32_t fmt = kFp16 ? 0u : 1u;
+    constexpr int kPer = kHalfTok / kR;
+    const uint32_t idesc_s = make_idesc_f16(kRows, kR, fmt, 0, 0);
+    const uint32_t idesc_pv = make_idesc_f16(kRows, 256, fmt, 0, 1);
+    const uint32_t tm = uniform(tbase), rank = uniform(static_cast<uint32_t>(c));
+    const uint32_t s0 = uniform(smem_u32(smem));
+    int pieces = 0;
+    auto scores = [&](int it, bool first, bool last) -> bool {
+      const uint32_t sa = uniform(it % kStagesA), sb = uniform(it % kStagesB);
+      if ((first && !mbar_wait_warp(&aux->q_full, pieces & 1)) ||
+          !mbar_wait_warp(&aux->b_full[sb], (it / kStagesB) & 1) ||
+          !mbar_wait_warp(&aux->a_full[sa], (it / kStagesA) & 1) ||
+          (it > 0 && !mbar_wait_warp(&aux->s_empty, (it - 1) & 1)))
+        return false;
+      tc_fence_after();
+      const uint64_t da = make_smem_desc(s0 + kOffA + sa * kBytesA, 16, 1024, 2);
+      const uint64_t db = make_smem_desc(s0 + kOffB + sb * kBytesV, 16, 1024, 2);
+      const uint64_t dq = make_smem_desc(s0 + kOffQ, 16, 1024, 2);
+      __syncwarp();
+      if (elect_one()) {
 #pragma unroll
         for (int g = 0; g < 9; ++g) {
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            const uint32_t k0 = g < 4   ? b + (i * 4 + g) * kR * 128
-                                : g < 8 ? a + (i * 4 + g - 4) * kR * 128
-                                        : a + 4 * kGroup + i * kR * 128;
-            const uint32_t d = tbase + kColS + sb * 32 + i * kR;
+            const uint64_t k0 = g < 4   ? db + (i * 4 + g) * kR * 8
+                                : g < 8 ? da + (i * 4 + g - 4) * kR * 8
+                                        : da + (4 * kGroup) / 16 + i * kR * 8;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint64_t bd = make_smem_desc(k0 + k * 32, 16, 1024, 2);
               if (g < kQTmem)
-                umma_f16_ts(d, tbase + kColQ + g * 32 + k * 8, bd, idesc_s, g + k > 0);
+                umma_f16_ts(tm + kColS + i * kR, tm + kColQ + g * 32 + k * 8, k0 + k * 2, idesc_s, g + k > 0);
               else
-                umma_f16_ss(d, make_smem_desc(sQ + (g - kQTmem) * kQGroup + k * 32, 16, 1024, 2), bd, idesc_s, 1u);
+                umma_f16_ss(tm + kColS + i * kR, dq + ((g - kQTmem) * kQGroup + k * 32) / 16, k0 + k * 2, idesc_s, 1u);
             }
           }
         }
-        umma_commit(&aux->a_empty[st]);
-        umma_commit(&aux->s_full[sb]);
+        umma_commit(&aux->a_empty[sa]);
+        umma_commit(&aux->s_full);
         if (last) umma_commit(&aux->q_empty);
-      };
-      auto values = [&](int it, bool first, bool last) {
-        const int st = it % kStages;
-        mbar_wait(&aux->c_full[st], (it / kStages) & 1);
-        mbar_wait_cluster(&aux->p_full, it & 1);
-        if (first && pieces > 0) mbar_wait(&aux->o_empty, (pieces - 1) & 1);
-        if (cta_aborted()) return;
-        tc_fence_after();
-        const uint32_t own = smem_u32(smem + kOffB + st * kBytesV), other = smem_u32(smem + kOffC + st * kBytesV);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto values = [&](int it, bool first, bool last) -> bool {
+      const uint32_t sb = uniform(it % kStagesB), sc = uniform(it % kStagesC), pb = uniform(it & 1);
+      if (!mbar_wait_warp(&aux->c_full[sc], (it / kStagesC) & 1) ||
+          !mbar_wait_cluster_warp(&aux->p_full[pb], (it >> 1) & 1) ||
+          (first && pieces > 0 && !mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1)))
+        return false;
+      tc_fence_after();
+      const uint32_t own = s0 + kOffB + sb * kBytesV, other = s0 + kOffC + sc * kBytesV;
+      // P: rows of 64 bytes, 64-byte swizzle; V: 64-column groups kR * 128 bytes apart
+      const uint64_t dp = make_smem_desc(s0 + kOffP + pb * 2 * kPHalf, 16, 512, 4);
+      const uint64_t dv0 = make_smem_desc(rank == 0 ? own : other, kR * 128, 1024, 2);
+      const uint64_t dv1 = make_smem_desc(rank == 0 ? other : own, kR * 128, 1024, 2);
+      __syncwarp();
+      if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t v = h == c ? own : other;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            // 16 cache rows: the second 16 follow at once (32-row boxes) or as the next box
-            const uint32_t v0 = v + (kR == 32 ? k * 2048 : k * 4 * kR * 128);
-            umma_f16_ss(tbase + kColO, make_smem_desc(sP + (h * 2 + k) * 32, 16, 1024, 2),
-                        make_smem_desc(v0, kR * 128, 1024, 2), idesc_pv, !first || h + k > 0);
-          }
+          for (int k = 0; k < 2; ++k)  // the second 16 cache rows follow at once (32-row boxes) or as the next box
+            umma_f16_ss(tm + kColO, dp + (h * kPHalf + k * 32) / 16,
+                        (h ? dv1 : dv0) + (kR == 32 ? k * 2048 : k * 4 * kR * 128) / 16, idesc_pv, !first || h + k > 0);
         }
-        umma_commit(&aux->b_empty[st]);
-        umma_commit(&aux->c_empty[st]);
-        umma_commit_cluster(&aux->pv_done, 3);
+        umma_commit(&aux->b_empty[sb]);
+        umma_commit(&aux->c_empty[sc]);
+        umma_commit_cluster(&aux->pv_done[pb], 3);
         if (last) umma_commit(&aux->o_full);
-      };
-      int it = 0;
-      while (w.next() && !cta_aborted()) {
-        // scores run one tile ahead of values, within a piece
-        scores(it, true, w.n == 1);
-        for (int j = 0; j < w.n && !cta_aborted(); ++j, ++it) {
-          if (j + 1 < w.n) scores(it + 1, false, j + 2 == w.n);
-          values(it, j == 0, j + 1 == w.n);
-        }
-        ++pieces;
       }
-      if (cta_aborted()) {
-        umma_commit(&aux->drain);
-        mbar_wait_drain(&aux->drain, 0);
-      }
+      __syncwarp();
+      return true;
+    };
+    int it = 0;
+    bool live = true;
+    while (live && w.next()) {
+      // scores run two tiles ahead of values, within a piece
+      live = scores(it, true, w.n == 1) && (w.n == 1 || scores(it + 1, false, w.n == 2));
+      for (int j = 0; live && j < w.n; ++j, ++it)
+        live = (j + 2 >= w.n || scores(it + 2, false, j + 3 == w.n)) && values(it, j == 0, j + 1 == w.n);
+      ++pieces;
+    }
+    if (!live && lane == 0) {
+      umma_commit(&aux->drain);
+      mbar_wait_drain(&aux->drain, 0);
     }
   } else if (warp < 4) {
     // -------------------------------------------------------------- softmax
@@ -446,54 +457,64 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
     const float sl2 = p.scale * 1.4426950408889634f;
     const uint32_t peer = static_cast<uint32_t>(1 - c);
-    uint8_t* prow = smem + kOffP;
-    const uint32_t peer_p = mapa_shared(smem_u32(prow), peer);
+    // this CTA's half of P, this row: 64 bytes, 16-byte chunk q at q ^ (row / 2 % 4); the warp's rows are 2 KB in one piece
+    uint8_t* half = smem + kOffP + c * kPHalf;
+    const uint32_t peer_half = mapa_shared(smem_u32(half + warp * 2048), peer);
     const uint32_t peer_bar_x = mapa_shared(smem_u32(&aux->x_full[0]), peer);
-    const uint32_t peer_bar_p = mapa_shared(smem_u32(&aux->p_full), peer);
+    const uint32_t peer_bar_p = mapa_shared(smem_u32(&aux->p_full[0]), peer);
     const uint32_t peer_bar_l = mapa_shared(smem_u32(&aux->l_full), peer);
     const uint32_t peer_max = mapa_shared(smem_u32(&aux->peer_max[0][r]), peer);
     const uint32_t peer_sum = mapa_shared(smem_u32(&aux->peer_sum[0][r]), peer);
     if (p.debug_stall) mbar_wait(&aux->stall, 0);  // test hook: runs into the wait limit
     int it = 0, pieces = 0;
-    while (!cta_aborted() && w.next()) {
+    bool live = true;
+    while (live && w.next()) {
       const int row = w.mt * kRows + r;
       const int valid = min(w.kv, w.u.cap);  // cache rows that hold anything
       const int lim = w.u.limit(w.q, w.kv, min(row / p.num_heads, w.q - 1));
       // tiles below this one are seen in full by every row (the first row sees the least)
       const int clean = w.u.limit(w.q, w.kv, w.mt * kRows / p.num_heads) / kTok;
       float m = -INFINITY, l = 0.f, lp = 0.f;
-      for (int j = 0; j < w.n; ++j, ++it) {
-        const int t = w.t0 + j, sb = it & 1;
-        mbar_wait(&aux->s_full[sb], (it >> 1) & 1);
-        if (cta_aborted()) break;
+      float s[32], s_next[32], mx = 0.f, mx_next = 0.f;
+      // scores of a tile from TMEM, masked, and their maximum on its way to the other CTA. The
+      // receiving slot is free: the other CTA's scores of tile i + 4 come after its P V of tile
+      // i + 1, which needs this CTA's P, written after slot i was read.
+      auto fetch = [&](int i, int t, float (&x)[32]) -> float {
+        live = live && mbar_wait_warp(&aux->s_full, i & 1);
+        if (!live) return 0.f;
         tc_fence_after();
         uint32_t sv[32];
-        tmem_ld_32x32b_x32(tbase + lane_off + kColS + sb * 32, sv);
+        tmem_ld_32x32b_x32(tbase + lane_off + kColS, sv);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->s_empty[sb]);
-        float s[32];
+        if (lane == 0) mbar_arrive(&aux->s_empty);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = __uint_as_float(sv[e]);
+        for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(sv[e]);
         if (t >= clean) {
           const int seen = lim - t * kTok - c * kHalfTok;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = e < seen ? s[e] : -INFINITY;
+          for (int e = 0; e < 32; ++e) x[e] = e < seen ? x[e] : -INFINITY;
         }
-        float mx = fmax3f(s[0], s[1], s[2]), my = fmax3f(s[3], s[4], s[5]);
+        float a = fmax3f(x[0], x[1], x[2]), b = fmax3f(x[3], x[4], x[5]);
 #pragma unroll
         for (int e = 6; e < 30; e += 4) {
-          mx = fmax3f(mx, s[e], s[e + 1]);
-          my = fmax3f(my, s[e + 2], s[e + 3]);
+          a = fmax3f(a, x[e], x[e + 1]);
+          b = fmax3f(b, x[e + 2], x[e + 3]);
         }
-        mx = fmax3f(mx, my, fmaxf(s[30], s[31]));
-        st_cluster_f32(peer_max + sb * kRows * 4, mx);
-        __syncwarp();
-        if (lane == 0) mbar_arrive_remote(peer_bar_x + sb * 8);
-        mbar_wait_cluster(&aux->x_full[sb], (it >> 1) & 1);
-        if (cta_aborted()) break;
-        mx = fmaxf(mx, aux->peer_max[sb][r]) * sl2;
+        a = fmax3f(a, b, fmaxf(x[30], x[31]));
+        const int slot = i % kXBuf;
+        if (tid == 0) mbar_arrive_expect_tx(&aux->x_full[slot], kRows * 4);
+        st_async_f32(peer_max + slot * kRows * 4, a, peer_bar_x + slot * 8);
+        return a;
+      };
+      mx = fetch(it, w.t0, s);
+      for (int j = 0; live && j < w.n; ++j, ++it) {
+        const int t = w.t0 + j, pb = it & 1;
+        if (j + 1 < w.n) mx_next = fetch(it + 1, t + 1, s_next);
+        live = live && mbar_wait_cluster_warp(&aux->x_full[it % kXBuf], (it / kXBuf) & 1);
+        if (!live) break;
+        mx = fmaxf(mx, aux->peer_max[it % kXBuf][r]) * sl2;
         // both CTAs take the same decision from the same two maxima
         const bool move = mx > m + 8.f;
         const float dm = move ? ex2(m - mx) : 1.f;  // 0 while nothing has been seen
@@ -513,10 +534,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         }
         l = l * dm + (r0 + r1);
         lp = lp * dm + (p0 + p1);
-        // P of the tile before has been read by both CTAs, and O holds it
-        if (it > 0) mbar_wait_cluster(&aux->pv_done, (it - 1) & 1);
-        if (cta_aborted()) break;
         if (j > 0 && __any_sync(0xffffffffu, move)) {
+          live = mbar_wait_cluster_warp(&aux->pv_done[pb ^ 1], ((it - 1) >> 1) & 1);  // O holds every tile before this one
+          if (!live) break;
           tc_fence_after();
 #pragma unroll 1
           for (int g = 0; g < 8; ++g) {
@@ -530,41 +550,45 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           tmem_wait_st();
           tc_fence_before();
         }
+        // this buffer's last P has been read by both CTAs (and copied)
+        live = it < kPBuf || mbar_wait_cluster_warp(&aux->pv_done[pb], (it / kPBuf - 1) & 1);
+        if (!live) break;
+        uint8_t* dst = half + pb * 2 * kPHalf;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t at = sw128(r, c * 4 + q);
-          *reinterpret_cast<uint4*>(prow + at) = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-          st_cluster_v4(peer_p + at, pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-        }
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(dst + r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) =
+              make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
         if ((t + 1) * kTok > valid) {
           // rows past the request's length may hold NaN: weight 0 does not hide
           // them from the product, so they are cleared
-          const int st = it % kStages;
-          mbar_wait(&aux->c_full[st], (it / kStages) & 1);
-          const int g = tid >> 5, i = lane;
+          live = mbar_wait_warp(&aux->c_full[it % kStagesC], (it / kStagesC) & 1);
+          if (!live) break;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (t * kTok + h * kHalfTok + i < valid) continue;
-            uint4* v = reinterpret_cast<uint4*>(smem + (h == c ? kOffB : kOffC) + st * kBytesV +
-                                                ((i / kR) * 4 + g) * kR * 128 + (i % kR) * 128);
+            if (t * kTok + h * kHalfTok + lane < valid) continue;
+            uint8_t* stage = smem + (h == c ? kOffB + it % kStagesB * kBytesV : kOffC + it % kStagesC * kBytesV);
+            uint4* v = reinterpret_cast<uint4*>(stage + ((lane / kR) * 4 + warp) * kR * 128 + (lane % kR) * 128);
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
-        fence_proxy_async_all();
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&aux->p_full);
-          mbar_arrive_remote(peer_bar_p);
+          bulk_copy_cluster(peer_half + pb * 2 * kPHalf, dst + warp * 2048, 2048, peer_bar_p + pb * 8);
+          mbar_arrive_expect_tx(&aux->p_full[pb], 2048);
         }
+        mx = mx_next;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) s[e] = s_next[e];
       }
-      if (cta_aborted()) break;
+      if (!live) break;
       // the row's sums over both CTAs' cache rows (a sum of two: the same in both CTAs)
       st_cluster_f32(peer_sum, l);
       st_cluster_f32(peer_sum + kRows * 4, lp);
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(peer_bar_l);
-      mbar_wait_cluster(&aux->l_full, pieces & 1);
+      live = mbar_wait_cluster_warp(&aux->l_full, pieces & 1);
       l += aux->peer_sum[0][r];
       lp += aux->peer_sum[1][r];
       aux->inv[pieces & 1][r] = lp > 0.f ? 1.f / lp : 0.f;
@@ -572,8 +596,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       mbar_arrive(&aux->stat_full);
       ++pieces;
     }
-    // the other CTA's last commit has arrived here before this CTA may leave
-    if (it > 0) mbar_wait_cluster(&aux->pv_done, (it - 1) & 1);
+    // the other CTA's last commits (and with them its copies of this CTA's P) have arrived
+    // before this CTA may leave
+    for (int i = max(0, it - kPBuf); live && i < it; ++i)
+      live = mbar_wait_cluster_warp(&aux->pv_done[i & 1], (i >> 1) & 1);
+    if (!live) {
+      // aborting: what is on its way to the other CTA (a few KB) gets a
+      // millisecond, hundreds of times what it takes, before either CTA leaves
+      for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000 * 1000;) {
+      }
+    }
   } else {
     // ------------------------------------------------ query loads, epilogue
     const int r = tid - 128;
@@ -612,10 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       fence_proxy_async_smem();
       mbar_arrive(&aux->q_full);
     };
-    auto store_o = [&](const Walk& x, int piece, int first_tile) {
-      mbar_wait(&aux->stat_full, piece & 1);
-      mbar_wait(&aux->o_full, piece & 1);
-      if (cta_aborted()) return;
+    auto store_o = [&](const Walk& x, int piece, int first_tile) -> bool {
+      if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
       tc_fence_after();
       const float inv = aux->inv[piece & 1][r], lse = aux->lse[piece & 1][r];
       const int row = x.mt * kRows + r;
@@ -666,22 +696,24 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           P.row_info[grow] = info;
         }
       }
+      return true;
     };
     // the next piece's query goes in as soon as the last scores of this one are
     // computed, before this one's epilogue
     bool more = w.next();
     if (more) load_q(w);
     int piece = 0, tiles_before = 0;
-    while (more && !cta_aborted()) {
+    bool live = true;
+    while (live && more) {
       const Walk now = w;
       more = w.next();
       if (more) {
-        mbar_wait(&aux->q_empty, piece & 1);
-        if (cta_aborted()) break;
+        live = mbar_wait_warp(&aux->q_empty, piece & 1);
+        if (!live) break;
         tc_fence_after();
         load_q(w);
       }
-      store_o(now, piece, tiles_before);
+      live = store_o(now, piece, tiles_before);
       tiles_before += now.n;
       ++piece;
     }
