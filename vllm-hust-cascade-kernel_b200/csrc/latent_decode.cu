@@ -21,8 +21,8 @@
 //     softmax warps for about 4,000 cycles a tile).
 // Per 64 cache rows a CTA loads its own 32 rows in full (keys, and its columns
 // of V) and its columns of the other 32: 52 KB for 36 KB from HBM.
-// Seven of the query tile's nine groups of 64 dims live in TMEM (224 columns),
-// two in shared memory: with A in shared memory a 128 x 32 x 16 MMA takes 43
+// Six of the query tile's nine groups of 64 dims live in TMEM (192 columns),
+// three in shared memory: with A in shared memory a 128 x 32 x 16 MMA takes 43
 // cycles (A's 4 KB), in TMEM 19.
 //
 // Softmax: running maximum m in the log2 domain that moves only when a score
@@ -38,8 +38,9 @@
 // A unit cut by a run boundary leaves fp32 partials that a second, dependent
 // launch merges in run order; all others are written directly.
 //
-// Warps: 0-3 softmax (thread = row = TMEM lane), 4-7 query loads and
-// epilogue, 8 keys (TMA), 9 MMA issue, 10 the other CTA's rows (TMA).
+// Warps: 0-3 softmax (thread = row = TMEM lane), 4-7 query tile and epilogue,
+// 8 keys (TMA), 9 MMA issue (one issuer: the two kinds of MMA interleaved from
+// two take a fifth longer), 10 the other CTA's rows (TMA).
 #include <algorithm>
 
 #include "kernels.h"
@@ -54,22 +55,24 @@ constexpr int kHalfTok = 32;   // per CTA
 constexpr int kThreads = 11 * 32;
 constexpr int kMaxClusters = kNumSMs / 2;
 
-constexpr int kStagesA = 2, kStagesB = 4, kStagesC = 3;  // keys outside the own columns; own columns; the other rows
+constexpr int kStagesA = 2, kStagesB = 4, kStagesC = 2;  // keys outside the own columns; own columns; the other rows
 constexpr int kPBuf = 2, kXBuf = 4;
+static_assert(kStagesA == 2 && kStagesB == 4 && kStagesC <= 4, "the barriers that free the stages");
 constexpr int kGroup = kHalfTok * 128;    // 32 cache rows x 64 dims
 constexpr int kBytesA = 5 * kGroup;       // keys outside the CTA's own columns
 constexpr int kBytesV = 4 * kGroup;       // the CTA's own columns
 constexpr int kQGroup = kRows * 128;      // 128 query rows x 64 dims
-constexpr int kQTmem = 7;                 // groups of 64 dims in TMEM, the last two in shared memory
+constexpr int kQTmem = 6;                 // groups of 64 dims in TMEM, the last three in shared memory
 constexpr int kPHalf = kRows * kHalfTok * 2;  // P of one CTA's cache rows
 constexpr int kOffQ = 0;
 constexpr int kOffP = kOffQ + (9 - kQTmem) * kQGroup;
 constexpr int kOffA = kOffP + kPBuf * 2 * kPHalf;
 constexpr int kOffB = kOffA + kStagesA * kBytesA;
 constexpr int kOffC = kOffB + kStagesB * kBytesV;
-constexpr int kOffAux = kOffC + kStagesC * kBytesV;
+constexpr int kOffE = kOffC + kStagesC * kBytesV;  // epilogue: per warp 32 rows x 32 bytes
+constexpr int kOffAux = kOffE + 4 * 1024;
 
-constexpr uint32_t kColO = 0, kColQ = 256, kColS = 480;  // TMEM columns: O 256, Q 224, S 32
+constexpr uint32_t kColO = 0, kColQ = 256, kColS = 448;  // TMEM columns: O 256, Q 192, S 2 x 32
 
 struct Sched {
   int64_t tiles, begin;  // all tiles; this cluster's first
@@ -82,9 +85,14 @@ struct __align__(16) Aux {
   float peer_sum[2][kRows];  // exponentials, rounded P
   float inv[2][kRows];       // 1 / sum, per unit parity
   float lse[2][kRows];
-  uint64_t a_full[kStagesA], a_empty[kStagesA], b_full[kStagesB], b_empty[kStagesB], c_full[kStagesC], c_empty[kStagesC];
-  uint64_t q_full, q_empty, s_full, s_empty, x_full[kXBuf], p_full[kPBuf], pv_done[kPBuf], o_full, o_empty, stat_full;
-  uint64_t l_full;
+  // One commit per MMA batch serves all that wait for it (a commit costs the
+  // tensor pipe 60 to 100 cycles): s_full[it % 2] = scores of tile it done (the
+  // softmax, and the keys' next load), pv_done[it % 4] = P V of tile it done in
+  // both CTAs (P, own columns, other rows). A waiter is never two phases behind:
+  // the next phase needs what it is about to do.
+  uint64_t kv_full[kStagesB], c_full[kStagesC];
+  uint64_t q_full, q_empty, s_full[2], s_empty[2], x_full[kXBuf], p_full[kPBuf], pv_done[4], o_full, o_empty, stat_full;
+  uint64_t l_full, qs_full[3], qs_empty[3];
   uint64_t stall, drain;
   uint32_t tmem_base;
   Sched sched;
@@ -96,6 +104,7 @@ static_assert(kSmemBytes + 16 <= 227 * 1024, "shared memory per CTA");
 struct Params {
   LatentDecodeLaunch L;
   CUtensorMap map4, map1;  // boxes of 64 dims x kR cache rows x 4 groups (1 group)
+  CUtensorMap map_q;       // 64 dims x 128 query rows
   int32_t* row_info;       // [tokens x heads]: how the row's partials are found, 0 = none
   float* part_o;           // [2 clusters][128][512]
   float* part_lse;         // [2 clusters][128]
@@ -282,19 +291,20 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 
   if (tid == 0) {
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
-    for (int s = 0; s < kStagesA; ++s) mbar_init(&aux->a_full[s], 1), mbar_init(&aux->a_empty[s], 1);
-    for (int s = 0; s < kStagesB; ++s) mbar_init(&aux->b_full[s], 1), mbar_init(&aux->b_empty[s], 1);
-    for (int s = 0; s < kStagesC; ++s) mbar_init(&aux->c_full[s], 1), mbar_init(&aux->c_empty[s], 1);
+    for (int s = 0; s < kStagesB; ++s) mbar_init(&aux->kv_full[s], 1);
+    for (int s = 0; s < kStagesC; ++s) mbar_init(&aux->c_full[s], 1);
     for (int s = 0; s < kXBuf; ++s) mbar_init(&aux->x_full[s], 1);
-    for (int s = 0; s < kPBuf; ++s) mbar_init(&aux->p_full[s], 4), mbar_init(&aux->pv_done[s], 2);
-    mbar_init(&aux->s_full, 1);
-    mbar_init(&aux->s_empty, 4);
+    for (int s = 0; s < kPBuf; ++s) mbar_init(&aux->p_full[s], 4), mbar_init(&aux->s_full[s], 1);
+    for (int s = 0; s < 4; ++s) mbar_init(&aux->pv_done[s], 2);
+    mbar_init(&aux->s_empty[0], 4);
+    mbar_init(&aux->s_empty[1], 4);
     mbar_init(&aux->q_full, 128);
     mbar_init(&aux->q_empty, 1);
     mbar_init(&aux->o_full, 1);
     mbar_init(&aux->o_empty, 128);
     mbar_init(&aux->stat_full, 128);
     mbar_init(&aux->l_full, 4);
+    for (int s = 0; s < 3; ++s) mbar_init(&aux->qs_full[s], 1), mbar_init(&aux->qs_empty[s], 4);
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
@@ -316,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // its own; 10: the other CTA's 32 rows, own columns
     const bool keys = warp == 8;
     PageRows<kR> rows(p, keys ? c : 1 - c);
-    int it = 0, issued_a = 0, issued_v = 0;
+    int it = 0, issued = 0;
     bool live = true;
     while (live && w.next()) {
       rows.start(w.b, w.kv);
@@ -324,66 +334,54 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         int y[PageRows<kR>::kPer];
 #pragma unroll
         for (int i = 0; i < PageRows<kR>::kPer; ++i) y[i] = rows.get(t, i, lane);
-        if (keys) {
-          const int st = it % kStagesA;
-          live = it < kStagesA || mbar_wait_warp(&aux->a_empty[st], (it / kStagesA - 1) & 1);
-          if (!live) break;
-          if (lane == 0) {
-            uint8_t* dst = smem + kOffA + st * kBytesA;
-            mbar_arrive_expect_tx(&aux->a_full[st], kBytesA);
-#pragma unroll
-            for (int i = 0; i < PageRows<kR>::kPer; ++i) {
-              tma_load_3d(dst + i * kR * 512, &P.map4, &aux->a_full[st], 0, y[i], 4 * (1 - c));
-              tma_load_3d(dst + 4 * kGroup + i * kR * 128, &P.map1, &aux->a_full[st], 0, y[i], 8);
-            }
-          }
-          ++issued_a;
-          __syncwarp();
-        }
         const int stages = keys ? kStagesB : kStagesC, st = it % stages;
-        uint64_t* full = keys ? &aux->b_full[st] : &aux->c_full[st];
-        live = it < stages || mbar_wait_warp(keys ? &aux->b_empty[st] : &aux->c_empty[st], (it / stages - 1) & 1);
+        live = it < stages || mbar_wait_cluster_warp(&aux->pv_done[(it - stages) & 3], ((it - stages) >> 2) & 1);
+        if (keys) live = live && (it < 2 || mbar_wait_warp(&aux->s_full[it & 1], ((it >> 1) - 1) & 1));
         if (!live) break;
         if (lane == 0) {
+          uint64_t* full = keys ? &aux->kv_full[st] : &aux->c_full[st];
           uint8_t* dst = smem + (keys ? kOffB : kOffC) + st * kBytesV;
-          mbar_arrive_expect_tx(full, kBytesV);
+          uint8_t* dsta = smem + kOffA + (it & 1) * kBytesA;
+          mbar_arrive_expect_tx(full, keys ? kBytesA + kBytesV : kBytesV);
 #pragma unroll
-          for (int i = 0; i < PageRows<kR>::kPer; ++i)
+          for (int i = 0; i < PageRows<kR>::kPer; ++i) {
+            if (keys) {
+              tma_load_3d(dsta + i * kR * 512, &P.map4, full, 0, y[i], 4 * (1 - c));
+              tma_load_3d(dsta + 4 * kGroup + i * kR * 128, &P.map1, full, 0, y[i], 8);
+            }
             tma_load_3d(dst + i * kR * 512, &P.map4, full, 0, y[i], 4 * c);
+          }
         }
-        ++issued_v;
+        ++issued;
         __syncwarp();
       }
     }
     // aborting: every load issued has landed before the CTA leaves
     if (!live && lane == 0) {
-      for (int j = max(0, issued_a - kStagesA); j < issued_a; ++j)
-        mbar_wait_drain(&aux->a_full[j % kStagesA], (j / kStagesA) & 1);
       const int stages = keys ? kStagesB : kStagesC;
-      for (int j = max(0, issued_v - stages); j < issued_v; ++j)
-        mbar_wait_drain(keys ? &aux->b_full[j % stages] : &aux->c_full[j % stages], (j / stages) & 1);
+      for (int j = max(0, issued - stages); j < issued; ++j)
+        mbar_wait_drain(keys ? &aux->kv_full[j % stages] : &aux->c_full[j % stages], (j / stages) & 1);
     }
   } else if (warp == 9) {
     // ----------------------------------------------------------- MMA issuer
-    // the whole warp walks; one elected lane issues
-    constexpr uint32_t fmt = kFp16 ? 0u : 1u;
+    // the whole warp walks and waits; one elected lane issues. Scores run two
+    // tiles ahead of P V, within a piece.
     constexpr int kPer = kHalfTok / kR;
-    const uint32_t idesc_s = make_idesc_f16(kRows, kR, fmt, 0, 0);
-    const uint32_t idesc_pv = make_idesc_f16(kRows, 256, fmt, 0, 1);
-    const uint32_t tm = uniform(tbase), rank = uniform(static_cast<uint32_t>(c));
-    const uint32_t s0 = uniform(smem_u32(smem));
+    const uint32_t idesc_s = make_idesc_f16(kRows, kR, kFp16 ? 0u : 1u, 0, 0);
+    const uint32_t idesc_pv = make_idesc_f16(kRows, 256, kFp16 ? 0u : 1u, 0, 1);
+    const uint32_t tm = uniform(tbase), rank = uniform(static_cast<uint32_t>(c)), s0 = uniform(smem_u32(smem));
+    const uint64_t dq = make_smem_desc(s0 + kOffQ, 16, 1024, 2);
     int pieces = 0;
     auto scores = [&](int it, bool first, bool last) -> bool {
-      const uint32_t sa = uniform(it % kStagesA), sb = uniform(it % kStagesB);
+      const uint32_t sa = uniform(it & 1), sb = uniform(it & 3);
       if ((first && !mbar_wait_warp(&aux->q_full, pieces & 1)) ||
-          !mbar_wait_warp(&aux->b_full[sb], (it / kStagesB) & 1) ||
-          !mbar_wait_warp(&aux->a_full[sa], (it / kStagesA) & 1) ||
-          (it > 0 && !mbar_wait_warp(&aux->s_empty, (it - 1) & 1)))
+          (it >= 2 && !mbar_wait_warp(&aux->s_empty[sa], ((it >> 1) - 1) & 1)) ||
+          !mbar_wait_warp(&aux->kv_full[sb], (it >> 2) & 1))
         return false;
       tc_fence_after();
       const uint64_t da = make_smem_desc(s0 + kOffA + sa * kBytesA, 16, 1024, 2);
       const uint64_t db = make_smem_desc(s0 + kOffB + sb * kBytesV, 16, 1024, 2);
-      const uint64_t dq = make_smem_desc(s0 + kOffQ, 16, 1024, 2);
+      const uint32_t d = tm + kColS + sa * 32;
       __syncwarp();
       if (elect_one()) {
 #pragma unroll
@@ -396,24 +394,23 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if (g < kQTmem)
-                umma_f16_ts(tm + kColS + i * kR, tm + kColQ + g * 32 + k * 8, k0 + k * 2, idesc_s, g + k > 0);
+                umma_f16_ts(d + i * kR, tm + kColQ + g * 32 + k * 8, k0 + k * 2, idesc_s, g + k > 0);
               else
-                umma_f16_ss(tm + kColS + i * kR, dq + ((g - kQTmem) * kQGroup + k * 32) / 16, k0 + k * 2, idesc_s, 1u);
+                umma_f16_ss(d + i * kR, dq + ((g - kQTmem) * kQGroup + k * 32) / 16, k0 + k * 2, idesc_s, 1u);
             }
           }
         }
-        umma_commit(&aux->a_empty[sa]);
-        umma_commit(&aux->s_full);
+        umma_commit(&aux->s_full[sa]);
         if (last) umma_commit(&aux->q_empty);
       }
       __syncwarp();
       return true;
     };
     auto values = [&](int it, bool first, bool last) -> bool {
-      const uint32_t sb = uniform(it % kStagesB), sc = uniform(it % kStagesC), pb = uniform(it & 1);
-      if (!mbar_wait_warp(&aux->c_full[sc], (it / kStagesC) & 1) ||
-          !mbar_wait_cluster_warp(&aux->p_full[pb], (it >> 1) & 1) ||
-          (first && pieces > 0 && !mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1)))
+      const uint32_t sb = uniform(it & 3), sc = uniform(it % kStagesC), pb = uniform(it & 1);
+      if ((first && pieces > 0 && !mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1)) ||
+          !mbar_wait_warp(&aux->c_full[sc], (it / kStagesC) & 1) ||
+          !mbar_wait_cluster_warp(&aux->p_full[pb], (it >> 1) & 1))
         return false;
       tc_fence_after();
       const uint32_t own = s0 + kOffB + sb * kBytesV, other = s0 + kOffC + sc * kBytesV;
@@ -430,9 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             umma_f16_ss(tm + kColO, dp + (h * kPHalf + k * 32) / 16,
                         (h ? dv1 : dv0) + (kR == 32 ? k * 2048 : k * 4 * kR * 128) / 16, idesc_pv, !first || h + k > 0);
         }
-        umma_commit(&aux->b_empty[sb]);
-        umma_commit(&aux->c_empty[sc]);
-        umma_commit_cluster(&aux->pv_done[pb], 3);
+        umma_commit_cluster(&aux->pv_done[sb], 3);
         if (last) umma_commit(&aux->o_full);
       }
       __syncwarp();
@@ -441,7 +436,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     int it = 0;
     bool live = true;
     while (live && w.next()) {
-      // scores run two tiles ahead of values, within a piece
       live = scores(it, true, w.n == 1) && (w.n == 1 || scores(it + 1, false, w.n == 2));
       for (int j = 0; live && j < w.n; ++j, ++it)
         live = (j + 2 >= w.n || scores(it + 2, false, j + 3 == w.n)) && values(it, j == 0, j + 1 == w.n);
@@ -475,44 +469,43 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       // tiles below this one are seen in full by every row (the first row sees the least)
       const int clean = w.u.limit(w.q, w.kv, w.mt * kRows / p.num_heads) / kTok;
       float m = -INFINITY, l = 0.f, lp = 0.f;
-      float s[32], s_next[32], mx = 0.f, mx_next = 0.f;
+      float s[32];
       // scores of a tile from TMEM, masked, and their maximum on its way to the other CTA. The
       // receiving slot is free: the other CTA's scores of tile i + 4 come after its P V of tile
       // i + 1, which needs this CTA's P, written after slot i was read.
-      auto fetch = [&](int i, int t, float (&x)[32]) -> float {
-        live = live && mbar_wait_warp(&aux->s_full, i & 1);
-        if (!live) return 0.f;
+      auto fetch = [&](int i, int t) -> float {
         tc_fence_after();
         uint32_t sv[32];
-        tmem_ld_32x32b_x32(tbase + lane_off + kColS, sv);
+        tmem_ld_32x32b_x32(tbase + lane_off + kColS + (i & 1) * 32, sv);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->s_empty);
+        if (lane == 0) mbar_arrive(&aux->s_empty[i & 1]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(sv[e]);
+        for (int e = 0; e < 32; ++e) s[e] = __uint_as_float(sv[e]);
         if (t >= clean) {
           const int seen = lim - t * kTok - c * kHalfTok;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = e < seen ? x[e] : -INFINITY;
+          for (int e = 0; e < 32; ++e) s[e] = e < seen ? s[e] : -INFINITY;
         }
-        float a = fmax3f(x[0], x[1], x[2]), b = fmax3f(x[3], x[4], x[5]);
+        float a = fmax3f(s[0], s[1], s[2]), b = fmax3f(s[3], s[4], s[5]);
 #pragma unroll
         for (int e = 6; e < 30; e += 4) {
-          a = fmax3f(a, x[e], x[e + 1]);
-          b = fmax3f(b, x[e + 2], x[e + 3]);
+          a = fmax3f(a, s[e], s[e + 1]);
+          b = fmax3f(b, s[e + 2], s[e + 3]);
         }
-        a = fmax3f(a, b, fmaxf(x[30], x[31]));
+        a = fmax3f(a, b, fmaxf(s[30], s[31]));
         const int slot = i % kXBuf;
         if (tid == 0) mbar_arrive_expect_tx(&aux->x_full[slot], kRows * 4);
         st_async_f32(peer_max + slot * kRows * 4, a, peer_bar_x + slot * 8);
         return a;
       };
-      mx = fetch(it, w.t0, s);
+      live = mbar_wait_warp(&aux->s_full[it & 1], (it >> 1) & 1);
+      if (!live) break;
+      float mx = fetch(it, w.t0);
       for (int j = 0; live && j < w.n; ++j, ++it) {
         const int t = w.t0 + j, pb = it & 1;
-        if (j + 1 < w.n) mx_next = fetch(it + 1, t + 1, s_next);
-        live = live && mbar_wait_cluster_warp(&aux->x_full[it % kXBuf], (it / kXBuf) & 1);
+        live = mbar_wait_cluster_warp(&aux->x_full[it % kXBuf], (it / kXBuf) & 1);
         if (!live) break;
         mx = fmaxf(mx, aux->peer_max[it % kXBuf][r]) * sl2;
         // both CTAs take the same decision from the same two maxima
@@ -535,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         l = l * dm + (r0 + r1);
         lp = lp * dm + (p0 + p1);
         if (j > 0 && __any_sync(0xffffffffu, move)) {
-          live = mbar_wait_cluster_warp(&aux->pv_done[pb ^ 1], ((it - 1) >> 1) & 1);  // O holds every tile before this one
+          live = mbar_wait_cluster_warp(&aux->pv_done[(it - 1) & 3], ((it - 1) >> 2) & 1);  // O holds every tile before this one
           if (!live) break;
           tc_fence_after();
 #pragma unroll 1
@@ -551,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           tc_fence_before();
         }
         // this buffer's last P has been read by both CTAs (and copied)
-        live = it < kPBuf || mbar_wait_cluster_warp(&aux->pv_done[pb], (it / kPBuf - 1) & 1);
+        live = it < kPBuf || mbar_wait_cluster_warp(&aux->pv_done[(it - kPBuf) & 3], ((it - kPBuf) >> 2) & 1);
         if (!live) break;
         uint8_t* dst = half + pb * 2 * kPHalf;
 #pragma unroll
@@ -578,9 +571,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           bulk_copy_cluster(peer_half + pb * 2 * kPHalf, dst + warp * 2048, 2048, peer_bar_p + pb * 8);
           mbar_arrive_expect_tx(&aux->p_full[pb], 2048);
         }
-        mx = mx_next;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = s_next[e];
+        // the next tile's scores, and its maximum on its way
+        if (j + 1 < w.n) {
+          live = mbar_wait_warp(&aux->s_full[(it + 1) & 1], ((it + 1) >> 1) & 1);
+          if (!live) break;
+          mx = fetch(it + 1, t + 1);
+        }
       }
       if (!live) break;
       // the row's sums over both CTAs' cache rows (a sum of two: the same in both CTAs)
@@ -599,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // the other CTA's last commits (and with them its copies of this CTA's P) have arrived
     // before this CTA may leave
     for (int i = max(0, it - kPBuf); live && i < it; ++i)
-      live = mbar_wait_cluster_warp(&aux->pv_done[i & 1], (i >> 1) & 1);
+      live = mbar_wait_cluster_warp(&aux->pv_done[i & 3], (i >> 2) & 1);
     if (!live) {
       // aborting: what is on its way to the other CTA (a few KB) gets a
       // millisecond, hundreds of times what it takes, before either CTA leaves
@@ -611,38 +607,52 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     const int r = tid - 128;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int64_t all_rows = p.num_tokens * p.num_heads;
-    auto load_q = [&](const Walk& x) {
-      const int row = x.mt * kRows + r;
-      const int64_t grow = x.tok * p.num_heads + row;
-      const bool ok = row < x.q * p.num_heads && grow < all_rows;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) + (ok ? grow : 0) * kLatentRow);
-#pragma unroll 1
+    // Query tile: the nine groups of 64 dims come by TMA, group g into slot g % 3 of 16 KB; six
+    // move on to TMEM, the last three stay. (Loads of a row per thread touch 32 lines per
+    // instruction: 14,000 cycles in which the softmax stood still too.)
+    int loads = 0;  // issued, by one lane
+    auto load_group = [&](const Walk& x, int g) {
+      // group order: the CTA's own columns, the other latent ones, the rotary part
+      const int col = g < 4 ? 4 * c + g : g < 8 ? 4 * (1 - c) + g - 4 : 8;
+      mbar_arrive_expect_tx(&aux->qs_full[g % 3], kQGroup);
+      tma_load_3d(smem + kOffQ + g % 3 * kQGroup, &P.map_q, &aux->qs_full[g % 3], 0,
+                  static_cast<int>(x.tok * p.num_heads + x.mt * kRows), col);
+      ++loads;
+    };
+    auto place_q = [&](const Walk& x, int piece) -> bool {
+      if (tid == 128)
+        for (int g = 0; g < 3; ++g) load_group(x, g);
       for (int g = 0; g < 9; ++g) {
-        // group order: the CTA's own columns, the other latent ones, the rotary part
-        const int col = g < 4 ? 4 * c + g : g < 8 ? 4 * (1 - c) + g - 4 : 8;
-        uint4 v[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = ok ? __ldg(src + col * 8 + k) : make_uint4(0u, 0u, 0u, 0u);
-        if (g < kQTmem) {
+        bool ok = mbar_wait_warp(&aux->qs_full[g % 3], (piece * 3 + g / 3) & 1);
+        if (ok && g < kQTmem) {
           uint32_t x32[32];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            x32[4 * k] = v[k].x;
-            x32[4 * k + 1] = v[k].y;
-            x32[4 * k + 2] = v[k].z;
-            x32[4 * k + 3] = v[k].w;
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + kOffQ + g % 3 * kQGroup + sw128(r, k));
+            x32[4 * k] = v.x;
+            x32[4 * k + 1] = v.y;
+            x32[4 * k + 2] = v.z;
+            x32[4 * k + 3] = v.w;
           }
           tmem_st_32x32b_x32(tbase + lane_off + kColQ + g * 32, x32);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            *reinterpret_cast<uint4*>(smem + kOffQ + (g - kQTmem) * kQGroup + sw128(r, k)) = v[k];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&aux->qs_empty[g % 3]);
+          if (warp == 4) {
+            ok = mbar_wait_warp(&aux->qs_empty[g % 3], (piece * 2 + g / 3) & 1);
+            if (ok && lane == 0) load_group(x, g + 3);
+            __syncwarp();
+          }
+        }
+        if (!ok) {
+          // aborting: the loads in flight land before the CTA leaves
+          for (int i = max(0, loads - 3); i < loads; ++i) mbar_wait_drain(&aux->qs_full[i % 3], (i / 3) & 1);
+          return false;
         }
       }
       tmem_wait_st();
       tc_fence_before();
-      fence_proxy_async_smem();
       mbar_arrive(&aux->q_full);
+      return true;
     };
     auto store_o = [&](const Walk& x, int piece, int first_tile) -> bool {
       if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
@@ -653,10 +663,32 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       const bool ok = row < x.q * p.num_heads && grow < all_rows;
       const bool whole = x.starts && x.ends;
       const int64_t slot = 2 * cluster + (x.starts ? 1 : 0);
+      // 32 bytes per row at a time through shared memory, so that a store instruction writes whole
+      // sectors of 16 rows (16-byte half h of row r at h ^ (r / 4 % 2): no bank conflicts)
+      uint8_t* stage = smem + kOffE + (warp & 3) * 1024;
+      const int row0 = x.mt * kRows + (r & ~31);  // this warp's first row of the unit
+      const int rows = min(32, static_cast<int>(min(static_cast<int64_t>(x.q) * p.num_heads - row0,
+                                                    all_rows - (x.tok * p.num_heads + row0))));
+      uint8_t* dst = whole ? static_cast<uint8_t*>(p.out) + (x.tok * p.num_heads + row0) * (kLatentDim * 2) + 512 * c
+                           : reinterpret_cast<uint8_t*>(P.part_o) +
+                                 (slot * kRows + (r & ~31)) * (kLatentDim * 4) + 1024 * c;
+      const int pitch = whole ? kLatentDim * 2 : kLatentDim * 4;
+      auto put = [&](int part, uint4 a, uint4 b) {
+        const int swap = (lane >> 2) & 1;
+        *reinterpret_cast<uint4*>(stage + lane * 32 + swap * 16) = a;
+        *reinterpret_cast<uint4*>(stage + lane * 32 + (swap ^ 1) * 16) = b;
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int rr = q * 16 + (lane >> 1);
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 32 + (((lane & 1) ^ ((rr >> 2) & 1)) << 4));
+          if (rr < rows) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(rr) * pitch + part * 32 + (lane & 1) * 16) = v;
+        }
+        __syncwarp();
+      };
 #pragma unroll 1
       for (int g = 0; g < 8; ++g) {
         uint32_t o[32];
-        __syncwarp();
         tmem_ld_32x32b_x32(tbase + lane_off + kColO + g * 32, o);
         tmem_wait_ld();
         if (g == 7) {
@@ -666,16 +698,20 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         float f[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) f[e] = inv > 0.f ? __uint_as_float(o[e]) * inv : 0.f;
-        if (ok && whole) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + grow * kLatentDim + 256 * c + g * 32);
+        if (whole) {
+          auto four = [&](int e) {
+            return make_uint4(pack2<kFp16>(f[e], f[e + 1]), pack2<kFp16>(f[e + 2], f[e + 3]),
+                              pack2<kFp16>(f[e + 4], f[e + 5]), pack2<kFp16>(f[e + 6], f[e + 7]));
+          };
+          put(g * 2, four(0), four(8));
+          put(g * 2 + 1, four(16), four(24));
+        } else {
+          auto four = [&](int e) {
+            return make_uint4(__float_as_uint(f[e]), __float_as_uint(f[e + 1]), __float_as_uint(f[e + 2]),
+                              __float_as_uint(f[e + 3]));
+          };
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            dst[q] = make_uint4(pack2<kFp16>(f[8 * q], f[8 * q + 1]), pack2<kFp16>(f[8 * q + 2], f[8 * q + 3]),
-                                pack2<kFp16>(f[8 * q + 4], f[8 * q + 5]), pack2<kFp16>(f[8 * q + 6], f[8 * q + 7]));
-        } else if (ok) {
-          float4* dst = reinterpret_cast<float4*>(P.part_o + (slot * kRows + r) * kLatentDim + 256 * c + g * 32);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) dst[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+          for (int q = 0; q < 4; ++q) put(g * 4 + q, four(8 * q), four(8 * q + 4));
         }
       }
       if (ok && c == 0) {
@@ -701,9 +737,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // the next piece's query goes in as soon as the last scores of this one are
     // computed, before this one's epilogue
     bool more = w.next();
-    if (more) load_q(w);
+    bool live = !more || place_q(w, 0);
     int piece = 0, tiles_before = 0;
-    bool live = true;
     while (live && more) {
       const Walk now = w;
       more = w.next();
@@ -711,7 +746,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         live = mbar_wait_warp(&aux->q_empty, piece & 1);
         if (!live) break;
         tc_fence_after();
-        load_q(w);
+        live = place_q(w, piece + 1);
+        if (!live) break;
       }
       live = store_o(now, piece, tiles_before);
       tiles_before += now.n;
@@ -847,7 +883,9 @@ cudaError_t launch_latent_decode(const LatentDecodeLaunch& p, bool fp16, void* w
   const void* base = p.num_blocks > 0 ? p.cache : p.query;
   const uint64_t extent[3] = {64, pool_rows, 9}, stride[2] = {kLatentRow * 2, 128};
   if (!encode_tmap_3d(&P.map4, base, extent, stride, {64, rows, 4}) ||
-      !encode_tmap_3d(&P.map1, base, extent, stride, {64, rows, 1}))
+      !encode_tmap_3d(&P.map1, base, extent, stride, {64, rows, 1}) ||
+      !encode_tmap_3d(&P.map_q, p.query, {64, static_cast<uint64_t>(p.num_tokens) * p.num_heads, 9}, stride,
+                      {64, kRows, 1}))
     return cudaErrorInvalidValue;
   if (rows == 16) return fp16 ? launch<true, 16>(P, stream) : launch<false, 16>(P, stream);
   return fp16 ? launch<true, 32>(P, stream) : launch<false, 32>(P, stream);

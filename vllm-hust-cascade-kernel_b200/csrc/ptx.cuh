@@ -206,6 +206,14 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* desc, 
       : "memory");
 }
 
+// The same box into L2 only.
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* desc, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(desc)),
+               "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 // Same, with an L2 cache-policy hint (e.g. evict_first for streamed KV).
 __device__ __forceinline__ void tma_load_2d_hint(void* dst, const CUtensorMap* desc, uint64_t* bar, int32_t x,
                                                  int32_t y, uint64_t policy) {
