@@ -38,9 +38,10 @@
 // A unit cut by a run boundary leaves fp32 partials that a second, dependent
 // launch merges in run order; all others are written directly.
 //
-// Warps: 0-3 softmax (thread = row = TMEM lane), 4-7 query tile and epilogue,
-// 8 keys (TMA), 9 MMA issue (one issuer: the two kinds of MMA interleaved from
-// two take a fifth longer), 10 the other CTA's rows (TMA).
+// Warps: 0-7 softmax (two threads per row = TMEM lane, 16 of the CTA's 32 cache
+// rows each: with one, its 1,900 cycles a tile set the pace), 8-11 query tile
+// and epilogue, 12 keys (TMA), 13 MMA issue (one issuer: the two kinds of MMA
+// interleaved from two take a fifth longer), 14 the other CTA's rows (TMA).
 #include <algorithm>
 
 #include "kernels.h"
@@ -52,25 +53,25 @@ namespace {
 constexpr int kRows = 128;     // query rows per tile
 constexpr int kTok = 64;       // cache rows per tile
 constexpr int kHalfTok = 32;   // per CTA
-constexpr int kThreads = 11 * 32;
+constexpr int kThreads = 15 * 32;
 constexpr int kMaxClusters = kNumSMs / 2;
 
 constexpr int kStagesA = 2, kStagesB = 4, kStagesC = 2;  // keys outside the own columns; own columns; the other rows
-constexpr int kPBuf = 2, kXBuf = 4;
+constexpr int kPBuf = 2;
 static_assert(kStagesA == 2 && kStagesB == 4 && kStagesC <= 4, "the barriers that free the stages");
 constexpr int kGroup = kHalfTok * 128;    // 32 cache rows x 64 dims
 constexpr int kBytesA = 5 * kGroup;       // keys outside the CTA's own columns
 constexpr int kBytesV = 4 * kGroup;       // the CTA's own columns
 constexpr int kQGroup = kRows * 128;      // 128 query rows x 64 dims
 constexpr int kQTmem = 6;                 // groups of 64 dims in TMEM, the last three in shared memory
-constexpr int kPHalf = kRows * kHalfTok * 2;  // P of one CTA's cache rows
+constexpr int kPPart = kRows * 16 * 2;        // P of 16 cache rows: one K step of the second product
 constexpr int kOffQ = 0;
 constexpr int kOffP = kOffQ + (9 - kQTmem) * kQGroup;
-constexpr int kOffA = kOffP + kPBuf * 2 * kPHalf;
+constexpr int kOffA = kOffP + kPBuf * 4 * kPPart;
 constexpr int kOffB = kOffA + kStagesA * kBytesA;
 constexpr int kOffC = kOffB + kStagesB * kBytesV;
 constexpr int kOffE = kOffC + kStagesC * kBytesV;  // epilogue: per warp 32 rows x 32 bytes
-constexpr int kOffAux = kOffE + 4 * 1024;
+constexpr int kTiles = kOffE + 4 * 1024;           // bytes from the first 1 KB boundary after Aux
 
 constexpr uint32_t kColO = 0, kColQ = 256, kColS = 448;  // TMEM columns: O 256, Q 192, S 2 x 32
 
@@ -81,25 +82,29 @@ struct Sched {
 };
 
 struct __align__(16) Aux {
-  float peer_max[kXBuf][kRows];  // written by the other CTA
-  float peer_sum[2][kRows];  // exponentials, rounded P
-  float inv[2][kRows];       // 1 / sum, per unit parity
-  float lse[2][kRows];
+  // What the four threads of a row (two per CTA) tell one another, in both CTAs: their maxima of a tile, their sums of
+  // a piece. Three slots: a thread tells the maximum of tile n + 3 when its scores are there; they were computed after
+  // P V of tile n, which needed the partners' P of tile n, written after they had read exchange n.
+  union {
+    float shared[3][4][kRows];
+    int64_t scan[2][kThreads / 32];  // find_run only
+  };
+  float inv[kRows];  // 1 / sum of the last piece
   // One commit per MMA batch serves all that wait for it (a commit costs the
   // tensor pipe 60 to 100 cycles): s_full[it % 2] = scores of tile it done (the
   // softmax, and the keys' next load), pv_done[it % 4] = P V of tile it done in
   // both CTAs (P, own columns, other rows). A waiter is never two phases behind:
   // the next phase needs what it is about to do.
   uint64_t kv_full[kStagesB], c_full[kStagesC];
-  uint64_t q_full, q_empty, s_full[2], s_empty[2], x_full[kXBuf], p_full[kPBuf], pv_done[4], o_full, o_empty, stat_full;
-  uint64_t l_full, qs_full[3], qs_empty[3];
+  uint64_t q_full, q_empty, s_full[2], s_empty[2], x_full[3], p_full[kPBuf], pv_done[4], o_full, o_empty, stat_full;
+  uint64_t qs_full[3], qs_empty[3];
   uint64_t stall, drain;
   uint32_t tmem_base;
   Sched sched;
-  int64_t scan[2][kThreads / 32];
 };
-constexpr int kSmemBytes = kOffAux + static_cast<int>(sizeof(Aux)) + 1024;
-static_assert(kSmemBytes + 16 <= 227 * 1024, "shared memory per CTA");
+constexpr int kStaticBytes = 32;  // the wait state comes first
+constexpr int kSmemBytes = (kStaticBytes + static_cast<int>(sizeof(Aux)) + 1023) / 1024 * 1024 + kTiles - kStaticBytes;
+static_assert(kSmemBytes + kStaticBytes <= 227 * 1024, "shared memory per CTA");
 
 struct Params {
   LatentDecodeLaunch L;
@@ -283,8 +288,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   pdl_launch_dependents();
   const LatentDecodeLaunch& p = P.L;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Aux* aux = reinterpret_cast<Aux*>(smem + kOffAux);
+  Aux* aux = reinterpret_cast<Aux*>(smem_raw);
+  uint8_t* smem = smem_raw + sizeof(Aux) + ((0u - (smem_u32(smem_raw) + static_cast<uint32_t>(sizeof(Aux)))) & 1023u);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int c = static_cast<int>(cluster_cta_rank());
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
@@ -293,23 +298,22 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
     for (int s = 0; s < kStagesB; ++s) mbar_init(&aux->kv_full[s], 1);
     for (int s = 0; s < kStagesC; ++s) mbar_init(&aux->c_full[s], 1);
-    for (int s = 0; s < kXBuf; ++s) mbar_init(&aux->x_full[s], 1);
-    for (int s = 0; s < kPBuf; ++s) mbar_init(&aux->p_full[s], 4), mbar_init(&aux->s_full[s], 1);
+    for (int s = 0; s < 3; ++s) mbar_init(&aux->x_full[s], 1);
+    for (int s = 0; s < kPBuf; ++s) mbar_init(&aux->p_full[s], 8), mbar_init(&aux->s_full[s], 1);
     for (int s = 0; s < 4; ++s) mbar_init(&aux->pv_done[s], 2);
-    mbar_init(&aux->s_empty[0], 4);
-    mbar_init(&aux->s_empty[1], 4);
+    mbar_init(&aux->s_empty[0], 8);
+    mbar_init(&aux->s_empty[1], 8);
     mbar_init(&aux->q_full, 128);
     mbar_init(&aux->q_empty, 1);
     mbar_init(&aux->o_full, 1);
     mbar_init(&aux->o_empty, 128);
     mbar_init(&aux->stat_full, 128);
-    mbar_init(&aux->l_full, 4);
     for (int s = 0; s < 3; ++s) mbar_init(&aux->qs_full[s], 1), mbar_init(&aux->qs_empty[s], 4);
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == 13) {
     tmem_alloc(&aux->tmem_base, 512);
     tmem_relinquish();
   }
@@ -320,11 +324,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   const uint32_t tbase = aux->tmem_base;
   Walk w(p, aux->sched);
 
-  if (warp == 8 || warp == 10) {
+  if (warp == 12 || warp == 14) {
     // ------------------------------------------------------------ producers
-    // 8: this CTA's 32 rows, first the groups outside its own columns, then
-    // its own; 10: the other CTA's 32 rows, own columns
-    const bool keys = warp == 8;
+    // 12: this CTA's 32 rows; 14: the other CTA's 32 rows, own columns
+    const bool keys = warp == 12;
     PageRows<kR> rows(p, keys ? c : 1 - c);
     int it = 0, issued = 0;
     bool live = true;
@@ -362,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       for (int j = max(0, issued - stages); j < issued; ++j)
         mbar_wait_drain(keys ? &aux->kv_full[j % stages] : &aux->c_full[j % stages], (j / stages) & 1);
     }
-  } else if (warp == 9) {
+  } else if (warp == 13) {
     // ----------------------------------------------------------- MMA issuer
     // the whole warp walks and waits; one elected lane issues. Scores run two
     // tiles ahead of P V, within a piece.
@@ -372,11 +375,25 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     const uint32_t tm = uniform(tbase), rank = uniform(static_cast<uint32_t>(c)), s0 = uniform(smem_u32(smem));
     const uint64_t dq = make_smem_desc(s0 + kOffQ, 16, 1024, 2);
     int pieces = 0;
-    auto scores = [&](int it, bool first, bool last) -> bool {
+    // What tile `it`'s scores (mask 3) and tile `iv`'s P V (mask 12) need, one barrier per lane: a wait
+    // that is over costs about 120 cycles, so all are looked at once, while the P V before still runs
+    auto ready = [&](int it, int iv) -> uint32_t {
+      bool ok = true;
+      if (lane < 4) {
+        uint64_t* bar = &aux->kv_full[it & 3];
+        uint32_t phase = (it >> 2) & 1;
+        if (lane == 1) bar = &aux->s_empty[it & 1], phase = ((it >> 1) - 1) & 1;
+        if (lane == 2) bar = &aux->p_full[iv & 1], phase = (iv >> 1) & 1;
+        if (lane == 3) bar = &aux->c_full[iv % kStagesC], phase = (iv / kStagesC) & 1;
+        ok = mbar_test_cluster(bar, phase);
+      }
+      return __ballot_sync(0xffffffffu, ok);
+    };
+    auto scores = [&](int it, bool first, bool last, uint32_t seen) -> bool {
       const uint32_t sa = uniform(it & 1), sb = uniform(it & 3);
       if ((first && !mbar_wait_warp(&aux->q_full, pieces & 1)) ||
-          (it >= 2 && !mbar_wait_warp(&aux->s_empty[sa], ((it >> 1) - 1) & 1)) ||
-          !mbar_wait_warp(&aux->kv_full[sb], (it >> 2) & 1))
+          ((seen & 3) != 3 && ((it >= 2 && !mbar_wait_warp(&aux->s_empty[sa], ((it >> 1) - 1) & 1)) ||
+                               !mbar_wait_warp(&aux->kv_full[sb], (it >> 2) & 1))))
         return false;
       tc_fence_after();
       const uint64_t da = make_smem_desc(s0 + kOffA + sa * kBytesA, 16, 1024, 2);
@@ -406,16 +423,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       __syncwarp();
       return true;
     };
-    auto values = [&](int it, bool first, bool last) -> bool {
+    auto values = [&](int it, bool first, bool last, uint32_t seen) -> bool {
       const uint32_t sb = uniform(it & 3), sc = uniform(it % kStagesC), pb = uniform(it & 1);
       if ((first && pieces > 0 && !mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1)) ||
-          !mbar_wait_warp(&aux->c_full[sc], (it / kStagesC) & 1) ||
-          !mbar_wait_cluster_warp(&aux->p_full[pb], (it >> 1) & 1))
+          ((seen & 12) != 12 && (!mbar_wait_warp(&aux->c_full[sc], (it / kStagesC) & 1) ||
+                                 !mbar_wait_cluster_warp(&aux->p_full[pb], (it >> 1) & 1))))
         return false;
       tc_fence_after();
       const uint32_t own = s0 + kOffB + sb * kBytesV, other = s0 + kOffC + sc * kBytesV;
-      // P: rows of 64 bytes, 64-byte swizzle; V: 64-column groups kR * 128 bytes apart
-      const uint64_t dp = make_smem_desc(s0 + kOffP + pb * 2 * kPHalf, 16, 512, 4);
+      // P: rows of 32 bytes, 32-byte swizzle; V: 64-column groups kR * 128 bytes apart
+      const uint64_t dp = make_smem_desc(s0 + kOffP + pb * 4 * kPPart, 16, 256, 6);
       const uint64_t dv0 = make_smem_desc(rank == 0 ? own : other, kR * 128, 1024, 2);
       const uint64_t dv1 = make_smem_desc(rank == 0 ? other : own, kR * 128, 1024, 2);
       __syncwarp();
@@ -424,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int k = 0; k < 2; ++k)  // the second 16 cache rows follow at once (32-row boxes) or as the next box
-            umma_f16_ss(tm + kColO, dp + (h * kPHalf + k * 32) / 16,
+            umma_f16_ss(tm + kColO, dp + (h * 2 + k) * kPPart / 16,
                         (h ? dv1 : dv0) + (kR == 32 ? k * 2048 : k * 4 * kR * 128) / 16, idesc_pv, !first || h + k > 0);
         }
         umma_commit_cluster(&aux->pv_done[sb], 3);
@@ -436,29 +453,49 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     int it = 0;
     bool live = true;
     while (live && w.next()) {
-      live = scores(it, true, w.n == 1) && (w.n == 1 || scores(it + 1, false, w.n == 2));
-      for (int j = 0; live && j < w.n; ++j, ++it)
-        live = (j + 2 >= w.n || scores(it + 2, false, j + 3 == w.n)) && values(it, j == 0, j + 1 == w.n);
+      live = scores(it, true, w.n == 1, 0) && (w.n == 1 || scores(it + 1, false, w.n == 2, 0));
+      for (int j = 0; live && j < w.n; ++j, ++it) {
+        const uint32_t seen = j + 2 < w.n ? ready(it + 2, it) : 0;
+        live = (j + 2 >= w.n || scores(it + 2, false, j + 3 == w.n, seen)) && values(it, j == 0, j + 1 == w.n, seen);
+      }
       ++pieces;
     }
     if (!live && lane == 0) {
       umma_commit(&aux->drain);
       mbar_wait_drain(&aux->drain, 0);
     }
-  } else if (warp < 4) {
+  } else if (warp < 8) {
     // -------------------------------------------------------------- softmax
-    const int r = tid;
-    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
+    const int r = tid & 127, hh = tid >> 7, part = 2 * c + hh;  // row, 16 of the CTA's 32 cache rows, of the tile's 64
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float sl2 = p.scale * 1.4426950408889634f;
     const uint32_t peer = static_cast<uint32_t>(1 - c);
-    // this CTA's half of P, this row: 64 bytes, 16-byte chunk q at q ^ (row / 2 % 4); the warp's rows are 2 KB in one piece
-    uint8_t* half = smem + kOffP + c * kPHalf;
-    const uint32_t peer_half = mapa_shared(smem_u32(half + warp * 2048), peer);
-    const uint32_t peer_bar_x = mapa_shared(smem_u32(&aux->x_full[0]), peer);
+    // P of this warp's 32 rows and 16 cache rows: 1 KB, 16-byte half h of row r at h ^ (r / 4 % 2)
+    uint8_t* mine = smem + kOffP + part * kPPart + (warp & 3) * 1024;
+    const uint32_t peer_mine = mapa_shared(smem_u32(mine), peer);
     const uint32_t peer_bar_p = mapa_shared(smem_u32(&aux->p_full[0]), peer);
-    const uint32_t peer_bar_l = mapa_shared(smem_u32(&aux->l_full), peer);
-    const uint32_t peer_max = mapa_shared(smem_u32(&aux->peer_max[0][r]), peer);
-    const uint32_t peer_sum = mapa_shared(smem_u32(&aux->peer_sum[0][r]), peer);
+    uint32_t to[2], to_bar[2];  // this CTA's and the other's
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      to[k] = mapa_shared(smem_u32(&aux->shared[0][part][r]), k);
+      to_bar[k] = mapa_shared(smem_u32(&aux->x_full[0]), k);
+    }
+    int told = 0, heard = 0;
+    auto tell = [&](float v) {
+      const int slot = told % 3;
+      if (tid == 0) mbar_arrive_expect_tx(&aux->x_full[slot], 4 * kRows * 4);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) st_async_f32(to[k] + slot * 4 * kRows * 4, v, to_bar[k] + slot * 8);
+      ++told;
+    };
+    auto hear = [&](float (&v)[4]) -> bool {
+      const int slot = heard % 3;
+      if (!mbar_wait_cluster_warp(&aux->x_full[slot], (heard / 3) & 1)) return false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = aux->shared[slot][k][r];
+      ++heard;
+      return true;
+    };
     if (p.debug_stall) mbar_wait(&aux->stall, 0);  // test hook: runs into the wait limit
     int it = 0, pieces = 0;
     bool live = true;
@@ -469,54 +506,52 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       // tiles below this one are seen in full by every row (the first row sees the least)
       const int clean = w.u.limit(w.q, w.kv, w.mt * kRows / p.num_heads) / kTok;
       float m = -INFINITY, l = 0.f, lp = 0.f;
-      float s[32];
-      // scores of a tile from TMEM, masked, and their maximum on its way to the other CTA. The
-      // receiving slot is free: the other CTA's scores of tile i + 4 come after its P V of tile
-      // i + 1, which needs this CTA's P, written after slot i was read.
-      auto fetch = [&](int i, int t) -> float {
+      float s[16], s_next[16];
+      // scores of a tile from TMEM, masked, and their maximum on its way
+      auto fetch = [&](int i, int t, float (&x)[16]) {
         tc_fence_after();
-        uint32_t sv[32];
-        tmem_ld_32x32b_x32(tbase + lane_off + kColS + (i & 1) * 32, sv);
+        uint32_t sv[16];
+        tmem_ld_32x32b_x16(tbase + lane_off + kColS + (i & 1) * 32 + hh * 16, sv);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&aux->s_empty[i & 1]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) s[e] = __uint_as_float(sv[e]);
+        for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(sv[e]);
         if (t >= clean) {
-          const int seen = lim - t * kTok - c * kHalfTok;
+          const int seen = lim - t * kTok - part * 16;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = e < seen ? s[e] : -INFINITY;
+          for (int e = 0; e < 16; ++e) x[e] = e < seen ? x[e] : -INFINITY;
         }
-        float a = fmax3f(s[0], s[1], s[2]), b = fmax3f(s[3], s[4], s[5]);
-#pragma unroll
-        for (int e = 6; e < 30; e += 4) {
-          a = fmax3f(a, s[e], s[e + 1]);
-          b = fmax3f(b, s[e + 2], s[e + 3]);
-        }
-        a = fmax3f(a, b, fmaxf(s[30], s[31]));
-        const int slot = i % kXBuf;
-        if (tid == 0) mbar_arrive_expect_tx(&aux->x_full[slot], kRows * 4);
-        st_async_f32(peer_max + slot * kRows * 4, a, peer_bar_x + slot * 8);
-        return a;
+        float a = fmax3f(x[0], x[1], x[2]), b = fmax3f(x[3], x[4], x[5]);
+        a = fmax3f(a, x[6], x[7]), b = fmax3f(b, x[8], x[9]);
+        a = fmax3f(a, x[10], x[11]), b = fmax3f(b, x[12], x[13]);
+        a = fmax3f(a, b, fmaxf(x[14], x[15]));
+        tell(a);
       };
       live = mbar_wait_warp(&aux->s_full[it & 1], (it >> 1) & 1);
       if (!live) break;
-      float mx = fetch(it, w.t0);
+      fetch(it, w.t0, s);
       for (int j = 0; live && j < w.n; ++j, ++it) {
         const int t = w.t0 + j, pb = it & 1;
-        live = mbar_wait_cluster_warp(&aux->x_full[it % kXBuf], (it / kXBuf) & 1);
+        // the next tile's scores, and its maximum on its way: now if they are there, which hides the
+        // exchange behind this tile's exponentials, else after this tile's P, which may be what they wait for
+        const bool early =
+            j + 1 < w.n && __all_sync(0xffffffffu, mbar_test_cluster(&aux->s_full[(it + 1) & 1], ((it + 1) >> 1) & 1));
+        if (early) fetch(it + 1, t + 1, s_next);
+        float of[4];
+        live = hear(of);
         if (!live) break;
-        mx = fmaxf(mx, aux->peer_max[it % kXBuf][r]) * sl2;
-        // both CTAs take the same decision from the same two maxima
+        const float mx = fmax3f(of[0], of[1], fmaxf(of[2], of[3])) * sl2;
+        // all four threads of the row take the same decision from the same maxima
         const bool move = mx > m + 8.f;
         const float dm = move ? ex2(m - mx) : 1.f;  // 0 while nothing has been seen
         if (move) m = mx;
         const float neg = m == -INFINITY ? 0.f : -m;
         float r0 = 0.f, r1 = 0.f, p0 = 0.f, p1 = 0.f;
-        uint32_t pk[16];
+        uint32_t pk[8];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
+        for (int e = 0; e < 16; e += 2) {
           float y0, y1;
           ffma2_bcast(y0, y1, s[e], s[e + 1], sl2, neg);
           y0 = ex2(y0), y1 = ex2(y1);
@@ -532,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           if (!live) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int g = 0; g < 8; ++g) {
+          for (int g = 4 * hh; g < 4 * hh + 4; ++g) {
             uint32_t o[32];
             tmem_ld_32x32b_x32(tbase + lane_off + kColO + g * 32, o);
             tmem_wait_ld();
@@ -546,21 +581,19 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         // this buffer's last P has been read by both CTAs (and copied)
         live = it < kPBuf || mbar_wait_cluster_warp(&aux->pv_done[(it - kPBuf) & 3], ((it - kPBuf) >> 2) & 1);
         if (!live) break;
-        uint8_t* dst = half + pb * 2 * kPHalf;
+        uint8_t* dst = mine + pb * 4 * kPPart;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *reinterpret_cast<uint4*>(dst + r * 64 + ((q ^ ((r >> 1) & 3)) << 4)) =
+        for (int q = 0; q < 2; ++q)
+          *reinterpret_cast<uint4*>(dst + lane * 32 + ((q ^ ((lane >> 2) & 1)) << 4)) =
               make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
         if ((t + 1) * kTok > valid) {
           // rows past the request's length may hold NaN: weight 0 does not hide
           // them from the product, so they are cleared
           live = mbar_wait_warp(&aux->c_full[it % kStagesC], (it / kStagesC) & 1);
           if (!live) break;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (t * kTok + h * kHalfTok + lane < valid) continue;
-            uint8_t* stage = smem + (h == c ? kOffB + it % kStagesB * kBytesV : kOffC + it % kStagesC * kBytesV);
-            uint4* v = reinterpret_cast<uint4*>(stage + ((lane / kR) * 4 + warp) * kR * 128 + (lane % kR) * 128);
+          if (t * kTok + hh * kHalfTok + lane >= valid) {
+            uint8_t* stage = smem + (hh == c ? kOffB + it % kStagesB * kBytesV : kOffC + it % kStagesC * kBytesV);
+            uint4* v = reinterpret_cast<uint4*>(stage + ((lane / kR) * 4 + (warp & 3)) * kR * 128 + (lane % kR) * 128);
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = make_uint4(0u, 0u, 0u, 0u);
           }
@@ -568,28 +601,54 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          bulk_copy_cluster(peer_half + pb * 2 * kPHalf, dst + warp * 2048, 2048, peer_bar_p + pb * 8);
-          mbar_arrive_expect_tx(&aux->p_full[pb], 2048);
+          bulk_copy_cluster(peer_mine + pb * 4 * kPPart, dst, 1024, peer_bar_p + pb * 8);
+          mbar_arrive_expect_tx(&aux->p_full[pb], 1024);
         }
-        // the next tile's scores, and its maximum on its way
-        if (j + 1 < w.n) {
+        if (j + 1 < w.n && !early) {
           live = mbar_wait_warp(&aux->s_full[(it + 1) & 1], ((it + 1) >> 1) & 1);
           if (!live) break;
-          mx = fetch(it + 1, t + 1);
+          fetch(it + 1, t + 1, s_next);
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = s_next[e];
       }
       if (!live) break;
-      // the row's sums over both CTAs' cache rows (a sum of two: the same in both CTAs)
-      st_cluster_f32(peer_sum, l);
-      st_cluster_f32(peer_sum + kRows * 4, lp);
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote(peer_bar_l);
-      live = mbar_wait_cluster_warp(&aux->l_full, pieces & 1);
-      l += aux->peer_sum[0][r];
-      lp += aux->peer_sum[1][r];
-      aux->inv[pieces & 1][r] = lp > 0.f ? 1.f / lp : 0.f;
-      aux->lse[pieces & 1][r] = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
-      mbar_arrive(&aux->stat_full);
+      // the row's sums over the four threads, added in one order by all
+      float of[4];
+      tell(l);
+      live = hear(of);
+      if (!live) break;
+      l = (of[0] + of[1]) + (of[2] + of[3]);
+      tell(lp);
+      live = hear(of);
+      if (!live) break;
+      lp = (of[0] + of[1]) + (of[2] + of[3]);
+      if (hh == 0) {
+        live = pieces == 0 || mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1);  // the last one has been read
+        if (!live) break;
+        aux->inv[r] = lp > 0.f ? 1.f / lp : 0.f;
+        mbar_arrive(&aux->stat_full);
+      }
+      const int64_t grow = w.tok * p.num_heads + row;
+      if (c == 0 && hh == 0 && row < w.q * p.num_heads && grow < p.num_tokens * p.num_heads) {
+        const float lse = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+        if (w.starts && w.ends)
+          p.lse[grow] = lse;
+        else
+          P.part_lse[(2 * cluster + (w.starts ? 1 : 0)) * kRows + r] = lse;
+        if (w.starts) {
+          int32_t info = 0;
+          if (!w.ends) {
+            // the run that holds the unit's last tile
+            const Sched& sc = aux->sched;
+            const int64_t runs = min(static_cast<int64_t>(clusters), sc.tiles);
+            const int64_t last = sc.begin + (it - w.n) + w.unit_tiles - 1;
+            const int64_t hi = ((last + 1) * runs + sc.tiles - 1) / sc.tiles - 1;
+            info = pack_info(cluster, static_cast<int>(hi) - cluster + 1, r);
+          }
+          P.row_info[grow] = info;
+        }
+      }
       ++pieces;
     }
     // the other CTA's last commits (and with them its copies of this CTA's P) have arrived
@@ -604,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     }
   } else {
     // ------------------------------------------------ query loads, epilogue
-    const int r = tid - 128;
+    const int r = tid - 256;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int64_t all_rows = p.num_tokens * p.num_heads;
     // Query tile: the nine groups of 64 dims come by TMA, group g into slot g % 3 of 16 KB; six
@@ -620,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       ++loads;
     };
     auto place_q = [&](const Walk& x, int piece) -> bool {
-      if (tid == 128)
+      if (tid == 256)
         for (int g = 0; g < 3; ++g) load_group(x, g);
       for (int g = 0; g < 9; ++g) {
         bool ok = mbar_wait_warp(&aux->qs_full[g % 3], (piece * 3 + g / 3) & 1);
@@ -637,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           tmem_st_32x32b_x32(tbase + lane_off + kColQ + g * 32, x32);
           __syncwarp();
           if (lane == 0) mbar_arrive(&aux->qs_empty[g % 3]);
-          if (warp == 4) {
+          if (warp == 8) {
             ok = mbar_wait_warp(&aux->qs_empty[g % 3], (piece * 2 + g / 3) & 1);
             if (ok && lane == 0) load_group(x, g + 3);
             __syncwarp();
@@ -654,13 +713,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       mbar_arrive(&aux->q_full);
       return true;
     };
-    auto store_o = [&](const Walk& x, int piece, int first_tile) -> bool {
+    auto store_o = [&](const Walk& x, int piece) -> bool {
       if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
       tc_fence_after();
-      const float inv = aux->inv[piece & 1][r], lse = aux->lse[piece & 1][r];
-      const int row = x.mt * kRows + r;
-      const int64_t grow = x.tok * p.num_heads + row;
-      const bool ok = row < x.q * p.num_heads && grow < all_rows;
+      const float inv = aux->inv[r];
       const bool whole = x.starts && x.ends;
       const int64_t slot = 2 * cluster + (x.starts ? 1 : 0);
       // 32 bytes per row at a time through shared memory, so that a store instruction writes whole
@@ -714,31 +770,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           for (int q = 0; q < 4; ++q) put(g * 4 + q, four(8 * q), four(8 * q + 4));
         }
       }
-      if (ok && c == 0) {
-        if (whole)
-          p.lse[grow] = lse;
-        else
-          P.part_lse[slot * kRows + r] = lse;
-        if (x.starts) {
-          int32_t info = 0;
-          if (!x.ends) {
-            // the run that holds the unit's last tile
-            const Sched& s = aux->sched;
-            const int64_t runs = min(static_cast<int64_t>(clusters), s.tiles);
-            const int64_t last = s.begin + first_tile + x.unit_tiles - 1;
-            const int64_t hi = ((last + 1) * runs + s.tiles - 1) / s.tiles - 1;
-            info = pack_info(cluster, static_cast<int>(hi) - cluster + 1, r);
-          }
-          P.row_info[grow] = info;
-        }
-      }
       return true;
     };
     // the next piece's query goes in as soon as the last scores of this one are
     // computed, before this one's epilogue
     bool more = w.next();
     bool live = !more || place_q(w, 0);
-    int piece = 0, tiles_before = 0;
+    int piece = 0;
     while (live && more) {
       const Walk now = w;
       more = w.next();
@@ -749,15 +787,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         live = place_q(w, piece + 1);
         if (!live) break;
       }
-      live = store_o(now, piece, tiles_before);
-      tiles_before += now.n;
+      live = store_o(now, piece);
       ++piece;
     }
   }
   tc_fence_before();
   __syncwarp();
   cluster_sync_all();  // no more stores or arrivals to the other CTA
-  if (warp == 9) {
+  if (warp == 13) {
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
