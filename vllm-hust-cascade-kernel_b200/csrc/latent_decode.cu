@@ -95,8 +95,13 @@ struct __align__(16) Aux {
   // softmax, and the keys' next load), pv_done[it % 4] = P V of tile it done in
   // both CTAs (P, own columns, other rows). A waiter is never two phases behind:
   // the next phase needs what it is about to do.
-  uint64_t kv_full[kStagesB], c_full[kStagesC];
-  uint64_t q_full, q_empty, s_full[2], s_empty[2], x_full[3], p_full[kPBuf], pv_done[4], o_full, o_empty, stat_full;
+  // What an MMA batch needs meets on one barrier too (a wait that is over costs
+  // 120 cycles): kv_full[it % 4] = tile it's keys loaded, and its score buffer
+  // read by the eight softmax warps; p_full[it % 2] = P of both CTAs, and the
+  // other CTA's rows loaded. The rows of a tile that ends in unused cache rows
+  // come over tail_full[it % 2] instead: the softmax clears those rows first.
+  uint64_t kv_full[kStagesB], p_full[kPBuf], tail_full[kPBuf], s_full[2], pv_done[4], x_full[3];
+  uint64_t q_full, q_empty, o_full, o_empty, stat_full;
   uint64_t qs_full[3], qs_empty[3];
   uint64_t stall, drain;
   uint32_t tmem_base;
@@ -296,13 +301,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 
   if (tid == 0) {
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
-    for (int s = 0; s < kStagesB; ++s) mbar_init(&aux->kv_full[s], 1);
-    for (int s = 0; s < kStagesC; ++s) mbar_init(&aux->c_full[s], 1);
+    for (int s = 0; s < kStagesB; ++s) mbar_init(&aux->kv_full[s], 9);
     for (int s = 0; s < 3; ++s) mbar_init(&aux->x_full[s], 1);
-    for (int s = 0; s < kPBuf; ++s) mbar_init(&aux->p_full[s], 8), mbar_init(&aux->s_full[s], 1);
+    for (int s = 0; s < kPBuf; ++s) mbar_init(&aux->p_full[s], 9), mbar_init(&aux->tail_full[s], 1), mbar_init(&aux->s_full[s], 1);
     for (int s = 0; s < 4; ++s) mbar_init(&aux->pv_done[s], 2);
-    mbar_init(&aux->s_empty[0], 8);
-    mbar_init(&aux->s_empty[1], 8);
     mbar_init(&aux->q_full, 128);
     mbar_init(&aux->q_empty, 1);
     mbar_init(&aux->o_full, 1);
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // 12: this CTA's 32 rows; 14: the other CTA's 32 rows, own columns
     const bool keys = warp == 12;
     PageRows<kR> rows(p, keys ? c : 1 - c);
-    int it = 0, issued = 0;
+    int it = 0;
     bool live = true;
     while (live && w.next()) {
       rows.start(w.b, w.kv);
@@ -338,14 +340,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < PageRows<kR>::kPer; ++i) y[i] = rows.get(t, i, lane);
         const int stages = keys ? kStagesB : kStagesC, st = it % stages;
-        live = it < stages || mbar_wait_cluster_warp(&aux->pv_done[(it - stages) & 3], ((it - stages) >> 2) & 1);
+        live = it < stages || mbar_wait_warp(&aux->pv_done[(it - stages) & 3], ((it - stages) >> 2) & 1);
         if (keys) live = live && (it < 2 || mbar_wait_warp(&aux->s_full[it & 1], ((it >> 1) - 1) & 1));
         if (!live) break;
+        const bool tail = !keys && (t + 1) * kTok > min(w.kv, w.u.cap);
         if (lane == 0) {
-          uint64_t* full = keys ? &aux->kv_full[st] : &aux->c_full[st];
+          uint64_t* full = keys ? &aux->kv_full[st] : tail ? &aux->tail_full[it & 1] : &aux->p_full[it & 1];
           uint8_t* dst = smem + (keys ? kOffB : kOffC) + st * kBytesV;
           uint8_t* dsta = smem + kOffA + (it & 1) * kBytesA;
           mbar_arrive_expect_tx(full, keys ? kBytesA + kBytesV : kBytesV);
+          if (tail) mbar_arrive(&aux->p_full[it & 1]);
 #pragma unroll
           for (int i = 0; i < PageRows<kR>::kPer; ++i) {
             if (keys) {
@@ -355,15 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             tma_load_3d(dst + i * kR * 512, &P.map4, full, 0, y[i], 4 * c);
           }
         }
-        ++issued;
         __syncwarp();
       }
-    }
-    // aborting: every load issued has landed before the CTA leaves
-    if (!live && lane == 0) {
-      const int stages = keys ? kStagesB : kStagesC;
-      for (int j = max(0, issued - stages); j < issued; ++j)
-        mbar_wait_drain(keys ? &aux->kv_full[j % stages] : &aux->c_full[j % stages], (j / stages) & 1);
     }
   } else if (warp == 13) {
     // ----------------------------------------------------------- MMA issuer
@@ -375,25 +372,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     const uint32_t tm = uniform(tbase), rank = uniform(static_cast<uint32_t>(c)), s0 = uniform(smem_u32(smem));
     const uint64_t dq = make_smem_desc(s0 + kOffQ, 16, 1024, 2);
     int pieces = 0;
-    // What tile `it`'s scores (mask 3) and tile `iv`'s P V (mask 12) need, one barrier per lane: a wait
-    // that is over costs about 120 cycles, so all are looked at once, while the P V before still runs
-    auto ready = [&](int it, int iv) -> uint32_t {
-      bool ok = true;
-      if (lane < 4) {
-        uint64_t* bar = &aux->kv_full[it & 3];
-        uint32_t phase = (it >> 2) & 1;
-        if (lane == 1) bar = &aux->s_empty[it & 1], phase = ((it >> 1) - 1) & 1;
-        if (lane == 2) bar = &aux->p_full[iv & 1], phase = (iv >> 1) & 1;
-        if (lane == 3) bar = &aux->c_full[iv % kStagesC], phase = (iv / kStagesC) & 1;
-        ok = mbar_test_cluster(bar, phase);
-      }
-      return __ballot_sync(0xffffffffu, ok);
-    };
-    auto scores = [&](int it, bool first, bool last, uint32_t seen) -> bool {
-      const uint32_t sa = uniform(it & 1), sb = uniform(it & 3);
-      if ((first && !mbar_wait_warp(&aux->q_full, pieces & 1)) ||
-          ((seen & 3) != 3 && ((it >= 2 && !mbar_wait_warp(&aux->s_empty[sa], ((it >> 1) - 1) & 1)) ||
-                               !mbar_wait_warp(&aux->kv_full[sb], (it >> 2) & 1))))
+    auto scores = [&](int it, bool first, bool last) -> bool {
+      const uint32_t u = uniform(it), sa = u & 1, sb = u & 3;
+      if ((first && !mbar_wait_warp(&aux->q_full, pieces & 1)) || !mbar_wait_warp(&aux->kv_full[sb], (u >> 2) & 1))
         return false;
       tc_fence_after();
       const uint64_t da = make_smem_desc(s0 + kOffA + sa * kBytesA, 16, 1024, 2);
@@ -423,11 +404,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       __syncwarp();
       return true;
     };
-    auto values = [&](int it, bool first, bool last, uint32_t seen) -> bool {
-      const uint32_t sb = uniform(it & 3), sc = uniform(it % kStagesC), pb = uniform(it & 1);
+    auto values = [&](int it, bool first, bool last) -> bool {
+      const uint32_t u = uniform(it), sb = u & 3, sc = u % kStagesC, pb = u & 1;
       if ((first && pieces > 0 && !mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1)) ||
-          ((seen & 12) != 12 && (!mbar_wait_warp(&aux->c_full[sc], (it / kStagesC) & 1) ||
-                                 !mbar_wait_cluster_warp(&aux->p_full[pb], (it >> 1) & 1))))
+          !mbar_wait_warp(&aux->p_full[pb], (u >> 1) & 1))
         return false;
       tc_fence_after();
       const uint32_t own = s0 + kOffB + sb * kBytesV, other = s0 + kOffC + sc * kBytesV;
@@ -453,11 +433,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     int it = 0;
     bool live = true;
     while (live && w.next()) {
-      live = scores(it, true, w.n == 1, 0) && (w.n == 1 || scores(it + 1, false, w.n == 2, 0));
-      for (int j = 0; live && j < w.n; ++j, ++it) {
-        const uint32_t seen = j + 2 < w.n ? ready(it + 2, it) : 0;
-        live = (j + 2 >= w.n || scores(it + 2, false, j + 3 == w.n, seen)) && values(it, j == 0, j + 1 == w.n, seen);
-      }
+      live = scores(it, true, w.n == 1) && (w.n == 1 || scores(it + 1, false, w.n == 2));
+      for (int j = 0; live && j < w.n; ++j, ++it)
+        live = (j + 2 >= w.n || scores(it + 2, false, j + 3 == w.n)) && values(it, j == 0, j + 1 == w.n);
       ++pieces;
     }
     if (!live && lane == 0) {
@@ -480,6 +458,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       to[k] = mapa_shared(smem_u32(&aux->shared[0][part][r]), k);
       to_bar[k] = mapa_shared(smem_u32(&aux->x_full[0]), k);
     }
+    // both score buffers are free
+    if (lane == 0) mbar_arrive(&aux->kv_full[0]), mbar_arrive(&aux->kv_full[1]);
     int told = 0, heard = 0;
     auto tell = [&](float v) {
       const int slot = told % 3;
@@ -490,14 +470,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     };
     auto hear = [&](float (&v)[4]) -> bool {
       const int slot = heard % 3;
-      if (!mbar_wait_cluster_warp(&aux->x_full[slot], (heard / 3) & 1)) return false;
+      if (!mbar_wait_warp(&aux->x_full[slot], (heard / 3) & 1)) return false;
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = aux->shared[slot][k][r];
       ++heard;
       return true;
     };
     if (p.debug_stall) mbar_wait(&aux->stall, 0);  // test hook: runs into the wait limit
-    int it = 0, pieces = 0;
+    int it = 0, pieces = 0, tails = 0;  // tails: phase bit per buffer
     bool live = true;
     while (live && w.next()) {
       const int row = w.mt * kRows + r;
@@ -515,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->s_empty[i & 1]);
+        if (lane == 0) mbar_arrive(&aux->kv_full[(i + 2) & 3]);
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(sv[e]);
         if (t >= clean) {
@@ -537,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         // the next tile's scores, and its maximum on its way: now if they are there, which hides the
         // exchange behind this tile's exponentials, else after this tile's P, which may be what they wait for
         const bool early =
-            j + 1 < w.n && __all_sync(0xffffffffu, mbar_test_cluster(&aux->s_full[(it + 1) & 1], ((it + 1) >> 1) & 1));
+            j + 1 < w.n && __all_sync(0xffffffffu, mbar_test(&aux->s_full[(it + 1) & 1], ((it + 1) >> 1) & 1));
         if (early) fetch(it + 1, t + 1, s_next);
         float of[4];
         live = hear(of);
@@ -563,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         l = l * dm + (r0 + r1);
         lp = lp * dm + (p0 + p1);
         if (j > 0 && __any_sync(0xffffffffu, move)) {
-          live = mbar_wait_cluster_warp(&aux->pv_done[(it - 1) & 3], ((it - 1) >> 2) & 1);  // O holds every tile before this one
+          live = mbar_wait_warp(&aux->pv_done[(it - 1) & 3], ((it - 1) >> 2) & 1);  // O holds every tile before this one
           if (!live) break;
           tc_fence_after();
 #pragma unroll 1
@@ -579,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           tc_fence_before();
         }
         // this buffer's last P has been read by both CTAs (and copied)
-        live = it < kPBuf || mbar_wait_cluster_warp(&aux->pv_done[(it - kPBuf) & 3], ((it - kPBuf) >> 2) & 1);
+        live = it < kPBuf || mbar_wait_warp(&aux->pv_done[(it - kPBuf) & 3], ((it - kPBuf) >> 2) & 1);
         if (!live) break;
         uint8_t* dst = mine + pb * 4 * kPPart;
 #pragma unroll
@@ -589,7 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         if ((t + 1) * kTok > valid) {
           // rows past the request's length may hold NaN: weight 0 does not hide
           // them from the product, so they are cleared
-          live = mbar_wait_warp(&aux->c_full[it % kStagesC], (it / kStagesC) & 1);
+          live = mbar_wait_warp(&aux->tail_full[pb], (tails >> pb) & 1);
+          tails ^= 1 << pb;
           if (!live) break;
           if (t * kTok + hh * kHalfTok + lane >= valid) {
             uint8_t* stage = smem + (hh == c ? kOffB + it % kStagesB * kBytesV : kOffC + it % kStagesC * kBytesV);
@@ -654,13 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // the other CTA's last commits (and with them its copies of this CTA's P) have arrived
     // before this CTA may leave
     for (int i = max(0, it - kPBuf); live && i < it; ++i)
-      live = mbar_wait_cluster_warp(&aux->pv_done[i & 3], (i >> 2) & 1);
-    if (!live) {
-      // aborting: what is on its way to the other CTA (a few KB) gets a
-      // millisecond, hundreds of times what it takes, before either CTA leaves
-      for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000 * 1000;) {
-      }
-    }
+      live = mbar_wait_warp(&aux->pv_done[i & 3], (i >> 2) & 1);
   } else {
     // ------------------------------------------------ query loads, epilogue
     const int r = tid - 256;
@@ -669,14 +644,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // Query tile: the nine groups of 64 dims come by TMA, group g into slot g % 3 of 16 KB; six
     // move on to TMEM, the last three stay. (Loads of a row per thread touch 32 lines per
     // instruction: 14,000 cycles in which the softmax stood still too.)
-    int loads = 0;  // issued, by one lane
     auto load_group = [&](const Walk& x, int g) {
       // group order: the CTA's own columns, the other latent ones, the rotary part
       const int col = g < 4 ? 4 * c + g : g < 8 ? 4 * (1 - c) + g - 4 : 8;
       mbar_arrive_expect_tx(&aux->qs_full[g % 3], kQGroup);
       tma_load_3d(smem + kOffQ + g % 3 * kQGroup, &P.map_q, &aux->qs_full[g % 3], 0,
                   static_cast<int>(x.tok * p.num_heads + x.mt * kRows), col);
-      ++loads;
     };
     auto place_q = [&](const Walk& x, int piece) -> bool {
       if (tid == 256)
@@ -702,11 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             __syncwarp();
           }
         }
-        if (!ok) {
-          // aborting: the loads in flight land before the CTA leaves
-          for (int i = max(0, loads - 3); i < loads; ++i) mbar_wait_drain(&aux->qs_full[i % 3], (i / 3) & 1);
-          return false;
-        }
+        if (!ok) return false;
       }
       tmem_wait_st();
       tc_fence_before();
@@ -789,6 +758,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       }
       live = store_o(now, piece);
       ++piece;
+    }
+  }
+  if (cta_aborted()) {
+    // loads into this CTA and copies into the other one may be in flight (a few hundred KB): they get a millisecond,
+    // hundreds of times what they take, before either CTA leaves
+    for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000 * 1000;) {
     }
   }
   tc_fence_before();

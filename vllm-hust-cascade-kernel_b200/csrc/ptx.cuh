@@ -127,13 +127,12 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Whether the phase with the given parity has completed (acquire at cluster
-// scope); never suspends.
-__device__ __forceinline__ bool mbar_test_cluster(uint64_t* bar, uint32_t parity) {
+// Whether the phase with the given parity has completed; never suspends.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
@@ -146,13 +145,14 @@ __device__ __forceinline__ bool mbar_test_cluster(uint64_t* bar, uint32_t parity
 // raises the abort flag and the device error bit) or another thread of the
 // CTA already gave up.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = 0;  // read at the first check: reading the timer takes longer than most waits
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 15) == 0) {
       if (cta_aborted()) return false;
-      if (globaltimer_ns() - t0 >= cta_wait_state()->limit_ns) {
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 >= cta_wait_state()->limit_ns) {
         cta_abort(kErrMbarTimeout);
         return false;
       }
@@ -518,10 +518,6 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       }
     }
   }
-}
-
-__device__ __forceinline__ bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity));
 }
 
 __device__ __forceinline__ bool mbar_wait_cluster_drain(uint64_t* bar, uint32_t parity) {
