@@ -449,17 +449,21 @@ bool encode_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t
   return r == CUDA_SUCCESS;
 }
 
-bool encode_tmap_3d(CUtensorMap* map, const void* base, const uint64_t (&extent)[3], const uint64_t (&stride_bytes)[2],
-                    const uint32_t (&box)[3]) {
+bool encode_tmap_nd(CUtensorMap* map, const void* base, int rank, const uint64_t* extent, const uint64_t* stride_bytes,
+                    const uint32_t* box) {
   auto fn = get_encode_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[3] = {extent[0], extent[1], extent[2]};
-  const cuuint64_t strides[2] = {stride_bytes[0], stride_bytes[1]};
-  const cuuint32_t boxes[3] = {box[0], box[1], box[2]};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, boxes, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  if (!fn || rank < 2 || rank > 5) return false;
+  cuuint64_t dims[5], strides[4];
+  cuuint32_t boxes[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    dims[i] = extent[i];
+    boxes[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) strides[i] = stride_bytes[i];
+  }
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims,
+            strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 cudaError_t ensure_smem_limit(const void* kernel, int bytes) {

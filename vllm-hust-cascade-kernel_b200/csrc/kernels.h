@@ -292,9 +292,10 @@ int set_error(int code, const char* msg);
 bool encode_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t row_stride_bytes,
                     uint32_t box_inner, uint32_t box_rows, bool swizzle128, CUtensorMapL2promotion promo);
 
-// Host: encode a 3-D tiled tensor map of 16-bit elements, 128-byte swizzle
-// (box[0] = 64 elements), innermost extent first; strides of the outer two.
-bool encode_tmap_3d(CUtensorMap* map, const void* base, const uint64_t (&extent)[3], const uint64_t (&stride_bytes)[2],
-                    const uint32_t (&box)[3]);
+// Host: encode a tiled tensor map of 16-bit elements, 128-byte swizzle (box[0]
+// = 64 elements), rank 2 to 5, innermost extent first; strides of the outer
+// rank - 1 dimensions.
+bool encode_tmap_nd(CUtensorMap* map, const void* base, int rank, const uint64_t* extent, const uint64_t* stride_bytes,
+                    const uint32_t* box);
 
 }  // namespace cascade

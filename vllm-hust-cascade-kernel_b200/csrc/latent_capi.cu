@@ -153,11 +153,16 @@ int cascade_latent_prefill(const cascade_latent_prefill_t* p, void* out, float* 
     return fail(CASCADE_ERR_INVALID, "%s: null device pointer", op);
   if (misaligned(p->query) || misaligned(p->key) || misaligned(p->key_rope) || misaligned(p->value) || misaligned(out))
     return fail(CASCADE_ERR_INVALID, "%s: tensors must be 16-byte aligned", op);
-  const int64_t strides[] = {p->key_token_stride, p->key_head_stride, p->rope_token_stride, p->value_token_stride,
-                             p->value_head_stride};
-  for (int64_t s : strides)
+  // the stride of a dimension of one is never used, whatever it is
+  const bool head = p->num_heads > 1, token = p->num_kv > 1;
+  const int64_t key_ts = token ? p->key_token_stride : kPrefillDv, value_ts = token ? p->value_token_stride : kPrefillDv;
+  const int64_t rope_ts = token ? p->rope_token_stride : kPrefillDv;
+  const int64_t key_hs = head ? p->key_head_stride : 0, value_hs = head ? p->value_head_stride : 0;
+  for (int64_t s : {key_ts, value_ts, rope_ts, key_hs, value_hs})
     if (s < 0 || s % 8 || s >= (int64_t(1) << 38))
       return fail(CASCADE_ERR_INVALID, "%s: strides must be non-negative multiples of 8 elements", op);
+  if (!key_ts || !value_ts || !rope_ts)
+    return fail(CASCADE_ERR_INVALID, "%s: token strides must be positive", op);
   LatentPrefillLaunch L = {};
   L.query = p->query;
   L.key = p->key;
@@ -169,11 +174,11 @@ int cascade_latent_prefill(const cascade_latent_prefill_t* p, void* out, float* 
   L.lse = lse;
   L.num_tokens = p->num_tokens;
   L.num_kv = p->num_kv;
-  L.key_ts = p->key_token_stride;
-  L.key_hs = p->key_head_stride;
-  L.rope_ts = p->rope_token_stride;
-  L.value_ts = p->value_token_stride;
-  L.value_hs = p->value_head_stride;
+  L.key_ts = key_ts;
+  L.key_hs = key_hs;
+  L.rope_ts = rope_ts;
+  L.value_ts = value_ts;
+  L.value_hs = value_hs;
   L.num_heads = static_cast<int32_t>(p->num_heads);
   L.batch = static_cast<int32_t>(p->batch);
   L.max_q = static_cast<int32_t>(std::min(p->max_q_seqlen, p->num_tokens));

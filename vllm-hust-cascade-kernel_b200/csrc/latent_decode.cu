@@ -894,10 +894,11 @@ cudaError_t launch_latent_decode(const LatentDecodeLaunch& p, bool fp16, void* w
   const uint64_t pool_rows = std::max<uint64_t>(1, static_cast<uint64_t>(p.num_blocks) * p.block_size);
   const void* base = p.num_blocks > 0 ? p.cache : p.query;
   const uint64_t extent[3] = {64, pool_rows, 9}, stride[2] = {kLatentRow * 2, 128};
-  if (!encode_tmap_3d(&P.map4, base, extent, stride, {64, rows, 4}) ||
-      !encode_tmap_3d(&P.map1, base, extent, stride, {64, rows, 1}) ||
-      !encode_tmap_3d(&P.map_q, p.query, {64, static_cast<uint64_t>(p.num_tokens) * p.num_heads, 9}, stride,
-                      {64, kRows, 1}))
+  const uint64_t extent_q[3] = {64, static_cast<uint64_t>(p.num_tokens) * p.num_heads, 9};
+  const uint32_t box4[3] = {64, rows, 4}, box1[3] = {64, rows, 1}, box_q[3] = {64, kRows, 1};
+  if (!encode_tmap_nd(&P.map4, base, 3, extent, stride, box4) ||
+      !encode_tmap_nd(&P.map1, base, 3, extent, stride, box1) ||
+      !encode_tmap_nd(&P.map_q, p.query, 3, extent_q, stride, box_q))
     return cudaErrorInvalidValue;
   if (rows == 16) return fp16 ? launch<true, 16>(P, stream) : launch<false, 16>(P, stream);
   return fp16 ? launch<true, 32>(P, stream) : launch<false, 32>(P, stream);

@@ -1,70 +1,399 @@
-// Latent attention, expanded form (cascade_latent_prefill).
+// Latent attention, expanded form (cascade_latent_prefill), on the tensor cores.
 //
 // For a query row of head h: s_t = scale (<q[0:128], k_th> + <q[128:192], r_t>)
-// over the sequence's keys it may see, out = sum_t softmax(s)_t v_th with the
-// running maximum and sum in fp32. One warp per query row.
+// over the sequence's keys it may see, out = sum_t softmax(s)_t v_th. 640 flops
+// per (query, key, head): bound by the tensor cores, with the exponentials (16
+// per clock and SM: 2,048 cycles for the 256 x 128 scores whose products take
+// 2,700) close behind.
+//
+// One CTA computes 256 query tokens of one (sequence, head) as two tiles of 128
+// that share the key and value tiles of 128 tokens; their softmax warpgroups
+// alternate, so the tensor pipe has one tile's products while the other's
+// softmax runs. Per key tile j the issue order is PV_A(j), S_A(j+1), PV_B(j),
+// S_B(j+1). Scores S (fp32) and P (16-bit, over the first half of S's columns)
+// of both tiles and both outputs fill the tensor memory (4 x 128 columns).
+// Shared memory: the query tiles (96 KB) and a ring of eight 16 KB chunks for
+// keys (three of 128 tokens x 64 dims, the third the shared rotary part) and
+// values (two of 64 tokens x 128 dims).
+//
+// Softmax: a thread holds its row's 128 scores in registers; the running
+// maximum moves only when a score exceeds it by more than 2^8, so the output is
+// rescaled rarely; fp32 sums of the exponentials (log-sum-exp) and of the
+// rounded P (by which the output is divided: rounding that all weights of a
+// row share then cancels).
+//
+// Causal: key tiles past a tile's last row are not computed, only tiles that
+// cross the diagonal or the sequence's end are masked. CTAs go to the longest
+// rows first, the pairs of one head next to one another (its keys and values
+// stay in L2).
+//
+// Warps: 0-3 softmax and output of tile A, 4-7 of tile B, 8 TMA, 9 MMA issue.
+#include <algorithm>
+#include <cstddef>
+
 #include "kernels.h"
 #include "ptx.cuh"
 
 namespace cascade {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kRows = 128, kTok = 128;
+constexpr int kThreads = 10 * 32;
+constexpr int kChunk = 16384;
+constexpr int kSlots = 8;
+constexpr int kOffQ = 0;                        // [tile][3 chunks]
+constexpr int kOffRing = kOffQ + 6 * kChunk;
+constexpr int kBytes = kOffRing + kSlots * kChunk;
+
+struct __align__(16) Aux {
+  uint64_t q_full, k_full[2], v_full[2], v_empty[2], s_full[2][2], p_full[2], o_final[2], stall, drain;
+  uint32_t tmem_base;
+};
+constexpr int kStaticBytes = 32;  // the wait state comes first
+constexpr int kSmemBytes = (kStaticBytes + static_cast<int>(sizeof(Aux)) + 1023) / 1024 * 1024 + kBytes - kStaticBytes;
+static_assert(kSmemBytes + kStaticBytes <= 227 * 1024, "shared memory per CTA");
+
+struct Params {
+  LatentPrefillLaunch L;
+  CUtensorMap q, k, rope, v;
+  int32_t k_head, v_head;  // 0: one head's keys (values) serve all
+};
 
 template <bool kFp16>
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if constexpr (kFp16) {
     return __half22float2(*reinterpret_cast<__half2*>(&v));
   } else {
-    return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
   }
 }
 
 template <bool kFp16>
-__global__ void __launch_bounds__(kWarps * 32) latent_prefill_kernel(const LatentPrefillLaunch p) {
-  const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x & 31;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __grid_constant__ Params P) {
+  const LatentPrefillLaunch& p = P.L;
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int row0 = static_cast<int>(gridDim.x - 1 - blockIdx.x) * 2 * kRows;
   const int64_t q0 = p.cu_q[b], k0 = p.cu_kv[b];
-  const int64_t n = p.cu_q[b + 1] - q0, m_kv = p.cu_kv[b + 1] - k0;
-  if (i >= n || q0 < 0 || q0 + n > p.num_tokens || k0 < 0 || k0 + m_kv > p.num_kv) return;
-  const int64_t row = (q0 + i) * p.num_heads + h;
-  const int64_t last = p.causal ? min(m_kv, m_kv - n + i + 1) : m_kv;
-  auto pair = [](const void* base, int64_t element) { return static_cast<const uint32_t*>(base) + element / 2; };
-  const uint32_t* q = pair(p.query, row * kPrefillDk);
-  const float2 x0 = unpack2<kFp16>(q[lane]), x1 = unpack2<kFp16>(q[lane + 32]), x2 = unpack2<kFp16>(q[lane + 64]);
-  float2 o0 = make_float2(0.f, 0.f), o1 = o0;
-  float m = -INFINITY, l = 0.f;
-  for (int64_t t = 0; t < last; ++t) {
-    const uint32_t* k = pair(p.key, (k0 + t) * p.key_ts + h * p.key_hs);
-    const uint32_t* r = pair(p.key_rope, (k0 + t) * p.rope_ts);
-    const uint32_t* v = pair(p.value, (k0 + t) * p.value_ts + h * p.value_hs);
-    const float2 a = unpack2<kFp16>(k[lane]), c = unpack2<kFp16>(k[lane + 32]), d = unpack2<kFp16>(r[lane]);
-    float s = x0.x * a.x + x0.y * a.y + x1.x * c.x + x1.y * c.y + x2.x * d.x + x2.y * d.y;
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= p.scale;
-    const float m_new = fmaxf(m, s);
-    const float dm = m == m_new ? 1.f : expf(m - m_new);
-    const float e = m_new == -INFINITY ? 0.f : expf(s - m_new);
-    const float2 v0 = unpack2<kFp16>(v[lane]), v1 = unpack2<kFp16>(v[lane + 32]);
-    l = l * dm + e;
-    o0 = make_float2(fmaf(e, v0.x, o0.x * dm), fmaf(e, v0.y, o0.y * dm));
-    o1 = make_float2(fmaf(e, v1.x, o1.x * dm), fmaf(e, v1.y, o1.y * dm));
-    m = m_new;
+  const int64_t nq = p.cu_q[b + 1] - q0, nk = p.cu_kv[b + 1] - k0;
+  if (row0 >= nq || q0 < 0 || q0 + nq > p.num_tokens || k0 < 0 || nk < 0 || k0 + nk > p.num_kv) return;
+  const int n = static_cast<int>(nq), m = static_cast<int>(nk);
+  // keys that query token i sees
+  auto limit = [&](int i) { return p.causal ? max(0, min(m, m - n + i + 1)) : m; };
+  // key tiles of query tile t (0 if it has no rows): B's are at least A's, or none
+  auto tiles = [&](int t) {
+    const int first = row0 + t * kRows;
+    return first < n ? (limit(min(n, first + kRows) - 1) + kTok - 1) / kTok : 0;
+  };
+  const int nt[2] = {tiles(0), tiles(1)};
+  const int steps = max(nt[0], nt[1]);
+  const int tl = nt[1] > 0 ? 1 : 0;  // the tile whose products come last in a step
+
+  extern __shared__ uint8_t smem_raw[];
+  Aux* aux = reinterpret_cast<Aux*>(smem_raw);
+  uint8_t* smem = smem_raw + sizeof(Aux) + ((0u - (smem_u32(smem_raw) + static_cast<uint32_t>(sizeof(Aux)))) & 1023u);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
+    mbar_init(&aux->q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&aux->k_full[i], 1);
+      mbar_init(&aux->v_full[i], 1);
+      mbar_init(&aux->v_empty[i], 1);
+      mbar_init(&aux->s_full[i][0], 1);
+      mbar_init(&aux->s_full[i][1], 1);
+      mbar_init(&aux->p_full[i], 4);
+      mbar_init(&aux->o_final[i], 1);
+    }
+    mbar_init(&aux->stall, 1);
+    mbar_init(&aux->drain, 1);
+    fence_mbar_init();
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  uint32_t* out = static_cast<uint32_t*>(p.out) + row * (kPrefillDv / 2);
-  out[lane] = pack2<kFp16>(o0.x * inv, o0.y * inv);
-  out[lane + 32] = pack2<kFp16>(o1.x * inv, o1.y * inv);
-  if (lane == 0) p.lse[row] = l > 0.f ? m + logf(l) : -INFINITY;
+  if (warp == 9) {
+    tmem_alloc(&aux->tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = aux->tmem_base;
+  auto slot_of = [&](int q) { return smem + kOffRing + (q % kSlots) * kChunk; };  // chunk q of the load order
+
+  if (warp == 8) {
+    // ------------------------------------------------------------- producer
+    // load order K(0), V(0), K(1), V(1), ...: chunks 5j + 0..2 and 5j + 3..4.
+    // A chunk's slot was chunk q - 8's: K(j) replaces the end of K(j-2) and
+    // V(j-2), V(j) the start of K(j-1). s_full of a tile also says that what
+    // was issued before it is done.
+    bool live = true;
+    if (steps > 0 && elect_one()) {
+      mbar_arrive_expect_tx(&aux->q_full, (tl + 1) * 3 * kChunk);
+      for (int t = 0; t <= tl; ++t)
+        for (int c = 0; c < 3; ++c)
+          tma_load_3d(smem + kOffQ + (t * 3 + c) * kChunk, &P.q, &aux->q_full, 0,
+                      static_cast<int>(q0) + row0 + t * kRows, h * 3 + c);
+    }
+    __syncwarp();
+    for (int j = 0; live && j < steps; ++j) {
+      const int tok = static_cast<int>(k0) + j * kTok;
+      live = j < 2 || mbar_wait_warp(&aux->v_empty[j & 1], ((j >> 1) - 1) & 1);
+      if (!live) break;
+      if (elect_one()) {
+        uint64_t* bar = &aux->k_full[j & 1];
+        mbar_arrive_expect_tx(bar, 3 * kChunk);
+        for (int c = 0; c < 2; ++c) tma_load_4d(slot_of(5 * j + c), &P.k, bar, 0, tok, c, h * P.k_head);
+        tma_load_3d(slot_of(5 * j + 2), &P.rope, bar, 0, tok, 0);
+      }
+      __syncwarp();
+      live = j < 1 || mbar_wait_warp(&aux->s_full[tl][(j - 1) & 1], ((j - 1) >> 1) & 1);
+      if (!live) break;
+      if (elect_one()) {
+        uint64_t* bar = &aux->v_full[j & 1];
+        mbar_arrive_expect_tx(bar, 2 * kChunk);
+        for (int c = 0; c < 2; ++c) tma_load_4d(slot_of(5 * j + 3 + c), &P.v, bar, 0, tok + c * 64, 0, h * P.v_head);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 9) {
+    // ----------------------------------------------------------- MMA issuer
+    constexpr uint32_t fmt = kFp16 ? 0u : 1u;
+    const uint32_t idesc_s = make_idesc_f16(kRows, kTok, fmt, 0, 0);
+    const uint32_t idesc_pv = make_idesc_f16(kRows, kPrefillDv, fmt, 0, 1);
+    const uint32_t tm = uniform(tbase), s0 = uniform(smem_u32(smem));
+    auto scores = [&](int t, int j) {
+      const uint32_t u = uniform(static_cast<uint32_t>(j));
+      const uint64_t dq = make_smem_desc(s0 + kOffQ + t * 3 * kChunk, 16, 1024, 2);
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 0; c < 3; ++c) {
+          const uint64_t dk = make_smem_desc(s0 + kOffRing + (5 * u + c) % kSlots * kChunk, 16, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ss(tm + t * 128, dq + (c * kChunk + k * 32) / 16, dk + k * 2, idesc_s, c + k > 0);
+        }
+        umma_commit(&aux->s_full[t][j & 1]);
+      }
+      __syncwarp();
+    };
+    auto values = [&](int t, int j, bool last) {
+      const uint32_t u = uniform(static_cast<uint32_t>(j));
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          // 64 tokens x two groups of 64 dims, 8 KB apart
+          const uint64_t dv = make_smem_desc(s0 + kOffRing + (5 * u + 3 + c) % kSlots * kChunk, kChunk / 2, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ts(tm + 256 + t * 128, tm + t * 128 + (c * 4 + k) * 8, dv + k * 128, idesc_pv,
+                        j > 0 || c + k > 0);
+        }
+        if (t == tl) umma_commit(&aux->v_empty[j & 1]);
+        if (last) umma_commit(&aux->o_final[t]);
+      }
+      __syncwarp();
+    };
+    bool live = steps > 0 && mbar_wait_warp(&aux->q_full, 0) && mbar_wait_warp(&aux->k_full[0], 0);
+    if (live) {
+      if (nt[0] > 0) scores(0, 0);
+      if (nt[1] > 0) scores(1, 0);
+    }
+    for (int j = 0; live && j < steps; ++j) {
+      live = mbar_wait_warp(&aux->v_full[j & 1], (j >> 1) & 1);
+      bool have_k = false;
+      for (int t = 0; live && t < 2; ++t) {
+        if (j >= nt[t]) continue;
+        live = mbar_wait_warp(&aux->p_full[t], j & 1);
+        if (!live) break;
+        values(t, j, j + 1 == nt[t]);
+        if (j + 1 < nt[t]) {
+          live = have_k || mbar_wait_warp(&aux->k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
+          have_k = true;
+          if (live) scores(t, j + 1);
+        }
+      }
+    }
+    if (steps > 0 && !live && lane == 0) {
+      umma_commit(&aux->drain);
+      mbar_wait_drain(&aux->drain, 0);
+    }
+  } else {
+    // ------------------------------------------------- softmax, output of tile t
+    const int t = warp >> 2, r = tid & 127, row = row0 + t * kRows + r;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t scol = tbase + lane_off + t * 128, ocol = tbase + lane_off + 256 + t * 128;
+    const float sl2 = p.scale * 1.4426950408889634f;
+    const int mine = t ? nt[1] : nt[0];
+    const int lim = limit(min(row, n - 1));
+    const int clean = limit(min(row0 + t * kRows, n - 1)) / kTok;  // tiles below are seen in full by every row
+    float mx = -INFINITY, l = 0.f, lp = 0.f;
+    bool live = true;
+    if (p.debug_stall) live = mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
+    for (int j = 0; live && j < mine; ++j) {
+      live = mbar_wait_warp(&aux->s_full[t][j & 1], (j >> 1) & 1);
+      if (!live) break;
+      tc_fence_after();
+      uint32_t s[128];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) tmem_ld_32x32b_x32(scol + g * 32, *reinterpret_cast<uint32_t(*)[32]>(s + g * 32));
+      tmem_wait_ld();
+      if (j >= clean) {
+        const int seen = lim - j * kTok;
+#pragma unroll
+        for (int e = 0; e < 128; ++e) s[e] = e < seen ? s[e] : 0xff800000u;
+      }
+      float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 128; e += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          a[i] = fmax3f(a[i], __uint_as_float(s[e + 2 * i]), __uint_as_float(s[e + 2 * i + 1]));
+      }
+      const float top = fmax3f(a[0], a[1], fmaxf(a[2], a[3])) * sl2;
+      const bool move = top > mx + 8.f;
+      const float dm = move ? ex2(mx - top) : 1.f;  // 0 while nothing has been seen
+      if (move) mx = top;
+      const float neg = mx == -INFINITY ? 0.f : -mx;
+      if (j > 0 && __any_sync(0xffffffffu, move)) {
+        // the scores of tile j come after P V of tile j - 1: the output is at rest
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(ocol + g * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * dm);
+          tmem_st_32x32b_x32(ocol + g * 32, o);
+        }
+      }
+      float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f, p0 = 0.f, p1 = 0.f, p2 = 0.f, p3 = 0.f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          float y0, y1, y2, y3;
+          const uint32_t* x = s + g * 32 + e;
+          ffma2_bcast(y0, y1, __uint_as_float(x[0]), __uint_as_float(x[1]), sl2, neg);
+          ffma2_bcast(y2, y3, __uint_as_float(x[2]), __uint_as_float(x[3]), sl2, neg);
+          y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
+          fadd2(r0, r1, y0, y1);
+          fadd2(r2, r3, y2, y3);
+          pk[e >> 1] = pack2<kFp16>(y0, y1);
+          pk[(e >> 1) + 1] = pack2<kFp16>(y2, y3);
+          const float2 u = unpack2<kFp16>(pk[e >> 1]), v = unpack2<kFp16>(pk[(e >> 1) + 1]);
+          fadd2(p0, p1, u.x, u.y);
+          fadd2(p2, p3, v.x, v.y);
+        }
+        tmem_st_32x32b_x16(scol + g * 16, pk);
+      }
+      l = l * dm + ((r0 + r1) + (r2 + r3));
+      lp = lp * dm + ((p0 + p1) + (p2 + p3));
+      if ((j + 1) * kTok > m && (t == 0 || j >= nt[0])) {
+        // rows past the sequence may hold NaN, which weight 0 does not hide from
+        // the product: the tile whose product comes first clears them
+        live = mbar_wait_warp(&aux->v_full[j & 1], (j >> 1) & 1);
+        if (!live) break;
+        if (j * kTok + r >= m) {
+          uint8_t* chunk = slot_of(5 * j + 3 + (r >> 6)) + (r & 63) * 128;
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            *reinterpret_cast<uint4*>(chunk + (q >> 3) * (kChunk / 2) + (q & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&aux->p_full[t]);
+    }
+    // output: 256 bytes per row through the query tile's shared memory (done with; 16-byte chunk q of
+    // row r at q ^ (r % 8)), so that a store instruction writes whole rows
+    const int rows = min(32, n - (row0 + t * kRows + (r & ~31)));  // this warp's
+    if (live && rows > 0) {
+      float inv = 0.f, lse = -INFINITY;
+      if (mine > 0) {
+        live = mbar_wait_warp(&aux->o_final[t], 0);
+        tc_fence_after();
+        if (lp > 0.f) inv = 1.f / lp;
+        if (l > 0.f) lse = (mx + __log2f(l)) * 0.6931471805599453f;
+      }
+      uint8_t* stage = smem + kOffQ + t * 3 * kChunk + (warp & 3) * 8192;
+      if (live) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint32_t o[32] = {};
+          if (mine > 0) {
+            tmem_ld_32x32b_x32(ocol + g * 32, o);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int e = q * 8 + i * 2;
+              w[i] = inv > 0.f ? pack2<kFp16>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv) : 0u;
+            }
+            *reinterpret_cast<uint4*>(stage + lane * 256 + (((g * 4 + q) ^ (lane & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+        const int64_t first = (q0 + row0 + t * kRows + (r & ~31)) * p.num_heads + h;
+        if (lane < rows) p.lse[first + static_cast<int64_t>(lane) * p.num_heads] = lse;
+#pragma unroll 4
+        for (int rr = lane >> 4; rr < rows; rr += 2) {
+          const int q = lane & 15;
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 256 + ((q ^ (rr & 7)) << 4));
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + (first + static_cast<int64_t>(rr) * p.num_heads) * kPrefillDv +
+                                    q * 8) = v;
+        }
+      }
+    }
+  }
+  if (cta_aborted()) {
+    // loads may be in flight (at most 224 KB): they get a millisecond before the CTA leaves
+    for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000 * 1000;) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
 }
 
 }  // namespace
 
 cudaError_t launch_latent_prefill(const LatentPrefillLaunch& p, bool fp16, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>((p.max_q + kWarps - 1) / kWarps), p.num_heads, p.batch);
+  Params P;
+  P.L = p;
+  P.k_head = p.key_hs != 0;
+  P.v_head = p.value_hs != 0;
+  // no keys at all: maps over the query stand in, nothing is loaded through them
+  const bool any = p.num_kv > 0;
+  const uint64_t T = static_cast<uint64_t>(p.num_tokens), S = any ? static_cast<uint64_t>(p.num_kv) : 1;
+  const uint64_t H = static_cast<uint64_t>(p.num_heads);
+  auto bytes = [](int64_t stride) { return static_cast<uint64_t>(stride) * 2; };
+  const uint64_t q_extent[3] = {64, T, 3 * H}, q_stride[2] = {H * kPrefillDk * 2, 128};
+  const uint32_t q_box[3] = {64, kRows, 1}, k_box[4] = {64, kTok, 1, 1}, v_box[4] = {64, 64, 2, 1}, r_box[3] = {64, kTok, 1};
+  const uint64_t k_extent[4] = {64, S, 2, P.k_head ? H : 1}, v_extent[4] = {64, S, 2, P.v_head ? H : 1};
+  const uint64_t k_stride[3] = {bytes(p.key_ts), 128, P.k_head ? bytes(p.key_hs) : 256};
+  const uint64_t v_stride[3] = {bytes(p.value_ts), 128, P.v_head ? bytes(p.value_hs) : 256};
+  const uint64_t r_extent[3] = {64, S, 1}, r_stride[2] = {bytes(p.rope_ts), 128};
+  if (!encode_tmap_nd(&P.q, p.query, 3, q_extent, q_stride, q_box) ||
+      !encode_tmap_nd(&P.k, any ? p.key : p.query, 4, k_extent, k_stride, k_box) ||
+      !encode_tmap_nd(&P.v, any ? p.value : p.query, 4, v_extent, v_stride, v_box) ||
+      !encode_tmap_nd(&P.rope, any ? p.key_rope : p.query, 3, r_extent, r_stride, r_box))
+    return cudaErrorInvalidValue;
   auto kern = fp16 ? latent_prefill_kernel<true> : latent_prefill_kernel<false>;
-  kern<<<grid, kWarps * 32, 0, stream>>>(p);
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), kSmemBytes);
+  if (e != cudaSuccess) return e;
+  const dim3 grid(static_cast<unsigned>((p.max_q + 2 * kRows - 1) / (2 * kRows)), p.num_heads, p.batch);
+  kern<<<grid, kThreads, kSmemBytes, stream>>>(P);
   return cudaGetLastError();
 }
 
