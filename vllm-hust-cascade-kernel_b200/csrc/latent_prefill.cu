@@ -16,18 +16,17 @@
 // keys (three of 128 tokens x 64 dims, the third the shared rotary part) and
 // values (two of 64 tokens x 128 dims).
 //
-// Softmax: a thread holds its row's 128 scores in registers; the running
-// maximum moves only when a score exceeds it by more than 2^8, so the output is
-// rescaled rarely; fp32 sums of the exponentials (log-sum-exp) and of the
-// rounded P (by which the output is divided: rounding that all weights of a
-// row share then cancels).
+// Softmax: two threads per row, 64 of a tile's 128 keys each (one thread took
+// 2,180 cycles from scores to P, in which its tile's products stood still); the
+// running maximum moves only when a score exceeds it by more than 2^8, so the
+// output is rescaled rarely; sums of the exponentials in fp32.
 //
 // Causal: key tiles past a tile's last row are not computed, only tiles that
 // cross the diagonal or the sequence's end are masked. CTAs go to the longest
 // rows first, the pairs of one head next to one another (its keys and values
 // stay in L2).
 //
-// Warps: 0-3 softmax and output of tile A, 4-7 of tile B, 8 TMA, 9 MMA issue.
+// Warps: 0-7 softmax and output of tile A, 8-15 of tile B, 16 TMA, 17 MMA issue.
 #include <algorithm>
 #include <cstddef>
 
@@ -38,7 +37,7 @@ namespace cascade {
 namespace {
 
 constexpr int kRows = 128, kTok = 128;
-constexpr int kThreads = 10 * 32;
+constexpr int kThreads = 18 * 32;
 constexpr int kChunk = 16384;
 constexpr int kSlots = 8;
 constexpr int kOffQ = 0;                        // [tile][3 chunks]
@@ -46,6 +45,7 @@ constexpr int kOffRing = kOffQ + 6 * kChunk;
 constexpr int kBytes = kOffRing + kSlots * kChunk;
 
 struct __align__(16) Aux {
+  float shared[2][2][kRows];  // [tile][half of the keys]: the row's maximum, at the end its sum
   uint64_t q_full, k_full[2], v_full[2], v_empty[2], s_full[2][2], p_full[2], o_final[2], stall, drain;
   uint32_t tmem_base;
 };
@@ -58,15 +58,6 @@ struct Params {
   CUtensorMap q, k, rope, v;
   int32_t k_head, v_head;  // 0: one head's keys (values) serve all
 };
-
-template <bool kFp16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if constexpr (kFp16) {
-    return __half22float2(*reinterpret_cast<__half2*>(&v));
-  } else {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  }
-}
 
 template <bool kFp16>
 __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __grid_constant__ Params P) {
@@ -102,14 +93,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
       mbar_init(&aux->v_empty[i], 1);
       mbar_init(&aux->s_full[i][0], 1);
       mbar_init(&aux->s_full[i][1], 1);
-      mbar_init(&aux->p_full[i], 4);
+      mbar_init(&aux->p_full[i], 8);
       mbar_init(&aux->o_final[i], 1);
     }
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
   }
-  if (warp == 9) {
+  if (warp == 17) {
     tmem_alloc(&aux->tmem_base, 512);
     tmem_relinquish();
   }
@@ -119,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
   const uint32_t tbase = aux->tmem_base;
   auto slot_of = [&](int q) { return smem + kOffRing + (q % kSlots) * kChunk; };  // chunk q of the load order
 
-  if (warp == 8) {
+  if (warp == 16) {
     // ------------------------------------------------------------- producer
     // load order K(0), V(0), K(1), V(1), ...: chunks 5j + 0..2 and 5j + 3..4.
     // A chunk's slot was chunk q - 8's: K(j) replaces the end of K(j-2) and
@@ -154,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
       }
       __syncwarp();
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // ----------------------------------------------------------- MMA issuer
     constexpr uint32_t fmt = kFp16 ? 0u : 1u;
     const uint32_t idesc_s = make_idesc_f16(kRows, kTok, fmt, 0, 0);
@@ -220,37 +211,47 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
     }
   } else {
     // ------------------------------------------------- softmax, output of tile t
-    const int t = warp >> 2, r = tid & 127, row = row0 + t * kRows + r;
+    const int t = warp >> 3, hh = (warp >> 2) & 1, r = tid & 127, row = row0 + t * kRows + r;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t scol = tbase + lane_off + t * 128, ocol = tbase + lane_off + 256 + t * 128;
+    const uint32_t scol = tbase + lane_off + t * 128, ocol = tbase + lane_off + 256 + t * 128 + hh * 64;
     const float sl2 = p.scale * 1.4426950408889634f;
     const int mine = t ? nt[1] : nt[0];
     const int lim = limit(min(row, n - 1));
     const int clean = limit(min(row0 + t * kRows, n - 1)) / kTok;  // tiles below are seen in full by every row
-    float mx = -INFINITY, l = 0.f, lp = 0.f;
-    bool live = true;
-    if (p.debug_stall) live = mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
-    for (int j = 0; live && j < mine; ++j) {
-      live = mbar_wait_warp(&aux->s_full[t][j & 1], (j >> 1) & 1);
-      if (!live) break;
+    // the two warps of 32 rows meet here; neither leaves the loop early (an aborted CTA's waits return at once), so
+    // neither is waited for in vain
+    auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
+    float mx = -INFINITY, l = 0.f;
+    if (p.debug_stall) mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
+    for (int j = 0; j < mine; ++j) {
+      mbar_wait_warp(&aux->s_full[t][j & 1], (j >> 1) & 1);
       tc_fence_after();
-      uint32_t s[128];
+      const int seen = j >= clean ? lim - j * kTok - hh * 64 : 64;
+      auto load = [&](int g, uint32_t (&x)[32]) {
+        tmem_ld_32x32b_x32(scol + hh * 64 + g * 32, x);
+        tmem_wait_ld();
+        if (j >= clean) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) tmem_ld_32x32b_x32(scol + g * 32, *reinterpret_cast<uint32_t(*)[32]>(s + g * 32));
-      tmem_wait_ld();
-      if (j >= clean) {
-        const int seen = lim - j * kTok;
+          for (int e = 0; e < 32; ++e) x[e] = g * 32 + e < seen ? x[e] : 0xff800000u;
+        }
+      };
+      float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 128; ++e) s[e] = e < seen ? s[e] : 0xff800000u;
+      for (int g = 0; g < 2; ++g) {
+        uint32_t x[32];
+        load(g, x);
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          a0 = fmax3f(a0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          a1 = fmax3f(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+          a2 = fmax3f(a2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
+          a3 = fmax3f(a3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
+        }
       }
-      float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int e = 0; e < 128; e += 8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          a[i] = fmax3f(a[i], __uint_as_float(s[e + 2 * i]), __uint_as_float(s[e + 2 * i + 1]));
-      }
-      const float top = fmax3f(a[0], a[1], fmaxf(a[2], a[3])) * sl2;
+      a0 = fmax3f(a0, a1, fmaxf(a2, a3));
+      aux->shared[t][hh][r] = a0;
+      meet();
+      const float top = fmaxf(a0, aux->shared[t][hh ^ 1][r]) * sl2;
       const bool move = top > mx + 8.f;
       const float dm = move ? ex2(mx - top) : 1.f;  // 0 while nothing has been seen
       if (move) mx = top;
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
       if (j > 0 && __any_sync(0xffffffffu, move)) {
         // the scores of tile j come after P V of tile j - 1: the output is at rest
 #pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
+        for (int g = 0; g < 2; ++g) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(ocol + g * 32, o);
           tmem_wait_ld();
@@ -267,34 +268,33 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
           tmem_st_32x32b_x32(ocol + g * 32, o);
         }
       }
-      float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f, p0 = 0.f, p1 = 0.f, p2 = 0.f, p3 = 0.f;
+      // P of the other half lies over this half's first scores (columns 32-63 of the tile's 128): each half is
+      // read into registers, and both have been, before either is overwritten
+      float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f;
+      uint32_t pk[32];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t pk[16];
+      for (int g = 0; g < 2; ++g) {
+        uint32_t x[32];
+        load(g, x);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           float y0, y1, y2, y3;
-          const uint32_t* x = s + g * 32 + e;
-          ffma2_bcast(y0, y1, __uint_as_float(x[0]), __uint_as_float(x[1]), sl2, neg);
-          ffma2_bcast(y2, y3, __uint_as_float(x[2]), __uint_as_float(x[3]), sl2, neg);
+          ffma2_bcast(y0, y1, __uint_as_float(x[e]), __uint_as_float(x[e + 1]), sl2, neg);
+          ffma2_bcast(y2, y3, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]), sl2, neg);
           y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
           fadd2(r0, r1, y0, y1);
           fadd2(r2, r3, y2, y3);
-          pk[e >> 1] = pack2<kFp16>(y0, y1);
-          pk[(e >> 1) + 1] = pack2<kFp16>(y2, y3);
-          const float2 u = unpack2<kFp16>(pk[e >> 1]), v = unpack2<kFp16>(pk[(e >> 1) + 1]);
-          fadd2(p0, p1, u.x, u.y);
-          fadd2(p2, p3, v.x, v.y);
+          pk[g * 16 + (e >> 1)] = pack2<kFp16>(y0, y1);
+          pk[g * 16 + (e >> 1) + 1] = pack2<kFp16>(y2, y3);
         }
-        tmem_st_32x32b_x16(scol + g * 16, pk);
       }
       l = l * dm + ((r0 + r1) + (r2 + r3));
-      lp = lp * dm + ((p0 + p1) + (p2 + p3));
-      if ((j + 1) * kTok > m && (t == 0 || j >= nt[0])) {
+      meet();
+      tmem_st_32x32b_x32(scol + hh * 32, pk);
+      if ((j + 1) * kTok > m && (t == 0 || j >= nt[0]) && hh == 0) {
         // rows past the sequence may hold NaN, which weight 0 does not hide from
         // the product: the tile whose product comes first clears them
-        live = mbar_wait_warp(&aux->v_full[j & 1], (j >> 1) & 1);
-        if (!live) break;
+        mbar_wait_warp(&aux->v_full[j & 1], (j >> 1) & 1);
         if (j * kTok + r >= m) {
           uint8_t* chunk = slot_of(5 * j + 3 + (r >> 6)) + (r & 63) * 128;
 #pragma unroll
@@ -308,48 +308,52 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
       __syncwarp();
       if (lane == 0) mbar_arrive(&aux->p_full[t]);
     }
-    // output: 256 bytes per row through the query tile's shared memory (done with; 16-byte chunk q of
-    // row r at q ^ (r % 8)), so that a store instruction writes whole rows
-    const int rows = min(32, n - (row0 + t * kRows + (r & ~31)));  // this warp's
-    if (live && rows > 0) {
-      float inv = 0.f, lse = -INFINITY;
-      if (mine > 0) {
-        live = mbar_wait_warp(&aux->o_final[t], 0);
-        tc_fence_after();
-        if (lp > 0.f) inv = 1.f / lp;
-        if (l > 0.f) lse = (mx + __log2f(l)) * 0.6931471805599453f;
+    float inv = 0.f, lse = -INFINITY;
+    if (mine > 0) {
+      mbar_wait_warp(&aux->o_final[t], 0);  // both warps have read the maxima: the slots take the sums
+      tc_fence_after();
+      aux->shared[t][hh][r] = l;
+      meet();
+      l = aux->shared[t][0][r] + aux->shared[t][1][r];
+      if (l > 0.f) {
+        inv = 1.f / l;
+        lse = (mx + __log2f(l)) * 0.6931471805599453f;
       }
-      uint8_t* stage = smem + kOffQ + t * 3 * kChunk + (warp & 3) * 8192;
-      if (live) {
+    }
+    // output: 128 bytes per row and warp through the query tile's shared memory (done with; 16-byte chunk q of
+    // row r at q ^ (r % 8)), so that a store instruction writes whole lines of four rows
+    const int rows = min(32, n - (row0 + t * kRows + (r & ~31)));  // this warp's
+    uint8_t* stage = smem + kOffQ + t * 3 * kChunk + (warp & 7) * 4096;
+    if (rows > 0 && !__any_sync(0xffffffffu, cta_aborted())) {
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          uint32_t o[32] = {};
-          if (mine > 0) {
-            tmem_ld_32x32b_x32(ocol + g * 32, o);
-            tmem_wait_ld();
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int e = q * 8 + i * 2;
-              w[i] = inv > 0.f ? pack2<kFp16>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv) : 0u;
-            }
-            *reinterpret_cast<uint4*>(stage + lane * 256 + (((g * 4 + q) ^ (lane & 7)) << 4)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
+      for (int g = 0; g < 2; ++g) {
+        uint32_t o[32] = {};
+        if (mine > 0) {
+          tmem_ld_32x32b_x32(ocol + g * 32, o);
+          tmem_wait_ld();
         }
-        __syncwarp();
-        const int64_t first = (q0 + row0 + t * kRows + (r & ~31)) * p.num_heads + h;
-        if (lane < rows) p.lse[first + static_cast<int64_t>(lane) * p.num_heads] = lse;
-#pragma unroll 4
-        for (int rr = lane >> 4; rr < rows; rr += 2) {
-          const int q = lane & 15;
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 256 + ((q ^ (rr & 7)) << 4));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = q * 8 + i * 2;
+            w[i] = inv > 0.f ? pack2<kFp16>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv) : 0u;
+          }
+          *reinterpret_cast<uint4*>(stage + lane * 128 + (((g * 4 + q) ^ (lane & 7)) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();
+      const int64_t first = (q0 + row0 + t * kRows + (r & ~31)) * p.num_heads + h;
+      if (hh == 0 && lane < rows) p.lse[first + static_cast<int64_t>(lane) * p.num_heads] = lse;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int rr = i * 4 + (lane >> 3), q = lane & 7;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((q ^ (rr & 7)) << 4));
+        if (rr < rows)
           *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + (first + static_cast<int64_t>(rr) * p.num_heads) * kPrefillDv +
-                                    q * 8) = v;
-        }
+                                    hh * 64 + q * 8) = v;
       }
     }
   }
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
