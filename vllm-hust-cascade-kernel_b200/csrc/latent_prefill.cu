@@ -10,7 +10,7 @@
 // that share the key and value tiles of 128 tokens; their softmax warpgroups
 // alternate, so the tensor pipe has one tile's products while the other's
 // softmax runs. Per key tile j the issue order is PV_A(j), S_A(j+1), PV_B(j),
-// S_B(j+1). Scores S (fp32) and P (16-bit, over the first half of S's columns)
+// S_B(j+1). Scores S (fp32) and P (16-bit, over S's columns)
 // of both tiles and both outputs fill the tensor memory (4 x 128 columns).
 // Shared memory: the query tiles (96 KB) and a ring of eight 16 KB chunks for
 // keys (three of 128 tokens x 64 dims, the third the shared rotary part) and
@@ -40,6 +40,8 @@ constexpr int kRows = 128, kTok = 128;
 constexpr int kThreads = 18 * 32;
 constexpr int kChunk = 16384;
 constexpr int kSlots = 8;
+constexpr int kPolyOf8 = 2;  // of eight groups of four exponentials, those with two on the FMA pipe (0: 438, 2: 427, 4: 426, 8: 449 us
+                             // on the two long prompts)
 constexpr int kOffQ = 0;                        // [tile][3 chunks]
 constexpr int kOffRing = kOffQ + 6 * kChunk;
 constexpr int kBytes = kOffRing + kSlots * kChunk;
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
           const uint64_t dv = make_smem_desc(s0 + kOffRing + (5 * u + 3 + c) % kSlots * kChunk, kChunk / 2, 1024, 2);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tm + 256 + t * 128, tm + t * 128 + (c * 4 + k) * 8, dv + k * 128, idesc_pv,
+            umma_f16_ts(tm + 256 + t * 128, tm + t * 128 + c * 64 + k * 8, dv + k * 128, idesc_pv,
                         j > 0 || c + k > 0);
         }
         if (t == tl) umma_commit(&aux->v_empty[j & 1]);
@@ -268,29 +270,31 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
           tmem_st_32x32b_x32(ocol + g * 32, o);
         }
       }
-      // P of the other half lies over this half's first scores (columns 32-63 of the tile's 128): each half is
-      // read into registers, and both have been, before either is overwritten
+      // P goes over the first 32 columns of this half's own scores, read by then
       float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f;
-      uint32_t pk[32];
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        uint32_t x[32];
+        uint32_t x[32], pk[16];
         load(g, x);
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           float y0, y1, y2, y3;
           ffma2_bcast(y0, y1, __uint_as_float(x[e]), __uint_as_float(x[e + 1]), sl2, neg);
           ffma2_bcast(y2, y3, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]), sl2, neg);
-          y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
+          y0 = ex2(y0), y1 = ex2(y1);
+          if (e / 4 < kPolyOf8) {
+            ex2_poly2(y2, y3);
+          } else {
+            y2 = ex2(y2), y3 = ex2(y3);
+          }
           fadd2(r0, r1, y0, y1);
           fadd2(r2, r3, y2, y3);
-          pk[g * 16 + (e >> 1)] = pack2<kFp16>(y0, y1);
-          pk[g * 16 + (e >> 1) + 1] = pack2<kFp16>(y2, y3);
+          pk[e >> 1] = pack2<kFp16>(y0, y1);
+          pk[(e >> 1) + 1] = pack2<kFp16>(y2, y3);
         }
+        tmem_st_32x32b_x16(scol + hh * 64 + g * 16, pk);
       }
       l = l * dm + ((r0 + r1) + (r2 + r3));
-      meet();
-      tmem_st_32x32b_x32(scol + hh * 32, pk);
       if ((j + 1) * kTok > m && (t == 0 || j >= nt[0]) && hh == 0) {
         // rows past the sequence may hold NaN, which weight 0 does not hide from
         // the product: the tile whose product comes first clears them
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
       aux->shared[t][hh][r] = l;
       meet();
       l = aux->shared[t][0][r] + aux->shared[t][1][r];
-      if (l > 0.f) {
+      if (mx > -INFINITY) {
         inv = 1.f / l;
         lse = (mx + __log2f(l)) * 0.6931471805599453f;
       }

@@ -645,6 +645,44 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 2^x for two values on the FMA pipe (packed fp32), for where the special
+// function unit (16 per clock and SM) is the limit: x = n + f with n the nearest
+// whole number (Cody and Waite's reduction, by adding 1.5 * 2^23), 2^f by the
+// degree-4 polynomial of least relative error on [-1/2, 1/2] (2.6e-6, Remez),
+// n into the exponent. x at most 127; below -126 the result stays near 2^-126.
+__device__ __forceinline__ void ex2_poly2(float& y0, float& y1) {
+  y0 = fmaxf(y0, -126.f);
+  y1 = fmaxf(y1, -126.f);
+  asm("{\n\t.reg .b64 x, t, f, p, c;\n\t.reg .b32 t0, t1, p0, p1;\n\t"
+      "mov.b64 x, {%0, %1};\n\t"
+      "mov.b64 c, {%2, %2};\n\t"
+      "add.rn.f32x2 t, x, c;\n\t"
+      "mov.b64 c, {%3, %3};\n\t"
+      "add.rn.f32x2 f, t, c;\n\t"
+      "mov.b64 c, {%4, %4};\n\t"
+      "fma.rn.f32x2 f, f, c, x;\n\t"
+      "mov.b64 p, {%5, %5};\n\t"
+      "mov.b64 c, {%6, %6};\n\t"
+      "fma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%7, %7};\n\t"
+      "fma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%8, %8};\n\t"
+      "fma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 c, {%9, %9};\n\t"
+      "fma.rn.f32x2 p, p, f, c;\n\t"
+      "mov.b64 {t0, t1}, t;\n\t"
+      "mov.b64 {p0, p1}, p;\n\t"
+      "shl.b32 t0, t0, 23;\n\t"
+      "shl.b32 t1, t1, 23;\n\t"
+      "add.s32 p0, p0, t0;\n\t"
+      "add.s32 p1, p1, t1;\n\t"
+      "mov.b32 %0, p0;\n\t"
+      "mov.b32 %1, p1;\n\t}"
+      : "+f"(y0), "+f"(y1)
+      : "f"(12582912.f), "f"(-12582912.f), "f"(-1.f), "f"(0.009570102207362652f), "f"(0.05591785907745361f),
+        "f"(0.240247443318367f), "f"(0.6931217908859253f), "f"(0.9999992847442627f));
+}
+
 // max(a, b, c): one three-input max instruction on sm_100.
 __device__ __forceinline__ float fmax3f(float a, float b, float c) {
   float d;
