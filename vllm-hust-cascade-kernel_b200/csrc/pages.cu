@@ -27,6 +27,7 @@ constexpr int kPlanCtas = 8;      // portable cluster size
 constexpr int kPlanThreads = 1024;
 constexpr int kCopyThreads = 256;
 constexpr int kCopyUnroll = 4;
+constexpr int kCopyPerSm = 4;     // CTAs per SM: 64 KB of loads in flight (6: 179, 4: 159, 3: 162 us on 8 pools x 1,500 pages of 37 KB)
 constexpr int kPieceBytes = kCopyThreads * kCopyUnroll * 16;
 
 struct Pools {
@@ -49,38 +50,36 @@ struct CopyJobs {
 };
 
 template <typename Id>
-__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyJobs<Id> j, const Pools pools) {
+__global__ void __launch_bounds__(kCopyThreads, kCopyPerSm) page_copy_kernel(const CopyJobs<Id> j, const Pools pools) {
   pdl_wait();  // the jobs come from the launch before this one (returns at once without one)
   const int64_t count = j.count_dev ? *j.count_dev : j.count;
-  const int64_t pieces = (j.page_bytes + kPieceBytes - 1) / kPieceBytes;
+  const int pieces = static_cast<int>((j.page_bytes + kPieceBytes - 1) / kPieceBytes);
+  const int64_t piece_bytes = ((j.page_bytes + pieces - 1) / pieces + 15) / 16 * 16;  // equal pieces
   const int64_t tasks = count * pools.count * pieces;
   for (int64_t task = blockIdx.x; task < tasks; task += gridDim.x) {
-    const int64_t piece = task % pieces, rest = task / pieces;
-    const int pool = static_cast<int>(rest % pools.count);
-    const int64_t i = rest / pools.count;
+    // consecutive CTAs: the pieces of one page, then the pools
+    const uint32_t per_job = static_cast<uint32_t>(pools.count) * pieces;
+    const int64_t i = task / per_job;
+    const uint32_t rest = static_cast<uint32_t>(task - i * per_job);
     const int64_t bytes = j.rows ? j.rows[i] * j.row_bytes : j.page_bytes;
-    const int64_t begin = piece * kPieceBytes;
-    if (begin >= bytes) continue;
     const int64_t src = static_cast<int64_t>(j.src[i]), dst = static_cast<int64_t>(j.dst[i]);
+    const int64_t begin = static_cast<int64_t>(rest % pieces) * piece_bytes;
+    if (begin >= bytes) continue;
     if (src < 0 || src >= j.num_blocks || dst < 0 || dst >= j.num_blocks) {
       if (threadIdx.x == 0) atomicOr(&g_cascade_device_error, kErrBadBlockId);
       continue;
     }
-    uint8_t* base = static_cast<uint8_t*>(pools.ptr[pool]);
-    const uint4* from = reinterpret_cast<const uint4*>(base + src * j.page_bytes + begin);
-    uint4* to = reinterpret_cast<uint4*>(base + dst * j.page_bytes + begin);
-    const int words = static_cast<int>(min(static_cast<int64_t>(kPieceBytes), bytes - begin) / 16);
+    uint8_t* base = static_cast<uint8_t*>(pools.ptr[rest / pieces]);
+    const uint4* from = reinterpret_cast<const uint4*>(base + src * j.page_bytes + begin) + threadIdx.x;
+    uint4* to = reinterpret_cast<uint4*>(base + dst * j.page_bytes + begin) + threadIdx.x;
+    const int words = static_cast<int>(min(piece_bytes, bytes - begin) / 16) - threadIdx.x;
     uint4 v[kCopyUnroll];
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u) {
-      const int w = threadIdx.x + u * kCopyThreads;
-      if (w < words) v[u] = from[w];
-    }
+    for (int u = 0; u < kCopyUnroll; ++u)
+      if (u * kCopyThreads < words) v[u] = from[u * kCopyThreads];
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u) {
-      const int w = threadIdx.x + u * kCopyThreads;
-      if (w < words) to[w] = v[u];
-    }
+    for (int u = 0; u < kCopyUnroll; ++u)
+      if (u * kCopyThreads < words) to[u * kCopyThreads] = v[u];
   }
 }
 
@@ -95,7 +94,7 @@ cudaError_t launch_copy(const CopyJobs<Id>& j, void* const* pools, int64_t num_p
     const int64_t tasks = j.count * args.count * pieces;
     if (tasks == 0) continue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tasks, kNumSMs * 8)));
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tasks, kNumSMs * kCopyPerSm)));
     cfg.blockDim = dim3(kCopyThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -171,6 +170,7 @@ __device__ __forceinline__ int64_t pages_of(int64_t len, int64_t block_size) {
 }
 
 struct ForkWork {
+  int64_t* len;                               // [count]: a child's length, -1 if it cannot be made
   int32_t *fresh, *rank, *src, *dst, *rows;  // [count] each
 };
 
@@ -200,6 +200,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   }
   for (int64_t i = kids.begin; i < kids.end; ++i) {
     const int64_t n = length(i);
+    w.len[i] = n;
     mine += n > 0 && n % bs ? 1 : 0;
   }
   uint64_t total, before, all;
@@ -215,7 +216,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   for (int64_t id = ids.begin; id < ids.end && f < count; ++id)
     if (s.refs[id] == 0) w.fresh[f++] = static_cast<int32_t>(id);
   for (int64_t i = kids.begin; i < kids.end; ++i) {
-    const int64_t n = length(i);
+    const int64_t n = w.len[i];  // this thread's own
     w.rank[i] = static_cast<int32_t>(k);
     k += n > 0 && n % bs ? 1 : 0;
   }
@@ -225,11 +226,15 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   const int lane = threadIdx.x & 31;
   const int64_t warps = kPlanCtas * (kPlanThreads / 32);
   for (int64_t i = static_cast<int64_t>(rank) * (kPlanThreads / 32) + (threadIdx.x >> 5); i < count; i += warps) {
-    int64_t n = length(i);
+    int64_t n = w.len[i];
+    const int64_t parent = parents[i];
+    const int32_t place = w.rank[i];
     const bool tail = n > 0 && n % bs;
-    if (tail && w.rank[i] >= num_free) n = -1;
+    if (tail && place >= num_free) n = -1;
     const int64_t full = n > 0 ? n / bs : 0;
-    const int32_t* from = s.table + (n >= 0 ? parents[i] : 0) * s.cols;
+    const int32_t* from = s.table + (n >= 0 ? parent : 0) * s.cols;
+    const bool job = tail && n > 0;
+    const int32_t page = job ? w.fresh[place] : 0;
     for (int64_t c = lane; c < s.cols; c += 32) {
       int32_t id = -1;
       if (c < full) {
@@ -239,16 +244,15 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
         else
           atomicOr(&g_cascade_device_error, kErrBadBlockId);
       } else if (c == full && tail && n > 0) {
-        id = w.fresh[w.rank[i]];
+        id = page;
         s.refs_out[id] = 1;
       }
       s.table_out[i * s.cols + c] = id;
     }
     if (lane == 0) {
-      const bool job = tail && n > 0;
       s.lens_out[i] = n;
       w.src[i] = job ? from[full] : 0;
-      w.dst[i] = job ? w.fresh[w.rank[i]] : 0;
+      w.dst[i] = page;
       w.rows[i] = job ? static_cast<int32_t>(n % bs) : 0;
     }
   }
@@ -357,12 +361,15 @@ cudaError_t launch_page_copy(void* const* pools, int64_t num_pools, int64_t num_
   return launch_copy(j, pools, num_pools, false, stream);
 }
 
-size_t page_fork_workspace(int64_t, int64_t count) { return static_cast<size_t>(count) * 5 * sizeof(int32_t); }
+size_t page_fork_workspace(int64_t, int64_t count) {
+  return static_cast<size_t>(count) * (sizeof(int64_t) + 5 * sizeof(int32_t));
+}
 
 cudaError_t launch_page_fork(const PageState& s, void* const* pools, int64_t num_pools, int64_t row_bytes,
                              const int64_t* parents, int64_t count, void* workspace, cudaStream_t stream) {
-  int32_t* w = static_cast<int32_t*>(workspace);
-  const ForkWork work = {w, w + count, w + 2 * count, w + 3 * count, w + 4 * count};
+  int64_t* len = static_cast<int64_t*>(workspace);
+  int32_t* w = reinterpret_cast<int32_t*>(len + count);
+  const ForkWork work = {len, w, w + count, w + 2 * count, w + 3 * count, w + 4 * count};
   fork_plan_kernel<<<kPlanCtas, kPlanThreads, 0, stream>>>(s, parents, count, work);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;

@@ -24,7 +24,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kPerSm = 4;    // CTAs resident per SM (64 registers): 24 loads in flight per thread, 96 KB per SM
 constexpr int kUnroll = 8;
 constexpr int kMaxCtas = 8;  // CTAs per request
 
@@ -45,7 +46,7 @@ __device__ __forceinline__ uint64_t make_key(float quotient, uint32_t v) {
 __device__ __forceinline__ uint64_t max_u64(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 template <int kType>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyLaunch p) {
+__global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const VerifyLaunch p) {
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks());
   const int rank = static_cast<int>(cluster.block_rank());
@@ -82,33 +83,56 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyLaunch p) 
   __syncthreads();
   const int64_t taken = s_taken;
   const bool refused = taken < n;
-  const int64_t prow = (b * (K + 1) + taken) * V, qrow = (b * K + taken) * V, erow = b * V;
+  // the three rows; the entries are walked with 32-bit indices
+  const int element = kType == 2 ? 4 : 2, n_v = static_cast<int>(V);
+  const void* prow = static_cast<const char*>(p.target) + (b * (K + 1) + taken) * V * element;
+  const void* qrow = refused && p.draft ? static_cast<const char*>(p.draft) + (b * K + taken) * V * element : nullptr;
+  const float* erow = p.noise + b * V;
   const int64_t out = refused && !p.draft ? p.tokens[b * K + taken] : -1;  // the token left out
 
   // the best entry of this cluster's row: pass 0 over `left`; pass 1, only
   // when left is 0 everywhere, over the target's row
   uint64_t best = 0;
   for (int pass = 0; pass < 2; ++pass) {
-    const bool minus = pass == 0 && refused && p.draft;
-    const int64_t stride = static_cast<int64_t>(ctas) * kThreads;
-    for (int64_t v0 = static_cast<int64_t>(rank) * kThreads + threadIdx.x; v0 < V; v0 += stride * kUnroll) {
+    const bool minus = pass == 0 && qrow;
+    const int skip = pass == 0 ? static_cast<int>(out) : -1;
+    const int stride = ctas * kThreads, block = stride * kUnroll;
+    int v0 = rank * kThreads + static_cast<int>(threadIdx.x);
+    // `best` as (quotient, index): the thread meets its indices in ascending order, so a later one has to be larger
+    float top = -1.f;
+    int at = 0;
+    auto take = [&](float t, float q, float e, int v) {
+      const float left = __fsub_rn(t, q);
+      if (left > 0.f && v != skip) {
+        const float quotient = __fdiv_rn(left, e);
+        if (quotient > top) top = quotient, at = v;
+      }
+    };
+    for (; v0 + (kUnroll - 1) * stride < n_v; v0 += block) {
       float t[kUnroll], q[kUnroll], e[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        const int64_t v = v0 + u * stride;
-        const bool in = v < V;
-        t[u] = in ? load<kType>(p.target, prow + v) : 0.f;
-        q[u] = in && minus ? load<kType>(p.draft, qrow + v) : 0.f;
-        e[u] = in ? __ldg(p.noise + erow + v) : 1.f;
+        t[u] = load<kType>(prow, v0 + u * stride);
+        e[u] = __ldg(erow + v0 + u * stride);
+        q[u] = minus ? load<kType>(qrow, v0 + u * stride) : 0.f;
       }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int64_t v = v0 + u * stride;
-        const float left = __fsub_rn(t[u], q[u]);
-        if (left > 0.f && !(pass == 0 && v == out))
-          best = max_u64(best, make_key(__fdiv_rn(left, e[u]), static_cast<uint32_t>(v)));
-      }
+      for (int u = 0; u < kUnroll; ++u) take(t[u], q[u], e[u], v0 + u * stride);
     }
+    {
+      float t[kUnroll - 1], q[kUnroll - 1], e[kUnroll - 1];
+#pragma unroll
+      for (int u = 0; u < kUnroll - 1; ++u) {
+        const int v = v0 + u * stride;
+        const bool in = v < n_v;
+        t[u] = in ? load<kType>(prow, v) : 0.f;
+        e[u] = in ? __ldg(erow + v) : 1.f;
+        q[u] = in && minus ? load<kType>(qrow, v) : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll - 1; ++u) take(t[u], q[u], e[u], v0 + u * stride);
+    }
+    best = top >= 0.f ? make_key(top, static_cast<uint32_t>(at)) : 0;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, d));
     if (lane == 0) s_best[warp] = best;
@@ -138,10 +162,11 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const VerifyLaunch p) 
 }  // namespace
 
 cudaError_t launch_verify_drafts(const VerifyLaunch& p, cudaStream_t stream) {
-  // as many CTAs per request as give the GPU two waves of two per SM, at
-  // least one unrolled round of the row each
+  // as many CTAs per request as run at once, with at least one unrolled round
+  // of the row each
   int ctas = 1;
-  while (ctas < kMaxCtas && p.batch * ctas < 4 * kNumSMs && p.vocab > static_cast<int64_t>(ctas) * kThreads * kUnroll)
+  while (ctas < kMaxCtas && p.batch * ctas * 2 <= kPerSm * kNumSMs &&
+         p.vocab > static_cast<int64_t>(ctas) * kThreads * kUnroll)
     ctas *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.batch * ctas));
