@@ -28,10 +28,8 @@
 // Softmax: running maximum m in the log2 domain that moves only when a score
 // exceeds it by more than 2^8 (the exponentials stay below 256, exact in
 // relative terms in both types), so the accumulator is rescaled rarely. P is
-// rounded to the inputs' type, which the second product needs. Two row sums in
-// fp32: of the exponentials, for the log-sum-exp, and of the rounded P, by
-// which the output is divided: what rounding adds to all weights of a row
-// alike then cancels (a row that sees one token returns it exactly).
+// rounded to the inputs' type, which the second product needs; the row's sum is
+// of the unrounded exponentials, in fp32.
 //
 // Work: the 64-row tiles of all (request, row tile) units, concatenated, are
 // cut into one equal run per cluster, computed on the device from the lengths.
@@ -79,6 +77,7 @@ struct Sched {
   int64_t tiles, begin;  // all tiles; this cluster's first
   int64_t tok;           // first query token of request b
   int b, mt, t0, left;
+  int q, kv;               // request b's lengths
 };
 
 struct __align__(16) Aux {
@@ -119,15 +118,6 @@ struct Params {
   float* part_o;           // [2 clusters][128][512]
   float* part_lse;         // [2 clusters][128]
 };
-
-template <bool kFp16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if constexpr (kFp16) {
-    return __half22float2(*reinterpret_cast<__half2*>(&v));
-  } else {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  }
-}
 
 // row_info of a unit cut into `count` >= 2 pieces, the first in run `c`: row r
 // of the slots 2c + 1 (first piece), 2 (c + 1), 2 (c + 2), ...
@@ -172,9 +162,7 @@ struct Walk {
   int64_t next_tok;
 
   __device__ Walk(const LatentDecodeLaunch& l, const Sched& s)
-      : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), left(s.left), next_tok(s.tok) {
-    if (left > 0) load();
-  }
+      : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), left(s.left), nq(s.q), nkv(s.kv), next_tok(s.tok) {}
   __device__ __forceinline__ void load() {
     nq = u.q_len(next_b);
     nkv = u.kv_len(next_b);
@@ -245,7 +233,7 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
         for (int mt = 0; mt < m; ++mt) {
           const int t = u.tiles(q, kv, mt);
           if (begin < at + t) {
-            aux->sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin)};
+            aux->sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin), q, kv};
             b = b1;
             break;
           }
@@ -288,6 +276,18 @@ struct PageRows {
   }
 };
 
+// Four groups of 64 dims of kR cache rows, each group kGroup bytes apart: at once
+// when a page gives all 32 rows, group by group when two pages share them.
+template <int kR>
+__device__ __forceinline__ void load_groups(uint8_t* dst, const Params& P, uint64_t* bar, int row, int group) {
+  if constexpr (kR == kHalfTok) {
+    tma_load_3d(dst, &P.map4, bar, 0, row, group);
+  } else {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) tma_load_3d(dst + g * kGroup, &P.map1, bar, 0, row, group + g);
+  }
+}
+
 template <bool kFp16, int kR>
 __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid_constant__ Params P) {
   pdl_launch_dependents();
@@ -319,10 +319,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     tmem_alloc(&aux->tmem_base, 512);
     tmem_relinquish();
   }
-  find_run(p, cluster, clusters, aux);
   tc_fence_before();
-  cluster_sync_all();  // both CTAs' barriers are initialised
+  find_run(p, cluster, clusters, aux);  // (with CTA barriers)
   tc_fence_after();
+  // Both CTAs' barriers are initialised once this barrier is passed; only the roles that reach into the other CTA
+  // wait for it first, the loads start before.
+  cluster_arrive();
+  const bool remote = warp < 8 || warp == 13;
+  if (remote) cluster_wait();
   const uint32_t tbase = aux->tmem_base;
   Walk w(p, aux->sched);
 
@@ -352,11 +356,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           if (tail) mbar_arrive(&aux->p_full[it & 1]);
 #pragma unroll
           for (int i = 0; i < PageRows<kR>::kPer; ++i) {
+            const int at = i * kR * 128;  // 32 rows per group, from one page or two
             if (keys) {
-              tma_load_3d(dsta + i * kR * 512, &P.map4, full, 0, y[i], 4 * (1 - c));
-              tma_load_3d(dsta + 4 * kGroup + i * kR * 128, &P.map1, full, 0, y[i], 8);
+              load_groups<kR>(dsta + at, P, full, y[i], 4 * (1 - c));
+              tma_load_3d(dsta + 4 * kGroup + at, &P.map1, full, 0, y[i], 8);
             }
-            tma_load_3d(dst + i * kR * 512, &P.map4, full, 0, y[i], 4 * c);
+            load_groups<kR>(dst + at, P, full, y[i], 4 * c);
           }
         }
         __syncwarp();
@@ -366,8 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // ----------------------------------------------------------- MMA issuer
     // the whole warp walks and waits; one elected lane issues. Scores run two
     // tiles ahead of P V, within a piece.
-    constexpr int kPer = kHalfTok / kR;
-    const uint32_t idesc_s = make_idesc_f16(kRows, kR, kFp16 ? 0u : 1u, 0, 0);
+    const uint32_t idesc_s = make_idesc_f16(kRows, kHalfTok, kFp16 ? 0u : 1u, 0, 0);
     const uint32_t idesc_pv = make_idesc_f16(kRows, 256, kFp16 ? 0u : 1u, 0, 1);
     const uint32_t tm = uniform(tbase), rank = uniform(static_cast<uint32_t>(c)), s0 = uniform(smem_u32(smem));
     const uint64_t dq = make_smem_desc(s0 + kOffQ, 16, 1024, 2);
@@ -384,18 +388,13 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       if (elect_one()) {
 #pragma unroll
         for (int g = 0; g < 9; ++g) {
+          const uint64_t k0 = (g < 4 ? db + g * kGroup / 16 : da + (g - 4) * kGroup / 16);
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const uint64_t k0 = g < 4   ? db + (i * 4 + g) * kR * 8
-                                : g < 8 ? da + (i * 4 + g - 4) * kR * 8
-                                        : da + (4 * kGroup) / 16 + i * kR * 8;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (g < kQTmem)
-                umma_f16_ts(d + i * kR, tm + kColQ + g * 32 + k * 8, k0 + k * 2, idesc_s, g + k > 0);
-              else
-                umma_f16_ss(d + i * kR, dq + ((g - kQTmem) * kQGroup + k * 32) / 16, k0 + k * 2, idesc_s, 1u);
-            }
+          for (int k = 0; k < 4; ++k) {
+            if (g < kQTmem)
+              umma_f16_ts(d, tm + kColQ + g * 32 + k * 8, k0 + k * 2, idesc_s, g + k > 0);
+            else
+              umma_f16_ss(d, dq + ((g - kQTmem) * kQGroup + k * 32) / 16, k0 + k * 2, idesc_s, 1u);
           }
         }
         umma_commit(&aux->s_full[sa]);
@@ -411,18 +410,18 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         return false;
       tc_fence_after();
       const uint32_t own = s0 + kOffB + sb * kBytesV, other = s0 + kOffC + sc * kBytesV;
-      // P: rows of 32 bytes, 32-byte swizzle; V: 64-column groups kR * 128 bytes apart
+      // P: rows of 32 bytes, 32-byte swizzle; V: 64-column groups kGroup bytes apart
       const uint64_t dp = make_smem_desc(s0 + kOffP + pb * 4 * kPPart, 16, 256, 6);
-      const uint64_t dv0 = make_smem_desc(rank == 0 ? own : other, kR * 128, 1024, 2);
-      const uint64_t dv1 = make_smem_desc(rank == 0 ? other : own, kR * 128, 1024, 2);
+      const uint64_t dv0 = make_smem_desc(rank == 0 ? own : other, kGroup, 1024, 2);
+      const uint64_t dv1 = make_smem_desc(rank == 0 ? other : own, kGroup, 1024, 2);
       __syncwarp();
       if (elect_one()) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k)  // the second 16 cache rows follow at once (32-row boxes) or as the next box
+          for (int k = 0; k < 2; ++k)
             umma_f16_ss(tm + kColO, dp + (h * 2 + k) * kPPart / 16,
-                        (h ? dv1 : dv0) + (kR == 32 ? k * 2048 : k * 4 * kR * 128) / 16, idesc_pv, !first || h + k > 0);
+                        (h ? dv1 : dv0) + k * 2048 / 16, idesc_pv, !first || h + k > 0);
         }
         umma_commit_cluster(&aux->pv_done[sb], 3);
         if (last) umma_commit(&aux->o_full);
@@ -485,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       const int lim = w.u.limit(w.q, w.kv, min(row / p.num_heads, w.q - 1));
       // tiles below this one are seen in full by every row (the first row sees the least)
       const int clean = w.u.limit(w.q, w.kv, w.mt * kRows / p.num_heads) / kTok;
-      float m = -INFINITY, l = 0.f, lp = 0.f;
+      float m = -INFINITY, l = 0.f;
       float s[16], s_next[16];
       // scores of a tile from TMEM, masked, and their maximum on its way
       auto fetch = [&](int i, int t, float (&x)[16]) {
@@ -528,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         const float dm = move ? ex2(m - mx) : 1.f;  // 0 while nothing has been seen
         if (move) m = mx;
         const float neg = m == -INFINITY ? 0.f : -m;
-        float r0 = 0.f, r1 = 0.f, p0 = 0.f, p1 = 0.f;
+        float r0 = 0.f, r1 = 0.f;
         uint32_t pk[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
@@ -537,11 +536,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           y0 = ex2(y0), y1 = ex2(y1);
           fadd2(r0, r1, y0, y1);
           pk[e >> 1] = pack2<kFp16>(y0, y1);
-          const float2 rounded = unpack2<kFp16>(pk[e >> 1]);
-          fadd2(p0, p1, rounded.x, rounded.y);
         }
         l = l * dm + (r0 + r1);
-        lp = lp * dm + (p0 + p1);
         if (j > 0 && __any_sync(0xffffffffu, move)) {
           live = mbar_wait_warp(&aux->pv_done[(it - 1) & 3], ((it - 1) >> 2) & 1);  // O holds every tile before this one
           if (!live) break;
@@ -574,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           if (!live) break;
           if (t * kTok + hh * kHalfTok + lane >= valid) {
             uint8_t* stage = smem + (hh == c ? kOffB + it % kStagesB * kBytesV : kOffC + it % kStagesC * kBytesV);
-            uint4* v = reinterpret_cast<uint4*>(stage + ((lane / kR) * 4 + (warp & 3)) * kR * 128 + (lane % kR) * 128);
+            uint4* v = reinterpret_cast<uint4*>(stage + (warp & 3) * kGroup + lane * 128);
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = make_uint4(0u, 0u, 0u, 0u);
           }
@@ -594,20 +590,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         for (int e = 0; e < 16; ++e) s[e] = s_next[e];
       }
       if (!live) break;
-      // the row's sums over the four threads, added in one order by all
+      // the row's sum over the four threads, added in one order by all
       float of[4];
       tell(l);
       live = hear(of);
       if (!live) break;
       l = (of[0] + of[1]) + (of[2] + of[3]);
-      tell(lp);
-      live = hear(of);
-      if (!live) break;
-      lp = (of[0] + of[1]) + (of[2] + of[3]);
       if (hh == 0) {
         live = pieces == 0 || mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1);  // the last one has been read
         if (!live) break;
-        aux->inv[r] = lp > 0.f ? 1.f / lp : 0.f;
+        aux->inv[r] = l > 0.f ? 1.f / l : 0.f;
         mbar_arrive(&aux->stat_full);
       }
       const int64_t grow = w.tok * p.num_heads + row;
@@ -651,6 +643,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       tma_load_3d(smem + kOffQ + g % 3 * kQGroup, &P.map_q, &aux->qs_full[g % 3], 0,
                   static_cast<int>(x.tok * p.num_heads + x.mt * kRows), col);
     };
+    auto prefetch_q = [&](const Walk& x) {
+      if (tid == 256)
+        for (int g = 0; g < 9; ++g)
+          tma_prefetch_3d(&P.map_q, 0, static_cast<int>(x.tok * p.num_heads + x.mt * kRows), g);
+    };
     auto place_q = [&](const Walk& x, int piece) -> bool {
       if (tid == 256)
         for (int g = 0; g < 3; ++g) load_group(x, g);
@@ -682,15 +679,17 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       mbar_arrive(&aux->q_full);
       return true;
     };
-    auto store_o = [&](const Walk& x, int piece) -> bool {
+    auto store_o = [&](const Walk& x, int piece, bool end_of_run) -> bool {
       if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
       tc_fence_after();
       const float inv = aux->inv[r];
       const bool whole = x.starts && x.ends;
       const int64_t slot = 2 * cluster + (x.starts ? 1 : 0);
-      // 32 bytes per row at a time through shared memory, so that a store instruction writes whole
-      // sectors of 16 rows (16-byte half h of row r at h ^ (r / 4 % 2): no bank conflicts)
+      // Through shared memory, so that a store instruction writes whole sectors: 32 bytes per row at a time
+      // (16-byte half h of row r at h ^ (r / 4 % 2): no bank conflicts), and 128 (chunk q at q ^ (r % 8)) at the end
+      // of the run, when the query slots are free.
       uint8_t* stage = smem + kOffE + (warp & 3) * 1024;
+      uint8_t* wide = smem + kOffQ + (warp & 3) * 4096;
       const int row0 = x.mt * kRows + (r & ~31);  // this warp's first row of the unit
       const int rows = min(32, static_cast<int>(min(static_cast<int64_t>(x.q) * p.num_heads - row0,
                                                     all_rows - (x.tok * p.num_heads + row0))));
@@ -711,6 +710,19 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         }
         __syncwarp();
       };
+      auto put_wide = [&](int chunk, uint4 a) {
+        *reinterpret_cast<uint4*>(wide + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = a;
+      };
+      auto flush_wide = [&](int line) {
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int rr = q * 4 + (lane >> 3);
+          const uint4 v = *reinterpret_cast<const uint4*>(wide + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+          if (rr < rows) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(rr) * pitch + line * 128 + (lane & 7) * 16) = v;
+        }
+        __syncwarp();
+      };
 #pragma unroll 1
       for (int g = 0; g < 8; ++g) {
         uint32_t o[32];
@@ -728,15 +740,27 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             return make_uint4(pack2<kFp16>(f[e], f[e + 1]), pack2<kFp16>(f[e + 2], f[e + 3]),
                               pack2<kFp16>(f[e + 4], f[e + 5]), pack2<kFp16>(f[e + 6], f[e + 7]));
           };
-          put(g * 2, four(0), four(8));
-          put(g * 2 + 1, four(16), four(24));
+          if (end_of_run) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) put_wide((g & 1) * 4 + q, four(8 * q));
+            if (g & 1) flush_wide(g >> 1);
+          } else {
+            put(g * 2, four(0), four(8));
+            put(g * 2 + 1, four(16), four(24));
+          }
         } else {
           auto four = [&](int e) {
             return make_uint4(__float_as_uint(f[e]), __float_as_uint(f[e + 1]), __float_as_uint(f[e + 2]),
                               __float_as_uint(f[e + 3]));
           };
+          if (end_of_run) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) put(g * 4 + q, four(8 * q), four(8 * q + 4));
+            for (int q = 0; q < 8; ++q) put_wide(q, four(4 * q));
+            flush_wide(g);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) put(g * 4 + q, four(8 * q), four(8 * q + 4));
+          }
         }
       }
       return true;
@@ -744,22 +768,26 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // the next piece's query goes in as soon as the last scores of this one are
     // computed, before this one's epilogue
     bool more = w.next();
+    if (more) prefetch_q(w);
     bool live = !more || place_q(w, 0);
     int piece = 0;
     while (live && more) {
       const Walk now = w;
       more = w.next();
       if (more) {
+        prefetch_q(w);
         live = mbar_wait_warp(&aux->q_empty, piece & 1);
         if (!live) break;
         tc_fence_after();
         live = place_q(w, piece + 1);
         if (!live) break;
       }
-      live = store_o(now, piece);
+      live = store_o(now, piece, !more);
       ++piece;
     }
   }
+  __syncwarp();
+  if (!remote) cluster_wait();
   if (cta_aborted()) {
     // loads into this CTA and copies into the other one may be in flight (a few hundred KB): they get a millisecond,
     // hundreds of times what they take, before either CTA leaves
@@ -788,25 +816,46 @@ __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_consta
   // rows of a call whose query lengths do not add up hold no info: nothing past the slots is read for them
   if (count < 2 || c0 + count > clusters) return;
   auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRows + r; };
-  float top = -INFINITY;
-  for (int i = lane; i < count; i += 32) top = fmaxf(top, P.part_lse[slot(i)]);
+  // the first 32 pieces' weights, one per lane
+  const float mine = lane < count ? P.part_lse[slot(lane)] : -INFINITY;
+  float top = mine;
+  for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, P.part_lse[slot(i)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   float4 acc[4] = {};
   float sum = 0.f;
-  for (int i = 0; i < count; ++i) {
-    const float lse = P.part_lse[slot(i)];
-    const float wgt = top == -INFINITY ? 0.f : __expf(lse - top);
+  auto weight = [&](int i) {
+    const float lse = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : P.part_lse[slot(i)];
+    return top == -INFINITY ? 0.f : __expf(lse - top);
+  };
+  auto read = [&](int i, float4 (&v)[4]) {
     const float4* src = reinterpret_cast<const float4*>(P.part_o + slot(i) * kLatentDim);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = src[lane + 32 * k];
+  };
+  auto add = [&](float wgt, const float4 (&v)[4]) {
     sum += wgt;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float4 v = src[lane + 32 * k];
-      acc[k].x = fmaf(wgt, v.x, acc[k].x);
-      acc[k].y = fmaf(wgt, v.y, acc[k].y);
-      acc[k].z = fmaf(wgt, v.z, acc[k].z);
-      acc[k].w = fmaf(wgt, v.w, acc[k].w);
+      acc[k].x = fmaf(wgt, v[k].x, acc[k].x);
+      acc[k].y = fmaf(wgt, v[k].y, acc[k].y);
+      acc[k].z = fmaf(wgt, v[k].z, acc[k].z);
+      acc[k].w = fmaf(wgt, v[k].w, acc[k].w);
     }
+  };
+  // two pieces' loads in flight (most rows have two or three)
+  int i = 0;
+  for (; i + 1 < count; i += 2) {
+    float4 a[4], b[4];
+    read(i, a);
+    read(i + 1, b);
+    add(weight(i), a);
+    add(weight(i + 1), b);
+  }
+  if (i < count) {
+    float4 a[4];
+    read(i, a);
+    add(weight(i), a);
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.L.out) + row * kLatentDim);

@@ -462,6 +462,10 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// the two halves of cluster_sync_all
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 // 16-byte store into the shared memory of a CTA of this cluster
 // (`cluster_addr` from mapa_shared); ordered before the reads of that CTA by
 // a cluster barrier (release / acquire) between them.
