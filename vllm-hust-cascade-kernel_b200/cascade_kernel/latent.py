@@ -1,0 +1,84 @@
+"""A paged latent cache and the steps that serve from it.
+
+``LatentCache`` keeps what the page operators read and write: one pool per
+layer ``[blocks, page, 576]`` (512 latent values and 64 rotary key values per
+token), a block table, the rows' lengths and the pages' reference counts. The
+operators return the new table, lengths and counts; the cache swaps them in.
+Attention over it is ``torch.ops.npu.cascade_latent_decode`` (absorbed form);
+prompts attend in the expanded form, ``torch.ops.npu.cascade_latent_prefill``,
+and drafted tokens are checked by ``torch.ops.npu.cascade_verify_drafts``.
+"""
+import torch
+
+LATENT, ROPE = 512, 64
+
+
+class LatentCache:
+    """Rows (sequences) over shared pages; every method keeps to the device."""
+
+    def __init__(self, layers, blocks, page, rows, cols, dtype=torch.bfloat16, device="cuda"):
+        self.page = page
+        self.pools = [torch.zeros((blocks, page, LATENT + ROPE), dtype=dtype, device=device) for _ in range(layers)]
+        self.table = torch.full((rows, cols), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(rows, dtype=torch.int64, device=device)
+        self.refs = torch.zeros(blocks, dtype=torch.int32, device=device)
+
+    def grow(self, tokens):
+        """Gives every row the pages for ``tokens`` (int64 [rows]) more tokens, free ones in ascending order, and
+        lengthens it. A partly filled last page is the row's own (``fork`` copies it), so it is filled in place.
+        Raises if the pages or the table's columns run out."""
+        have, want = (self.lens + self.page - 1) // self.page, (self.lens + tokens + self.page - 1) // self.page
+        col = torch.arange(self.table.shape[1], device=self.table.device)
+        new = (col >= have[:, None]) & (col < want[:, None])
+        free = torch.nonzero(self.refs == 0).squeeze(1).to(torch.int32)
+        need = int((want - have).sum())
+        if need > free.numel() or int(want.max()) > self.table.shape[1]:
+            raise RuntimeError(f"LatentCache: {need} pages needed, {free.numel()} free, {self.table.shape[1]} columns")
+        self.table[new] = free[:need]
+        self.refs[free[:need].long()] = 1
+        self.lens = self.lens + tokens
+
+    def write(self, layer, latents, counts):
+        """Stores ``latents`` [sum(counts), 576] as the last ``counts`` (host list) tokens of the rows."""
+        rows = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts)).to(self.table.device)
+        back = torch.cat([torch.arange(n, 0, -1) for n in counts]).to(self.table.device)
+        at = self.lens[rows] - back
+        page = self.table[rows, at // self.page].long()
+        self.pools[layer][page, at % self.page] = latents
+
+    def attend(self, layer, query, q_len, scale, rows=None):
+        """The last ``q_len`` tokens of every row (their queries [rows * q_len, heads, 576]) over the row's cache."""
+        table, lens = (self.table, self.lens) if rows is None else (self.table[rows].contiguous(), self.lens[rows])
+        ones = torch.full_like(lens, q_len)
+        return torch.ops.npu.cascade_latent_decode(query, self.pools[layer], table, ones, lens, q_len, scale, True)
+
+    def attend_shared(self, layer, query, prefix_table, prefix_lens, scale, own_from):
+        """One token per row whose first ``own_from`` tokens (whole pages) are one prefix shared by all rows: the prefix
+        is read once for the batch, each row's rest by itself, and the two are merged."""
+        B = query.shape[0]
+        skip = own_from // self.page
+        if own_from % self.page:
+            raise ValueError("attend_shared: the shared prefix must be whole pages")
+        qs = torch.full_like(prefix_lens, B)
+        o1, l1 = torch.ops.npu.cascade_latent_decode(query, self.pools[layer], prefix_table, qs, prefix_lens, B, scale, False)
+        rest = self.table[:, skip:].contiguous()
+        ones = torch.ones_like(self.lens)
+        o2, l2 = torch.ops.npu.cascade_latent_decode(query, self.pools[layer], rest, ones, self.lens - own_from, 1, scale, True)
+        code = {torch.bfloat16: 1, torch.float16: 3}[query.dtype]
+        return torch.ops.npu.cascade_lse_merge(o1, o2, l1, l2, code)
+
+    def fork(self, parents):
+        """The rows become copies of rows ``parents`` (int64): shared full pages, an own copy of a partly filled last
+        one. The old rows give their pages back afterwards."""
+        child, lens, refs = torch.ops.npu.cascade_page_fork(self.pools, self.table, self.lens, self.refs, parents)
+        _, _, refs = torch.ops.npu.cascade_page_free(self.table, self.lens, refs, torch.zeros_like(self.lens), self.page)
+        self.table, self.lens, self.refs = child, lens, refs
+
+    def truncate(self, keep):
+        """Cuts the rows to ``keep`` tokens (int64 [rows]) and frees the pages past them."""
+        self.table, self.lens, self.refs = torch.ops.npu.cascade_page_free(self.table, self.lens, self.refs, keep, self.page)
+
+    def compact(self):
+        """Moves the live pages to the front of the pools; returns their number (int32 [1], on the device)."""
+        self.table, self.refs, live = torch.ops.npu.cascade_page_compact(self.pools, self.table, self.lens, self.refs)
+        return live
