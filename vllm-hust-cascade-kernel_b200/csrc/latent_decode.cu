@@ -224,7 +224,12 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
   }
   const int64_t runs = min(static_cast<int64_t>(clusters), total);
   if (cluster < runs) {
-    const int64_t begin = cluster * total / runs, end = (cluster + 1) * total / runs;
+    // floor(cluster total / runs) and floor((cluster + 1) total / runs), with one wide division
+    const int n_runs = static_cast<int>(runs);
+    const int64_t each = total >> 31 ? total / runs : static_cast<uint32_t>(total) / static_cast<uint32_t>(n_runs);
+    const int rest = static_cast<int>(total - each * runs);
+    const int64_t begin = cluster * each + cluster * rest / n_runs;
+    const int64_t end = (cluster + 1) * each + (cluster + 1) * rest / n_runs;
     int64_t at = st - tiles;
     if (begin >= at && begin < st) {
       int64_t tok = sq - toks;
@@ -276,6 +281,75 @@ struct PageRows {
   }
 };
 
+// Writes columns [32 g0, 32 g1) of the CTA's 256 of a piece's output, 32 rows per
+// warp: divided by the sums to `out` when the piece is its whole unit, else as
+// an fp32 partial. They go through shared memory, so that a store instruction
+// writes whole sectors: kWide, 128 bytes per row at a time (4 KB of `stage`,
+// 16-byte chunk q of row r at q ^ (r % 8)), else 32 (1 KB, half h at
+// h ^ (r / 4 % 2)); no bank conflicts either way. `released` (if given) gets an
+// arrival per thread once the accumulator has been read.
+template <bool kFp16, bool kWide>
+__device__ __forceinline__ void write_rows(const Params& P, const Walk& x, int cluster, int c, float inv, uint32_t tmem,
+                                           uint8_t* stage, int g0, int g1, uint64_t* released) {
+  const LatentDecodeLaunch& p = P.L;
+  const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
+  const bool whole = x.starts && x.ends;
+  const int row0 = x.mt * kRows + quarter * 32;  // this warp's first row of the unit
+  const int64_t grow0 = x.tok * p.num_heads + row0;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(32), min(static_cast<int64_t>(x.q) * p.num_heads - row0,
+                                                                      p.num_tokens * p.num_heads - grow0)));
+  const int64_t slot = 2 * cluster + (x.starts ? 1 : 0);
+  uint8_t* dst = whole ? static_cast<uint8_t*>(p.out) + grow0 * (kLatentDim * 2) + 512 * c
+                       : reinterpret_cast<uint8_t*>(P.part_o) + (slot * kRows + quarter * 32) * (kLatentDim * 4) + 1024 * c;
+  const int pitch = whole ? kLatentDim * 2 : kLatentDim * 4;
+  constexpr int kPerRow = kWide ? 8 : 2;  // 16-byte chunks staged per row
+  auto place = [&](int chunk) -> uint4* {
+    const int swap = kWide ? lane & 7 : (lane >> 2) & 1;
+    return reinterpret_cast<uint4*>(stage + lane * (kPerRow * 16) + ((chunk ^ swap) << 4));
+  };
+  auto flush = [&](int part) {
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < kPerRow; ++q) {
+      const int rr = q * (32 / kPerRow) + lane / kPerRow, chunk = lane % kPerRow;
+      const int swap = kWide ? rr & 7 : (rr >> 2) & 1;
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * (kPerRow * 16) + ((chunk ^ swap) << 4));
+      if (rr < rows)
+        *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(rr) * pitch + part * (kPerRow * 16) + chunk * 16) = v;
+    }
+    __syncwarp();
+  };
+#pragma unroll 1
+  for (int g = g0; g < g1; ++g) {
+    uint32_t o[32];
+    tmem_ld_32x32b_x32(tmem + kColO + g * 32, o);
+    tmem_wait_ld();
+    if (released && g + 1 == g1) {
+      tc_fence_before();
+      mbar_arrive(released);
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = inv > 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+    if (whole) {  // 64 bytes per row
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        auto two = [&](int e) { return pack2<kFp16>(__uint_as_float(o[e]), __uint_as_float(o[e + 1])); };
+        const int e = q * 8;
+        *place(kWide ? (g & 1) * 4 + q : q & 1) = make_uint4(two(e), two(e + 2), two(e + 4), two(e + 6));
+        if (!kWide && (q & 1)) flush(g * 2 + (q >> 1));
+      }
+      if (kWide && (g & 1)) flush(g >> 1);
+    } else {  // 128 bytes per row
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        *place(kWide ? q : q & 1) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        if (!kWide && (q & 1)) flush(g * 4 + (q >> 1));
+      }
+      if (kWide) flush(g);
+    }
+  }
+}
+
 // Four groups of 64 dims of kR cache rows, each group kGroup bytes apart: at once
 // when a page gives all 32 rows, group by group when two pages share them.
 template <int kR>
@@ -314,6 +388,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
+  }
+  if (tid == 32) {
+    tma_prefetch_desc(&P.map_q);
+    tma_prefetch_desc(&P.map4);
+    tma_prefetch_desc(&P.map1);
   }
   if (warp == 13) {
     tmem_alloc(&aux->tmem_base, 512);
@@ -596,10 +675,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       live = hear(of);
       if (!live) break;
       l = (of[0] + of[1]) + (of[2] + of[3]);
-      if (hh == 0) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const bool last = w.left <= 0;  // of the run
+      if (hh == 0 && !last) {
         live = pieces == 0 || mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1);  // the last one has been read
         if (!live) break;
-        aux->inv[r] = l > 0.f ? 1.f / l : 0.f;
+        aux->inv[r] = inv;
         mbar_arrive(&aux->stat_full);
       }
       const int64_t grow = w.tok * p.num_heads + row;
@@ -622,6 +703,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           P.row_info[grow] = info;
         }
       }
+      if (last) {
+        // the query slots are free: staging for eight warps, half of the columns each
+        live = mbar_wait_warp(&aux->o_full, pieces & 1);
+        if (!live) break;
+        tc_fence_after();
+        write_rows<kFp16, true>(P, w, cluster, c, inv, tbase + lane_off, smem + kOffQ + warp * 4096, 4 * hh, 4 * hh + 4,
+                                nullptr);
+      }
       ++pieces;
     }
     // the other CTA's last commits (and with them its copies of this CTA's P) have arrived
@@ -632,7 +721,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // ------------------------------------------------ query loads, epilogue
     const int r = tid - 256;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const int64_t all_rows = p.num_tokens * p.num_heads;
     // Query tile: the nine groups of 64 dims come by TMA, group g into slot g % 3 of 16 KB; six
     // move on to TMEM, the last three stay. (Loads of a row per thread touch 32 lines per
     // instruction: 14,000 cycles in which the softmax stood still too.)
@@ -679,90 +767,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       mbar_arrive(&aux->q_full);
       return true;
     };
-    auto store_o = [&](const Walk& x, int piece, bool end_of_run) -> bool {
+    auto store_o = [&](const Walk& x, int piece) -> bool {
       if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
       tc_fence_after();
-      const float inv = aux->inv[r];
-      const bool whole = x.starts && x.ends;
-      const int64_t slot = 2 * cluster + (x.starts ? 1 : 0);
-      // Through shared memory, so that a store instruction writes whole sectors: 32 bytes per row at a time
-      // (16-byte half h of row r at h ^ (r / 4 % 2): no bank conflicts), and 128 (chunk q at q ^ (r % 8)) at the end
-      // of the run, when the query slots are free.
-      uint8_t* stage = smem + kOffE + (warp & 3) * 1024;
-      uint8_t* wide = smem + kOffQ + (warp & 3) * 4096;
-      const int row0 = x.mt * kRows + (r & ~31);  // this warp's first row of the unit
-      const int rows = min(32, static_cast<int>(min(static_cast<int64_t>(x.q) * p.num_heads - row0,
-                                                    all_rows - (x.tok * p.num_heads + row0))));
-      uint8_t* dst = whole ? static_cast<uint8_t*>(p.out) + (x.tok * p.num_heads + row0) * (kLatentDim * 2) + 512 * c
-                           : reinterpret_cast<uint8_t*>(P.part_o) +
-                                 (slot * kRows + (r & ~31)) * (kLatentDim * 4) + 1024 * c;
-      const int pitch = whole ? kLatentDim * 2 : kLatentDim * 4;
-      auto put = [&](int part, uint4 a, uint4 b) {
-        const int swap = (lane >> 2) & 1;
-        *reinterpret_cast<uint4*>(stage + lane * 32 + swap * 16) = a;
-        *reinterpret_cast<uint4*>(stage + lane * 32 + (swap ^ 1) * 16) = b;
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int rr = q * 16 + (lane >> 1);
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 32 + (((lane & 1) ^ ((rr >> 2) & 1)) << 4));
-          if (rr < rows) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(rr) * pitch + part * 32 + (lane & 1) * 16) = v;
-        }
-        __syncwarp();
-      };
-      auto put_wide = [&](int chunk, uint4 a) {
-        *reinterpret_cast<uint4*>(wide + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = a;
-      };
-      auto flush_wide = [&](int line) {
-        __syncwarp();
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int rr = q * 4 + (lane >> 3);
-          const uint4 v = *reinterpret_cast<const uint4*>(wide + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
-          if (rr < rows) *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(rr) * pitch + line * 128 + (lane & 7) * 16) = v;
-        }
-        __syncwarp();
-      };
-#pragma unroll 1
-      for (int g = 0; g < 8; ++g) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(tbase + lane_off + kColO + g * 32, o);
-        tmem_wait_ld();
-        if (g == 7) {
-          tc_fence_before();
-          mbar_arrive(&aux->o_empty);
-        }
-        float f[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = inv > 0.f ? __uint_as_float(o[e]) * inv : 0.f;
-        if (whole) {
-          auto four = [&](int e) {
-            return make_uint4(pack2<kFp16>(f[e], f[e + 1]), pack2<kFp16>(f[e + 2], f[e + 3]),
-                              pack2<kFp16>(f[e + 4], f[e + 5]), pack2<kFp16>(f[e + 6], f[e + 7]));
-          };
-          if (end_of_run) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) put_wide((g & 1) * 4 + q, four(8 * q));
-            if (g & 1) flush_wide(g >> 1);
-          } else {
-            put(g * 2, four(0), four(8));
-            put(g * 2 + 1, four(16), four(24));
-          }
-        } else {
-          auto four = [&](int e) {
-            return make_uint4(__float_as_uint(f[e]), __float_as_uint(f[e + 1]), __float_as_uint(f[e + 2]),
-                              __float_as_uint(f[e + 3]));
-          };
-          if (end_of_run) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) put_wide(q, four(4 * q));
-            flush_wide(g);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) put(g * 4 + q, four(8 * q), four(8 * q + 4));
-          }
-        }
-      }
+      write_rows<kFp16, false>(P, x, cluster, c, aux->inv[r], tbase + lane_off, smem + kOffE + (warp & 3) * 1024, 0, 8,
+                               &aux->o_empty);
       return true;
     };
     // the next piece's query goes in as soon as the last scores of this one are
@@ -782,7 +791,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         live = place_q(w, piece + 1);
         if (!live) break;
       }
-      live = store_o(now, piece, !more);
+      if (!more) break;  // the softmax warps, done by then, write the run's last piece
+      live = store_o(now, piece);
       ++piece;
     }
   }
@@ -803,13 +813,21 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   }
 }
 
-// Merges the partials of the rows whose unit was cut: one warp per row, in run
-// order, weights exp(lse_i - max).
-template <bool kFp16>
+// Merges the partials of the rows whose unit was cut, in run order, weights
+// exp(lse_i - max): one warp per row and 512 / kParts of its columns. Bound by
+// the chain row info -> partials (and log-sum-exps), so a lane loads kDepth
+// pieces before it adds the first. Few rows: four warps per row, twelve pieces
+// in flight (16 rows of 11 pieces: 17.5 us for the call, 19.1 with one warp and
+// two pieces); many rows have two or three pieces each, and one warp with four
+// (16,384 rows: 213 us for the call, 232 with four and twelve).
+constexpr int64_t kFewRows = 1024;
+template <bool kFp16, int kParts, int kDepth>
 __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_constant__ Params P, int clusters) {
   pdl_wait();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  constexpr int kVec = 4 / kParts;  // float4 of a piece per lane
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t row = job / kParts;
+  const int lane = threadIdx.x & 31, part = static_cast<int>(job % kParts);
   if (row >= P.L.num_tokens * P.L.num_heads) return;
   const int32_t info = P.row_info[row];
   const int count = info >> 17, c0 = (info >> 7) & 1023, r = info & 127;
@@ -818,51 +836,47 @@ __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_consta
   auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRows + r; };
   // the first 32 pieces' weights, one per lane
   const float mine = lane < count ? P.part_lse[slot(lane)] : -INFINITY;
+  float4 v[kDepth][kVec];
+  auto read = [&](int first) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      if (first + d >= count) break;
+      const float4* src = reinterpret_cast<const float4*>(P.part_o + slot(first + d) * kLatentDim) + part * kVec * 32 + lane;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) v[d][k] = src[32 * k];
+    }
+  };
+  read(0);
   float top = mine;
   for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, P.part_lse[slot(i)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  float4 acc[4] = {};
+  float4 acc[kVec] = {};
   float sum = 0.f;
-  auto weight = [&](int i) {
-    const float lse = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : P.part_lse[slot(i)];
-    return top == -INFINITY ? 0.f : __expf(lse - top);
-  };
-  auto read = [&](int i, float4 (&v)[4]) {
-    const float4* src = reinterpret_cast<const float4*>(P.part_o + slot(i) * kLatentDim);
+  for (int first = 0; first < count; first += kDepth) {
+    if (first > 0) read(first);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = src[lane + 32 * k];
-  };
-  auto add = [&](float wgt, const float4 (&v)[4]) {
-    sum += wgt;
+    for (int d = 0; d < kDepth; ++d) {
+      const int i = first + d;
+      if (i >= count) break;
+      const float lse = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : P.part_lse[slot(i)];
+      const float wgt = top == -INFINITY ? 0.f : __expf(lse - top);
+      sum += wgt;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      acc[k].x = fmaf(wgt, v[k].x, acc[k].x);
-      acc[k].y = fmaf(wgt, v[k].y, acc[k].y);
-      acc[k].z = fmaf(wgt, v[k].z, acc[k].z);
-      acc[k].w = fmaf(wgt, v[k].w, acc[k].w);
+      for (int k = 0; k < kVec; ++k) {
+        acc[k].x = fmaf(wgt, v[d][k].x, acc[k].x);
+        acc[k].y = fmaf(wgt, v[d][k].y, acc[k].y);
+        acc[k].z = fmaf(wgt, v[d][k].z, acc[k].z);
+        acc[k].w = fmaf(wgt, v[d][k].w, acc[k].w);
+      }
     }
-  };
-  // two pieces' loads in flight (most rows have two or three)
-  int i = 0;
-  for (; i + 1 < count; i += 2) {
-    float4 a[4], b[4];
-    read(i, a);
-    read(i + 1, b);
-    add(weight(i), a);
-    add(weight(i + 1), b);
-  }
-  if (i < count) {
-    float4 a[4];
-    read(i, a);
-    add(weight(i), a);
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.L.out) + row * kLatentDim);
+  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.L.out) + row * kLatentDim) + part * kVec * 32 + lane;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    dst[lane + 32 * k] = make_uint2(pack2<kFp16>(acc[k].x * inv, acc[k].y * inv), pack2<kFp16>(acc[k].z * inv, acc[k].w * inv));
-  if (lane == 0) P.L.lse[row] = sum > 0.f ? top + __logf(sum) : -INFINITY;
+  for (int k = 0; k < kVec; ++k)
+    dst[32 * k] = make_uint2(pack2<kFp16>(acc[k].x * inv, acc[k].y * inv), pack2<kFp16>(acc[k].z * inv, acc[k].w * inv));
+  if (lane == 0 && part == 0) P.L.lse[row] = sum > 0.f ? top + __logf(sum) : -INFINITY;
 }
 
 // More clusters than tiles would stay idle, whatever the lengths.
@@ -912,8 +926,10 @@ cudaError_t launch(Params& P, cudaStream_t stream) {
   cfg.gridDim = dim3(2 * clusters);
   e = cudaLaunchKernelEx(&cfg, kern, P);
   if (e != cudaSuccess || clusters == 1) return e;
+  const int64_t rows = P.L.num_tokens * P.L.num_heads;
+  const bool few = rows <= kFewRows;
   cudaLaunchConfig_t cc = {};
-  cc.gridDim = dim3(static_cast<unsigned>((P.L.num_tokens * P.L.num_heads + 7) / 8));
+  cc.gridDim = dim3(static_cast<unsigned>((rows * (few ? 4 : 1) + 7) / 8));
   cc.blockDim = dim3(256);
   cc.stream = stream;
   cudaLaunchAttribute pdl[1];
@@ -921,7 +937,8 @@ cudaError_t launch(Params& P, cudaStream_t stream) {
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cc.attrs = pdl;
   cc.numAttrs = 1;
-  return cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16>, P, clusters);
+  return few ? cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, 4, 12>, P, clusters)
+             : cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, 1, 4>, P, clusters);
 }
 
 }  // namespace
