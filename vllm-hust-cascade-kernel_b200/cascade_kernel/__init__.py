@@ -4,7 +4,9 @@
 tensors, the reference's torch ops (``torch.ops.npu.fa_fp32_stage1``,
 ``torch.ops.npu.lse_merge``, ``torch.ops.npu.f3_gateup_epilogue``) plus the
 extended-domain siblings (``cascade_prefix_attention``,
-``cascade_suffix_decode``, ``cascade_lse_merge``, ``cascade_gateup_swiglu``).
+``cascade_suffix_decode``, ``cascade_lse_merge``, ``cascade_gateup_swiglu``)
+and the paged latent cache's ops (``cascade_latent_decode``,
+``cascade_latent_prefill``, ``cascade_page_*``, ``cascade_verify_drafts``).
 Like the reference package (ascend-kernel/python/ascend_kernel/ascend_kernel/
 __init__.py:5-15) it only loads the library; it never imports vllm.
 
@@ -25,5 +27,6 @@ if not os.path.exists(_EXT):
 torch.ops.load_library(_EXT)
 
 from . import cascade  # noqa: E402,F401  composed cascade step helpers
+from . import latent  # noqa: E402,F401  paged latent cache
 
-__all__ = ["LIB_DIR", "CAPI_PATH", "cascade"]
+__all__ = ["LIB_DIR", "CAPI_PATH", "cascade", "latent"]

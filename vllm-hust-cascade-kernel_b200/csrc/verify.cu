@@ -9,7 +9,11 @@
 // batches, and for small ones bound by the chain draft token -> its two
 // probabilities -> the row. A cluster of CTAs shares a request's row; every CTA
 // repeats the acceptance (a few gathered loads) instead of waiting for another's,
-// and the CTAs' best entries meet in shared memory of rank 0.
+// and the CTAs' best entries meet in every CTA's shared memory.
+//
+// Measured: 128 requests x 128,256 entries in fp32 (170 MB, floor 26 us) 41 us,
+// 4.1 TB/s; 4 requests x 32,000 entries 6.4 us on the device, a launch and four
+// dependent loads.
 //
 // Each value is one rounded product, difference and quotient in fp32, and the
 // best entry is the largest (quotient, lowest index), so the answer does not
