@@ -251,6 +251,9 @@ CASCADE_API int cascade_probe_hbm_read(const void *src, size_t bytes, int32_t mo
  * Rows that see no token (kv_len 0, or causal with kv_len < q_len - i) give
  * out = 0 and lse = -inf. What the pages hold past kv_len is never used, NaN
  * or infinities included.
+ * A NaN, or a score of +infinity, among the tokens a row sees makes its out and
+ * lse NaN. A token of the request that only the causal mask hides has weight 0:
+ * its cache row must be finite, 0 times a NaN value is NaN.
  *   query  [num_tokens, num_heads, 576], contiguous, 16-byte aligned
  *   cache  [num_blocks, block_size, 576], contiguous, 16-byte aligned
  *   block_table int32 [batch, block_cols]; kv lengths are cut to

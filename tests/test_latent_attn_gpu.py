@@ -265,6 +265,24 @@ def test_decode_prefix_and_suffix_merge():
         assert (np.abs(Hh.dev_to_f64(out)[b] - w[0]) <= 2 * w[2]).all()
 
 
+@pytest.mark.parametrize("heads,kv", [(16, [90, 200, 5]), (128, [6000, 70, 131])])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+def test_decode_nan_in_a_seen_row_reaches_the_output(bad, heads, kv):
+    """A NaN key, or a score of +inf, makes the softmax of its request NaN; the others' stay."""
+    import torch
+    Hh.need_cuda()
+    q, cache, bt, qs, kvs = _decode_inputs(kv, [1] * 3, heads, 32, "bf16", poison=False)
+    q[:, :, 520] = 1.0
+    cache[:, :, 520] = 0.0
+    at = kv[0] - 7
+    cache[int(bt[0, at // 32]), at % 32, 520] = float(bad)  # a rotary value: the product with V has none
+    want = _decode_want(q[1:], cache, bt[1:], qs[1:], kvs[1:], True, "bf16")
+    out, lse = _decode(q, cache, bt, qs, kvs, 1)
+    lse = lse.view(3, heads)
+    assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all()
+    _check(Hh.dev_to_f64(out)[1:], Hh.dev_to_f64(lse)[1:], want)
+
+
 # ---------------------------------------------------------------- expanded
 
 
@@ -366,6 +384,20 @@ def test_prefill_sequences_do_not_touch_each_other():
     out, lse = Hh.ops().cascade_latent_prefill(*args, 90, SCALE, True)
     keep = np.r_[0:70, 120:210]
     _check(Hh.dev_to_f64(out)[keep], Hh.dev_to_f64(lse).reshape(210, 2)[keep], [w[keep] for w in want])
+
+
+@pytest.mark.parametrize("at", [0, 2, 3, 66, 130, 255])
+def test_prefill_nan_in_a_seen_key_reaches_the_output(at):
+    import torch
+    Hh.need_cuda()
+    args = _prefill_inputs([(256, 256), (40, 40)], 2, "bf16", "plain")
+    want = _prefill_want(args, True, "bf16")
+    args[2][at, 5] = float("nan")  # rotary key: the values stay finite
+    out, lse = Hh.ops().cascade_latent_prefill(*args, 256, SCALE, True)
+    lse = lse.view(296, 2)
+    assert torch.isnan(out[at:256]).all() and torch.isnan(lse[at:256]).all()
+    keep = np.r_[0:at, 256:296]
+    _check(Hh.dev_to_f64(out)[keep], Hh.dev_to_f64(lse)[keep], [w[keep] for w in want])
 
 
 def test_prefill_max_length_may_be_larger():

@@ -340,7 +340,7 @@ __device__ __forceinline__ void write_rows(const Params& P, const Walk& x, int c
       mbar_arrive(released);
     }
 #pragma unroll
-    for (int e = 0; e < 32; ++e) o[e] = inv > 0.f ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;
+    for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
     if (whole) {  // 64 bytes per row
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       live = hear(of);
       if (!live) break;
       l = (of[0] + of[1]) + (of[2] + of[3]);
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN among the scores stays one
       const bool last = w.left <= 0;  // of the run
       if (hh == 0 && !last) {
         live = pieces == 0 || mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1);  // the last one has been read
@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       }
       const int64_t grow = w.tok * p.num_heads + row;
       if (c == 0 && hh == 0 && row < w.q * p.num_heads && grow < p.num_tokens * p.num_heads) {
-        const float lse = l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY;
+        const float lse = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
         if (w.starts && w.ends)
           p.lse[grow] = lse;
         else
@@ -871,7 +871,7 @@ __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_consta
       const int i = first + d;
       if (i >= count) break;
       const float lse = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : P.part_lse[slot(i)];
-      const float wgt = top == -INFINITY ? 0.f : __expf(lse - top);
+      const float wgt = lse == -INFINITY ? 0.f : __expf(lse - top);
       sum += wgt;
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
@@ -882,12 +882,12 @@ __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_consta
       }
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.L.out) + row * kLatentDim) + part * kVec * 32 + lane;
 #pragma unroll
   for (int k = 0; k < kVec; ++k)
     dst[32 * k] = make_uint2(pack2<kFp16>(acc[k].x * inv, acc[k].y * inv), pack2<kFp16>(acc[k].z * inv, acc[k].w * inv));
-  if (lane == 0 && part == 0) P.L.lse[row] = sum > 0.f ? top + __logf(sum) : -INFINITY;
+  if (lane == 0 && part == 0) P.L.lse[row] = sum == 0.f ? -INFINITY : top + __logf(sum);
 }
 
 // More clusters than tiles would stay idle, whatever the lengths.

@@ -250,16 +250,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
         load(g, x);
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
-          a0 = fmax3f(a0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          a1 = fmax3f(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-          a2 = fmax3f(a2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
-          a3 = fmax3f(a3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
+          a0 = fmax3f_nan(a0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          a1 = fmax3f_nan(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+          a2 = fmax3f_nan(a2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
+          a3 = fmax3f_nan(a3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
         }
       }
-      a0 = fmax3f(a0, a1, fmaxf(a2, a3));
+      a0 = fmax3f_nan(fmax3f_nan(a0, a1, a2), a3, a3);
       aux->shared[t][hh][r] = a0;
       meet();
-      const float top = fmaxf(a0, aux->shared[t][hh ^ 1][r]) * sl2;
+      const float top = fmax3f_nan(a0, aux->shared[t][hh ^ 1][r], a0) * sl2;
       const bool move = top > mx + 8.f;
       const float dm = move ? ex2(mx - top) : 1.f;  // 0 while nothing has been seen
       if (move) mx = top;
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
         tmem_st_32x32b_x16(scol + hh * 64 + g * 16, pk);
       }
       l = l * dm + ((r0 + r1) + (r2 + r3));
+      if (top != top) l = top;  // the exponentials on the FMA pipe lose a NaN
       if ((j + 1) * kTok > m && (t == 0 || j >= nt[0]) && hh == 0) {
         // rows past the sequence may hold NaN, which weight 0 does not hide from
         // the product: the tile whose product comes first clears them
@@ -325,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
       aux->shared[t][hh][r] = l;
       meet();
       l = aux->shared[t][0][r] + aux->shared[t][1][r];
-      if (mx > -INFINITY) {
+      if (mx > -INFINITY || l != l) {  // (a NaN is no maximum)
         inv = 1.f / l;
         lse = (mx + __log2f(l)) * 0.6931471805599453f;
       }
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int e = q * 8 + i * 2;
-            w[i] = inv > 0.f ? pack2<kFp16>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv) : 0u;
+            w[i] = inv == 0.f ? 0u : pack2<kFp16>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
           }
           *reinterpret_cast<uint4*>(stage + lane * 128 + (((g * 4 + q) ^ (lane & 7)) << 4)) =
               make_uint4(w[0], w[1], w[2], w[3]);

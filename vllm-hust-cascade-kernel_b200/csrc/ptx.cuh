@@ -650,6 +650,7 @@ __device__ __forceinline__ float ex2(float x) {
 // whole number (Cody and Waite's reduction, by adding 1.5 * 2^23), 2^f by the
 // degree-4 polynomial of least relative error on [-1/2, 1/2] (2.6e-6, Remez),
 // n into the exponent. x at most 127; below -126 the result stays near 2^-126.
+// A NaN does not survive it: the caller looks for them.
 __device__ __forceinline__ void ex2_poly2(float& y0, float& y1) {
   y0 = fmaxf(y0, -126.f);
   y1 = fmaxf(y1, -126.f);
@@ -687,6 +688,13 @@ __device__ __forceinline__ void ex2_poly2(float& y0, float& y1) {
 __device__ __forceinline__ float fmax3f(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// The same, but NaN if any of the three is.
+__device__ __forceinline__ float fmax3f_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
