@@ -220,6 +220,8 @@ struct LatentDecodeLaunch {
 };
 cudaError_t launch_latent_decode(const LatentDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream);
 size_t latent_decode_workspace(const LatentDecodeLaunch& p);
+cudaError_t launch_latent_decode_pair(const LatentDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream);
+size_t latent_decode_pair_workspace(const LatentDecodeLaunch& p);
 
 struct LatentPrefillLaunch {
   const void* query;

@@ -53,8 +53,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "kernels.h"
-#include "ptx.cuh"
+#include "latent_decode.cuh"
 
 namespace cascade {
 namespace {
@@ -83,13 +82,6 @@ constexpr int kOffE = kOffC + kStagesC * kBytesV;  // epilogue: per warp 32 rows
 constexpr int kTiles = kOffE + 4 * 1024;           // bytes from the first 1 KB boundary after Aux
 
 constexpr uint32_t kColO = 0, kColQ = 256, kColS = 448;  // TMEM columns: O 256, Q 192, S 2 x 32
-
-struct Sched {
-  int64_t tiles, begin;  // all tiles; this cluster's first
-  int64_t tok;           // first query token of request b
-  int b, mt, t0, left;
-  int q, kv;               // request b's lengths
-};
 
 struct __align__(16) Aux {
   // What the four threads of a row (two per CTA) tell one another, in both CTAs: their maxima of a tile, their sums of
@@ -125,142 +117,8 @@ struct Params {
   LatentDecodeLaunch L;
   CUtensorMap map4, map1;  // boxes of 64 dims x kR cache rows x 4 groups (1 group)
   CUtensorMap map_q;       // 64 dims x 128 query rows
-  int32_t* row_info;       // [tokens x heads]: how the row's partials are found, 0 = none
-  float* part_o;           // [2 clusters][128][512]
-  float* part_lse;         // [2 clusters][128]
+  Partials parts;
 };
-
-// row_info of a unit cut into `count` >= 2 pieces, the first in run `c`: row r
-// of the slots 2c + 1 (first piece), 2 (c + 1), 2 (c + 2), ...
-__device__ __forceinline__ int32_t pack_info(int c, int count, int r) { return (count << 17) | (c << 7) | r; }
-
-// The (request, row tile) units' geometry, and the walk over a cluster's run.
-struct Unit {
-  const LatentDecodeLaunch& p;
-  int cap;
-  __device__ explicit Unit(const LatentDecodeLaunch& l) : p(l), cap(l.block_cols * l.block_size) {}
-  __device__ __forceinline__ int q_len(int b) const {
-    return p.q_len > 0 ? p.q_len
-                       : static_cast<int>(min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens));
-  }
-  __device__ __forceinline__ int kv_len(int b) const {
-    return static_cast<int>(min(max(p.kv_lens[b], static_cast<int64_t>(0)), static_cast<int64_t>(1 << 30)));
-  }
-  __device__ __forceinline__ int row_tiles(int q) const {
-    return static_cast<int>((static_cast<int64_t>(q) * p.num_heads + kRows - 1) / kRows);
-  }
-  // cache rows that query token i of a request sees
-  __device__ __forceinline__ int limit(int q, int kv, int i) const {
-    return max(0, p.causal ? min(cap, kv - q + i + 1) : min(cap, kv));
-  }
-  // tiles of a unit: up to what its last row sees, at least one
-  __device__ __forceinline__ int tiles(int q, int kv, int mt) const {
-    const int last = static_cast<int>(min(static_cast<int64_t>(q) * p.num_heads, static_cast<int64_t>(mt + 1) * kRows) - 1) /
-                     p.num_heads;
-    return max(1, (limit(q, kv, last) + kTok - 1) / kTok);
-  }
-};
-
-struct Walk {
-  Unit u;
-  // the current piece
-  int b, mt, t0, n, q, kv;
-  int64_t tok;
-  bool starts, ends;
-  int unit_tiles;
-
-  int next_b, next_mt, next_t0, left, nq, nkv;
-  int64_t next_tok;
-
-  __device__ Walk(const LatentDecodeLaunch& l, const Sched& s)
-      : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), left(s.left), nq(s.q), nkv(s.kv), next_tok(s.tok) {}
-  __device__ __forceinline__ void load() {
-    nq = u.q_len(next_b);
-    nkv = u.kv_len(next_b);
-  }
-  __device__ __forceinline__ bool next() {
-    if (left <= 0) return false;
-    b = next_b, mt = next_mt, t0 = next_t0, q = nq, kv = nkv, tok = next_tok;
-    unit_tiles = u.tiles(q, kv, mt);
-    n = min(left, unit_tiles - t0);
-    starts = t0 == 0;
-    ends = t0 + n == unit_tiles;
-    left -= n;
-    if (left > 0) {  // the next unit's lengths, loaded a piece ahead
-      next_t0 = 0;
-      if (++next_mt == u.row_tiles(q)) {
-        next_mt = 0;
-        do {
-          next_tok += nq;
-          ++next_b;
-          if (next_b >= u.p.batch) {
-            left = 0;
-            break;
-          }
-          load();
-        } while (nq == 0);
-      }
-    }
-    return true;
-  }
-};
-
-// Finds this cluster's run: the block sums the units' tiles (and the query
-// tokens) per contiguous chunk of requests, then the thread whose chunk holds
-// the run's first tile walks to it.
-__device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluster, int clusters, Aux* aux) {
-  const Unit u(p);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-  int64_t tiles = 0, toks = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
-    for (int mt = 0; mt < m; ++mt) tiles += u.tiles(q, kv, mt);
-    toks += q;
-  }
-  int64_t st = tiles, sq = toks;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t a = __shfl_up_sync(0xffffffffu, st, d), c = __shfl_up_sync(0xffffffffu, sq, d);
-    if (lane >= d) st += a, sq += c;
-  }
-  if (lane == 31) aux->scan[0][warp] = st, aux->scan[1][warp] = sq;
-  if (tid == 0) aux->sched.left = 0;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) st += aux->scan[0][w], sq += aux->scan[1][w];
-    total += aux->scan[0][w];
-  }
-  const int64_t runs = min(static_cast<int64_t>(clusters), total);
-  if (cluster < runs) {
-    // floor(cluster total / runs) and floor((cluster + 1) total / runs), with one wide division
-    const int n_runs = static_cast<int>(runs);
-    const int64_t each = total >> 31 ? total / runs : static_cast<uint32_t>(total) / static_cast<uint32_t>(n_runs);
-    const int rest = static_cast<int>(total - each * runs);
-    const int64_t begin = cluster * each + cluster * rest / n_runs;
-    const int64_t end = (cluster + 1) * each + (cluster + 1) * rest / n_runs;
-    int64_t at = st - tiles;
-    if (begin >= at && begin < st) {
-      int64_t tok = sq - toks;
-      for (int b = b0; b < b1; ++b) {
-        const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
-        for (int mt = 0; mt < m; ++mt) {
-          const int t = u.tiles(q, kv, mt);
-          if (begin < at + t) {
-            aux->sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin), q, kv};
-            b = b1;
-            break;
-          }
-          at += t;
-        }
-        tok += q;
-      }
-    }
-  }
-  __syncthreads();
-}
 
 // Loads one box column of a tile: kR cache rows x groups per load, for the 32
 // rows that start at cache row `first`. The warp's lanes hold the pool rows of
@@ -300,7 +158,7 @@ struct PageRows {
 // h ^ (r / 4 % 2)); no bank conflicts either way. `released` (if given) gets an
 // arrival per thread once the accumulator has been read.
 template <bool kFp16, bool kWide>
-__device__ __forceinline__ void write_rows(const Params& P, const Walk& x, int cluster, int c, float inv, uint32_t tmem,
+__device__ __forceinline__ void write_rows(const Params& P, const Walk<kRows, kTok>& x, int cluster, int c, float inv, uint32_t tmem,
                                            uint8_t* stage, int g0, int g1, uint64_t* released) {
   const LatentDecodeLaunch& p = P.L;
   const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
@@ -311,7 +169,7 @@ __device__ __forceinline__ void write_rows(const Params& P, const Walk& x, int c
                                                                       p.num_tokens * p.num_heads - grow0)));
   const int64_t slot = 2 * cluster + (x.starts ? 1 : 0);
   uint8_t* dst = whole ? static_cast<uint8_t*>(p.out) + grow0 * (kLatentDim * 2) + 512 * c
-                       : reinterpret_cast<uint8_t*>(P.part_o) + (slot * kRows + quarter * 32) * (kLatentDim * 4) + 1024 * c;
+                       : reinterpret_cast<uint8_t*>(P.parts.o) + (slot * kRows + quarter * 32) * (kLatentDim * 4) + 1024 * c;
   const int pitch = whole ? kLatentDim * 2 : kLatentDim * 4;
   constexpr int kPerRow = kWide ? 8 : 2;  // 16-byte chunks staged per row
   auto place = [&](int chunk) -> uint4* {
@@ -410,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     tmem_relinquish();
   }
   tc_fence_before();
-  find_run(p, cluster, clusters, aux);  // (with CTA barriers)
+  find_run<kRows, kTok, kThreads>(p, cluster, clusters, aux->scan, &aux->sched);  // (with CTA barriers)
   tc_fence_after();
   // Both CTAs' barriers are initialised once this barrier is passed; only the roles that reach into the other CTA
   // wait for it first, the loads start before.
@@ -418,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   const bool remote = warp < 8 || warp == 13;
   if (remote) cluster_wait();
   const uint32_t tbase = aux->tmem_base;
-  Walk w(p, aux->sched);
+  Walk<kRows, kTok> w(p, aux->sched);
 
   if (warp == 12 || warp == 14) {
     // ------------------------------------------------------------ producers
@@ -700,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         if (w.starts && w.ends)
           p.lse[grow] = lse;
         else
-          P.part_lse[(2 * cluster + (w.starts ? 1 : 0)) * kRows + r] = lse;
+          P.parts.lse[(2 * cluster + (w.starts ? 1 : 0)) * kRows + r] = lse;
         if (w.starts) {
           int32_t info = 0;
           if (!w.ends) {
@@ -711,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             const int64_t hi = ((last + 1) * runs + sc.tiles - 1) / sc.tiles - 1;
             info = pack_info(cluster, static_cast<int>(hi) - cluster + 1, r);
           }
-          P.row_info[grow] = info;
+          P.parts.row_info[grow] = info;
         }
       }
       if (last) {
@@ -735,19 +593,19 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // Query tile: the nine groups of 64 dims come by TMA, group g into slot g % 3 of 16 KB; six
     // move on to TMEM, the last three stay. (Loads of a row per thread touch 32 lines per
     // instruction: 14,000 cycles in which the softmax stood still too.)
-    auto load_group = [&](const Walk& x, int g) {
+    auto load_group = [&](const Walk<kRows, kTok>& x, int g) {
       // group order: the CTA's own columns, the other latent ones, the rotary part
       const int col = g < 4 ? 4 * c + g : g < 8 ? 4 * (1 - c) + g - 4 : 8;
       mbar_arrive_expect_tx(&aux->qs_full[g % 3], kQGroup);
       tma_load_3d(smem + kOffQ + g % 3 * kQGroup, &P.map_q, &aux->qs_full[g % 3], 0,
                   static_cast<int>(x.tok * p.num_heads + x.mt * kRows), col);
     };
-    auto prefetch_q = [&](const Walk& x) {
+    auto prefetch_q = [&](const Walk<kRows, kTok>& x) {
       if (tid == 256)
         for (int g = 0; g < 9; ++g)
           tma_prefetch_3d(&P.map_q, 0, static_cast<int>(x.tok * p.num_heads + x.mt * kRows), g);
     };
-    auto place_q = [&](const Walk& x, int piece) -> bool {
+    auto place_q = [&](const Walk<kRows, kTok>& x, int piece) -> bool {
       if (tid == 256)
         for (int g = 0; g < 3; ++g) load_group(x, g);
       for (int g = 0; g < 9; ++g) {
@@ -778,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       mbar_arrive(&aux->q_full);
       return true;
     };
-    auto store_o = [&](const Walk& x, int piece) -> bool {
+    auto store_o = [&](const Walk<kRows, kTok>& x, int piece) -> bool {
       if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
       tc_fence_after();
       write_rows<kFp16, false>(P, x, cluster, c, aux->inv[r], tbase + lane_off, smem + kOffE + (warp & 3) * 1024, 0, 8,
@@ -792,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     bool live = !more || place_q(w, 0);
     int piece = 0;
     while (live && more) {
-      const Walk now = w;
+      const Walk<kRows, kTok> now = w;
       more = w.next();
       if (more) {
         prefetch_q(w);
@@ -822,84 +680,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
-}
-
-// Merges the partials of the rows whose unit was cut, in run order, weights
-// exp(lse_i - max): one warp per row and 512 / kParts of its columns. Bound by
-// the chain row info -> partials (and log-sum-exps), so a lane loads kDepth
-// pieces before it adds the first. Few rows: four warps per row, twelve pieces
-// in flight (16 rows of 11 pieces: 17.5 us for the call, 19.1 with one warp and
-// two pieces); many rows have two or three pieces each, and one warp with four
-// (16,384 rows: 213 us for the call, 232 with four and twelve).
-constexpr int64_t kFewRows = 1024;
-template <bool kFp16, int kParts, int kDepth>
-__global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_constant__ Params P, int clusters) {
-  pdl_wait();
-  constexpr int kVec = 4 / kParts;  // float4 of a piece per lane
-  const int64_t job = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t row = job / kParts;
-  const int lane = threadIdx.x & 31, part = static_cast<int>(job % kParts);
-  if (row >= P.L.num_tokens * P.L.num_heads) return;
-  const int32_t info = P.row_info[row];
-  const int count = info >> 17, c0 = (info >> 7) & 1023, r = info & 127;
-  // rows of a call whose query lengths do not add up hold no info: nothing past the slots is read for them
-  if (count < 2 || c0 + count > clusters) return;
-  auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRows + r; };
-  // the first 32 pieces' weights, one per lane
-  const float mine = lane < count ? P.part_lse[slot(lane)] : -INFINITY;
-  float4 v[kDepth][kVec];
-  auto read = [&](int first) {
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
-      if (first + d >= count) break;
-      const float4* src = reinterpret_cast<const float4*>(P.part_o + slot(first + d) * kLatentDim) + part * kVec * 32 + lane;
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) v[d][k] = src[32 * k];
-    }
-  };
-  read(0);
-  float top = mine;
-  for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, P.part_lse[slot(i)]);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  float4 acc[kVec] = {};
-  float sum = 0.f;
-  for (int first = 0; first < count; first += kDepth) {
-    if (first > 0) read(first);
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
-      const int i = first + d;
-      if (i >= count) break;
-      const float lse = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : P.part_lse[slot(i)];
-      const float wgt = lse == -INFINITY ? 0.f : __expf(lse - top);
-      sum += wgt;
-#pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        acc[k].x = fmaf(wgt, v[d][k].x, acc[k].x);
-        acc[k].y = fmaf(wgt, v[d][k].y, acc[k].y);
-        acc[k].z = fmaf(wgt, v[d][k].z, acc[k].z);
-        acc[k].w = fmaf(wgt, v[d][k].w, acc[k].w);
-      }
-    }
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(P.L.out) + row * kLatentDim) + part * kVec * 32 + lane;
-#pragma unroll
-  for (int k = 0; k < kVec; ++k)
-    dst[32 * k] = make_uint2(pack2<kFp16>(acc[k].x * inv, acc[k].y * inv), pack2<kFp16>(acc[k].z * inv, acc[k].w * inv));
-  if (lane == 0 && part == 0) P.L.lse[row] = sum == 0.f ? -INFINITY : top + __logf(sum);
-}
-
-// More clusters than tiles would stay idle, whatever the lengths.
-int cluster_bound(const LatentDecodeLaunch& p) {
-  const int64_t rows = p.num_tokens * p.num_heads;
-  const int64_t units = p.batch + rows / kRows;
-  const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(p.block_cols) * p.block_size + kTok - 1) / kTok);
-  return static_cast<int>(std::min<int64_t>(kMaxClusters, std::min<int64_t>(units, 1 << 20) * tiles));
-}
-
-size_t info_bytes(const LatentDecodeLaunch& p) {
-  return (static_cast<size_t>(p.num_tokens) * p.num_heads * sizeof(int32_t) + 255) / 256 * 256;
 }
 
 template <bool kFp16, int kR>
@@ -934,38 +714,23 @@ cudaError_t launch(Params& P, cudaStream_t stream) {
     n = std::min(found, kMaxClusters);
     resident[dev & 63] = n;
   }
-  const int clusters = std::min(n, cluster_bound(P.L));
+  const int clusters = std::min(n, run_bound<kRows, kTok>(P.L, kMaxClusters));
   cfg.gridDim = dim3(2 * clusters);
   e = cudaLaunchKernelEx(&cfg, kern, P);
   if (e != cudaSuccess || clusters == 1) return e;
-  const int64_t rows = P.L.num_tokens * P.L.num_heads;
-  const bool few = rows <= kFewRows;
-  cudaLaunchConfig_t cc = {};
-  cc.gridDim = dim3(static_cast<unsigned>((rows * (few ? 4 : 1) + 7) / 8));
-  cc.blockDim = dim3(256);
-  cc.stream = stream;
-  cudaLaunchAttribute pdl[1];
-  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  pdl[0].val.programmaticStreamSerializationAllowed = 1;
-  cc.attrs = pdl;
-  cc.numAttrs = 1;
-  return few ? cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, 4, 12>, P, clusters)
-             : cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, 1, 4>, P, clusters);
+  return launch_combine<kFp16, kRows>(P.L, P.parts, clusters, stream);
 }
 
 }  // namespace
 
-size_t latent_decode_workspace(const LatentDecodeLaunch& p) {
-  return info_bytes(p) + static_cast<size_t>(cluster_bound(p)) * 2 * kRows * (kLatentDim + 1) * sizeof(float);
+size_t latent_decode_pair_workspace(const LatentDecodeLaunch& p) {
+  return partial_bytes<kRows>(p, run_bound<kRows, kTok>(p, kMaxClusters));
 }
 
-cudaError_t launch_latent_decode(const LatentDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
+cudaError_t launch_latent_decode_pair(const LatentDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
   Params P;
   P.L = p;
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  P.row_info = reinterpret_cast<int32_t*>(ws);
-  P.part_o = reinterpret_cast<float*>(ws + info_bytes(p));
-  P.part_lse = P.part_o + static_cast<size_t>(cluster_bound(p)) * 2 * kRows * kLatentDim;
+  P.parts = partials<kRows>(p, run_bound<kRows, kTok>(p, kMaxClusters), workspace);
   // cache rows as 9 groups of 64 dims; a load is the rows of one page (at most 32) x 4 groups (or 1).
   // A cache without pages: a map over one row that nothing in bounds reads.
   const uint32_t rows = p.block_size < kHalfTok ? 16 : 32;

@@ -1,0 +1,272 @@
+// What the two latent decode kernels share: how the work is cut into equal runs
+// (one per CTA or cluster), the walk over a run, and the merge of the units that
+// run boundaries cut. kRows: query rows per tile, kTok: cache rows per tile.
+#pragma once
+#include <algorithm>
+
+#include "kernels.h"
+#include "ptx.cuh"
+
+namespace cascade {
+namespace {
+
+struct Partials {
+  int32_t* row_info;  // [tokens x heads]: how the row's partials are found, 0 = none
+  float* o;           // [2 runs][kRows][512]
+  float* lse;         // [2 runs][kRows]
+};
+
+struct Sched {
+  int64_t tiles, begin;  // all tiles; this cluster's first
+  int64_t tok;           // first query token of request b
+  int b, mt, t0, left;
+  int q, kv;               // request b's lengths
+};
+
+// row_info of a unit cut into `count` >= 2 pieces, the first in run `c`: row r
+// of the slots 2c + 1 (first piece), 2 (c + 1), 2 (c + 2), ...
+__device__ __forceinline__ int32_t pack_info(int c, int count, int r) { return (count << 17) | (c << 7) | r; }
+
+// The (request, row tile) units' geometry, and the walk over a cluster's run.
+template <int kRows, int kTok>
+struct Unit {
+  const LatentDecodeLaunch& p;
+  int cap;
+  __device__ explicit Unit(const LatentDecodeLaunch& l) : p(l), cap(l.block_cols * l.block_size) {}
+  __device__ __forceinline__ int q_len(int b) const {
+    return p.q_len > 0 ? p.q_len
+                       : static_cast<int>(min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens));
+  }
+  __device__ __forceinline__ int kv_len(int b) const {
+    return static_cast<int>(min(max(p.kv_lens[b], static_cast<int64_t>(0)), static_cast<int64_t>(1 << 30)));
+  }
+  __device__ __forceinline__ int row_tiles(int q) const {
+    return static_cast<int>((static_cast<int64_t>(q) * p.num_heads + kRows - 1) / kRows);
+  }
+  // cache rows that query token i of a request sees
+  __device__ __forceinline__ int limit(int q, int kv, int i) const {
+    return max(0, p.causal ? min(cap, kv - q + i + 1) : min(cap, kv));
+  }
+  // tiles of a unit: up to what its last row sees, at least one
+  __device__ __forceinline__ int tiles(int q, int kv, int mt) const {
+    const int last = static_cast<int>(min(static_cast<int64_t>(q) * p.num_heads, static_cast<int64_t>(mt + 1) * kRows) - 1) /
+                     p.num_heads;
+    return max(1, (limit(q, kv, last) + kTok - 1) / kTok);
+  }
+};
+
+template <int kRows, int kTok>
+struct Walk {
+  Unit<kRows, kTok> u;
+  // the current piece
+  int b, mt, t0, n, q, kv;
+  int64_t tok;
+  bool starts, ends;
+  int unit_tiles;
+
+  int next_b, next_mt, next_t0, left, nq, nkv;
+  int64_t next_tok;
+
+  __device__ Walk(const LatentDecodeLaunch& l, const Sched& s)
+      : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), left(s.left), nq(s.q), nkv(s.kv), next_tok(s.tok) {}
+  __device__ __forceinline__ void load() {
+    nq = u.q_len(next_b);
+    nkv = u.kv_len(next_b);
+  }
+  __device__ __forceinline__ bool next() {
+    if (left <= 0) return false;
+    b = next_b, mt = next_mt, t0 = next_t0, q = nq, kv = nkv, tok = next_tok;
+    unit_tiles = u.tiles(q, kv, mt);
+    n = min(left, unit_tiles - t0);
+    starts = t0 == 0;
+    ends = t0 + n == unit_tiles;
+    left -= n;
+    if (left > 0) {  // the next unit's lengths, loaded a piece ahead
+      next_t0 = 0;
+      if (++next_mt == u.row_tiles(q)) {
+        next_mt = 0;
+        do {
+          next_tok += nq;
+          ++next_b;
+          if (next_b >= u.p.batch) {
+            left = 0;
+            break;
+          }
+          load();
+        } while (nq == 0);
+      }
+    }
+    return true;
+  }
+};
+
+// Finds this cluster's run: the block sums the units' tiles (and the query
+// tokens) per contiguous chunk of requests, then the thread whose chunk holds
+// the run's first tile walks to it.
+template <int kRows, int kTok, int kThreads>
+__device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluster, int clusters,
+                                         int64_t (*scan)[kThreads / 32], Sched* sched) {
+  const Unit<kRows, kTok> u(p);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+  int64_t tiles = 0, toks = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
+    for (int mt = 0; mt < m; ++mt) tiles += u.tiles(q, kv, mt);
+    toks += q;
+  }
+  int64_t st = tiles, sq = toks;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t a = __shfl_up_sync(0xffffffffu, st, d), c = __shfl_up_sync(0xffffffffu, sq, d);
+    if (lane >= d) st += a, sq += c;
+  }
+  if (lane == 31) scan[0][warp] = st, scan[1][warp] = sq;
+  if (tid == 0) sched->left = 0;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) st += scan[0][w], sq += scan[1][w];
+    total += scan[0][w];
+  }
+  const int64_t runs = min(static_cast<int64_t>(clusters), total);
+  if (cluster < runs) {
+    // floor(cluster total / runs) and floor((cluster + 1) total / runs), with one wide division
+    const int n_runs = static_cast<int>(runs);
+    const int64_t each = total >> 31 ? total / runs : static_cast<uint32_t>(total) / static_cast<uint32_t>(n_runs);
+    const int rest = static_cast<int>(total - each * runs);
+    const int64_t begin = cluster * each + cluster * rest / n_runs;
+    const int64_t end = (cluster + 1) * each + (cluster + 1) * rest / n_runs;
+    int64_t at = st - tiles;
+    if (begin >= at && begin < st) {
+      int64_t tok = sq - toks;
+      for (int b = b0; b < b1; ++b) {
+        const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
+        for (int mt = 0; mt < m; ++mt) {
+          const int t = u.tiles(q, kv, mt);
+          if (begin < at + t) {
+            *sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin), q, kv};
+            b = b1;
+            break;
+          }
+          at += t;
+        }
+        tok += q;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// Merges the partials of the rows whose unit was cut, in run order, weights
+// exp(lse_i - max): one warp per row and 512 / kParts of its columns. Bound by
+// the chain row info -> partials (and log-sum-exps), so a lane loads kDepth
+// pieces before it adds the first. Few rows: four warps per row, twelve pieces
+// in flight (16 rows of 11 pieces: 17.5 us for the call, 19.1 with one warp and
+// two pieces); many rows have two or three pieces each, and one warp with four
+// (16,384 rows: 213 us for the call, 232 with four and twelve).
+constexpr int64_t kFewRows = 1024;
+template <bool kFp16, int kRows, int kParts, int kDepth>
+__global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_constant__ LatentDecodeLaunch L,
+                                                             const __grid_constant__ Partials P, int clusters) {
+  pdl_wait();
+  constexpr int kVec = 4 / kParts;  // float4 of a piece per lane
+  const int64_t job = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t row = job / kParts;
+  const int lane = threadIdx.x & 31, part = static_cast<int>(job % kParts);
+  if (row >= L.num_tokens * L.num_heads) return;
+  const int32_t info = P.row_info[row];
+  const int count = info >> 17, c0 = (info >> 7) & 1023, r = info & 127;
+  // rows of a call whose query lengths do not add up hold no info: nothing past the slots is read for them
+  if (count < 2 || c0 + count > clusters) return;
+  auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRows + r; };
+  // the first 32 pieces' weights, one per lane
+  const float mine = lane < count ? P.lse[slot(lane)] : -INFINITY;
+  float4 v[kDepth][kVec];
+  auto read = [&](int first) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      if (first + d >= count) break;
+      const float4* src = reinterpret_cast<const float4*>(P.o + slot(first + d) * kLatentDim) + part * kVec * 32 + lane;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) v[d][k] = src[32 * k];
+    }
+  };
+  read(0);
+  float top = mine;
+  for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, P.lse[slot(i)]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float4 acc[kVec] = {};
+  float sum = 0.f;
+  for (int first = 0; first < count; first += kDepth) {
+    if (first > 0) read(first);
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int i = first + d;
+      if (i >= count) break;
+      const float lse = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : P.lse[slot(i)];
+      const float wgt = lse == -INFINITY ? 0.f : __expf(lse - top);
+      sum += wgt;
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) {
+        acc[k].x = fmaf(wgt, v[d][k].x, acc[k].x);
+        acc[k].y = fmaf(wgt, v[d][k].y, acc[k].y);
+        acc[k].z = fmaf(wgt, v[d][k].z, acc[k].z);
+        acc[k].w = fmaf(wgt, v[d][k].w, acc[k].w);
+      }
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + row * kLatentDim) + part * kVec * 32 + lane;
+#pragma unroll
+  for (int k = 0; k < kVec; ++k)
+    dst[32 * k] = make_uint2(pack2<kFp16>(acc[k].x * inv, acc[k].y * inv), pack2<kFp16>(acc[k].z * inv, acc[k].w * inv));
+  if (lane == 0 && part == 0) L.lse[row] = sum == 0.f ? -INFINITY : top + __logf(sum);
+}
+
+inline size_t info_bytes(const LatentDecodeLaunch& p) {
+  return (static_cast<size_t>(p.num_tokens) * p.num_heads * sizeof(int32_t) + 255) / 256 * 256;
+}
+
+template <int kRows>
+size_t partial_bytes(const LatentDecodeLaunch& p, int runs) {
+  return info_bytes(p) + static_cast<size_t>(runs) * 2 * kRows * (kLatentDim + 1) * sizeof(float);
+}
+
+template <int kRows>
+Partials partials(const LatentDecodeLaunch& p, int runs, void* workspace) {
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* o = reinterpret_cast<float*>(ws + info_bytes(p));
+  return {reinterpret_cast<int32_t*>(ws), o, o + static_cast<size_t>(runs) * 2 * kRows * kLatentDim};
+}
+
+// Runs of a launch: more than tiles would stay idle, whatever the lengths.
+template <int kRows, int kTok>
+int run_bound(const LatentDecodeLaunch& p, int most) {
+  const int64_t rows = p.num_tokens * p.num_heads;
+  const int64_t units = p.batch + rows / kRows;
+  const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(p.block_cols) * p.block_size + kTok - 1) / kTok);
+  return static_cast<int>(std::min<int64_t>(most, std::min<int64_t>(units, 1 << 20) * tiles));
+}
+
+template <bool kFp16, int kRows>
+cudaError_t launch_combine(const LatentDecodeLaunch& p, const Partials& parts, int runs, cudaStream_t stream) {
+  const int64_t rows = p.num_tokens * p.num_heads;
+  const bool few = rows <= kFewRows;
+  cudaLaunchConfig_t cc = {};
+  cc.gridDim = dim3(static_cast<unsigned>((rows * (few ? 4 : 1) + 7) / 8));
+  cc.blockDim = dim3(256);
+  cc.stream = stream;
+  cudaLaunchAttribute pdl[1];
+  pdl[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl[0].val.programmaticStreamSerializationAllowed = 1;
+  cc.attrs = pdl;
+  cc.numAttrs = 1;
+  return few ? cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, kRows, 4, 12>, p, parts, runs)
+             : cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, kRows, 1, 4>, p, parts, runs);
+}
+
+}  // namespace
+}  // namespace cascade
