@@ -1,13 +1,11 @@
 // Latent attention, absorbed form (cascade_latent_decode), for requests of up to
 // 32 query rows (a few heads per GPU): bound by reading the cache, 1,152 bytes
-// per token. The 128 rows that a tensor-core tile has go to the cache:
-//   S^T [128 tokens x kN rows]  = C [128 x 576] X^T
-//   O^T [4 x 128 values x kN rows] += V^T [512 x 128] P
+// per token. The rows that a tensor-core tile has go to the cache:
+//   S^T [64 tokens x kN rows]     = C [64 x 576] X^T
+//   O^T [4 x 128 values x kN rows] += V^T [512 x 64] P
 // with kN = 16 or 32 query rows as the MMA's N, so a CTA holds a whole output
 // (4 kN TMEM columns) and needs no other. Both products read the cache tile from
-// shared memory as it was loaded (K-major, then M-major): 36 + 32 steps of 43
-// cycles for 128 tokens, 2,900 cycles against the 6,500 that an SM's share of
-// HBM takes for their 147 KB.
+// shared memory as it was loaded (K-major, then M-major).
 //
 // Softmax: a thread per token. The rows' running maxima are the same in every
 // thread; they move only when some score exceeds its row's by more than 2^8 (a
@@ -15,9 +13,12 @@
 // sums stay per thread and row until the piece ends, in fp32, of the unrounded
 // exponentials. P is rounded to the inputs' type, which the second product needs.
 //
-// Shared memory: a ring of five 32 KB slots for pairs of 64-value groups
-// (128 tokens x 128 values: one M block of the second product), freed block by block as
-// P V goes, and kRope slots of 16 KB for the rotary group, freed by the scores.
+// Shared memory: a tile's eight boxes of 8 tokens x 576 values (page sizes are
+// multiples of 16) each come in two parts, six (four) groups of 64 values in a ring of
+// three slots and the rest in one of two, so that 1.7 (1.5) tiles are on their way
+// while one is worked on: it takes about 2,300 cycles from the last load to the free
+// slot, an SM's share of HBM 3,250 for its 74 KB. (Tiles of 128 tokens leave
+// 48 KB to be on their way.)
 //
 // Warps: 0-3 softmax and output, 4 cache loads, 5 MMA issue, 6 query loads.
 #include <algorithm>
@@ -27,24 +28,29 @@
 namespace cascade {
 namespace {
 
-constexpr int kTok = 128;
+constexpr int kTok = 64;
 constexpr int kThreads = 7 * 32;
-constexpr int kPairs = 5;
-constexpr int kGroup = kTok * 128;  // 128 tokens x 64 values
+constexpr int kBox = 8;  // cache rows per load
+constexpr int kBoxes = kTok / kBox;
+constexpr int kAtom = kBox * 128;  // 8 rows x 64 values
 
 template <int kN>
 struct Few {
-  static constexpr int kRope = kN == 16 ? 2 : 1;
+  // a tile's nine groups of 64 values in two parts, with rings of their own
+  static constexpr int kGroupsA = kN == 16 ? 6 : 4, kGroupsB = 9 - kGroupsA;
+  static constexpr int kSlotsA = 3, kSlotsB = 2;
+  static constexpr int kBytesA = kBoxes * kGroupsA * kAtom, kBytesB = kBoxes * kGroupsB * kAtom;
   static constexpr int kQGroup = kN * 128;
   static constexpr int kRowBytes = kN * 2;  // of P: a token's weights
   static constexpr int kOffQ = 0;
   static constexpr int kOffP = kOffQ + 9 * kQGroup;
-  static constexpr int kOffV = kOffP + kTok * kRowBytes;
-  static constexpr int kOffR = kOffV + kPairs * 2 * kGroup;
-  static constexpr int kTiles = kOffR + kRope * kGroup;
+  static constexpr int kOffA = kOffP + kTok * kRowBytes;
+  static constexpr int kOffB = kOffA + kSlotsA * kBytesA;
+  static constexpr int kTiles = kOffB + kSlotsB * kBytesB;
   static constexpr int kColS = 0, kColO = kN;  // TMEM columns
   static constexpr int kTmem = kN == 16 ? 128 : 256;
-  static_assert(kColO + 4 * kN <= kTmem && kOffP % 1024 == 0 && kOffV % 1024 == 0, "layout");
+  static_assert(kColO + 4 * kN <= kTmem && kOffP % 1024 == 0 && kOffA % 1024 == 0, "layout");
+  static_assert(kGroupsA % 2 == 0, "an M block of the second product lies in one part");
 
   struct __align__(16) Aux {
     union {
@@ -52,8 +58,9 @@ struct Few {
       int64_t scan[2][kThreads / 32];  // find_run only
     };
     float sum[4][kN];
+    float inv[kN];  // 1 / the rows' sums
     int lim[kN];  // tokens that a row sees
-    uint64_t v_full[kPairs], v_free[kPairs], r_full[kRope], r_free[kRope];
+    uint64_t a_full[kSlotsA], b_full[kSlotsB], pv_done[kSlotsA];
     uint64_t q_full, q_free, s_full, p_full, o_full, stall, drain;
     uint32_t tmem_base;
     Sched sched;
@@ -65,9 +72,8 @@ struct Few {
 
 struct Params {
   LatentDecodeLaunch L;
-  CUtensorMap map;    // 64 values x box_rows cache rows
-  CUtensorMap map_q;  // 64 values x kN query rows x 9 groups
-  int box_rows;
+  CUtensorMap map_a, map_b;  // 64 values x 8 cache rows x the part's groups
+  CUtensorMap map_q;         // 64 values x kN query rows x 9 groups
   Partials parts;
 };
 
@@ -132,8 +138,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
 
   if (tid == 0) {
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
-    for (int s = 0; s < kPairs; ++s) mbar_init(&aux->v_full[s], 1), mbar_init(&aux->v_free[s], 1);
-    for (int s = 0; s < F::kRope; ++s) mbar_init(&aux->r_full[s], 1), mbar_init(&aux->r_free[s], 1);
+    for (int s = 0; s < F::kSlotsA; ++s) mbar_init(&aux->a_full[s], 1), mbar_init(&aux->pv_done[s], 1);
+    for (int s = 0; s < F::kSlotsB; ++s) mbar_init(&aux->b_full[s], 1);
     mbar_init(&aux->q_full, 1);
     mbar_init(&aux->q_free, 1);
     mbar_init(&aux->s_full, 1);
@@ -143,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
   }
-  if (tid == 32) tma_prefetch_desc(&P.map);
+  if (tid == 32) tma_prefetch_desc(&P.map_a), tma_prefetch_desc(&P.map_b);
   if (tid == 64) tma_prefetch_desc(&P.map_q);
   if (warp == 5) {
     tmem_alloc(&aux->tmem_base, F::kTmem);
@@ -157,42 +163,47 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
 
   if (warp == 4) {
     // ---------------------------------------------------------- cache loads
-    const int boxes = kTok / P.box_rows, oob = max(1, p.num_blocks * p.block_size);
+    const int oob = max(1, p.num_blocks * p.block_size);
     int it = 0;
     bool live = true;
     while (live && w.next()) {
       const int32_t* bt = p.block_table + static_cast<int64_t>(w.b) * p.block_cols;
       const int pages = (min(w.kv, w.u.cap) + p.block_size - 1) / p.block_size;
-      // lane i holds the pool row of box i of the next tile
-      auto row_of = [&](int t) {
-        const int tok = t * kTok + lane * P.box_rows, page = tok / p.block_size;
-        return lane < boxes && page < pages ? paged_row(bt[page], tok, p.block_size, p.num_blocks, oob) : oob;
-      };
-      int y = row_of(w.t0);
+      // lane i holds the pool row of the i-th eight rows from tile t on: four tiles' worth
+      int y = oob;
       for (int t = w.t0; t < w.t0 + w.n; ++t, ++it) {
-        const int y_next = t + 1 < w.t0 + w.n ? row_of(t + 1) : 0;
-        for (int j = 0; j < 5; ++j) {  // four pairs of latent groups, then the rotary one
-          const int i = j < 4 ? 4 * it + j : it, slots = j < 4 ? kPairs : F::kRope, s = i % slots;
-          uint64_t* full = j < 4 ? &aux->v_full[s] : &aux->r_full[s];
-          live = i < slots || mbar_wait_warp(j < 4 ? &aux->v_free[s] : &aux->r_free[s], (i / slots - 1) & 1);
-          if (!live) break;
-          uint8_t* dst = smem + (j < 4 ? F::kOffV + s * 2 * kGroup : F::kOffR + s * kGroup) + lane * P.box_rows * 128;
-          if (lane == 0) mbar_arrive_expect_tx(full, j < 4 ? 2 * kGroup : kGroup);
-          __syncwarp();
-          if (lane < boxes) {
-            tma_load_3d(dst, &P.map, full, 0, y, 2 * j);
-            if (j < 4) tma_load_3d(dst + kGroup, &P.map, full, 0, y, 2 * j + 1);
-          }
-          __syncwarp();
+        const int ahead = (t - w.t0) & 3;
+        if (ahead == 0) {
+          const int tok = t * kTok + lane * kBox, page = tok / p.block_size;
+          y = page < pages ? paged_row(bt[page], tok, p.block_size, p.num_blocks, oob) : oob;
         }
+        const int row = __shfl_sync(0xffffffffu, y, ahead * kBoxes + (lane & (kBoxes - 1)));
+        const int sa = it % F::kSlotsA, sb = it % F::kSlotsB;
+        // P V of the tile that had the slot is done
+        auto freed = [&](int slots) {
+          const int old = it - slots;
+          return old < 0 || mbar_wait_warp(&aux->pv_done[old % F::kSlotsA], (old / F::kSlotsA) & 1);
+        };
+        live = freed(F::kSlotsA);
         if (!live) break;
-        y = y_next;
+        if (lane == 0) mbar_arrive_expect_tx(&aux->a_full[sa], F::kBytesA);
+        __syncwarp();
+        if (lane < kBoxes)
+          tma_load_3d(smem + F::kOffA + sa * F::kBytesA + lane * F::kGroupsA * kAtom, &P.map_a, &aux->a_full[sa], 0, row, 0);
+        live = freed(F::kSlotsB);
+        if (!live) break;
+        if (lane == 0) mbar_arrive_expect_tx(&aux->b_full[sb], F::kBytesB);
+        __syncwarp();
+        if (lane < kBoxes)
+          tma_load_3d(smem + F::kOffB + sb * F::kBytesB + lane * F::kGroupsB * kAtom, &P.map_b, &aux->b_full[sb], 0, row,
+                      F::kGroupsA);
+        __syncwarp();
       }
     }
   } else if (warp == 5) {
     // ------------------------------------------------------------ MMA issue
     const uint32_t idesc_s = make_idesc_f16(kTok, kN, kFp16 ? 0u : 1u, 0, 0);
-    const uint32_t idesc_o = make_idesc_f16(kTok, kN, kFp16 ? 0u : 1u, 1, 1);
+    const uint32_t idesc_o = make_idesc_f16(128, kN, kFp16 ? 0u : 1u, 1, 1);
     const uint32_t tm = uniform(tbase), s0 = uniform(smem_u32(smem));
     const uint64_t dq = make_smem_desc(s0 + F::kOffQ, 16, 1024, 2);
     // P: a token's kN weights in a row of 32 (64) bytes, swizzled in as many
@@ -202,46 +213,52 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     while (live && w.next()) {
       live = mbar_wait_warp(&aux->q_full, piece & 1);
       for (int t = 0; live && t < w.n; ++t, ++it) {
-        for (int j = 0; live && j < 5; ++j) {
-          const uint32_t i = uniform(j < 4 ? 4 * it + j : it), slots = j < 4 ? kPairs : F::kRope, s = i % slots;
-          live = mbar_wait_warp(j < 4 ? &aux->v_full[s] : &aux->r_full[s], (i / slots) & 1);
-          if (!live) break;
+        const uint32_t u = uniform(it), sa = u % F::kSlotsA, sb = u % F::kSlotsB;
+        const uint32_t a = s0 + F::kOffA + sa * F::kBytesA, b = s0 + F::kOffB + sb * F::kBytesB;
+        // groups [g0, g1) of a part whose boxes are `pitch` bytes apart
+        auto scores = [&](uint32_t part, int pitch, int g0, int g1) {
+          const uint64_t da = make_smem_desc(part, 16, pitch, 2);
           tc_fence_after();
-          const uint64_t da = make_smem_desc(s0 + (j < 4 ? F::kOffV + s * 2 * kGroup : F::kOffR + s * kGroup), 16, 1024, 2);
-          const uint64_t db = dq + j * 2 * F::kQGroup / 16;
           __syncwarp();
           if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) umma_f16_ss(tm + F::kColS, da + k * 2, db + k * 2, idesc_s, j + k > 0);
-            if (j < 4) {
+#pragma unroll 1
+            for (int g = g0; g < g1; ++g) {
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                umma_f16_ss(tm + F::kColS, da + kGroup / 16 + k * 2, db + F::kQGroup / 16 + k * 2, idesc_s, 1u);
-            } else {
+                umma_f16_ss(tm + F::kColS, da + (g - g0) * kAtom / 16 + k * 2, dq + g * F::kQGroup / 16 + k * 2, idesc_s,
+                            g + k > 0);
+            }
+            if (g1 == 9) {
               umma_commit(&aux->s_full);
-              umma_commit(&aux->r_free[s]);
               if (t + 1 == w.n) umma_commit(&aux->q_free);
             }
           }
           __syncwarp();
-        }
-        live = live && mbar_wait_warp(&aux->p_full, it & 1);
+        };
+        live = mbar_wait_warp(&aux->a_full[sa], (u / F::kSlotsA) & 1);
+        if (!live) break;
+        scores(a, F::kGroupsA * kAtom, 0, F::kGroupsA);
+        live = mbar_wait_warp(&aux->b_full[sb], (u / F::kSlotsB) & 1);
+        if (!live) break;
+        scores(b, F::kGroupsB * kAtom, F::kGroupsA, 9);
+        live = mbar_wait_warp(&aux->p_full, u & 1);
         if (!live) break;
         tc_fence_after();
+        __syncwarp();
+        if (elect_one()) {
 #pragma unroll 1
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t s = uniform(static_cast<uint32_t>(4 * it + j) % kPairs);
-          const uint64_t dv = make_smem_desc(s0 + F::kOffV + s * 2 * kGroup, kGroup, 1024, 2);
-          __syncwarp();
-          if (elect_one()) {
+          for (int j = 0; j < 4; ++j) {
+            const bool in_a = 2 * j < F::kGroupsA;
+            const int pitch = (in_a ? F::kGroupsA : F::kGroupsB) * kAtom;
+            const uint64_t dv = make_smem_desc((in_a ? a + 2 * j * kAtom : b + (2 * j - F::kGroupsA) * kAtom), kAtom, pitch, 2);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16_ss(tm + F::kColO + j * kN, dv + k * 2048 / 16, dp + k * 16 * F::kRowBytes / 16, idesc_o, t + k > 0);
-            umma_commit(&aux->v_free[s]);
-            if (j == 3 && t + 1 == w.n) umma_commit(&aux->o_full);
+            for (int k = 0; k < kTok / 16; ++k)
+              umma_f16_ss(tm + F::kColO + j * kN, dv + k * 2 * pitch / 16, dp + k * 16 * F::kRowBytes / 16, idesc_o, t + k > 0);
           }
-          __syncwarp();
+          umma_commit(&aux->pv_done[sa]);
+          if (t + 1 == w.n) umma_commit(&aux->o_full);
         }
+        __syncwarp();
       }
       ++piece;
     }
@@ -265,6 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     // is waited for in vain.
     const uint32_t tl = tbase + (static_cast<uint32_t>(warp * 32) << 16);
     const float sl2 = p.scale * 1.4426950408889634f;
+    const int mine = warp * 16 + lane;  // token of the tile: 64 rows of scores lie in the first 16 lanes of each quarter
+    const int my_col = tid & (kN - 1);
     if (p.debug_stall) mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
     int it = 0, piece = 0;
     while (w.next()) {
@@ -272,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
       const int clean = w.u.limit(w.q, w.kv, row0 / p.num_heads) / kTok;  // tiles below are seen in full by every row
       if (tid < kN) aux->lim[tid] = w.u.limit(w.q, w.kv, min((row0 + tid) / p.num_heads, w.q - 1));
       meet();
-      float m[kN], l[kN];
+      float m[kN], l[kN], my_m = -INFINITY;  // my_m: row my_col's
 #pragma unroll
       for (int j = 0; j < kN; ++j) m[j] = -INFINITY, l[j] = 0.f;
       for (int t = w.t0; t < w.t0 + w.n; ++t, ++it) {
@@ -281,7 +300,11 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
         uint32_t x[kN];
         tmem_ld_row<kN>(tl + F::kColS, x);
         tmem_wait_ld();
-        const int tok = t * kTok + tid;
+        const int tok = t * kTok + mine;
+        if (lane >= 16) {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) x[j] = 0xff800000u;
+        }
         if (t >= clean) {
 #pragma unroll
           for (int j = 0; j < kN; ++j) x[j] = tok < aux->lim[j] ? x[j] : 0xff800000u;
@@ -297,10 +320,14 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
           const float top = reduce_columns<kN>(v, lane, col, [](float a, float b) { return fmaxf(a, b); });
           aux->top[warp][col] = top;
           meet();
+          auto top_of = [&](int j) {
+            return sl2 * fmaxf(fmaxf(aux->top[0][j], aux->top[1][j]), fmaxf(aux->top[2][j], aux->top[3][j]));
+          };
+          if (top_of(my_col) > my_m + 8.f) my_m = top_of(my_col);
           float dm[kN];
 #pragma unroll
           for (int j = 0; j < kN; ++j) {
-            const float mx = sl2 * fmaxf(fmaxf(aux->top[0][j], aux->top[1][j]), fmaxf(aux->top[2][j], aux->top[3][j]));
+            const float mx = top_of(j);
             const bool up = mx > m[j] + 8.f;
             dm[j] = up ? ex2(m[j] - mx) : 1.f;  // 0 while nothing has been seen
             if (up) m[j] = mx;
@@ -332,20 +359,25 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
           }
           pk[j / 2] = pack2<kFp16>(y[0], y[1]);
         }
-        uint8_t* dst = smem + F::kOffP + tid * F::kRowBytes;
-        const int swap = kN == 16 ? (tid >> 2) & 1 : (tid >> 1) & 3;
+        if (lane < 16) {
+          uint8_t* dst = smem + F::kOffP + mine * F::kRowBytes;
+          const int swap = kN == 16 ? (mine >> 2) & 1 : (mine >> 1) & 3;
 #pragma unroll
-        for (int q = 0; q < kN / 8; ++q)
-          *reinterpret_cast<uint4*>(dst + ((q ^ swap) << 4)) =
-              make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-        if (tok >= valid) {
-          // rows past the request's length may hold NaN: weight 0 does not hide
-          // them from the product, so they are cleared (the scores have read them)
-          for (int j = 0; j < 4; ++j) {
-            uint8_t* slot = smem + F::kOffV + (4 * it + j) % kPairs * 2 * kGroup + tid * 128;
+          for (int q = 0; q < kN / 8; ++q)
+            *reinterpret_cast<uint4*>(dst + ((q ^ swap) << 4)) =
+                make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+          if (tok >= valid) {
+            // rows past the request's length may hold NaN: weight 0 does not hide
+            // them from the product, so they are cleared (the scores have read them)
+#pragma unroll 1
+            for (int g = 0; g < 8; ++g) {
+              uint8_t* at = g < F::kGroupsA ? smem + F::kOffA + it % F::kSlotsA * F::kBytesA + ((mine >> 3) * F::kGroupsA + g) * kAtom
+                                            : smem + F::kOffB + it % F::kSlotsB * F::kBytesB +
+                                                  ((mine >> 3) * F::kGroupsB + g - F::kGroupsA) * kAtom;
 #pragma unroll
-            for (int q = 0; q < 16; ++q)
-              *reinterpret_cast<uint4*>(slot + (q >> 3) * kGroup + (q & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int q = 0; q < 8; ++q)
+                *reinterpret_cast<uint4*>(at + (mine & 7) * 128 + q * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
           }
         }
         fence_proxy_async_smem();
@@ -363,46 +395,53 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
                                                                         p.num_tokens * p.num_heads - grow0)));
       const bool whole = w.starts && w.ends;
       const int64_t slot = (2 * run + (w.starts ? 1 : 0)) * kN;
-      float inv[kN];
-      int32_t info = 0;
-      if (w.starts && !w.ends) {
-        // the run that holds the unit's last tile
-        const Sched& sc = aux->sched;
-        const int64_t n_runs = min(static_cast<int64_t>(runs), sc.tiles);
-        const int64_t last = sc.begin + (it - w.n) + w.unit_tiles - 1;
-        const int64_t hi = ((last + 1) * n_runs + sc.tiles - 1) / sc.tiles - 1;
-        info = pack_info(run, static_cast<int>(hi) - run + 1, tid & (kN - 1));
-      }
       const bool write = !cta_aborted();
-#pragma unroll
-      for (int j = 0; j < kN; ++j) {
-        const float s = (aux->sum[0][j] + aux->sum[1][j]) + (aux->sum[2][j] + aux->sum[3][j]);
-        inv[j] = s == 0.f ? 0.f : 1.f / s;  // a NaN among the scores stays one
-        if (tid == j && j < rows && write) {
-          const float lse = s == 0.f ? -INFINITY : (m[j] + __log2f(s)) * 0.6931471805599453f;
+      if (tid < kN) {
+        const float s = (aux->sum[0][tid] + aux->sum[1][tid]) + (aux->sum[2][tid] + aux->sum[3][tid]);
+        aux->inv[tid] = s == 0.f ? 0.f : 1.f / s;  // a NaN among the scores stays one
+        if (tid < rows && write) {
+          const float lse = s == 0.f ? -INFINITY : (my_m + __log2f(s)) * 0.6931471805599453f;
           if (whole)
-            p.lse[grow0 + j] = lse;
+            p.lse[grow0 + tid] = lse;
           else
-            P.parts.lse[slot + j] = lse;
-          if (w.starts) P.parts.row_info[grow0 + j] = info;
+            P.parts.lse[slot + tid] = lse;
+          if (w.starts) {
+            int32_t info = 0;
+            if (!w.ends) {
+              // the run that holds the unit's last tile
+              const Sched& sc = aux->sched;
+              const int64_t n_runs = min(static_cast<int64_t>(runs), sc.tiles);
+              const int64_t last = sc.begin + (it - w.n) + w.unit_tiles - 1;
+              const int64_t hi = ((last + 1) * n_runs + sc.tiles - 1) / sc.tiles - 1;
+              info = pack_info(run, static_cast<int>(hi) - run + 1, tid);
+            }
+            P.parts.row_info[grow0 + tid] = info;
+          }
         }
       }
+      meet();
       mbar_wait_warp(&aux->o_full, piece & 1);
       tc_fence_after();
+      // (few instructions: they run once or twice, fetching them is what takes time)
 #pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
-        uint32_t o[kN];
-        tmem_ld_row<kN>(tl + F::kColO + b * kN, o);
+      for (int j0 = 0; j0 < kN && j0 < rows; j0 += 4) {
+        uint32_t o[4][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) tmem_ld_32x32b_x4(tl + F::kColO + b * kN + j0, o[b]);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-          const float v = inv[j] == 0.f ? 0.f : __uint_as_float(o[j]) * inv[j];
-          if (j < rows && write) {
+        for (int j = 0; j < 4; ++j) {
+          const float inv = aux->inv[j0 + j];
+          if (j0 + j >= rows || !write) break;
+          uint16_t* to = static_cast<uint16_t*>(p.out) + (grow0 + j0 + j) * kLatentDim + tid;
+          float* part = P.parts.o + (slot + j0 + j) * kLatentDim + tid;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            const float v = inv == 0.f ? 0.f : __uint_as_float(o[b][j]) * inv;
             if (whole)
-              static_cast<uint16_t*>(p.out)[(grow0 + j) * kLatentDim + b * kTok + tid] =
-                  static_cast<uint16_t>(pack2<kFp16>(v, 0.f));
+              to[b * 128] = static_cast<uint16_t>(pack2<kFp16>(v, 0.f));
             else
-              P.parts.o[(slot + j) * kLatentDim + b * kTok + tid] = v;
+              part[b * 128] = v;
           }
         }
       }
@@ -429,15 +468,15 @@ cudaError_t launch(const LatentDecodeLaunch& p, void* workspace, cudaStream_t st
   Params P;
   P.L = p;
   P.parts = partials<kN>(p, bound, workspace);
-  P.box_rows = std::min(p.block_size, kTok);
-  // cache rows as 9 groups of 64 values; a load is one group of one page (at most 128 rows). A cache without pages: a
-  // map over one row that nothing in bounds reads.
+  // cache rows as 9 groups of 64 values; a load is eight rows of one page and a part's groups. A cache without pages:
+  // a map over one row that nothing in bounds reads.
   const uint64_t pool_rows = std::max<uint64_t>(1, static_cast<uint64_t>(p.num_blocks) * p.block_size);
   const void* base = p.num_blocks > 0 ? p.cache : p.query;
   const uint64_t extent[3] = {64, pool_rows, 9}, stride[2] = {kLatentRow * 2, 128};
   const uint64_t extent_q[3] = {64, static_cast<uint64_t>(p.num_tokens) * p.num_heads, 9};
-  const uint32_t box[3] = {64, static_cast<uint32_t>(P.box_rows), 1}, box_q[3] = {64, kN, 9};
-  if (!encode_tmap_nd(&P.map, base, 3, extent, stride, box) || !encode_tmap_nd(&P.map_q, p.query, 3, extent_q, stride, box_q))
+  const uint32_t box_a[3] = {64, kBox, Few<kN>::kGroupsA}, box_b[3] = {64, kBox, Few<kN>::kGroupsB}, box_q[3] = {64, kN, 9};
+  if (!encode_tmap_nd(&P.map_a, base, 3, extent, stride, box_a) || !encode_tmap_nd(&P.map_b, base, 3, extent, stride, box_b) ||
+      !encode_tmap_nd(&P.map_q, p.query, 3, extent_q, stride, box_q))
     return cudaErrorInvalidValue;
   auto kern = latent_decode_few_kernel<kFp16, kN>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), Few<kN>::kSmem);
