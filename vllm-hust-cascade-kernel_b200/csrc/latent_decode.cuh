@@ -160,54 +160,53 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
 }
 
 // Merges the partials of the rows whose unit was cut, in run order, weights
-// exp(lse_i - max): one warp per row and 512 / kParts of its columns. Bound by
-// the chain row info -> partials (and log-sum-exps), so a lane loads kDepth
-// pieces before it adds the first. Few rows: four warps per row, twelve pieces
-// in flight (16 rows of 11 pieces: 17.5 us for the call, 19.1 with one warp and
-// two pieces); many rows have two or three pieces each, and one warp with four
-// (16,384 rows: 213 us for the call, 232 with four and twelve).
+// exp(lse_i - max): kWarps warps per row take every kWarps-th piece, four in
+// flight each, and their sums meet in shared memory. Bound by the chain row info
+// -> partials and log-sum-exps. Few rows (they may have a piece per run) get eight
+// warps, many rows, with two or three pieces each, one.
 constexpr int64_t kFewRows = 1024;
-template <bool kFp16, int kRows, int kParts, int kDepth>
+template <bool kFp16, int kRows, int kWarps>
 __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_constant__ LatentDecodeLaunch L,
                                                              const __grid_constant__ Partials P, int clusters) {
+  constexpr int kDepth = 4, kVec = 4;  // pieces in flight, float4 of a piece per lane
+  __shared__ float4 part[kWarps == 1 ? 1 : 8][kLatentDim / 4];
+  __shared__ float part_sum[8];
   pdl_wait();
-  constexpr int kVec = 4 / kParts;  // float4 of a piece per lane
-  const int64_t job = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t row = job / kParts;
-  const int lane = threadIdx.x & 31, part = static_cast<int>(job % kParts);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 8 + warp) / kWarps;
   if (row >= L.num_tokens * L.num_heads) return;
   const int32_t info = P.row_info[row];
   const int count = info >> 17, c0 = (info >> 7) & 1023, r = info & 127;
   // rows of a call whose query lengths do not add up hold no info: nothing past the slots is read for them
   if (count < 2 || c0 + count > clusters) return;
   auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRows + r; };
-  // the first 32 pieces' weights, one per lane
-  const float mine = lane < count ? P.lse[slot(lane)] : -INFINITY;
+  const int first = kWarps == 1 ? 0 : warp;
   float4 v[kDepth][kVec];
-  auto read = [&](int first) {
+  float lse[kDepth];
+  auto read = [&](int i0) {
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
-      if (first + d >= count) break;
-      const float4* src = reinterpret_cast<const float4*>(P.o + slot(first + d) * kLatentDim) + part * kVec * 32 + lane;
+      const int i = i0 + d * kWarps;
+      if (i >= count) break;
+      lse[d] = P.lse[slot(i)];
+      const float4* src = reinterpret_cast<const float4*>(P.o + slot(i) * kLatentDim) + lane;
 #pragma unroll
       for (int k = 0; k < kVec; ++k) v[d][k] = src[32 * k];
     }
   };
-  read(0);
-  float top = mine;
-  for (int i = lane + 32; i < count; i += 32) top = fmaxf(top, P.lse[slot(i)]);
+  read(first);
+  float top = -INFINITY;
+  for (int i = lane; i < count; i += 32) top = fmaxf(top, P.lse[slot(i)]);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   float4 acc[kVec] = {};
   float sum = 0.f;
-  for (int first = 0; first < count; first += kDepth) {
-    if (first > 0) read(first);
+  for (int i0 = first; i0 < count; i0 += kDepth * kWarps) {
+    if (i0 > first) read(i0);
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
-      const int i = first + d;
-      if (i >= count) break;
-      const float lse = i < 32 ? __shfl_sync(0xffffffffu, mine, i) : P.lse[slot(i)];
-      const float wgt = lse == -INFINITY ? 0.f : __expf(lse - top);
+      if (i0 + d * kWarps >= count) break;
+      const float wgt = lse[d] == -INFINITY ? 0.f : __expf(lse[d] - top);
       sum += wgt;
 #pragma unroll
       for (int k = 0; k < kVec; ++k) {
@@ -218,12 +217,33 @@ __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_consta
       }
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  uint2* dst = reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + row * kLatentDim) + part * kVec * 32 + lane;
+  uint2* out = reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + row * kLatentDim);
+  auto write = [&](int at, float4 a, float inv) {
+    out[at] = make_uint2(pack2<kFp16>(a.x * inv, a.y * inv), pack2<kFp16>(a.z * inv, a.w * inv));
+  };
+  if constexpr (kWarps == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int k = 0; k < kVec; ++k)
-    dst[32 * k] = make_uint2(pack2<kFp16>(acc[k].x * inv, acc[k].y * inv), pack2<kFp16>(acc[k].z * inv, acc[k].w * inv));
-  if (lane == 0 && part == 0) L.lse[row] = sum == 0.f ? -INFINITY : top + __logf(sum);
+    for (int k = 0; k < kVec; ++k) write(32 * k + lane, acc[k], inv);
+  } else {  // (the block has one row, all its warps are here)
+#pragma unroll
+    for (int k = 0; k < kVec; ++k) part[warp][32 * k + lane] = acc[k];
+    if (lane == 0) part_sum[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += part_sum[i];
+    if (threadIdx.x < kLatentDim / 4) {
+      float4 a = part[0][threadIdx.x];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        const float4 b = part[i][threadIdx.x];
+        a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
+      }
+      write(threadIdx.x, a, sum == 0.f ? 0.f : 1.f / sum);
+    }
+  }
+  if (threadIdx.x % (32 * kWarps) == 0) L.lse[row] = sum == 0.f ? -INFINITY : top + __logf(sum);
 }
 
 inline size_t info_bytes(const LatentDecodeLaunch& p) {
@@ -256,7 +276,7 @@ cudaError_t launch_combine(const LatentDecodeLaunch& p, const Partials& parts, i
   const int64_t rows = p.num_tokens * p.num_heads;
   const bool few = rows <= kFewRows;
   cudaLaunchConfig_t cc = {};
-  cc.gridDim = dim3(static_cast<unsigned>((rows * (few ? 4 : 1) + 7) / 8));
+  cc.gridDim = dim3(static_cast<unsigned>(few ? rows : (rows + 7) / 8));
   cc.blockDim = dim3(256);
   cc.stream = stream;
   cudaLaunchAttribute pdl[1];
@@ -264,8 +284,8 @@ cudaError_t launch_combine(const LatentDecodeLaunch& p, const Partials& parts, i
   pdl[0].val.programmaticStreamSerializationAllowed = 1;
   cc.attrs = pdl;
   cc.numAttrs = 1;
-  return few ? cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, kRows, 4, 12>, p, parts, runs)
-             : cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, kRows, 1, 4>, p, parts, runs);
+  return few ? cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, kRows, 8>, p, parts, runs)
+             : cudaLaunchKernelEx(&cc, latent_combine_kernel<kFp16, kRows, 1>, p, parts, runs);
 }
 
 }  // namespace
