@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
             uint8_t* stage = smem + (hh == c ? kOffB + it % kStagesB * kBytesV : kOffC + it % kStagesC * kBytesV);
             uint4* v = reinterpret_cast<uint4*>(stage + (warp & 3) * kGroup + lane * 128);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = make_uint4(0u, 0u, 0u, 0u);
+            for (int q = 0; q < 8; ++q) v[q ^ (lane & 7)] = make_uint4(0u, 0u, 0u, 0u);
           }
         }
         fence_proxy_async_smem();
@@ -560,16 +560,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         else
           P.parts.lse[(2 * cluster + (w.starts ? 1 : 0)) * kRows + r] = lse;
         if (w.starts) {
-          int32_t info = 0;
-          if (!w.ends) {
-            // the run that holds the unit's last tile
-            const Sched& sc = aux->sched;
-            const int64_t runs = min(static_cast<int64_t>(clusters), sc.tiles);
-            const int64_t last = sc.begin + (it - w.n) + w.unit_tiles - 1;
-            const int64_t hi = ((last + 1) * runs + sc.tiles - 1) / sc.tiles - 1;
-            info = pack_info(cluster, static_cast<int>(hi) - cluster + 1, r);
-          }
-          P.parts.row_info[grow] = info;
+          P.parts.row_info[grow] =
+              w.ends ? 0 : cut_info(aux->sched, cluster, aux->sched.begin + (it - w.n), w.unit_tiles, r);
         }
       }
       if (last) {

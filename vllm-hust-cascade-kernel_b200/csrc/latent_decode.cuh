@@ -20,7 +20,9 @@ struct Sched {
   int64_t tiles, begin;  // all tiles; this cluster's first
   int64_t tok;           // first query token of request b
   int b, mt, t0, left;
-  int q, kv;               // request b's lengths
+  int q, kv;             // request b's lengths
+  int64_t each;          // tiles of a run; `rest` runs of all have one more
+  int rest, runs;
 };
 
 // row_info of a unit cut into `count` >= 2 pieces, the first in run `c`: row r
@@ -37,8 +39,8 @@ struct Unit {
     return p.q_len > 0 ? p.q_len
                        : static_cast<int>(min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens));
   }
-  __device__ __forceinline__ int kv_len(int b) const {
-    return static_cast<int>(min(max(p.kv_lens[b], static_cast<int64_t>(0)), static_cast<int64_t>(1 << 30)));
+  static __device__ __forceinline__ int kv_len(int64_t n) {
+    return static_cast<int>(min(max(n, static_cast<int64_t>(0)), static_cast<int64_t>(1 << 30)));
   }
   __device__ __forceinline__ int row_tiles(int q) const {
     return static_cast<int>((static_cast<int64_t>(q) * p.num_heads + kRows - 1) / kRows);
@@ -64,18 +66,18 @@ struct Walk {
   bool starts, ends;
   int unit_tiles;
 
-  int next_b, next_mt, next_t0, left, nq, nkv;
-  int64_t next_tok;
+  int next_b, next_mt, next_t0, left, nq;
+  int64_t next_tok, nkv;  // (nkv as loaded: it is not used, and so not waited for, until the next piece)
 
   __device__ Walk(const LatentDecodeLaunch& l, const Sched& s)
       : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), left(s.left), nq(s.q), nkv(s.kv), next_tok(s.tok) {}
   __device__ __forceinline__ void load() {
     nq = u.q_len(next_b);
-    nkv = u.kv_len(next_b);
+    nkv = u.p.kv_lens[next_b];
   }
   __device__ __forceinline__ bool next() {
     if (left <= 0) return false;
-    b = next_b, mt = next_mt, t0 = next_t0, q = nq, kv = nkv, tok = next_tok;
+    b = next_b, mt = next_mt, t0 = next_t0, q = nq, kv = u.kv_len(nkv), tok = next_tok;
     unit_tiles = u.tiles(q, kv, mt);
     n = min(left, unit_tiles - t0);
     starts = t0 == 0;
@@ -100,6 +102,22 @@ struct Walk {
   }
 };
 
+// First tile of run c: floor(c total / runs), without a wide division.
+__device__ __forceinline__ int64_t run_begin(int c, int64_t each, int rest, int runs) {
+  return c * each + static_cast<uint32_t>(c * rest) / static_cast<uint32_t>(runs);
+}
+
+// row_info of row r of a unit whose first piece is this run's, of `unit_tiles`
+// tiles from `first` on (of all tiles): finds the run that holds its last tile.
+__device__ __forceinline__ int32_t cut_info(const Sched& s, int run, int64_t first, int unit_tiles, int r) {
+  const int64_t last = first + unit_tiles - 1;
+  int hi = run + static_cast<int>(min(static_cast<float>(s.runs - 1 - run),
+                                      static_cast<float>(last - s.begin) / static_cast<float>(s.each + (s.rest > 0))));
+  while (hi + 1 < s.runs && run_begin(hi + 1, s.each, s.rest, s.runs) <= last) ++hi;
+  while (hi > run && run_begin(hi, s.each, s.rest, s.runs) > last) --hi;
+  return pack_info(run, hi - run + 1, r);
+}
+
 // Finds this cluster's run: the block sums the units' tiles (and the query
 // tokens) per contiguous chunk of requests, then the thread whose chunk holds
 // the run's first tile walks to it.
@@ -112,7 +130,7 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
   const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
   int64_t tiles = 0, toks = 0;
   for (int b = b0; b < b1; ++b) {
-    const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
+    const int q = u.q_len(b), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
     for (int mt = 0; mt < m; ++mt) tiles += u.tiles(q, kv, mt);
     toks += q;
   }
@@ -132,21 +150,20 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
   }
   const int64_t runs = min(static_cast<int64_t>(clusters), total);
   if (cluster < runs) {
-    // floor(cluster total / runs) and floor((cluster + 1) total / runs), with one wide division
     const int n_runs = static_cast<int>(runs);
     const int64_t each = total >> 31 ? total / runs : static_cast<uint32_t>(total) / static_cast<uint32_t>(n_runs);
     const int rest = static_cast<int>(total - each * runs);
-    const int64_t begin = cluster * each + cluster * rest / n_runs;
-    const int64_t end = (cluster + 1) * each + (cluster + 1) * rest / n_runs;
+    const int64_t begin = run_begin(cluster, each, rest, n_runs), end = run_begin(cluster + 1, each, rest, n_runs);
     int64_t at = st - tiles;
     if (begin >= at && begin < st) {
       int64_t tok = sq - toks;
       for (int b = b0; b < b1; ++b) {
-        const int q = u.q_len(b), kv = u.kv_len(b), m = u.row_tiles(q);
+        const int q = u.q_len(b), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
         for (int mt = 0; mt < m; ++mt) {
           const int t = u.tiles(q, kv, mt);
           if (begin < at + t) {
-            *sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin), q, kv};
+            *sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin), q, kv,
+                      each, rest, n_runs};
             b = b1;
             break;
           }

@@ -20,8 +20,9 @@
 // slot, an SM's share of HBM 3,250 for its 74 KB. (Tiles of 128 tokens leave
 // 48 KB to be on their way.)
 //
-// Warps: 0-3 softmax and output, 4 cache loads, 5 MMA issue, 6 query loads.
+// Warps: 0-3 softmax and output (a piece's after the next one's first tile), 4 cache loads, 5 MMA issue, 6 query loads.
 #include <algorithm>
+#include <climits>
 
 #include "latent_decode.cuh"
 
@@ -44,12 +45,13 @@ struct Few {
   static constexpr int kRowBytes = kN * 2;  // of P: a token's weights
   static constexpr int kOffQ = 0;
   static constexpr int kOffP = kOffQ + 9 * kQGroup;
-  static constexpr int kOffA = kOffP + kTok * kRowBytes;
+  static constexpr int kBytesP = kTok * kRowBytes;
+  static constexpr int kOffA = kOffP + 2 * kBytesP;
   static constexpr int kOffB = kOffA + kSlotsA * kBytesA;
   static constexpr int kTiles = kOffB + kSlotsB * kBytesB;
-  static constexpr int kColS = 0, kColO = kN;  // TMEM columns
-  static constexpr int kTmem = kN == 16 ? 128 : 256;
-  static_assert(kColO + 4 * kN <= kTmem && kOffP % 1024 == 0 && kOffA % 1024 == 0, "layout");
+  static constexpr int kColS = 0, kColO = 2 * kN;  // TMEM columns: scores of two tiles, outputs of two pieces
+  static constexpr int kTmem = kN == 16 ? 256 : 512;
+  static_assert(kColO + 8 * kN <= kTmem && kOffP % 1024 == 0 && kOffA % 1024 == 0, "layout");
   static_assert(kGroupsA % 2 == 0, "an M block of the second product lies in one part");
 
   struct __align__(16) Aux {
@@ -61,7 +63,7 @@ struct Few {
     float inv[kN];  // 1 / the rows' sums
     int lim[kN];  // tokens that a row sees
     uint64_t a_full[kSlotsA], b_full[kSlotsB], pv_done[kSlotsA];
-    uint64_t q_full, q_free, s_full, p_full, o_full, stall, drain;
+    uint64_t q_full, q_free, s_full[2], p_full[2], o_full[2], stall, drain;
     uint32_t tmem_base;
     Sched sched;
   };
@@ -142,9 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     for (int s = 0; s < F::kSlotsB; ++s) mbar_init(&aux->b_full[s], 1);
     mbar_init(&aux->q_full, 1);
     mbar_init(&aux->q_free, 1);
-    mbar_init(&aux->s_full, 1);
-    mbar_init(&aux->p_full, 4);
-    mbar_init(&aux->o_full, 1);
+    for (int s = 0; s < 2; ++s) mbar_init(&aux->o_full[s], 1), mbar_init(&aux->s_full[s], 1), mbar_init(&aux->p_full[s], 4);
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
@@ -163,20 +163,24 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
 
   if (warp == 4) {
     // ---------------------------------------------------------- cache loads
+    // Lane i takes care of the i-th eight rows of four tiles; their page ids are read four tiles (or a piece) ahead.
     const int oob = max(1, p.num_blocks * p.block_size);
-    int it = 0;
-    bool live = true;
-    while (live && w.next()) {
-      const int32_t* bt = p.block_table + static_cast<int64_t>(w.b) * p.block_cols;
-      const int pages = (min(w.kv, w.u.cap) + p.block_size - 1) / p.block_size;
-      // lane i holds the pool row of the i-th eight rows from tile t on: four tiles' worth
-      int y = oob;
-      for (int t = w.t0; t < w.t0 + w.n; ++t, ++it) {
-        const int ahead = (t - w.t0) & 3;
-        if (ahead == 0) {
-          const int tok = t * kTok + lane * kBox, page = tok / p.block_size;
-          y = page < pages ? paged_row(bt[page], tok, p.block_size, p.num_blocks, oob) : oob;
-        }
+    constexpr int kNoPage = INT_MIN;
+    auto first_row = [&](int t) { return t * kTok + lane * kBox; };
+    auto page_id = [&](const Walk<kN, kTok>& x, int t) {
+      const int pages = (min(x.kv, x.u.cap) + p.block_size - 1) / p.block_size, page = first_row(t) / p.block_size;
+      return page < pages ? p.block_table[static_cast<int64_t>(x.b) * p.block_cols + page] : kNoPage;
+    };
+    int it = 0, id_next = kNoPage, y = oob;
+    bool live = true, more = w.next();
+    if (more) id_next = page_id(w, w.t0);
+    while (live && more) {
+      const int t0 = w.t0, t1 = w.t0 + w.n;
+      const Walk<kN, kTok> now = w;
+      more = false;
+      for (int t = t0; t < t1; ++t, ++it) {
+        const int ahead = (t - t0) & 3;
+        if (ahead == 0) y = id_next == kNoPage ? oob : paged_row(id_next, first_row(t), p.block_size, p.num_blocks, oob);
         const int row = __shfl_sync(0xffffffffu, y, ahead * kBoxes + (lane & (kBoxes - 1)));
         const int sa = it % F::kSlotsA, sb = it % F::kSlotsB;
         // P V of the tile that had the slot is done
@@ -198,6 +202,12 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
           tma_load_3d(smem + F::kOffB + sb * F::kBytesB + lane * F::kGroupsB * kAtom, &P.map_b, &aux->b_full[sb], 0, row,
                       F::kGroupsA);
         __syncwarp();
+        if (ahead == 0) {
+          if (t + 4 < t1)
+            id_next = page_id(now, t + 4);
+          else if ((more = w.next()))
+            id_next = page_id(w, w.t0);
+        }
       }
     }
   } else if (warp == 5) {
@@ -208,59 +218,88 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     const uint64_t dq = make_smem_desc(s0 + F::kOffQ, 16, 1024, 2);
     // P: a token's kN weights in a row of 32 (64) bytes, swizzled in as many
     const uint64_t dp = make_smem_desc(s0 + F::kOffP, 16, 8 * F::kRowBytes, kN == 16 ? 6 : 4);
-    int it = 0, piece = 0;
-    bool live = true;
-    while (live && w.next()) {
-      live = mbar_wait_warp(&aux->q_full, piece & 1);
-      for (int t = 0; live && t < w.n; ++t, ++it) {
-        const uint32_t u = uniform(it), sa = u % F::kSlotsA, sb = u % F::kSlotsB;
-        const uint32_t a = s0 + F::kOffA + sa * F::kBytesA, b = s0 + F::kOffB + sb * F::kBytesB;
-        // groups [g0, g1) of a part whose boxes are `pitch` bytes apart
-        auto scores = [&](uint32_t part, int pitch, int g0, int g1) {
-          const uint64_t da = make_smem_desc(part, 16, pitch, 2);
-          tc_fence_after();
-          __syncwarp();
-          if (elect_one()) {
-#pragma unroll 1
-            for (int g = g0; g < g1; ++g) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16_ss(tm + F::kColS, da + (g - g0) * kAtom / 16 + k * 2, dq + g * F::kQGroup / 16 + k * 2, idesc_s,
-                            g + k > 0);
-            }
-            if (g1 == 9) {
-              umma_commit(&aux->s_full);
-              if (t + 1 == w.n) umma_commit(&aux->q_free);
-            }
-          }
-          __syncwarp();
-        };
-        live = mbar_wait_warp(&aux->a_full[sa], (u / F::kSlotsA) & 1);
-        if (!live) break;
-        scores(a, F::kGroupsA * kAtom, 0, F::kGroupsA);
-        live = mbar_wait_warp(&aux->b_full[sb], (u / F::kSlotsB) & 1);
-        if (!live) break;
-        scores(b, F::kGroupsB * kAtom, F::kGroupsA, 9);
-        live = mbar_wait_warp(&aux->p_full, u & 1);
-        if (!live) break;
+    // One tile's P V is owed at any time. The next tile's scores go before it if their data is there by then (the
+    // softmax takes as long as a product), else after it, so that its slots do not wait for loads.
+    int it = 0, piece = 0, t = 0;  // the next tile to score
+    bool more = w.next(), live = true;
+    auto ready = [&] {
+      return __all_sync(0xffffffffu, (t > 0 || mbar_test(&aux->q_full, piece & 1)) &&
+                                         mbar_test(&aux->a_full[it % F::kSlotsA], (it / F::kSlotsA) & 1) &&
+                                         mbar_test(&aux->b_full[it % F::kSlotsB], (it / F::kSlotsB) & 1));
+    };
+    auto score = [&] {
+      const uint32_t u = uniform(it), sa = u % F::kSlotsA, sb = u % F::kSlotsB;
+      const bool last = t + 1 == w.n;
+      // groups [g0, g1) of a part whose boxes are `pitch` bytes apart
+      auto groups = [&](uint32_t part, int pitch, int g0, int g1) {
+        const uint64_t da = make_smem_desc(part, 16, pitch, 2);
+        const uint32_t d = tm + F::kColS + (u & 1) * kN;
         tc_fence_after();
         __syncwarp();
         if (elect_one()) {
 #pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            const bool in_a = 2 * j < F::kGroupsA;
-            const int pitch = (in_a ? F::kGroupsA : F::kGroupsB) * kAtom;
-            const uint64_t dv = make_smem_desc((in_a ? a + 2 * j * kAtom : b + (2 * j - F::kGroupsA) * kAtom), kAtom, pitch, 2);
+          for (int g = g0; g < g1; ++g) {
 #pragma unroll
-            for (int k = 0; k < kTok / 16; ++k)
-              umma_f16_ss(tm + F::kColO + j * kN, dv + k * 2 * pitch / 16, dp + k * 16 * F::kRowBytes / 16, idesc_o, t + k > 0);
+            for (int k = 0; k < 4; ++k)
+              umma_f16_ss(d, da + (g - g0) * kAtom / 16 + k * 2, dq + g * F::kQGroup / 16 + k * 2, idesc_s, g + k > 0);
           }
-          umma_commit(&aux->pv_done[sa]);
-          if (t + 1 == w.n) umma_commit(&aux->o_full);
+          if (g1 == 9) {
+            umma_commit(&aux->s_full[u & 1]);
+            if (last) umma_commit(&aux->q_free);
+          }
         }
         __syncwarp();
+      };
+      live = live && (t > 0 || mbar_wait_warp(&aux->q_full, piece & 1)) &&
+             mbar_wait_warp(&aux->a_full[sa], (u / F::kSlotsA) & 1);
+      if (live) groups(s0 + F::kOffA + sa * F::kBytesA, F::kGroupsA * kAtom, 0, F::kGroupsA);
+      live = live && mbar_wait_warp(&aux->b_full[sb], (u / F::kSlotsB) & 1);
+      if (live) groups(s0 + F::kOffB + sb * F::kBytesB, F::kGroupsB * kAtom, F::kGroupsA, 9);
+      ++it;
+      if (last) {
+        t = 0;
+        ++piece;
+        more = w.next();
+      } else {
+        ++t;
       }
-      ++piece;
+    };
+    auto value = [&](int tile, int of, bool first, bool last) {
+      const uint32_t u = uniform(tile), sa = u % F::kSlotsA, sb = u % F::kSlotsB, o = uniform(of & 1);
+      const uint32_t a = s0 + F::kOffA + sa * F::kBytesA, b = s0 + F::kOffB + sb * F::kBytesB;
+      live = live && mbar_wait_warp(&aux->p_full[u & 1], (u >> 1) & 1);
+      if (!live) return;
+      tc_fence_after();
+      __syncwarp();
+      if (elect_one()) {
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) {
+          const bool in_a = 2 * j < F::kGroupsA;
+          const int pitch = (in_a ? F::kGroupsA : F::kGroupsB) * kAtom;
+          const uint64_t dv = make_smem_desc((in_a ? a + 2 * j * kAtom : b + (2 * j - F::kGroupsA) * kAtom), kAtom, pitch, 2);
+#pragma unroll
+          for (int k = 0; k < kTok / 16; ++k)
+            umma_f16_ss(tm + F::kColO + (o * 4 + j) * kN, dv + k * 2 * pitch / 16,
+                        dp + (u & 1) * F::kBytesP / 16 + k * 16 * F::kRowBytes / 16, idesc_o, !first || k > 0);
+        }
+        umma_commit(&aux->pv_done[sa]);
+        if (last) umma_commit(&aux->o_full[o]);
+      }
+      __syncwarp();
+    };
+    if (more) score();
+    for (int n = 0, of = 0, done = 0; live && n < it; ++n) {
+      // tile n is number `done` of piece `of`; the last one if the tile after it is a first one
+      const bool last = t == 0;
+      if (more && ready()) {
+        score();
+        value(n, of, done == 0, last);
+      } else {
+        value(n, of, done == 0, last);
+        if (more && live) score();
+      }
+      done = last ? 0 : done + 1;
+      of += last;
     }
     if (!live && lane == 0) {
       umma_commit(&aux->drain);
@@ -269,7 +308,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
   } else if (warp == 6) {
     // ---------------------------------------------------------- query loads
     for (int piece = 0; w.next(); ++piece) {
-      if (piece > 0 && !mbar_wait_warp(&aux->q_free, (piece - 1) & 1)) break;
+      if (piece > 0) {
+        if (lane == 0) tma_prefetch_3d(&P.map_q, 0, static_cast<int>(w.tok * p.num_heads + w.mt * kN), 0);
+        if (!mbar_wait_warp(&aux->q_free, (piece - 1) & 1)) break;
+      }
       if (lane == 0) {
         mbar_arrive_expect_tx(&aux->q_full, 9 * F::kQGroup);
         tma_load_3d(smem + F::kOffQ, &P.map_q, &aux->q_full, 0, static_cast<int>(w.tok * p.num_heads + w.mt * kN), 0);
@@ -285,20 +327,35 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     const int mine = warp * 16 + lane;  // token of the tile: 64 rows of scores lie in the first 16 lanes of each quarter
     const int my_col = tid & (kN - 1);
     if (p.debug_stall) mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
-    int it = 0, piece = 0;
-    while (w.next()) {
-      const int row0 = w.mt * kN, valid = min(w.kv, w.u.cap);
-      const int clean = w.u.limit(w.q, w.kv, row0 / p.num_heads) / kTok;  // tiles below are seen in full by every row
-      if (tid < kN) aux->lim[tid] = w.u.limit(w.q, w.kv, min((row0 + tid) / p.num_heads, w.q - 1));
-      meet();
-      float m[kN], l[kN], my_m = -INFINITY;  // my_m: row my_col's
+    float m[kN], l[kN], my_m = -INFINITY;  // my_m: row my_col's
+    // A piece's output is written after the next piece's first P: the products go on meanwhile, into the other
+    // accumulator.
+    struct {
+      int64_t grow0, slot, first;
+      int rows, unit_tiles;
+      bool starts, ends;
+      float m;
+    } done = {};
+    int it = 0, piece = 0, t = 0;
+    int valid = 0, clean = 0;  // tokens that hold anything; tiles below `clean` are seen in full by every row
+    bool more = w.next(), start = true, pending = false;
+    while (true) {
+      if (more) {
+        if (start) {
+          const int row0 = w.mt * kN;
+          valid = min(w.kv, w.u.cap);
+          clean = w.u.limit(w.q, w.kv, row0 / p.num_heads) / kTok;
+          if (tid < kN) aux->lim[tid] = w.u.limit(w.q, w.kv, min((row0 + tid) / p.num_heads, w.q - 1));
+          meet();
 #pragma unroll
-      for (int j = 0; j < kN; ++j) m[j] = -INFINITY, l[j] = 0.f;
-      for (int t = w.t0; t < w.t0 + w.n; ++t, ++it) {
-        mbar_wait_warp(&aux->s_full, it & 1);
+          for (int j = 0; j < kN; ++j) m[j] = -INFINITY, l[j] = 0.f;
+          my_m = -INFINITY;
+          t = w.t0;
+        }
+        mbar_wait_warp(&aux->s_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
         uint32_t x[kN];
-        tmem_ld_row<kN>(tl + F::kColS, x);
+        tmem_ld_row<kN>(tl + F::kColS + (it & 1) * kN, x);
         tmem_wait_ld();
         const int tok = t * kTok + mine;
         if (lane >= 16) {
@@ -333,20 +390,22 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
             if (up) m[j] = mx;
             l[j] *= dm[j];
           }
-          if (t > w.t0) {  // the scores came after the last tile's P V: the output is at rest
+          if (!start) {
+            mbar_wait_warp(&aux->pv_done[(it - 1) % F::kSlotsA], ((it - 1) / F::kSlotsA) & 1);  // the output is at rest
+            tc_fence_after();
 #pragma unroll 1
             for (int b = 0; b < 4; ++b) {
               uint32_t o[kN];
-              tmem_ld_row<kN>(tl + F::kColO + b * kN, o);
+              tmem_ld_row<kN>(tl + F::kColO + ((piece & 1) * 4 + b) * kN, o);
               tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < kN; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * dm[j]);
-              tmem_st_row<kN>(tl + F::kColO + b * kN, o);
+              tmem_st_row<kN>(tl + F::kColO + ((piece & 1) * 4 + b) * kN, o);
             }
             tmem_wait_st();
           }
         }
-        // P over the last tile's, which its product has read by now
+        // P over that of two tiles ago: its product came before these scores
         uint32_t pk[kN / 2];
 #pragma unroll
         for (int j = 0; j < kN; j += 2) {
@@ -360,93 +419,99 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
           pk[j / 2] = pack2<kFp16>(y[0], y[1]);
         }
         if (lane < 16) {
-          uint8_t* dst = smem + F::kOffP + mine * F::kRowBytes;
+          uint8_t* dst = smem + F::kOffP + (it & 1) * F::kBytesP + mine * F::kRowBytes;
           const int swap = kN == 16 ? (mine >> 2) & 1 : (mine >> 1) & 3;
 #pragma unroll
           for (int q = 0; q < kN / 8; ++q)
             *reinterpret_cast<uint4*>(dst + ((q ^ swap) << 4)) =
                 make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
-          if (tok >= valid) {
-            // rows past the request's length may hold NaN: weight 0 does not hide
-            // them from the product, so they are cleared (the scores have read them)
+        }
+        if ((t + 1) * kTok > valid) {
+          // rows past the request's length may hold NaN: weight 0 does not hide
+          // them from the product, so they are cleared (the scores have read them);
+          // two lanes per row, eight rows' 16-byte chunks in different banks
+          const int r = warp * 16 + (lane & 15);
+          if (t * kTok + r >= valid) {
 #pragma unroll 1
-            for (int g = 0; g < 8; ++g) {
-              uint8_t* at = g < F::kGroupsA ? smem + F::kOffA + it % F::kSlotsA * F::kBytesA + ((mine >> 3) * F::kGroupsA + g) * kAtom
-                                            : smem + F::kOffB + it % F::kSlotsB * F::kBytesB +
-                                                  ((mine >> 3) * F::kGroupsB + g - F::kGroupsA) * kAtom;
+            for (int g = lane >> 4; g < 8; g += 2) {
+              uint8_t* at = g < F::kGroupsA
+                                ? smem + F::kOffA + it % F::kSlotsA * F::kBytesA + ((r >> 3) * F::kGroupsA + g) * kAtom
+                                : smem + F::kOffB + it % F::kSlotsB * F::kBytesB +
+                                      ((r >> 3) * F::kGroupsB + g - F::kGroupsA) * kAtom;
 #pragma unroll
               for (int q = 0; q < 8; ++q)
-                *reinterpret_cast<uint4*>(at + (mine & 7) * 128 + q * 16) = make_uint4(0u, 0u, 0u, 0u);
+                *reinterpret_cast<uint4*>(at + (r & 7) * 128 + ((q ^ (r & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
             }
           }
         }
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->p_full);
+        if (lane == 0) mbar_arrive(&aux->p_full[it & 1]);
+        ++it;
       }
-      // the rows' sums, added in one order by all
-      int col;
-      const float sum = reduce_columns<kN>(l, lane, col, [](float a, float b) { return a + b; });
-      aux->sum[warp][col] = sum;
-      meet();
-      const int64_t grow0 = w.tok * p.num_heads + row0;
-      const int rows = static_cast<int>(min(static_cast<int64_t>(kN), min(static_cast<int64_t>(w.q) * p.num_heads - row0,
-                                                                        p.num_tokens * p.num_heads - grow0)));
-      const bool whole = w.starts && w.ends;
-      const int64_t slot = (2 * run + (w.starts ? 1 : 0)) * kN;
-      const bool write = !cta_aborted();
-      if (tid < kN) {
-        const float s = (aux->sum[0][tid] + aux->sum[1][tid]) + (aux->sum[2][tid] + aux->sum[3][tid]);
-        aux->inv[tid] = s == 0.f ? 0.f : 1.f / s;  // a NaN among the scores stays one
-        if (tid < rows && write) {
-          const float lse = s == 0.f ? -INFINITY : (my_m + __log2f(s)) * 0.6931471805599453f;
-          if (whole)
-            p.lse[grow0 + tid] = lse;
-          else
-            P.parts.lse[slot + tid] = lse;
-          if (w.starts) {
-            int32_t info = 0;
-            if (!w.ends) {
-              // the run that holds the unit's last tile
-              const Sched& sc = aux->sched;
-              const int64_t n_runs = min(static_cast<int64_t>(runs), sc.tiles);
-              const int64_t last = sc.begin + (it - w.n) + w.unit_tiles - 1;
-              const int64_t hi = ((last + 1) * n_runs + sc.tiles - 1) / sc.tiles - 1;
-              info = pack_info(run, static_cast<int>(hi) - run + 1, tid);
-            }
-            P.parts.row_info[grow0 + tid] = info;
+      if (pending) {
+        pending = false;
+        const bool whole = done.starts && done.ends;
+        meet();
+        if (tid < kN) {  // the rows' sums, added in one order
+          const float s = (aux->sum[0][tid] + aux->sum[1][tid]) + (aux->sum[2][tid] + aux->sum[3][tid]);
+          aux->inv[tid] = s == 0.f ? 0.f : 1.f / s;  // a NaN among the scores stays one
+          if (tid < done.rows && !cta_aborted()) {
+            const float lse = s == 0.f ? -INFINITY : (done.m + __log2f(s)) * 0.6931471805599453f;
+            (whole ? p.lse + done.grow0 : P.parts.lse + done.slot)[tid] = lse;
+            if (done.starts)
+              P.parts.row_info[done.grow0 + tid] =
+                  done.ends ? 0 : cut_info(aux->sched, run, done.first, done.unit_tiles, tid);
           }
         }
-      }
-      meet();
-      mbar_wait_warp(&aux->o_full, piece & 1);
-      tc_fence_after();
-      // (few instructions: they run once or twice, fetching them is what takes time)
+        meet();
+        const int o_buf = more ? (piece & 1) ^ 1 : piece & 1, at = more ? piece - 1 : piece;
+        const bool write = mbar_wait_warp(&aux->o_full[o_buf], (at >> 1) & 1);
+        tc_fence_after();
+        // (few instructions: they run once or twice, fetching them is what takes time)
 #pragma unroll 1
-      for (int j0 = 0; j0 < kN && j0 < rows; j0 += 4) {
-        uint32_t o[4][4];
+        for (int j0 = 0; j0 < kN && j0 < done.rows && write; j0 += 4) {
+          uint32_t o[4][4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) tmem_ld_32x32b_x4(tl + F::kColO + b * kN + j0, o[b]);
-        tmem_wait_ld();
+          for (int b = 0; b < 4; ++b) tmem_ld_32x32b_x4(tl + F::kColO + (o_buf * 4 + b) * kN + j0, o[b]);
+          tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float inv = aux->inv[j0 + j];
-          if (j0 + j >= rows || !write) break;
-          uint16_t* to = static_cast<uint16_t*>(p.out) + (grow0 + j0 + j) * kLatentDim + tid;
-          float* part = P.parts.o + (slot + j0 + j) * kLatentDim + tid;
+          for (int j = 0; j < 4; ++j) {
+            const float inv = aux->inv[j0 + j];
+            if (j0 + j >= done.rows) break;
+            uint16_t* to = static_cast<uint16_t*>(p.out) + (done.grow0 + j0 + j) * kLatentDim + tid;
+            float* part = P.parts.o + (done.slot + j0 + j) * kLatentDim + tid;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            const float v = inv == 0.f ? 0.f : __uint_as_float(o[b][j]) * inv;
-            if (whole)
-              to[b * 128] = static_cast<uint16_t>(pack2<kFp16>(v, 0.f));
-            else
-              part[b * 128] = v;
+            for (int b = 0; b < 4; ++b) {
+              const float v = inv == 0.f ? 0.f : __uint_as_float(o[b][j]) * inv;
+              if (whole)
+                to[b * 128] = static_cast<uint16_t>(pack2<kFp16>(v, 0.f));
+              else
+                part[b * 128] = v;
+            }
           }
         }
+        tc_fence_before();
       }
-      tc_fence_before();  // the next piece's first product comes after its P
-      ++piece;
+      if (!more) break;
+      start = ++t == w.t0 + w.n;
+      if (start) {
+        int col;
+        const float sum = reduce_columns<kN>(l, lane, col, [](float a, float b) { return a + b; });
+        aux->sum[warp][col] = sum;
+        pending = true;
+        done.grow0 = w.tok * p.num_heads + w.mt * kN;
+        done.slot = (2 * run + (w.starts ? 1 : 0)) * kN;
+        done.first = aux->sched.begin + (it - w.n);
+        done.rows = static_cast<int>(min(static_cast<int64_t>(kN), min(static_cast<int64_t>(w.q) * p.num_heads - w.mt * kN,
+                                                                      p.num_tokens * p.num_heads - done.grow0)));
+        done.unit_tiles = w.unit_tiles;
+        done.starts = w.starts, done.ends = w.ends;
+        done.m = my_m;
+        more = w.next();
+        if (more) ++piece;
+      }
     }
   }
   if (cta_aborted()) {

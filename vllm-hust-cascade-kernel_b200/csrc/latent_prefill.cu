@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
           uint8_t* chunk = slot_of(5 * j + 3 + (r >> 6)) + (r & 63) * 128;
 #pragma unroll
           for (int q = 0; q < 16; ++q)
-            *reinterpret_cast<uint4*>(chunk + (q >> 3) * (kChunk / 2) + (q & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(chunk + (q >> 3) * (kChunk / 2) + (((q ^ r) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
         }
         fence_proxy_async_smem();
       }
