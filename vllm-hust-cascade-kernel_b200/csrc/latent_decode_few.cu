@@ -46,10 +46,10 @@ struct Few {
   static constexpr int kOffQ = 0;
   static constexpr int kOffP = kOffQ + 9 * kQGroup;
   static constexpr int kBytesP = kTok * kRowBytes;
-  static constexpr int kOffA = kOffP + 2 * kBytesP;
+  static constexpr int kOffA = kOffP + kBytesP;
   static constexpr int kOffB = kOffA + kSlotsA * kBytesA;
   static constexpr int kTiles = kOffB + kSlotsB * kBytesB;
-  static constexpr int kColS = 0, kColO = 2 * kN;  // TMEM columns: scores of two tiles, outputs of two pieces
+  static constexpr int kColS = 0, kColO = kN;  // TMEM columns: scores, outputs of two pieces
   static constexpr int kTmem = kN == 16 ? 256 : 512;
   static_assert(kColO + 8 * kN <= kTmem && kOffP % 1024 == 0 && kOffA % 1024 == 0, "layout");
   static_assert(kGroupsA % 2 == 0, "an M block of the second product lies in one part");
@@ -63,7 +63,7 @@ struct Few {
     float inv[kN];  // 1 / the rows' sums
     int lim[kN];  // tokens that a row sees
     uint64_t a_full[kSlotsA], b_full[kSlotsB], pv_done[kSlotsA];
-    uint64_t q_full, q_free, s_full[2], p_full[2], o_full[2], stall, drain;
+    uint64_t q_full, q_free, s_full, p_full, o_full[2], stall, drain;
     uint32_t tmem_base;
     Sched sched;
   };
@@ -144,7 +144,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     for (int s = 0; s < F::kSlotsB; ++s) mbar_init(&aux->b_full[s], 1);
     mbar_init(&aux->q_full, 1);
     mbar_init(&aux->q_free, 1);
-    for (int s = 0; s < 2; ++s) mbar_init(&aux->o_full[s], 1), mbar_init(&aux->s_full[s], 1), mbar_init(&aux->p_full[s], 4);
+    for (int s = 0; s < 2; ++s) mbar_init(&aux->o_full[s], 1);
+    mbar_init(&aux->s_full, 1);
+    mbar_init(&aux->p_full, 4);
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
@@ -218,88 +220,61 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     const uint64_t dq = make_smem_desc(s0 + F::kOffQ, 16, 1024, 2);
     // P: a token's kN weights in a row of 32 (64) bytes, swizzled in as many
     const uint64_t dp = make_smem_desc(s0 + F::kOffP, 16, 8 * F::kRowBytes, kN == 16 ? 6 : 4);
-    // One tile's P V is owed at any time. The next tile's scores go before it if their data is there by then (the
-    // softmax takes as long as a product), else after it, so that its slots do not wait for loads.
-    int it = 0, piece = 0, t = 0;  // the next tile to score
-    bool more = w.next(), live = true;
-    auto ready = [&] {
-      return __all_sync(0xffffffffu, (t > 0 || mbar_test(&aux->q_full, piece & 1)) &&
-                                         mbar_test(&aux->a_full[it % F::kSlotsA], (it / F::kSlotsA) & 1) &&
-                                         mbar_test(&aux->b_full[it % F::kSlotsB], (it / F::kSlotsB) & 1));
-    };
-    auto score = [&] {
-      const uint32_t u = uniform(it), sa = u % F::kSlotsA, sb = u % F::kSlotsB;
-      const bool last = t + 1 == w.n;
-      // groups [g0, g1) of a part whose boxes are `pitch` bytes apart
-      auto groups = [&](uint32_t part, int pitch, int g0, int g1) {
-        const uint64_t da = make_smem_desc(part, 16, pitch, 2);
-        const uint32_t d = tm + F::kColS + (u & 1) * kN;
+    int it = 0, piece = 0;
+    bool live = true;
+    while (live && w.next()) {
+      live = mbar_wait_warp(&aux->q_full, piece & 1);
+      for (int t = 0; live && t < w.n; ++t, ++it) {
+        const uint32_t u = uniform(it), sa = u % F::kSlotsA, sb = u % F::kSlotsB, o = uniform(piece & 1);
+        const uint32_t a = s0 + F::kOffA + sa * F::kBytesA, b = s0 + F::kOffB + sb * F::kBytesB;
+        const bool last = t + 1 == w.n;
+        // groups [g0, g1) of a part whose boxes are `pitch` bytes apart
+        auto scores = [&](uint32_t part, int pitch, int g0, int g1) {
+          const uint64_t da = make_smem_desc(part, 16, pitch, 2);
+          tc_fence_after();
+          __syncwarp();
+          if (elect_one()) {
+#pragma unroll 1
+            for (int g = g0; g < g1; ++g) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                umma_f16_ss(tm + F::kColS, da + (g - g0) * kAtom / 16 + k * 2, dq + g * F::kQGroup / 16 + k * 2, idesc_s,
+                            g + k > 0);
+            }
+            if (g1 == 9) {
+              umma_commit(&aux->s_full);
+              if (last) umma_commit(&aux->q_free);
+            }
+          }
+          __syncwarp();
+        };
+        live = mbar_wait_warp(&aux->a_full[sa], (u / F::kSlotsA) & 1);
+        if (!live) break;
+        scores(a, F::kGroupsA * kAtom, 0, F::kGroupsA);
+        live = mbar_wait_warp(&aux->b_full[sb], (u / F::kSlotsB) & 1);
+        if (!live) break;
+        scores(b, F::kGroupsB * kAtom, F::kGroupsA, 9);
+        live = mbar_wait_warp(&aux->p_full, u & 1);
+        if (!live) break;
         tc_fence_after();
         __syncwarp();
         if (elect_one()) {
 #pragma unroll 1
-          for (int g = g0; g < g1; ++g) {
+          for (int j = 0; j < 4; ++j) {
+            const bool in_a = 2 * j < F::kGroupsA;
+            const int pitch = (in_a ? F::kGroupsA : F::kGroupsB) * kAtom;
+            const uint64_t dv = make_smem_desc((in_a ? a + 2 * j * kAtom : b + (2 * j - F::kGroupsA) * kAtom), kAtom, pitch, 2);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16_ss(d, da + (g - g0) * kAtom / 16 + k * 2, dq + g * F::kQGroup / 16 + k * 2, idesc_s, g + k > 0);
+            for (int k = 0; k < kTok / 16; ++k)
+              umma_f16_ss(tm + F::kColO + (o * 4 + j) * kN, dv + k * 2 * pitch / 16, dp + k * 16 * F::kRowBytes / 16, idesc_o,
+                          t + k > 0);
           }
-          if (g1 == 9) {
-            umma_commit(&aux->s_full[u & 1]);
-            if (last) umma_commit(&aux->q_free);
-          }
+          umma_commit(&aux->pv_done[sa]);
+          if (last) umma_commit(&aux->o_full[o]);
         }
         __syncwarp();
-      };
-      live = live && (t > 0 || mbar_wait_warp(&aux->q_full, piece & 1)) &&
-             mbar_wait_warp(&aux->a_full[sa], (u / F::kSlotsA) & 1);
-      if (live) groups(s0 + F::kOffA + sa * F::kBytesA, F::kGroupsA * kAtom, 0, F::kGroupsA);
-      live = live && mbar_wait_warp(&aux->b_full[sb], (u / F::kSlotsB) & 1);
-      if (live) groups(s0 + F::kOffB + sb * F::kBytesB, F::kGroupsB * kAtom, F::kGroupsA, 9);
-      ++it;
-      if (last) {
-        t = 0;
-        ++piece;
-        more = w.next();
-      } else {
-        ++t;
       }
-    };
-    auto value = [&](int tile, int of, bool first, bool last) {
-      const uint32_t u = uniform(tile), sa = u % F::kSlotsA, sb = u % F::kSlotsB, o = uniform(of & 1);
-      const uint32_t a = s0 + F::kOffA + sa * F::kBytesA, b = s0 + F::kOffB + sb * F::kBytesB;
-      live = live && mbar_wait_warp(&aux->p_full[u & 1], (u >> 1) & 1);
-      if (!live) return;
-      tc_fence_after();
-      __syncwarp();
-      if (elect_one()) {
-#pragma unroll 1
-        for (int j = 0; j < 4; ++j) {
-          const bool in_a = 2 * j < F::kGroupsA;
-          const int pitch = (in_a ? F::kGroupsA : F::kGroupsB) * kAtom;
-          const uint64_t dv = make_smem_desc((in_a ? a + 2 * j * kAtom : b + (2 * j - F::kGroupsA) * kAtom), kAtom, pitch, 2);
-#pragma unroll
-          for (int k = 0; k < kTok / 16; ++k)
-            umma_f16_ss(tm + F::kColO + (o * 4 + j) * kN, dv + k * 2 * pitch / 16,
-                        dp + (u & 1) * F::kBytesP / 16 + k * 16 * F::kRowBytes / 16, idesc_o, !first || k > 0);
-        }
-        umma_commit(&aux->pv_done[sa]);
-        if (last) umma_commit(&aux->o_full[o]);
-      }
-      __syncwarp();
-    };
-    if (more) score();
-    for (int n = 0, of = 0, done = 0; live && n < it; ++n) {
-      // tile n is number `done` of piece `of`; the last one if the tile after it is a first one
-      const bool last = t == 0;
-      if (more && ready()) {
-        score();
-        value(n, of, done == 0, last);
-      } else {
-        value(n, of, done == 0, last);
-        if (more && live) score();
-      }
-      done = last ? 0 : done + 1;
-      of += last;
+      ++piece;
     }
     if (!live && lane == 0) {
       umma_commit(&aux->drain);
@@ -352,10 +327,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
           my_m = -INFINITY;
           t = w.t0;
         }
-        mbar_wait_warp(&aux->s_full[it & 1], (it >> 1) & 1);
+        mbar_wait_warp(&aux->s_full, it & 1);
         tc_fence_after();
         uint32_t x[kN];
-        tmem_ld_row<kN>(tl + F::kColS + (it & 1) * kN, x);
+        tmem_ld_row<kN>(tl + F::kColS, x);
         tmem_wait_ld();
         const int tok = t * kTok + mine;
         if (lane >= 16) {
@@ -390,9 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
             if (up) m[j] = mx;
             l[j] *= dm[j];
           }
-          if (!start) {
-            mbar_wait_warp(&aux->pv_done[(it - 1) % F::kSlotsA], ((it - 1) / F::kSlotsA) & 1);  // the output is at rest
-            tc_fence_after();
+          if (!start) {  // the scores came after the last tile's P V: the output is at rest
 #pragma unroll 1
             for (int b = 0; b < 4; ++b) {
               uint32_t o[kN];
@@ -405,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
             tmem_wait_st();
           }
         }
-        // P over that of two tiles ago: its product came before these scores
+        // P over the last tile's, whose product came before these scores
         uint32_t pk[kN / 2];
 #pragma unroll
         for (int j = 0; j < kN; j += 2) {
@@ -419,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
           pk[j / 2] = pack2<kFp16>(y[0], y[1]);
         }
         if (lane < 16) {
-          uint8_t* dst = smem + F::kOffP + (it & 1) * F::kBytesP + mine * F::kRowBytes;
+          uint8_t* dst = smem + F::kOffP + mine * F::kRowBytes;
           const int swap = kN == 16 ? (mine >> 2) & 1 : (mine >> 1) & 3;
 #pragma unroll
           for (int q = 0; q < kN / 8; ++q)
@@ -447,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
         fence_proxy_async_smem();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->p_full[it & 1]);
+        if (lane == 0) mbar_arrive(&aux->p_full);
         ++it;
       }
       if (pending) {
