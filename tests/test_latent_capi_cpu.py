@@ -118,6 +118,14 @@ def test_verify_refusals():
     assert f(*put(7, 0)) == C.OK
 
 
+def test_verify_refuses_rows_near_the_32_bit_limit():
+    """The kernel's 32-bit indices step past the end of a row before they are compared with it."""
+    from cascade_kernel import capi as C
+    f = C.load().cascade_verify_drafts
+    for vocab in ((1 << 31) - 1, 1 << 30):
+        _refused(f(4096, 4096, 4096, 4096, 4096, 4096, C.FP32, 2, 3, vocab, 4096, 4096, None), "too large")
+
+
 def test_schemas():
     import torch
     import cascade_kernel  # noqa: F401

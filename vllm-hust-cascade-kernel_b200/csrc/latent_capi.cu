@@ -279,7 +279,8 @@ int cascade_verify_drafts(const int64_t* tokens, const int64_t* draft_lens, cons
     return fail(CASCADE_ERR_INVALID, "%s: probabilities must be bf16, fp16 or fp32", op);
   if (batch < 0 || max_drafts < 0) return fail(CASCADE_ERR_INVALID, "%s: negative size", op);
   if (vocab < 1) return fail(CASCADE_ERR_INVALID, "%s: vocabulary must not be empty", op);
-  if (vocab > kI32 || max_drafts > kI32 || batch > kI32 / 8)
+  // (the kernel's 32-bit indices step up to two rounds of 16,384 entries past the row)
+  if (vocab >= kI32 / 2 || max_drafts > kI32 || batch > kI32 / 8)
     return fail(CASCADE_ERR_UNSUPPORTED, "%s: problem too large", op);
   if (batch == 0) return CASCADE_OK;
   if (!draft_lens || !target_probs || !noise || !out_tokens || !accepted || (max_drafts && (!tokens || !uniform)))
