@@ -61,6 +61,10 @@ namespace {
 constexpr int kRows = 128;     // query rows per tile
 constexpr int kTok = 64;       // cache rows per tile
 constexpr int kHalfTok = 32;   // per CTA
+// What going from one unit to the next costs, in tiles (about 10,000 cycles), for cutting the work into equal runs.
+// 24 requests x 4 tokens x 128 heads over 9-4,999 tokens: 0 137 us, 3 97, 4 90, 6 88; 128 requests x 128 heads over
+// 1,506-8,145 tokens: 217, 212, 212, 213.
+constexpr int kSetup = 5;
 constexpr int kThreads = 15 * 32;
 constexpr int kMaxClusters = kNumSMs / 2;
 
@@ -158,7 +162,7 @@ struct PageRows {
 // h ^ (r / 4 % 2)); no bank conflicts either way. `released` (if given) gets an
 // arrival per thread once the accumulator has been read.
 template <bool kFp16, bool kWide>
-__device__ __forceinline__ void write_rows(const Params& P, const Walk<kRows, kTok>& x, int cluster, int c, float inv, uint32_t tmem,
+__device__ __forceinline__ void write_rows(const Params& P, const Walk<kRows, kTok, kSetup>& x, int cluster, int c, float inv, uint32_t tmem,
                                            uint8_t* stage, int g0, int g1, uint64_t* released) {
   const LatentDecodeLaunch& p = P.L;
   const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3;
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     tmem_relinquish();
   }
   tc_fence_before();
-  find_run<kRows, kTok, kThreads>(p, cluster, clusters, aux->scan, &aux->sched);  // (with CTA barriers)
+  find_run<kRows, kTok, kSetup, kThreads>(p, cluster, clusters, aux->scan, &aux->sched);  // (with CTA barriers)
   tc_fence_after();
   // Both CTAs' barriers are initialised once this barrier is passed; only the roles that reach into the other CTA
   // wait for it first, the loads start before.
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
   const bool remote = warp < 8 || warp == 13;
   if (remote) cluster_wait();
   const uint32_t tbase = aux->tmem_base;
-  Walk<kRows, kTok> w(p, aux->sched);
+  Walk<kRows, kTok, kSetup> w(p, aux->sched);
 
   if (warp == 12 || warp == 14) {
     // ------------------------------------------------------------ producers
@@ -545,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       if (!live) break;
       l = (of[0] + of[1]) + (of[2] + of[3]);
       const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN among the scores stays one
-      const bool last = w.left <= 0;  // of the run
+      const bool last = w.last;  // of the run
       if (hh == 0 && !last) {
         live = pieces == 0 || mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1);  // the last one has been read
         if (!live) break;
@@ -561,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
           P.parts.lse[(2 * cluster + (w.starts ? 1 : 0)) * kRows + r] = lse;
         if (w.starts) {
           P.parts.row_info[grow] =
-              w.ends ? 0 : cut_info(aux->sched, cluster, aux->sched.begin + (it - w.n), w.unit_tiles, r);
+              w.ends ? 0 : cut_info(aux->sched, cluster, w.base + w.unit_tiles - 1, r);
         }
       }
       if (last) {
@@ -585,19 +589,19 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     // Query tile: the nine groups of 64 dims come by TMA, group g into slot g % 3 of 16 KB; six
     // move on to TMEM, the last three stay. (Loads of a row per thread touch 32 lines per
     // instruction: 14,000 cycles in which the softmax stood still too.)
-    auto load_group = [&](const Walk<kRows, kTok>& x, int g) {
+    auto load_group = [&](const Walk<kRows, kTok, kSetup>& x, int g) {
       // group order: the CTA's own columns, the other latent ones, the rotary part
       const int col = g < 4 ? 4 * c + g : g < 8 ? 4 * (1 - c) + g - 4 : 8;
       mbar_arrive_expect_tx(&aux->qs_full[g % 3], kQGroup);
       tma_load_3d(smem + kOffQ + g % 3 * kQGroup, &P.map_q, &aux->qs_full[g % 3], 0,
                   static_cast<int>(x.tok * p.num_heads + x.mt * kRows), col);
     };
-    auto prefetch_q = [&](const Walk<kRows, kTok>& x) {
+    auto prefetch_q = [&](const Walk<kRows, kTok, kSetup>& x) {
       if (tid == 256)
         for (int g = 0; g < 9; ++g)
           tma_prefetch_3d(&P.map_q, 0, static_cast<int>(x.tok * p.num_heads + x.mt * kRows), g);
     };
-    auto place_q = [&](const Walk<kRows, kTok>& x, int piece) -> bool {
+    auto place_q = [&](const Walk<kRows, kTok, kSetup>& x, int piece) -> bool {
       if (tid == 256)
         for (int g = 0; g < 3; ++g) load_group(x, g);
       for (int g = 0; g < 9; ++g) {
@@ -628,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       mbar_arrive(&aux->q_full);
       return true;
     };
-    auto store_o = [&](const Walk<kRows, kTok>& x, int piece) -> bool {
+    auto store_o = [&](const Walk<kRows, kTok, kSetup>& x, int piece) -> bool {
       if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
       tc_fence_after();
       write_rows<kFp16, false>(P, x, cluster, c, aux->inv[r], tbase + lane_off, smem + kOffE + (warp & 3) * 1024, 0, 8,
@@ -642,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     bool live = !more || place_q(w, 0);
     int piece = 0;
     while (live && more) {
-      const Walk<kRows, kTok> now = w;
+      const Walk<kRows, kTok, kSetup> now = w;
       more = w.next();
       if (more) {
         prefetch_q(w);
@@ -706,23 +710,23 @@ cudaError_t launch(Params& P, cudaStream_t stream) {
     n = std::min(found, kMaxClusters);
     resident[dev & 63] = n;
   }
-  const int clusters = std::min(n, run_bound<kRows, kTok>(P.L, kMaxClusters));
+  const int clusters = std::min(n, run_bound<kRows, kTok, kSetup>(P.L, kMaxClusters));
   cfg.gridDim = dim3(2 * clusters);
   e = cudaLaunchKernelEx(&cfg, kern, P);
-  if (e != cudaSuccess || clusters == 1) return e;
-  return launch_combine<kFp16, kRows>(P.L, P.parts, clusters, stream);
+  if (e != cudaSuccess) return e;
+  return launch_combine<kFp16, kRows, kTok>(P.L, P.parts, clusters, stream);
 }
 
 }  // namespace
 
 size_t latent_decode_pair_workspace(const LatentDecodeLaunch& p) {
-  return partial_bytes<kRows>(p, run_bound<kRows, kTok>(p, kMaxClusters));
+  return partial_bytes<kRows>(p, run_bound<kRows, kTok, kSetup>(p, kMaxClusters));
 }
 
 cudaError_t launch_latent_decode_pair(const LatentDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
   Params P;
   P.L = p;
-  P.parts = partials<kRows>(p, run_bound<kRows, kTok>(p, kMaxClusters), workspace);
+  P.parts = partials<kRows>(p, run_bound<kRows, kTok, kSetup>(p, kMaxClusters), workspace);
   // cache rows as 9 groups of 64 dims; a load is the rows of one page (at most 32) x 4 groups (or 1).
   // A cache without pages: a map over one row that nothing in bounds reads.
   const uint32_t rows = p.block_size < kHalfTok ? 16 : 32;

@@ -17,11 +17,13 @@ struct Partials {
 };
 
 struct Sched {
-  int64_t tiles, begin;  // all tiles; this cluster's first
-  int64_t tok;           // first query token of request b
-  int b, mt, t0, left;
-  int q, kv;             // request b's lengths
-  int64_t each;          // tiles of a run; `rest` runs of all have one more
+  // A unit takes kSetup + its tiles on the axis that the runs divide, the tiles last.
+  int64_t begin, end;  // this run
+  int64_t base;        // where the tiles of its first unit begin
+  int64_t each;        // length of a run; `rest` runs of all have one more
+  int64_t tok;         // first query token of request b
+  int b, mt, t0;       // the first unit, and the run's first tile of it
+  int q, kv;           // request b's lengths
   int rest, runs;
 };
 
@@ -57,41 +59,43 @@ struct Unit {
   }
 };
 
-template <int kRows, int kTok>
+template <int kRows, int kTok, int kSetup>
 struct Walk {
   Unit<kRows, kTok> u;
   // the current piece
   int b, mt, t0, n, q, kv;
-  int64_t tok;
-  bool starts, ends;
+  int64_t tok, base;
+  bool starts, ends, last;  // last: of the run
   int unit_tiles;
 
-  int next_b, next_mt, next_t0, left, nq;
-  int64_t next_tok, nkv;  // (nkv as loaded: it is not used, and so not waited for, until the next piece)
+  int next_b, next_mt, next_t0, nq;
+  int64_t next_tok, nkv, next_base, end;  // (nkv as loaded: not used, and so not waited for, until the next piece)
 
   __device__ Walk(const LatentDecodeLaunch& l, const Sched& s)
-      : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), left(s.left), nq(s.q), nkv(s.kv), next_tok(s.tok) {}
+      : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), nq(s.q), next_tok(s.tok), nkv(s.kv), next_base(s.base), end(s.end) {}
   __device__ __forceinline__ void load() {
     nq = u.q_len(next_b);
     nkv = u.p.kv_lens[next_b];
   }
   __device__ __forceinline__ bool next() {
-    if (left <= 0) return false;
-    b = next_b, mt = next_mt, t0 = next_t0, q = nq, kv = u.kv_len(nkv), tok = next_tok;
+    if (next_base + next_t0 >= end) return false;
+    b = next_b, mt = next_mt, t0 = next_t0, q = nq, kv = u.kv_len(nkv), tok = next_tok, base = next_base;
     unit_tiles = u.tiles(q, kv, mt);
-    n = min(left, unit_tiles - t0);
+    n = static_cast<int>(min(static_cast<int64_t>(unit_tiles), end - base)) - t0;
     starts = t0 == 0;
     ends = t0 + n == unit_tiles;
-    left -= n;
-    if (left > 0) {  // the next unit's lengths, loaded a piece ahead
-      next_t0 = 0;
+    next_base = base + unit_tiles + kSetup;
+    next_t0 = 0;
+    last = next_base >= end;
+    if (!last) {  // the next unit's lengths, loaded a piece ahead
       if (++next_mt == u.row_tiles(q)) {
         next_mt = 0;
         do {
           next_tok += nq;
           ++next_b;
           if (next_b >= u.p.batch) {
-            left = 0;
+            last = true;
+            next_base = end;
             break;
           }
           load();
@@ -102,15 +106,14 @@ struct Walk {
   }
 };
 
-// First tile of run c: floor(c total / runs), without a wide division.
+// Start of run c: floor(c total / runs), without a wide division.
 __device__ __forceinline__ int64_t run_begin(int c, int64_t each, int rest, int runs) {
   return c * each + static_cast<uint32_t>(c * rest) / static_cast<uint32_t>(runs);
 }
 
-// row_info of row r of a unit whose first piece is this run's, of `unit_tiles`
-// tiles from `first` on (of all tiles): finds the run that holds its last tile.
-__device__ __forceinline__ int32_t cut_info(const Sched& s, int run, int64_t first, int unit_tiles, int r) {
-  const int64_t last = first + unit_tiles - 1;
+// row_info of row r of a unit whose first piece is this run's and whose last
+// tile is at `last`: finds the run that holds it.
+__device__ __forceinline__ int32_t cut_info(const Sched& s, int run, int64_t last, int r) {
   int hi = run + static_cast<int>(min(static_cast<float>(s.runs - 1 - run),
                                       static_cast<float>(last - s.begin) / static_cast<float>(s.each + (s.rest > 0))));
   while (hi + 1 < s.runs && run_begin(hi + 1, s.each, s.rest, s.runs) <= last) ++hi;
@@ -118,10 +121,11 @@ __device__ __forceinline__ int32_t cut_info(const Sched& s, int run, int64_t fir
   return pack_info(run, hi - run + 1, r);
 }
 
-// Finds this cluster's run: the block sums the units' tiles (and the query
-// tokens) per contiguous chunk of requests, then the thread whose chunk holds
-// the run's first tile walks to it.
-template <int kRows, int kTok, int kThreads>
+// Finds this cluster's run: the block sums the units' lengths on the axis (and the
+// query tokens) per contiguous chunk of requests, then the thread whose chunk holds
+// the run's start walks to it. A run that ends in a unit's set-up has none of its
+// tiles, one that starts there has them from the first on; a few runs may be empty.
+template <int kRows, int kTok, int kSetup, int kThreads>
 __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluster, int clusters,
                                          int64_t (*scan)[kThreads / 32], Sched* sched) {
   const Unit<kRows, kTok> u(p);
@@ -131,7 +135,7 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
   int64_t tiles = 0, toks = 0;
   for (int b = b0; b < b1; ++b) {
     const int q = u.q_len(b), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
-    for (int mt = 0; mt < m; ++mt) tiles += u.tiles(q, kv, mt);
+    for (int mt = 0; mt < m; ++mt) tiles += kSetup + u.tiles(q, kv, mt);
     toks += q;
   }
   int64_t st = tiles, sq = toks;
@@ -141,7 +145,7 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
     if (lane >= d) st += a, sq += c;
   }
   if (lane == 31) scan[0][warp] = st, scan[1][warp] = sq;
-  if (tid == 0) sched->left = 0;
+  if (tid == 0) sched->base = sched->end = 0, sched->t0 = 0;  // no run
   __syncthreads();
   int64_t total = 0;
   for (int w = 0; w < kThreads / 32; ++w) {
@@ -160,10 +164,10 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
       for (int b = b0; b < b1; ++b) {
         const int q = u.q_len(b), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
         for (int mt = 0; mt < m; ++mt) {
-          const int t = u.tiles(q, kv, mt);
+          const int t = kSetup + u.tiles(q, kv, mt);
           if (begin < at + t) {
-            *sched = {total, begin, tok, b, mt, static_cast<int>(begin - at), static_cast<int>(end - begin), q, kv,
-                      each, rest, n_runs};
+            *sched = {begin, end, at + kSetup, each, tok, b, mt, static_cast<int>(max(begin - at - kSetup, static_cast<int64_t>(0))),
+                      q, kv, rest, n_runs};
             b = b1;
             break;
           }
@@ -279,17 +283,19 @@ Partials partials(const LatentDecodeLaunch& p, int runs, void* workspace) {
   return {reinterpret_cast<int32_t*>(ws), o, o + static_cast<size_t>(runs) * 2 * kRows * kLatentDim};
 }
 
-// Runs of a launch: more than tiles would stay idle, whatever the lengths.
-template <int kRows, int kTok>
+// Runs of a launch: more would stay empty, whatever the lengths.
+template <int kRows, int kTok, int kSetup>
 int run_bound(const LatentDecodeLaunch& p, int most) {
   const int64_t rows = p.num_tokens * p.num_heads;
   const int64_t units = p.batch + rows / kRows;
   const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(p.block_cols) * p.block_size + kTok - 1) / kTok);
-  return static_cast<int>(std::min<int64_t>(most, std::min<int64_t>(units, 1 << 20) * tiles));
+  return static_cast<int>(std::min<int64_t>(most, std::min<int64_t>(units, 1 << 20) * (kSetup + tiles)));
 }
 
-template <bool kFp16, int kRows>
+template <bool kFp16, int kRows, int kTok>
 cudaError_t launch_combine(const LatentDecodeLaunch& p, const Partials& parts, int runs, cudaStream_t stream) {
+  // one run, or units of one tile: none is cut
+  if (runs == 1 || static_cast<int64_t>(p.block_cols) * p.block_size <= kTok) return cudaSuccess;
   const int64_t rows = p.num_tokens * p.num_heads;
   const bool few = rows <= kFewRows;
   cudaLaunchConfig_t cc = {};

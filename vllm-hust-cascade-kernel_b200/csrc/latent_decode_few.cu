@@ -30,6 +30,7 @@ namespace cascade {
 namespace {
 
 constexpr int kTok = 64;
+constexpr int kSetup = 1;  // what a new unit costs, in tiles (see find_run): 48 requests x 16 heads 0 47.1 us, 1 42.1, 2 42.7
 constexpr int kThreads = 7 * 32;
 constexpr int kBox = 8;  // cache rows per load
 constexpr int kBoxes = kTok / kBox;
@@ -158,10 +159,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     tmem_relinquish();
   }
   tc_fence_before();
-  find_run<kN, kTok, kThreads>(p, run, runs, aux->scan, &aux->sched);  // (with CTA barriers)
+  find_run<kN, kTok, kSetup, kThreads>(p, run, runs, aux->scan, &aux->sched);  // (with CTA barriers)
   tc_fence_after();
   const uint32_t tbase = aux->tmem_base;
-  Walk<kN, kTok> w(p, aux->sched);
+  Walk<kN, kTok, kSetup> w(p, aux->sched);
 
   if (warp == 4) {
     // ---------------------------------------------------------- cache loads
@@ -169,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     const int oob = max(1, p.num_blocks * p.block_size);
     constexpr int kNoPage = INT_MIN;
     auto first_row = [&](int t) { return t * kTok + lane * kBox; };
-    auto page_id = [&](const Walk<kN, kTok>& x, int t) {
+    auto page_id = [&](const Walk<kN, kTok, kSetup>& x, int t) {
       const int pages = (min(x.kv, x.u.cap) + p.block_size - 1) / p.block_size, page = first_row(t) / p.block_size;
       return page < pages ? p.block_table[static_cast<int64_t>(x.b) * p.block_cols + page] : kNoPage;
     };
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     if (more) id_next = page_id(w, w.t0);
     while (live && more) {
       const int t0 = w.t0, t1 = w.t0 + w.n;
-      const Walk<kN, kTok> now = w;
+      const Walk<kN, kTok, kSetup> now = w;
       more = false;
       for (int t = t0; t < t1; ++t, ++it) {
         const int ahead = (t - t0) & 3;
@@ -306,8 +307,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     // A piece's output is written after the next piece's first P: the products go on meanwhile, into the other
     // accumulator.
     struct {
-      int64_t grow0, slot, first;
-      int rows, unit_tiles;
+      int64_t grow0, slot, last_tile;
+      int rows;
       bool starts, ends;
       float m;
     } done = {};
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
             (whole ? p.lse + done.grow0 : P.parts.lse + done.slot)[tid] = lse;
             if (done.starts)
               P.parts.row_info[done.grow0 + tid] =
-                  done.ends ? 0 : cut_info(aux->sched, run, done.first, done.unit_tiles, tid);
+                  done.ends ? 0 : cut_info(aux->sched, run, done.last_tile, tid);
           }
         }
         meet();
@@ -476,10 +477,9 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
         pending = true;
         done.grow0 = w.tok * p.num_heads + w.mt * kN;
         done.slot = (2 * run + (w.starts ? 1 : 0)) * kN;
-        done.first = aux->sched.begin + (it - w.n);
+        done.last_tile = w.base + w.unit_tiles - 1;
         done.rows = static_cast<int>(min(static_cast<int64_t>(kN), min(static_cast<int64_t>(w.q) * p.num_heads - w.mt * kN,
                                                                       p.num_tokens * p.num_heads - done.grow0)));
-        done.unit_tiles = w.unit_tiles;
         done.starts = w.starts, done.ends = w.ends;
         done.m = my_m;
         more = w.next();
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
 
 template <bool kFp16, int kN>
 cudaError_t launch(const LatentDecodeLaunch& p, void* workspace, cudaStream_t stream) {
-  const int bound = run_bound<kN, kTok>(p, kNumSMs);
+  const int bound = run_bound<kN, kTok, kSetup>(p, kNumSMs);
   Params P;
   P.L = p;
   P.parts = partials<kN>(p, bound, workspace);
@@ -521,8 +521,8 @@ cudaError_t launch(const LatentDecodeLaunch& p, void* workspace, cudaStream_t st
   if (e != cudaSuccess) return e;
   kern<<<bound, kThreads, Few<kN>::kSmem, stream>>>(P);
   e = cudaGetLastError();
-  if (e != cudaSuccess || bound == 1) return e;
-  return launch_combine<kFp16, kN>(p, P.parts, bound, stream);
+  if (e != cudaSuccess) return e;
+  return launch_combine<kFp16, kN, kTok>(p, P.parts, bound, stream);
 }
 
 // Query rows per request, on average (the lengths may be on the device).
@@ -532,8 +532,8 @@ int64_t mean_rows(const LatentDecodeLaunch& p) { return (p.num_tokens + p.batch 
 
 size_t latent_decode_workspace(const LatentDecodeLaunch& p) {
   const int64_t rows = mean_rows(p);
-  return rows <= 16   ? partial_bytes<16>(p, run_bound<16, kTok>(p, kNumSMs))
-         : rows <= 32 ? partial_bytes<32>(p, run_bound<32, kTok>(p, kNumSMs))
+  return rows <= 16   ? partial_bytes<16>(p, run_bound<16, kTok, kSetup>(p, kNumSMs))
+         : rows <= 32 ? partial_bytes<32>(p, run_bound<32, kTok, kSetup>(p, kNumSMs))
                       : latent_decode_pair_workspace(p);
 }
 
