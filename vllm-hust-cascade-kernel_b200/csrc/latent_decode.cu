@@ -1,4 +1,5 @@
-// Latent attention, absorbed form (cascade_latent_decode), on the tensor cores.
+// Latent attention, absorbed form (cascade_latent_decode), on the tensor cores,
+// for more than 32 query rows per request (latent_decode_few.cu has the rest).
 //
 // For a query row x (576 values) of a request: s_t = scale <x, c_t> over the
 // request's cache rows c_t (576 values), out = sum_t softmax(s)_t c_t[0:512].
@@ -32,13 +33,13 @@
 // of the unrounded exponentials, in fp32.
 //
 // Work: the 64-row tiles of all (request, row tile) units, concatenated, are
-// cut into one equal run per cluster, computed on the device from the lengths.
+// cut into one run of equal cost per cluster, computed on the device from the lengths.
 // A unit cut by a run boundary leaves fp32 partials that a second, dependent
 // launch merges in run order; all others are written directly.
 //
 // Measured (128 requests x 128 heads over 1,500-8,200 tokens: 754 MB, 174
-// GFLOP, floor 117 us): 245 us, 3.1 TB/s and 710 TFLOP/s. A tile takes about
-// 2,300 cycles of a pair; its MMAs take 1,430 (960 for the scores, 43-cycle
+// GFLOP, floor 117 us): 242 us, 3.1 TB/s and 718 TFLOP/s. A tile takes about
+// 2,100 cycles of a pair; its MMAs take 1,430 (960 for the scores, 43-cycle
 // shared-memory and 19-cycle TMEM steps; 530 for P V, less overlap), its 52 KB
 // per SM from L2 1,390 at the measured 37 bytes per clock and SM. The rest is
 // the chain P -> other CTA -> P V -> buffer free, two deep: with neither MMAs nor
@@ -47,8 +48,8 @@
 // stages: 296 us); fetching the keys into L2 ahead of their load changes nothing.
 //
 // Warps: 0-7 softmax (two threads per row = TMEM lane, 16 of the CTA's 32 cache
-// rows each: with one, its 1,900 cycles a tile set the pace), 8-11 query tile
-// and epilogue, 12 keys (TMA), 13 MMA issue (one issuer: the two kinds of MMA
+// rows each: with one, its 1,900 cycles a tile set the pace) and output, 8-11 query
+// tile, 12 keys (TMA), 13 MMA issue (one issuer: the two kinds of MMA
 // interleaved from two take a fifth longer), 14 the other CTA's rows (TMA).
 #include <algorithm>
 #include <atomic>
@@ -82,8 +83,7 @@ constexpr int kOffP = kOffQ + (9 - kQTmem) * kQGroup;
 constexpr int kOffA = kOffP + kPBuf * 4 * kPPart;
 constexpr int kOffB = kOffA + kStagesA * kBytesA;
 constexpr int kOffC = kOffB + kStagesB * kBytesV;
-constexpr int kOffE = kOffC + kStagesC * kBytesV;  // epilogue: per warp 32 rows x 32 bytes
-constexpr int kTiles = kOffE + 4 * 1024;           // bytes from the first 1 KB boundary after Aux
+constexpr int kTiles = kOffC + kStagesC * kBytesV;  // bytes from the first 1 KB boundary after Aux
 
 constexpr uint32_t kColO = 0, kColQ = 256, kColS = 448;  // TMEM columns: O 256, Q 192, S 2 x 32
 
@@ -95,7 +95,6 @@ struct __align__(16) Aux {
     float shared[3][4][kRows];
     int64_t scan[2][kThreads / 32];  // find_run only
   };
-  float inv[kRows];  // 1 / sum of the last piece
   // One commit per MMA batch serves all that wait for it (a commit costs the
   // tensor pipe 60 to 100 cycles): s_full[it % 2] = scores of tile it done (the
   // softmax, and the keys' next load), pv_done[it % 4] = P V of tile it done in
@@ -107,7 +106,7 @@ struct __align__(16) Aux {
   // other CTA's rows loaded. The rows of a tile that ends in unused cache rows
   // come over tail_full[it % 2] instead: the softmax clears those rows first.
   uint64_t kv_full[kStagesB], p_full[kPBuf], tail_full[kPBuf], s_full[2], pv_done[4], x_full[3];
-  uint64_t q_full, q_empty, o_full, o_empty, stat_full;
+  uint64_t q_full, q_empty, o_empty;
   uint64_t qs_full[3], qs_empty[3];
   uint64_t stall, drain;
   uint32_t tmem_base;
@@ -160,7 +159,7 @@ struct PageRows {
 // writes whole sectors: kWide, 128 bytes per row at a time (4 KB of `stage`,
 // 16-byte chunk q of row r at q ^ (r % 8)), else 32 (1 KB, half h at
 // h ^ (r / 4 % 2)); no bank conflicts either way. `released` (if given) gets an
-// arrival per thread once the accumulator has been read.
+// arrival per warp once the accumulator has been read.
 template <bool kFp16, bool kWide>
 __device__ __forceinline__ void write_rows(const Params& P, const Walk<kRows, kTok, kSetup>& x, int cluster, int c, float inv, uint32_t tmem,
                                            uint8_t* stage, int g0, int g1, uint64_t* released) {
@@ -199,7 +198,8 @@ __device__ __forceinline__ void write_rows(const Params& P, const Walk<kRows, kT
     tmem_wait_ld();
     if (released && g + 1 == g1) {
       tc_fence_before();
-      mbar_arrive(released);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(released);
     }
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
@@ -254,9 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     for (int s = 0; s < 4; ++s) mbar_init(&aux->pv_done[s], 2);
     mbar_init(&aux->q_full, 128);
     mbar_init(&aux->q_empty, 1);
-    mbar_init(&aux->o_full, 1);
-    mbar_init(&aux->o_empty, 128);
-    mbar_init(&aux->stat_full, 128);
+    mbar_init(&aux->o_empty, 8);
     for (int s = 0; s < 3; ++s) mbar_init(&aux->qs_full[s], 1), mbar_init(&aux->qs_empty[s], 4);
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
@@ -376,7 +374,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
                         (h ? dv1 : dv0) + k * 2048 / 16, idesc_pv, !first || h + k > 0);
         }
         umma_commit_cluster(&aux->pv_done[sb], 3);
-        if (last) umma_commit(&aux->o_full);
       }
       __syncwarp();
       return true;
@@ -550,12 +547,6 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       l = (of[0] + of[1]) + (of[2] + of[3]);
       const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN among the scores stays one
       const bool last = w.last;  // of the run
-      if (hh == 0 && !last) {
-        live = pieces == 0 || mbar_wait_warp(&aux->o_empty, (pieces - 1) & 1);  // the last one has been read
-        if (!live) break;
-        aux->inv[r] = inv;
-        mbar_arrive(&aux->stat_full);
-      }
       const int64_t grow = w.tok * p.num_heads + row;
       if (c == 0 && hh == 0 && row < w.q * p.num_heads && grow < p.num_tokens * p.num_heads) {
         const float lse = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
@@ -568,14 +559,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
               w.ends ? 0 : cut_info(aux->sched, cluster, w.base + w.unit_tiles - 1, r);
         }
       }
-      if (last) {
-        // the query slots are free: staging for eight warps, half of the columns each
-        live = mbar_wait_warp(&aux->o_full, pieces & 1);
-        if (!live) break;
-        tc_fence_after();
+      // P V of the last tile is done in both CTAs: this warp's own P is free, 1 KB to stage its half of the columns,
+      // while warps 8-11 place the next query tile; at the end of the run the query's shared memory, 4 KB
+      live = mbar_wait_warp(&aux->pv_done[(it - 1) & 3], ((it - 1) >> 2) & 1);
+      if (!live) break;
+      tc_fence_after();
+      if (last)
         write_rows<kFp16, true>(P, w, cluster, c, inv, tbase + lane_off, smem + kOffQ + warp * 4096, 4 * hh, 4 * hh + 4,
                                 nullptr);
-      }
+      else
+        write_rows<kFp16, false>(P, w, cluster, c, inv, tbase + lane_off, mine, 4 * hh, 4 * hh + 4, &aux->o_empty);
       ++pieces;
     }
     // the other CTA's last commits (and with them its copies of this CTA's P) have arrived
@@ -583,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     for (int i = max(0, it - kPBuf); live && i < it; ++i)
       live = mbar_wait_warp(&aux->pv_done[i & 3], (i >> 2) & 1);
   } else {
-    // ------------------------------------------------ query loads, epilogue
+    // --------------------------------------------------------- query loads
     const int r = tid - 256;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     // Query tile: the nine groups of 64 dims come by TMA, group g into slot g % 3 of 16 KB; six
@@ -632,33 +625,16 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
       mbar_arrive(&aux->q_full);
       return true;
     };
-    auto store_o = [&](const Walk<kRows, kTok, kSetup>& x, int piece) -> bool {
-      if (!mbar_wait_warp(&aux->stat_full, piece & 1) || !mbar_wait_warp(&aux->o_full, piece & 1)) return false;
-      tc_fence_after();
-      write_rows<kFp16, false>(P, x, cluster, c, aux->inv[r], tbase + lane_off, smem + kOffE + (warp & 3) * 1024, 0, 8,
-                               &aux->o_empty);
-      return true;
-    };
-    // the next piece's query goes in as soon as the last scores of this one are
-    // computed, before this one's epilogue
-    bool more = w.next();
-    if (more) prefetch_q(w);
-    bool live = !more || place_q(w, 0);
-    int piece = 0;
-    while (live && more) {
-      const Walk<kRows, kTok, kSetup> now = w;
-      more = w.next();
-      if (more) {
-        prefetch_q(w);
-        live = mbar_wait_warp(&aux->q_empty, piece & 1);
+    // the next piece's query goes in as soon as the last scores of this one are computed
+    bool live = true;
+    for (int piece = 0; live && w.next(); ++piece) {
+      prefetch_q(w);
+      if (piece > 0) {
+        live = mbar_wait_warp(&aux->q_empty, (piece - 1) & 1);
         if (!live) break;
         tc_fence_after();
-        live = place_q(w, piece + 1);
-        if (!live) break;
       }
-      if (!more) break;  // the softmax warps, done by then, write the run's last piece
-      live = store_o(now, piece);
-      ++piece;
+      live = place_q(w, piece);
     }
   }
   __syncwarp();
