@@ -162,3 +162,40 @@ def test_verify_refusals():
     for args, text in bad:
         with pytest.raises(RuntimeError, match=text):
             Hh.ops().cascade_verify_drafts(*args)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V", [4, 8, 1020, 1028, 4096, 8192, 16388, 40004])
+def test_verify_rows_of_whole_groups(V, dtype):
+    """Rows that are read in groups of four, around whole rounds."""
+    _case(_inputs(9, 3, V, dtype, seed=V))
+
+
+@pytest.mark.parametrize("which", [2, 3, 5])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_verify_tensors_off_the_group_alignment(which, dtype):
+    """One tensor an element past 16 bytes: the same answer from single entries."""
+    import torch
+    args = _inputs(7, 3, 5000, dtype, seed=which)
+    x = args[which]
+    room = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
+    off = room[1:].view(x.shape)
+    off.copy_(x)
+    want = _case(args)
+    args[which] = off
+    assert np.array_equal(_case(args)[0], want[0])
+
+
+def test_verify_equal_quotients_take_the_lowest_index():
+    """Equal best quotients in different rounds, lanes, warps and CTAs."""
+    import torch
+    V = 40000
+    target = torch.full((6, 1, V), 1e-6, device="cuda")
+    noise = torch.ones((6, V), device="cuda")
+    places = [[39999, 20000], [33, 32], [16384, 8191, 30000], [7, 6, 5, 4], [12345, 12345 + 8192], [39998]]
+    for b, p in enumerate(places):
+        target[b, 0, p] = 0.25
+    empty = torch.zeros((6, 0), device="cuda")
+    out, acc = Hh.ops().cascade_verify_drafts(empty.long(), torch.zeros(6, dtype=torch.int64, device="cuda"), None, target,
+                                              empty, noise)
+    assert out[:, 0].tolist() == [min(p) for p in places] and acc.tolist() == [0] * 6

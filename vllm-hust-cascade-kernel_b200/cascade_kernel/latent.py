@@ -14,7 +14,7 @@ LATENT, ROPE = 512, 64
 
 
 class LatentCache:
-    """Rows (sequences) over shared pages; every method keeps to the device."""
+    """Rows (sequences) over shared pages. Only ``grow`` waits for the device (it raises when pages run out)."""
 
     def __init__(self, layers, blocks, page, rows, cols, dtype=torch.bfloat16, device="cuda"):
         self.page = page
@@ -69,7 +69,8 @@ class LatentCache:
 
     def fork(self, parents):
         """The rows become copies of rows ``parents`` (int64): shared full pages, an own copy of a partly filled last
-        one. The old rows give their pages back afterwards."""
+        one. The old rows give their pages back afterwards, so the copies need free pages: a row that found none has
+        length -1 (attention over it sees nothing)."""
         child, lens, refs = torch.ops.npu.cascade_page_fork(self.pools, self.table, self.lens, self.refs, parents)
         _, _, refs = torch.ops.npu.cascade_page_free(self.table, self.lens, refs, torch.zeros_like(self.lens), self.page)
         self.table, self.lens, self.refs = child, lens, refs
