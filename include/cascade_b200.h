@@ -399,7 +399,8 @@ CASCADE_API int cascade_page_compact(void *const *pools, int64_t num_pools, int6
  *   target_probs [B, K+1, V] in `dtype` (any of the three); uniform fp32
  *   [B, K]; noise fp32 [B, V], positive; out_tokens int64 [B, K+1]: the
  *   accepted drafts, the last token, then -1; accepted int64 [B].
- * A drafted token outside [0, V) is refused, and nothing is left out for it. */
+ * A drafted token outside [0, V) is refused, and nothing is left out for it.
+ * V of 2^30 - 1 and more is unsupported. */
 CASCADE_API int cascade_verify_drafts(const int64_t *tokens, const int64_t *draft_lens, const void *draft_probs,
                                       const void *target_probs, const float *uniform, const float *noise,
                                       int32_t dtype, int64_t batch, int64_t max_drafts, int64_t vocab,
