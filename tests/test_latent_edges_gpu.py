@@ -1,0 +1,28 @@
+"""Latent attention where its inputs leave the ordinary: large values that a weight of 0 has to hide."""
+import numpy as np
+import pytest
+
+import helpers as Hh
+from test_latent_attn_gpu import SCALE, _check, _prefill_inputs, _prefill_want
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("hidden", ["by the causal mask", "by its score"])
+def test_prefill_weight_of_zero_hides_large_values(hidden):
+    """Finite values of 1e38 whose weight is 0, or e^-300 (1e38 e^-300 is far below the tolerance), leave nothing."""
+    Hh.need_cuda()
+    n, first = 300, 200
+    args = _prefill_inputs([(n, n)], 2, "bf16", "plain")
+    if hidden == "by its score":
+        first = n
+        args[0][:, :, 128 + 5] = 1.0
+        args[2][:, 5] = 0.0
+        args[2][1:n:2, 5] = args[2][2:n:4, 5] = -300 / SCALE
+        args[3][1:n:2] = args[3][2:n:4] = 1e38
+    want = _prefill_want(args, True, "bf16")
+    if hidden == "by the causal mask":
+        args[3][first:] = 1e38
+    out, lse = Hh.ops().cascade_latent_prefill(*args, n, SCALE, True)
+    assert np.array_equal(np.isfinite(Hh.dev_to_f64(out)[:first]), np.ones((first, 2, 128), bool))
+    _check(Hh.dev_to_f64(out)[:first], Hh.dev_to_f64(lse).reshape(n, 2)[:first], [w[:first] for w in want])

@@ -655,11 +655,10 @@ __device__ __forceinline__ float ex2(float x) {
 // function unit (16 per clock and SM) is the limit: x = n + f with n the nearest
 // whole number (Cody and Waite's reduction, by adding 1.5 * 2^23), 2^f by the
 // degree-4 polynomial of least relative error on [-1/2, 1/2] (2.6e-6, Remez),
-// n into the exponent. x at most 127; below -126 the result stays near 2^-126.
-// A NaN does not survive it: the caller looks for them.
+// n into the exponent. x at most 127; below -126 the result is 0.
+// A NaN gives 0 too: the caller looks for them.
 __device__ __forceinline__ void ex2_poly2(float& y0, float& y1) {
-  y0 = fmaxf(y0, -126.f);
-  y1 = fmaxf(y1, -126.f);
+  const float x0 = y0, x1 = y1;
   asm("{\n\t.reg .b64 x, t, f, p, c;\n\t.reg .b32 t0, t1, p0, p1;\n\t"
       "mov.b64 x, {%0, %1};\n\t"
       "mov.b64 c, {%2, %2};\n\t"
@@ -688,6 +687,9 @@ __device__ __forceinline__ void ex2_poly2(float& y0, float& y1) {
       : "+f"(y0), "+f"(y1)
       : "f"(12582912.f), "f"(-12582912.f), "f"(-1.f), "f"(0.009570102207362652f), "f"(0.05591785907745361f),
         "f"(0.240247443318367f), "f"(0.6931217908859253f), "f"(0.9999992847442627f));
+  // (not a clamp of x: a weight of 2^-126 is a normal number in bf16, and a masked value may be 1e38)
+  y0 = x0 >= -126.f ? y0 : 0.f;
+  y1 = x1 >= -126.f ? y1 : 0.f;
 }
 
 // max(a, b, c): one three-input max instruction on sm_100.
