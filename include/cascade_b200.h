@@ -300,7 +300,10 @@ CASCADE_API int cascade_latent_decode(const cascade_latent_attn_t *p, void *out,
  * with n query and m key tokens, query i sees keys t < m, and with causal != 0
  * t <= m - n + i (the last query sees every key).
  *   s_t = scale * (<query[i,h,0:128], key[t,h]> + <query[i,h,128:192], key_rope[t]>)
- * Rows that see no key give out = 0 and lse = -inf.
+ * Rows that see no key give out = 0 and lse = -inf. A NaN, or a score of
+ * +infinity, among the keys a row sees makes its out and lse NaN. A key that
+ * only the causal mask hides has weight 0: its value must be finite, 0 times a
+ * NaN is NaN (its key may be anything). Other sequences' rows never matter.
  *   query     [num_tokens, num_heads, 192], contiguous
  *   key       [num_kv, num_heads, 128], strides in elements, last dim contiguous
  *   key_rope  [num_kv, 64], token stride in elements, last dim contiguous

@@ -1,4 +1,5 @@
-"""Latent attention where its inputs leave the ordinary: large values that a weight of 0 has to hide."""
+"""Latent attention where its inputs leave the ordinary: scores of +infinity, large values that a weight of 0 has
+to hide."""
 import numpy as np
 import pytest
 
@@ -6,6 +7,25 @@ import helpers as Hh
 from test_latent_attn_gpu import SCALE, _check, _prefill_inputs, _prefill_want
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("at", [0, 2, 3, 5, 6, 7, 34, 66, 97, 130, 255])
+def test_prefill_infinite_score_makes_its_rows_nan(at, dtype):
+    """A score of +inf: inf - inf under the softmax of every row that sees it, wherever the key lies; the rows before it and
+    the other sequence keep theirs."""
+    import torch
+    Hh.need_cuda()
+    args = _prefill_inputs([(256, 256), (40, 40)], 2, dtype, "plain")
+    args[0][:, :, 128 + 5] = 1.0
+    args[2][:, 5] = 0.0
+    want = _prefill_want(args, True, dtype)
+    args[2][at, 5] = float("inf")  # a rotary value: the values stay finite
+    out, lse = Hh.ops().cascade_latent_prefill(*args, 256, SCALE, True)
+    lse = lse.view(296, 2)
+    assert torch.isnan(out[at:256]).all() and torch.isnan(lse[at:256]).all()
+    keep = np.r_[0:at, 256:296]
+    _check(Hh.dev_to_f64(out)[keep], Hh.dev_to_f64(lse)[keep], [w[keep] for w in want])
 
 
 @pytest.mark.parametrize("hidden", ["by the causal mask", "by its score"])

@@ -301,7 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
         tmem_st_32x32b_x16(scol + hh * 64 + g * 16, pk);
       }
       l = l * dm + ((r0 + r1) + (r2 + r3));
-      if (top != top) l = top;  // the exponentials on the FMA pipe lose a NaN
+      // the exponentials on the FMA pipe lose a NaN: a score's own, or inf - inf of a score of +inf
+      if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
       if ((j + 1) * kTok > m && (t == 0 || j >= nt[0]) && hh == 0) {
         // rows past the sequence may hold NaN, which weight 0 does not hide from
         // the product: the tile whose product comes first clears them
