@@ -199,3 +199,16 @@ def test_verify_equal_quotients_take_the_lowest_index():
     out, acc = Hh.ops().cascade_verify_drafts(empty.long(), torch.zeros(6, dtype=torch.int64, device="cuda"), None, target,
                                               empty, noise)
     assert out[:, 0].tolist() == [min(p) for p in places] and acc.tolist() == [0] * 6
+
+
+@pytest.mark.parametrize("token", [(1 << 32) + 5, (1 << 33) + 5, -(1 << 32) + 5, 900, -1])
+def test_verify_tokens_outside_the_vocabulary_leave_nothing_out(token):
+    """Without draft probabilities a refused token is left out of the target's row; one that is no entry leaves the
+    row whole, whatever its low 32 bits are."""
+    Hh.need_cuda()
+    args = _inputs(4, 2, 900, lens=[1, 2, 1, 2])
+    args[2] = None
+    args[0][:, 0] = token
+    args[5][:, 5] = 1e-12  # the best entry
+    out, acc = _case(args)
+    assert (acc == 0).all() and (out[:, 0] == 5).all()

@@ -115,14 +115,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const VerifyLa
   const void* prow = static_cast<const char*>(p.target) + (b * (K + 1) + taken) * V * element;
   const void* qrow = refused && p.draft ? static_cast<const char*>(p.draft) + (b * K + taken) * V * element : nullptr;
   const float* erow = p.noise + b * V;
-  const int64_t out = refused && !p.draft ? p.tokens[b * K + taken] : -1;  // the token left out
+  // the token left out: -1 where it is no entry of the row, before it is narrowed to the entries' 32 bits
+  const int64_t token = refused && !p.draft ? p.tokens[b * K + taken] : -1;
+  const int out = token >= 0 && token < V ? static_cast<int>(token) : -1;
 
   // the best entry of this cluster's row: pass 0 over `left`; pass 1, only
   // when left is 0 everywhere, over the target's row
   uint64_t best = 0;
   for (int pass = 0; pass < 2; ++pass) {
     const bool minus = pass == 0 && qrow;
-    const int skip = pass == 0 ? static_cast<int>(out) : -1;
+    const int skip = pass == 0 ? out : -1;
     const int stride = ctas * kThreads * kW, block = stride * kUnroll<kW>;
     int v0 = (rank * kThreads + static_cast<int>(threadIdx.x)) * kW;
     // `best` as (quotient, index): the thread meets its indices in ascending order, so a later one has to be larger
