@@ -402,7 +402,10 @@ CASCADE_API int cascade_page_compact(void *const *pools, int64_t num_pools, int6
  *   target_probs [B, K+1, V] in `dtype` (any of the three); uniform fp32
  *   [B, K]; noise fp32 [B, V], positive; out_tokens int64 [B, K+1]: the
  *   accepted drafts, the last token, then -1; accepted int64 [B].
- * A drafted token outside [0, V) is refused, and nothing is left out for it.
+ * A drafted token outside [0, V) is refused, and nothing is left out for it. A
+ * NaN among the probabilities refuses its draft and counts as 0 in `left` and
+ * in the row that stands in (an argmax over quotients would choose it); a row
+ * without any positive number gives token 0.
  * V of 2^30 - 1 and more is unsupported. */
 CASCADE_API int cascade_verify_drafts(const int64_t *tokens, const int64_t *draft_lens, const void *draft_probs,
                                       const void *target_probs, const float *uniform, const float *noise,

@@ -212,3 +212,44 @@ def test_verify_tokens_outside_the_vocabulary_leave_nothing_out(token):
     args[5][:, 5] = 1e-12  # the best entry
     out, acc = _case(args)
     assert (acc == 0).all() and (out[:, 0] == 5).all()
+
+
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_verify_nan_probabilities_accept_and_sample_nothing(dtype, draft):
+    """A NaN refuses its draft and counts as 0 in what is left, in the target's row that stands in too."""
+    import torch
+    Hh.need_cuda()
+    B, V = 6, 900
+    args = _inputs(B, 2, V, dtype, lens=[2] * B)
+    args[4][:] = 0.0                      # accepted wherever the target is positive
+    args[3][0, 0, args[0][0, 0]] = float("nan")
+    args[3][1, 2, ::2] = float("nan")     # the row after the last draft
+    args[3][2, 1] = float("nan")          # nothing but NaN: index 0
+    args[3][3, 1, args[0][3, 1]] = 0.0
+    args[3][3, 1, 1::3] = float("nan")
+    if draft:
+        args[2][4, 0, 7::2] = float("nan")
+        args[4][4, 0] = 2.0               # refused, whatever the draft's probability is
+        args[2][5, 0] = args[3][5, 0]     # nothing is left but what NaN hides: the target's row stands in
+        args[4][5, 0] = 2.0
+        args[3][5, 0, ::2] = float("nan")
+    else:
+        args[2] = None
+    got = Hh.ops().cascade_verify_drafts(*args)
+    f = lambda x: x.float().cpu().numpy()  # noqa: E731
+    p, q, e, tok = f(args[3]), f(args[2]) if draft else None, f(args[5]), args[0].cpu().numpy()
+    u = f(args[4])
+    for b in range(B):
+        i = 0
+        while i < 2 and np.float32(u[b, i]) * (q[b, i, tok[b, i]] if draft else np.float32(1)) < p[b, i, tok[b, i]]:
+            i += 1
+        left = p[b, i].copy()
+        if i < 2 and draft:
+            left = left - q[b, i]
+        elif i < 2:
+            left[tok[b, i]] = 0
+        left = np.where(left > 0, left, 0)
+        if not left.any():
+            left = np.where(p[b, i] > 0, p[b, i], 0)
+        assert got[1][b] == i and got[0][b].tolist() == tok[b, :i].tolist() + [int(np.argmax(left / e[b]))] + [-1] * (2 - i)
