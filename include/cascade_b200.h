@@ -370,7 +370,9 @@ CASCADE_API int cascade_page_fork(void *const *pools, int64_t num_pools, int64_t
                                   void *workspace, size_t workspace_bytes, cascade_stream_t stream);
 
 /* Cuts row r to keep_lens[r] tokens (clamped to [0, kv_lens[r]]; 0 frees the
- * row) and drops its reference to each page it no longer needs. */
+ * row) and drops its reference to each page it no longer needs. A page that
+ * the cut leaves partly filled stays shared if it was: copy it
+ * (cascade_page_copy) before writing past the cut. */
 CASCADE_API int cascade_page_free(const int32_t *block_table, int64_t rows, int64_t cols, const int64_t *kv_lens,
                                   const int32_t *page_refs, int64_t num_blocks, const int64_t *keep_lens,
                                   int64_t block_size, int32_t *table_out, int64_t *lens_out, int32_t *refs_out,

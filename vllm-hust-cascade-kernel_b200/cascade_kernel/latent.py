@@ -25,17 +25,33 @@ class LatentCache:
 
     def grow(self, tokens):
         """Gives every row the pages for ``tokens`` (int64 [rows]) more tokens, free ones in ascending order, and
-        lengthens it. A partly filled last page is the row's own (``fork`` copies it), so it is filled in place.
-        Raises if the pages or the table's columns run out."""
+        lengthens it. A row that goes on inside a page that others hold too (``truncate`` cut it there) gets a copy of
+        the page first; if all its holders go on, the lowest row keeps it. Raises, and changes nothing, if the pages or
+        the table's columns run out."""
         have, want = (self.lens + self.page - 1) // self.page, (self.lens + tokens + self.page - 1) // self.page
-        col = torch.arange(self.table.shape[1], device=self.table.device)
+        rows, cols = self.table.shape
+        col = torch.arange(cols, device=self.table.device)
         new = (col >= have[:, None]) & (col < want[:, None])
         free = torch.nonzero(self.refs == 0).squeeze(1).to(torch.int32)
+        # the rows that go on inside a page, and of those the ones that have to leave it to others
+        row = torch.nonzero((tokens > 0) & (self.lens > 0) & (self.lens % self.page > 0)).squeeze(1)
+        end = self.lens[row] // self.page
+        old = self.table[row, end].long()
+        going = torch.bincount(old, minlength=self.refs.numel())
+        first = torch.full_like(going, rows).scatter_reduce_(0, old, row, "amin")
+        leaves = (self.refs[old] > 1) & ((going[old] < self.refs[old]) | (first[old] < row))
+        row, end, old = row[leaves], end[leaves], old[leaves]
         need = int((want - have).sum())
-        if need > free.numel() or int(want.max()) > self.table.shape[1]:
-            raise RuntimeError(f"LatentCache: {need} pages needed, {free.numel()} free, {self.table.shape[1]} columns")
+        total = need + row.numel()
+        if total > free.numel() or bool((want > cols).any()):
+            raise RuntimeError(f"LatentCache: {total} pages needed, {free.numel()} free, {cols} columns")
+        if row.numel():
+            copies = free[need:total]
+            torch.ops.npu.cascade_page_copy(self.pools, old, copies.long())
+            self.table[row, end] = copies
+            self.refs.index_add_(0, old, torch.full_like(copies, -1))
         self.table[new] = free[:need]
-        self.refs[free[:need].long()] = 1
+        self.refs[free[:total].long()] = 1
         self.lens = self.lens + tokens
 
     def write(self, layer, latents, counts):
