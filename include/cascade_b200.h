@@ -359,9 +359,9 @@ CASCADE_API int cascade_page_copy(void *const *pools, int64_t num_pools, int64_t
  * (their counts rise by one) and gets a fresh page holding a copy of the
  * filled rows of a partly filled last page. Fresh pages are the free pages in
  * ascending order, given to the children in order. A child whose parent is
- * outside [0, rows), or that finds no free page left, gets a row of -1 and
- * length -1. child_table: int32 [count, cols]; child_lens: int64 [count];
- * refs_out: int32 [num_blocks]. */
+ * outside [0, rows) or has a negative length, or that finds no free page left,
+ * gets a row of -1 and length -1. child_table: int32 [count, cols];
+ * child_lens: int64 [count]; refs_out: int32 [num_blocks]. */
 CASCADE_API size_t cascade_page_fork_workspace_size(int64_t num_blocks, int64_t count);
 CASCADE_API int cascade_page_fork(void *const *pools, int64_t num_pools, int64_t num_blocks, int64_t block_size,
                                   int64_t row_bytes, const int32_t *block_table, int64_t rows, int64_t cols,

@@ -118,3 +118,41 @@ def test_random_steps_leave_every_row_its_own_tokens(seed):
             m.grow([int(rng.integers(0, min(20, 192 - n) + 1)) for n in lens])
         m.check()
     assert Hh.capi().device_error() == 0
+
+
+def test_row_that_could_not_be_made_stays_so():
+    """A fork that runs out of pages leaves a row of length -1: it cannot grow, be written or become an empty row by itself."""
+    import torch
+    Hh.need_cuda()
+    m = Model(blocks=4, cols=4)
+    m.grow([20])
+    m.fork([0, 0, 0])  # 2 pages, 2 free ones for the last page's copies
+    assert m.cache.lens.tolist() == [20, 20, -1]
+    m.check()
+    with pytest.raises(RuntimeError, match="row 2"):
+        m.cache.grow(torch.tensor([0, 0, 1], device="cuda"))
+    with pytest.raises(RuntimeError, match="no token"):
+        m.cache.write(0, torch.ones((1, 576), dtype=torch.bfloat16, device="cuda"), [0, 0, 1])
+    m.check()
+    m.grow([1, 2, 0])
+    m.truncate([21, 21, 30])
+    m.check()
+    m.fork([1, 2])
+    assert m.cache.lens.tolist() == [21, -1]
+    m.check()
+    m.truncate([21, 0])  # an empty row, from now on like any other
+    m.rows[1] = m.rows[0][:, :0]
+    m.grow([0, 3])
+    m.check()
+
+
+def test_write_refuses_places_outside_the_rows():
+    import torch
+    Hh.need_cuda()
+    m = Model()
+    m.grow([3])
+    with pytest.raises(RuntimeError, match="no token"):
+        m.cache.write(0, torch.ones((4, 576), dtype=torch.bfloat16, device="cuda"), [4])
+    with pytest.raises(RuntimeError, match="row 0"):
+        m.cache.grow(torch.tensor([-1], device="cuda"))
+    m.check()

@@ -14,7 +14,8 @@ LATENT, ROPE = 512, 64
 
 
 class LatentCache:
-    """Rows (sequences) over shared pages. Only ``grow`` waits for the device (it raises when pages run out)."""
+    """Rows (sequences) over shared pages. A row of length -1 could not be made: it stays so, neither grows nor forks, until
+    it is cut to 0 tokens. ``grow`` and ``write`` wait for the device (what they cannot do raises), the others do not."""
 
     def __init__(self, layers, blocks, page, rows, cols, dtype=torch.bfloat16, device="cuda"):
         self.page = page
@@ -27,8 +28,11 @@ class LatentCache:
         """Gives every row the pages for ``tokens`` (int64 [rows]) more tokens, free ones in ascending order, and
         lengthens it. A row that goes on inside a page that others hold too (``truncate`` cut it there) gets a copy of
         the page first; if all its holders go on, the lowest row keeps it. Raises, and changes nothing, if the pages or
-        the table's columns run out."""
-        have, want = (self.lens + self.page - 1) // self.page, (self.lens + tokens + self.page - 1) // self.page
+        the table's columns run out, and for a row that cannot grow."""
+        bad = torch.nonzero((tokens < 0) | ((self.lens < 0) & (tokens != 0))).squeeze(1).tolist()
+        if bad:
+            raise RuntimeError(f"LatentCache.grow: row {bad[0]} could not be made (length -1), or tokens are negative")
+        have, want = ((n.clamp(min=0) + self.page - 1) // self.page for n in (self.lens, self.lens + tokens))
         rows, cols = self.table.shape
         col = torch.arange(cols, device=self.table.device)
         new = (col >= have[:, None]) & (col < want[:, None])
@@ -55,10 +59,16 @@ class LatentCache:
         self.lens = self.lens + tokens
 
     def write(self, layer, latents, counts):
-        """Stores ``latents`` [sum(counts), 576] as the last ``counts`` (host list) tokens of the rows."""
+        """Stores ``latents`` [sum(counts), 576] as the last ``counts`` (host list) tokens of the rows, which ``grow`` gave
+        them."""
+        if len(counts) > self.table.shape[0]:
+            raise RuntimeError(f"LatentCache.write: {len(counts)} counts, {self.table.shape[0]} rows")
         rows = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts)).to(self.table.device)
         back = torch.cat([torch.arange(n, 0, -1) for n in counts]).to(self.table.device)
         at = self.lens[rows] - back
+        bad = rows[at < 0].tolist()
+        if bad:
+            raise RuntimeError(f"LatentCache.write: row {bad[0]} has no token there")
         page = self.table[rows, at // self.page].long()
         self.pools[layer][page, at % self.page] = latents
 
@@ -85,15 +95,18 @@ class LatentCache:
 
     def fork(self, parents):
         """The rows become copies of rows ``parents`` (int64): shared full pages, an own copy of a partly filled last
-        one. The old rows give their pages back afterwards, so the copies need free pages: a row that found none has
-        length -1 (attention over it sees nothing)."""
+        one. The old rows give their pages back afterwards, so the copies need free pages: a row that found none, or
+        whose parent could not be made, has length -1 (attention over it sees nothing)."""
         child, lens, refs = torch.ops.npu.cascade_page_fork(self.pools, self.table, self.lens, self.refs, parents)
         _, _, refs = torch.ops.npu.cascade_page_free(self.table, self.lens, refs, torch.zeros_like(self.lens), self.page)
         self.table, self.lens, self.refs = child, lens, refs
 
     def truncate(self, keep):
-        """Cuts the rows to ``keep`` tokens (int64 [rows]) and frees the pages past them."""
-        self.table, self.lens, self.refs = torch.ops.npu.cascade_page_free(self.table, self.lens, self.refs, keep, self.page)
+        """Cuts the rows to ``keep`` tokens (int64 [rows]) and frees the pages past them. 0 empties a row, one that could
+        not be made as well."""
+        made = (self.lens >= 0) | (keep <= 0)
+        self.table, lens, self.refs = torch.ops.npu.cascade_page_free(self.table, self.lens, self.refs, keep, self.page)
+        self.lens = torch.where(made, lens, -1)
 
     def compact(self):
         """Moves the live pages to the front of the pools; returns their number (int32 [1], on the device)."""

@@ -190,8 +190,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
   auto length = [&](int64_t i) -> int64_t {
     const int64_t p = parents[i];
     if (p < 0 || p >= s.rows) return -1;
-    const int64_t n = max(s.kv_lens[p], static_cast<int64_t>(0));
-    return pages_of(n, bs) <= s.cols ? n : -1;
+    const int64_t n = s.kv_lens[p];  // (negative: the parent could not be made itself)
+    return n >= 0 && pages_of(n, bs) <= s.cols ? n : -1;
   };
 
   // counts: free pages (high half) and children that need one (low half)
