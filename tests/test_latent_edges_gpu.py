@@ -1,10 +1,10 @@
 """Latent attention where its inputs leave the ordinary: scores of +infinity, large values that a weight of 0 has
-to hide."""
+to hide, lengths that the tables do not hold."""
 import numpy as np
 import pytest
 
 import helpers as Hh
-from test_latent_attn_gpu import SCALE, _check, _prefill_inputs, _prefill_want
+from test_latent_attn_gpu import SCALE, _check, _decode, _decode_inputs, _decode_want, _prefill_inputs, _prefill_want
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +46,15 @@ def test_prefill_weight_of_zero_hides_large_values(hidden):
     out, lse = Hh.ops().cascade_latent_prefill(*args, n, SCALE, True)
     assert np.array_equal(np.isfinite(Hh.dev_to_f64(out)[:first]), np.ones((first, 2, 128), bool))
     _check(Hh.dev_to_f64(out)[:first], Hh.dev_to_f64(lse).reshape(n, 2)[:first], [w[:first] for w in want])
+
+
+@pytest.mark.parametrize("heads", [4, 12, 64])
+def test_decode_lengths_past_the_table_are_cut(heads):
+    """A length past the block table's columns counts as all of them, for the causal mask's end too."""
+    Hh.need_cuda()
+    q, cache, bt, qs, kvs = _decode_inputs([96, 96, 96], [3] * 3, heads, 32, "bf16", poison=False)
+    want = _decode_want(q, cache, bt, qs, kvs, True, "bf16")
+    for i, n in enumerate((97, 98, 1 << 62)):
+        kvs[i] = n
+    out, lse = _decode(q, cache, bt, qs, kvs, 3)
+    _check(Hh.dev_to_f64(out), Hh.dev_to_f64(lse).reshape(9, heads), want)

@@ -137,7 +137,7 @@ struct PageRows {
   // tiles [t, ...) of request b with kv valid cache rows
   __device__ __forceinline__ void start(int b, int kv) {
     bt = p.block_table + static_cast<int64_t>(b) * p.block_cols;
-    pages = (min(kv, p.block_cols * p.block_size) + p.block_size - 1) / p.block_size;
+    pages = (kv + p.block_size - 1) / p.block_size;
     base = -(1 << 30);
   }
   // pool row of load i of tile t (called by the whole warp)
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
         live = it < stages || mbar_wait_warp(&aux->pv_done[(it - stages) & 3], ((it - stages) >> 2) & 1);
         if (keys) live = live && (it < 2 || mbar_wait_warp(&aux->s_full[it & 1], ((it >> 1) - 1) & 1));
         if (!live) break;
-        const bool tail = !keys && (t + 1) * kTok > min(w.kv, w.u.cap);
+        const bool tail = !keys && (t + 1) * kTok > w.kv;
         if (lane == 0) {
           uint64_t* full = keys ? &aux->kv_full[st] : tail ? &aux->tail_full[it & 1] : &aux->p_full[it & 1];
           uint8_t* dst = smem + (keys ? kOffB : kOffC) + st * kBytesV;
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     bool live = true;
     while (live && w.next()) {
       const int row = w.mt * kRows + r;
-      const int valid = min(w.kv, w.u.cap);  // cache rows that hold anything
+      const int valid = w.kv;  // cache rows that hold anything
       const int lim = w.u.limit(w.q, w.kv, min(row / p.num_heads, w.q - 1));
       // tiles below this one are seen in full by every row (the first row sees the least)
       const int clean = w.u.limit(w.q, w.kv, w.mt * kRows / p.num_heads) / kTok;

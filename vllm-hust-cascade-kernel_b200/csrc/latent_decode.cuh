@@ -41,15 +41,16 @@ struct Unit {
     return p.q_len > 0 ? p.q_len
                        : static_cast<int>(min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens));
   }
-  static __device__ __forceinline__ int kv_len(int64_t n) {
-    return static_cast<int>(min(max(n, static_cast<int64_t>(0)), static_cast<int64_t>(1 << 30)));
+  // cut to what the block table holds (2^30 - 1 at most), before the causal mask counts from its end
+  __device__ __forceinline__ int kv_len(int64_t n) const {
+    return static_cast<int>(min(max(n, static_cast<int64_t>(0)), static_cast<int64_t>(cap)));
   }
   __device__ __forceinline__ int row_tiles(int q) const {
     return static_cast<int>((static_cast<int64_t>(q) * p.num_heads + kRows - 1) / kRows);
   }
-  // cache rows that query token i of a request sees
+  // cache rows that query token i < q of a request sees
   __device__ __forceinline__ int limit(int q, int kv, int i) const {
-    return max(0, p.causal ? min(cap, kv - q + i + 1) : min(cap, kv));
+    return max(0, p.causal ? kv - q + i + 1 : kv);
   }
   // tiles of a unit: up to what its last row sees, at least one
   __device__ __forceinline__ int tiles(int q, int kv, int mt) const {

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     constexpr int kNoPage = INT_MIN;
     auto first_row = [&](int t) { return t * kTok + lane * kBox; };
     auto page_id = [&](const Walk<kN, kTok, kSetup>& x, int t) {
-      const int pages = (min(x.kv, x.u.cap) + p.block_size - 1) / p.block_size, page = first_row(t) / p.block_size;
+      const int pages = (x.kv + p.block_size - 1) / p.block_size, page = first_row(t) / p.block_size;
       return page < pages ? p.block_table[static_cast<int64_t>(x.b) * p.block_cols + page] : kNoPage;
     };
     int it = 0, id_next = kNoPage, y = oob;
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
       if (more) {
         if (start) {
           const int row0 = w.mt * kN;
-          valid = min(w.kv, w.u.cap);
+          valid = w.kv;
           clean = w.u.limit(w.q, w.kv, row0 / p.num_heads) / kTok;
           if (tid < kN) aux->lim[tid] = w.u.limit(w.q, w.kv, min((row0 + tid) / p.num_heads, w.q - 1));
           meet();
