@@ -58,3 +58,25 @@ def test_decode_lengths_past_the_table_are_cut(heads):
         kvs[i] = n
     out, lse = _decode(q, cache, bt, qs, kvs, 3)
     _check(Hh.dev_to_f64(out), Hh.dev_to_f64(lse).reshape(9, heads), want)
+
+
+@pytest.mark.parametrize("heads", [4, 8, 64])
+def test_decode_tokens_of_no_request_keep_their_rows(heads):
+    """Query lengths on the device that add up to less than num_tokens, in a workspace that holds what another call might
+    have left: the requests' rows are right, the rest of out and lse is not touched."""
+    import torch
+    Hh.need_cuda()
+    C = Hh.capi()
+    kv, lens, T = [1000, 300, 2500], [2, 1, 2], 8
+    q, cache, bt, qs, kvs = _decode_inputs(kv, [2, 1, 5], heads, 32, "bf16")
+    want = _decode_want(q[:5], cache, bt, torch.tensor(lens), kvs, True, "bf16")
+    qs = torch.tensor(lens, dtype=torch.int64, device="cuda")
+    d = C.latent_desc(q, cache, bt, qs, kvs, 0, SCALE)
+    n = C.latent_decode_workspace_size(d)
+    for count, first, row in ((2, 0, 0), (2, 0, 15), (3, 1, 127), (100, 40, 31)):
+        ws = torch.full((n // 4,), (count << 17) | (first << 7) | row, dtype=torch.int32, device="cuda")
+        out, lse = torch.full((T, heads, 512), 7.0, dtype=q.dtype, device="cuda"), torch.full((T * heads,), 7.0, device="cuda")
+        C.latent_decode(d, out, lse, ws)
+        assert (out[5:] == 7).all() and (lse[5 * heads:] == 7).all()
+        _check(Hh.dev_to_f64(out)[:5], Hh.dev_to_f64(lse).reshape(T, heads)[:5], want)
+    assert C.device_error() == 0

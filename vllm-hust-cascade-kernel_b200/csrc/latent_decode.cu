@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_kernel(const __grid
     tmem_relinquish();
   }
   tc_fence_before();
-  find_run<kRows, kTok, kSetup, kThreads>(p, cluster, clusters, aux->scan, &aux->sched);  // (with CTA barriers)
+  find_run<kRows, kTok, kSetup, kThreads>(p, P.parts.row_info, cluster, clusters, aux->scan, &aux->sched);  // (with CTA barriers)
   tc_fence_after();
   // Both CTAs' barriers are initialised once this barrier is passed; only the roles that reach into the other CTA
   // wait for it first, the loads start before.

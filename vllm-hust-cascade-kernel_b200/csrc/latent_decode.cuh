@@ -126,8 +126,10 @@ __device__ __forceinline__ int32_t cut_info(const Sched& s, int run, int64_t las
 // query tokens) per contiguous chunk of requests, then the thread whose chunk holds
 // the run's start walks to it. A run that ends in a unit's set-up has none of its
 // tiles, one that starts there has them from the first on; a few runs may be empty.
+// Rows past the requests' tokens (lengths on the device may add up to less than
+// num_tokens) belong to no unit: their row_info is cleared here, for the merge to pass them by.
 template <int kRows, int kTok, int kSetup, int kThreads>
-__device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluster, int clusters,
+__device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int32_t* row_info, int cluster, int clusters,
                                          int64_t (*scan)[kThreads / 32], Sched* sched) {
   const Unit<kRows, kTok> u(p);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -152,6 +154,12 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int cluste
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) st += scan[0][w], sq += scan[1][w];
     total += scan[0][w];
+  }
+  if (p.q_len == 0) {
+    int64_t i = 0;
+    for (int w = 0; w < kThreads / 32; ++w) i += scan[1][w];
+    for (i = i * p.num_heads + cluster * kThreads + tid; i < p.num_tokens * p.num_heads; i += clusters * kThreads)
+      row_info[i] = 0;
   }
   const int64_t runs = min(static_cast<int64_t>(clusters), total);
   if (cluster < runs) {
@@ -199,8 +207,8 @@ __global__ void __launch_bounds__(256) latent_combine_kernel(const __grid_consta
   if (row >= L.num_tokens * L.num_heads) return;
   const int32_t info = P.row_info[row];
   const int count = info >> 17, c0 = (info >> 7) & 1023, r = info & 127;
-  // rows of a call whose query lengths do not add up hold no info: nothing past the slots is read for them
-  if (count < 2 || c0 + count > clusters) return;
+  // (an aborted run may have left its rows' info as the workspace held it: nothing past the slots is read for them)
+  if (count < 2 || c0 + count > clusters || r >= kRows) return;
   auto slot = [&](int i) { return static_cast<int64_t>(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * kRows + r; };
   const int first = kWarps == 1 ? 0 : warp;
   float4 v[kDepth][kVec];

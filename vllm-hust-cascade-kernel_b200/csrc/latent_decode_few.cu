@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) latent_decode_few_kernel(const __
     tmem_relinquish();
   }
   tc_fence_before();
-  find_run<kN, kTok, kSetup, kThreads>(p, run, runs, aux->scan, &aux->sched);  // (with CTA barriers)
+  find_run<kN, kTok, kSetup, kThreads>(p, P.parts.row_info, run, runs, aux->scan, &aux->sched);  // (with CTA barriers)
   tc_fence_after();
   const uint32_t tbase = aux->tmem_base;
   Walk<kN, kTok, kSetup> w(p, aux->sched);
