@@ -261,9 +261,9 @@ CASCADE_API int cascade_probe_hbm_read(const void *src, size_t bytes, int32_t mo
  *   actual_q_seqlens / actual_kv_seqlens int64 [batch], device memory;
  *          q_seqlen_value > 0: every request has that many query tokens
  *          (actual_q_seqlens may be NULL); 0: read from actual_q_seqlens on
- *          the device. Their sum must be num_tokens: this is not checked, but
- *          nothing outside the tensors is read or written if it is not, and
- *          the rows of tokens that are no request's stay as they are.
+ *          the device. Their sum must be num_tokens. If it is larger, the
+ *          lengths are cut where the tokens end; if it is smaller, the rows of
+ *          tokens that are no request's stay as they are.
  * Neither path reads back to the host, so both can be captured in a graph.
  * A block id outside [0, num_blocks) reads as zeros and sets (word & 2) of
  * cascade_device_error(). */

@@ -80,3 +80,35 @@ def test_decode_tokens_of_no_request_keep_their_rows(heads):
         assert (out[5:] == 7).all() and (lse[5 * heads:] == 7).all()
         _check(Hh.dev_to_f64(out)[:5], Hh.dev_to_f64(lse).reshape(T, heads)[:5], want)
     assert C.device_error() == 0
+
+
+@pytest.mark.parametrize("tokens,heads", [(8192, 64), (16384, 16)])
+def test_decode_query_lengths_past_the_tokens_are_cut(tokens, heads):
+    """Every one of `tokens` requests claims all the tokens, 2^32 rows in all: the first one has them, the others none."""
+    import torch
+    Hh.need_cuda()
+    g = torch.Generator(device="cuda").manual_seed(0)
+    n, page = 100, 16
+    cache = torch.randn((7, page, 576), generator=g, device="cuda").bfloat16()
+    q = torch.randn((tokens, heads, 576), generator=g, device="cuda", dtype=torch.bfloat16)
+    bt = torch.arange(7, dtype=torch.int32, device="cuda").expand(tokens, 7).contiguous()
+    qs, kvs = (torch.full((tokens,), m, dtype=torch.int64, device="cuda") for m in (tokens, n))
+    out, lse = _decode(q, cache, bt, qs, kvs, 0, causal=False)
+    pick = torch.randint(0, tokens, (40,), generator=g, device="cuda")
+    pick[:2] = torch.tensor([0, tokens - 1])
+    one = torch.tensor([40], device="cuda")
+    want = _decode_want(q[pick], cache, bt[:1], one, kvs[:1], False, "bf16")
+    _check(Hh.dev_to_f64(out[pick]), Hh.dev_to_f64(lse.view(tokens, heads)[pick]), want)
+    assert Hh.capi().device_error() == 0
+
+
+def test_decode_query_lengths_past_the_tokens_in_a_batch():
+    """The request in which the tokens end gets what is left of them, as the first of its tokens."""
+    import torch
+    Hh.need_cuda()
+    for heads in (4, 10, 48):
+        q, cache, bt, qs, kvs = _decode_inputs([300, 90, 40, 7], [3, 2, 1, 0], heads, 32, "bf16", poison=False)
+        want = _decode_want(q, cache, bt, qs, kvs, False, "bf16")
+        claim = torch.tensor([3, 2, 9, 1 << 40], dtype=torch.int64, device="cuda")
+        out, lse = _decode(q, cache, bt, claim, kvs, 0, causal=False)
+        _check(Hh.dev_to_f64(out), Hh.dev_to_f64(lse).reshape(6, heads), want)

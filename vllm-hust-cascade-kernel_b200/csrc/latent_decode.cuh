@@ -37,9 +37,11 @@ struct Unit {
   const LatentDecodeLaunch& p;
   int cap;
   __device__ explicit Unit(const LatentDecodeLaunch& l) : p(l), cap(l.block_cols * l.block_size) {}
-  __device__ __forceinline__ int q_len(int b) const {
+  // query tokens of request b, whose first one is `tok` <= num_tokens: lengths on the device that add up to more than
+  // num_tokens are cut there, so that no unit, row or offset lies past the tensors
+  __device__ __forceinline__ int q_len(int b, int64_t tok) const {
     return p.q_len > 0 ? p.q_len
-                       : static_cast<int>(min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens));
+                       : static_cast<int>(min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens - tok));
   }
   // cut to what the block table holds (2^30 - 1 at most), before the causal mask counts from its end
   __device__ __forceinline__ int kv_len(int64_t n) const {
@@ -75,7 +77,7 @@ struct Walk {
   __device__ Walk(const LatentDecodeLaunch& l, const Sched& s)
       : u(l), next_b(s.b), next_mt(s.mt), next_t0(s.t0), nq(s.q), next_tok(s.tok), nkv(s.kv), next_base(s.base), end(s.end) {}
   __device__ __forceinline__ void load() {
-    nq = u.q_len(next_b);
+    nq = u.q_len(next_b, next_tok);
     nkv = u.p.kv_lens[next_b];
   }
   __device__ __forceinline__ bool next() {
@@ -122,9 +124,9 @@ __device__ __forceinline__ int32_t cut_info(const Sched& s, int run, int64_t las
   return pack_info(run, hi - run + 1, r);
 }
 
-// Finds this cluster's run: the block sums the units' lengths on the axis (and the
-// query tokens) per contiguous chunk of requests, then the thread whose chunk holds
-// the run's start walks to it. A run that ends in a unit's set-up has none of its
+// Finds this cluster's run: the block sums the query tokens (if their lengths are on
+// the device) and the units' lengths on the axis per contiguous chunk of requests, then
+// the thread whose chunk holds the run's start walks to it. A run that ends in a unit's set-up has none of its
 // tiles, one that starts there has them from the first on; a few runs may be empty.
 // Rows past the requests' tokens (lengths on the device may add up to less than
 // num_tokens) belong to no unit: their row_info is cleared here, for the merge to pass them by.
@@ -135,32 +137,41 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int32_t* r
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.batch + kThreads - 1) / kThreads;
   const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-  int64_t tiles = 0, toks = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int q = u.q_len(b), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
-    for (int mt = 0; mt < m; ++mt) tiles += kSetup + u.tiles(q, kv, mt);
-    toks += q;
-  }
-  int64_t st = tiles, sq = toks;
+  // the sum over this thread and those before it in `sum`, over all in the result
+  auto scan_sum = [&](int64_t& sum, int64_t* slot) {
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t a = __shfl_up_sync(0xffffffffu, st, d), c = __shfl_up_sync(0xffffffffu, sq, d);
-    if (lane >= d) st += a, sq += c;
-  }
-  if (lane == 31) scan[0][warp] = st, scan[1][warp] = sq;
-  if (tid == 0) sched->base = sched->end = 0, sched->t0 = 0;  // no run
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) st += scan[0][w], sq += scan[1][w];
-    total += scan[0][w];
-  }
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t a = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += a;
+    }
+    if (lane == 31) slot[warp] = sum;
+    __syncthreads();
+    int64_t all = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) sum += slot[w];
+      all += slot[w];
+    }
+    return all;
+  };
+  int64_t tok0 = static_cast<int64_t>(b0) * p.q_len;  // the first query token of request b0
   if (p.q_len == 0) {
-    int64_t i = 0;
-    for (int w = 0; w < kThreads / 32; ++w) i += scan[1][w];
-    for (i = i * p.num_heads + cluster * kThreads + tid; i < p.num_tokens * p.num_heads; i += clusters * kThreads)
+    int64_t toks = 0;
+    for (int b = b0; b < b1; ++b) toks += u.q_len(b, 0);
+    tok0 = -toks;
+    const int64_t own = min(scan_sum(toks, scan[1]), p.num_tokens);  // tokens that belong to requests
+    tok0 = min(tok0 + toks, p.num_tokens);
+    for (int64_t i = own * p.num_heads + cluster * kThreads + tid; i < p.num_tokens * p.num_heads; i += clusters * kThreads)
       row_info[i] = 0;
   }
+  int64_t tiles = 0, tok = tok0;
+  for (int b = b0; b < b1; ++b) {
+    const int q = u.q_len(b, tok), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
+    for (int mt = 0; mt < m; ++mt) tiles += kSetup + u.tiles(q, kv, mt);
+    tok += q;
+  }
+  int64_t st = tiles;
+  if (tid == 0) sched->base = sched->end = 0, sched->t0 = 0;  // no run
+  const int64_t total = scan_sum(st, scan[0]);
   const int64_t runs = min(static_cast<int64_t>(clusters), total);
   if (cluster < runs) {
     const int n_runs = static_cast<int>(runs);
@@ -169,9 +180,9 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int32_t* r
     const int64_t begin = run_begin(cluster, each, rest, n_runs), end = run_begin(cluster + 1, each, rest, n_runs);
     int64_t at = st - tiles;
     if (begin >= at && begin < st) {
-      int64_t tok = sq - toks;
+      tok = tok0;
       for (int b = b0; b < b1; ++b) {
-        const int q = u.q_len(b), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
+        const int q = u.q_len(b, tok), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
         for (int mt = 0; mt < m; ++mt) {
           const int t = kSetup + u.tiles(q, kv, mt);
           if (begin < at + t) {
