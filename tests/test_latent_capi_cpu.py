@@ -132,3 +132,12 @@ def test_schemas():
     for name in ("cascade_latent_decode", "cascade_latent_prefill", "cascade_page_copy", "cascade_page_fork",
                  "cascade_page_free", "cascade_page_compact", "cascade_verify_drafts"):
         assert str(getattr(torch.ops.npu, name).default._schema).startswith("npu::" + name)
+
+
+@pytest.mark.parametrize("batch,tokens,q_seqlen", [(3, 5, 0x5555555555555557), (4, 4, (1 << 62) + 1), (1, 1 << 31, 1 << 31)])
+def test_decode_refuses_query_lengths_past_32_bits(batch, tokens, q_seqlen):
+    """3 x 0x5555555555555557 is 5 modulo 2^64: the product must not be taken for num_tokens."""
+    from cascade_kernel import capi as C
+    d = _desc(batch=batch, num_tokens=tokens, q_seqlen_value=q_seqlen)
+    _refused(C.load().cascade_latent_decode(ctypes.byref(d), None, None, None, 0, None), "too large")
+    assert C.load().cascade_latent_decode_workspace_size(ctypes.byref(d)) == 0

@@ -51,11 +51,13 @@ int check_decode(const cascade_latent_attn_t* p, const char* op) {
     return fail(CASCADE_ERR_INVALID, "%s: negative size", op);
   if (p->q_seqlen_value < 0)
     return fail(CASCADE_ERR_INVALID, "%s: q_seqlen_value must be >= 0 (0 = per request)", op);
+  if (p->batch > kI32 || p->q_seqlen_value > kI32)  // their product has to hold in 64 bits
+    return fail(CASCADE_ERR_UNSUPPORTED, "%s: problem too large for 32-bit row indices", op);
   if (p->q_seqlen_value > 0 && p->num_tokens != p->batch * p->q_seqlen_value)
     return fail(CASCADE_ERR_INVALID, "%s: with q_seqlen_value=%lld, query.size(0) must equal batch * q_seqlen_value",
                 op, static_cast<long long>(p->q_seqlen_value));
   if (p->num_heads > kI32 || p->num_tokens > kI32 || p->num_tokens * p->num_heads > kI32 ||
-      p->batch > kI32 || p->block_cols > kI32 || p->num_blocks > kI32 || p->num_blocks * bs > kI32 ||
+      p->block_cols > kI32 || p->num_blocks > kI32 || p->num_blocks * bs > kI32 ||
       p->block_cols * bs > kI32 / 2)
     return fail(CASCADE_ERR_UNSUPPORTED, "%s: problem too large for 32-bit row indices", op);
   if (!(p->scale > 0.f) || p->scale > 3e38f) return fail(CASCADE_ERR_INVALID, "%s: scale must be positive", op);
