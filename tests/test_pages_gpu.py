@@ -243,3 +243,27 @@ def test_refusals():
     for call, text in bad:
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+def test_lengths_near_the_end_of_64_bits():
+    """A length that no table holds: no child can be made of such a row, freeing and compacting see all its columns."""
+    import torch
+    Hh.need_cuda()
+    for n in ((1 << 63) - 1, (1 << 63) - 16, 1 << 62):
+        pools, bt, lens, refs = _state(3, [64, 40], 16, 9, cols=4)
+        lens[0] = n
+        table, out, counts = Hh.ops().cascade_page_fork(pools, bt, lens, refs, torch.tensor([0, 1, 0], device="cuda"))
+        assert out.tolist() == [-1, 40, -1] and (table[0] == -1).all() and (table[2] == -1).all()
+        assert torch.equal(counts, refs + torch.bincount(table[1, :3].long(), minlength=9).int())
+        keep = torch.tensor([n, 40], device="cuda")
+        table, out, counts = Hh.ops().cascade_page_free(bt, lens, refs, keep, 16)
+        assert torch.equal(table, bt) and out.tolist() == [n, 40] and torch.equal(counts, refs)
+        table, out, counts = Hh.ops().cascade_page_free(bt, lens, refs, torch.tensor([17, 40], device="cuda"), 16)
+        assert torch.equal(table[0, :2], bt[0, :2]) and (table[0, 2:] == -1).all() and out.tolist() == [17, 40]
+        assert int(counts.sum()) == int(refs.sum()) - 2
+        old = [p.clone() for p in pools]
+        table, counts, live = Hh.ops().cascade_page_compact(pools, bt, lens, refs)
+        assert int(live) == 7 and (table[0] >= 0).all()
+        for p, o in zip(pools, old):
+            assert torch.equal(p[table[0].long()], o[bt[0].long()])
+    assert Hh.capi().device_error() == 0

@@ -170,7 +170,7 @@ __device__ __forceinline__ void cluster_totals(cg::cluster_group& cluster, uint6
 }
 
 __device__ __forceinline__ int64_t pages_of(int64_t len, int64_t block_size) {
-  return len > 0 ? (len + block_size - 1) / block_size : 0;
+  return len > 0 ? (len - 1) / block_size + 1 : 0;  // (no sum that a length near 2^63 makes negative)
 }
 
 struct ForkWork {
