@@ -112,3 +112,26 @@ def test_decode_query_lengths_past_the_tokens_in_a_batch():
         claim = torch.tensor([3, 2, 9, 1 << 40], dtype=torch.int64, device="cuda")
         out, lse = _decode(q, cache, bt, claim, kvs, 0, causal=False)
         _check(Hh.dev_to_f64(out), Hh.dev_to_f64(lse).reshape(6, heads), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_prefill_first_rows_without_keys(dtype):
+    """Fewer keys than queries: the first 128 rows of a block see none, the next ones do. The query, which must not show in
+    the first rows' zeros, is large; many blocks start at once."""
+    import torch
+    Hh.need_cuda()
+    pairs = [(256, 100), (250, 3), (256, 128), (384, 120), (129, 1)]
+    args = _prefill_inputs(pairs, 48, dtype, "plain")
+    args[0][:, 2:] = 1000.0
+    want = _prefill_want([args[0][:, :2], args[1][:, :2], args[2], args[3][:, :2], *args[4:]], True, dtype)
+    first = None
+    for _ in range(20):
+        out, lse = Hh.ops().cascade_latent_prefill(*args, 384, SCALE, True)
+        lse = lse.view(-1, 48)
+        at = 0
+        for n, m in pairs:
+            assert float(out[at:at + n - m].abs().max()) == 0 and torch.isneginf(lse[at:at + n - m]).all()
+            at += n
+        first = out if first is None else first
+        assert torch.equal(out, first)
+    _check(Hh.dev_to_f64(out[:, :2]), Hh.dev_to_f64(lse[:, :2]), want)

@@ -126,8 +126,10 @@ __global__ void __launch_bounds__(kThreads, 1) latent_prefill_kernel(const __gri
     // was issued before it is done.
     bool live = true;
     if (steps > 0 && elect_one()) {
-      mbar_arrive_expect_tx(&aux->q_full, (tl + 1) * 3 * kChunk);
-      for (int t = 0; t <= tl; ++t)
+      // (a tile without products stages its rows of zeros in its part at once: nothing may land there)
+      const int first = nt[0] > 0 ? 0 : 1;
+      mbar_arrive_expect_tx(&aux->q_full, (tl + 1 - first) * 3 * kChunk);
+      for (int t = first; t <= tl; ++t)
         for (int c = 0; c < 3; ++c)
           tma_load_3d(smem + kOffQ + (t * 3 + c) * kChunk, &P.q, &aux->q_full, 0,
                       static_cast<int>(q0) + row0 + t * kRows, h * 3 + c);
