@@ -56,6 +56,8 @@ struct Unit {
   }
   // tiles of a unit: up to what its last row sees, at least one
   __device__ __forceinline__ int tiles(int q, int kv, int mt) const {
+    // (find_run adds these up tile by tile: with the division below, 256 tokens x 128 heads take 30 us more in all)
+    if (!p.causal) return max(1, (kv + kTok - 1) / kTok);
     const int last = static_cast<int>(min(static_cast<int64_t>(q) * p.num_heads, static_cast<int64_t>(mt + 1) * kRows) - 1) /
                      p.num_heads;
     return max(1, (limit(q, kv, last) + kTok - 1) / kTok);
@@ -154,6 +156,7 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int32_t* r
     return all;
   };
   int64_t tok0 = static_cast<int64_t>(b0) * p.q_len;  // the first query token of request b0
+  const int64_t kv0 = b0 < b1 ? p.kv_lens[b0] : 0;     // (on its way during the scan)
   if (p.q_len == 0) {
     int64_t toks = 0;
     for (int b = b0; b < b1; ++b) toks += u.q_len(b, 0);
@@ -165,7 +168,7 @@ __device__ __forceinline__ void find_run(const LatentDecodeLaunch& p, int32_t* r
   }
   int64_t tiles = 0, tok = tok0;
   for (int b = b0; b < b1; ++b) {
-    const int q = u.q_len(b, tok), kv = u.kv_len(p.kv_lens[b]), m = u.row_tiles(q);
+    const int q = u.q_len(b, tok), kv = u.kv_len(b == b0 ? kv0 : p.kv_lens[b]), m = u.row_tiles(q);
     for (int mt = 0; mt < m; ++mt) tiles += kSetup + u.tiles(q, kv, mt);
     tok += q;
   }
