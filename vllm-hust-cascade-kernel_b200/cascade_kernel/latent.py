@@ -79,8 +79,9 @@ class LatentCache:
         return torch.ops.npu.cascade_latent_decode(query, self.pools[layer], table, ones, lens, q_len, scale, True)
 
     def attend_shared(self, layer, query, prefix_table, prefix_lens, scale, own_from):
-        """One token per row whose first ``own_from`` tokens (whole pages) are one prefix shared by all rows: the prefix
-        is read once for the batch, each row's rest by itself, and the two are merged."""
+        """One token per row whose first ``own_from`` tokens (whole pages; no row may be shorter) are one prefix shared by
+        all rows. The prefix is one request of all rows' queries, read once per 128 of its [row x head] query rows (per
+        16 or 32 if there are no more), not once per row; each row's rest is read by itself, and the two are merged."""
         B = query.shape[0]
         skip = own_from // self.page
         if own_from % self.page:

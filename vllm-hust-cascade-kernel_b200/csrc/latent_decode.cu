@@ -38,14 +38,15 @@
 // launch merges in run order; all others are written directly.
 //
 // Measured (128 requests x 128 heads over 1,500-8,200 tokens: 754 MB, 174
-// GFLOP, floor 117 us): 242 us, 3.1 TB/s and 718 TFLOP/s. A tile takes about
+// GFLOP, floor 117 us): 250 us per call in a loop, 3.0 TB/s and 695 TFLOP/s; 210
+// replayed in a graph. A tile takes about
 // 2,100 cycles of a pair; its MMAs take 1,430 (960 for the scores, 43-cycle
 // shared-memory and 19-cycle TMEM steps; 530 for P V, less overlap), its 52 KB
 // per SM from L2 1,390 at the measured 37 bytes per clock and SM. The rest is
 // the chain P -> other CTA -> P V -> buffer free, two deep: with neither MMAs nor
 // loads the waits alone take 1,600 cycles a tile. A third P buffer would have to
 // come out of the ring of own columns, whose fourth stage is worth more (three
-// stages: 296 us); fetching the keys into L2 ahead of their load changes nothing.
+// stages 296 us, four 231, in a graph); fetching the keys into L2 ahead of their load changes nothing.
 //
 // Warps: 0-7 softmax (two threads per row = TMEM lane, 16 of the CTA's 32 cache
 // rows each: with one, its 1,900 cycles a tile set the pace) and output, 8-11 query
@@ -63,8 +64,8 @@ constexpr int kRows = 128;     // query rows per tile
 constexpr int kTok = 64;       // cache rows per tile
 constexpr int kHalfTok = 32;   // per CTA
 // What going from one unit to the next costs, in tiles (about 10,000 cycles), for cutting the work into equal runs.
-// 24 requests x 4 tokens x 128 heads over 9-4,999 tokens: 0 137 us, 3 97, 4 90, 6 88; 128 requests x 128 heads over
-// 1,506-8,145 tokens: 217, 212, 212, 213.
+// In a graph, 24 requests x 4 tokens x 128 heads over 4-5,003 tokens: 0 137 us, 4, 5 and 6 all 94 to 105 from run to
+// run; 128 requests x 128 heads over 1,500-8,200 tokens: 0 217 us, 4 210.9, 5 210.5, 6 211.3.
 constexpr int kSetup = 5;
 constexpr int kThreads = 15 * 32;
 constexpr int kMaxClusters = kNumSMs / 2;

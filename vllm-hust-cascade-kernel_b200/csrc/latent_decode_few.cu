@@ -533,8 +533,8 @@ cudaError_t launch(const LatentDecodeLaunch& p, void* workspace, cudaStream_t st
 }
 
 // Query rows per request, on average (the lengths may be on the device). Up to 16 and up to 32 rows this kernel is
-// the faster one (48 requests: 16 rows 42 against 69 us, 32 rows 48 against 70), above, where it would read the cache
-// once per 32 rows, the pair kernel (48 rows 90 against 71, 64 rows 95 against 73).
+// the faster one (48 requests, in a graph: 16 rows 42 against 69 us, 32 rows 48 against 70), above, where it would read
+// the cache once per 32 rows, the pair kernel (48 rows 90 against 71, 64 rows 95 against 73).
 int64_t mean_rows(const LatentDecodeLaunch& p) { return (p.num_tokens + p.batch - 1) / p.batch * p.num_heads; }
 
 }  // namespace

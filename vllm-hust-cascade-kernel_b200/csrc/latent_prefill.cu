@@ -27,7 +27,8 @@
 // stay in L2).
 //
 // Measured (two prompts of 6,350 and 7,150 tokens x 16 heads, 468 GFLOP, floor
-// 282 us): 480 us, 975 TFLOP/s sustained. A step (256 x 128 scores) takes about
+// 282 us): 489 us per call in a loop, 956 TFLOP/s; 435 to 470 replayed in a graph,
+// with the power cap. A step (256 x 128 scores) takes about
 // 3,870 cycles, its products 2,700: a tile's scores wait for its P V, which waits
 // for its softmax (1,900 cycles, 1,450 of them exponentials at 11 per clock) and
 // two barrier hops, and tensor memory has no room for a third tile's scores.
