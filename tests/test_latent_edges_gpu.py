@@ -135,3 +135,26 @@ def test_prefill_first_rows_without_keys(dtype):
         first = out if first is None else first
         assert torch.equal(out, first)
     _check(Hh.dev_to_f64(out[:, :2]), Hh.dev_to_f64(lse[:, :2]), want)
+
+
+@pytest.mark.parametrize("batch,q_len,heads", [(1, 75, 128), (150, 1, 16)])
+def test_decode_units_that_take_longer_than_a_tenth_of_a_second(batch, q_len, heads):
+    """Requests of 8 million cached tokens, the same two pages over and over: the query of the unit after one of them waits
+    for 150 ms. Attention over r copies of the tokens is attention over the tokens, its log-sum-exp ln r more.
+
+    Tolerance: sums of 8 million terms in fp32, 16 (values) or 64 (weights) at a time, each addition off by at most 2^-23
+    (the tensor cores' may truncate) or 2^-24 of the sum: (2^23 / 16) 2^-23 + (2^23 / 64) 2^-24 = 0.0703 of sum |p v|, which
+    the tolerance of one copy holds 2^-8 times at least."""
+    import torch
+    Hh.need_cuda()
+    page, cols = 512, 1 << 14
+    n, copies = page * cols, cols // 2
+    q, cache, bt, qs, kvs = _decode_inputs([2 * page], [batch * q_len], heads, page, "bf16", poison=False)
+    out, lse, tol, tol_l = _decode_want(q, cache, bt, qs, kvs, False, "bf16")
+    table = bt.repeat(batch, copies)
+    kvs = torch.full((batch,), n, dtype=torch.int64, device="cuda")
+    got, got_l = _decode(q, cache, table, torch.full_like(kvs, q_len), kvs, q_len, causal=False)
+    assert Hh.capi().device_error() == 0
+    off = n / 16 * 2.0 ** -23 + n / 64 * 2.0 ** -24
+    _check(Hh.dev_to_f64(got), Hh.dev_to_f64(got_l).reshape(batch * q_len, heads),
+           (out, lse + np.log(copies), tol * (1 + 256 * off), tol_l + off + 2.0 ** -18 * np.log(copies)))

@@ -84,7 +84,9 @@ LatentDecodeLaunch decode_launch(const cascade_latent_attn_t* p, void* out, floa
   L.causal = p->causal != 0;
   L.scale = p->scale;
   L.debug_stall = (p->flags & CASCADE_FLAG_DEBUG_STALL) != 0;
-  L.wait_limit_us = L.debug_stall ? 1000 : 0;
+  // The warps that load a unit's query wait while the unit before it is worked on: 1 to 2 us per 64 cached tokens
+  // (measured), so 4 on top of the 100 ms of the other waits.
+  L.wait_limit_us = L.debug_stall ? 1000 : static_cast<uint32_t>(100000 + p->block_cols * p->block_size / 16);
   return L;
 }
 
