@@ -29,46 +29,54 @@ class LatentCache:
         lengthens it. A row that goes on inside a page that others hold too (``truncate`` cut it there) gets a copy of
         the page first; if all its holders go on, the lowest row keeps it. Raises, and changes nothing, if the pages or
         the table's columns run out, and for a row that cannot grow."""
-        bad = torch.nonzero((tokens < 0) | ((self.lens < 0) & (tokens != 0))).squeeze(1).tolist()
-        if bad:
-            raise RuntimeError(f"LatentCache.grow: row {bad[0]} could not be made (length -1), or tokens are negative")
-        have, want = ((n.clamp(min=0) + self.page - 1) // self.page for n in (self.lens, self.lens + tokens))
-        rows, cols = self.table.shape
-        col = torch.arange(cols, device=self.table.device)
-        new = (col >= have[:, None]) & (col < want[:, None])
-        free = torch.nonzero(self.refs == 0).squeeze(1).to(torch.int32)
-        # the rows that go on inside a page, and of those the ones that have to leave it to others
-        row = torch.nonzero((tokens > 0) & (self.lens > 0) & (self.lens % self.page > 0)).squeeze(1)
-        end = self.lens[row] // self.page
-        old = self.table[row, end].long()
-        going = torch.bincount(old, minlength=self.refs.numel())
-        first = torch.full_like(going, rows).scatter_reduce_(0, old, row, "amin")
-        leaves = (self.refs[old] > 1) & ((going[old] < self.refs[old]) | (first[old] < row))
-        row, end, old = row[leaves], end[leaves], old[leaves]
-        need = int((want - have).sum())
+        cols, page = self.table.shape[1], self.page
+        grown = self.lens + tokens
+        have, want = (self.lens + page - 1) // page, (grown + page - 1) // page
+        free = torch.nonzero(self.refs == 0).squeeze(1)
+        # one look at the host: pages needed, rows inside a shared page, rows past the columns, rows that cannot grow
+        inside = (self.lens % page > 0) & (tokens > 0)
+        end = self.lens.clamp(0, max(cols * page - 1, 0)) // page
+        old = self.table.gather(1, end[:, None]).squeeze(1).long() if cols else torch.zeros_like(end)
+        shared = inside & (self.refs[old] > 1) if free.numel() < self.refs.numel() else torch.zeros_like(inside)
+        bad = (tokens < 0) | ((self.lens < 0) & (tokens > 0))
+        need, some, over, wrong = torch.stack((want - have, shared, want > cols, bad)).sum(1).tolist()
+        if wrong:
+            raise RuntimeError(f"LatentCache.grow: row {int(torch.nonzero(bad)[0])} could not be made (length -1), or its "
+                               "tokens are negative")
+        row = self._leaving(shared, inside, old) if some else end[:0]
         total = need + row.numel()
-        if total > free.numel() or bool((want > cols).any()):
+        if total > free.numel() or over:
             raise RuntimeError(f"LatentCache: {total} pages needed, {free.numel()} free, {cols} columns")
         if row.numel():
             copies = free[need:total]
-            torch.ops.npu.cascade_page_copy(self.pools, old, copies.long())
-            self.table[row, end] = copies
-            self.refs.index_add_(0, old, torch.full_like(copies, -1))
-        self.table[new] = free[:need]
-        self.refs[free[:total].long()] = 1
-        self.lens = self.lens + tokens
+            torch.ops.npu.cascade_page_copy(self.pools, old[row], copies)
+            self.refs.index_add_(0, old[row], torch.full_like(self.refs[copies], -1))
+            self.table[row, end[row]] = copies.int()
+        if total:
+            col = torch.arange(cols, device=end.device)
+            self.table.masked_scatter_((col >= have[:, None]) & (col < want[:, None]), free[:total].int())
+            self.refs.index_fill_(0, free[:total], 1)
+        self.lens = grown
+
+    def _leaving(self, shared, inside, page):
+        """The rows of `shared` that have to leave their last page `page` to others: all but the lowest one if every holder
+        goes on inside it."""
+        row, rows = torch.nonzero(inside).squeeze(1), inside.numel()
+        at = page[row]
+        going = torch.bincount(at, minlength=self.refs.numel())
+        first = torch.full_like(going, rows).scatter_reduce_(0, at, row, "amin")
+        return row[shared[row] & ((going[at] < self.refs[at]) | (first[at] < row))]
 
     def write(self, layer, latents, counts):
         """Stores ``latents`` [sum(counts), 576] as the last ``counts`` (host list) tokens of the rows, which ``grow`` gave
         them."""
         if len(counts) > self.table.shape[0]:
             raise RuntimeError(f"LatentCache.write: {len(counts)} counts, {self.table.shape[0]} rows")
-        rows = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts)).to(self.table.device)
-        back = torch.cat([torch.arange(n, 0, -1) for n in counts]).to(self.table.device)
+        rows = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts))
+        rows, back = torch.stack((rows, torch.cat([torch.arange(n, 0, -1) for n in counts]))).to(self.table.device)
         at = self.lens[rows] - back
-        bad = rows[at < 0].tolist()
-        if bad:
-            raise RuntimeError(f"LatentCache.write: row {bad[0]} has no token there")
+        if bool((at < 0).any()):
+            raise RuntimeError(f"LatentCache.write: row {int(rows[at < 0][0])} has no token there")
         page = self.table[rows, at // self.page].long()
         self.pools[layer][page, at % self.page] = latents
 
