@@ -416,6 +416,111 @@ CASCADE_API int cascade_verify_drafts(const int64_t *tokens, const int64_t *draf
                                       int32_t dtype, int64_t batch, int64_t max_drafts, int64_t vocab,
                                       int64_t *out_tokens, int64_t *accepted, cascade_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * A key-value cache held in 4 bits, and log probabilities of tokens.
+ * (No counterpart in the reference.)
+ *
+ * A cache row is one token's key or value of one kv head: 128 values in 80
+ * bytes. Values d = 32 i .. 32 i + 31 are group i; a group has a centre and a
+ * scale in fp16 and a code of 4 bits per value,
+ *   value = (code - 7.5) * scale + centre.
+ * Bytes 0..63: the code of value d is nibble d % 8 (lowest first) of the
+ * little-endian 32-bit word 4 * (d % 32 / 8) + d / 32. Bytes 64..79: centre and
+ * scale of groups 0, 1, 2, 3. A row of zero bytes holds zeros. (A thread of the
+ * attention kernel gets its codes, of all four groups, with one load.)
+ * A cache is uint8 [num_blocks, block_size, kv_heads, 80], contiguous, 16-byte
+ * aligned, one for keys and one for values: the page operators above take it
+ * with row_bytes = kv_heads * 80.
+ * ------------------------------------------------------------------------ */
+#define CASCADE_QUANT_ROW_BYTES 80
+
+/* Quantises keys and values as they are written: for each group, in fp32,
+ *   centre = fp16((lo + hi) / 2), scale = fp16((hi - lo) / 15),
+ *   code = min(max(round(fl(fl(x - centre) * fl(1 / scale)) + 7.5), 0), 15),
+ * halves to even (scale 0: every code 8). Token t's row of kv head h goes to
+ * slot slots[t] = page * block_size + place in the page. A negative slot is
+ * skipped; one past the cache is skipped and sets (word & 2) of
+ * cascade_device_error(). A slot may appear once. A group with a NaN, an infinity or
+ * a value beyond +-32768 reads back as NaN.
+ *   key, value  [num_tokens, kv_heads, 128] in `dtype` (BF16 or FP16), last
+ *               dimension contiguous, 16-byte aligned, strides in elements,
+ *               multiples of 8
+ *   slots       int64 [num_tokens], device memory */
+CASCADE_API int cascade_quant_write(const void *key, int64_t key_token_stride, int64_t key_head_stride,
+                                    const void *value, int64_t value_token_stride, int64_t value_head_stride,
+                                    void *key_cache, void *value_cache, const int64_t *slots, int64_t num_tokens,
+                                    int64_t kv_heads, int64_t head_dim, int64_t num_blocks, int64_t block_size,
+                                    int32_t dtype, cascade_stream_t stream);
+
+/* Reads rows back: key, value [num_tokens, kv_heads, 128] in `dtype` (any of the
+ * three), contiguous, 16-byte aligned. A negative slot gives zeros; so does one
+ * past the cache, which sets (word & 2) of cascade_device_error(). A slot may
+ * appear any number of times. */
+CASCADE_API int cascade_quant_read(const void *key_cache, const void *value_cache, const int64_t *slots, void *key,
+                                   void *value, int64_t num_tokens, int64_t kv_heads, int64_t head_dim,
+                                   int64_t num_blocks, int64_t block_size, int32_t dtype, cascade_stream_t stream);
+
+/* Attention over a 4-bit cache, for single tokens, drafted tokens, chunks of
+ * prompts and prefixes that a batch shares. Query head h reads kv head
+ * h / (num_heads / kv_heads). For query token i of a request with q_len query
+ * tokens and kv_len cached tokens (its own included):
+ *   s_t = scale * <query[i,h], key[t]>,  t < kv_len, and with causal != 0
+ *         t <= kv_len - q_len + i
+ *   out[i,h] = sum_t softmax(s)_t value[t],  lse[i,h] = ln sum_t exp(s_t)
+ * Rows that see no token give out = 0 and lse = -inf. What the pages hold past
+ * kv_len, and what only the causal mask hides, is never used, NaN included.
+ * A NaN in a key that a row sees, or a score of +infinity, makes its out and
+ * lse NaN; a NaN in a value at least the group's 32 values of out. A query row
+ * with a NaN or an infinity that sees a token gives NaN.
+ *   query  [num_tokens, num_heads, 128] in `dtype`, contiguous, 16-byte aligned
+ * The other fields, the lengths and the block ids are as in cascade_latent_attn_t. */
+typedef struct cascade_quant_attn {
+  const void *query;
+  const void *key_cache;
+  const void *value_cache;
+  const int32_t *block_table;
+  const int64_t *actual_q_seqlens;
+  const int64_t *actual_kv_seqlens;
+  int64_t num_tokens;
+  int64_t num_heads;
+  int64_t kv_heads;
+  int64_t head_dim; /* 128 */
+  int64_t num_blocks;
+  int64_t block_size; /* 16, 32, 64, 128, 256 or 512 */
+  int64_t batch;
+  int64_t block_cols;
+  int64_t q_seqlen_value;
+  float scale;
+  int32_t causal;
+  int32_t dtype; /* CASCADE_BF16 or CASCADE_FP16: query and out */
+  int32_t flags; /* 0 or CASCADE_FLAG_DEBUG_STALL */
+} cascade_quant_attn_t;
+
+/* out: [num_tokens, num_heads, 128] in p->dtype; lse: fp32 [num_tokens * num_heads]
+ * (natural log, the compact layout cascade_lse_merge takes with stride 1). */
+CASCADE_API size_t cascade_quant_decode_workspace_size(const cascade_quant_attn_t *p);
+CASCADE_API int cascade_quant_decode(const cascade_quant_attn_t *p, void *out, float *lse, void *workspace,
+                                     size_t workspace_bytes, cascade_stream_t stream);
+
+/* Log probabilities: for row n of the logits x, p = softmax(x[n]),
+ *   logprob[n] = ln p[tokens[n]], entropy[n] = -sum p ln p (0 ln 0 = 0),
+ *   rank[n] = how many entries come before tokens[n] in the order "larger logit
+ *   first, lower index first among equals",
+ *   top_tokens[n][0..top) the first entries in that order, top_logprobs their ln p.
+ * A token outside [0, vocab) has logprob -inf and rank -1. A logit of -inf has
+ * probability 0. A NaN, a +inf, or a row of nothing but -inf makes all
+ * log probabilities and the entropy of the row NaN; for the order a NaN counts as -inf.
+ *   logits  [rows, vocab] in `dtype` (any of the three), row stride in elements,
+ *           aligned to its elements; tokens int64 [rows]; logprob, entropy fp32 [rows];
+ *           rank int64 [rows]; top_logprobs fp32, top_tokens int64 [rows, top],
+ *           0 <= top <= min(32, vocab)
+ * A vocab of 2^30 - 1 and more is unsupported. */
+CASCADE_API size_t cascade_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int32_t dtype, int64_t top);
+CASCADE_API int cascade_token_logprobs(const void *logits, int64_t row_stride, const int64_t *tokens, int32_t dtype,
+                                       int64_t rows, int64_t vocab, int64_t top, float *logprob, float *entropy,
+                                       int64_t *rank, float *top_logprobs, int64_t *top_tokens, void *workspace,
+                                       size_t workspace_bytes, cascade_stream_t stream);
+
 /* Last error message of this thread ("" if none). */
 CASCADE_API const char *cascade_last_error(void);
 

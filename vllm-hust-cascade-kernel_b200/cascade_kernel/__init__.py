@@ -6,7 +6,9 @@ tensors, the reference's torch ops (``torch.ops.npu.fa_fp32_stage1``,
 extended-domain siblings (``cascade_prefix_attention``,
 ``cascade_suffix_decode``, ``cascade_lse_merge``, ``cascade_gateup_swiglu``)
 and the paged latent cache's ops (``cascade_latent_decode``,
-``cascade_latent_prefill``, ``cascade_page_*``, ``cascade_verify_drafts``).
+``cascade_latent_prefill``, ``cascade_page_*``, ``cascade_verify_drafts``), the
+4-bit key-value cache's (``cascade_quant_write``, ``cascade_quant_read``,
+``cascade_quant_decode``) and ``cascade_token_logprobs``.
 Like the reference package (ascend-kernel/python/ascend_kernel/ascend_kernel/
 __init__.py:5-15) it only loads the library; it never imports vllm.
 
@@ -28,5 +30,6 @@ torch.ops.load_library(_EXT)
 
 from . import cascade  # noqa: E402,F401  composed cascade step helpers
 from . import latent  # noqa: E402,F401  paged latent cache
+from . import quant  # noqa: E402,F401  4-bit key-value cache
 
-__all__ = ["LIB_DIR", "CAPI_PATH", "cascade", "latent"]
+__all__ = ["LIB_DIR", "CAPI_PATH", "cascade", "latent", "quant"]

@@ -93,6 +93,15 @@ class LatentPrefill(ctypes.Structure):
         ("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32)]
 
 
+class QuantAttn(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "query", "key_cache", "value_cache", "block_table", "actual_q_seqlens", "actual_kv_seqlens")] + [
+        (n, ctypes.c_int64) for n in (
+            "num_tokens", "num_heads", "kv_heads", "head_dim", "num_blocks", "block_size", "batch", "block_cols",
+            "q_seqlen_value")] + [
+        ("scale", ctypes.c_float), ("causal", ctypes.c_int32), ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32)]
+
+
 _lib = None
 
 
@@ -157,6 +166,18 @@ def load():
     lib.cascade_page_compact.restype = ctypes.c_int
     lib.cascade_verify_drafts.argtypes = [vp, vp, vp, vp, vp, vp, i32, i64, i64, i64, vp, vp, vp]
     lib.cascade_verify_drafts.restype = ctypes.c_int
+    lib.cascade_quant_write.argtypes = [vp, i64, i64, vp, i64, i64, vp, vp, vp, i64, i64, i64, i64, i64, i32, vp]
+    lib.cascade_quant_write.restype = ctypes.c_int
+    lib.cascade_quant_read.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i32, vp]
+    lib.cascade_quant_read.restype = ctypes.c_int
+    lib.cascade_quant_decode_workspace_size.argtypes = [ctypes.POINTER(QuantAttn)]
+    lib.cascade_quant_decode_workspace_size.restype = sz
+    lib.cascade_quant_decode.argtypes = [ctypes.POINTER(QuantAttn), vp, vp, vp, sz, vp]
+    lib.cascade_quant_decode.restype = ctypes.c_int
+    lib.cascade_token_logprobs_workspace_size.argtypes = [i64, i64, i32, i64]
+    lib.cascade_token_logprobs_workspace_size.restype = sz
+    lib.cascade_token_logprobs.argtypes = [vp, i64, vp, i32, i64, i64, i64, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.cascade_token_logprobs.restype = ctypes.c_int
     _lib = lib
     return lib
 
@@ -358,3 +379,27 @@ def page_copy(pools, src, dst, stream=None):
     page = pools[0][0].numel() * pools[0].element_size()
     return check(load().cascade_page_copy(ptrs, len(pools), pools[0].shape[0], page, _ptr(src), _ptr(dst),
                                           src.numel(), stream_ptr(stream)))
+
+
+def quant_desc(query, key_cache, value_cache, block_table, q_seqlens, kv_seqlens, q_seqlen_value, scale, causal=True, flags=0):
+    """The C descriptor of attention over a 4-bit cache, from device tensors."""
+    d = QuantAttn()
+    d.query, d.key_cache, d.value_cache = query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr()
+    d.block_table, d.actual_kv_seqlens = block_table.data_ptr(), kv_seqlens.data_ptr()
+    d.actual_q_seqlens = None if q_seqlens is None else q_seqlens.data_ptr()
+    d.num_tokens, d.num_heads, d.head_dim = query.shape
+    d.num_blocks, d.block_size, d.kv_heads = key_cache.shape[:3]
+    d.batch, d.block_cols = kv_seqlens.numel(), block_table.shape[1]
+    d.dtype = dtype_code(query.dtype)
+    d.q_seqlen_value, d.scale, d.causal, d.flags = q_seqlen_value, scale, int(causal), flags
+    return d
+
+
+def quant_decode_workspace_size(desc):
+    return load().cascade_quant_decode_workspace_size(ctypes.byref(desc))
+
+
+def quant_decode(desc, out, lse, workspace=None, stream=None):
+    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    return check(load().cascade_quant_decode(ctypes.byref(desc), _ptr(out), _ptr(lse), _ptr(workspace), ws_bytes,
+                                             stream_ptr(stream)))

@@ -41,12 +41,12 @@ class LatentCache:
         bad = (tokens < 0) | ((self.lens < 0) & (tokens > 0))
         need, some, over, wrong = torch.stack((want - have, shared, want > cols, bad)).sum(1).tolist()
         if wrong:
-            raise RuntimeError(f"LatentCache.grow: row {int(torch.nonzero(bad)[0])} could not be made (length -1), or its "
-                               "tokens are negative")
+            raise RuntimeError(f"{type(self).__name__}.grow: row {int(torch.nonzero(bad)[0])} could not be made (length "
+                               "-1), or its tokens are negative")
         row = self._leaving(shared, inside, old) if some else end[:0]
         total = need + row.numel()
         if total > free.numel() or over:
-            raise RuntimeError(f"LatentCache: {total} pages needed, {free.numel()} free, {cols} columns")
+            raise RuntimeError(f"{type(self).__name__}: {total} pages needed, {free.numel()} free, {cols} columns")
         if row.numel():
             copies = free[need:total]
             torch.ops.npu.cascade_page_copy(self.pools, old[row], copies)
@@ -70,15 +70,19 @@ class LatentCache:
     def write(self, layer, latents, counts):
         """Stores ``latents`` [sum(counts), 576] as the last ``counts`` (host list) tokens of the rows, which ``grow`` gave
         them."""
+        page, place = self._last(counts, "write")
+        self.pools[layer][page, place] = latents
+
+    def _last(self, counts, what):
+        """Where the last ``counts`` (host list) tokens of the rows lie: (page, place in it), int64 [sum(counts)] each."""
         if len(counts) > self.table.shape[0]:
-            raise RuntimeError(f"LatentCache.write: {len(counts)} counts, {self.table.shape[0]} rows")
+            raise RuntimeError(f"{type(self).__name__}.{what}: {len(counts)} counts, {self.table.shape[0]} rows")
         rows = torch.repeat_interleave(torch.arange(len(counts)), torch.tensor(counts))
         rows, back = torch.stack((rows, torch.cat([torch.arange(n, 0, -1) for n in counts]))).to(self.table.device)
         at = self.lens[rows] - back
         if bool((at < 0).any()):
-            raise RuntimeError(f"LatentCache.write: row {int(rows[at < 0][0])} has no token there")
-        page = self.table[rows, at // self.page].long()
-        self.pools[layer][page, at % self.page] = latents
+            raise RuntimeError(f"{type(self).__name__}.{what}: row {int(rows[at < 0][0])} has no token there")
+        return self.table[rows, at // self.page].long(), at % self.page
 
     def attend(self, layer, query, q_len, scale, rows=None):
         """The last ``q_len`` tokens of every row (their queries [rows * q_len, heads, 576]) over the row's cache."""

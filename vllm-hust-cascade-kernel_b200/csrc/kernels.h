@@ -283,6 +283,64 @@ struct VerifyLaunch {
 };
 cudaError_t launch_verify_drafts(const VerifyLaunch& p, cudaStream_t stream);
 
+// ----------------------------------------------------------------------------
+// A key-value cache held in 4 bits
+// ----------------------------------------------------------------------------
+constexpr int kQuantRow = 80;    // bytes of a cache row: 64 of codes, then four groups' (centre, scale) in fp16
+constexpr int kQuantCodes = 64;
+
+struct QuantRowsLaunch {
+  const void* src[2];    // keys, values (write)
+  void* dst[2];          // keys, values (read)
+  int64_t token_stride[2], head_stride[2];  // of src, in elements
+  uint8_t* cache[2];
+  const int64_t* slots;
+  int64_t num_tokens, num_slots;
+  int32_t kv_heads;
+};
+cudaError_t launch_quant_write(const QuantRowsLaunch& p, bool fp16, cudaStream_t stream);
+cudaError_t launch_quant_read(const QuantRowsLaunch& p, int dtype, cudaStream_t stream);
+
+struct QuantDecodeLaunch {
+  const void* query;
+  const uint8_t* key;
+  const uint8_t* value;
+  const int32_t* block_table;
+  const int64_t* q_lens;   // null when q_len > 0
+  const int64_t* kv_lens;
+  void* out;               // [num_tokens, num_heads, 128]
+  float* lse;              // [num_tokens * num_heads]
+  int64_t num_tokens;
+  int32_t num_heads, kv_heads, group, num_blocks, block_size, batch, block_cols;
+  int32_t q_len;           // 0 = per request
+  int32_t causal;
+  float scale;
+  uint32_t wait_limit_us;
+  int32_t debug_stall;
+};
+cudaError_t launch_quant_decode(const QuantDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream);
+size_t quant_decode_workspace(const QuantDecodeLaunch& p);
+
+// ----------------------------------------------------------------------------
+// Log probabilities of tokens
+// ----------------------------------------------------------------------------
+constexpr int kMaxTop = 32;
+
+struct LogprobsLaunch {
+  const void* logits;
+  const int64_t* tokens;
+  float* logprob;
+  float* entropy;
+  int64_t* rank;
+  float* top_logprobs;
+  int64_t* top_tokens;
+  int64_t rows, vocab, row_stride;
+  int32_t top;
+  int32_t dtype;           // 0 bf16, 1 fp16, 2 fp32
+};
+cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void* workspace, cudaStream_t stream);
+size_t token_logprobs_workspace(const LogprobsLaunch& p);
+
 // Host: raise a kernel's dynamic shared memory limit once per (kernel,
 // device) instead of on every launch.
 cudaError_t ensure_smem_limit(const void* kernel, int bytes);
