@@ -1,95 +1,520 @@
-// Attention over a 4-bit key-value cache (cascade_quant_decode): one warp per
-// (query token, head), tokens one after the other, 4 values per lane, fp32.
-#include "kernels.h"
-#include "ptx.cuh"
+// Attention over a 4-bit key-value cache (cascade_quant_decode) for few query
+// rows per request and kv head: bound by reading the cache, 160 bytes per token
+// and kv head, with the unpacking of its 256 codes close behind.
+//
+// The codes go to the tensor cores as they are. With a group's centre c and scale
+// s, a key's score is sum over its groups of
+//   s <q, code> + (c - 7.5 s) sum q,
+// so a nibble, masked in place, is an operand: in fp16 the bits 0..3 hold code *
+// 2^-24 and the bits 4..7 code * 2^-20 (subnormals, exact), and q takes the factors
+// 2^24 and 2^20 (a row is first scaled by a power of two to [2^13, 2^14), so 16-bit
+// queries stay exact down to 2^-27 of their row's largest value). One AND per two
+// codes, and a shift per eight. The term of centres and scales is one more product
+// of 16 columns: (c, s) of four groups against sum q and -7.5 sum q, each as two
+// fp16 numbers. fp32 holds every sum.
+// Values are converted, (code - 7.5) s + c in one fused multiply-add, rounded to
+// fp16, as P is: fp16 holds 2^-11 of both where bf16 would hold 2^-8.
+//
+// mma.sync m16n8k16 has the tokens as its M (scores) and the head's values as its
+// M (output), the query rows as its N, so eight rows cost eight columns, and the
+// probabilities' fragments turn by one movmatrix. (tcgen05 would need M = 128 of
+// tokens, converted through shared memory; here 16 of 128 lanes' worth of rows
+// exist, and the products take a third of the time that HBM does.)
+//
+// A warp is on its own: it has a run of 32-token tiles of one kv head, a ring of
+// tiles that the TMA fills, and its rows' softmax; neighbouring warps take the
+// other heads of the same tokens. The place of a token in the MMA's rows (first_token, value_token)
+// keeps every shared-memory load of 80-byte rows free of bank conflicts.
+// The running maxima move only when a score exceeds its row's by more than 2^8.
+#include <algorithm>
+
+#include "quant_decode.cuh"
 
 namespace cascade {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kTok = 32;     // tokens per tile
+constexpr int kSetup = 2;    // what a new unit costs, in tiles
+constexpr int kWarps = 4;
+constexpr int kTileBytes = kTok * kQuantRow;  // of keys or of values
+constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kMagic = 0x64006400u;
 
-// the lane's 4 values of a cache row: d = 4 lane .. 4 lane + 3
-__device__ __forceinline__ float4 row_values(const uint8_t* row, int lane) {
-  const int d = 4 * lane;
-  const uint16_t code = *reinterpret_cast<const uint16_t*>(row + 16 * (d % 32 / 8) + 4 * (d / 32) + d % 8 / 2);
-  const float2 cs = __half22float2(*reinterpret_cast<const __half2*>(row + kQuantCodes + 4 * (d / 32)));
-  float x[4];
+template <int kN>  // query rows / 8
+struct Shape {
+  static constexpr int kRows = 8 * kN;
+  static constexpr int kCtas = kN == 1 ? 4 : 3;    // per SM
+  static constexpr int kStages = kN == 1 ? 2 : 3;  // tiles of keys and values per warp
+  static constexpr int kSmem = kWarps * kStages * 2 * kTileBytes + 128;  // (to align the ring: the TMA writes to 128-byte boundaries)
+};
+
+struct Params {
+  QuantDecodeLaunch L;
+  CUtensorMap key, value;  // 80 bytes x box_rows cache rows
+  QuantPartials parts;
+  int32_t box_rows;
+};
+
+__device__ __forceinline__ uint32_t trans8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+__device__ __forceinline__ float high_half(uint32_t x) { return __high2float(as_half2(x)); }
+// One nibble of two tokens' half words as code - 7.5, exactly: over fp16's 1024 the bits 1..4 are 1024 + 2 code, the bits 5..8
+// 1024 + 32 code. (At bit 0 the 7.5 would be half a step.)
+__device__ __forceinline__ __half2 low_code(uint32_t x) {
+  return __hfma2(as_half2((x & 0x001E001Eu) | kMagic), __float2half2_rn(0.5f), __float2half2_rn(-519.5f));
+}
+__device__ __forceinline__ __half2 high_code(uint32_t x) {
+  return __hfma2(as_half2((x & 0x01E001E0u) | kMagic), __float2half2_rn(0.03125f), __float2half2_rn(-39.5f));
+}
+// centre or scale NaN (or infinite) in either half
+__device__ __forceinline__ bool odd_par(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
+
+// Token (of 16) of row m = g or g + 8 of the scores' product.
+__device__ __forceinline__ int token_lo(int g) { return g & 1 ? 8 + ((g + 3) & 7) : g; }
+__device__ __forceinline__ int token_hi(int g) { return g & 1 ? 8 + ((g + 4) & 7) : g + 1; }
+
+template <bool kFp16, int kN>
+__global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_kernel(const __grid_constant__ Params P) {
+  using S = Shape<kN>;
+  constexpr int kRows = S::kRows, kStages = S::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ uint64_t stall;
+  const QuantDecodeLaunch& p = P.L;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
+    for (int w = 0; w < kWarps; ++w)
+      for (int i = 0; i < kStages; ++i) mbar_init(&full[w][i], 1);
+    mbar_init(&stall, 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int id = blockIdx.x * kWarps + warp, h = id % p.kv_heads, c = id / p.kv_heads;
+  const QuantUnit<kRows, kTok> unit(p);
+  int runs = P.parts.runs;
+  int64_t total;
+  const QuantRun run = find_run<kRows, kTok, kSetup>(unit, c, runs, total);
+  if (p.q_len == 0) {  // rows of tokens that are no request's: nothing to merge
+    int64_t own = 0;
+    for (int b = lane; b < p.batch; b += 32) own += min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = fmaf(static_cast<float>((code >> (4 * i)) & 15) - 7.5f, cs.y, cs.x);
-  return make_float4(x[0], x[1], x[2], x[3]);
+    for (int d = 16; d > 0; d >>= 1) own += __shfl_xor_sync(0xffffffffu, own, d);
+    for (int64_t i = min(own, p.num_tokens) * p.num_heads + blockIdx.x * blockDim.x + threadIdx.x;
+         i < p.num_tokens * p.num_heads; i += static_cast<int64_t>(gridDim.x) * blockDim.x)
+      P.parts.row_info[i] = 0;
+  }
+  if (c >= runs) return;
+
+  uint8_t* mine = smem_raw + ((0u - smem_u32(smem_raw)) & 127u) + warp * kStages * 2 * kTileBytes;
+  uint64_t* bar = full[warp];
+  const uint32_t base = smem_u32(mine);
+  bool live = true;
+  if (p.debug_stall) live = mbar_wait_warp(&stall, 0);  // test hook: runs into the wait limit
+
+  // ------------------------------------------------------------------ loads
+  QuantWalk<kRows, kTok, kSetup> load(p, run);
+  int load_left = 0, load_tile = 0;
+  int issued = 0, done = 0;
+  int ids = 0, ids_next = 0, ids_at = 0;  // this lane's of 32 page ids from page ids_at on, and of the 32 after them
+  const int shift = __ffs(p.block_size) - 1, oob = p.num_blocks ? p.num_blocks * p.block_size : 1;
+  auto page_ids = [&](int at) {
+    const int i = at + lane;
+    return i < p.block_cols ? p.block_table[static_cast<int64_t>(load.b) * p.block_cols + i] : -1;
+  };
+  auto issue = [&] {
+    if (load_left == 0) {
+      if (!load.next()) return;
+      load_left = load.n, load_tile = load.t0;
+      ids_at = (load_tile * kTok) >> shift;
+      ids = page_ids(ids_at), ids_next = page_ids(ids_at + 32);
+    }
+    const int tok = load_tile * kTok, stage = issued % kStages;
+    uint8_t* dst = mine + stage * 2 * kTileBytes;
+    const int boxes = kTok / P.box_rows;  // one or two
+    int rows[2];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int at = tok + i * P.box_rows;
+      if (i >= boxes || (i > 0 && at >= load.kv) ) break;
+      const int page = at >> shift;
+      if (page >= ids_at + 32) ids_at += 32, ids = ids_next, ids_next = page_ids(ids_at + 32);
+      const int32_t page_id = __shfl_sync(0xffffffffu, ids, page - ids_at);
+      // (a unit without tokens has a tile all the same: nothing of it is used)
+      rows[n++] = at >= load.kv ? oob : static_cast<uint32_t>(page_id) < static_cast<uint32_t>(p.num_blocks)
+                      ? page_id * p.block_size + (at & (p.block_size - 1))
+                      : -1;
+    }
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&bar[stage], n * 2 * P.box_rows * kQuantRow);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i >= n) break;
+        if (rows[i] < 0) {
+          atomicOr(&g_cascade_device_error, kErrBadBlockId);
+          rows[i] = oob;
+        }
+        tma_load_2d(dst + i * P.box_rows * kQuantRow, &P.key, &bar[stage], h * kQuantRow, rows[i]);
+        tma_load_2d(dst + kTileBytes + i * P.box_rows * kQuantRow, &P.value, &bar[stage], h * kQuantRow, rows[i]);
+      }
+    }
+    __syncwarp();
+    ++issued, ++load_tile, --load_left;
+  };
+  if (live)
+    for (int i = 0; i < kStages; ++i) issue();
+
+  // per-lane offsets in a 16-token step
+  const int tok_a = token_lo(g), tok_b = token_hi(g);
+  const int vt[4] = {2 * t, 8 + ((2 * t + 4) & 7), 2 * t + 1, 8 + ((2 * t + 5) & 7)};
+
+  QuantWalk<kRows, kTok, kSetup> walk(p, run);
+  while (live && walk.next()) {
+    // ---------------------------------------------------------------- query
+    // row n of this block as the products' columns: lane (g, t) has d = 32 i + 8 t + 0..7 of row 8 n + g
+    const int rows = min(kRows, walk.q * p.group - walk.block * kRows);  // of this unit
+    uint32_t qf[kN][16], zf[kN][2];
+    float mult[kN][2];   // of columns 2 t, 2 t + 1: score * scale * log2(e) per unit of the products
+    int lim[kN][2];
+    auto row_of = [&](int r, int& i) {  // output row of row r of the unit, and its query token
+      const int at = walk.block * kRows + r;
+      i = at / p.group;
+      return (walk.tok + i) * p.num_heads + h * p.group + (at - i * p.group);
+    };
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      int i;
+      const bool real = n * 8 + g < rows;
+      const uint16_t* src = static_cast<const uint16_t*>(p.query) + row_of(real ? n * 8 + g : 0, i) * kHeadDim + 8 * t;
+      float x[32], top = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 v = real ? *reinterpret_cast<const uint4*>(src + 32 * k) : make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = kFp16 ? __half22float2(as_half2(w[e]))
+                                 : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
+          x[8 * k + 2 * e] = f.x, x[8 * k + 2 * e + 1] = f.y;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) top = fmax3f_nan(top, fabsf(x[e]), top);
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) top = fmax3f_nan(top, __shfl_xor_sync(0xffffffffu, top, d), top);
+      // times 2^(13 - exponent): [2^13, 2^14). A row with a NaN or an infinity is NaN.
+      const int ex = max((__float_as_int(top) >> 23) & 255, 1);
+      const bool nan = ex == 255;
+      // (in two factors: each of them, and its inverse, is a normal number)
+      const int up = 140 - ex, up0 = up / 2;
+      const float f0 = __int_as_float((127 + up0) << 23), f1 = nan ? __int_as_float(0x7fffffff) : __int_as_float((127 + up - up0) << 23);
+      float sums[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[8 * k + e] = x[8 * k + e] * f0 * f1, s += x[8 * k + e];
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        sums[k] = s + __shfl_xor_sync(0xffffffffu, s, 2);
+        const float* y = x + 8 * k;
+        qf[n][4 * k] = pack2<true>(y[0], y[4]);
+        qf[n][4 * k + 1] = pack2<true>(y[1] * 0.0625f, y[5] * 0.0625f);
+        qf[n][4 * k + 2] = pack2<true>(y[2], y[6]);
+        qf[n][4 * k + 3] = pack2<true>(y[3] * 0.0625f, y[7] * 0.0625f);
+      }
+      const float z = (t == 0 ? sums[0] : t == 1 ? sums[1] : t == 2 ? sums[2] : sums[3]) * 0x1p-14f, y = -7.5f * z;
+      zf[n][0] = pack2<true>(z, y);
+      const float2 hi = __half22float2(as_half2(zf[n][0]));
+      zf[n][1] = pack2<true>(z - hi.x, y - hi.y);
+      const float m = (0x1p24f / f0 / f1) * (p.scale * 1.4426950408889634f);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        mult[n][k] = __shfl_sync(0xffffffffu, m, (2 * t + k) * 4);
+        row_of(min(n * 8 + 2 * t + k, rows - 1), i);
+        lim[n][k] = unit.limit(walk.q, walk.kv, i);
+      }
+    }
+    int first_token;
+    row_of(0, first_token);
+    const int clean = min(walk.kv, unit.limit(walk.q, walk.kv, first_token));  // tokens below are seen by every row
+    row_of(rows - 1, first_token);
+    const int most = unit.limit(walk.q, walk.kv, first_token);  // tokens from here on by none
+
+    float o[kN][8][4], sum[kN][2], ref[kN][2], bar_at[kN][2];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) sum[n][k] = ref[n][k] = 0.f, bar_at[n][k] = -INFINITY;
+    }
+
+    // 16 tokens from `tok` on, their keys at shared address `ka`
+    auto step = [&](uint32_t ka, int tok, auto masked) {
+      float s[kN][4];
+      {
+        const uint32_t aa = ka + tok_a * kQuantRow, ab = ka + tok_b * kQuantRow;
+        const uint4 wa4 = lds128(aa + 16 * t), wb4 = lds128(ab + 16 * t);
+        const uint32_t za = lds32(aa + kQuantCodes + 4 * t), zb = lds32(ab + kQuantCodes + 4 * t);
+        const uint4 pa4 = lds128(aa + kQuantCodes), pb4 = lds128(ab + kQuantCodes);
+        const uint32_t wa[4] = {wa4.x, wa4.y, wa4.z, wa4.w}, wb[4] = {wb4.x, wb4.y, wb4.z, wb4.w};
+        const uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
+        const uint32_t za_frag[4] = {za, zb, za, zb};
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+          mma_16816<true>(s[n], za_frag, zf[n][0], zf[n][1]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[n][k] *= 0x1p-10f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a0[4] = {wa[i] & kLow, wb[i] & kLow, wa[i] & kHigh, wb[i] & kHigh};
+          const uint32_t xa = wa[i] >> 8, xb = wb[i] >> 8;
+          const uint32_t a1[4] = {xa & kLow, xb & kLow, xa & kHigh, xb & kHigh};
+          const float fa = high_half(pa[i]), fb = high_half(pb[i]);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_16816<true>(x, a0, qf[n][4 * i], qf[n][4 * i + 1]);
+            mma_16816<true>(x, a1, qf[n][4 * i + 2], qf[n][4 * i + 3]);
+            s[n][0] = fmaf(fa, x[0], s[n][0]), s[n][1] = fmaf(fa, x[1], s[n][1]);
+            s[n][2] = fmaf(fb, x[2], s[n][2]), s[n][3] = fmaf(fb, x[3], s[n][3]);
+          }
+        }
+      }
+      const uint32_t va = ka + kTileBytes;
+      if constexpr (masked.value) {
+        // a value that is NaN makes the scores of its token NaN, and is 0 itself (below): rows that do not see it keep
+        // their sums
+        const uint4 pa = lds128(va + tok_a * kQuantRow + kQuantCodes), pb = lds128(va + tok_b * kQuantRow + kQuantCodes);
+        const bool na = odd_par(pa.x) || odd_par(pa.y) || odd_par(pa.z) || odd_par(pa.w);
+        const bool nb = odd_par(pb.x) || odd_par(pb.y) || odd_par(pb.z) || odd_par(pb.w);
+        const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            s[n][k] = tok + tok_a < lim[n][k] ? (na ? nan : s[n][k]) : -INFINITY;
+            s[n][2 + k] = tok + tok_b < lim[n][k] ? (nb ? nan : s[n][2 + k]) : -INFINITY;
+          }
+        }
+      }
+      bool move = false;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // (a masked score times a factor of 0 or infinity stays -inf)
+          if (masked.value)
+            s[n][k] = s[n][k] == -INFINITY ? -INFINITY : s[n][k] * mult[n][k & 1];
+          else
+            s[n][k] *= mult[n][k & 1];
+        }
+        move = move || fmaxf(s[n][0], s[n][2]) > bar_at[n][0] || fmaxf(s[n][1], s[n][3]) > bar_at[n][1];
+      }
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float top = fmaxf(s[n][k], s[n][2 + k]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            if (top > bar_at[n][k]) {
+              // weights up to 2^6 from here on, to 2^14 before the next move: fp16 holds 2^-24 of them
+              const float f = bar_at[n][k] == -INFINITY ? 0.f : ex2(ref[n][k] - (top - 6.f));
+              ref[n][k] = top - 6.f, bar_at[n][k] = top + 8.f;
+              sum[n][k] *= f;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[n][j][k] *= f, o[n][j][2 + k] *= f;
+            }
+          }
+        }
+      }
+      uint32_t pf[kN][2];
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e[k] = ex2(s[n][k] - ref[n][k & 1]);
+        sum[n][0] += e[0] + e[2], sum[n][1] += e[1] + e[3];
+        pf[n][0] = trans8x8(pack2<true>(e[0], e[1]));
+        pf[n][1] = trans8x8(pack2<true>(e[2], e[3]));
+      }
+      // values: lane (g, t) has d = words 2 g, 2 g + 1 of four tokens, whose groups are 2 (g % 2) and the next
+      uint2 w[4], par[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = lds64(va + vt[j] * kQuantRow + 8 * g);
+        par[j] = lds64(va + vt[j] * kQuantRow + kQuantCodes + 8 * (g & 1));
+        if constexpr (masked.value) {
+          if (tok + vt[j] >= most || odd_par(par[j].x)) par[j].x = 0;
+          if (tok + vt[j] >= most || odd_par(par[j].y)) par[j].y = 0;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        auto word = [&](int j) { return i ? w[j].y : w[j].x; };
+        auto pr = [&](int j) { return i ? par[j].y : par[j].x; };
+        __half2 sc[2], off[2];
+        uint32_t x[2][2];  // [token pair][half of the word]
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          sc[j] = as_half2(__byte_perm(pr(2 * j), pr(2 * j + 1), 0x7632));
+          off[j] = as_half2(__byte_perm(pr(2 * j), pr(2 * j + 1), 0x5410));
+          x[j][0] = __byte_perm(word(2 * j), word(2 * j + 1), 0x5410);
+          x[j][1] = __byte_perm(word(2 * j), word(2 * j + 1), 0x7632);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t a[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t y = k < 2 ? x[j >> 1][j & 1] << 1 : x[j >> 1][j & 1] >> 7;
+            a[j] = as_u32(__hfma2(k & 1 ? high_code(y) : low_code(y), sc[j >> 1], off[j >> 1]));
+          }
+#pragma unroll
+          for (int n = 0; n < kN; ++n) mma_16816<true>(o[n][4 * i + k], a, pf[n][0], pf[n][1]);
+        }
+      }
+    };
+
+    for (int j = 0; j < walk.n; ++j) {
+      const int stage = done % kStages;
+      live = mbar_wait_warp(&bar[stage], (done / kStages) & 1);
+      if (!live) break;
+      const uint32_t at = base + stage * 2 * kTileBytes;
+      const int tok = (walk.t0 + j) * kTok;
+#pragma unroll 1
+      for (int k = 0; k < kTok; k += 16) {
+        if (tok + k + 16 <= clean)
+          step(at + k * kQuantRow, tok + k, std::false_type());
+        else if (tok + k < most)
+          step(at + k * kQuantRow, tok + k, std::true_type());
+      }
+      __syncwarp();
+      ++done;
+      issue();
+    }
+    if (!live) break;
+
+    // --------------------------------------------------------------- output
+    const bool whole = walk.starts && walk.ends;
+    const int32_t info =
+        walk.starts && !walk.ends ? cut_info(c, walk.base + unit.tiles(walk.q, walk.kv, walk.block) - 1, total, runs) : 0;
+    const int64_t slot = (static_cast<int64_t>(walk.starts ? 2 * c + 1 : 2 * c) * p.kv_heads + h) * kRows;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float l = sum[n][k];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        const int r = n * 8 + 2 * t + k;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float lse = l == 0.f ? -INFINITY : (ref[n][k] + __log2f(l)) * 0.6931471805599453f;
+        if (r >= rows) continue;
+        int i;
+        const int64_t row = row_of(r, i);
+        if (g == 0) {
+          if (walk.starts) P.parts.row_info[row] = info ? info + r : 0;
+          if (whole)
+            p.lse[row] = lse;
+          else
+            P.parts.lse[slot + r] = lse;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = 32 * ((2 * g + j) & 3) + 8 * ((2 * g + j) >> 2);
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = o[n][4 * j + e][k] * inv, y[4 + e] = o[n][4 * j + e][2 + k] * inv;
+          if (whole) {
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * kHeadDim + d) =
+                make_uint4(pack2<kFp16>(y[0], y[1]), pack2<kFp16>(y[2], y[3]), pack2<kFp16>(y[4], y[5]), pack2<kFp16>(y[6], y[7]));
+          } else {
+            float4* dst = reinterpret_cast<float4*>(P.parts.o + (slot + r) * kHeadDim + d);
+            dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+            dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+          }
+        }
+      }
+    }
+  }
+  if (!live) {  // an aborted call: this warp's loads in flight land before it leaves
+    for (; done < issued; ++done) mbar_wait_drain(&bar[done % kStages], (done / kStages) & 1);
+  }
 }
 
-template <bool kFp16>
-__global__ void __launch_bounds__(kThreads) quant_decode_kernel(const __grid_constant__ QuantDecodeLaunch p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / 32;
-  if (row >= p.num_tokens * p.num_heads) return;
-  const int64_t tok = row / p.num_heads;
-  const int h = static_cast<int>(row % p.num_heads) / p.group;
-  int64_t b = 0, first = 0, q = p.q_len;
-  if (p.q_len > 0) {
-    b = tok / p.q_len, first = b * p.q_len;
-  } else {
-    for (; b < p.batch; ++b) {
-      q = min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens - first);
-      if (tok < first + q) break;
-      first += q;
-    }
-    if (b == p.batch) return;  // no request's token
-  }
-  const int64_t kv = min(max(p.kv_lens[b], static_cast<int64_t>(0)), static_cast<int64_t>(p.block_cols) * p.block_size);
-  const int64_t n = p.causal ? max(static_cast<int64_t>(0), kv - q + (tok - first) + 1) : kv;
-  const uint2 qw = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.query) + row * kHeadDim + 4 * lane);
-  const uint32_t w[2] = {qw.x, qw.y};
-  float x[4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float2 f = kFp16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[i]))
-                           : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-    x[2 * i] = f.x, x[2 * i + 1] = f.y;
-  }
-  float m = -INFINITY, o[4] = {};
-  double sum = 0.;  // (one after the other: n roundings of fp32 would show)
-  bool nan = false;
-  for (int64_t t = 0; t < n; ++t) {
-    const int64_t page = p.block_table[b * p.block_cols + t / p.block_size];
-    const bool bad = page < 0 || page >= p.num_blocks;
-    if (bad && lane == 0) atomicOr(&g_cascade_device_error, kErrBadBlockId);
-    const int64_t at = ((page * p.block_size + t % p.block_size) * p.kv_heads + h) * kQuantRow;
-    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4 k = bad ? zero : row_values(p.key + at, lane), v = bad ? zero : row_values(p.value + at, lane);
-    float s = x[0] * k.x + x[1] * k.y + x[2] * k.z + x[3] * k.w;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= p.scale * 1.4426950408889634f;
-    nan = nan || !(s < INFINITY);
-    if (s > m) {
-      const float f = ex2(m - s);
-      sum *= f, m = s;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] *= f;
-    }
-    const float e = m == -INFINITY ? 0.f : ex2(s - m);
-    sum += e;
-    o[0] = fmaf(e, v.x, o[0]), o[1] = fmaf(e, v.y, o[1]), o[2] = fmaf(e, v.z, o[2]), o[3] = fmaf(e, v.w, o[3]);
-  }
-  float l = static_cast<float>(sum);
-  if (nan) l = __int_as_float(0x7fffffff);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + row * kHeadDim + 4 * lane) =
-      make_uint2(pack2<kFp16>(o[0] * inv, o[1] * inv), pack2<kFp16>(o[2] * inv, o[3] * inv));
-  if (lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+// Runs per kv head: as many warps as are resident, no more than there are tiles.
+template <int kN>
+int run_count(const QuantDecodeLaunch& p) {
+  const int64_t warps = static_cast<int64_t>(kNumSMs) * Shape<kN>::kCtas * kWarps;
+  const int64_t rows = p.num_tokens * p.group, units = p.batch + rows / Shape<kN>::kRows;
+  const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(p.block_cols) * p.block_size + kTok - 1) / kTok);
+  const int64_t most = std::min<int64_t>(units, 1 << 20) * (kSetup + tiles);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, warps / p.kv_heads, kMaxRuns})));
 }
+
+template <bool kFp16, int kN>
+cudaError_t launch(const QuantDecodeLaunch& p, void* workspace, cudaStream_t stream) {
+  using S = Shape<kN>;
+  Params P;
+  P.L = p;
+  const int runs = run_count<kN>(p);
+  P.parts = quant_partials(p, runs, S::kRows, workspace);
+  P.box_rows = std::min(kTok, p.block_size);
+  // no pages at all: maps over one row of the query stand in, nothing is loaded through them
+  const bool any = p.num_blocks > 0;
+  const uint64_t inner = any ? static_cast<uint64_t>(p.kv_heads) * kQuantRow : 128;
+  const uint64_t rows = any ? static_cast<uint64_t>(p.num_blocks) * p.block_size : 1;
+  if (!encode_tmap_bytes(&P.key, any ? p.key : p.query, inner, rows, inner, kQuantRow, P.box_rows) ||
+      !encode_tmap_bytes(&P.value, any ? p.value : p.query, inner, rows, inner, kQuantRow, P.box_rows))
+    return cudaErrorInvalidValue;
+  auto kern = quant_decode_kernel<kFp16, kN>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), S::kSmem);
+  if (e != cudaSuccess) return e;
+  const int64_t warps = static_cast<int64_t>(runs) * p.kv_heads;
+  kern<<<static_cast<unsigned>((warps + kWarps - 1) / kWarps), 32 * kWarps, S::kSmem, stream>>>(P);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || runs == 1) return e;
+  return launch_quant_combine<kFp16, S::kRows>(p, P.parts, stream);
+}
+
+// Query rows per warp: 16 where a request has more than 8 (known from the shapes: the mean, with lengths on the device).
+bool wide(const QuantDecodeLaunch& p) { return p.num_tokens * p.group > 8 * static_cast<int64_t>(p.batch); }
 
 }  // namespace
 
-size_t quant_decode_workspace(const QuantDecodeLaunch&) { return 0; }
+size_t quant_decode_workspace(const QuantDecodeLaunch& p) {
+  return wide(p) ? quant_partial_bytes(p, run_count<2>(p), Shape<2>::kRows) : quant_partial_bytes(p, run_count<1>(p), Shape<1>::kRows);
+}
 
-cudaError_t launch_quant_decode(const QuantDecodeLaunch& p, bool fp16, void*, cudaStream_t stream) {
-  const int64_t rows = p.num_tokens * p.num_heads;
-  (fp16 ? quant_decode_kernel<true> : quant_decode_kernel<false>)
-      <<<static_cast<unsigned>((rows * 32 + kThreads - 1) / kThreads), kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_quant_decode(const QuantDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
+  if (wide(p)) return fp16 ? launch<true, 2>(p, workspace, stream) : launch<false, 2>(p, workspace, stream);
+  return fp16 ? launch<true, 1>(p, workspace, stream) : launch<false, 1>(p, workspace, stream);
 }
 
 }  // namespace cascade
