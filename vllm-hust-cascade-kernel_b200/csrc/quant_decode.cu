@@ -35,16 +35,16 @@ namespace {
 
 constexpr int kTok = 32;     // tokens per tile
 constexpr int kSetup = 2;    // what a new unit costs, in tiles
-constexpr int kWarps = 4;
 constexpr int kTileBytes = kTok * kQuantRow;  // of keys or of values
 constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kMagic = 0x64006400u;
 
 template <int kN>  // query rows / 8
 struct Shape {
   static constexpr int kRows = 8 * kN;
-  static constexpr int kCtas = kN == 1 ? 4 : 3;    // per SM
+  static constexpr int kWarps = kN == 1 ? 16 : 12;
   static constexpr int kStages = kN == 1 ? 2 : 3;  // tiles of keys and values per warp
-  static constexpr int kSmem = kWarps * kStages * 2 * kTileBytes + 128;  // (to align the ring: the TMA writes to 128-byte boundaries)
+  static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;
+  static constexpr int kSmem = kRing + 128;  // (to align the ring: the TMA writes to 128-byte boundaries)
 };
 
 struct Params {
@@ -88,19 +88,29 @@ __device__ __forceinline__ __half2 high_code(uint32_t x) {
 // centre or scale NaN (or infinite) in either half
 __device__ __forceinline__ bool odd_par(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
 
-// Token (of 16) of row m = g or g + 8 of the scores' product.
-__device__ __forceinline__ int token_lo(int g) { return g & 1 ? 8 + ((g + 3) & 7) : g; }
-__device__ __forceinline__ int token_hi(int g) { return g & 1 ? 8 + ((g + 4) & 7) : g + 1; }
+// d = a b, nothing added
+__device__ __forceinline__ void mma_fresh(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Token (of 16) of row m = g of the scores' product; row g + 8 is the token after it. Two rows next to one another are 4 (or
+// 12) tokens apart, 16 banks; the tokens 2 t, 2 t + 1 and 8 + (2 t + 4) % 8 and its next are the columns 2 t, 2 t + 8, 2 t + 1
+// and 2 t + 9 of the probabilities.
+__device__ __forceinline__ int token_of(int g) { return g & 1 ? 8 + ((g + 3) & 7) : g; }
 
 template <bool kFp16, int kN>
-__global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_kernel(const __grid_constant__ Params P) {
+__global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel(const __grid_constant__ Params P) {
   using S = Shape<kN>;
-  constexpr int kRows = S::kRows, kStages = S::kStages;
+  constexpr int kRows = S::kRows, kStages = S::kStages, kWarps = S::kWarps;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ uint64_t stall;
   const QuantDecodeLaunch& p = P.L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem_raw + ((0u - smem_u32(smem_raw)) & 127u);
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
@@ -126,71 +136,62 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_ke
   }
   if (c >= runs) return;
 
-  uint8_t* mine = smem_raw + ((0u - smem_u32(smem_raw)) & 127u) + warp * kStages * 2 * kTileBytes;
-  uint64_t* bar = full[warp];
+  uint8_t* mine = ring + warp * kStages * 2 * kTileBytes;
   const uint32_t base = smem_u32(mine);
+  int issued = 0, done = 0;
   bool live = true;
   if (p.debug_stall) live = mbar_wait_warp(&stall, 0);  // test hook: runs into the wait limit
 
-  // ------------------------------------------------------------------ loads
-  QuantWalk<kRows, kTok, kSetup> load(p, run);
-  int load_left = 0, load_tile = 0;
-  int issued = 0, done = 0;
-  int ids = 0, ids_next = 0, ids_at = 0;  // this lane's of 32 page ids from page ids_at on, and of the 32 after them
-  const int shift = __ffs(p.block_size) - 1, oob = p.num_blocks ? p.num_blocks * p.block_size : 1;
-  auto page_ids = [&](int at) {
-    const int i = at + lane;
-    return i < p.block_cols ? p.block_table[static_cast<int64_t>(load.b) * p.block_cols + i] : -1;
-  };
-  auto issue = [&] {
-    if (load_left == 0) {
-      if (!load.next()) return;
-      load_left = load.n, load_tile = load.t0;
-      ids_at = (load_tile * kTok) >> shift;
-      ids = page_ids(ids_at), ids_next = page_ids(ids_at + 32);
-    }
-    const int tok = load_tile * kTok, stage = issued % kStages;
-    uint8_t* dst = mine + stage * 2 * kTileBytes;
-    const int boxes = kTok / P.box_rows;  // one or two
-    int rows[2];
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int at = tok + i * P.box_rows;
-      if (i >= boxes || (i > 0 && at >= load.kv) ) break;
-      const int page = at >> shift;
-      if (page >= ids_at + 32) ids_at += 32, ids = ids_next, ids_next = page_ids(ids_at + 32);
-      const int32_t page_id = __shfl_sync(0xffffffffu, ids, page - ids_at);
-      // (a unit without tokens has a tile all the same: nothing of it is used)
-      rows[n++] = at >= load.kv ? oob : static_cast<uint32_t>(page_id) < static_cast<uint32_t>(p.num_blocks)
-                      ? page_id * p.block_size + (at & (p.block_size - 1))
-                      : -1;
-    }
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&bar[stage], n * 2 * P.box_rows * kQuantRow);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (i >= n) break;
-        if (rows[i] < 0) {
-          atomicOr(&g_cascade_device_error, kErrBadBlockId);
-          rows[i] = oob;
-        }
-        tma_load_2d(dst + i * P.box_rows * kQuantRow, &P.key, &bar[stage], h * kQuantRow, rows[i]);
-        tma_load_2d(dst + kTileBytes + i * P.box_rows * kQuantRow, &P.value, &bar[stage], h * kQuantRow, rows[i]);
-      }
-    }
-    __syncwarp();
-    ++issued, ++load_tile, --load_left;
-  };
-  if (live)
-    for (int i = 0; i < kStages; ++i) issue();
-
-  // per-lane offsets in a 16-token step
-  const int tok_a = token_lo(g), tok_b = token_hi(g);
-  const int vt[4] = {2 * t, 8 + ((2 * t + 4) & 7), 2 * t + 1, 8 + ((2 * t + 5) & 7)};
+  // this lane's places in 16 tokens: keys' codes, their centres and scales; values' (of two of four tokens)
+  const uint32_t off_k = token_of(g) * kQuantRow + 16 * t, off_kp = token_of(g) * kQuantRow + kQuantCodes;
+  const uint32_t off_v0 = 2 * t * kQuantRow + 8 * g, off_v1 = (8 + ((2 * t + 4) & 7)) * kQuantRow + 8 * g;
+  const uint32_t off_p0 = 2 * t * kQuantRow + kQuantCodes + 8 * (g & 1), off_p1 = off_p0 + off_v1 - off_v0;
 
   QuantWalk<kRows, kTok, kSetup> walk(p, run);
+  const int shift = __ffs(p.block_size) - 1, oob = p.num_blocks ? p.num_blocks * p.block_size : 1;
   while (live && walk.next()) {
+    // ---------------------------------------------------------------- loads
+    // cache rows of the boxes (one or two per tile) of this lane's of 32 tiles, and of the 32 after them
+    const bool two = P.box_rows < kTok;
+    int rows_now[2], rows_next[2];
+    int next_tile = walk.t0, rows_at = walk.t0;
+    auto tile_rows = [&](int tile, int (&row)[2]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = tile * kTok + i * 16;
+        row[i] = oob;  // (a unit without tokens has a tile all the same: nothing of it is used)
+        if (at < walk.kv && tile < walk.t0 + walk.n && (i == 0 || two)) {
+          const int32_t page = p.block_table[static_cast<int64_t>(walk.b) * p.block_cols + (at >> shift)];
+          if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.num_blocks))
+            row[i] = page * p.block_size + (at & (p.block_size - 1));
+          else
+            atomicOr(&g_cascade_device_error, kErrBadBlockId);
+        }
+      }
+    };
+    tile_rows(walk.t0 + lane, rows_now);
+    auto issue = [&] {
+      if (next_tile - rows_at == 32) rows_at = next_tile, rows_now[0] = rows_next[0], rows_now[1] = rows_next[1];
+      if (next_tile == rows_at) tile_rows(next_tile + 32 + lane, rows_next);
+      const int row0 = __shfl_sync(0xffffffffu, rows_now[0], next_tile - rows_at);
+      const int row1 = two ? __shfl_sync(0xffffffffu, rows_now[1], next_tile - rows_at) : 0;
+      if (elect_one()) {
+        const int stage = issued % kStages;
+        uint64_t* bar = &full[warp][stage];
+        uint8_t* dst = mine + stage * 2 * kTileBytes;
+        mbar_arrive_expect_tx(bar, 2 * kTileBytes);
+        tma_load_2d(dst, &P.key, bar, h * kQuantRow, row0);
+        tma_load_2d(dst + kTileBytes, &P.value, bar, h * kQuantRow, row0);
+        if (two) {
+          tma_load_2d(dst + kTileBytes / 2, &P.key, bar, h * kQuantRow, row1);
+          tma_load_2d(dst + kTileBytes + kTileBytes / 2, &P.value, bar, h * kQuantRow, row1);
+        }
+      }
+      __syncwarp();
+      ++issued, ++next_tile;
+    };
+    for (int i = 0; i < min(kStages, walk.n); ++i) issue();
+
     // ---------------------------------------------------------------- query
     // row n of this block as the products' columns: lane (g, t) has d = 32 i + 8 t + 0..7 of row 8 n + g
     const int rows = min(kRows, walk.q * p.group - walk.block * kRows);  // of this unit
@@ -270,23 +271,23 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_ke
       for (int k = 0; k < 2; ++k) sum[n][k] = ref[n][k] = 0.f, bar_at[n][k] = -INFINITY;
     }
 
-    // 16 tokens from `tok` on, their keys at shared address `ka`
+    // a tile: 32 tokens from `tok` on, their keys at shared address `ka`
     auto step = [&](uint32_t ka, int tok, auto masked) {
-      float s[kN][4];
-      {
-        const uint32_t aa = ka + tok_a * kQuantRow, ab = ka + tok_b * kQuantRow;
-        const uint4 wa4 = lds128(aa + 16 * t), wb4 = lds128(ab + 16 * t);
-        const uint32_t za = lds32(aa + kQuantCodes + 4 * t), zb = lds32(ab + kQuantCodes + 4 * t);
-        const uint4 pa4 = lds128(aa + kQuantCodes), pb4 = lds128(ab + kQuantCodes);
+      float s[2][kN][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t a = ka + u * 16 * kQuantRow;
+        const uint4 wa4 = lds128(a + off_k), wb4 = lds128(a + off_k + kQuantRow);
+        const uint4 pa4 = lds128(a + off_kp), pb4 = lds128(a + off_kp + kQuantRow);
+        const uint32_t za = lds32(a + off_kp + 4 * t), zb = lds32(a + off_kp + kQuantRow + 4 * t);
         const uint32_t wa[4] = {wa4.x, wa4.y, wa4.z, wa4.w}, wb[4] = {wb4.x, wb4.y, wb4.z, wb4.w};
         const uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
-        const uint32_t za_frag[4] = {za, zb, za, zb};
+        const uint32_t z[4] = {za, zb, za, zb};
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
-          s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-          mma_16816<true>(s[n], za_frag, zf[n][0], zf[n][1]);
+          mma_fresh(s[u][n], z, zf[n][0], zf[n][1]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[n][k] *= 0x1p-10f;
+          for (int k = 0; k < 4; ++k) s[u][n][k] *= 0x1p-10f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -296,11 +297,11 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_ke
           const float fa = high_half(pa[i]), fb = high_half(pb[i]);
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
-            float x[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_16816<true>(x, a0, qf[n][4 * i], qf[n][4 * i + 1]);
+            float x[4];
+            mma_fresh(x, a0, qf[n][4 * i], qf[n][4 * i + 1]);
             mma_16816<true>(x, a1, qf[n][4 * i + 2], qf[n][4 * i + 3]);
-            s[n][0] = fmaf(fa, x[0], s[n][0]), s[n][1] = fmaf(fa, x[1], s[n][1]);
-            s[n][2] = fmaf(fb, x[2], s[n][2]), s[n][3] = fmaf(fb, x[3], s[n][3]);
+            s[u][n][0] = fmaf(fa, x[0], s[u][n][0]), s[u][n][1] = fmaf(fa, x[1], s[u][n][1]);
+            s[u][n][2] = fmaf(fb, x[2], s[u][n][2]), s[u][n][3] = fmaf(fb, x[3], s[u][n][3]);
           }
         }
       }
@@ -308,16 +309,21 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_ke
       if constexpr (masked.value) {
         // a value that is NaN makes the scores of its token NaN, and is 0 itself (below): rows that do not see it keep
         // their sums
-        const uint4 pa = lds128(va + tok_a * kQuantRow + kQuantCodes), pb = lds128(va + tok_b * kQuantRow + kQuantCodes);
-        const bool na = odd_par(pa.x) || odd_par(pa.y) || odd_par(pa.z) || odd_par(pa.w);
-        const bool nb = odd_par(pb.x) || odd_par(pb.y) || odd_par(pb.z) || odd_par(pb.w);
-        const float nan = __int_as_float(0x7fffffff);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t at = va + u * 16 * kQuantRow + off_kp;
+          const uint4 pa = lds128(at), pb = lds128(at + kQuantRow);
+          const bool na = odd_par(pa.x) || odd_par(pa.y) || odd_par(pa.z) || odd_par(pa.w);
+          const bool nb = odd_par(pb.x) || odd_par(pb.y) || odd_par(pb.z) || odd_par(pb.w);
+          const float nan = __int_as_float(0x7fffffff);
+          const int mine = tok + u * 16 + token_of(g);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            s[n][k] = tok + tok_a < lim[n][k] ? (na ? nan : s[n][k]) : -INFINITY;
-            s[n][2 + k] = tok + tok_b < lim[n][k] ? (nb ? nan : s[n][2 + k]) : -INFINITY;
+          for (int n = 0; n < kN; ++n) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              s[u][n][k] = mine < lim[n][k] ? (na ? nan : s[u][n][k]) : -INFINITY;
+              s[u][n][2 + k] = mine + 1 < lim[n][k] ? (nb ? nan : s[u][n][2 + k]) : -INFINITY;
+            }
           }
         }
       }
@@ -325,21 +331,26 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_ke
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          // (a masked score times a factor of 0 or infinity stays -inf)
-          if (masked.value)
-            s[n][k] = s[n][k] == -INFINITY ? -INFINITY : s[n][k] * mult[n][k & 1];
-          else
-            s[n][k] *= mult[n][k & 1];
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            // (a masked score times a factor of 0 or infinity stays -inf)
+            if (masked.value)
+              s[u][n][k] = s[u][n][k] == -INFINITY ? -INFINITY : s[u][n][k] * mult[n][k & 1];
+            else
+              s[u][n][k] *= mult[n][k & 1];
+          }
         }
-        move = move || fmaxf(s[n][0], s[n][2]) > bar_at[n][0] || fmaxf(s[n][1], s[n][3]) > bar_at[n][1];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          move = move || fmaxf(fmax3f(s[0][n][k], s[0][n][2 + k], s[1][n][k]), s[1][n][2 + k]) > bar_at[n][k];
       }
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            float top = fmaxf(s[n][k], s[n][2 + k]);
+            float top = fmaxf(fmax3f(s[0][n][k], s[0][n][2 + k], s[1][n][k]), s[1][n][2 + k]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             if (top > bar_at[n][k]) {
@@ -353,70 +364,71 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_ke
           }
         }
       }
-      uint32_t pf[kN][2];
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        float e[4];
+      for (int u = 0; u < 2; ++u) {
+        uint32_t pf[kN][2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = ex2(s[n][k] - ref[n][k & 1]);
-        sum[n][0] += e[0] + e[2], sum[n][1] += e[1] + e[3];
-        pf[n][0] = trans8x8(pack2<true>(e[0], e[1]));
-        pf[n][1] = trans8x8(pack2<true>(e[2], e[3]));
-      }
-      // values: lane (g, t) has d = words 2 g, 2 g + 1 of four tokens, whose groups are 2 (g % 2) and the next
-      uint2 w[4], par[4];
+        for (int n = 0; n < kN; ++n) {
+          float e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = lds64(va + vt[j] * kQuantRow + 8 * g);
-        par[j] = lds64(va + vt[j] * kQuantRow + kQuantCodes + 8 * (g & 1));
+          for (int k = 0; k < 4; ++k) e[k] = ex2(s[u][n][k] - ref[n][k & 1]);
+          sum[n][0] += e[0] + e[2], sum[n][1] += e[1] + e[3];
+          pf[n][0] = trans8x8(pack2<true>(e[0], e[1]));
+          pf[n][1] = trans8x8(pack2<true>(e[2], e[3]));
+        }
+        // values: lane (g, t) has d = words 2 g, 2 g + 1 of four tokens, whose groups are 2 (g % 2) and the next
+        const uint32_t a = va + u * 16 * kQuantRow;
+        const uint2 w[4] = {lds64(a + off_v0), lds64(a + off_v1), lds64(a + off_v0 + kQuantRow), lds64(a + off_v1 + kQuantRow)};
+        uint2 par[4] = {lds64(a + off_p0), lds64(a + off_p1), lds64(a + off_p0 + kQuantRow), lds64(a + off_p1 + kQuantRow)};
         if constexpr (masked.value) {
-          if (tok + vt[j] >= most || odd_par(par[j].x)) par[j].x = 0;
-          if (tok + vt[j] >= most || odd_par(par[j].y)) par[j].y = 0;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        auto word = [&](int j) { return i ? w[j].y : w[j].x; };
-        auto pr = [&](int j) { return i ? par[j].y : par[j].x; };
-        __half2 sc[2], off[2];
-        uint32_t x[2][2];  // [token pair][half of the word]
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          sc[j] = as_half2(__byte_perm(pr(2 * j), pr(2 * j + 1), 0x7632));
-          off[j] = as_half2(__byte_perm(pr(2 * j), pr(2 * j + 1), 0x5410));
-          x[j][0] = __byte_perm(word(2 * j), word(2 * j + 1), 0x5410);
-          x[j][1] = __byte_perm(word(2 * j), word(2 * j + 1), 0x7632);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t a[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint32_t y = k < 2 ? x[j >> 1][j & 1] << 1 : x[j >> 1][j & 1] >> 7;
-            a[j] = as_u32(__hfma2(k & 1 ? high_code(y) : low_code(y), sc[j >> 1], off[j >> 1]));
+            const int mine = tok + u * 16 + (j & 1 ? 8 + ((2 * t + 4) & 7) : 2 * t) + (j >> 1);
+            if (mine >= most || odd_par(par[j].x)) par[j].x = 0;
+            if (mine >= most || odd_par(par[j].y)) par[j].y = 0;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          auto word = [&](int j) { return i ? w[j].y : w[j].x; };
+          auto pr = [&](int j) { return i ? par[j].y : par[j].x; };
+          __half2 sc[2], off[2];
+          uint32_t x[2][2];  // [token pair][half of the word]
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            sc[j] = as_half2(__byte_perm(pr(2 * j), pr(2 * j + 1), 0x7632));
+            off[j] = as_half2(__byte_perm(pr(2 * j), pr(2 * j + 1), 0x5410));
+            x[j][0] = __byte_perm(word(2 * j), word(2 * j + 1), 0x5410);
+            x[j][1] = __byte_perm(word(2 * j), word(2 * j + 1), 0x7632);
           }
 #pragma unroll
-          for (int n = 0; n < kN; ++n) mma_16816<true>(o[n][4 * i + k], a, pf[n][0], pf[n][1]);
+          for (int k = 0; k < 4; ++k) {
+            uint32_t f[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t y = k < 2 ? x[j >> 1][j & 1] << 1 : x[j >> 1][j & 1] >> 7;
+              f[j] = as_u32(__hfma2(k & 1 ? high_code(y) : low_code(y), sc[j >> 1], off[j >> 1]));
+            }
+#pragma unroll
+            for (int n = 0; n < kN; ++n) mma_16816<true>(o[n][4 * i + k], f, pf[n][0], pf[n][1]);
+          }
         }
       }
     };
 
     for (int j = 0; j < walk.n; ++j) {
       const int stage = done % kStages;
-      live = mbar_wait_warp(&bar[stage], (done / kStages) & 1);
+      live = mbar_wait_warp(&full[warp][stage], (done / kStages) & 1);
       if (!live) break;
       const uint32_t at = base + stage * 2 * kTileBytes;
       const int tok = (walk.t0 + j) * kTok;
-#pragma unroll 1
-      for (int k = 0; k < kTok; k += 16) {
-        if (tok + k + 16 <= clean)
-          step(at + k * kQuantRow, tok + k, std::false_type());
-        else if (tok + k < most)
-          step(at + k * kQuantRow, tok + k, std::true_type());
-      }
+      if (tok + kTok <= clean)
+        step(at, tok, std::false_type());
+      else if (tok < most)
+        step(at, tok, std::true_type());
       __syncwarp();
       ++done;
-      issue();
+      if (next_tile < walk.t0 + walk.n) issue();
     }
     if (!live) break;
 
@@ -464,14 +476,14 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<kN>::kCtas) quant_decode_ke
     }
   }
   if (!live) {  // an aborted call: this warp's loads in flight land before it leaves
-    for (; done < issued; ++done) mbar_wait_drain(&bar[done % kStages], (done / kStages) & 1);
+    for (; done < issued; ++done) mbar_wait_drain(&full[warp][done % kStages], (done / kStages) & 1);
   }
 }
 
 // Runs per kv head: as many warps as are resident, no more than there are tiles.
 template <int kN>
 int run_count(const QuantDecodeLaunch& p) {
-  const int64_t warps = static_cast<int64_t>(kNumSMs) * Shape<kN>::kCtas * kWarps;
+  const int64_t warps = static_cast<int64_t>(kNumSMs) * Shape<kN>::kWarps;
   const int64_t rows = p.num_tokens * p.group, units = p.batch + rows / Shape<kN>::kRows;
   const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(p.block_cols) * p.block_size + kTok - 1) / kTok);
   const int64_t most = std::min<int64_t>(units, 1 << 20) * (kSetup + tiles);
@@ -497,7 +509,7 @@ cudaError_t launch(const QuantDecodeLaunch& p, void* workspace, cudaStream_t str
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), S::kSmem);
   if (e != cudaSuccess) return e;
   const int64_t warps = static_cast<int64_t>(runs) * p.kv_heads;
-  kern<<<static_cast<unsigned>((warps + kWarps - 1) / kWarps), 32 * kWarps, S::kSmem, stream>>>(P);
+  kern<<<static_cast<unsigned>((warps + S::kWarps - 1) / S::kWarps), 32 * S::kWarps, S::kSmem, stream>>>(P);
   e = cudaGetLastError();
   if (e != cudaSuccess || runs == 1) return e;
   return launch_quant_combine<kFp16, S::kRows>(p, P.parts, stream);
