@@ -36,7 +36,7 @@ namespace {
 constexpr int kTok = 32;     // tokens per tile
 constexpr int kSetup = 2;    // what a new unit costs, in tiles
 constexpr int kTileBytes = kTok * kQuantRow;  // of keys or of values
-constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kMagic = 0x64006400u;
+constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
 
 template <int kN>  // query rows / 8
 struct Shape {
@@ -77,13 +77,18 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 __device__ __forceinline__ float high_half(uint32_t x) { return __high2float(as_half2(x)); }
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
 // One nibble of two tokens' half words as code - 7.5, exactly: over fp16's 1024 the bits 1..4 are 1024 + 2 code, the bits 5..8
 // 1024 + 32 code. (At bit 0 the 7.5 would be half a step.)
-__device__ __forceinline__ __half2 low_code(uint32_t x) {
-  return __hfma2(as_half2((x & 0x001E001Eu) | kMagic), __float2half2_rn(0.5f), __float2half2_rn(-519.5f));
+__device__ __forceinline__ __half2 low_code(uint32_t x, uint32_t magic) {
+  return __hfma2(as_half2(and_or(x, 0x001E001Eu, magic)), __float2half2_rn(0.5f), __float2half2_rn(-519.5f));
 }
-__device__ __forceinline__ __half2 high_code(uint32_t x) {
-  return __hfma2(as_half2((x & 0x01E001E0u) | kMagic), __float2half2_rn(0.03125f), __float2half2_rn(-39.5f));
+__device__ __forceinline__ __half2 high_code(uint32_t x, uint32_t magic) {
+  return __hfma2(as_half2(and_or(x, 0x01E001E0u, magic)), __float2half2_rn(0.03125f), __float2half2_rn(-39.5f));
 }
 // centre or scale NaN (or infinite) in either half
 __device__ __forceinline__ bool odd_par(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
@@ -141,6 +146,9 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
   int issued = 0, done = 0;
   bool live = true;
   if (p.debug_stall) live = mbar_wait_warp(&stall, 0);  // test hook: runs into the wait limit
+
+  uint32_t magic;  // (kept in a register: an immediate in the AND and one in the OR would take two instructions)
+  asm volatile("mov.u32 %0, 0x64006400;" : "=r"(magic));
 
   // this lane's places in 16 tokens: keys' codes, their centres and scales; values' (of two of four tokens)
   const uint32_t off_k = token_of(g) * kQuantRow + 16 * t, off_kp = token_of(g) * kQuantRow + kQuantCodes;
@@ -248,7 +256,8 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
       zf[n][0] = pack2<true>(z, y);
       const float2 hi = __half22float2(as_half2(zf[n][0]));
       zf[n][1] = pack2<true>(z - hi.x, y - hi.y);
-      const float m = (0x1p24f / f0 / f1) * (p.scale * 1.4426950408889634f);
+      // (not 0, nor NaN: a masked score, -inf, stays -inf)
+      const float m = fmaxf((0x1p24f / f0 / f1) * (p.scale * 1.4426950408889634f), 1e-37f);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         mult[n][k] = __shfl_sync(0xffffffffu, m, (2 * t + k) * 4);
@@ -331,17 +340,6 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // (a masked score times a factor of 0 or infinity stays -inf)
-            if (masked.value)
-              s[u][n][k] = s[u][n][k] == -INFINITY ? -INFINITY : s[u][n][k] * mult[n][k & 1];
-            else
-              s[u][n][k] *= mult[n][k & 1];
-          }
-        }
-#pragma unroll
         for (int k = 0; k < 2; ++k)
           move = move || fmaxf(fmax3f(s[0][n][k], s[0][n][2 + k], s[1][n][k]), s[1][n][2 + k]) > bar_at[n][k];
       }
@@ -355,8 +353,9 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             if (top > bar_at[n][k]) {
               // weights up to 2^6 from here on, to 2^14 before the next move: fp16 holds 2^-24 of them
-              const float f = bar_at[n][k] == -INFINITY ? 0.f : ex2(ref[n][k] - (top - 6.f));
-              ref[n][k] = top - 6.f, bar_at[n][k] = top + 8.f;
+              const float now = fmaf(top, mult[n][k], -6.f);
+              const float f = bar_at[n][k] == -INFINITY ? 0.f : ex2(ref[n][k] - now);
+              ref[n][k] = now, bar_at[n][k] = top + 8.f / mult[n][k];
               sum[n][k] *= f;
 #pragma unroll
               for (int j = 0; j < 8; ++j) o[n][j][k] *= f, o[n][j][2 + k] *= f;
@@ -371,7 +370,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
         for (int n = 0; n < kN; ++n) {
           float e[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) e[k] = ex2(s[u][n][k] - ref[n][k & 1]);
+          for (int k = 0; k < 4; ++k) e[k] = ex2(fmaf(s[u][n][k], mult[n][k & 1], -ref[n][k & 1]));
           sum[n][0] += e[0] + e[2], sum[n][1] += e[1] + e[3];
           pf[n][0] = trans8x8(pack2<true>(e[0], e[1]));
           pf[n][1] = trans8x8(pack2<true>(e[2], e[3]));
@@ -407,7 +406,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const uint32_t y = k < 2 ? x[j >> 1][j & 1] << 1 : x[j >> 1][j & 1] >> 7;
-              f[j] = as_u32(__hfma2(k & 1 ? high_code(y) : low_code(y), sc[j >> 1], off[j >> 1]));
+              f[j] = as_u32(__hfma2(k & 1 ? high_code(y, magic) : low_code(y, magic), sc[j >> 1], off[j >> 1]));
             }
 #pragma unroll
             for (int n = 0; n < kN; ++n) mma_16816<true>(o[n][4 * i + k], f, pf[n][0], pf[n][1]);
