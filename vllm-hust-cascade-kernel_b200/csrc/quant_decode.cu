@@ -36,6 +36,7 @@ namespace {
 constexpr int kTok = 32;     // tokens per tile
 constexpr int kSetup = 2;    // what a new unit costs, in tiles
 constexpr int kTileBytes = kTok * kQuantRow;  // of keys or of values
+constexpr int32_t kNoPage = INT32_MIN;
 constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
 
 template <int kN>  // query rows / 8
@@ -117,19 +118,21 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem_raw + ((0u - smem_u32(smem_raw)) & 127u);
   pdl_launch_dependents();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < kWarps * kStages) {
+    mbar_init(&full[0][0] + threadIdx.x, 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 32 * (kWarps - 1)) {
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
-    for (int w = 0; w < kWarps; ++w)
-      for (int i = 0; i < kStages; ++i) mbar_init(&full[w][i], 1);
     mbar_init(&stall, 1);
     fence_mbar_init();
+    tma_prefetch_desc(&P.key);
+    tma_prefetch_desc(&P.value);
   }
   __syncthreads();
   const int id = blockIdx.x * kWarps + warp, h = id % p.kv_heads, c = id / p.kv_heads;
   const QuantUnit<kRows, kTok> unit(p);
-  int runs = P.parts.runs;
-  int64_t total;
-  const QuantRun run = find_run<kRows, kTok, kSetup>(unit, c, runs, total);
+  const QuantRun run = find_run<kRows, kTok, kSetup>(unit, c, P.parts.runs);
   if (p.q_len == 0) {  // rows of tokens that are no request's: nothing to merge
     int64_t own = 0;
     for (int b = lane; b < p.batch; b += 32) own += min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens);
@@ -139,7 +142,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
          i < p.num_tokens * p.num_heads; i += static_cast<int64_t>(gridDim.x) * blockDim.x)
       P.parts.row_info[i] = 0;
   }
-  if (c >= runs) return;
+  if (c >= run.runs) return;
 
   uint8_t* mine = ring + warp * kStages * 2 * kTileBytes;
   const uint32_t base = smem_u32(mine);
@@ -159,28 +162,35 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
   const int shift = __ffs(p.block_size) - 1, oob = p.num_blocks ? p.num_blocks * p.block_size : 1;
   while (live && walk.next()) {
     // ---------------------------------------------------------------- loads
-    // cache rows of the boxes (one or two per tile) of this lane's of 32 tiles, and of the 32 after them
+    // page ids of the boxes (one or two per tile) of this lane's of 32 tiles, as cache rows, and of the 32 after them
     const bool two = P.box_rows < kTok;
-    int rows_now[2], rows_next[2];
-    int next_tile = walk.t0, rows_at = walk.t0;
-    auto tile_rows = [&](int tile, int (&row)[2]) {
+    int rows_now[2], next_tile = walk.t0, rows_at = walk.t0;
+    int32_t ids[2];
+    auto load_ids = [&](int tile) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int at = tile * kTok + i * 16;
-        row[i] = oob;  // (a unit without tokens has a tile all the same: nothing of it is used)
-        if (at < walk.kv && tile < walk.t0 + walk.n && (i == 0 || two)) {
-          const int32_t page = p.block_table[static_cast<int64_t>(walk.b) * p.block_cols + (at >> shift)];
-          if (static_cast<uint32_t>(page) < static_cast<uint32_t>(p.num_blocks))
-            row[i] = page * p.block_size + (at & (p.block_size - 1));
-          else
-            atomicOr(&g_cascade_device_error, kErrBadBlockId);
-        }
+        // (a unit without tokens has a tile all the same: nothing of it is used)
+        ids[i] = at < walk.kv && tile < walk.t0 + walk.n && (i == 0 || two)
+                     ? p.block_table[static_cast<int64_t>(walk.b) * p.block_cols + (at >> shift)]
+                     : kNoPage;
       }
     };
-    tile_rows(walk.t0 + lane, rows_now);
+    auto to_rows = [&](int tile) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int at = tile * kTok + i * 16;
+        const bool good = static_cast<uint32_t>(ids[i]) < static_cast<uint32_t>(p.num_blocks);
+        rows_now[i] = good ? ids[i] * p.block_size + (at & (p.block_size - 1)) : oob;
+        if (!good && ids[i] != kNoPage) atomicOr(&g_cascade_device_error, kErrBadBlockId);
+      }
+    };
     auto issue = [&] {
-      if (next_tile - rows_at == 32) rows_at = next_tile, rows_now[0] = rows_next[0], rows_now[1] = rows_next[1];
-      if (next_tile == rows_at) tile_rows(next_tile + 32 + lane, rows_next);
+      if (next_tile - rows_at == 32) {
+        rows_at = next_tile;
+        to_rows(next_tile + lane);
+        load_ids(next_tile + 32 + lane);
+      }
       const int row0 = __shfl_sync(0xffffffffu, rows_now[0], next_tile - rows_at);
       const int row1 = two ? __shfl_sync(0xffffffffu, rows_now[1], next_tile - rows_at) : 0;
       if (elect_one()) {
@@ -198,55 +208,61 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
       __syncwarp();
       ++issued, ++next_tile;
     };
-    for (int i = 0; i < min(kStages, walk.n); ++i) issue();
+    load_ids(walk.t0 + lane);
 
     // ---------------------------------------------------------------- query
     // row n of this block as the products' columns: lane (g, t) has d = 32 i + 8 t + 0..7 of row 8 n + g
     const int rows = min(kRows, walk.q * p.group - walk.block * kRows);  // of this unit
-    uint32_t qf[kN][16], zf[kN][2];
-    float mult[kN][2];   // of columns 2 t, 2 t + 1: score * scale * log2(e) per unit of the products
-    int lim[kN][2];
     auto row_of = [&](int r, int& i) {  // output row of row r of the unit, and its query token
       const int at = walk.block * kRows + r;
-      i = at / p.group;
+      i = at < p.group ? 0 : at / p.group;
       return (walk.tok + i) * p.num_heads + h * p.group + (at - i * p.group);
     };
+    uint4 raw[kN][4];
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
       int i;
       const bool real = n * 8 + g < rows;
       const uint16_t* src = static_cast<const uint16_t*>(p.query) + row_of(real ? n * 8 + g : 0, i) * kHeadDim + 8 * t;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        raw[n][k] = real ? __ldg(reinterpret_cast<const uint4*>(src + 32 * k)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    to_rows(walk.t0 + lane);
+    load_ids(walk.t0 + 32 + lane);
+    for (int i = 0; i < min(kStages, walk.n); ++i) issue();
+
+    uint32_t qf[kN][16], zf[kN][2];
+    float mult[kN][2];   // of columns 2 t, 2 t + 1: score * scale * log2(e) per unit of the products
+    int lim[kN][2];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
       float x[32], top = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint4 v = real ? *reinterpret_cast<const uint4*>(src + 32 * k) : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t w[4] = {raw[n][k].x, raw[n][k].y, raw[n][k].z, raw[n][k].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = kFp16 ? __half22float2(as_half2(w[e]))
                                  : make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u));
           x[8 * k + 2 * e] = f.x, x[8 * k + 2 * e + 1] = f.y;
+          top = fmax3f_nan(top, fabsf(f.x), fabsf(f.y));
         }
       }
 #pragma unroll
-      for (int e = 0; e < 32; ++e) top = fmax3f_nan(top, fabsf(x[e]), top);
-#pragma unroll
       for (int d = 1; d < 4; d <<= 1) top = fmax3f_nan(top, __shfl_xor_sync(0xffffffffu, top, d), top);
-      // times 2^(13 - exponent): [2^13, 2^14). A row with a NaN or an infinity is NaN.
-      const int ex = max((__float_as_int(top) >> 23) & 255, 1);
-      const bool nan = ex == 255;
-      // (in two factors: each of them, and its inverse, is a normal number)
-      const int up = 140 - ex, up0 = up / 2;
-      const float f0 = __int_as_float((127 + up0) << 23), f1 = nan ? __int_as_float(0x7fffffff) : __int_as_float((127 + up - up0) << 23);
+      // times 2^up: [2^13, 2^14), or less for rows below 2^-114. A row with a NaN or an infinity is NaN.
+      const int ex = max((__float_as_int(top) >> 23) & 255, 13), up = 140 - ex;
+      const float f = ex == 255 ? __int_as_float(0x7fffffff) : __int_as_float((127 + up) << 23);
       float sums[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float s = 0.f;
+        float* y = x + 8 * k;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[8 * k + e] = x[8 * k + e] * f0 * f1, s += x[8 * k + e];
+        for (int e = 0; e < 8; ++e) y[e] *= f;
+        float s = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         sums[k] = s + __shfl_xor_sync(0xffffffffu, s, 2);
-        const float* y = x + 8 * k;
         qf[n][4 * k] = pack2<true>(y[0], y[4]);
         qf[n][4 * k + 1] = pack2<true>(y[1] * 0.0625f, y[5] * 0.0625f);
         qf[n][4 * k + 2] = pack2<true>(y[2], y[6]);
@@ -257,19 +273,20 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
       const float2 hi = __half22float2(as_half2(zf[n][0]));
       zf[n][1] = pack2<true>(z - hi.x, y - hi.y);
       // (not 0, nor NaN: a masked score, -inf, stays -inf)
-      const float m = fmaxf((0x1p24f / f0 / f1) * (p.scale * 1.4426950408889634f), 1e-37f);
+      const float m = fmaxf(__int_as_float((127 - up) << 23) * 0x1p24f * (p.scale * 1.4426950408889634f), 1e-37f);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
+        int i;
         mult[n][k] = __shfl_sync(0xffffffffu, m, (2 * t + k) * 4);
         row_of(min(n * 8 + 2 * t + k, rows - 1), i);
         lim[n][k] = unit.limit(walk.q, walk.kv, i);
       }
     }
-    int first_token;
-    row_of(0, first_token);
-    const int clean = min(walk.kv, unit.limit(walk.q, walk.kv, first_token));  // tokens below are seen by every row
-    row_of(rows - 1, first_token);
-    const int most = unit.limit(walk.q, walk.kv, first_token);  // tokens from here on by none
+    int token;
+    row_of(0, token);
+    const int clean = min(walk.kv, unit.limit(walk.q, walk.kv, token));  // tokens below are seen by every row
+    row_of(rows - 1, token);
+    const int most = unit.limit(walk.q, walk.kv, token);  // tokens from here on by none
 
     float o[kN][8][4], sum[kN][2], ref[kN][2], bar_at[kN][2];
 #pragma unroll
@@ -434,7 +451,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
     // --------------------------------------------------------------- output
     const bool whole = walk.starts && walk.ends;
     const int32_t info =
-        walk.starts && !walk.ends ? cut_info(c, walk.base + unit.tiles(walk.q, walk.kv, walk.block) - 1, total, runs) : 0;
+        walk.starts && !walk.ends ? cut_info(run, c, walk.base + unit.tiles(walk.q, walk.kv, walk.block) - 1) : 0;
     const int64_t slot = (static_cast<int64_t>(walk.starts ? 2 * c + 1 : 2 * c) * p.kv_heads + h) * kRows;
 #pragma unroll
     for (int n = 0; n < kN; ++n) {

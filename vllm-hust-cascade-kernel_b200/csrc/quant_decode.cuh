@@ -57,17 +57,19 @@ struct QuantRun {
   int64_t begin, end;  // on the axis; no run: end = begin
   int64_t base;        // where the tiles of the first unit begin
   int64_t tok;         // first query token of request b
+  int64_t each;        // length of a run; `rest` of the `runs` runs have one more
   int b, block, t0, q, kv;
+  int rest, runs;
 };
 
-__device__ __forceinline__ int64_t run_begin(int c, int64_t total, int runs) {
-  const int64_t each = total / runs;
-  return c * each + (c * (total - each * runs)) / runs;
+// Start of run c: floor(c total / runs), without a wide division.
+__device__ __forceinline__ int64_t run_begin(int c, int64_t each, int rest, int runs) {
+  return c * each + static_cast<uint32_t>(c * rest) / static_cast<uint32_t>(runs);
 }
 
 // Finds run c of one kv head's axis (the same for every head); one warp.
 template <int kRows, int kTok, int kSetup>
-__device__ __forceinline__ QuantRun find_run(const QuantUnit<kRows, kTok>& u, int c, int& runs, int64_t& total) {
+__device__ __forceinline__ QuantRun find_run(const QuantUnit<kRows, kTok>& u, int c, int runs) {
   const int lane = threadIdx.x & 31;
   const QuantDecodeLaunch& p = u.p;
   const int per = (p.batch + 31) / 32;
@@ -88,8 +90,9 @@ __device__ __forceinline__ QuantRun find_run(const QuantUnit<kRows, kTok>& u, in
     tok0 = min(before(n), p.num_tokens);
   }
   int64_t mine = 0, tok = tok0;
+  int last_kv = 0;
   for (int b = b0; b < b1; ++b) {
-    const int q = u.q_len(b, tok), kv = u.kv_len(b), m = u.blocks(q);
+    const int q = u.q_len(b, tok), kv = last_kv = u.kv_len(b), m = u.blocks(q);
     if (!p.causal)
       mine += static_cast<int64_t>(m) * (kSetup + u.tiles(q, kv, 0));
     else
@@ -97,18 +100,20 @@ __device__ __forceinline__ QuantRun find_run(const QuantUnit<kRows, kTok>& u, in
     tok += q;
   }
   int64_t at = before(mine);
-  total = __shfl_sync(0xffffffffu, at + mine, 31);
-  runs = static_cast<int>(min(static_cast<int64_t>(runs), total));
+  const int64_t total = __shfl_sync(0xffffffffu, at + mine, 31);
   QuantRun r = {};
+  r.runs = runs = static_cast<int>(min(static_cast<int64_t>(runs), total));
   if (c >= runs) return r;
-  r.begin = run_begin(c, total, runs), r.end = run_begin(c + 1, total, runs);
+  r.each = total >> 31 ? total / runs : static_cast<uint32_t>(total) / static_cast<uint32_t>(runs);
+  r.rest = static_cast<int>(total - r.each * runs);
+  r.begin = run_begin(c, r.each, r.rest, runs), r.end = run_begin(c + 1, r.each, r.rest, runs);
   const uint32_t who = __ballot_sync(0xffffffffu, r.begin >= at && r.begin < at + mine);
   const int owner = __ffs(who) - 1;
   if (lane == owner) {
     tok = tok0;
     bool found = false;
     for (int b = b0; b < b1 && !found; ++b) {
-      const int q = u.q_len(b, tok), kv = u.kv_len(b), m = u.blocks(q);
+      const int q = u.q_len(b, tok), kv = per == 1 ? last_kv : u.kv_len(b), m = u.blocks(q);
       for (int i = 0; i < m; ++i) {
         const int t = kSetup + u.tiles(q, kv, i);
         if (r.begin < at + t) {
@@ -132,7 +137,7 @@ __device__ __forceinline__ QuantRun find_run(const QuantUnit<kRows, kTok>& u, in
   return r;
 }
 
-// The walk over a run, piece by piece (a piece: the run's part of a unit).
+// The walk over a run, piece by piece (a piece: the run's part of a unit). The next request's lengths are loaded a piece ahead.
 template <int kRows, int kTok, int kSetup>
 struct QuantWalk {
   QuantUnit<kRows, kTok> u;
@@ -140,28 +145,20 @@ struct QuantWalk {
   int64_t tok, base;
   bool starts, ends;
   int64_t next_base, end;
-  int next_t0;
-  bool first;
+  int next_t0, next_b, next_q;
+  int64_t next_kv;  // as loaded: not used, and so not waited for, until the next piece
+  bool fresh;       // the next piece is the first block of request next_b
   __device__ QuantWalk(const QuantDecodeLaunch& l, const QuantRun& r)
-      : u(l), b(r.b), block(r.block), t0(0), n(0), q(r.q), kv(r.kv), tok(r.tok), base(0), starts(false), ends(false),
-        next_base(r.base), end(r.end), next_t0(r.t0), first(true) {}
+      : u(l), b(r.b), block(r.block - 1), t0(0), n(0), q(r.q), kv(r.kv), tok(r.tok), base(0), starts(false), ends(false),
+        next_base(r.base), end(r.end), next_t0(r.t0), next_b(0), next_q(0), next_kv(0), fresh(false) {}
   __device__ __forceinline__ bool next() {
     if (next_base + next_t0 >= end) return false;
-    if (!first) {
-      if (++block >= u.blocks(q)) {
-        block = 0;
-        do {
-          tok += q;
-          if (++b >= u.p.batch) {
-            next_base = end;
-            return false;
-          }
-          q = u.q_len(b, tok);
-        } while (q == 0);
-        kv = u.kv_len(b);
-      }
+    if (fresh) {
+      block = 0, tok += q, b = next_b, q = next_q;
+      kv = static_cast<int>(min(max(next_kv, static_cast<int64_t>(0)), static_cast<int64_t>(u.cap)));
+    } else {
+      ++block;
     }
-    first = false;
     base = next_base;
     const int all = u.tiles(q, kv, block);
     t0 = next_t0;
@@ -170,15 +167,29 @@ struct QuantWalk {
     ends = t0 + n == all;
     next_base = base + all + kSetup;
     next_t0 = 0;
+    fresh = false;
+    if (next_base < end && block + 1 >= u.blocks(q)) {
+      fresh = true;
+      for (next_b = b + 1;; ++next_b) {  // requests without query tokens have no units
+        if (next_b >= u.p.batch) {
+          next_base = end;
+          break;
+        }
+        next_q = u.q_len(next_b, tok + q);
+        if (next_q > 0) break;
+      }
+      if (next_base < end) next_kv = u.p.kv_lens[next_b];
+    }
     return true;
   }
 };
 
 // row_info of a unit whose first piece is run c's and whose last tile is at `last` of the axis, without its row
-__device__ __forceinline__ int32_t cut_info(int c, int64_t last, int64_t total, int runs) {
-  int hi = static_cast<int>(min(static_cast<int64_t>(runs - 1), last / (total / runs)));
-  while (hi > c && run_begin(hi, total, runs) > last) --hi;
-  while (hi + 1 < runs && run_begin(hi + 1, total, runs) <= last) ++hi;
+__device__ __forceinline__ int32_t cut_info(const QuantRun& run, int c, int64_t last) {
+  const float total = static_cast<float>(run.each * run.runs + run.rest);
+  int hi = max(c, min(run.runs - 1, static_cast<int>(static_cast<float>(last) / total * static_cast<float>(run.runs))));
+  while (hi + 1 < run.runs && run_begin(hi + 1, run.each, run.rest, run.runs) <= last) ++hi;
+  while (hi > c && run_begin(hi, run.each, run.rest, run.runs) > last) --hi;
   return pack_info(c, hi - c + 1, 0);
 }
 
