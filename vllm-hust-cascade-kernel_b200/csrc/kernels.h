@@ -352,10 +352,11 @@ int set_error(int code, const char* msg);
 bool encode_tmap_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t row_stride_bytes,
                     uint32_t box_inner, uint32_t box_rows, bool swizzle128, CUtensorMapL2promotion promo);
 
-// Host: encode a 2-D tiled tensor map of bytes, no swizzle; inner box, row stride
-// and base address multiples of 16.
-bool encode_tmap_bytes(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t row_stride_bytes,
-                       uint32_t box_inner, uint32_t box_rows);
+// Host: encode a 3-D tiled tensor map of bytes, no swizzle, innermost extent first;
+// the inner extent of tensor and box (up to 1,024), strides and base address are
+// multiples of 16.
+bool encode_tmap_bytes(CUtensorMap* map, const void* base, const uint64_t (&extent)[3], const uint64_t (&stride_bytes)[2],
+                       const uint32_t (&box)[3]);
 
 // Host: encode a tiled tensor map of 16-bit elements, 128-byte swizzle (box[0]
 // = 64 elements), rank 2 to 5, innermost extent first; strides of the outer
