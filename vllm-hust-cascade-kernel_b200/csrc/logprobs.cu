@@ -1,85 +1,365 @@
-// Log probabilities of tokens (cascade_token_logprobs): one CTA per row, a pass
-// for the maximum, the sums and the rank, and one per alternative.
+// Log probabilities of tokens (cascade_token_logprobs).
+//
+// One pass over a row's logits keeps, per thread, the running maximum m, the sum of
+// e = exp(x - m) and of e (x - m): ln p(x) = x - m - ln sum, and the entropy is
+// ln sum - (sum of e (x - m)) / sum, differences of small numbers whatever the
+// logits' size. A batch of 16 (8 in fp32) logits per thread is looked at by its
+// maximum alone: it moves m, it says whether the batch holds logits that come
+// before the given token (few do for a likely one), and it is kept in shared
+// memory for the alternatives.
+//
+// The `top` first entries: with w full warps, the lowest of the warps'
+// ceil(top / w)-th largest thread maxima is a bound that at least `top` entries
+// reach. The batches whose maximum reaches it are read again (from L2, about `top`
+// of them), their entries that reach it, some 30 for top = 20, are ordered by
+// counting. A bound is a (logit, index) pair, so equal logits need no care but
+// where a thread hides very many entries: then the CTA takes one maximum after the
+// other.
+//
+// Bound by HBM for large batches, with the instructions per logit (5.5 and a
+// special function) close behind in 16 bits; few rows are shared by a cluster of
+// CTAs, which meet in the first one's shared memory.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "kernels.h"
 #include "ptx.cuh"
 
 namespace cascade {
 namespace {
 
-constexpr int kThreads = 512;
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kPerSm = 4;      // CTAs
+constexpr int kMaxCtas = 8;    // per row
+constexpr int kSlots = 32;     // of batches per thread whose maxima are kept
+constexpr int kList = 1024;    // entries that may reach the bound
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int kType>
-__device__ __forceinline__ float load(const void* base, int64_t i) {
-  if constexpr (kType == 2) return __ldg(static_cast<const float*>(base) + i);
-  const uint16_t b = __ldg(static_cast<const uint16_t*>(base) + i);
+struct Vec {  // 16 bytes of logits
+  static constexpr int kW = kType == 2 ? 4 : 8;
+};
+
+template <int kType>
+__device__ __forceinline__ float load_one(const void* row, int i) {
+  if constexpr (kType == 2) return __ldg(static_cast<const float*>(row) + i);
+  const uint16_t b = __ldg(static_cast<const uint16_t*>(row) + i);
   if constexpr (kType == 1) return __half2float(__ushort_as_half(b));
   return __uint_as_float(static_cast<uint32_t>(b) << 16);
 }
 
-// a logit's place in the order: larger first, lower index first among equals, a NaN as -inf; never 0
-__device__ __forceinline__ uint64_t make_key(float x, uint32_t v) {
-  const uint32_t b = __float_as_uint(x != x ? -INFINITY : x + 0.f);
-  const uint32_t up = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (static_cast<uint64_t>(up) << 32) | (0xffffffffu - v);
+template <int kType>
+__device__ __forceinline__ void unpack(const uint4& v, float* x) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (kType == 2) {
+      x[i] = __uint_as_float(w[i]);
+    } else if constexpr (kType == 1) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
 }
 
-template <class T, class Op>
-__device__ __forceinline__ T block_reduce(T v, T* slot, Op op) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, d));
-  if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = slot[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = op(v, slot[w]);
-  __syncthreads();
-  return v;
+// A logit's place in the order: larger first, lower index first among equals, a NaN as -inf; never 0, nor all ones.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t b = __float_as_uint(x != x ? -INFINITY : x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ uint64_t make_key(float x, uint32_t v) {
+  return (static_cast<uint64_t>(order_bits(x)) << 32) | (0xffffffffu - v);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xffffffffu - static_cast<uint32_t>(k); }
+
+struct Stats {  // of a thread, a CTA, a row
+  float m, sum, dot;  // dot: of e log2(e); sums relative to m
+  int ahead;
+  int nan;
+};
+
+// sums relative to the larger maximum
+__device__ __forceinline__ void rebase(Stats& s, float m) {
+  if (s.m == m) return;
+  if (s.m == -INFINITY) {
+    s.m = m;  // (nothing but zeros so far)
+    return;
+  }
+  const float d = (s.m - m) * kLog2e, f = ex2(d);  // d <= 0; -inf only if m is +inf: the row is NaN
+  s.dot = f == 0.f ? 0.f : f * fmaf(s.sum, d, s.dot);
+  s.sum *= f;
+  s.m = m;
+}
+__device__ __forceinline__ void add(Stats& s, Stats o) {
+  const float m = fmaxf(s.m, o.m);
+  rebase(s, m);
+  rebase(o, m);
+  s.sum += o.sum, s.dot += o.dot, s.ahead += o.ahead, s.nan |= o.nan;
+}
+
+__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(k >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
+struct Shared {
+  float batch_max[kSlots][kThreads];
+  uint64_t list[kList];
+  uint64_t sorted[kMaxTop];
+  uint64_t gather[kMaxCtas * kMaxTop];  // the first CTA's: every CTA's `sorted`
+  Stats cta[kMaxCtas];                  // the first CTA's: every CTA's sums
+  Stats warp[kWarps];
+  uint64_t bound[kWarps];
+  int count;
+};
 
 template <int kType>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsLaunch p) {
-  __shared__ float slots[kThreads / 32];
-  __shared__ uint64_t keys[kThreads / 32];
-  const int64_t n = blockIdx.x;
-  const void* row = static_cast<const char*>(p.logits) + n * p.row_stride * (kType == 2 ? 4 : 2);
-  const int64_t V = p.vocab, token = p.tokens[n];
+__global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const LogprobsLaunch p) {
+  constexpr int kW = Vec<kType>::kW;
+  constexpr int kBatch = 2 * kW;  // a thread's logits per batch: two loads, 32 vectors apart
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  cluster.barrier_arrive();  // waited for before the first write to another CTA: all have started by then
+  const int64_t n = blockIdx.x / ctas;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, V = static_cast<int>(p.vocab), top = p.top;
+  const char* row = static_cast<const char*>(p.logits) + n * p.row_stride * (kType == 2 ? 4 : 2);
+  const int64_t token = p.tokens[n];
   const bool given = token >= 0 && token < V;
-  const float mine = given ? load<kType>(row, token) : 0.f;
-  const uint64_t key = given ? make_key(mine, static_cast<uint32_t>(token)) : 0;
-  float top = -INFINITY;
-  uint64_t ahead = 0;
-  for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-    const float x = load<kType>(row, v);
-    top = fmaxf(top, x);
-    ahead += make_key(x, static_cast<uint32_t>(v)) > key;
-  }
-  top = block_reduce(top, slots, [](float a, float b) { return fmaxf(a, b); });
-  ahead = block_reduce(ahead, keys, [](uint64_t a, uint64_t b) { return a + b; });
-  float sum = 0.f, dot = 0.f;
-  for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-    const float d = load<kType>(row, v) - top, e = expf(d);
-    sum += e;
-    dot += e > 0.f ? e * d : e != e ? e : 0.f;
-  }
-  sum = block_reduce(sum, slots, [](float a, float b) { return a + b; });
-  dot = block_reduce(dot, slots, [](float a, float b) { return a + b; });
-  const float norm = logf(sum);
-  if (threadIdx.x == 0) {
-    p.logprob[n] = given ? (mine - top) - norm : -INFINITY;
-    p.entropy[n] = norm - dot / sum;
-    p.rank[n] = given ? static_cast<int64_t>(ahead) : -1;
-  }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < p.top; ++k) {
-    uint64_t best = 0;
-    for (int64_t v = threadIdx.x; v < V; v += kThreads) {
-      const uint64_t a = make_key(load<kType>(row, v), static_cast<uint32_t>(v));
-      if (a < last && a > best) best = a;
+  // vectors at 16-byte boundaries: vector v holds the entries v kW - shift .. + kW; those at the ends may be cut
+  const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16) / (kType == 2 ? 4 : 2);
+  const int vectors = (V + shift + kW - 1) / kW;
+  const int batches = (vectors + 63) / 64;
+  const int first = static_cast<int>(static_cast<int64_t>(batches) * rank / ctas);        // this CTA's batches
+  const int last = static_cast<int>(static_cast<int64_t>(batches) * (rank + 1) / ctas);
+  const int per_slot = ((last - first + kWarps - 1) / kWarps + kSlots - 1) / kSlots;
+  const float mine = given ? load_one<kType>(row, static_cast<int>(token)) : INFINITY;
+  const float bar = given ? (mine == mine ? mine : -INFINITY) : INFINITY;  // batches below it hold nothing ahead of the token
+  const uint64_t key = given ? make_key(mine, static_cast<uint32_t>(token)) : ~0ull;
+
+  auto whole = [&](int v) { return v * kW >= shift && (v + 1) * kW - shift <= V; };
+  auto fetch = [&](int v) {
+    return whole(v) ? __ldg(reinterpret_cast<const uint4*>(row - shift * (16 / kW)) + v) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  auto expand = [&](const uint4& raw, int v, float* x) {
+    if (whole(v)) {
+      unpack<kType>(raw, x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        const int i = v * kW - shift + j;
+        x[j] = i >= 0 && i < V ? load_one<kType>(row, i) : -INFINITY;
+      }
     }
-    last = block_reduce(best, keys, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-    if (threadIdx.x == 0) {
-      const int64_t v = 0xffffffffu - static_cast<uint32_t>(last);
-      p.top_tokens[n * p.top + k] = v;
-      p.top_logprobs[n * p.top + k] = (load<kType>(row, v) - top) - norm;
+  };
+
+  // ------------------------------------------------------------- the pass
+  Stats s = {-INFINITY, 0.f, 0.f, 0, 0};
+  uint64_t best = 0;  // (the maximum, an index that it is not behind)
+  float slot_max = -INFINITY;
+  int slot = 0, in_slot = 0;
+  uint4 raw[2];
+  int b = first + warp;
+  if (b < last) raw[0] = fetch(b * 64 + lane), raw[1] = fetch(b * 64 + 32 + lane);
+  for (; b < last; b += kWarps) {
+    const int v0 = b * 64 + lane;
+    float x[kBatch];
+    expand(raw[0], v0, x);
+    expand(raw[1], v0 + 32, x + kW);
+    if (b + kWarps < last) raw[0] = fetch(v0 + 64 * kWarps), raw[1] = fetch(v0 + 64 * kWarps + 32);
+    float most = x[0];
+#pragma unroll
+    for (int j = 1; j + 1 < kBatch; j += 2) most = fmax3f_nan(most, x[j], x[j + 1]);
+    most = fmax3f_nan(most, x[kBatch - 1], x[kBatch - 1]);
+    if (most != most) {  // for the order a NaN is -inf
+      s.nan = 1;
+      most = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) most = fmaxf(most, x[j]);
+    }
+    if (most > s.m || best == 0) {
+      rebase(s, most);
+      best = make_key(most, static_cast<uint32_t>(min(V - 1, (v0 + 32) * kW - shift + kW - 1)));
+    }
+    slot_max = fmaxf(slot_max, most);
+    if (++in_slot == per_slot) {
+      sh.batch_max[slot++][threadIdx.x] = slot_max;
+      slot_max = -INFINITY, in_slot = 0;
+    }
+    if (most >= bar) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = (v0 + (j >= kW ? 32 : 0)) * kW - shift + j % kW;
+        s.ahead += i >= 0 && i < V && make_key(x[j], static_cast<uint32_t>(i)) > key;
+      }
+    }
+    // (nothing but -inf so far: any finite number stands in for the maximum)
+    const float neg = s.m == -INFINITY ? 0.f : -s.m;
+    float sum0 = 0.f, sum1 = 0.f, dot0 = 0.f, dot1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < kBatch; j += 2) {
+      float y0 = x[j], y1 = x[j + 1];
+      fadd2(y0, y1, neg, neg);
+      // 2^-200 is 0 next to the sum's 1, and 0 times -inf would be NaN
+      y0 = fmaxf(y0 * kLog2e, -200.f), y1 = fmaxf(y1 * kLog2e, -200.f);
+      const float e0 = ex2(y0), e1 = ex2(y1);
+      fadd2(sum0, sum1, e0, e1);
+      dot0 = fmaf(e0, y0, dot0), dot1 = fmaf(e1, y1, dot1);
+    }
+    s.sum += sum0 + sum1, s.dot += dot0 + dot1;
+  }
+  if (in_slot > 0) sh.batch_max[slot++][threadIdx.x] = slot_max;
+
+  // ------------------------------------------------------------- the sums
+  const float thread_max = s.m;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    Stats o;
+    o.m = __shfl_xor_sync(0xffffffffu, s.m, d);
+    o.sum = __shfl_xor_sync(0xffffffffu, s.sum, d);
+    o.dot = __shfl_xor_sync(0xffffffffu, s.dot, d);
+    o.ahead = __shfl_xor_sync(0xffffffffu, s.ahead, d);
+    o.nan = __shfl_xor_sync(0xffffffffu, s.nan, d);
+    add(s, o);
+  }
+  if (lane == 0) sh.warp[warp] = s;
+  __syncthreads();
+
+  // ------------------------------------------------------------- the alternatives
+  if (top > 0) {
+    // warps whose first batch is whole: all lanes have entries (a cut vector has one at least)
+    const int full = min(kWarps, max(0, min(last, vectors / 64) - first));
+    // the lowest of the warps' nth largest, nth = top / warps, or (where that leaves too many: equal logits) the highest of
+    // their `top`-th
+    auto find_bound = [&](bool one) {
+      const int nth = one ? top : full > 0 ? (top + full - 1) / full : 0;
+      uint64_t k = best, at = 0;
+      for (int i = 0; i < nth; ++i) {
+        at = warp_max(k);
+        if (k == at) k = 0;
+      }
+      if (lane == 0) sh.bound[warp] = warp < full ? at : one ? 0 : ~0ull;
+      if (threadIdx.x == 0) sh.count = 0;
+      __syncthreads();
+      uint64_t bound = sh.bound[0];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) bound = one ? max(bound, sh.bound[w]) : min(bound, sh.bound[w]);
+      return full > 0 ? bound : 0;
+    };
+    int count = 0;
+    for (int round = 0; round < 2; ++round) {
+      const uint64_t bound = find_bound(round > 0);
+      const uint32_t bound_hi = static_cast<uint32_t>(bound >> 32);
+      if (order_bits(thread_max) >= bound_hi) {
+        for (int i = 0; i < slot; ++i) {
+          if (order_bits(sh.batch_max[i][threadIdx.x]) < bound_hi) continue;
+          for (int j = 0; j < per_slot; ++j) {
+            const int bb = first + warp + (i * per_slot + j) * kWarps;
+            if (bb >= last) break;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int v = bb * 64 + q * 32 + lane;
+              float x[kW];
+              expand(fetch(v), v, x);
+#pragma unroll
+              for (int e = 0; e < kW; ++e) {
+                const int idx = v * kW - shift + e;
+                if (idx < 0 || idx >= V) continue;
+                const uint64_t a = make_key(x[e], static_cast<uint32_t>(idx));
+                if (a >= bound) {
+                  const int to = atomicAdd(&sh.count, 1);
+                  if (to < kList) sh.list[to] = a;
+                }
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();
+      count = sh.count;
+      if (count <= kList) break;
+      __syncthreads();  // (all have read the count)
+    }
+    if (count <= kList) {
+      for (int i = threadIdx.x; i < max(count, top); i += kThreads) {
+        if (i >= count) {
+          sh.sorted[i] = 0;  // (fewer entries than `top` in this CTA's part)
+          continue;
+        }
+        const uint64_t a = sh.list[i];
+        int before = 0;
+        for (int j = 0; j < count; ++j) before += sh.list[j] > a;
+        if (before < top) sh.sorted[before] = a;
+      }
+    } else {
+      // a thread hides more than the list holds: one maximum after the other
+      uint64_t limit = ~0ull;
+      for (int k = 0; k < top; ++k) {
+        uint64_t most = 0;
+        for (int i = first * 64 * kW + static_cast<int>(threadIdx.x); i < last * 64 * kW; i += kThreads) {
+          const int idx = i - shift;
+          if (idx < 0 || idx >= V) continue;
+          const uint64_t a = make_key(load_one<kType>(row, idx), static_cast<uint32_t>(idx));
+          if (a < limit && a > most) most = a;
+        }
+        most = warp_max(most);
+        if (lane == 0) sh.bound[warp] = most;
+        __syncthreads();
+        limit = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) limit = max(limit, sh.bound[w]);
+        if (threadIdx.x == 0) sh.sorted[k] = limit;
+        __syncthreads();
+      }
+    }
+    __syncthreads();
+  }
+
+  // ------------------------------------------------------------- the row
+  if (warp == 0) {
+    s = sh.warp[0];
+    for (int w = 1; w < kWarps; ++w) add(s, sh.warp[w]);
+  }
+  cluster.barrier_wait();
+  if (ctas > 1) {
+    Shared& root = *cluster.map_shared_rank(&sh, 0);
+    if (threadIdx.x == 0) root.cta[rank] = s;
+    if (threadIdx.x < top) root.gather[rank * top + threadIdx.x] = sh.sorted[threadIdx.x];
+    cluster.sync();
+    if (rank > 0) return;
+    if (warp == 0) {
+      s = sh.cta[0];
+      for (int c = 1; c < ctas; ++c) add(s, sh.cta[c]);
+    }
+    const int all = ctas * top;
+    if (static_cast<int>(threadIdx.x) < all) {
+      const uint64_t a = sh.gather[threadIdx.x];
+      int before = 0;
+      for (int j = 0; j < all; ++j) before += sh.gather[j] > a;
+      if (a != 0 && before < top) sh.sorted[before] = a;
+    }
+    __syncthreads();
+  }
+  if (warp == 0) {
+    const bool nan = s.nan || !(s.m < INFINITY) || s.m == -INFINITY;
+    const float norm = nan ? __int_as_float(0x7fffffff) : __logf(s.sum);
+    if (lane == 0) {
+      p.logprob[n] = given ? (mine - s.m) - norm : -INFINITY;
+      p.entropy[n] = norm - s.dot / s.sum * kLn2;
+      p.rank[n] = given ? s.ahead : -1;
+    }
+    if (lane < top) {
+      const uint64_t a = sh.sorted[lane];
+      const uint32_t idx = key_index(a);
+      p.top_tokens[n * top + lane] = idx;
+      p.top_logprobs[n * top + lane] = (load_one<kType>(row, static_cast<int>(idx)) - s.m) - norm;
     }
   }
 }
@@ -89,9 +369,26 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsLaunch
 size_t token_logprobs_workspace(const LogprobsLaunch&) { return 0; }
 
 cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void*, cudaStream_t stream) {
-  (p.dtype == 2 ? logprobs_kernel<2> : p.dtype == 1 ? logprobs_kernel<1> : logprobs_kernel<0>)
-      <<<static_cast<unsigned>(p.rows), kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  // as many CTAs per row as run at once, with a batch for each of their warps
+  const int64_t batch = 64 * (p.dtype == 2 ? 4 : 8);
+  int ctas = 1;
+  while (ctas < kMaxCtas && p.rows * ctas * 2 <= kPerSm * kNumSMs && p.vocab >= 2 * ctas * kWarps * batch) ctas *= 2;
+  auto kern = p.dtype == 2 ? logprobs_kernel<2> : p.dtype == 1 ? logprobs_kernel<1> : logprobs_kernel<0>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), sizeof(Shared));
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.rows * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
 
 }  // namespace cascade
