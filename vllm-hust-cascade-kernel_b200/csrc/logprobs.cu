@@ -3,15 +3,13 @@
 // One pass over a row's logits keeps, per thread, the running maximum m, the sum of
 // e = exp(x - m) and of e (x - m): ln p(x) = x - m - ln sum, and the entropy is
 // ln sum - (sum of e (x - m)) / sum, differences of small numbers whatever the
-// logits' size. A batch of 16 (8 in fp32) logits per thread is looked at by its
-// maximum alone: it moves m, it says whether the batch holds logits that come
-// before the given token (few do for a likely one), and it is kept in shared
-// memory for the alternatives.
+// logits' size. The maximum of a thread's batch of 32 (16 in fp32) logits is kept
+// in shared memory for the alternatives.
 //
 // The `top` first entries: with w full warps, the lowest of the warps'
 // ceil(top / w)-th largest thread maxima is a bound that at least `top` entries
-// reach. The batches whose maximum reaches it are read again (from L2, about `top`
-// of them), their entries that reach it, some 30 for top = 20, are ordered by
+// reach. The batches whose maximum reaches it are read again (from L2, a few more
+// than `top` of them, a lane per entry), their entries that reach it are ordered by
 // counting. A bound is a (logit, index) pair, so equal logits need no care but
 // where a thread hides very many entries: then the CTA takes one maximum after the
 // other.
@@ -22,6 +20,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 #include "ptx.cuh"
@@ -31,11 +30,12 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+constexpr int kVecs = 4;       // vectors of a batch per thread, 32 apart
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPerSm = 4;      // CTAs
 constexpr int kMaxCtas = 8;    // per row
 constexpr int kSlots = 32;     // of batches per thread whose maxima are kept
-constexpr int kList = 1024;    // entries that may reach the bound
+constexpr int kList = 1024;    // entries, or batches, that may reach the bound
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 template <int kType>
@@ -65,6 +65,95 @@ __device__ __forceinline__ void unpack(const uint4& v, float* x) {
       x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
+}
+
+// maximum of a batch; NaN does not count
+template <int kType>
+__device__ __forceinline__ float batch_max(const uint4 (&v)[kVecs]) {
+  if constexpr (kType == 2) {
+    float m = __uint_as_float(v[0].x);
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      m = fmax3f(m, __uint_as_float(v[i].x), __uint_as_float(v[i].y));
+      m = fmax3f(m, __uint_as_float(v[i].z), __uint_as_float(v[i].w));
+    }
+    return m;
+  } else if constexpr (kType == 1) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    __half2 m[4] = {h[0], h[1], h[2], h[3]};
+#pragma unroll
+    for (int i = 4; i < 4 * kVecs; ++i) m[i & 3] = __hmax2(m[i & 3], h[i]);
+    m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    return __half2float(__hmax(__low2half(m[0]), __high2half(m[0])));
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    __nv_bfloat162 m[4] = {h[0], h[1], h[2], h[3]};
+#pragma unroll
+    for (int i = 4; i < 4 * kVecs; ++i) m[i & 3] = __hmax2(m[i & 3], h[i]);
+    m[0] = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    return __bfloat162float(__hmax(__low2bfloat16(m[0]), __high2bfloat16(m[0])));
+  }
+}
+
+// how many of a batch's logits are above `bar`, which the type holds
+template <int kType>
+__device__ __forceinline__ int count_above(const uint4 (&v)[kVecs], float bar) {
+  if constexpr (kType == 2) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      n += (__uint_as_float(v[i].x) > bar) + (__uint_as_float(v[i].y) > bar) + (__uint_as_float(v[i].z) > bar) +
+           (__uint_as_float(v[i].w) > bar);
+    return n;
+  } else if constexpr (kType == 1) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 b = __float2half2_rn(bar);
+    __half2 n[2] = {__hgt2(h[0], b), __hgt2(h[1], b)};
+#pragma unroll
+    for (int i = 2; i < 4 * kVecs; ++i) n[i & 1] = __hadd2(n[i & 1], __hgt2(h[i], b));
+    n[0] = __hadd2(n[0], n[1]);  // (whole numbers up to 32)
+    return static_cast<int>(__low2float(n[0]) + __high2float(n[0]));
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 b = __float2bfloat162_rn(bar);
+    __nv_bfloat162 n[2] = {__hgt2(h[0], b), __hgt2(h[1], b)};
+#pragma unroll
+    for (int i = 2; i < 4 * kVecs; ++i) n[i & 1] = __hadd2(n[i & 1], __hgt2(h[i], b));
+    n[0] = __hadd2(n[0], n[1]);
+    return static_cast<int>(__low2float(n[0]) + __high2float(n[0]));
+  }
+}
+
+// -inf (and what lies below -1e38) as a finite number; NaN stays
+template <int kType>
+__device__ __forceinline__ uint4 clamp_low(uint4 v) {
+  if constexpr (kType == 1) {
+    __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], __float2half2_rn(-65504.f));
+  } else if constexpr (kType == 0) {
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], __float2bfloat162_rn(-1e38f));
+  }
+  if constexpr (kType == 2) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(fmax3f_nan(__uint_as_float(w[i]), -1e38f, -1e38f));
+  }
+  return v;
+}
+
+// the largest number of the type below x (x finite or +infinity)
+template <int kType>
+__device__ __forceinline__ float next_below(float x) {
+  if (x == 0.f) return kType == 2 ? __int_as_float(0x80000001) : kType == 1 ? -0x1p-24f : __int_as_float(0x80010000);
+  if constexpr (kType == 1) {
+    const uint16_t b = __half_as_ushort(__float2half_rn(x));
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(x > 0.f ? b - 1 : b + 1)));
+  }
+  const int step = kType == 2 ? 1 : 0x10000;
+  return __int_as_float(x > 0.f ? __float_as_int(x) - step : __float_as_int(x) + step);
 }
 
 // A logit's place in the order: larger first, lower index first among equals, a NaN as -inf; never 0, nor all ones.
@@ -111,18 +200,20 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
 struct Shared {
   float batch_max[kSlots][kThreads];
   uint64_t list[kList];
+  uint32_t hits[kList];  // slot, thread
   uint64_t sorted[kMaxTop];
   uint64_t gather[kMaxCtas * kMaxTop];  // the first CTA's: every CTA's `sorted`
   Stats cta[kMaxCtas];                  // the first CTA's: every CTA's sums
   Stats warp[kWarps];
   uint64_t bound[kWarps];
-  int count;
+  int count, hit_count;
 };
 
 template <int kType>
 __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const LogprobsLaunch p) {
   constexpr int kW = Vec<kType>::kW;
-  constexpr int kBatch = 2 * kW;  // a thread's logits per batch: two loads, 32 vectors apart
+  constexpr int kBatch = kVecs * kW;         // a thread's logits per batch
+  constexpr int kSpan = 32 * kVecs;          // a warp's vectors per batch
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
@@ -136,86 +227,120 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   // vectors at 16-byte boundaries: vector v holds the entries v kW - shift .. + kW; those at the ends may be cut
   const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) % 16) / (kType == 2 ? 4 : 2);
   const int vectors = (V + shift + kW - 1) / kW;
-  const int batches = (vectors + 63) / 64;
+  const int batches = (vectors + kSpan - 1) / kSpan;
   const int first = static_cast<int>(static_cast<int64_t>(batches) * rank / ctas);        // this CTA's batches
   const int last = static_cast<int>(static_cast<int64_t>(batches) * (rank + 1) / ctas);
   const int per_slot = ((last - first + kWarps - 1) / kWarps + kSlots - 1) / kSlots;
   const float mine = given ? load_one<kType>(row, static_cast<int>(token)) : INFINITY;
-  const float bar = given ? (mine == mine ? mine : -INFINITY) : INFINITY;  // batches below it hold nothing ahead of the token
   const uint64_t key = given ? make_key(mine, static_cast<uint32_t>(token)) : ~0ull;
+  // The entries ahead of the token: those above its logit, and its equals before it. A batch before the token counts what is
+  // above the next lower number, one after it what is above its own. The batch that has it goes entry by entry; so do those
+  // that are cut by the row's ends, and all of them for a logit of -inf or NaN (equal here).
+  const float above = given ? mine : INFINITY, above_before = given ? next_below<kType>(mine) : INFINITY;
+  const int token_batch = given ? static_cast<int>((token + shift) / (kSpan * kW)) : -1;
+  const bool odd = given && !(mine > -INFINITY);
+  const int whole_from = shift > 0, whole_to = (V + shift) / (kSpan * kW);  // batches of whole vectors alone
 
-  auto whole = [&](int v) { return v * kW >= shift && (v + 1) * kW - shift <= V; };
-  auto fetch = [&](int v) {
-    return whole(v) ? __ldg(reinterpret_cast<const uint4*>(row - shift * (16 / kW)) + v) : make_uint4(0u, 0u, 0u, 0u);
-  };
-  auto expand = [&](const uint4& raw, int v, float* x) {
-    if (whole(v)) {
-      unpack<kType>(raw, x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kW; ++j) {
-        const int i = v * kW - shift + j;
-        x[j] = i >= 0 && i < V ? load_one<kType>(row, i) : -INFINITY;
-      }
-    }
-  };
+  const uint4* vecs = reinterpret_cast<const uint4*>(row - shift * (16 / kW));
+  auto index_of = [&](int v, int j) { return (v + j / kW * 32) * kW - shift + j % kW; };  // entry j of a thread's batch from v on
 
   // ------------------------------------------------------------- the pass
   Stats s = {-INFINITY, 0.f, 0.f, 0, 0};
-  uint64_t best = 0;  // (the maximum, an index that it is not behind)
+  int best_at = -1;  // batch of the maximum
   float slot_max = -INFINITY;
   int slot = 0, in_slot = 0;
-  uint4 raw[2];
-  int b = first + warp;
-  if (b < last) raw[0] = fetch(b * 64 + lane), raw[1] = fetch(b * 64 + 32 + lane);
-  for (; b < last; b += kWarps) {
-    const int v0 = b * 64 + lane;
-    float x[kBatch];
-    expand(raw[0], v0, x);
-    expand(raw[1], v0 + 32, x + kW);
-    if (b + kWarps < last) raw[0] = fetch(v0 + 64 * kWarps), raw[1] = fetch(v0 + 64 * kWarps + 32);
-    float most = x[0];
-#pragma unroll
-    for (int j = 1; j + 1 < kBatch; j += 2) most = fmax3f_nan(most, x[j], x[j + 1]);
-    most = fmax3f_nan(most, x[kBatch - 1], x[kBatch - 1]);
-    if (most != most) {  // for the order a NaN is -inf
-      s.nan = 1;
-      most = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) most = fmaxf(most, x[j]);
-    }
-    if (most > s.m || best == 0) {
-      rebase(s, most);
-      best = make_key(most, static_cast<uint32_t>(min(V - 1, (v0 + 32) * kW - shift + kW - 1)));
+  auto note = [&](float most, int b) {
+    if (most > s.m || best_at < 0) {
+      rebase(s, fmaxf(most, s.m));
+      best_at = b;
     }
     slot_max = fmaxf(slot_max, most);
     if (++in_slot == per_slot) {
       sh.batch_max[slot++][threadIdx.x] = slot_max;
       slot_max = -INFINITY, in_slot = 0;
     }
-    if (most >= bar) {
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int i = (v0 + (j >= kW ? 32 : 0)) * kW - shift + j % kW;
-        s.ahead += i >= 0 && i < V && make_key(x[j], static_cast<uint32_t>(i)) > key;
-      }
+  };
+  // Entry by entry, and with logits of any size: sums of e and e y, y = (x - m) log2(e).
+  auto careful = [&](int b) {
+    const int v = b * kSpan + lane;
+    float most = -INFINITY;
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = index_of(v, j);
+      if (i < 0 || i >= V) continue;
+      const float x = load_one<kType>(row, i);
+      most = fmaxf(most, x);
+      s.ahead += make_key(x, static_cast<uint32_t>(i)) > key;
+      if (x != x) s.sum = x;
     }
-    // (nothing but -inf so far: any finite number stands in for the maximum)
+    note(most, b);
     const float neg = s.m == -INFINITY ? 0.f : -s.m;
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = index_of(v, j);
+      if (i < 0 || i >= V) continue;
+      const float y = fmaxf((load_one<kType>(row, i) + neg) * kLog2e, -200.f), e = ex2(y);  // (2^-200 is 0 next to the sum's 1)
+      s.sum += e, s.dot = fmaf(e, y, s.dot);
+    }
+  };
+  // The others, with a maximum below 1e37 in size: a finite number can stand in for -inf (0 times infinity would be NaN).
+  auto batch = [&](const uint4 (&raw)[kVecs], int b) {
+    note(batch_max<kType>(raw), b);
+    if (!(fabsf(s.m) < 1e37f)) return false;
+    s.ahead += count_above<kType>(raw, b < token_batch ? above_before : above);
+    const float neg = -s.m;
     float sum0 = 0.f, sum1 = 0.f, dot0 = 0.f, dot1 = 0.f;
 #pragma unroll
-    for (int j = 0; j < kBatch; j += 2) {
-      float y0 = x[j], y1 = x[j + 1];
-      fadd2(y0, y1, neg, neg);
-      // 2^-200 is 0 next to the sum's 1, and 0 times -inf would be NaN
-      y0 = fmaxf(y0 * kLog2e, -200.f), y1 = fmaxf(y1 * kLog2e, -200.f);
-      const float e0 = ex2(y0), e1 = ex2(y1);
-      fadd2(sum0, sum1, e0, e1);
-      dot0 = fmaf(e0, y0, dot0), dot1 = fmaf(e1, y1, dot1);
+    for (int q = 0; q < kVecs; ++q) {
+      float x[kW];
+      unpack<kType>(clamp_low<kType>(raw[q]), x);
+#pragma unroll
+      for (int j = 0; j < kW; j += 2) {
+        float y0 = x[j], y1 = x[j + 1];
+        fadd2(y0, y1, neg, neg);
+        fmul2(y0, y1, kLog2e);
+        const float e0 = ex2(y0), e1 = ex2(y1);
+        fadd2(sum0, sum1, e0, e1);
+        ffma2(dot0, dot1, e0, e1, y0, y1);
+      }
     }
     s.sum += sum0 + sum1, s.dot += dot0 + dot1;
+    return true;
+  };
+  auto simple = [&](int b) { return b >= whole_from && b < whole_to && b != token_batch && !odd; };
+  uint4 next[kVecs];
+  auto read = [&](int b) {
+    if (b < last && simple(b)) {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q) next[q] = __ldg(vecs + b * kSpan + q * 32 + lane);
+    }
+  };
+  read(first + warp);
+  for (int b = first + warp; b < last; b += kWarps) {
+    bool done = false;
+    if (simple(b)) {
+      uint4 raw[kVecs];
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q) raw[q] = next[q];
+      read(b + kWarps);
+      done = batch(raw, b);
+      if (!done) {  // (its maximum is noted; the sums below are over the same numbers)
+        const float neg = s.m == -INFINITY ? 0.f : -s.m;
+        s.ahead += count_above<kType>(raw, b < token_batch ? above_before : above);
+        for (int j = 0; j < kBatch; ++j) {
+          const float x = load_one<kType>(row, index_of(b * kSpan + lane, j));
+          const float y = fmaxf((x + neg) * kLog2e, -200.f), e = ex2(y);
+          s.sum += x != x ? x : e, s.dot = fmaf(e, y, s.dot);
+        }
+      }
+    } else {
+      careful(b);
+      read(b + kWarps);
+    }
   }
   if (in_slot > 0) sh.batch_max[slot++][threadIdx.x] = slot_max;
+  s.nan = s.sum != s.sum;
+  // the thread's maximum, with an index that it is not behind
+  const uint64_t best =
+      best_at < 0 ? 0 : make_key(s.m, static_cast<uint32_t>(min(V - 1, max(0, index_of(best_at * kSpan + lane, kBatch - 1)))));
 
   // ------------------------------------------------------------- the sums
   const float thread_max = s.m;
@@ -235,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   // ------------------------------------------------------------- the alternatives
   if (top > 0) {
     // warps whose first batch is whole: all lanes have entries (a cut vector has one at least)
-    const int full = min(kWarps, max(0, min(last, vectors / 64) - first));
+    const int full = min(kWarps, max(0, min(last, vectors / kSpan) - first));
     // the lowest of the warps' nth largest, nth = top / warps, or (where that leaves too many: equal logits) the highest of
     // their `top`-th
     auto find_bound = [&](bool one) {
@@ -246,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
         if (k == at) k = 0;
       }
       if (lane == 0) sh.bound[warp] = warp < full ? at : one ? 0 : ~0ull;
-      if (threadIdx.x == 0) sh.count = 0;
+      if (threadIdx.x == 0) sh.count = sh.hit_count = 0;
       __syncthreads();
       uint64_t bound = sh.bound[0];
 #pragma unroll
@@ -260,27 +385,32 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       if (order_bits(thread_max) >= bound_hi) {
         for (int i = 0; i < slot; ++i) {
           if (order_bits(sh.batch_max[i][threadIdx.x]) < bound_hi) continue;
+          const int to = atomicAdd(&sh.hit_count, 1);
+          if (to < kList) sh.hits[to] = static_cast<uint32_t>(i) << 16 | threadIdx.x;
+        }
+      }
+      __syncthreads();
+      const int hits = sh.hit_count;
+      if (hits <= kList) {
+        // a lane per entry (fp32: two batches at once)
+        constexpr int kAtOnce = 32 / kBatch;
+        for (int i = warp * kAtOnce + lane / kBatch; i < hits; i += kWarps * kAtOnce) {
+          const uint32_t hit = sh.hits[i];
+          const int who = hit & 0xffff, b0 = first + (who >> 5) + static_cast<int>(hit >> 16) * per_slot * kWarps;
           for (int j = 0; j < per_slot; ++j) {
-            const int bb = first + warp + (i * per_slot + j) * kWarps;
-            if (bb >= last) break;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int v = bb * 64 + q * 32 + lane;
-              float x[kW];
-              expand(fetch(v), v, x);
-#pragma unroll
-              for (int e = 0; e < kW; ++e) {
-                const int idx = v * kW - shift + e;
-                if (idx < 0 || idx >= V) continue;
-                const uint64_t a = make_key(x[e], static_cast<uint32_t>(idx));
-                if (a >= bound) {
-                  const int to = atomicAdd(&sh.count, 1);
-                  if (to < kList) sh.list[to] = a;
-                }
-              }
+            const int b = b0 + j * kWarps;
+            if (b >= last) break;
+            const int idx = index_of(b * kSpan + (who & 31), lane % kBatch);
+            if (idx < 0 || idx >= V) continue;
+            const uint64_t a = make_key(load_one<kType>(row, idx), static_cast<uint32_t>(idx));
+            if (a >= bound) {
+              const int to = atomicAdd(&sh.count, 1);
+              if (to < kList) sh.list[to] = a;
             }
           }
         }
+      } else if (threadIdx.x == 0) {
+        sh.count = kList + 1;
       }
       __syncthreads();
       count = sh.count;
@@ -303,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       uint64_t limit = ~0ull;
       for (int k = 0; k < top; ++k) {
         uint64_t most = 0;
-        for (int i = first * 64 * kW + static_cast<int>(threadIdx.x); i < last * 64 * kW; i += kThreads) {
+        for (int i = first * kSpan * kW + static_cast<int>(threadIdx.x); i < last * kSpan * kW; i += kThreads) {
           const int idx = i - shift;
           if (idx < 0 || idx >= V) continue;
           const uint64_t a = make_key(load_one<kType>(row, idx), static_cast<uint32_t>(idx));
@@ -370,7 +500,7 @@ size_t token_logprobs_workspace(const LogprobsLaunch&) { return 0; }
 
 cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void*, cudaStream_t stream) {
   // as many CTAs per row as run at once, with a batch for each of their warps
-  const int64_t batch = 64 * (p.dtype == 2 ? 4 : 8);
+  const int64_t batch = 32 * kVecs * (p.dtype == 2 ? 4 : 8);
   int ctas = 1;
   while (ctas < kMaxCtas && p.rows * ctas * 2 <= kPerSm * kNumSMs && p.vocab >= 2 * ctas * kWarps * batch) ctas *= 2;
   auto kern = p.dtype == 2 ? logprobs_kernel<2> : p.dtype == 1 ? logprobs_kernel<1> : logprobs_kernel<0>;

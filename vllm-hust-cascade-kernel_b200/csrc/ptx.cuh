@@ -730,6 +730,29 @@ __device__ __forceinline__ void fadd2(float& a0, float& a1, float b0, float b1) 
       : "f"(b0), "f"(b1));
 }
 
+// (a0, a1) *= b in one packed-fp32 instruction.
+__device__ __forceinline__ void fmul2(float& a0, float& a1, float b) {
+  asm("{\n\t.reg .b64 ra, rb;\n\t"
+      "mov.b64 ra, {%0, %1};\n\t"
+      "mov.b64 rb, {%2, %2};\n\t"
+      "mul.rn.f32x2 ra, ra, rb;\n\t"
+      "mov.b64 {%0, %1}, ra;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b));
+}
+
+// (d0, d1) += (a0 * b0, a1 * b1), each rounded once, in one packed-fp32 instruction.
+__device__ __forceinline__ void ffma2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\t"
+      "mov.b64 rb, {%4, %5};\n\t"
+      "mov.b64 rd, {%0, %1};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rd;\n\t"
+      "mov.b64 {%0, %1}, rd;\n\t}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
 // Byte offset of 16-byte chunk `chunk` (0..7) of row `row` in a 128-byte
 // swizzled tile (the TMA / UMMA SWIZZLE_128B pattern: chunk ^= row % 8).
 __device__ __forceinline__ uint32_t sw128(uint32_t row, uint32_t chunk) {
