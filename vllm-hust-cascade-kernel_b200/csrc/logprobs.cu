@@ -96,12 +96,12 @@ __device__ __forceinline__ float batch_max(const uint4 (&v)[kVecs]) {
 }
 
 // how many of a batch's logits are above `bar`, which the type holds
-template <int kType>
-__device__ __forceinline__ int count_above(const uint4 (&v)[kVecs], float bar) {
+template <int kType, int kN>
+__device__ __forceinline__ int count_above(const uint4 (&v)[kN], float bar) {
   if constexpr (kType == 2) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
+    for (int i = 0; i < kN; ++i)
       n += (__uint_as_float(v[i].x) > bar) + (__uint_as_float(v[i].y) > bar) + (__uint_as_float(v[i].z) > bar) +
            (__uint_as_float(v[i].w) > bar);
     return n;
@@ -110,7 +110,7 @@ __device__ __forceinline__ int count_above(const uint4 (&v)[kVecs], float bar) {
     const __half2 b = __float2half2_rn(bar);
     __half2 n[2] = {__hgt2(h[0], b), __hgt2(h[1], b)};
 #pragma unroll
-    for (int i = 2; i < 4 * kVecs; ++i) n[i & 1] = __hadd2(n[i & 1], __hgt2(h[i], b));
+    for (int i = 2; i < 4 * kN; ++i) n[i & 1] = __hadd2(n[i & 1], __hgt2(h[i], b));
     n[0] = __hadd2(n[0], n[1]);  // (whole numbers up to 32)
     return static_cast<int>(__low2float(n[0]) + __high2float(n[0]));
   } else {
@@ -118,7 +118,7 @@ __device__ __forceinline__ int count_above(const uint4 (&v)[kVecs], float bar) {
     const __nv_bfloat162 b = __float2bfloat162_rn(bar);
     __nv_bfloat162 n[2] = {__hgt2(h[0], b), __hgt2(h[1], b)};
 #pragma unroll
-    for (int i = 2; i < 4 * kVecs; ++i) n[i & 1] = __hadd2(n[i & 1], __hgt2(h[i], b));
+    for (int i = 2; i < 4 * kN; ++i) n[i & 1] = __hadd2(n[i & 1], __hgt2(h[i], b));
     n[0] = __hadd2(n[0], n[1]);
     return static_cast<int>(__low2float(n[0]) + __high2float(n[0]));
   }
@@ -233,11 +233,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
   const int per_slot = ((last - first + kWarps - 1) / kWarps + kSlots - 1) / kSlots;
   const float mine = given ? load_one<kType>(row, static_cast<int>(token)) : INFINITY;
   const uint64_t key = given ? make_key(mine, static_cast<uint32_t>(token)) : ~0ull;
-  // The entries ahead of the token: those above its logit, and its equals before it. A batch before the token counts what is
-  // above the next lower number, one after it what is above its own. The batch that has it goes entry by entry; so do those
-  // that are cut by the row's ends, and all of them for a logit of -inf or NaN (equal here).
+  // The entries ahead of the token: those above its logit, and its equals before it, which are above the next lower number.
+  // (For a logit of -inf or NaN, equal here, by their keys.)
   const float above = given ? mine : INFINITY, above_before = given ? next_below<kType>(mine) : INFINITY;
   const int token_batch = given ? static_cast<int>((token + shift) / (kSpan * kW)) : -1;
+  const int at = given ? static_cast<int>(token) : 0;
   const bool odd = given && !(mine > -INFINITY);
   const int whole_from = shift > 0, whole_to = (V + shift) / (kSpan * kW);  // batches of whole vectors alone
 
@@ -260,32 +260,58 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       slot_max = -INFINITY, in_slot = 0;
     }
   };
-  // Entry by entry, and with logits of any size: sums of e and e y, y = (x - m) log2(e).
+  // Batches that the row's ends cut, with logits of any size: sums of e and e y, y = (x - m) log2(e).
   auto careful = [&](int b) {
     const int v = b * kSpan + lane;
     float most = -INFINITY;
-    for (int j = 0; j < kBatch; ++j) {
-      const int i = index_of(v, j);
-      if (i < 0 || i >= V) continue;
-      const float x = load_one<kType>(row, i);
-      most = fmaxf(most, x);
-      s.ahead += make_key(x, static_cast<uint32_t>(i)) > key;
-      if (x != x) s.sum = x;
+    auto load = [&](int q, float (&x)[kW]) {
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        const int i = index_of(v, q * kW) + j;
+        x[j] = i >= 0 && i < V ? load_one<kType>(row, i) : -INFINITY;
+      }
+    };
+#pragma unroll 1
+    for (int q = 0; q < kVecs; ++q) {
+      float x[kW];
+      load(q, x);
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        const int i = index_of(v, q * kW) + j;
+        most = fmaxf(most, x[j]);
+        s.ahead += odd ? i >= 0 && i < V && make_key(x[j], static_cast<uint32_t>(i)) > key : x[j] > (i < at ? above_before : above);
+      }
     }
     note(most, b);
     const float neg = s.m == -INFINITY ? 0.f : -s.m;
-    for (int j = 0; j < kBatch; ++j) {
-      const int i = index_of(v, j);
-      if (i < 0 || i >= V) continue;
-      const float y = fmaxf((load_one<kType>(row, i) + neg) * kLog2e, -200.f), e = ex2(y);  // (2^-200 is 0 next to the sum's 1)
-      s.sum += e, s.dot = fmaf(e, y, s.dot);
+#pragma unroll 1
+    for (int q = 0; q < kVecs; ++q) {
+      float x[kW];
+      load(q, x);
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        const float y = fmaxf((x[j] + neg) * kLog2e, -200.f), e = ex2(y);  // (2^-200 is 0 next to the sum's 1)
+        s.sum += x[j] != x[j] ? x[j] : e, s.dot = fmaf(e, y, s.dot);
+      }
     }
   };
   // The others, with a maximum below 1e37 in size: a finite number can stand in for -inf (0 times infinity would be NaN).
   auto batch = [&](const uint4 (&raw)[kVecs], int b) {
-    note(batch_max<kType>(raw), b);
-    if (!(fabsf(s.m) < 1e37f)) return false;
-    s.ahead += count_above<kType>(raw, b < token_batch ? above_before : above);
+    const float most = batch_max<kType>(raw);
+    if (__any_sync(0xffffffffu, !(fabsf(fmaxf(s.m, most)) < 1e37f))) return false;
+    note(most, b);
+    if (b != token_batch) {
+      s.ahead += count_above<kType>(raw, b < token_batch ? above_before : above);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kVecs; ++q) {
+        const int i = index_of(b * kSpan + lane, q * kW);
+        const uint4 one[1] = {raw[q]};
+        s.ahead += count_above<kType>(one, i + kW <= at ? above_before : above);
+        if (i <= at && at < i + kW)  // the equals before the token in its own vector
+          for (int j = i; j < at; ++j) s.ahead += load_one<kType>(row, j) == mine;
+      }
+    }
     const float neg = -s.m;
     float sum0 = 0.f, sum1 = 0.f, dot0 = 0.f, dot1 = 0.f;
 #pragma unroll
@@ -305,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
     s.sum += sum0 + sum1, s.dot += dot0 + dot1;
     return true;
   };
-  auto simple = [&](int b) { return b >= whole_from && b < whole_to && b != token_batch && !odd; };
+  auto simple = [&](int b) { return b >= whole_from && b < whole_to && !odd; };
   uint4 next[kVecs];
   auto read = [&](int b) {
     if (b < last && simple(b)) {
@@ -322,19 +348,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       for (int q = 0; q < kVecs; ++q) raw[q] = next[q];
       read(b + kWarps);
       done = batch(raw, b);
-      if (!done) {  // (its maximum is noted; the sums below are over the same numbers)
-        const float neg = s.m == -INFINITY ? 0.f : -s.m;
-        s.ahead += count_above<kType>(raw, b < token_batch ? above_before : above);
-        for (int j = 0; j < kBatch; ++j) {
-          const float x = load_one<kType>(row, index_of(b * kSpan + lane, j));
-          const float y = fmaxf((x + neg) * kLog2e, -200.f), e = ex2(y);
-          s.sum += x != x ? x : e, s.dot = fmaf(e, y, s.dot);
-        }
-      }
     } else {
-      careful(b);
       read(b + kWarps);
     }
+    if (!done) careful(b);
   }
   if (in_slot > 0) sh.batch_max[slot++][threadIdx.x] = slot_max;
   s.nan = s.sum != s.sum;
@@ -383,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
       const uint64_t bound = find_bound(round > 0);
       const uint32_t bound_hi = static_cast<uint32_t>(bound >> 32);
       if (order_bits(thread_max) >= bound_hi) {
+#pragma unroll 1
         for (int i = 0; i < slot; ++i) {
           if (order_bits(sh.batch_max[i][threadIdx.x]) < bound_hi) continue;
           const int to = atomicAdd(&sh.hit_count, 1);
@@ -425,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_kernel(const Logpro
         }
         const uint64_t a = sh.list[i];
         int before = 0;
+#pragma unroll 4
         for (int j = 0; j < count; ++j) before += sh.list[j] > a;
         if (before < top) sh.sorted[before] = a;
       }
