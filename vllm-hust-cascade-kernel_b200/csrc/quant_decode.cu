@@ -27,6 +27,7 @@
 // keeps every shared-memory load of 80-byte rows free of bank conflicts.
 // The running maxima move only when a score exceeds its row's by more than 2^8.
 #include <algorithm>
+#include <type_traits>
 
 #include "quant_decode.cuh"
 
@@ -42,11 +43,14 @@ constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
 template <int kN>  // query rows / 8
 struct Shape {
   static constexpr int kRows = 8 * kN;
-  static constexpr int kWarps = kN == 1 ? 16 : 12;
-  static constexpr int kStages = kN == 1 ? 2 : 3;     // tiles per group
-  static constexpr int kHeads = kN == 1 ? 8 : 4;      // most kv heads per group
+  static constexpr int kWarps = kN == 1 ? 16 : kN == 2 ? 12 : 8;  // (128, 168, 255 registers)
+  static constexpr int kStages = kN < 3 ? 2 : 3;                  // tiles per group
+  static constexpr int kHeads = kN == 2 ? 4 : 8;                  // most kv heads per group
   static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;
-  static constexpr int kSmem = kRing + 128;  // (to align the ring: the TMA writes to 128-byte boundaries)
+  // the queries' fragments: in registers, or in shared memory ([warp][8 rows][group of 32 values][lane])
+  static constexpr int kQuery = kN == 1 ? 0 : kWarps * kN * 4 * 32 * 16;
+  static constexpr int kSmem = kRing + kQuery + 128;  // (to align the ring: the TMA writes to 128-byte boundaries)
+  static_assert(kSmem + 1024 <= 227 * 1024, "shared memory per CTA");
 };
 
 struct Params {
@@ -171,6 +175,8 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
   const uint32_t head_off = (kStride == 160 ? member >> 1 : member) * P.box_rows * kStride + (kStride == 160 ? (member & 1) * kQuantRow : 0);
   const uint32_t base = smem_u32(mine) + head_off;
   const uint32_t value_off = P.heads * kTileBytes, half_off = P.box_rows == 16 ? nz * 16 * kStride : 16 * kStride;  // (16 tokens on)
+  uint8_t* query = ring + S::kRing + warp * (S::kQuery / kWarps);  // this warp's
+  const uint32_t query_at = smem_u32(query);
   int issued = 0, done = 0;
   bool live = true;
   if (p.debug_stall) live = mbar_wait_warp(&stall, 0);  // test hook: runs into the wait limit
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
       for (int i = 0; i < min(kStages, walk.n); ++i) issue();
     }
 
-    uint32_t qf[kN][16], zf[kN][2];
+    uint32_t qf[1][16], zf[kN][2];  // qf: one block of rows' (others read theirs back)
     float mult[kN][2];   // of columns 2 t, 2 t + 1: score * scale * log2(e) per unit of the products
     int lim[kN][2];
 #pragma unroll
@@ -294,10 +300,14 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
         float s = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         sums[k] = s + __shfl_xor_sync(0xffffffffu, s, 2);
-        qf[n][4 * k] = pack2<true>(y[0], y[4]);
-        qf[n][4 * k + 1] = pack2<true>(y[1] * 0.0625f, y[5] * 0.0625f);
-        qf[n][4 * k + 2] = pack2<true>(y[2], y[6]);
-        qf[n][4 * k + 3] = pack2<true>(y[3] * 0.0625f, y[7] * 0.0625f);
+        const uint32_t f[4] = {pack2<true>(y[0], y[4]), pack2<true>(y[1] * 0.0625f, y[5] * 0.0625f), pack2<true>(y[2], y[6]),
+                               pack2<true>(y[3] * 0.0625f, y[7] * 0.0625f)};
+        if constexpr (kN == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[0][4 * k + e] = f[e];
+        } else {
+          *reinterpret_cast<uint4*>(query + ((n * 4 + k) * 32 + lane) * 16) = make_uint4(f[0], f[1], f[2], f[3]);
+        }
       }
       const float z = (t == 0 ? sums[0] : t == 1 ? sums[1] : t == 2 ? sums[2] : sums[3]) * 0x1p-14f, y = -7.5f * z;
       zf[n][0] = pack2<true>(z, y);
@@ -313,6 +323,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
         lim[n][k] = unit.limit(walk.q, walk.kv, i);
       }
     }
+    if constexpr (kN > 1) __syncwarp();  // (a lane reads back what it wrote alone; this orders the asm loads behind it)
     int token;
     row_of(0, token);
     const int clean = min(walk.kv, unit.limit(walk.q, walk.kv, token));  // tokens below are seen by every row
@@ -331,14 +342,17 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
     // a tile: 32 tokens from `tok` on, their keys at shared address `ka`
     auto step = [&](uint32_t ka, int tok, auto masked) {
       float s[2][kN][4];
+      uint32_t wa[2][4], wb[2][4], pa[2][4], pb[2][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const uint32_t a = ka + (u ? half_off : 0);
         const uint4 wa4 = lds128(a + off_k), wb4 = lds128(a + off_k + kNext);
         const uint4 pa4 = lds128(a + off_kp), pb4 = lds128(a + off_kp + kNext);
         const uint32_t za = lds32(a + off_kp + 4 * t), zb = lds32(a + off_kp + kNext + 4 * t);
-        const uint32_t wa[4] = {wa4.x, wa4.y, wa4.z, wa4.w}, wb[4] = {wb4.x, wb4.y, wb4.z, wb4.w};
-        const uint32_t pa[4] = {pa4.x, pa4.y, pa4.z, pa4.w}, pb[4] = {pb4.x, pb4.y, pb4.z, pb4.w};
+        wa[u][0] = wa4.x, wa[u][1] = wa4.y, wa[u][2] = wa4.z, wa[u][3] = wa4.w;
+        wb[u][0] = wb4.x, wb[u][1] = wb4.y, wb[u][2] = wb4.z, wb[u][3] = wb4.w;
+        pa[u][0] = pa4.x, pa[u][1] = pa4.y, pa[u][2] = pa4.z, pa[u][3] = pa4.w;
+        pb[u][0] = pb4.x, pb[u][1] = pb4.y, pb[u][2] = pb4.z, pb[u][3] = pb4.w;
         const uint32_t z[4] = {za, zb, za, zb};
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
@@ -346,19 +360,35 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
 #pragma unroll
           for (int k = 0; k < 4; ++k) s[u][n][k] *= 0x1p-10f;
         }
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t a0[4] = {wa[i] & kLow, wb[i] & kLow, wa[i] & kHigh, wb[i] & kHigh};
-          const uint32_t xa = wa[i] >> 8, xb = wb[i] >> 8;
-          const uint32_t a1[4] = {xa & kLow, xb & kLow, xa & kHigh, xb & kHigh};
-          const float fa = high_half(pa[i]), fb = high_half(pb[i]);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a0[2][4], a1[2][4];
+        float fa[2], fb[2];
 #pragma unroll
-          for (int n = 0; n < kN; ++n) {
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t xa = wa[u][i] >> 8, xb = wb[u][i] >> 8;
+          a0[u][0] = wa[u][i] & kLow, a0[u][1] = wb[u][i] & kLow, a0[u][2] = wa[u][i] & kHigh, a0[u][3] = wb[u][i] & kHigh;
+          a1[u][0] = xa & kLow, a1[u][1] = xb & kLow, a1[u][2] = xa & kHigh, a1[u][3] = xb & kHigh;
+          fa[u] = high_half(pa[u][i]), fb[u] = high_half(pb[u][i]);
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          uint32_t q[4];
+          if constexpr (kN == 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = qf[0][4 * i + e];
+          } else {
+            const uint4 v = lds128(query_at + ((n * 4 + i) * 32 + lane) * 16);
+            q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w;
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
             float x[4];
-            mma_fresh(x, a0, qf[n][4 * i], qf[n][4 * i + 1]);
-            mma_16816<true>(x, a1, qf[n][4 * i + 2], qf[n][4 * i + 3]);
-            s[u][n][0] = fmaf(fa, x[0], s[u][n][0]), s[u][n][1] = fmaf(fa, x[1], s[u][n][1]);
-            s[u][n][2] = fmaf(fb, x[2], s[u][n][2]), s[u][n][3] = fmaf(fb, x[3], s[u][n][3]);
+            mma_fresh(x, a0[u], q[0], q[1]);
+            mma_16816<true>(x, a1[u], q[2], q[3]);
+            s[u][n][0] = fmaf(fa[u], x[0], s[u][n][0]), s[u][n][1] = fmaf(fa[u], x[1], s[u][n][1]);
+            s[u][n][2] = fmaf(fb[u], x[2], s[u][n][2]), s[u][n][3] = fmaf(fb[u], x[3], s[u][n][3]);
           }
         }
       }
@@ -590,18 +620,33 @@ cudaError_t launch(const QuantDecodeLaunch& p, void* workspace, cudaStream_t str
   return launch_quant_combine<kFp16, S::kRows>(p, P.parts, stream);
 }
 
-// Query rows per warp: 16 where a request has more than 8 (known from the shapes: the mean, with lengths on the device).
-bool wide(const QuantDecodeLaunch& p) { return p.num_tokens * p.group > 8 * static_cast<int64_t>(p.batch); }
+// Blocks of 8 query rows per warp: as a request has rows, up to four (known from the shapes: the mean, with lengths on the
+// device). Unpacking is shared by a warp's blocks: 259 instructions per 16 tokens for one block, some 60 for each more.
+int row_blocks(const QuantDecodeLaunch& p) {
+  const int64_t rows = (p.num_tokens * p.group + p.batch - 1) / p.batch;
+  return static_cast<int>(std::min<int64_t>(4, (rows + 7) / 8));
+}
+
+template <int kN>
+size_t workspace_of(const QuantDecodeLaunch& p) {
+  return quant_partial_bytes(p, run_count<kN>(p), Shape<kN>::kRows);
+}
 
 }  // namespace
 
 size_t quant_decode_workspace(const QuantDecodeLaunch& p) {
-  return wide(p) ? quant_partial_bytes(p, run_count<2>(p), Shape<2>::kRows) : quant_partial_bytes(p, run_count<1>(p), Shape<1>::kRows);
+  const int n = row_blocks(p);
+  return n == 1 ? workspace_of<1>(p) : n == 2 ? workspace_of<2>(p) : n == 3 ? workspace_of<3>(p) : workspace_of<4>(p);
 }
 
 cudaError_t launch_quant_decode(const QuantDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
-  if (wide(p)) return fp16 ? launch<true, 2>(p, workspace, stream) : launch<false, 2>(p, workspace, stream);
-  return fp16 ? launch<true, 1>(p, workspace, stream) : launch<false, 1>(p, workspace, stream);
+  auto go = [&](auto n) { return fp16 ? launch<true, n.value>(p, workspace, stream) : launch<false, n.value>(p, workspace, stream); };
+  switch (row_blocks(p)) {
+    case 1: return go(std::integral_constant<int, 1>());
+    case 2: return go(std::integral_constant<int, 2>());
+    case 3: return go(std::integral_constant<int, 3>());
+    default: return go(std::integral_constant<int, 4>());
+  }
 }
 
 }  // namespace cascade
