@@ -320,6 +320,9 @@ struct QuantDecodeLaunch {
 };
 cudaError_t launch_quant_decode(const QuantDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream);
 size_t quant_decode_workspace(const QuantDecodeLaunch& p);
+// The same on the tensor cores' 128-row tiles, for many query rows per request.
+cudaError_t launch_quant_tiles(const QuantDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream);
+size_t quant_tiles_workspace(const QuantDecodeLaunch& p);
 
 // ----------------------------------------------------------------------------
 // Log probabilities of tokens

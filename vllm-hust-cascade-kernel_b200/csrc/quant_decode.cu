@@ -620,11 +620,12 @@ cudaError_t launch(const QuantDecodeLaunch& p, void* workspace, cudaStream_t str
   return launch_quant_combine<kFp16, S::kRows>(p, P.parts, stream);
 }
 
-// Blocks of 8 query rows per warp: as a request has rows, up to four (known from the shapes: the mean, with lengths on the
-// device). Unpacking is shared by a warp's blocks: 259 instructions per 16 tokens for one block, some 60 for each more.
+// Blocks of 8 query rows per warp: as a request has rows (known from the shapes: the mean, with lengths on the device).
+// Unpacking is shared by a warp's blocks: 259 instructions per 16 tokens for one block, some 60 for each more. More than
+// four go to the 128-row tiles (0).
 int row_blocks(const QuantDecodeLaunch& p) {
   const int64_t rows = (p.num_tokens * p.group + p.batch - 1) / p.batch;
-  return static_cast<int>(std::min<int64_t>(4, (rows + 7) / 8));
+  return rows <= 32 ? static_cast<int>((rows + 7) / 8) : 0;
 }
 
 template <int kN>
@@ -636,12 +637,14 @@ size_t workspace_of(const QuantDecodeLaunch& p) {
 
 size_t quant_decode_workspace(const QuantDecodeLaunch& p) {
   const int n = row_blocks(p);
+  if (n == 0) return quant_tiles_workspace(p);
   return n == 1 ? workspace_of<1>(p) : n == 2 ? workspace_of<2>(p) : n == 3 ? workspace_of<3>(p) : workspace_of<4>(p);
 }
 
 cudaError_t launch_quant_decode(const QuantDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
   auto go = [&](auto n) { return fp16 ? launch<true, n.value>(p, workspace, stream) : launch<false, n.value>(p, workspace, stream); };
   switch (row_blocks(p)) {
+    case 0: return launch_quant_tiles(p, fp16, workspace, stream);
     case 1: return go(std::integral_constant<int, 1>());
     case 2: return go(std::integral_constant<int, 2>());
     case 3: return go(std::integral_constant<int, 3>());

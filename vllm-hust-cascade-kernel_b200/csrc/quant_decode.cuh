@@ -49,8 +49,10 @@ struct QuantPartials {
   int32_t runs;
 };
 // row r of a unit cut into `count` >= 2 pieces, the first in run c
-__device__ __forceinline__ int32_t pack_info(int c, int count, int r) { return (count << 18) | (c << 6) | r; }
-constexpr int kMaxRuns = 4095, kMaxBlockRows = 64;
+__device__ __forceinline__ int32_t pack_info(int c, int count, int r) {
+  return static_cast<int32_t>(static_cast<uint32_t>(count) << 20 | static_cast<uint32_t>(c) << 8 | static_cast<uint32_t>(r));
+}
+constexpr int kMaxRuns = 4095, kMaxBlockRows = 256;
 
 // A run, as its first unit and the place in it.
 struct QuantRun {
@@ -207,8 +209,8 @@ __global__ void __launch_bounds__(kWarps == 1 ? 256 : 32 * kWarps)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = kWarps == 1 ? static_cast<int64_t>(blockIdx.x) * 8 + warp : blockIdx.x;
   if (row >= L.num_tokens * L.num_heads) return;
-  const int32_t info = P.row_info[row];
-  const int count = info >> 18, c0 = (info >> 6) & kMaxRuns, r = info & (kMaxBlockRows - 1);
+  const uint32_t info = static_cast<uint32_t>(P.row_info[row]);
+  const int count = static_cast<int>(info >> 20), c0 = static_cast<int>(info >> 8) & kMaxRuns, r = static_cast<int>(info) & (kMaxBlockRows - 1);
   // (an aborted run may have left its rows' info as the workspace held it: nothing past the slots is read for them)
   if (count < 2 || c0 + count > P.runs || r >= kBlockRows) return;
   const int h = static_cast<int>(row % L.num_heads) / L.group;

@@ -1,0 +1,612 @@
+// Attention over a 4-bit key-value cache (cascade_quant_decode) for many query rows
+// per request and kv head (chunks of prompts, prefixes that a batch shares), on the
+// tensor cores: bound by them, with the exponentials (16 per clock and SM) close
+// behind.
+//
+// A block of 256 query rows (token and head of the group, in that order) of one
+// request and kv head are two tiles of 128 that share the unpacked tokens, 128 at a
+// time. Keys stay exact: with a group's centre c and scale s a value is
+// (code - 7.5) s + c, and s is split in two, s = s1 + s2, of 7 and 4 significant
+// bits, so that (code - 7.5) s1 and (code - 7.5) s2 are fp16 numbers; the centres
+// meet the groups' sums of the query in a product of 16 more columns. 272 columns for
+// 128 (a key rounded to fp16 would be 2^-11 off in each of its 128 products, the
+// scores' sums in fp32 are not). Queries are fp16 too, each row times a power of two. Values are
+// rounded to fp16 once.
+//
+// Warps: 0-7 softmax and output of tile A, 8-15 of tile B, 16 MMA issue, 17-19
+// unpack (17 loads, too). Per step j of 128 tokens the issue order is PV_A(j),
+// S_A(j+1), PV_B(j), S_B(j+1); the keys of step j + 1 are unpacked when both tiles'
+// scores of step j are done, the values when both tiles' outputs are, while the other
+// tile's softmax runs. P lies over its scores in tensor memory, which the two tiles'
+// scores and outputs fill (4 x 128 columns).
+//
+// A CTA takes an equal run of steps over the units (request, block) of one kv head;
+// what run boundaries cut is merged by quant_combine_kernel.
+#include <algorithm>
+#include <cstddef>
+
+#include "quant_decode.cuh"
+
+namespace cascade {
+namespace {
+
+constexpr int kBlock = 256, kRows = 128, kTok = 128;
+constexpr int kSetup = 1;
+constexpr int kThreads = 20 * 32;
+constexpr int kUnpackWarps = 3;
+constexpr int kRaw = kTok * kQuantRow;           // keys or values of a step as they lie
+constexpr int kChunk = 16384;                    // 128 rows x 64 values
+constexpr int kOffQ = 0;                         // [tile][2 chunks]
+constexpr int kOffK = kOffQ + 4 * kChunk;        // [part of the scale][2 chunks]
+constexpr int kOffV = kOffK + 4 * kChunk;        // [64 tokens][64 values' group][token]
+constexpr int kOffZq = kOffV + 2 * kChunk;       // [tile][2 x 8 columns][128 rows][16 bytes]
+constexpr int kOffZk = kOffZq + 2 * 4096;
+constexpr int kOffRaw = kOffZk + 4096;           // [stage][keys, values]
+constexpr int kBytes = kOffRaw + 4 * kRaw;
+
+struct __align__(16) Aux {
+  float shared[2][2][kRows];  // [tile][half]: the row's maximum, at the end its sum
+  uint64_t raw_full[2], raw_empty[2], k_full, k_empty, v_full, v_empty, q_full[2], s_full[2], p_full[2], o_final[2], stall, drain;
+  uint32_t tmem_base;
+  QuantRun run;
+};
+constexpr int kStaticBytes = 32;  // the wait state comes first
+constexpr int kSmemBytes = (kStaticBytes + static_cast<int>(sizeof(Aux)) + 1023) / 1024 * 1024 + kBytes - kStaticBytes;
+static_assert(kSmemBytes + kStaticBytes <= 227 * 1024, "shared memory per CTA");
+
+struct Params {
+  QuantDecodeLaunch L;
+  CUtensorMap key, value;  // box: 80 bytes x box_rows cache rows of one head
+  QuantPartials parts;
+  int32_t box_rows;        // 16 .. 128
+};
+
+using Unit = QuantUnit<kBlock, kTok>;
+using Walk = QuantWalk<kBlock, kTok, kSetup>;
+
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
+__device__ __forceinline__ bool odd_par(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
+// the codes of a word, less 7.5: pairs of values (n, n + 4), n = 0..3
+__device__ __forceinline__ void codes(uint32_t w, __half2 (&c)[4]) {
+  const uint32_t lo = w << 1, hi = w >> 7, magic = 0x64006400u;
+  const __half2 a = __float2half2_rn(0.5f), b = __float2half2_rn(-519.5f), d = __float2half2_rn(0.03125f), e = __float2half2_rn(-39.5f);
+  c[0] = __hfma2(as_half2(and_or(lo, 0x001E001Eu, magic)), a, b);
+  c[1] = __hfma2(as_half2(and_or(lo, 0x01E001E0u, magic)), d, e);
+  c[2] = __hfma2(as_half2(and_or(hi, 0x001E001Eu, magic)), a, b);
+  c[3] = __hfma2(as_half2(and_or(hi, 0x01E001E0u, magic)), d, e);
+}
+
+// steps of tile t (128 rows) of a block, of the piece's `n` from step t0 on
+__device__ __forceinline__ int tile_steps(const Unit& u, const Walk& w, int t) {
+  const int first = w.block * kBlock + t * kRows, all = w.q * u.p.group;
+  if (first >= all) return 0;
+  const int last = (min(all, first + kRows) - 1) / u.p.group;
+  return max(0, min(w.n, (u.limit(w.q, w.kv, last) + kTok - 1) / kTok - w.t0));
+}
+
+template <bool kFp16>
+__global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_constant__ Params P) {
+  const QuantDecodeLaunch& p = P.L;
+  const Unit unit(p);
+  const int h = static_cast<int>(blockIdx.x) % p.kv_heads, c = static_cast<int>(blockIdx.x) / p.kv_heads;
+  extern __shared__ uint8_t smem_raw[];
+  Aux* aux = reinterpret_cast<Aux*>(smem_raw);
+  uint8_t* smem = smem_raw + sizeof(Aux) + ((0u - (smem_u32(smem_raw) + static_cast<uint32_t>(sizeof(Aux)))) & 1023u);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_launch_dependents();
+
+  if (tid == 0) {
+    cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&aux->raw_full[i], 1);
+      mbar_init(&aux->raw_empty[i], kUnpackWarps);
+      mbar_init(&aux->q_full[i], 8);
+      mbar_init(&aux->s_full[i], 1);
+      mbar_init(&aux->p_full[i], 8);
+      mbar_init(&aux->o_final[i], 1);
+    }
+    mbar_init(&aux->k_full, kUnpackWarps);
+    mbar_init(&aux->v_full, kUnpackWarps);
+    mbar_init(&aux->k_empty, 1);
+    mbar_init(&aux->v_empty, 1);
+    mbar_init(&aux->stall, 1);
+    mbar_init(&aux->drain, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&P.key);
+    tma_prefetch_desc(&P.value);
+  }
+  if (warp == 16) {
+    tmem_alloc(&aux->tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (warp == 17) {
+    const QuantRun r = find_run<kBlock, kTok, kSetup>(unit, c, P.parts.runs);
+    if (lane == 0) aux->run = r;
+  }
+  if (warp == 18 && p.q_len == 0) {  // rows of tokens that are no request's: nothing to merge
+    int64_t own = 0;
+    for (int b = lane; b < p.batch; b += 32) own += min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) own += __shfl_xor_sync(0xffffffffu, own, d);
+    for (int64_t i = min(own, p.num_tokens) * p.num_heads + blockIdx.x * 32 + lane; i < p.num_tokens * p.num_heads;
+         i += static_cast<int64_t>(gridDim.x) * 32)
+      P.parts.row_info[i] = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = aux->tmem_base;
+  const QuantRun run = aux->run;
+  const bool any = c < run.runs;
+  Walk walk(p, run);
+
+  if (warp >= 17) {
+    // ------------------------------------------------------------- unpack
+    const int w = warp - 17;
+    Walk load(p, run);
+    const int shift = __ffs(p.block_size) - 1, oob = p.num_blocks ? p.num_blocks * p.block_size : 1, boxes = kTok / P.box_rows;
+    int left = 0, step = 0, issued = 0;
+    int32_t id = 0;
+    bool more = any && w == 0;
+    // (warp 17) page id of this lane's box of the next step, as loaded: not used, and so not waited for, until then
+    auto next_ids = [&] {
+      if (left == 0) {
+        more = more && load.next();
+        if (!more) return;
+        left = load.n, step = load.t0;
+      }
+      const int at = step * kTok + lane * P.box_rows;
+      id = lane < boxes && at < load.kv ? p.block_table[static_cast<int64_t>(load.b) * p.block_cols + (at >> shift)] : INT32_MIN;
+    };
+    auto issue = [&] {
+      const int at = step * kTok + lane * P.box_rows, stage = issued & 1;
+      const bool good = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks);
+      if (!good && id != INT32_MIN) atomicOr(&g_cascade_device_error, kErrBadBlockId);
+      const int row = good ? id * p.block_size + (at & (p.block_size - 1)) : oob;
+      uint8_t* dst = smem + kOffRaw + stage * 2 * kRaw + lane * P.box_rows * kQuantRow;
+      if (lane == 0) mbar_arrive_expect_tx(&aux->raw_full[stage], 2 * kRaw);
+      __syncwarp();
+      if (lane < boxes) {
+        tma_load_3d(dst, &P.key, &aux->raw_full[stage], 0, row, h);
+        tma_load_3d(dst + kRaw, &P.value, &aux->raw_full[stage], 0, row, h);
+      }
+      __syncwarp();
+      ++issued, ++step, --left;
+      next_ids();
+    };
+    if (more) {
+      next_ids();
+      for (int i = 0; i < 2 && more; ++i) issue();
+    }
+    const int t = lane & 3, g8 = (lane >> 3) + 4 * ((lane >> 2) & 1);  // rows 4 apart are 16 banks apart
+    int n = 0;
+    bool live = any;
+    while (live && walk.next()) {
+      for (int j = 0; live && j < walk.n; ++j, ++n) {
+        const uint8_t* raw = smem + kOffRaw + (n & 1) * 2 * kRaw;
+        const int tok = (walk.t0 + j) * kTok;
+        live = mbar_wait_warp(&aux->raw_full[n & 1], (n >> 1) & 1) && (n < 1 || mbar_wait_warp(&aux->k_empty, (n - 1) & 1));
+        if (!live) break;
+        for (int i = w; i < kTok / 8; i += kUnpackWarps) {
+          const int r = i * 8 + g8;
+          const uint4 word = *reinterpret_cast<const uint4*>(raw + r * kQuantRow + 16 * t);
+          uint4 par = *reinterpret_cast<const uint4*>(raw + r * kQuantRow + kQuantCodes);
+          const uint32_t ws[4] = {word.x, word.y, word.z, word.w}, ps[4] = {par.x, par.y, par.z, par.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            __half2 cd[4];
+            codes(ws[k], cd);
+            const __half2 s = __high2half2(as_half2(ps[k]));
+            const __half2 s1 = as_half2(as_u32(s) & 0xFFF0FFF0u), s2 = __hsub2(s, s1);
+            uint32_t x[4], y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = as_u32(__hmul2(cd[e], s1)), y[e] = as_u32(__hmul2(cd[e], s2));
+            const int q = 4 * k + t;  // eight values
+            uint8_t* dst = smem + kOffK + (q >> 3) * kChunk + r * 128 + (((q ^ r) & 7) << 4);
+            *reinterpret_cast<uint4*>(dst) = make_uint4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint4*>(dst + 2 * kChunk) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+          if (t < 2) {
+            // the columns of centres (and scales, which meet zeros). A value that is NaN makes its token's scores NaN, and
+            // is 0 itself (below): rows that do not see it keep their sums.
+            const uint4 pv = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + kQuantCodes);
+            if (odd_par(pv.x) || odd_par(pv.y) || odd_par(pv.z) || odd_par(pv.w)) par.x = 0x7fffu;
+            *reinterpret_cast<uint4*>(smem + kOffZk + t * 2048 + r * 16) = par;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&aux->k_full);
+        live = n < 1 || mbar_wait_warp(&aux->v_empty, (n - 1) & 1);
+        if (!live) break;
+        for (int i = w; i < kTok / 8; i += kUnpackWarps) {
+          const int r = i * 8 + g8;
+          const uint4 word = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + 16 * t);
+          const uint4 par = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + kQuantCodes);
+          const uint32_t ws[4] = {word.x, word.y, word.z, word.w}, ps[4] = {par.x, par.y, par.z, par.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            __half2 cd[4];
+            codes(ws[k], cd);
+            const uint32_t pk = tok + r >= walk.kv || odd_par(ps[k]) ? 0u : ps[k];
+            const __half2 s = __high2half2(as_half2(pk)), off = __low2half2(as_half2(pk));
+            uint32_t x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = as_u32(__hfma2(cd[e], s, off));
+            const int q = 4 * k + t;
+            *reinterpret_cast<uint4*>(smem + kOffV + (r >> 6) * kChunk + (q >> 3) * (kChunk / 2) + (r & 63) * 128 +
+                                      (((q ^ r) & 7) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&aux->v_full);
+          mbar_arrive(&aux->raw_empty[n & 1]);
+        }
+        if (w == 0 && more) {
+          live = mbar_wait_warp(&aux->raw_empty[n & 1], (n >> 1) & 1);
+          if (live) issue();
+        }
+      }
+    }
+  } else if (warp == 16) {
+    // ----------------------------------------------------------- MMA issuer
+    const uint32_t idesc_s = make_idesc_f16(kRows, kTok, 0u, 0, 0);
+    const uint32_t idesc_pv = make_idesc_f16(kRows, kHeadDim, 0u, 0, 1);
+    const uint32_t tm = uniform(tbase), s0 = uniform(smem_u32(smem));
+    auto scores = [&](int t, bool last) {
+      const uint64_t dq = make_smem_desc(s0 + kOffQ + t * 2 * kChunk, 16, 1024, 2);
+      const uint64_t dk = make_smem_desc(s0 + kOffK, 16, 1024, 2);
+      const uint64_t zq = make_smem_desc(s0 + kOffZq + t * 4096, 2048, 128, 0), zk = make_smem_desc(s0 + kOffZk, 2048, 128, 0);
+      tc_fence_after();
+      if (elect_one()) {
+        umma_f16_ss(tm + t * 128, zq, zk, idesc_s, 0);
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+#pragma unroll
+          for (int ch = 0; ch < 2; ++ch) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_f16_ss(tm + t * 128, dq + (ch * kChunk + k * 32) / 16, dk + ((part * 2 + ch) * kChunk + k * 32) / 16, idesc_s, 1);
+          }
+        }
+        umma_commit(&aux->s_full[t]);
+        if (last) umma_commit(&aux->k_empty);
+      }
+      __syncwarp();
+    };
+    auto values = [&](int t, bool fresh, bool last, bool final) {
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          // 64 tokens x two groups of 64 values, 8 KB apart
+          const uint64_t dv = make_smem_desc(s0 + kOffV + ch * kChunk, kChunk / 2, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16_ts(tm + 256 + t * 128, tm + t * 128 + ch * 64 + k * 8, dv + k * 128, idesc_pv, !fresh || ch + k > 0);
+        }
+        if (last) umma_commit(&aux->v_empty);
+        if (final) umma_commit(&aux->o_final[t]);
+      }
+      __syncwarp();
+    };
+    int n = 0, sc[2] = {0, 0}, pieces[2] = {0, 0};  // steps, scores and pieces so far
+    bool live = any, used = false;
+    while (live && walk.next()) {
+      const int nt[2] = {tile_steps(unit, walk, 0), tile_steps(unit, walk, 1)};
+      // (the last tile with rows has all the piece's steps; a unit whose rows see nothing has a step all the same: its
+      // products go unread)
+      const int tl = nt[1] > 0 ? 1 : 0;
+      if (nt[0] == 0 && nt[1] == 0) {
+        live = mbar_wait_warp(&aux->k_full, n & 1) && mbar_wait_warp(&aux->v_full, n & 1);
+        if (live && elect_one()) {
+          umma_commit(&aux->k_empty);
+          umma_commit(&aux->v_empty);
+        }
+        __syncwarp();
+        used = true;
+        ++n;
+        continue;
+      }
+      for (int t = 0; live && t < 2; ++t)
+        if (nt[t] > 0) live = mbar_wait_warp(&aux->q_full[t], pieces[t]++ & 1);
+      live = live && mbar_wait_warp(&aux->k_full, n & 1);
+      if (!live) break;
+      used = true;
+      for (int t = 0; t < 2; ++t)
+        if (nt[t] > 0) scores(t, t == tl);
+      for (int j = 0; live && j < walk.n; ++j, ++n) {
+        live = mbar_wait_warp(&aux->v_full, n & 1);
+        bool have_k = false;
+        for (int t = 0; live && t < 2; ++t) {
+          if (j >= nt[t]) continue;
+          live = mbar_wait_warp(&aux->p_full[t], sc[t]++ & 1);
+          if (!live) break;
+          values(t, j == 0, t == tl, j + 1 == nt[t]);
+          if (j + 1 < nt[t]) {
+            live = have_k || mbar_wait_warp(&aux->k_full, (n + 1) & 1);
+            have_k = true;
+            if (live) scores(t, t == tl);
+          }
+        }
+      }
+    }
+    if (used && !live && lane == 0) {
+      umma_commit(&aux->drain);
+      mbar_wait_drain(&aux->drain, 0);
+    }
+  } else {
+    // ------------------------------------------------- softmax, output of tile t
+    const int t = warp >> 3, hh = (warp >> 2) & 1, r = tid & 127;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t scol = tbase + lane_off + t * 128, ocol = tbase + lane_off + 256 + t * 128 + hh * 64;
+    // the two warps of 32 rows meet here, and the eight of a tile; none leaves its loop early (an aborted CTA's waits
+    // return at once), so none is waited for in vain
+    auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
+    auto meet_tile = [&] { asm volatile("bar.sync %0, 256;" ::"r"(9 + t) : "memory"); };
+    if (p.debug_stall && any) mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
+    int sc = 0, pieces = 0;
+    while (any && walk.next()) {
+      const int rows = min(kBlock, walk.q * p.group - walk.block * kBlock);  // of the block
+      const int row = t * kRows + r, at = walk.block * kBlock + row, i = at / p.group;
+      const bool real = row < rows;
+      const int64_t out_row = real ? (walk.tok + i) * p.num_heads + h * p.group + (at - i * p.group) : 0;
+      const int mine = tile_steps(unit, walk, t);
+      float mult = 0.f, mx = -INFINITY, l = 0.f;
+      if (mine > 0) {
+        // ------------------------------------------------------------ query
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) + out_row * kHeadDim + hh * 64);
+        uint4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = real ? __ldg(src + k) : make_uint4(0u, 0u, 0u, 0u);
+        auto value = [&](int k, int e) {
+          const uint32_t w = e < 2 ? v[k].x : e < 4 ? v[k].y : e < 6 ? v[k].z : v[k].w;
+          if constexpr (kFp16) return e & 1 ? __high2float(as_half2(w)) : __low2float(as_half2(w));
+          return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+        };
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) top = fmax3f_nan(top, fabsf(value(k, e)), fabsf(value(k, e + 1)));
+        }
+        aux->shared[t][hh][r] = top;
+        meet();
+        top = fmax3f_nan(top, aux->shared[t][hh ^ 1][r], top);
+        // times 2^up: [2^8, 2^9), or less for rows below 2^-119. A row with a NaN or an infinity is NaN.
+        const int ex = max((__float_as_int(top) >> 23) & 255, 8), up = 135 - ex;
+        const float f = ex == 255 ? __int_as_float(0x7fffffff) : __int_as_float((127 + up) << 23);
+        float sums[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = value(k, e) * f;
+          sums[k >> 2] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+          *reinterpret_cast<uint4*>(smem + kOffQ + (t * 2 + hh) * kChunk + r * 128 + (((k ^ r) & 7) << 4)) =
+              make_uint4(pack2<true>(y[0], y[4]), pack2<true>(y[1], y[5]), pack2<true>(y[2], y[6]), pack2<true>(y[3], y[7]));
+        }
+        const uint32_t z0 = pack2<true>(sums[0], 0.f), z1 = pack2<true>(sums[1], 0.f);
+        uint8_t* z = smem + kOffZq + t * 4096 + r * 16 + hh * 8;
+        *reinterpret_cast<uint2*>(z) = make_uint2(z0, z1);
+        *reinterpret_cast<uint2*>(z + 2048) = make_uint2(pack2<true>(sums[0] - __low2float(as_half2(z0)), 0.f),
+                                                          pack2<true>(sums[1] - __low2float(as_half2(z1)), 0.f));
+        // (not 0, nor NaN: a masked score, -inf, stays -inf)
+        mult = fmaxf(__int_as_float((127 - up) << 23) * (p.scale * 1.4426950408889634f), 1e-37f);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&aux->q_full[t]);
+      }
+      // ---------------------------------------------------------- softmax
+      const int lim = unit.limit(walk.q, walk.kv, min(at, walk.q * p.group - 1) / p.group) - walk.t0 * kTok;
+      // steps below are seen in full by every row of the tile
+      const int clean = min(walk.kv, unit.limit(walk.q, walk.kv, (walk.block * kBlock + t * kRows) / p.group)) / kTok - walk.t0;
+      for (int j = 0; j < mine; ++j, ++sc) {
+        mbar_wait_warp(&aux->s_full[t], sc & 1);
+        tc_fence_after();
+        const int seen = j >= clean ? lim - j * kTok - hh * 64 : 64;
+        auto load = [&](int g, uint32_t (&x)[32]) {
+          tmem_ld_32x32b_x32(scol + hh * 64 + g * 32, x);
+          tmem_wait_ld();
+          if (j >= clean) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = g * 32 + e < seen ? x[e] : 0xff800000u;
+          }
+        };
+        float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t x[32];
+          load(g, x);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            a0 = fmax3f_nan(a0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+            a1 = fmax3f_nan(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+            a2 = fmax3f_nan(a2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
+            a3 = fmax3f_nan(a3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
+          }
+        }
+        a0 = fmax3f_nan(fmax3f_nan(a0, a1, a2), a3, a3);
+        aux->shared[t][hh][r] = a0;
+        meet();
+        const float top = fmax3f_nan(a0, aux->shared[t][hh ^ 1][r], a0) * mult;
+        // weights up to 2^6 after a move, to 2^14 before the next: fp16 holds 2^-24 of them
+        const bool move = top > mx + 14.f;
+        const float dm = move ? ex2(mx - (top - 6.f)) : 1.f;  // 0 while nothing has been seen
+        if (move) mx = top - 6.f;
+        const float neg = mx == -INFINITY ? 0.f : -mx;
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+          // the scores of step j come after P V of step j - 1: the output is at rest
+#pragma unroll 1
+          for (int g = 0; g < 2; ++g) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(ocol + g * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * dm);
+            tmem_st_32x32b_x32(ocol + g * 32, o);
+          }
+        }
+        // P goes over the first 32 columns of this half's own scores, read by then
+        float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint32_t x[32], pk[16];
+          load(g, x);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            float y0, y1, y2, y3;
+            ffma2_bcast(y0, y1, __uint_as_float(x[e]), __uint_as_float(x[e + 1]), mult, neg);
+            ffma2_bcast(y2, y3, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]), mult, neg);
+            y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
+            fadd2(r0, r1, y0, y1);
+            fadd2(r2, r3, y2, y3);
+            pk[e >> 1] = pack2<true>(y0, y1);
+            pk[(e >> 1) + 1] = pack2<true>(y2, y3);
+          }
+          tmem_st_32x32b_x16(scol + hh * 64 + g * 16, pk);
+        }
+        l = l * dm + ((r0 + r1) + (r2 + r3));
+        if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&aux->p_full[t]);
+      }
+      // ----------------------------------------------------------- output
+      float inv = 0.f, lse = -INFINITY;
+      if (mine > 0) {
+        mbar_wait_warp(&aux->o_final[t], pieces++ & 1);  // both warps have read the maxima: the slots take the sums
+        tc_fence_after();
+        aux->shared[t][hh][r] = l;
+        meet();
+        l = aux->shared[t][0][r] + aux->shared[t][1][r];
+        if (mx > -INFINITY || l != l) {  // (a NaN is no maximum)
+          inv = 1.f / l;
+          lse = (mx + __log2f(l)) * 0.6931471805599453f;
+        }
+      }
+      const bool whole = walk.starts && walk.ends, aborted = __any_sync(0xffffffffu, cta_aborted());
+      const int64_t slot = ((static_cast<int64_t>(walk.starts ? 2 * c + 1 : 2 * c) * p.kv_heads + h) * kBlock) + t * kRows;
+      if (hh == 0 && real && !aborted) {
+        if (walk.starts)
+          P.parts.row_info[out_row] =
+              walk.ends ? 0 : cut_info(run, c, walk.base + unit.tiles(walk.q, walk.kv, walk.block) - 1) + row;
+        if (whole)
+          p.lse[out_row] = lse;
+        else
+          P.parts.lse[slot + r] = lse;
+      }
+      // Through the query tile's shared memory (done with; 16-byte part q of row r at q ^ (r % 8)), so that a store
+      // instruction writes whole lines of a few rows. Values lie as their codes' pairs do: n, n + 4 of each eight.
+      const int first_row = (r & ~31), here = min(32, rows - (t * kRows + first_row));
+      uint8_t* stage = smem + kOffQ + t * 2 * kChunk + (warp & 7) * 4096;
+      if (here > 0 && !aborted) {
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {
+          uint32_t o[32] = {};
+          if (mine > 0) {
+            tmem_ld_32x32b_x32(ocol + g * 32, o);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+          auto y = [&](int q, int n) { return __uint_as_float(o[q * 8 + n]); };
+          if (whole) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((g * 4 + q) ^ (lane & 7)) << 4)) =
+                  make_uint4(pack2<kFp16>(y(q, 0), y(q, 2)), pack2<kFp16>(y(q, 4), y(q, 6)), pack2<kFp16>(y(q, 1), y(q, 3)),
+                             pack2<kFp16>(y(q, 5), y(q, 7)));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((2 * q) ^ (lane & 7)) << 4)) =
+                  make_uint4(o[q * 8], o[q * 8 + 2], o[q * 8 + 4], o[q * 8 + 6]);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((2 * q + 1) ^ (lane & 7)) << 4)) =
+                  make_uint4(o[q * 8 + 1], o[q * 8 + 3], o[q * 8 + 5], o[q * 8 + 7]);
+            }
+          }
+          if (whole && g == 0) continue;
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int rr = k * 4 + (lane >> 3), q = lane & 7;
+            const int64_t to = __shfl_sync(0xffffffffu, out_row, rr);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((q ^ (rr & 7)) << 4));
+            if (rr >= here) continue;
+            if (whole)
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * kHeadDim + hh * 64 + q * 8) = v;
+            else
+              *reinterpret_cast<uint4*>(P.parts.o + (slot + first_row + rr) * kHeadDim + hh * 64 + g * 32 + q * 4) = v;
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      meet_tile();  // the stage becomes the next piece's query
+    }
+  }
+  if (cta_aborted()) {
+    // loads may be in flight (at most 40 KB): they get a millisecond before the CTA leaves
+    for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000 * 1000;) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 16) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+// Runs per kv head: a CTA per SM, no more than there are steps.
+int run_count(const QuantDecodeLaunch& p) {
+  const int64_t rows = p.num_tokens * p.group, units = p.batch + rows / kBlock;
+  const int64_t steps = std::max<int64_t>(1, (static_cast<int64_t>(p.block_cols) * p.block_size + kTok - 1) / kTok);
+  const int64_t most = std::min<int64_t>(units, 1 << 20) * (kSetup + steps);
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, kNumSMs / p.kv_heads, kMaxRuns})));
+}
+
+template <bool kFp16>
+cudaError_t launch(const QuantDecodeLaunch& p, void* workspace, cudaStream_t stream) {
+  Params P;
+  P.L = p;
+  const int runs = run_count(p);
+  P.parts = quant_partials(p, runs, kBlock, workspace);
+  P.box_rows = std::min(kTok, p.block_size);
+  // no pages at all: maps over a row of the query's stand in, nothing is loaded through them
+  const bool any = p.num_blocks > 0;
+  const uint64_t extent[3] = {kQuantRow, any ? static_cast<uint64_t>(p.num_blocks) * p.block_size : 1,
+                              any ? static_cast<uint64_t>(p.kv_heads) : 1};
+  const uint64_t stride[2] = {static_cast<uint64_t>(p.kv_heads) * kQuantRow, kQuantRow};
+  const uint32_t box[3] = {kQuantRow, static_cast<uint32_t>(P.box_rows), 1};
+  if (!encode_tmap_bytes(&P.key, any ? p.key : p.query, extent, stride, box) ||
+      !encode_tmap_bytes(&P.value, any ? p.value : p.query, extent, stride, box))
+    return cudaErrorInvalidValue;
+  auto kern = quant_tiles_kernel<kFp16>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), kSmemBytes);
+  if (e != cudaSuccess) return e;
+  kern<<<static_cast<unsigned>(runs * p.kv_heads), kThreads, kSmemBytes, stream>>>(P);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || runs == 1) return e;
+  return launch_quant_combine<kFp16, kBlock>(p, P.parts, stream);
+}
+
+}  // namespace
+
+size_t quant_tiles_workspace(const QuantDecodeLaunch& p) { return quant_partial_bytes(p, run_count(p), kBlock); }
+
+cudaError_t launch_quant_tiles(const QuantDecodeLaunch& p, bool fp16, void* workspace, cudaStream_t stream) {
+  return fp16 ? launch<true>(p, workspace, stream) : launch<false>(p, workspace, stream);
+}
+
+}  // namespace cascade
