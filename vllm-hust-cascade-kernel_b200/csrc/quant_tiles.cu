@@ -13,12 +13,11 @@
 // scores' sums in fp32 are not). Queries are fp16 too, each row times a power of two. Values are
 // rounded to fp16 once.
 //
-// Warps: 0-7 softmax and output of tile A, 8-15 of tile B, 16 MMA issue, 17-19
-// unpack (17 loads, too). Per step j of 128 tokens the issue order is PV_A(j),
-// S_A(j+1), PV_B(j), S_B(j+1); the keys of step j + 1 are unpacked when both tiles'
-// scores of step j are done, the values when both tiles' outputs are, while the other
-// tile's softmax runs. P lies over its scores in tensor memory, which the two tiles'
-// scores and outputs fill (4 x 128 columns).
+// Warps: 0-7 softmax and output of tile A, 8-15 of tile B, 16 MMA issue, 17-23
+// unpack (17 loads, too). Everything but the query and the outputs has two buffers of
+// 64 tokens: while the softmax of step j runs, the scores of step j + 1 are computed
+// and the keys and values of j + 2 unpacked. P lies over its scores in tensor memory,
+// which the two tiles' scores (2 x 64 columns) and outputs (128) fill.
 //
 // A CTA takes an equal run of steps over the units (request, block) of one kv head;
 // what run boundaries cut is merged by quant_combine_kernel.
@@ -30,23 +29,26 @@
 namespace cascade {
 namespace {
 
-constexpr int kBlock = 256, kRows = 128, kTok = 128;
-constexpr int kSetup = 1;
-constexpr int kThreads = 20 * 32;
-constexpr int kUnpackWarps = 3;
+constexpr int kBlock = 256, kRows = 128, kTok = 64;
+constexpr int kSetup = 2;
+constexpr int kThreads = 24 * 32;
+constexpr int kUnpackWarps = 7;
+constexpr int kStages = 4;                       // steps loaded ahead, less one
 constexpr int kRaw = kTok * kQuantRow;           // keys or values of a step as they lie
-constexpr int kChunk = 16384;                    // 128 rows x 64 values
+constexpr int kChunk = 16384;                    // of the query: 128 rows x 64 values
+constexpr int kPart = 8192;                      // of keys or values: 64 tokens x 64 values
 constexpr int kOffQ = 0;                         // [tile][2 chunks]
-constexpr int kOffK = kOffQ + 4 * kChunk;        // [part of the scale][2 chunks]
-constexpr int kOffV = kOffK + 4 * kChunk;        // [64 tokens][64 values' group][token]
-constexpr int kOffZq = kOffV + 2 * kChunk;       // [tile][2 x 8 columns][128 rows][16 bytes]
-constexpr int kOffZk = kOffZq + 2 * 4096;
-constexpr int kOffRaw = kOffZk + 4096;           // [stage][keys, values]
-constexpr int kBytes = kOffRaw + 4 * kRaw;
+constexpr int kOffK = kOffQ + 4 * kChunk;        // [buffer][part of the scale][64 values' group][token]
+constexpr int kOffV = kOffK + 8 * kPart;         // [buffer][64 values' group][token]
+constexpr int kOffZq = kOffV + 4 * kPart;        // [tile][2 x 8 columns][128 rows][16 bytes]
+constexpr int kOffZk = kOffZq + 2 * 4096;        // [buffer][2 x 8 columns][64 tokens][16 bytes]
+constexpr int kOffRaw = kOffZk + 2 * 2048;       // [stage][keys, values]
+constexpr int kBytes = kOffRaw + kStages * 2 * kRaw;
 
 struct __align__(16) Aux {
-  float shared[2][2][kRows];  // [tile][half]: the row's maximum, at the end its sum
-  uint64_t raw_full[2], raw_empty[2], k_full, k_empty, v_full, v_empty, q_full[2], s_full[2], p_full[2], o_final[2], stall, drain;
+  float shared[2][2][2][kRows];  // [step's parity][tile][half]: the row's maximum, at the end its sum
+  uint64_t raw_full[kStages], raw_empty[kStages], k_full[2], k_empty[2], v_full[2], v_empty[2];  // per buffer
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], stall, drain;                   // per tile (and buffer)
   uint32_t tmem_base;
   QuantRun run;
 };
@@ -58,7 +60,7 @@ struct Params {
   QuantDecodeLaunch L;
   CUtensorMap key, value;  // box: 80 bytes x box_rows cache rows of one head
   QuantPartials parts;
-  int32_t box_rows;        // 16 .. 128
+  int32_t box_rows;        // 16, 32 or 64
 };
 
 using Unit = QuantUnit<kBlock, kTok>;
@@ -103,18 +105,22 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 
   if (tid == 0) {
     cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&aux->raw_full[i], 1);
       mbar_init(&aux->raw_empty[i], kUnpackWarps);
-      mbar_init(&aux->q_full[i], 8);
-      mbar_init(&aux->s_full[i], 1);
-      mbar_init(&aux->p_full[i], 8);
-      mbar_init(&aux->o_final[i], 1);
     }
-    mbar_init(&aux->k_full, kUnpackWarps);
-    mbar_init(&aux->v_full, kUnpackWarps);
-    mbar_init(&aux->k_empty, 1);
-    mbar_init(&aux->v_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&aux->k_full[i], kUnpackWarps);
+      mbar_init(&aux->v_full[i], kUnpackWarps);
+      mbar_init(&aux->k_empty[i], 1);
+      mbar_init(&aux->v_empty[i], 1);
+      mbar_init(&aux->q_full[i], 8);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&aux->s_full[i][k], 1);
+        mbar_init(&aux->pv_done[i][k], 1);
+        mbar_init(&aux->p_full[i][k], 8);
+      }
+    }
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       id = lane < boxes && at < load.kv ? p.block_table[static_cast<int64_t>(load.b) * p.block_cols + (at >> shift)] : INT32_MIN;
     };
     auto issue = [&] {
-      const int at = step * kTok + lane * P.box_rows, stage = issued & 1;
+      const int at = step * kTok + lane * P.box_rows, stage = issued % kStages;
       const bool good = static_cast<uint32_t>(id) < static_cast<uint32_t>(p.num_blocks);
       if (!good && id != INT32_MIN) atomicOr(&g_cascade_device_error, kErrBadBlockId);
       const int row = good ? id * p.block_size + (at & (p.block_size - 1)) : oob;
@@ -182,18 +188,26 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     };
     if (more) {
       next_ids();
-      for (int i = 0; i < 2 && more; ++i) issue();
+      for (int i = 0; i < kStages - 1 && more; ++i) issue();
     }
     const int t = lane & 3, g8 = (lane >> 3) + 4 * ((lane >> 2) & 1);  // rows 4 apart are 16 banks apart
     int n = 0;
     bool live = any;
     while (live && walk.next()) {
       for (int j = 0; live && j < walk.n; ++j, ++n) {
-        const uint8_t* raw = smem + kOffRaw + (n & 1) * 2 * kRaw;
-        const int tok = (walk.t0 + j) * kTok;
-        live = mbar_wait_warp(&aux->raw_full[n & 1], (n >> 1) & 1) && (n < 1 || mbar_wait_warp(&aux->k_empty, (n - 1) & 1));
+        const int stage = n % kStages, buf = n & 1, before = ((n >> 1) - 1) & 1;
+        const uint8_t* raw = smem + kOffRaw + stage * 2 * kRaw;
+        const int tok = (walk.t0 + j) * kTok, turn = (w + n) % kUnpackWarps;  // 8 tokens of keys, or values, at a time
+        if (w == 0 && more && n > 0) {  // the stage of the step before is free, or nearly
+          live = mbar_wait_warp(&aux->raw_empty[(n - 1) % kStages], ((n - 1) / kStages) & 1);
+          if (live) issue();
+        } else if (w == 0 && more) {
+          issue();
+        }
+        live = live && mbar_wait_warp(&aux->raw_full[stage], (n / kStages) & 1) &&
+               (n < 2 || mbar_wait_warp(&aux->k_empty[buf], before));
         if (!live) break;
-        for (int i = w; i < kTok / 8; i += kUnpackWarps) {
+        for (int i = turn; i < kTok / 8; i += kUnpackWarps) {
           const int r = i * 8 + g8;
           const uint4 word = *reinterpret_cast<const uint4*>(raw + r * kQuantRow + 16 * t);
           uint4 par = *reinterpret_cast<const uint4*>(raw + r * kQuantRow + kQuantCodes);
@@ -208,24 +222,24 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = as_u32(__hmul2(cd[e], s1)), y[e] = as_u32(__hmul2(cd[e], s2));
             const int q = 4 * k + t;  // eight values
-            uint8_t* dst = smem + kOffK + (q >> 3) * kChunk + r * 128 + (((q ^ r) & 7) << 4);
+            uint8_t* dst = smem + kOffK + (buf * 4 + (q >> 3)) * kPart + r * 128 + (((q ^ r) & 7) << 4);
             *reinterpret_cast<uint4*>(dst) = make_uint4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<uint4*>(dst + 2 * kChunk) = make_uint4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint4*>(dst + 2 * kPart) = make_uint4(y[0], y[1], y[2], y[3]);
           }
           if (t < 2) {
             // the columns of centres (and scales, which meet zeros). A value that is NaN makes its token's scores NaN, and
             // is 0 itself (below): rows that do not see it keep their sums.
             const uint4 pv = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + kQuantCodes);
             if (odd_par(pv.x) || odd_par(pv.y) || odd_par(pv.z) || odd_par(pv.w)) par.x = 0x7fffu;
-            *reinterpret_cast<uint4*>(smem + kOffZk + t * 2048 + r * 16) = par;
+            *reinterpret_cast<uint4*>(smem + kOffZk + buf * 2048 + t * 1024 + r * 16) = par;
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->k_full);
-        live = n < 1 || mbar_wait_warp(&aux->v_empty, (n - 1) & 1);
+        if (lane == 0) mbar_arrive(&aux->k_full[buf]);
+        live = n < 2 || mbar_wait_warp(&aux->v_empty[buf], before);
         if (!live) break;
-        for (int i = w; i < kTok / 8; i += kUnpackWarps) {
+        for (int i = kUnpackWarps - 1 - turn; i < kTok / 8; i += kUnpackWarps) {
           const int r = i * 8 + g8;
           const uint4 word = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + 16 * t);
           const uint4 par = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + kQuantCodes);
@@ -240,19 +254,15 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = as_u32(__hfma2(cd[e], s, off));
             const int q = 4 * k + t;
-            *reinterpret_cast<uint4*>(smem + kOffV + (r >> 6) * kChunk + (q >> 3) * (kChunk / 2) + (r & 63) * 128 +
-                                      (((q ^ r) & 7) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<uint4*>(smem + kOffV + (buf * 2 + (q >> 3)) * kPart + r * 128 + (((q ^ r) & 7) << 4)) =
+                make_uint4(x[0], x[1], x[2], x[3]);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&aux->v_full);
-          mbar_arrive(&aux->raw_empty[n & 1]);
-        }
-        if (w == 0 && more) {
-          live = mbar_wait_warp(&aux->raw_empty[n & 1], (n >> 1) & 1);
-          if (live) issue();
+          mbar_arrive(&aux->v_full[buf]);
+          mbar_arrive(&aux->raw_empty[stage]);
         }
       }
     }
@@ -261,83 +271,83 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     const uint32_t idesc_s = make_idesc_f16(kRows, kTok, 0u, 0, 0);
     const uint32_t idesc_pv = make_idesc_f16(kRows, kHeadDim, 0u, 0, 1);
     const uint32_t tm = uniform(tbase), s0 = uniform(smem_u32(smem));
-    auto scores = [&](int t, bool last) {
+    // counts of a tile's scores (sc) and products with values (pc): the low bit is the buffer
+    int sc[2] = {0, 0}, pc[2] = {0, 0};
+    auto scores = [&](int t, int buf, bool last) {
       const uint64_t dq = make_smem_desc(s0 + kOffQ + t * 2 * kChunk, 16, 1024, 2);
-      const uint64_t dk = make_smem_desc(s0 + kOffK, 16, 1024, 2);
-      const uint64_t zq = make_smem_desc(s0 + kOffZq + t * 4096, 2048, 128, 0), zk = make_smem_desc(s0 + kOffZk, 2048, 128, 0);
+      const uint64_t dk = make_smem_desc(s0 + kOffK + buf * 4 * kPart, 16, 1024, 2);
+      const uint64_t zq = make_smem_desc(s0 + kOffZq + t * 4096, 2048, 128, 0);
+      const uint64_t zk = make_smem_desc(s0 + kOffZk + buf * 2048, 1024, 128, 0);
+      const uint32_t b = uniform(sc[t] & 1), d = tm + t * 128 + b * 64;
       tc_fence_after();
       if (elect_one()) {
-        umma_f16_ss(tm + t * 128, zq, zk, idesc_s, 0);
+        umma_f16_ss(d, zq, zk, idesc_s, 0);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
 #pragma unroll
           for (int ch = 0; ch < 2; ++ch) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_f16_ss(tm + t * 128, dq + (ch * kChunk + k * 32) / 16, dk + ((part * 2 + ch) * kChunk + k * 32) / 16, idesc_s, 1);
+              umma_f16_ss(d, dq + (ch * kChunk + k * 32) / 16, dk + ((part * 2 + ch) * kPart + k * 32) / 16, idesc_s, 1);
           }
         }
-        umma_commit(&aux->s_full[t]);
-        if (last) umma_commit(&aux->k_empty);
+        umma_commit(&aux->s_full[t][b]);
+        if (last) umma_commit(&aux->k_empty[buf]);
       }
       __syncwarp();
+      ++sc[t];
     };
-    auto values = [&](int t, bool fresh, bool last, bool final) {
+    auto values = [&](int t, int buf, bool fresh, bool last) {
+      const uint32_t a = tm + t * 128 + uniform(pc[t] & 1) * 64;
       tc_fence_after();
       if (elect_one()) {
+        // 64 tokens x two groups of 64 values, 8 KB apart
+        const uint64_t dv = make_smem_desc(s0 + kOffV + buf * 2 * kPart, kPart, 1024, 2);
 #pragma unroll
-        for (int ch = 0; ch < 2; ++ch) {
-          // 64 tokens x two groups of 64 values, 8 KB apart
-          const uint64_t dv = make_smem_desc(s0 + kOffV + ch * kChunk, kChunk / 2, 1024, 2);
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16_ts(tm + 256 + t * 128, tm + t * 128 + ch * 64 + k * 8, dv + k * 128, idesc_pv, !fresh || ch + k > 0);
-        }
-        if (last) umma_commit(&aux->v_empty);
-        if (final) umma_commit(&aux->o_final[t]);
+        for (int k = 0; k < 4; ++k) umma_f16_ts(tm + 256 + t * 128, a + k * 8, dv + k * 128, idesc_pv, !fresh || k > 0);
+        umma_commit(&aux->pv_done[t][pc[t] & 1]);
+        if (last) umma_commit(&aux->v_empty[buf]);
       }
       __syncwarp();
+      ++pc[t];
     };
-    int n = 0, sc[2] = {0, 0}, pieces[2] = {0, 0};  // steps, scores and pieces so far
+    int n = 0, pieces[2] = {0, 0};  // steps and pieces so far
     bool live = any, used = false;
     while (live && walk.next()) {
       const int nt[2] = {tile_steps(unit, walk, 0), tile_steps(unit, walk, 1)};
-      // (the last tile with rows has all the piece's steps; a unit whose rows see nothing has a step all the same: its
-      // products go unread)
+      // (the last tile with rows has all the piece's steps, but for a unit whose rows see nothing: it has a step all the
+      // same, without products)
       const int tl = nt[1] > 0 ? 1 : 0;
-      if (nt[0] == 0 && nt[1] == 0) {
-        live = mbar_wait_warp(&aux->k_full, n & 1) && mbar_wait_warp(&aux->v_full, n & 1);
-        if (live && elect_one()) {
-          umma_commit(&aux->k_empty);
-          umma_commit(&aux->v_empty);
-        }
-        __syncwarp();
-        used = true;
-        ++n;
-        continue;
-      }
-      for (int t = 0; live && t < 2; ++t)
-        if (nt[t] > 0) live = mbar_wait_warp(&aux->q_full[t], pieces[t]++ & 1);
-      live = live && mbar_wait_warp(&aux->k_full, n & 1);
-      if (!live) break;
       used = true;
+#pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (nt[t] > 0) scores(t, t == tl);
-      for (int j = 0; live && j < walk.n; ++j, ++n) {
-        live = mbar_wait_warp(&aux->v_full, n & 1);
-        bool have_k = false;
-        for (int t = 0; live && t < 2; ++t) {
-          if (j >= nt[t]) continue;
-          live = mbar_wait_warp(&aux->p_full[t], sc[t]++ & 1);
-          if (!live) break;
-          values(t, j == 0, t == tl, j + 1 == nt[t]);
-          if (j + 1 < nt[t]) {
-            live = have_k || mbar_wait_warp(&aux->k_full, (n + 1) & 1);
-            have_k = true;
-            if (live) scores(t, t == tl);
-          }
+        if (live && nt[t] > 0) live = mbar_wait_warp(&aux->q_full[t], pieces[t]++ & 1);
+      auto step_scores = [&](int j) {
+        const int buf = uniform((n + j) & 1);
+        if (live) live = mbar_wait_warp(&aux->k_full[buf], ((n + j) >> 1) & 1);
+        if (!live) return;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (j < nt[t]) scores(t, buf, t == tl);
+        if (nt[0] + nt[1] == 0 && elect_one()) umma_commit(&aux->k_empty[buf]);
+        __syncwarp();
+      };
+      step_scores(0);
+      for (int j = 0; live && j < walk.n; ++j) {
+        // (into the buffers of step j - 1, whose products with values are issued)
+        if (j + 1 < walk.n) step_scores(j + 1);
+        const int buf = uniform((n + j) & 1);
+        live = live && mbar_wait_warp(&aux->v_full[buf], ((n + j) >> 1) & 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (!live || j >= nt[t]) continue;
+          live = mbar_wait_warp(&aux->p_full[t][pc[t] & 1], (pc[t] >> 1) & 1);
+          if (live) values(t, buf, j == 0, t == tl);
         }
+        if (live && nt[0] + nt[1] == 0 && elect_one()) umma_commit(&aux->v_empty[buf]);
+        __syncwarp();
       }
+      n += walk.n;
     }
     if (used && !live && lane == 0) {
       umma_commit(&aux->drain);
@@ -347,13 +357,13 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     // ------------------------------------------------- softmax, output of tile t
     const int t = warp >> 3, hh = (warp >> 2) & 1, r = tid & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t scol = tbase + lane_off + t * 128, ocol = tbase + lane_off + 256 + t * 128 + hh * 64;
+    const uint32_t sbase = tbase + lane_off + t * 128, ocol = tbase + lane_off + 256 + t * 128 + hh * 64;
     // the two warps of 32 rows meet here, and the eight of a tile; none leaves its loop early (an aborted CTA's waits
     // return at once), so none is waited for in vain
     auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
     auto meet_tile = [&] { asm volatile("bar.sync %0, 256;" ::"r"(9 + t) : "memory"); };
     if (p.debug_stall && any) mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
-    int sc = 0, pieces = 0;
+    int sc = 0;  // steps of this tile so far: the low bit is the buffer
     while (any && walk.next()) {
       const int rows = min(kBlock, walk.q * p.group - walk.block * kBlock);  // of the block
       const int row = t * kRows + r, at = walk.block * kBlock + row, i = at / p.group;
@@ -378,9 +388,9 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
           for (int e = 0; e < 8; e += 2) top = fmax3f_nan(top, fabsf(value(k, e)), fabsf(value(k, e + 1)));
         }
-        aux->shared[t][hh][r] = top;
+        aux->shared[0][t][hh][r] = top;
         meet();
-        top = fmax3f_nan(top, aux->shared[t][hh ^ 1][r], top);
+        top = fmax3f_nan(top, aux->shared[0][t][hh ^ 1][r], top);
         // times 2^up: [2^8, 2^9), or less for rows below 2^-119. A row with a NaN or an infinity is NaN.
         const int ex = max((__float_as_int(top) >> 23) & 255, 8), up = 135 - ex;
         const float f = ex == 255 ? __int_as_float(0x7fffffff) : __int_as_float((127 + up) << 23);
@@ -410,85 +420,76 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       // steps below are seen in full by every row of the tile
       const int clean = min(walk.kv, unit.limit(walk.q, walk.kv, (walk.block * kBlock + t * kRows) / p.group)) / kTok - walk.t0;
       for (int j = 0; j < mine; ++j, ++sc) {
-        mbar_wait_warp(&aux->s_full[t], sc & 1);
+        // (each phase of pv_done is waited for, so that none is taken for the one after the next)
+        if (sc > 1) mbar_wait_warp(&aux->pv_done[t][sc & 1], ((sc >> 1) - 1) & 1);
+        mbar_wait_warp(&aux->s_full[t][sc & 1], (sc >> 1) & 1);
         tc_fence_after();
-        const int seen = j >= clean ? lim - j * kTok - hh * 64 : 64;
-        auto load = [&](int g, uint32_t (&x)[32]) {
-          tmem_ld_32x32b_x32(scol + hh * 64 + g * 32, x);
-          tmem_wait_ld();
-          if (j >= clean) {
+        const uint32_t scol = sbase + (sc & 1) * 64;
+        uint32_t x[32];
+        tmem_ld_32x32b_x32(scol + hh * 32, x);
+        tmem_wait_ld();
+        if (j >= clean) {
+          const int seen = lim - j * kTok - hh * 32;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = g * 32 + e < seen ? x[e] : 0xff800000u;
-          }
-        };
-        float a0 = -INFINITY, a1 = -INFINITY, a2 = -INFINITY, a3 = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t x[32];
-          load(g, x);
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            a0 = fmax3f_nan(a0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-            a1 = fmax3f_nan(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-            a2 = fmax3f_nan(a2, __uint_as_float(x[e + 4]), __uint_as_float(x[e + 5]));
-            a3 = fmax3f_nan(a3, __uint_as_float(x[e + 6]), __uint_as_float(x[e + 7]));
-          }
+          for (int e = 0; e < 32; ++e) x[e] = e < seen ? x[e] : 0xff800000u;
         }
-        a0 = fmax3f_nan(fmax3f_nan(a0, a1, a2), a3, a3);
-        aux->shared[t][hh][r] = a0;
-        meet();
-        const float top = fmax3f_nan(a0, aux->shared[t][hh ^ 1][r], a0) * mult;
+        float a0 = -INFINITY, a1 = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          a0 = fmax3f_nan(a0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          a1 = fmax3f_nan(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+        }
+        a0 = fmax3f_nan(a0, a1, a1);
+        aux->shared[sc & 1][t][hh][r] = a0;
+        meet();  // (both halves have their scores in registers: P goes over the first 32 columns)
+        const float top = fmax3f_nan(a0, aux->shared[sc & 1][t][hh ^ 1][r], a0) * mult;
         // weights up to 2^6 after a move, to 2^14 before the next: fp16 holds 2^-24 of them
         const bool move = top > mx + 14.f;
         const float dm = move ? ex2(mx - (top - 6.f)) : 1.f;  // 0 while nothing has been seen
         if (move) mx = top - 6.f;
         const float neg = mx == -INFINITY ? 0.f : -mx;
         if (j > 0 && __any_sync(0xffffffffu, move)) {
-          // the scores of step j come after P V of step j - 1: the output is at rest
+          mbar_wait_warp(&aux->pv_done[t][(sc - 1) & 1], ((sc - 1) >> 1) & 1);
+          tc_fence_after();
 #pragma unroll 1
-          for (int g = 0; g < 2; ++g) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(ocol + g * 32, o);
+          for (int g = 0; g < 4; ++g) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(ocol + g * 16, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * dm);
-            tmem_st_32x32b_x32(ocol + g * 32, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * dm);
+            tmem_st_32x32b_x16(ocol + g * 16, o);
           }
         }
-        // P goes over the first 32 columns of this half's own scores, read by then
         float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f;
+        uint32_t pk[16];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint32_t x[32], pk[16];
-          load(g, x);
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float y0, y1, y2, y3;
-            ffma2_bcast(y0, y1, __uint_as_float(x[e]), __uint_as_float(x[e + 1]), mult, neg);
-            ffma2_bcast(y2, y3, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]), mult, neg);
-            y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
-            fadd2(r0, r1, y0, y1);
-            fadd2(r2, r3, y2, y3);
-            pk[e >> 1] = pack2<true>(y0, y1);
-            pk[(e >> 1) + 1] = pack2<true>(y2, y3);
-          }
-          tmem_st_32x32b_x16(scol + hh * 64 + g * 16, pk);
+        for (int e = 0; e < 32; e += 4) {
+          float y0, y1, y2, y3;
+          ffma2_bcast(y0, y1, __uint_as_float(x[e]), __uint_as_float(x[e + 1]), mult, neg);
+          ffma2_bcast(y2, y3, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]), mult, neg);
+          y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
+          fadd2(r0, r1, y0, y1);
+          fadd2(r2, r3, y2, y3);
+          pk[e >> 1] = pack2<true>(y0, y1);
+          pk[(e >> 1) + 1] = pack2<true>(y2, y3);
         }
+        tmem_st_32x32b_x16(scol + hh * 16, pk);
         l = l * dm + ((r0 + r1) + (r2 + r3));
         if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->p_full[t]);
+        if (lane == 0) mbar_arrive(&aux->p_full[t][sc & 1]);
       }
       // ----------------------------------------------------------- output
       float inv = 0.f, lse = -INFINITY;
       if (mine > 0) {
-        mbar_wait_warp(&aux->o_final[t], pieces++ & 1);  // both warps have read the maxima: the slots take the sums
+        mbar_wait_warp(&aux->pv_done[t][(sc - 1) & 1], ((sc - 1) >> 1) & 1);  // both warps have read the maxima: the slots take the sums
         tc_fence_after();
-        aux->shared[t][hh][r] = l;
+        aux->shared[0][t][hh][r] = l;
         meet();
-        l = aux->shared[t][0][r] + aux->shared[t][1][r];
+        l = aux->shared[0][t][0][r] + aux->shared[0][t][1][r];
         if (mx > -INFINITY || l != l) {  // (a NaN is no maximum)
           inv = 1.f / l;
           lse = (mx + __log2f(l)) * 0.6931471805599453f;
