@@ -14,10 +14,11 @@
 // rounded to fp16 once.
 //
 // Warps: 0-7 softmax and output of tile A, 8-15 of tile B, 16 MMA issue, 17-23
-// unpack (17 loads, too). Everything but the query and the outputs has two buffers of
-// 64 tokens: while the softmax of step j runs, the scores of step j + 1 are computed
-// and the keys and values of j + 2 unpacked. P lies over its scores in tensor memory,
-// which the two tiles' scores (2 x 64 columns) and outputs (128) fill.
+// unpack (17 loads, too). Per step j of 64 tokens the issue order is PV_A(j),
+// S_A(j+1), PV_B(j), S_B(j+1), so one tile's products run beside the other's softmax;
+// unpacked keys and values have two buffers. Tensor memory holds both tiles' queries
+// (64 columns each; from shared memory a product with 64 tokens would wait for its
+// 128 query rows, 49 cycles for 32), scores (64, P over them) and outputs (128).
 //
 // A CTA takes an equal run of steps over the units (request, block) of one kv head;
 // what run boundaries cut is merged by quant_combine_kernel.
@@ -35,10 +36,10 @@ constexpr int kThreads = 24 * 32;
 constexpr int kUnpackWarps = 7;
 constexpr int kStages = 4;                       // steps loaded ahead, less one
 constexpr int kRaw = kTok * kQuantRow;           // keys or values of a step as they lie
-constexpr int kChunk = 16384;                    // of the query: 128 rows x 64 values
+constexpr int kStageOut = 32768;                 // a tile's output on its way
 constexpr int kPart = 8192;                      // of keys or values: 64 tokens x 64 values
-constexpr int kOffQ = 0;                         // [tile][2 chunks]
-constexpr int kOffK = kOffQ + 4 * kChunk;        // [buffer][part of the scale][64 values' group][token]
+constexpr int kOffOut = 0;                       // [tile]
+constexpr int kOffK = kOffOut + 2 * kStageOut;   // [buffer][part of the scale][64 values' group][token]
 constexpr int kOffV = kOffK + 8 * kPart;         // [buffer][64 values' group][token]
 constexpr int kOffZq = kOffV + 4 * kPart;        // [tile][2 x 8 columns][128 rows][16 bytes]
 constexpr int kOffZk = kOffZq + 2 * 4096;        // [buffer][2 x 8 columns][64 tokens][16 bytes]
@@ -46,9 +47,9 @@ constexpr int kOffRaw = kOffZk + 2 * 2048;       // [stage][keys, values]
 constexpr int kBytes = kOffRaw + kStages * 2 * kRaw;
 
 struct __align__(16) Aux {
-  float shared[2][2][2][kRows];  // [step's parity][tile][half]: the row's maximum, at the end its sum
+  float shared[2][2][kRows];  // [tile][half]: the row's maximum, at the end its sum
   uint64_t raw_full[kStages], raw_empty[kStages], k_full[2], k_empty[2], v_full[2], v_empty[2];  // per buffer
-  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], stall, drain;                   // per tile (and buffer)
+  uint64_t q_full[2], s_full[2], p_full[2], o_final[2], stall, drain;                                      // per tile
   uint32_t tmem_base;
   QuantRun run;
 };
@@ -115,11 +116,9 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       mbar_init(&aux->k_empty[i], 1);
       mbar_init(&aux->v_empty[i], 1);
       mbar_init(&aux->q_full[i], 8);
-      for (int k = 0; k < 2; ++k) {
-        mbar_init(&aux->s_full[i][k], 1);
-        mbar_init(&aux->pv_done[i][k], 1);
-        mbar_init(&aux->p_full[i][k], 8);
-      }
+      mbar_init(&aux->s_full[i], 1);
+      mbar_init(&aux->p_full[i], 8);
+      mbar_init(&aux->o_final[i], 1);
     }
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
@@ -271,47 +270,37 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     const uint32_t idesc_s = make_idesc_f16(kRows, kTok, 0u, 0, 0);
     const uint32_t idesc_pv = make_idesc_f16(kRows, kHeadDim, 0u, 0, 1);
     const uint32_t tm = uniform(tbase), s0 = uniform(smem_u32(smem));
-    // counts of a tile's scores (sc) and products with values (pc): the low bit is the buffer
-    int sc[2] = {0, 0}, pc[2] = {0, 0};
     auto scores = [&](int t, int buf, bool last) {
-      const uint64_t dq = make_smem_desc(s0 + kOffQ + t * 2 * kChunk, 16, 1024, 2);
       const uint64_t dk = make_smem_desc(s0 + kOffK + buf * 4 * kPart, 16, 1024, 2);
       const uint64_t zq = make_smem_desc(s0 + kOffZq + t * 4096, 2048, 128, 0);
       const uint64_t zk = make_smem_desc(s0 + kOffZk + buf * 2048, 1024, 128, 0);
-      const uint32_t b = uniform(sc[t] & 1), d = tm + t * 128 + b * 64;
       tc_fence_after();
       if (elect_one()) {
-        umma_f16_ss(d, zq, zk, idesc_s, 0);
+        umma_f16_ss(tm + t * 64, zq, zk, idesc_s, 0);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
 #pragma unroll
-          for (int ch = 0; ch < 2; ++ch) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_f16_ss(d, dq + (ch * kChunk + k * 32) / 16, dk + ((part * 2 + ch) * kPart + k * 32) / 16, idesc_s, 1);
-          }
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ts(tm + t * 64, tm + 128 + t * 64 + k * 8, dk + ((part * 2 + k / 4) * kPart + k % 4 * 32) / 16, idesc_s, 1);
         }
-        umma_commit(&aux->s_full[t][b]);
+        umma_commit(&aux->s_full[t]);
         if (last) umma_commit(&aux->k_empty[buf]);
       }
       __syncwarp();
-      ++sc[t];
     };
-    auto values = [&](int t, int buf, bool fresh, bool last) {
-      const uint32_t a = tm + t * 128 + uniform(pc[t] & 1) * 64;
+    auto values = [&](int t, int buf, bool fresh, bool last, bool final) {
       tc_fence_after();
       if (elect_one()) {
         // 64 tokens x two groups of 64 values, 8 KB apart
         const uint64_t dv = make_smem_desc(s0 + kOffV + buf * 2 * kPart, kPart, 1024, 2);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_f16_ts(tm + 256 + t * 128, a + k * 8, dv + k * 128, idesc_pv, !fresh || k > 0);
-        umma_commit(&aux->pv_done[t][pc[t] & 1]);
+        for (int k = 0; k < 4; ++k) umma_f16_ts(tm + 256 + t * 128, tm + t * 64 + k * 8, dv + k * 128, idesc_pv, !fresh || k > 0);
         if (last) umma_commit(&aux->v_empty[buf]);
+        if (final) umma_commit(&aux->o_final[t]);
       }
       __syncwarp();
-      ++pc[t];
     };
-    int n = 0, pieces[2] = {0, 0};  // steps and pieces so far
+    int n = 0, sc[2] = {0, 0}, pieces[2] = {0, 0};  // steps, and a tile's steps and pieces, so far
     bool live = any, used = false;
     while (live && walk.next()) {
       const int nt[2] = {tile_steps(unit, walk, 0), tile_steps(unit, walk, 1)};
@@ -322,32 +311,37 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         if (live && nt[t] > 0) live = mbar_wait_warp(&aux->q_full[t], pieces[t]++ & 1);
-      auto step_scores = [&](int j) {
-        const int buf = uniform((n + j) & 1);
-        if (live) live = mbar_wait_warp(&aux->k_full[buf], ((n + j) >> 1) & 1);
-        if (!live) return;
+      live = live && mbar_wait_warp(&aux->k_full[n & 1], (n >> 1) & 1);
+      if (!live) break;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (j < nt[t]) scores(t, buf, t == tl);
-        if (nt[0] + nt[1] == 0 && elect_one()) umma_commit(&aux->k_empty[buf]);
+      for (int t = 0; t < 2; ++t)
+        if (nt[t] > 0) scores(t, uniform(n & 1), t == tl);
+      if (nt[tl] == 0) {
+        live = mbar_wait_warp(&aux->v_full[n & 1], (n >> 1) & 1);
+        if (live && elect_one()) {
+          umma_commit(&aux->k_empty[n & 1]);
+          umma_commit(&aux->v_empty[n & 1]);
+        }
         __syncwarp();
-      };
-      step_scores(0);
-      for (int j = 0; live && j < walk.n; ++j) {
-        // (into the buffers of step j - 1, whose products with values are issued)
-        if (j + 1 < walk.n) step_scores(j + 1);
-        const int buf = uniform((n + j) & 1);
-        live = live && mbar_wait_warp(&aux->v_full[buf], ((n + j) >> 1) & 1);
+        ++n;
+        continue;
+      }
+      for (int j = 0; live && j < walk.n; ++j, ++n) {
+        const int buf = uniform(n & 1);
+        live = mbar_wait_warp(&aux->v_full[buf], (n >> 1) & 1);
+        bool have_k = false;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (!live || j >= nt[t]) continue;
-          live = mbar_wait_warp(&aux->p_full[t][pc[t] & 1], (pc[t] >> 1) & 1);
-          if (live) values(t, buf, j == 0, t == tl);
+          live = mbar_wait_warp(&aux->p_full[t], sc[t]++ & 1);
+          if (live) values(t, buf, j == 0, t == tl, j + 1 == nt[t]);
+          if (live && j + 1 < nt[t]) {
+            live = have_k || mbar_wait_warp(&aux->k_full[buf ^ 1], ((n + 1) >> 1) & 1);
+            have_k = true;
+            if (live) scores(t, buf ^ 1, t == tl);
+          }
         }
-        if (live && nt[0] + nt[1] == 0 && elect_one()) umma_commit(&aux->v_empty[buf]);
-        __syncwarp();
       }
-      n += walk.n;
     }
     if (used && !live && lane == 0) {
       umma_commit(&aux->drain);
@@ -357,13 +351,13 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     // ------------------------------------------------- softmax, output of tile t
     const int t = warp >> 3, hh = (warp >> 2) & 1, r = tid & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t sbase = tbase + lane_off + t * 128, ocol = tbase + lane_off + 256 + t * 128 + hh * 64;
+    const uint32_t scol = tbase + lane_off + t * 64, qcol = tbase + lane_off + 128 + t * 64, ocol = tbase + lane_off + 256 + t * 128 + hh * 64;
     // the two warps of 32 rows meet here, and the eight of a tile; none leaves its loop early (an aborted CTA's waits
     // return at once), so none is waited for in vain
     auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
     auto meet_tile = [&] { asm volatile("bar.sync %0, 256;" ::"r"(9 + t) : "memory"); };
     if (p.debug_stall && any) mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
-    int sc = 0;  // steps of this tile so far: the low bit is the buffer
+    int sc = 0, pieces = 0;  // steps and pieces of this tile so far
     while (any && walk.next()) {
       const int rows = min(kBlock, walk.q * p.group - walk.block * kBlock);  // of the block
       const int row = t * kRows + r, at = walk.block * kBlock + row, i = at / p.group;
@@ -388,22 +382,24 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
           for (int e = 0; e < 8; e += 2) top = fmax3f_nan(top, fabsf(value(k, e)), fabsf(value(k, e + 1)));
         }
-        aux->shared[0][t][hh][r] = top;
+        aux->shared[t][hh][r] = top;
         meet();
-        top = fmax3f_nan(top, aux->shared[0][t][hh ^ 1][r], top);
+        top = fmax3f_nan(top, aux->shared[t][hh ^ 1][r], top);
         // times 2^up: [2^8, 2^9), or less for rows below 2^-119. A row with a NaN or an infinity is NaN.
         const int ex = max((__float_as_int(top) >> 23) & 255, 8), up = 135 - ex;
         const float f = ex == 255 ? __int_as_float(0x7fffffff) : __int_as_float((127 + up) << 23);
         float sums[2] = {0.f, 0.f};
+        uint32_t qw[32];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           float y[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] = value(k, e) * f;
           sums[k >> 2] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-          *reinterpret_cast<uint4*>(smem + kOffQ + (t * 2 + hh) * kChunk + r * 128 + (((k ^ r) & 7) << 4)) =
-              make_uint4(pack2<true>(y[0], y[4]), pack2<true>(y[1], y[5]), pack2<true>(y[2], y[6]), pack2<true>(y[3], y[7]));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qw[k * 4 + e] = pack2<true>(y[e], y[e + 4]);
         }
+        tmem_st_32x32b_x32(qcol + hh * 32, qw);
         const uint32_t z0 = pack2<true>(sums[0], 0.f), z1 = pack2<true>(sums[1], 0.f);
         uint8_t* z = smem + kOffZq + t * 4096 + r * 16 + hh * 8;
         *reinterpret_cast<uint2*>(z) = make_uint2(z0, z1);
@@ -412,6 +408,8 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         // (not 0, nor NaN: a masked score, -inf, stays -inf)
         mult = fmaxf(__int_as_float((127 - up) << 23) * (p.scale * 1.4426950408889634f), 1e-37f);
         fence_proxy_async_smem();
+        tmem_wait_st();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&aux->q_full[t]);
       }
@@ -420,11 +418,8 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       // steps below are seen in full by every row of the tile
       const int clean = min(walk.kv, unit.limit(walk.q, walk.kv, (walk.block * kBlock + t * kRows) / p.group)) / kTok - walk.t0;
       for (int j = 0; j < mine; ++j, ++sc) {
-        // (each phase of pv_done is waited for, so that none is taken for the one after the next)
-        if (sc > 1) mbar_wait_warp(&aux->pv_done[t][sc & 1], ((sc >> 1) - 1) & 1);
-        mbar_wait_warp(&aux->s_full[t][sc & 1], (sc >> 1) & 1);
+        mbar_wait_warp(&aux->s_full[t], sc & 1);
         tc_fence_after();
-        const uint32_t scol = sbase + (sc & 1) * 64;
         uint32_t x[32];
         tmem_ld_32x32b_x32(scol + hh * 32, x);
         tmem_wait_ld();
@@ -440,17 +435,16 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
           a1 = fmax3f_nan(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
         }
         a0 = fmax3f_nan(a0, a1, a1);
-        aux->shared[sc & 1][t][hh][r] = a0;
+        aux->shared[t][hh][r] = a0;
         meet();  // (both halves have their scores in registers: P goes over the first 32 columns)
-        const float top = fmax3f_nan(a0, aux->shared[sc & 1][t][hh ^ 1][r], a0) * mult;
+        const float top = fmax3f_nan(a0, aux->shared[t][hh ^ 1][r], a0) * mult;
         // weights up to 2^6 after a move, to 2^14 before the next: fp16 holds 2^-24 of them
         const bool move = top > mx + 14.f;
         const float dm = move ? ex2(mx - (top - 6.f)) : 1.f;  // 0 while nothing has been seen
         if (move) mx = top - 6.f;
         const float neg = mx == -INFINITY ? 0.f : -mx;
         if (j > 0 && __any_sync(0xffffffffu, move)) {
-          mbar_wait_warp(&aux->pv_done[t][(sc - 1) & 1], ((sc - 1) >> 1) & 1);
-          tc_fence_after();
+          // the scores of step j come after P V of step j - 1: the output is at rest
 #pragma unroll 1
           for (int g = 0; g < 4; ++g) {
             uint32_t o[16];
@@ -480,16 +474,16 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&aux->p_full[t][sc & 1]);
+        if (lane == 0) mbar_arrive(&aux->p_full[t]);
       }
       // ----------------------------------------------------------- output
       float inv = 0.f, lse = -INFINITY;
       if (mine > 0) {
-        mbar_wait_warp(&aux->pv_done[t][(sc - 1) & 1], ((sc - 1) >> 1) & 1);  // both warps have read the maxima: the slots take the sums
+        mbar_wait_warp(&aux->o_final[t], pieces++ & 1);  // both warps have read the maxima: the slots take the sums
         tc_fence_after();
-        aux->shared[0][t][hh][r] = l;
+        aux->shared[t][hh][r] = l;
         meet();
-        l = aux->shared[0][t][0][r] + aux->shared[0][t][1][r];
+        l = aux->shared[t][0][r] + aux->shared[t][1][r];
         if (mx > -INFINITY || l != l) {  // (a NaN is no maximum)
           inv = 1.f / l;
           lse = (mx + __log2f(l)) * 0.6931471805599453f;
@@ -506,10 +500,10 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         else
           P.parts.lse[slot + r] = lse;
       }
-      // Through the query tile's shared memory (done with; 16-byte part q of row r at q ^ (r % 8)), so that a store
+      // Through shared memory (16-byte part q of row r at q ^ (r % 8)), so that a store
       // instruction writes whole lines of a few rows. Values lie as their codes' pairs do: n, n + 4 of each eight.
       const int first_row = (r & ~31), here = min(32, rows - (t * kRows + first_row));
-      uint8_t* stage = smem + kOffQ + t * 2 * kChunk + (warp & 7) * 4096;
+      uint8_t* stage = smem + kOffOut + t * kStageOut + (warp & 7) * 4096;
       if (here > 0 && !aborted) {
 #pragma unroll 1
         for (int g = 0; g < 2; ++g) {
@@ -553,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         }
       }
       tc_fence_before();
-      meet_tile();  // the stage becomes the next piece's query
+      meet_tile();  // (the maxima's places are the next piece's from here on)
     }
   }
   if (cta_aborted()) {
