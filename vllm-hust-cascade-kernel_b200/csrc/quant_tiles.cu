@@ -13,8 +13,8 @@
 // scores' sums in fp32 are not). Queries are fp16 too, each row times a power of two. Values are
 // rounded to fp16 once.
 //
-// Warps: 0-7 softmax and output of tile A, 8-15 of tile B, 16 MMA issue, 17-23
-// unpack (17 loads, too). Per step j of 64 tokens the issue order is PV_A(j),
+// Warps: 0-3 softmax and output of tile A, a thread per row, 4-7 of tile B, 8 MMA
+// issue, 9-15 unpack (9 loads, too). Per step j of 64 tokens the issue order is PV_A(j),
 // S_A(j+1), PV_B(j), S_B(j+1), so one tile's products run beside the other's softmax;
 // unpacked keys and values have two buffers. Tensor memory holds both tiles' queries
 // (64 columns each; from shared memory a product with 64 tokens would wait for its
@@ -32,7 +32,7 @@ namespace {
 
 constexpr int kBlock = 256, kRows = 128, kTok = 64;
 constexpr int kSetup = 2;
-constexpr int kThreads = 24 * 32;
+constexpr int kThreads = 16 * 32;
 constexpr int kUnpackWarps = 7;
 constexpr int kStages = 4;                       // steps loaded ahead, less one
 constexpr int kRaw = kTok * kQuantRow;           // keys or values of a step as they lie
@@ -47,7 +47,6 @@ constexpr int kOffRaw = kOffZk + 2 * 2048;       // [stage][keys, values]
 constexpr int kBytes = kOffRaw + kStages * 2 * kRaw;
 
 struct __align__(16) Aux {
-  float shared[2][2][kRows];  // [tile][half]: the row's maximum, at the end its sum
   uint64_t raw_full[kStages], raw_empty[kStages], k_full[2], k_empty[2], v_full[2], v_empty[2];  // per buffer
   uint64_t q_full[2], s_full[2], p_full[2], o_final[2], stall, drain;                                      // per tile
   uint32_t tmem_base;
@@ -115,9 +114,9 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       mbar_init(&aux->v_full[i], kUnpackWarps);
       mbar_init(&aux->k_empty[i], 1);
       mbar_init(&aux->v_empty[i], 1);
-      mbar_init(&aux->q_full[i], 8);
+      mbar_init(&aux->q_full[i], 4);
       mbar_init(&aux->s_full[i], 1);
-      mbar_init(&aux->p_full[i], 8);
+      mbar_init(&aux->p_full[i], 4);
       mbar_init(&aux->o_final[i], 1);
     }
     mbar_init(&aux->stall, 1);
@@ -126,15 +125,15 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     tma_prefetch_desc(&P.key);
     tma_prefetch_desc(&P.value);
   }
-  if (warp == 16) {
+  if (warp == 8) {
     tmem_alloc(&aux->tmem_base, 512);
     tmem_relinquish();
   }
-  if (warp == 17) {
+  if (warp == 9) {
     const QuantRun r = find_run<kBlock, kTok, kSetup>(unit, c, P.parts.runs);
     if (lane == 0) aux->run = r;
   }
-  if (warp == 18 && p.q_len == 0) {  // rows of tokens that are no request's: nothing to merge
+  if (warp == 10 && p.q_len == 0) {  // rows of tokens that are no request's: nothing to merge
     int64_t own = 0;
     for (int b = lane; b < p.batch; b += 32) own += min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens);
 #pragma unroll
@@ -151,15 +150,15 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
   const bool any = c < run.runs;
   Walk walk(p, run);
 
-  if (warp >= 17) {
+  if (warp >= 9) {
     // ------------------------------------------------------------- unpack
-    const int w = warp - 17;
+    const int w = warp - 9;
     Walk load(p, run);
     const int shift = __ffs(p.block_size) - 1, oob = p.num_blocks ? p.num_blocks * p.block_size : 1, boxes = kTok / P.box_rows;
     int left = 0, step = 0, issued = 0;
     int32_t id = 0;
     bool more = any && w == 0;
-    // (warp 17) page id of this lane's box of the next step, as loaded: not used, and so not waited for, until then
+    // (warp 9) page id of this lane's box of the next step, as loaded: not used, and so not waited for, until then
     auto next_ids = [&] {
       if (left == 0) {
         more = more && load.next();
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         }
       }
     }
-  } else if (warp == 16) {
+  } else if (warp == 8) {
     // ----------------------------------------------------------- MMA issuer
     const uint32_t idesc_s = make_idesc_f16(kRows, kTok, 0u, 0, 0);
     const uint32_t idesc_pv = make_idesc_f16(kRows, kHeadDim, 0u, 0, 1);
@@ -349,13 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     }
   } else {
     // ------------------------------------------------- softmax, output of tile t
-    const int t = warp >> 3, hh = (warp >> 2) & 1, r = tid & 127;
+    const int t = warp >> 2, r = tid & 127;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t scol = tbase + lane_off + t * 64, qcol = tbase + lane_off + 128 + t * 64, ocol = tbase + lane_off + 256 + t * 128 + hh * 64;
-    // the two warps of 32 rows meet here, and the eight of a tile; none leaves its loop early (an aborted CTA's waits
-    // return at once), so none is waited for in vain
-    auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
-    auto meet_tile = [&] { asm volatile("bar.sync %0, 256;" ::"r"(9 + t) : "memory"); };
+    const uint32_t scol = tbase + lane_off + t * 64, qcol = tbase + lane_off + 128 + t * 64, ocol = tbase + lane_off + 256 + t * 128;
     if (p.debug_stall && any) mbar_wait_warp(&aux->stall, 0);  // test hook: runs into the wait limit
     int sc = 0, pieces = 0;  // steps and pieces of this tile so far
     while (any && walk.next()) {
@@ -367,10 +362,10 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       float mult = 0.f, mx = -INFINITY, l = 0.f;
       if (mine > 0) {
         // ------------------------------------------------------------ query
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) + out_row * kHeadDim + hh * 64);
-        uint4 v[8];
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) + out_row * kHeadDim);
+        uint4 v[16];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = real ? __ldg(src + k) : make_uint4(0u, 0u, 0u, 0u);
+        for (int k = 0; k < 16; ++k) v[k] = real ? __ldg(src + k) : make_uint4(0u, 0u, 0u, 0u);
         auto value = [&](int k, int e) {
           const uint32_t w = e < 2 ? v[k].x : e < 4 ? v[k].y : e < 6 ? v[k].z : v[k].w;
           if constexpr (kFp16) return e & 1 ? __high2float(as_half2(w)) : __low2float(as_half2(w));
@@ -378,33 +373,33 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         };
         float top = 0.f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < 16; ++k) {
 #pragma unroll
           for (int e = 0; e < 8; e += 2) top = fmax3f_nan(top, fabsf(value(k, e)), fabsf(value(k, e + 1)));
         }
-        aux->shared[t][hh][r] = top;
-        meet();
-        top = fmax3f_nan(top, aux->shared[t][hh ^ 1][r], top);
         // times 2^up: [2^8, 2^9), or less for rows below 2^-119. A row with a NaN or an infinity is NaN.
         const int ex = max((__float_as_int(top) >> 23) & 255, 8), up = 135 - ex;
         const float f = ex == 255 ? __int_as_float(0x7fffffff) : __int_as_float((127 + up) << 23);
-        float sums[2] = {0.f, 0.f};
-        uint32_t qw[32];
+        uint8_t* z = smem + kOffZq + t * 4096 + r * 16;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          float y[8];
+        for (int half = 0; half < 2; ++half) {
+          float sums[2] = {0.f, 0.f};
+          uint32_t qw[32];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = value(k, e) * f;
-          sums[k >> 2] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+          for (int k = 0; k < 8; ++k) {
+            float y[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) qw[k * 4 + e] = pack2<true>(y[e], y[e + 4]);
+            for (int e = 0; e < 8; ++e) y[e] = value(half * 8 + k, e) * f;
+            sums[k >> 2] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qw[k * 4 + e] = pack2<true>(y[e], y[e + 4]);
+          }
+          tmem_st_32x32b_x32(qcol + half * 32, qw);
+          const uint32_t z0 = pack2<true>(sums[0], 0.f), z1 = pack2<true>(sums[1], 0.f);
+          *reinterpret_cast<uint2*>(z + half * 8) = make_uint2(z0, z1);
+          *reinterpret_cast<uint2*>(z + 2048 + half * 8) = make_uint2(pack2<true>(sums[0] - __low2float(as_half2(z0)), 0.f),
+                                                                      pack2<true>(sums[1] - __low2float(as_half2(z1)), 0.f));
         }
-        tmem_st_32x32b_x32(qcol + hh * 32, qw);
-        const uint32_t z0 = pack2<true>(sums[0], 0.f), z1 = pack2<true>(sums[1], 0.f);
-        uint8_t* z = smem + kOffZq + t * 4096 + r * 16 + hh * 8;
-        *reinterpret_cast<uint2*>(z) = make_uint2(z0, z1);
-        *reinterpret_cast<uint2*>(z + 2048) = make_uint2(pack2<true>(sums[0] - __low2float(as_half2(z0)), 0.f),
-                                                          pack2<true>(sums[1] - __low2float(as_half2(z1)), 0.f));
         // (not 0, nor NaN: a masked score, -inf, stays -inf)
         mult = fmaxf(__int_as_float((127 - up) << 23) * (p.scale * 1.4426950408889634f), 1e-37f);
         fence_proxy_async_smem();
@@ -420,24 +415,20 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       for (int j = 0; j < mine; ++j, ++sc) {
         mbar_wait_warp(&aux->s_full[t], sc & 1);
         tc_fence_after();
-        uint32_t x[32];
-        tmem_ld_32x32b_x32(scol + hh * 32, x);
+        uint32_t x[2][32];
+        tmem_ld_32x32b_x32(scol, x[0]);
+        tmem_ld_32x32b_x32(scol + 32, x[1]);
         tmem_wait_ld();
         if (j >= clean) {
-          const int seen = lim - j * kTok - hh * 32;
+          const int seen = lim - j * kTok;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = e < seen ? x[e] : 0xff800000u;
+          for (int e = 0; e < 64; ++e) x[e >> 5][e & 31] = e < seen ? x[e >> 5][e & 31] : 0xff800000u;
         }
-        float a0 = -INFINITY, a1 = -INFINITY;
+        float a[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          a0 = fmax3f_nan(a0, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-          a1 = fmax3f_nan(a1, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-        }
-        a0 = fmax3f_nan(a0, a1, a1);
-        aux->shared[t][hh][r] = a0;
-        meet();  // (both halves have their scores in registers: P goes over the first 32 columns)
-        const float top = fmax3f_nan(a0, aux->shared[t][hh ^ 1][r], a0) * mult;
+        for (int e = 0; e < 64; e += 2)
+          a[(e >> 1) & 3] = fmax3f_nan(a[(e >> 1) & 3], __uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1]));
+        const float top = fmax3f_nan(fmax3f_nan(a[0], a[1], a[2]), a[3], a[3]) * mult;
         // weights up to 2^6 after a move, to 2^14 before the next: fp16 holds 2^-24 of them
         const bool move = top > mx + 14.f;
         const float dm = move ? ex2(mx - (top - 6.f)) : 1.f;  // 0 while nothing has been seen
@@ -446,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         if (j > 0 && __any_sync(0xffffffffu, move)) {
           // the scores of step j come after P V of step j - 1: the output is at rest
 #pragma unroll 1
-          for (int g = 0; g < 4; ++g) {
+          for (int g = 0; g < 8; ++g) {
             uint32_t o[16];
             tmem_ld_32x32b_x16(ocol + g * 16, o);
             tmem_wait_ld();
@@ -456,19 +447,20 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
           }
         }
         float r0 = 0.f, r1 = 0.f, r2 = 0.f, r3 = 0.f;
-        uint32_t pk[16];
+        uint32_t pk[32];
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
+        for (int e = 0; e < 64; e += 4) {
+          const uint32_t* s = &x[e >> 5][e & 31];
           float y0, y1, y2, y3;
-          ffma2_bcast(y0, y1, __uint_as_float(x[e]), __uint_as_float(x[e + 1]), mult, neg);
-          ffma2_bcast(y2, y3, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]), mult, neg);
+          ffma2_bcast(y0, y1, __uint_as_float(s[0]), __uint_as_float(s[1]), mult, neg);
+          ffma2_bcast(y2, y3, __uint_as_float(s[2]), __uint_as_float(s[3]), mult, neg);
           y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
           fadd2(r0, r1, y0, y1);
           fadd2(r2, r3, y2, y3);
           pk[e >> 1] = pack2<true>(y0, y1);
           pk[(e >> 1) + 1] = pack2<true>(y2, y3);
         }
-        tmem_st_32x32b_x16(scol + hh * 16, pk);
+        tmem_st_32x32b_x32(scol, pk);  // over the scores' first half
         l = l * dm + ((r0 + r1) + (r2 + r3));
         if (!(top < INFINITY)) l = __int_as_float(0x7fffffff);
         tmem_wait_st();
@@ -479,11 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       // ----------------------------------------------------------- output
       float inv = 0.f, lse = -INFINITY;
       if (mine > 0) {
-        mbar_wait_warp(&aux->o_final[t], pieces++ & 1);  // both warps have read the maxima: the slots take the sums
+        mbar_wait_warp(&aux->o_final[t], pieces++ & 1);
         tc_fence_after();
-        aux->shared[t][hh][r] = l;
-        meet();
-        l = aux->shared[t][0][r] + aux->shared[t][1][r];
         if (mx > -INFINITY || l != l) {  // (a NaN is no maximum)
           inv = 1.f / l;
           lse = (mx + __log2f(l)) * 0.6931471805599453f;
@@ -491,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       }
       const bool whole = walk.starts && walk.ends, aborted = __any_sync(0xffffffffu, cta_aborted());
       const int64_t slot = ((static_cast<int64_t>(walk.starts ? 2 * c + 1 : 2 * c) * p.kv_heads + h) * kBlock) + t * kRows;
-      if (hh == 0 && real && !aborted) {
+      if (real && !aborted) {
         if (walk.starts)
           P.parts.row_info[out_row] =
               walk.ends ? 0 : cut_info(run, c, walk.base + unit.tiles(walk.q, walk.kv, walk.block) - 1) + row;
@@ -500,13 +489,13 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         else
           P.parts.lse[slot + r] = lse;
       }
-      // Through shared memory (16-byte part q of row r at q ^ (r % 8)), so that a store
-      // instruction writes whole lines of a few rows. Values lie as their codes' pairs do: n, n + 4 of each eight.
+      // Through shared memory, 128 bytes of a row at a time (16-byte part q of row r at q ^ (r % 8)), so that a store
+      // instruction writes whole lines of four rows. Values lie as their codes' pairs do: n, n + 4 of each eight.
       const int first_row = (r & ~31), here = min(32, rows - (t * kRows + first_row));
-      uint8_t* stage = smem + kOffOut + t * kStageOut + (warp & 7) * 4096;
+      uint8_t* stage = smem + kOffOut + warp * 4096;
       if (here > 0 && !aborted) {
 #pragma unroll 1
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < 4; ++g) {  // 32 values
           uint32_t o[32] = {};
           if (mine > 0) {
             tmem_ld_32x32b_x32(ocol + g * 32, o);
@@ -518,9 +507,10 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
           if (whole) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-              *reinterpret_cast<uint4*>(stage + lane * 128 + (((g * 4 + q) ^ (lane & 7)) << 4)) =
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((((g & 1) * 4 + q) ^ (lane & 7)) << 4)) =
                   make_uint4(pack2<kFp16>(y(q, 0), y(q, 2)), pack2<kFp16>(y(q, 4), y(q, 6)), pack2<kFp16>(y(q, 1), y(q, 3)),
                              pack2<kFp16>(y(q, 5), y(q, 7)));
+            if (!(g & 1)) continue;
           } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -530,24 +520,22 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
                   make_uint4(o[q * 8 + 1], o[q * 8 + 3], o[q * 8 + 5], o[q * 8 + 7]);
             }
           }
-          if (whole && g == 0) continue;
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int rr = k * 4 + (lane >> 3), q = lane & 7;
             const int64_t to = __shfl_sync(0xffffffffu, out_row, rr);
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((q ^ (rr & 7)) << 4));
+            const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((q ^ (rr & 7)) << 4));
             if (rr >= here) continue;
             if (whole)
-              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * kHeadDim + hh * 64 + q * 8) = v;
+              *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to * kHeadDim + (g >> 1) * 64 + q * 8) = w;
             else
-              *reinterpret_cast<uint4*>(P.parts.o + (slot + first_row + rr) * kHeadDim + hh * 64 + g * 32 + q * 4) = v;
+              *reinterpret_cast<uint4*>(P.parts.o + (slot + first_row + rr) * kHeadDim + g * 32 + q * 4) = w;
           }
           __syncwarp();
         }
       }
       tc_fence_before();
-      meet_tile();  // (the maxima's places are the next piece's from here on)
     }
   }
   if (cta_aborted()) {
@@ -557,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
