@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
   constexpr int kNext = Pl::kNext * kStride;
   __shared__ uint64_t full[kWarps][kStages], empty[kWarps][kStages];  // per group
   __shared__ uint64_t stall;
+  __shared__ QuantRun found[kWarps];
   const QuantDecodeLaunch& p = P.L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem_raw + ((0u - smem_u32(smem_raw)) & 127u);
@@ -155,9 +156,13 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
     tma_prefetch_desc(&P.key);
     tma_prefetch_desc(&P.value);
   }
-  __syncthreads();
   const QuantUnit<kRows, kTok> unit(p);
-  const QuantRun run = find_run<kRows, kTok, kSetup>(unit, c, P.parts.runs);
+  if (member == 0) {
+    const QuantRun r = find_run<kRows, kTok, kSetup>(unit, c, P.parts.runs);
+    if (lane == 0) found[group] = r;
+  }
+  __syncthreads();
+  const QuantRun run = found[group];
   if (p.q_len == 0) {  // rows of tokens that are no request's: nothing to merge
     int64_t own = 0;
     for (int b = lane; b < p.batch; b += 32) own += min(max(p.q_lens[b], static_cast<int64_t>(0)), p.num_tokens);
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
         for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
         const int r = n * 8 + 2 * t + k;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const float lse = l == 0.f ? -INFINITY : (ref[n][k] + __log2f(l)) * 0.6931471805599453f;
+        const float lse = l == 0.f ? -INFINITY : (ref[n][k] + log2f(l)) * 0.6931471805599453f;
         if (r >= rows) continue;
         int i;
         const int64_t row = row_of(r, i);

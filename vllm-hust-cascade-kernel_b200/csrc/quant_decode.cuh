@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kWarps == 1 ? 256 : 32 * kWarps)
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   reinterpret_cast<uint2*>(static_cast<uint16_t*>(L.out) + row * kHeadDim)[lane] =
       make_uint2(pack2<kFp16>(acc.x * inv, acc.y * inv), pack2<kFp16>(acc.z * inv, acc.w * inv));
-  if (lane == 0) L.lse[row] = sum == 0.f ? -INFINITY : top + __logf(sum);
+  if (lane == 0) L.lse[row] = sum == 0.f ? -INFINITY : top + logf(sum);
 }
 
 inline size_t quant_info_bytes(const QuantDecodeLaunch& p) {

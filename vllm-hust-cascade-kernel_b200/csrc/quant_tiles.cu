@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         tc_fence_after();
         if (mx > -INFINITY || l != l) {  // (a NaN is no maximum)
           inv = 1.f / l;
-          lse = (mx + __log2f(l)) * 0.6931471805599453f;
+          lse = (mx + log2f(l)) * 0.6931471805599453f;
         }
       }
       const bool whole = walk.starts && walk.ends, aborted = __any_sync(0xffffffffu, cta_aborted());
