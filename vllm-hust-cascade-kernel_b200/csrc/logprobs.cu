@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const
   }
   if (warp == 0) {
     const bool nan = s.nan || !(s.m < INFINITY) || s.m == -INFINITY;
-    const float norm = nan ? __int_as_float(0x7fffffff) : __logf(s.sum);
+    const float norm = nan ? __int_as_float(0x7fffffff) : logf(s.sum);
     if (lane == 0) {
       p.logprob[n] = given ? (mine - s.m) - norm : -INFINITY;
       p.entropy[n] = norm - s.dot / s.sum * kLn2;

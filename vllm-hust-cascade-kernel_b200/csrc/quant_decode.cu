@@ -19,13 +19,17 @@
 // M (output), the query rows as its N, so eight rows cost eight columns, and the
 // probabilities' fragments turn by one movmatrix. (tcgen05 would need M = 128 of
 // tokens, converted through shared memory; here 16 of 128 lanes' worth of rows
-// exist, and the products take a third of the time that HBM does.)
+// exist. With 32 rows the tcgen05 kernel is the slower one, as row_blocks says.)
 //
-// A warp is on its own: it has a run of 32-token tiles of one kv head, a ring of
-// tiles that the TMA fills, and its rows' softmax; neighbouring warps take the
-// other heads of the same tokens. The place of a token in the MMA's rows (first_token, value_token)
+// A warp has one kv head's rows, their softmax and output, over a run of 32-token
+// tiles; the warps of up to eight heads share the tiles' ring, which the first of
+// them keeps filled by TMA. The place of a token in the MMA's rows (first_token, value_token)
 // keeps every shared-memory load of 80-byte rows free of bank conflicts.
 // The running maxima move only when a score exceeds its row's by more than 2^8.
+//
+// 8 kv heads x 4 query heads: 128 requests of 1,200 to 7,800 tokens (788 MB) 165 us,
+// 4.8 TB/s; 149 without the arithmetic, of which 8 for the start (lengths, run, page
+// ids, first tile) and 4 for the merge. One request of 900 tokens 13.9 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,7 +39,10 @@ namespace cascade {
 namespace {
 
 constexpr int kTok = 32;     // tokens per tile
-constexpr int kSetup = 2;    // what a new unit costs, in tiles
+// What a new unit costs, in tiles: its page ids, query rows and output. 24 to 48 requests of 1 to 6,000 tokens and 4 to 8
+// heads' rows: 52.4, 57.3, 54.1 us with 6, 63.1, 63.7, 59.4 with 2, 51.4, 58.2, 54.9 with 10, 53.3, 59.6, 56.6 with 16; 96
+// requests of up to 700 tokens would have it less: 25.9 with 6, 25.0 with 2.
+constexpr int kSetup = 6;
 constexpr int kTileBytes = kTok * kQuantRow;  // of keys or of values
 constexpr int32_t kNoPage = INT32_MIN;
 constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
@@ -626,8 +633,11 @@ cudaError_t launch(const QuantDecodeLaunch& p, void* workspace, cudaStream_t str
 }
 
 // Blocks of 8 query rows per warp: as a request has rows (known from the shapes: the mean, with lengths on the device).
-// Unpacking is shared by a warp's blocks: 259 instructions per 16 tokens for one block, some 60 for each more. More than
-// four go to the 128-row tiles (0).
+// Unpacking, most of a block's some 330 instructions per 16 tokens, is shared by a warp's blocks. More than four would
+// take a second walk over the tokens, and go to the 256-row blocks of quant_tiles.cu (0). Both ways, 8 kv heads: 96 requests
+// over 4,000 tokens with 32 rows 301 us here against 537, with 36 rows 537 (in two walks) against 538, with 64 rows 559
+// against 545, with 128 rows 1,035 against 562; one request over 32,768 tokens with 32 rows 54 against 60, with 36 67
+// against 57, with 128 112 against 62.
 int row_blocks(const QuantDecodeLaunch& p) {
   const int64_t rows = (p.num_tokens * p.group + p.batch - 1) / p.batch;
   return rows <= 32 ? static_cast<int>((rows + 7) / 8) : 0;
