@@ -14,9 +14,11 @@
 // where a thread hides very many entries: then the CTA takes one maximum after the
 // other.
 //
-// Bound by HBM for large batches, with the instructions per logit (5.5 and a
-// special function) close behind in 16 bits; few rows are shared by a cluster of
-// CTAs, which meet in the first one's shared memory.
+// Bound by HBM in fp32 (1,500 rows of 128,256 without alternatives: 125 us, 6.2
+// TB/s) and by instructions in 16 bits (some ten per logit, one for the special
+// function unit: 74 us, 5.2 TB/s); an alternative adds 9 us there, 20 add 14. Few
+// rows are shared by a cluster of CTAs, which meet in the first one's shared memory
+// (128 rows with 20 alternatives 18.2 us, 4 of 32,000 with 5 8.4).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -31,9 +33,12 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kVecs = 4;       // vectors of a batch per thread, 32 apart
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+// Threads of a CTA: 256, and 128 for rows of 16 bits that have a CTA each. Its warps wait for one another to find the
+// alternatives, its SM's other CTAs do not: 1,500 rows with one alternative 82 us with 128, 92 with 256, 133 with 512; but a row
+// that has eight CTAs is done in 9.1 us with 256 and 10.0 with 128. fp32 rows have HBM to wait for: 125 us with 256, 154 with 128.
+// Threads per SM: 768 in 16 bits (1,024 with 64 registers: 94 us for 77), 1,024 in fp32.
 template <int kType>
-constexpr int kPerSm = kType == 2 ? 4 : 3;  // CTAs (16 bits with 64 registers: 102 us for 86 on 1,500 rows)
+constexpr int kSmThreads = kType == 2 ? 1024 : 768;
 constexpr int kMaxCtas = 8;    // per row
 constexpr int kSlots = 32;     // of batches per thread whose maxima are kept
 constexpr int kList = 1024;    // entries, or batches, that may reach the bound
@@ -198,7 +203,9 @@ __device__ __forceinline__ uint64_t warp_max(uint64_t k) {
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
+template <int kThreads>
 struct Shared {
+  static constexpr int kWarps = kThreads / 32;
   float batch_max[kSlots][kThreads];
   uint64_t list[kList];
   uint32_t hits[kList];  // slot, thread
@@ -210,13 +217,13 @@ struct Shared {
   int count, hit_count;
 };
 
-template <int kType>
-__global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const LogprobsLaunch p) {
-  constexpr int kW = Vec<kType>::kW;
+template <int kType, int kThreads>
+__global__ void __launch_bounds__(kThreads, kSmThreads<kType> / kThreads) logprobs_kernel(const LogprobsLaunch p) {
+  constexpr int kW = Vec<kType>::kW, kWarps = kThreads / 32;
   constexpr int kBatch = kVecs * kW;         // a thread's logits per batch
   constexpr int kSpan = 32 * kVecs;          // a warp's vectors per batch
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  Shared& sh = *reinterpret_cast<Shared*>(smem_raw);
+  Shared<kThreads>& sh = *reinterpret_cast<Shared<kThreads>*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   cluster.barrier_arrive();  // waited for before the first write to another CTA: all have started by then
@@ -298,11 +305,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const
   };
   // The others, with a maximum below 1e37 in size: a finite number can stand in for -inf (0 times infinity would be NaN).
   auto batch = [&](const uint4 (&raw)[kVecs], int b) {
-    const float most = batch_max<kType>(raw);
+    const float most = batch_max<kType>(raw), bar = b < token_batch ? above_before : above;
+    const bool ahead = __any_sync(0xffffffffu, most > bar);
     if (!(fabsf(fmaxf(s.m, most)) < 1e37f)) return false;
     note(most, b);
     if (b != token_batch) {
-      s.ahead += count_above<kType>(raw, b < token_batch ? above_before : above);
+      if (ahead) s.ahead += count_above<kType>(raw, bar);
     } else {
 #pragma unroll
       for (int q = 0; q < kVecs; ++q) {
@@ -314,22 +322,30 @@ __global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const
       }
     }
     const float neg = -s.m;
-    float sum0 = 0.f, sum1 = 0.f, dot0 = 0.f, dot1 = 0.f;
+    float sum = 0.f, dot = 0.f;
+    auto sums = [&](auto low) {
+      float sum0 = 0.f, sum1 = 0.f, dot0 = 0.f, dot1 = 0.f;
 #pragma unroll
-    for (int q = 0; q < kVecs; ++q) {
-      float x[kW];
-      unpack<kType>(clamp_low<kType>(raw[q]), x);
+      for (int q = 0; q < kVecs; ++q) {
+        float x[kW];
+        unpack<kType>(low ? clamp_low<kType>(raw[q]) : raw[q], x);
 #pragma unroll
-      for (int j = 0; j < kW; j += 2) {
-        float y0 = x[j], y1 = x[j + 1];
-        fadd2(y0, y1, neg, neg);
-        fmul2(y0, y1, kLog2e);
-        const float e0 = ex2(y0), e1 = ex2(y1);
-        fadd2(sum0, sum1, e0, e1);
-        ffma2(dot0, dot1, e0, e1, y0, y1);
+        for (int j = 0; j < kW; j += 2) {
+          float y0 = x[j], y1 = x[j + 1];
+          fadd2(y0, y1, neg, neg);
+          fmul2(y0, y1, kLog2e);
+          const float e0 = ex2(y0), e1 = ex2(y1);
+          fadd2(sum0, sum1, e0, e1);
+          ffma2(dot0, dot1, e0, e1, y0, y1);
+        }
       }
-    }
-    s.sum += sum0 + sum1, s.dot += dot0 + dot1;
+      sum = sum0 + sum1, dot = dot0 + dot1;
+    };
+    // In 16 bits, where instructions count, first as if there were no -inf; then 0 times infinity is a NaN. (In fp32, 130 us for
+    // 1,500 rows, the second form costs registers: 173.)
+    if constexpr (kType != 2) sums(std::false_type());
+    if (kType == 2 || dot != dot) sums(std::true_type());
+    s.sum += sum, s.dot += dot;
     return true;
   };
   int b = first + warp;
@@ -406,20 +422,34 @@ __global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const
       __syncthreads();
       const int hits = sh.hit_count;
       if (hits <= kList) {
-        // a lane per entry (fp32: two batches at once)
-        constexpr int kAtOnce = 32 / kBatch;
-        for (int i = warp * kAtOnce + lane / kBatch; i < hits; i += kWarps * kAtOnce) {
-          const uint32_t hit = sh.hits[i];
-          const int who = hit & 0xffff, b0 = first + (who >> 5) + static_cast<int>(hit >> 16) * per_slot * kWarps;
+        // a lane per entry (fp32: two batches at once), a warp's next loads under way before it looks at these
+        constexpr int kAtOnce = 32 / kBatch, kAhead = 4;
+        for (int i = warp * kAtOnce + lane / kBatch; i < hits; i += kWarps * kAtOnce * kAhead) {
+          int b[kAhead], v[kAhead];
+#pragma unroll
+          for (int k = 0; k < kAhead; ++k) {
+            const uint32_t hit = i + k * kWarps * kAtOnce < hits ? sh.hits[i + k * kWarps * kAtOnce] : 0xffffu;
+            const int who = hit & 0xffff;
+            b[k] = who == 0xffff ? last : first + (who >> 5) + static_cast<int>(hit >> 16) * per_slot * kWarps;
+            v[k] = who & 31;
+          }
           for (int j = 0; j < per_slot; ++j) {
-            const int b = b0 + j * kWarps;
-            if (b >= last) break;
-            const int idx = index_of(b * kSpan + (who & 31), lane % kBatch);
-            if (idx < 0 || idx >= V) continue;
-            const uint64_t a = make_key(load_one<kType>(row, idx), static_cast<uint32_t>(idx));
-            if (a >= bound) {
-              const int to = atomicAdd(&sh.count, 1);
-              if (to < kList) sh.list[to] = a;
+            float x[kAhead];
+            int idx[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+              idx[k] = b[k] < last ? index_of(b[k] * kSpan + v[k], lane % kBatch) : -1;
+              if (idx[k] >= V) idx[k] = -1;
+              x[k] = idx[k] >= 0 ? load_one<kType>(row, idx[k]) : 0.f;
+              b[k] += kWarps;
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+              const uint64_t a = make_key(x[k], static_cast<uint32_t>(idx[k]));
+              if (idx[k] >= 0 && a >= bound) {
+                const int to = atomicAdd(&sh.count, 1);
+                if (to < kList) sh.list[to] = a;
+              }
             }
           }
         }
@@ -474,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const
   }
   cluster.barrier_wait();
   if (ctas > 1) {
-    Shared& root = *cluster.map_shared_rank(&sh, 0);
+    Shared<kThreads>& root = *cluster.map_shared_rank(&sh, 0);
     if (threadIdx.x == 0) root.cta[rank] = s;
     if (threadIdx.x < top) root.gather[rank * top + threadIdx.x] = sh.sorted[threadIdx.x];
     cluster.sync();
@@ -484,8 +514,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const
       for (int c = 1; c < ctas; ++c) add(s, sh.cta[c]);
     }
     const int all = ctas * top;
-    if (static_cast<int>(threadIdx.x) < all) {
-      const uint64_t a = sh.gather[threadIdx.x];
+    for (int i = threadIdx.x; i < all; i += kThreads) {
+      const uint64_t a = sh.gather[i];
       int before = 0;
       for (int j = 0; j < all; ++j) before += sh.gather[j] > a;
       if (a != 0 && before < top) sh.sorted[before] = a;
@@ -513,19 +543,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm<kType>) logprobs_kernel(const
 
 size_t token_logprobs_workspace(const LogprobsLaunch&) { return 0; }
 
-cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void*, cudaStream_t stream) {
-  // as many CTAs per row as run at once, with a batch for each of their warps
-  const int64_t batch = 32 * kVecs * (p.dtype == 2 ? 4 : 8);
-  const int per_sm = p.dtype == 2 ? kPerSm<2> : kPerSm<0>;
-  int ctas = 1;
-  while (ctas < kMaxCtas && p.rows * ctas * 2 <= per_sm * kNumSMs && p.vocab >= 2 * ctas * kWarps * batch) ctas *= 2;
-  auto kern = p.dtype == 2 ? logprobs_kernel<2> : p.dtype == 1 ? logprobs_kernel<1> : logprobs_kernel<0>;
-  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), sizeof(Shared));
+template <int kType, int kThreads>
+static cudaError_t launch(const LogprobsLaunch& p, int ctas, cudaStream_t stream) {
+  auto kern = logprobs_kernel<kType, kThreads>;
+  cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), sizeof(Shared<kThreads>));
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(p.rows * ctas));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.dynamicSmemBytes = sizeof(Shared<kThreads>);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -535,6 +561,20 @@ cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void*, cudaStream_t s
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+template <int kType>
+static cudaError_t launch(const LogprobsLaunch& p, cudaStream_t stream) {
+  // as many CTAs per row as run at once, with a batch for each of their warps
+  constexpr int kMost = kSmThreads<kType> / 256 * kNumSMs, kSpan = 256 * kVecs * Vec<kType>::kW;
+  int ctas = 1;
+  while (ctas < kMaxCtas && p.rows * ctas * 2 <= kMost && p.vocab >= 2 * ctas * kSpan) ctas *= 2;
+  if (kType != 2 && ctas == 1) return launch<kType, 128>(p, 1, stream);
+  return launch<kType, 256>(p, ctas, stream);
+}
+
+cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void*, cudaStream_t stream) {
+  return p.dtype == 2 ? launch<2>(p, stream) : p.dtype == 1 ? launch<1>(p, stream) : launch<0>(p, stream);
 }
 
 }  // namespace cascade
