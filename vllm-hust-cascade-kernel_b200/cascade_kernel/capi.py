@@ -40,6 +40,12 @@ EXPORTED = [
     "cascade_page_compact_workspace_size",
     "cascade_page_compact",
     "cascade_verify_drafts",
+    "cascade_quant_write",
+    "cascade_quant_read",
+    "cascade_quant_decode_workspace_size",
+    "cascade_quant_decode",
+    "cascade_token_logprobs_workspace_size",
+    "cascade_token_logprobs",
 ]
 
 
