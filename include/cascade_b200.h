@@ -515,17 +515,17 @@ CASCADE_API int cascade_quant_decode(const cascade_quant_attn_t *p, void *out, f
  *           rank int64 [rows]; top_logprobs fp32, top_tokens int64 [rows, top],
  *           0 <= top <= min(32, vocab)
  * A vocab of 2^30 - 1 and more is unsupported. */
-CASCADE_API size_t cascade_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int32_t dtype, int64_t top);
 CASCADE_API int cascade_token_logprobs(const void *logits, int64_t row_stride, const int64_t *tokens, int32_t dtype,
                                        int64_t rows, int64_t vocab, int64_t top, float *logprob, float *entropy,
-                                       int64_t *rank, float *top_logprobs, int64_t *top_tokens, void *workspace,
-                                       size_t workspace_bytes, cascade_stream_t stream);
+                                       int64_t *rank, float *top_logprobs, int64_t *top_tokens,
+                                       cascade_stream_t stream);
 
 /* Last error message of this thread ("" if none). */
 CASCADE_API const char *cascade_last_error(void);
 
 /* Reads and clears the device error word. Bits: 1 = a kernel's bounded wait
- * gave up; 2 = a block id outside the pool was read as a zero page; 4 = a
+ * gave up; 2 = a block id outside the pool was read as a zero page, or a slot
+ * outside a 4-bit cache was skipped or read as zeros; 4 = a
  * stage-1 piece fell outside its planned partial planes and was skipped (its
  * rows are garbage; the planner's bound rules this out). Synchronises the
  * current device. */

@@ -99,8 +99,8 @@ def test_write_and_read_refusals():
 def test_logprobs_refusals():
     from cascade_kernel import capi as C
     lib = C.load()
-    names = ("logits", "stride", "tokens", "dtype", "rows", "vocab", "top", "logprob", "entropy", "rank", "tl", "tt", "ws", "n")
-    ok = dict(zip(names, (4096, 100, 4096, C.BF16, 3, 100, 5, 4096, 4096, 4096, 4096, 4096, 4096, 1 << 40)))
+    names = ("logits", "stride", "tokens", "dtype", "rows", "vocab", "top", "logprob", "entropy", "rank", "tl", "tt")
+    ok = dict(zip(names, (4096, 100, 4096, C.BF16, 3, 100, 5, 4096, 4096, 4096, 4096, 4096)))
 
     def call(**kw):
         return lib.cascade_token_logprobs(*{**ok, **kw}.values(), None)
@@ -113,9 +113,6 @@ def test_logprobs_refusals():
                      (dict(rank=4100), "aligned to their elements")]:
         _refused(call(**kw), text)
     assert call(rows=0, logits=None) == C.OK
-    need = lib.cascade_token_logprobs_workspace_size(3, 100, C.BF16, 5)
-    if need:
-        _refused(call(n=need - 1), "workspace too small")
 
 
 def test_schemas():

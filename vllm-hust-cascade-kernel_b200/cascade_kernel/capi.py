@@ -44,7 +44,6 @@ EXPORTED = [
     "cascade_quant_read",
     "cascade_quant_decode_workspace_size",
     "cascade_quant_decode",
-    "cascade_token_logprobs_workspace_size",
     "cascade_token_logprobs",
 ]
 
@@ -180,9 +179,7 @@ def load():
     lib.cascade_quant_decode_workspace_size.restype = sz
     lib.cascade_quant_decode.argtypes = [ctypes.POINTER(QuantAttn), vp, vp, vp, sz, vp]
     lib.cascade_quant_decode.restype = ctypes.c_int
-    lib.cascade_token_logprobs_workspace_size.argtypes = [i64, i64, i32, i64]
-    lib.cascade_token_logprobs_workspace_size.restype = sz
-    lib.cascade_token_logprobs.argtypes = [vp, i64, vp, i32, i64, i64, i64, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.cascade_token_logprobs.argtypes = [vp, i64, vp, i32, i64, i64, i64, vp, vp, vp, vp, vp, vp]
     lib.cascade_token_logprobs.restype = ctypes.c_int
     _lib = lib
     return lib

@@ -341,8 +341,7 @@ struct LogprobsLaunch {
   int32_t top;
   int32_t dtype;           // 0 bf16, 1 fp16, 2 fp32
 };
-cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void* workspace, cudaStream_t stream);
-size_t token_logprobs_workspace(const LogprobsLaunch& p);
+cudaError_t launch_token_logprobs(const LogprobsLaunch& p, cudaStream_t stream);
 
 // Host: raise a kernel's dynamic shared memory limit once per (kernel,
 // device) instead of on every launch.

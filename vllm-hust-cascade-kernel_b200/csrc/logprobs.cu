@@ -541,8 +541,6 @@ __global__ void __launch_bounds__(kThreads, kSmThreads<kType> / kThreads) logpro
 
 }  // namespace
 
-size_t token_logprobs_workspace(const LogprobsLaunch&) { return 0; }
-
 template <int kType, int kThreads>
 static cudaError_t launch(const LogprobsLaunch& p, int ctas, cudaStream_t stream) {
   auto kern = logprobs_kernel<kType, kThreads>;
@@ -573,7 +571,7 @@ static cudaError_t launch(const LogprobsLaunch& p, cudaStream_t stream) {
   return launch<kType, 256>(p, ctas, stream);
 }
 
-cudaError_t launch_token_logprobs(const LogprobsLaunch& p, void*, cudaStream_t stream) {
+cudaError_t launch_token_logprobs(const LogprobsLaunch& p, cudaStream_t stream) {
   return p.dtype == 2 ? launch<2>(p, stream) : p.dtype == 1 ? launch<1>(p, stream) : launch<0>(p, stream);
 }
 

@@ -163,20 +163,9 @@ int cascade_quant_decode(const cascade_quant_attn_t* p, void* out, float* lse, v
                                         reinterpret_cast<cudaStream_t>(stream)));
 }
 
-size_t cascade_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int32_t dtype, int64_t top) {
-  if (rows < 1 || vocab < 1 || top < 0 || top > kMaxTop || (!half_type(dtype) && dtype != CASCADE_FP32)) return 0;
-  LogprobsLaunch L = {};
-  L.rows = rows;
-  L.vocab = vocab;
-  L.dtype = dtype;
-  L.top = static_cast<int32_t>(top);
-  return token_logprobs_workspace(L);
-}
-
 int cascade_token_logprobs(const void* logits, int64_t row_stride, const int64_t* tokens, int32_t dtype, int64_t rows,
                            int64_t vocab, int64_t top, float* logprob, float* entropy, int64_t* rank,
-                           float* top_logprobs, int64_t* top_tokens, void* workspace, size_t workspace_bytes,
-                           cascade_stream_t stream) {
+                           float* top_logprobs, int64_t* top_tokens, cascade_stream_t stream) {
   const char* op = "cascade_token_logprobs";
   if (!half_type(dtype) && dtype != CASCADE_FP32)
     return fail(CASCADE_ERR_INVALID, "%s: logits must be bf16, fp16 or fp32", op);
@@ -196,9 +185,7 @@ int cascade_token_logprobs(const void* logits, int64_t row_stride, const int64_t
   const LogprobsLaunch L = {logits,       tokens,     logprob, entropy, rank,
                             top_logprobs, top_tokens, rows,    vocab,   rows > 1 ? row_stride : vocab,
                             static_cast<int32_t>(top), dtype};
-  int rc = check_workspace(op, workspace, workspace_bytes, token_logprobs_workspace(L));
-  if (rc) return rc;
-  return finish(op, launch_token_logprobs(L, workspace, reinterpret_cast<cudaStream_t>(stream)));
+  return finish(op, launch_token_logprobs(L, reinterpret_cast<cudaStream_t>(stream)));
 }
 
 }  // extern "C"

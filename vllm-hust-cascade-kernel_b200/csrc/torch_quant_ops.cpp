@@ -150,14 +150,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> cascade_t
   auto f32 = logits.options().dtype(at::kFloat);
   auto logprob = at::empty({N}, f32), entropy = at::empty({N}, f32), top_logprobs = at::empty({N, top}, f32);
   auto rank = at::empty({N}, tokens.options()), top_tokens = at::empty({N, top}, tokens.options());
-  const size_t ws_bytes = cascade_token_logprobs_workspace_size(N, V, type, top);
-  at::Tensor ws;
-  if (ws_bytes) ws = at::empty({static_cast<int64_t>(ws_bytes)}, logits.options().dtype(at::kByte));
   check_rc(::cascade_token_logprobs(logits.data_ptr(), logits.stride(0), tokens.data_ptr<int64_t>(), type, N, V, top,
                                     logprob.data_ptr<float>(), entropy.data_ptr<float>(), rank.data_ptr<int64_t>(),
                                     top ? top_logprobs.data_ptr<float>() : nullptr,
-                                    top ? top_tokens.data_ptr<int64_t>() : nullptr, ws_bytes ? ws.data_ptr() : nullptr,
-                                    ws_bytes, current_stream(logits)));
+                                    top ? top_tokens.data_ptr<int64_t>() : nullptr, current_stream(logits)));
   return {logprob, entropy, rank, top_logprobs, top_tokens};
 }
 
