@@ -22,6 +22,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "kernels.h"
@@ -542,23 +543,47 @@ __global__ void __launch_bounds__(kThreads, kSmThreads<kType> / kThreads) logpro
 }  // namespace
 
 template <int kType, int kThreads>
+static cudaLaunchConfig_t config(int64_t rows, int ctas, cudaStream_t stream, cudaLaunchAttribute& attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared<kThreads>);
+  cfg.stream = stream;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+template <int kType, int kThreads>
 static cudaError_t launch(const LogprobsLaunch& p, int ctas, cudaStream_t stream) {
   auto kern = logprobs_kernel<kType, kThreads>;
   cudaError_t e = ensure_smem_limit(reinterpret_cast<const void*>(kern), sizeof(Shared<kThreads>));
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.rows * ctas));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared<kThreads>);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr;
+  const cudaLaunchConfig_t cfg = config<kType, kThreads>(p.rows, ctas, stream, attr);
   return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
+// Rows that run at once with `ctas` = 2, 4 or 8 CTAs each. Fewer than the SMs hold: a cluster lies within a part of the GPU whose
+// SMs need not divide by it (16 bits: 48 rows of 8, 104 of 4; one more takes a second round, 16.5 us for 13.2).
+template <int kType>
+static int resident_rows(int ctas) {
+  static std::atomic<int> known[kMaxCtas + 1];
+  int n = known[ctas].load(std::memory_order_relaxed);
+  if (n == 0) {
+    auto kern = logprobs_kernel<kType, 256>;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = config<kType, 256>(1, ctas, nullptr, attr);
+    if (ensure_smem_limit(reinterpret_cast<const void*>(kern), sizeof(Shared<256>)) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess)
+      return 0;
+    known[ctas].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 template <int kType>
@@ -566,7 +591,8 @@ static cudaError_t launch(const LogprobsLaunch& p, cudaStream_t stream) {
   // as many CTAs per row as run at once, with a batch for each of their warps
   constexpr int kMost = kSmThreads<kType> / 256 * kNumSMs, kSpan = 256 * kVecs * Vec<kType>::kW;
   int ctas = 1;
-  while (ctas < kMaxCtas && p.rows * ctas * 2 <= kMost && p.vocab >= 2 * ctas * kSpan) ctas *= 2;
+  while (ctas < kMaxCtas && p.rows * ctas * 2 <= kMost && p.vocab >= 2 * ctas * kSpan && p.rows <= resident_rows<kType>(2 * ctas))
+    ctas *= 2;
   if (kType != 2 && ctas == 1) return launch<kType, 128>(p, 1, stream);
   return launch<kType, 256>(p, ctas, stream);
 }
