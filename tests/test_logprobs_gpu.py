@@ -50,6 +50,28 @@ def test_many_rows_of_a_large_vocabulary(dtype):
     _check(*_logits(200, 128256, dtype, seed=1), 20)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("N,V", [(48, 40001), (49, 40001), (105, 33000), (145, 33000), (223, 20011), (300, 70000)])
+def test_rows_shared_by_clusters_of_every_size(N, V, dtype):
+    Hh.need_cuda()
+    _check(*_logits(N, V, dtype, seed=N), 32)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("share", [0.001, 0.5, 0.999])
+@pytest.mark.parametrize("N", [3, 230])
+def test_minus_infinity_among_the_others(N, share, dtype):
+    """Also with the token ahead of all others, and behind them."""
+    import torch
+    Hh.need_cuda()
+    x, tokens = _logits(N, 30001, dtype, seed=N)
+    gone = torch.rand(x.shape, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda") < share
+    gone[:, 17] = False
+    x[gone] = -float("inf")
+    tokens[0], tokens[1] = x[0].argmax(), x[1].argmin()
+    _check(x, tokens, 5)
+
+
 @pytest.mark.parametrize("V", [40, 1003, 70000])
 def test_equal_logits_go_to_the_lowest_index(V):
     import torch
