@@ -6,7 +6,7 @@
 // values (a 16-byte load or store of 16-bit values, one 32-bit word of codes)
 // each; a group is four neighbouring threads. Bound by HBM (512 bytes of
 // 16-bit values and 160 of cache per token and kv head) and, the write, by its
-// instructions, some 65 for eight values. A thread takes the key and
+// instructions, some 135 for eight values. A thread takes the key and
 // the value of kUnroll rows at once: its chain slot -> row -> store is two
 // latencies long. 60,001 tokens x 4 kv heads: written in 38 us (4.2 TB/s), read back
 // in 29.7 us (5.4 TB/s; the same with four rows at once, 32.7 with eight).
