@@ -272,6 +272,10 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         }
       }
     }
+    // an aborted call: the loads in flight (at most kStages steps') land before their warp leaves
+    if (w == 0) {
+      for (; n < issued; ++n) mbar_wait_drain(&aux->raw_full[n % kStages], (n / kStages) & 1);
+    }
   } else if (warp == 8) {
     // ----------------------------------------------------------- MMA issuer
     const uint32_t idesc_s = make_idesc_f16(kRows, kTok, 0u, 0, 0);
@@ -350,9 +354,13 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         }
       }
     }
-    if (used && !live && lane == 0) {
-      umma_commit(&aux->drain);
-      mbar_wait_drain(&aux->drain, 0);
+    // Products may be in flight when another warp gives up, also after the last one was issued: they end before this warp
+    // frees the tensor memory.
+    if (used) {
+      if (elect_one()) umma_commit(&aux->drain);
+      __syncwarp();
+      if (lane == 0) mbar_wait_drain(&aux->drain, 0);
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------- softmax, output of tile t
@@ -544,11 +552,6 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         }
       }
       tc_fence_before();
-    }
-  }
-  if (cta_aborted()) {
-    // loads may be in flight (at most 40 KB): they get a millisecond before the CTA leaves
-    for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 1000 * 1000;) {
     }
   }
   tc_fence_before();
