@@ -473,7 +473,8 @@ CASCADE_API int cascade_quant_read(const void *key_cache, const void *value_cach
  * lse NaN; a NaN in a value at least the group's 32 values of out. A query row
  * with a NaN or an infinity that sees a token gives NaN.
  *   query  [num_tokens, num_heads, 128] in `dtype`, contiguous, 16-byte aligned
- * The other fields, the lengths and the block ids are as in cascade_latent_attn_t. */
+ * The other fields, the lengths and the block ids are as in cascade_latent_attn_t.
+ * A batch of 2^30 and more is unsupported. */
 typedef struct cascade_quant_attn {
   const void *query;
   const void *key_cache;

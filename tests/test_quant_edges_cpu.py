@@ -1,0 +1,19 @@
+"""CPU-only checks of sizes that the 4-bit cache's entry points have to refuse."""
+import ctypes
+
+import pytest
+
+
+@pytest.mark.parametrize("batch", [(1 << 30), (1 << 31) - 32, (1 << 31) - 1])
+def test_decode_refuses_batches_whose_steps_wrap(batch):
+    """With query lengths on the device a batch need not have a token per request; the kernels walk it in steps of a warp."""
+    from cascade_kernel import capi as C
+    p = C.QuantAttn()
+    for k, v in dict(num_tokens=3, num_heads=16, kv_heads=4, head_dim=128, num_blocks=100, block_size=64, batch=batch, block_cols=0,
+                     q_seqlen_value=0, scale=0.1, causal=1, dtype=C.BF16, flags=0).items():
+        setattr(p, k, v)
+    lib = C.load()
+    assert lib.cascade_quant_decode(ctypes.byref(p), None, None, None, 0, None) != C.OK and "too large" in C.last_error()
+    assert lib.cascade_quant_decode_workspace_size(ctypes.byref(p)) == 0
+    p.batch = (1 << 30) - 1
+    assert lib.cascade_quant_decode(ctypes.byref(p), None, None, None, 0, None) != C.OK and "null device pointer" in C.last_error()
