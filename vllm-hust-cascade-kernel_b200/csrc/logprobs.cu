@@ -131,14 +131,11 @@ __device__ __forceinline__ int count_above(const uint4 (&v)[kN], float bar) {
   }
 }
 
-// -inf (and what lies below -1e38) as a finite number; NaN stays
+// -inf (and what lies below -1e38) as a finite number; NaN stays. fp16 has no number that far below all others: there the
+// differences are cut (below).
 template <int kType>
 __device__ __forceinline__ uint4 clamp_low(uint4 v) {
-  if constexpr (kType == 1) {
-    __half2* h = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], __float2half2_rn(-65504.f));
-  } else if constexpr (kType == 0) {
+  if constexpr (kType == 0) {
     __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], __float2bfloat162_rn(-1e38f));
@@ -335,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, kSmThreads<kType> / kThreads) logpro
           float y0 = x[j], y1 = x[j + 1];
           fadd2(y0, y1, neg, neg);
           fmul2(y0, y1, kLog2e);
+          if constexpr (kType == 1 && decltype(low)::value) y0 = fmax3f_nan(y0, -1e30f, -1e30f), y1 = fmax3f_nan(y1, -1e30f, -1e30f);
           const float e0 = ex2(y0), e1 = ex2(y1);
           fadd2(sum0, sum1, e0, e1);
           ffma2(dot0, dot1, e0, e1, y0, y1);
