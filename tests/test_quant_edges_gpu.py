@@ -27,3 +27,45 @@ def test_a_call_behind_a_stalled_one(q_len, G):
             C.quant_decode(d, out, lse, ws)
         assert torch.equal(outs[1][0], want[0]) and torch.equal(outs[1][1], want[1])
         assert C.device_error() == 1
+
+
+@pytest.mark.parametrize("dtype,size,keys", [("fp16", 3e4, 1.0), ("fp16", 6e4, 100.0), ("bf16", 1e7, 1.0), ("bf16", 3e9, 1.0),
+                                             ("bf16", 1e12, 1.0), ("bf16", 1e20, 30.0), ("bf16", 1e30, 1.0), ("bf16", 1e35, 1.0),
+                                             ("bf16", 1e-30, 100.0)])
+@pytest.mark.parametrize("q_len,KVH,G,lens", [(1, 2, 4, [40, 1000, 7]), (4, 1, 5, [333, 90]), (4, 2, 8, [700, 31]),
+                                              (40, 1, 4, [100, 2000]), (100, 2, 4, [333, 90])])
+def test_scores_of_any_size(q_len, KVH, G, lens, dtype, size, keys):
+    """Finite scores, whatever their size: with large ones a single token has all the weight.
+
+    The third token's key is 6 (times `keys`) and more in every value against some 1 of the others, and the query positive, so that
+    it wins by half of its score at least; a token that half of the queries see beats it in the same way. All their products
+    have one sign: a score is the sum of 17 times 16 of them (scales in two parts, centres), one after the other in fp32, each
+    addition off by at most 2^-23 (the tensor cores may truncate); its factor and the logarithm's are 2^-22 of it off."""
+    import torch
+    Hh.need_cuda()
+    args = _inputs(lens, [q_len] * len(lens), KVH, G, 16, dtype, seed=q_len + G, loud=False)
+    args[0].copy_((args[0].float().abs().clamp(0.1, 1) * size).to(args[0].dtype))
+    par = args[1][..., 64:].contiguous().view(torch.float16)
+    par = (par.float() * 0.5 * keys).half().unflatten(-1, (4, 2))
+    args[1][..., 64:] = par.flatten(-2).contiguous().view(torch.uint8)
+    for b, n in enumerate(lens):
+        for t, c in ((2, 6.0 * keys), (n - 1 - q_len // 2, 20.0 * keys)):
+            if 0 <= t < n and (t != 2 or n > 3):
+                par[int(args[3][b, t // 16]), t % 16, ..., 0] = c
+    args[1][..., 64:] = par.flatten(-2).contiguous().view(torch.uint8)
+    out, lse, (weight, reach) = Q.attend(args[0], *args[1:4], args[4].tolist(), args[5].tolist(), SCALE, True)
+    assert bool((lse.abs() < 2.0 ** 127).all() | lse.isinf().any())
+    got = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, True)
+    o, l = got[0].double(), got[1].double().view(lse.shape)
+    half = torch.finfo(args[0].dtype).eps / 2
+    # Large scores: weights of 1 and of e^-1000 and less, so that only the value's rounding (2^-11) and the output's are left.
+    # Rows too early to see the third token, and small scores: as everywhere.
+    sees = torch.cat([torch.arange(n - q_len, n, device="cuda") >= 2 for n in lens])[:, None]
+    ds = torch.where(sees & (size > 1e3), 0.0, reach * 17 * 2.0 ** -23 + 2.0 ** -21)
+    tol = out.abs() * half * 1.01 + (2 * 2.0 ** -11 + 2 * ds)[..., None] * 1.05 * weight + 2.0 ** -25
+    assert bool(o.isfinite().all()), int(o.isnan().sum())
+    assert bool(((o - out).abs() <= tol).all()), float(((o - out).abs() / tol).max())
+    seen = lse.isfinite()
+    assert torch.equal(l.isfinite(), seen)
+    tol = reach * 17 * 2.0 ** -23 + 2.0 ** -21 + 2.0 ** -22 * lse.abs() + 2.0 ** -20
+    assert bool(((l - lse).abs() <= tol)[seen].all()), float(((l - lse).abs() / tol)[seen].max())

@@ -342,13 +342,13 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
     row_of(rows - 1, token);
     const int most = unit.limit(walk.q, walk.kv, token);  // tokens from here on by none
 
-    float o[kN][8][4], sum[kN][2], ref[kN][2], bar_at[kN][2];
+    float o[kN][8][4], sum[kN][2], less[kN][2], bar_at[kN][2];  // less: the negative of the score whose weight is 2^6
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) sum[n][k] = ref[n][k] = 0.f, bar_at[n][k] = -INFINITY;
+      for (int k = 0; k < 2; ++k) sum[n][k] = less[n][k] = 0.f, bar_at[n][k] = -INFINITY;
     }
 
     // a tile: 32 tokens from `tok` on, their keys at shared address `ka`
@@ -443,9 +443,8 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             if (top > bar_at[n][k]) {
               // weights up to 2^6 from here on, to 2^14 before the next move: fp16 holds 2^-24 of them
-              const float now = fmaf(top, mult[n][k], -6.f);
-              const float f = bar_at[n][k] == -INFINITY ? 0.f : ex2(ref[n][k] - now);
-              ref[n][k] = now, bar_at[n][k] = top + 8.f / mult[n][k];
+              const float f = bar_at[n][k] == -INFINITY ? 0.f : ex2((-less[n][k] - top) * mult[n][k]);
+              less[n][k] = -top, bar_at[n][k] = __fadd_rd(top, 8.f / mult[n][k]);
               sum[n][k] *= f;
 #pragma unroll
               for (int j = 0; j < 8; ++j) o[n][j][k] *= f, o[n][j][2 + k] *= f;
@@ -460,7 +459,11 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
         for (int n = 0; n < kN; ++n) {
           float e[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) e[k] = ex2(fmaf(s[u][n][k], mult[n][k & 1], -ref[n][k & 1]));
+          for (int k = 0; k < 4; k += 2) {
+            // (the difference first: beside a large product the rounding of a reference would be the weight)
+            fadd2(s[u][n][k], s[u][n][k + 1], less[n][0], less[n][1]);
+            e[k] = ex2(fmaf(s[u][n][k], mult[n][0], 6.f)), e[k + 1] = ex2(fmaf(s[u][n][k + 1], mult[n][1], 6.f));
+          }
           sum[n][0] += e[0] + e[2], sum[n][1] += e[1] + e[3];
           pf[n][0] = trans8x8(pack2<true>(e[0], e[1]));
           pf[n][1] = trans8x8(pack2<true>(e[2], e[3]));
@@ -535,8 +538,9 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
         const int r = n * 8 + 2 * t + k;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const float lse = l == 0.f ? -INFINITY : (ref[n][k] + log2f(l)) * 0.6931471805599453f;
+        float inv = l == 0.f ? 0.f : 1.f / l;
+        float lse = l == 0.f ? -INFINITY : fmaf(-less[n][k], mult[n][k] * 0.6931471805599453f, (log2f(l) - 6.f) * 0.6931471805599453f);
+        if (lse == INFINITY) inv = lse = __int_as_float(0x7fffffff);  // a score beyond fp32
         if (r >= rows) continue;
         int i;
         const int64_t row = row_of(r, i);

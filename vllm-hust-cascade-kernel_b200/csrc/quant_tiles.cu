@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       const bool real = row < rows;
       const int64_t out_row = real ? (walk.tok + i) * p.num_heads + h * p.group + (at - i * p.group) : 0;
       const int mine = tile_steps(unit, walk, t);
-      float mult = 0.f, mx = -INFINITY, l = 0.f;
+      float mult = 0.f, ref = -INFINITY, bar_at = -INFINITY, gap = 0.f, l = 0.f;  // ref: the score whose weight is 2^6
       if (mine > 0) {
         // ------------------------------------------------------------ query
         const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.query) + out_row * kHeadDim);
@@ -418,6 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         }
         // (not 0, nor NaN: a masked score, -inf, stays -inf)
         mult = fmaxf(__int_as_float((127 - up) << 23) * (p.scale * 1.4426950408889634f), 1e-37f);
+        gap = 8.f / mult;
         fence_proxy_async_smem();
         tmem_wait_st();
         tc_fence_before();
@@ -444,12 +445,12 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 64; e += 2)
           a[(e >> 1) & 3] = fmax3f_nan(a[(e >> 1) & 3], __uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1]));
-        const float top = fmax3f_nan(fmax3f_nan(a[0], a[1], a[2]), a[3], a[3]) * mult;
+        const float top = fmax3f_nan(fmax3f_nan(a[0], a[1], a[2]), a[3], a[3]);
         // weights up to 2^6 after a move, to 2^14 before the next: fp16 holds 2^-24 of them
-        const bool move = top > mx + 14.f;
-        const float dm = move ? ex2(mx - (top - 6.f)) : 1.f;  // 0 while nothing has been seen
-        if (move) mx = top - 6.f;
-        const float neg = mx == -INFINITY ? 0.f : -mx;
+        const bool move = top > bar_at;
+        const float dm = move ? ex2((ref - top) * mult) : 1.f;  // 0 while nothing has been seen
+        if (move) ref = top, bar_at = __fadd_rd(top, gap);
+        const float less = ref == -INFINITY ? 0.f : -ref;
         if (j > 0 && __any_sync(0xffffffffu, move)) {
           // the scores of step j come after P V of step j - 1: the output is at rest
 #pragma unroll 1
@@ -467,9 +468,12 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 64; e += 4) {
           const uint32_t* s = &x[e >> 5][e & 31];
-          float y0, y1, y2, y3;
-          ffma2_bcast(y0, y1, __uint_as_float(s[0]), __uint_as_float(s[1]), mult, neg);
-          ffma2_bcast(y2, y3, __uint_as_float(s[2]), __uint_as_float(s[3]), mult, neg);
+          // (the difference first: beside a large product the rounding of a reference would be the weight)
+          float y0 = __uint_as_float(s[0]), y1 = __uint_as_float(s[1]), y2 = __uint_as_float(s[2]), y3 = __uint_as_float(s[3]);
+          fadd2(y0, y1, less, less);
+          fadd2(y2, y3, less, less);
+          ffma2_bcast(y0, y1, y0, y1, mult, 6.f);
+          ffma2_bcast(y2, y3, y2, y3, mult, 6.f);
           y0 = ex2(y0), y1 = ex2(y1), y2 = ex2(y2), y3 = ex2(y3);
           fadd2(r0, r1, y0, y1);
           fadd2(r2, r3, y2, y3);
@@ -489,9 +493,10 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       if (mine > 0) {
         mbar_wait_warp(&aux->o_final[t], pieces++ & 1);
         tc_fence_after();
-        if (mx > -INFINITY || l != l) {  // (a NaN is no maximum)
+        if (ref > -INFINITY || l != l) {  // (a NaN is no maximum)
           inv = 1.f / l;
-          lse = (mx + log2f(l)) * 0.6931471805599453f;
+          lse = fmaf(ref, mult * 0.6931471805599453f, (log2f(l) - 6.f) * 0.6931471805599453f);
+          if (lse == INFINITY) inv = lse = __int_as_float(0x7fffffff);  // a score beyond fp32
         }
       }
       const bool whole = walk.starts && walk.ends, aborted = __any_sync(0xffffffffu, cta_aborted());
