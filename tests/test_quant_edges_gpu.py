@@ -69,3 +69,33 @@ def test_scores_of_any_size(q_len, KVH, G, lens, dtype, size, keys):
     assert torch.equal(l.isfinite(), seen)
     tol = reach * 17 * 2.0 ** -23 + 2.0 ** -21 + 2.0 ** -22 * lse.abs() + 2.0 ** -20
     assert bool(((l - lse).abs() <= tol)[seen].all()), float(((l - lse).abs() / tol)[seen].max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("power", [-10, -13, -14, -17, -20, -22, -24])
+@pytest.mark.parametrize("q_len,KVH,G", [(1, 2, 4), (4, 1, 5), (40, 1, 4), (64, 2, 5)])
+def test_keys_of_small_scales(q_len, KVH, G, power, dtype):
+    """Key scales down to fp16's smallest number, met by queries that make scores of ordinary size of them.
+
+    Few query rows: mma.sync aligns its products as if an operand below 2^-14 were 2^-14 (measured; the tiles' products do
+    not), so each of a row's 16 products of centres and scales is cut at 2^-23 of 2^-14 times the largest 7.5 |sum q|."""
+    import torch
+    Hh.need_cuda()
+    lens = [100, 333]
+    args = _inputs(lens, [q_len] * 2, KVH, G, 16, dtype, seed=-power, loud=False)
+    par = args[1][..., 64:].contiguous().view(torch.float16).unflatten(-1, (4, 2))
+    used = par[..., 1].isfinite()
+    g = torch.Generator(device="cuda").manual_seed(power + 100)
+    scale = (1 + torch.rand(used.shape, generator=g, device="cuda")) * 2.0 ** power
+    centre = torch.randn(used.shape, generator=g, device="cuda") * 2.0 ** power
+    par[..., 0][used], par[..., 1][used] = centre.half()[used], scale.half()[used]
+    args[1][..., 64:] = par.flatten(-2).contiguous().view(torch.uint8)
+    most = 2.0 ** 14 if dtype == "fp16" else 2.0 ** 21
+    q = args[0].float() * min(most, 2.0 ** (-2 - power))
+    args[0].copy_((q.clamp(-6e4, 6e4) if dtype == "fp16" else q).to(args[0].dtype))
+    scale = SCALE * max(1.0, 2.0 ** (-2 - power) / most)
+    want = out, lse, (size, reach) = Q.attend(args[0], *args[1:4], args[4].tolist(), args[5].tolist(), scale, True)
+    if q_len * G <= 32:
+        sums = args[0].double().unflatten(-1, (4, 32)).sum(-1).abs().amax(-1)
+        want = out, lse, (size, reach + 2.0 ** 20 * scale * 16 * 2.0 ** -37 * 7.5 * sums)
+    _close(Hh.ops().cascade_quant_decode(*args, q_len, scale, True), args, True, scale, want)

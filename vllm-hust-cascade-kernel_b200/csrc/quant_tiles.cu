@@ -6,8 +6,9 @@
 // A block of 256 query rows (token and head of the group, in that order) of one
 // request and kv head are two tiles of 128 that share the unpacked tokens, 128 at a
 // time. Keys stay exact: with a group's centre c and scale s a value is
-// (code - 7.5) s + c, and s is split in two, s = s1 + s2, of 7 and 4 significant
-// bits, so that (code - 7.5) s1 and (code - 7.5) s2 are fp16 numbers; the centres
+// (code - 8) s + s / 2 + c, and s is split in two, s = s1 + s2, of 7 and 4 significant
+// bits, so that the whole numbers code - 8 times s1 and s2 are fp16 numbers for every s
+// ((code - 7.5) s has a bit more than the smallest of them); the centres and scales
 // meet the groups' sums of the query in a product of 16 more columns. 272 columns for
 // 128 (a key rounded to fp16 would be 2^-11 off in each of its 128 products, the
 // scores' sums in fp32 are not). Queries are fp16 too, each row times a power of two. Values are
@@ -82,10 +83,12 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t b
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
   return y;
 }
-// the codes of a word, less 7.5: pairs of values (n, n + 4), n = 0..3
+// the codes of a word, less 7.5 or (keys) 8: pairs of values (n, n + 4), n = 0..3
+template <bool kKeys>
 __device__ __forceinline__ void codes(uint32_t w, __half2 (&c)[4]) {
   const uint32_t lo = w << 1, hi = w >> 7, magic = 0x64006400u;
-  const __half2 a = __float2half2_rn(0.5f), b = __float2half2_rn(-519.5f), d = __float2half2_rn(0.03125f), e = __float2half2_rn(-39.5f);
+  const float less = kKeys ? 8.f : 7.5f;
+  const __half2 a = __float2half2_rn(0.5f), b = __float2half2_rn(-512.f - less), d = __float2half2_rn(0.03125f), e = __float2half2_rn(-32.f - less);
   c[0] = __hfma2(as_half2(and_or(lo, 0x001E001Eu, magic)), a, b);
   c[1] = __hfma2(as_half2(and_or(lo, 0x01E001E0u, magic)), d, e);
   c[2] = __hfma2(as_half2(and_or(hi, 0x001E001Eu, magic)), a, b);
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             __half2 cd[4];
-            codes(ws[k], cd);
+            codes<true>(ws[k], cd);
             const __half2 s = __high2half2(as_half2(ps[k]));
             const __half2 s1 = as_half2(as_u32(s) & 0xFFF0FFF0u), s2 = __hsub2(s, s1);
             uint32_t x[4], y[4];
@@ -233,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
             *reinterpret_cast<uint4*>(dst + 2 * kPart) = make_uint4(y[0], y[1], y[2], y[3]);
           }
           if (t < 2) {
-            // the columns of centres (and scales, which meet zeros). A value that is NaN makes its token's scores NaN, and
+            // the columns of centres and scales. A value that is NaN makes its token's scores NaN, and
             // is 0 itself (below): rows that do not see it keep their sums.
             const uint4 pv = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + kQuantCodes);
             if (odd_par(pv.x) || odd_par(pv.y) || odd_par(pv.z) || odd_par(pv.w)) par.x = 0x7fffu;
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             __half2 cd[4];
-            codes(ws[k], cd);
+            codes<false>(ws[k], cd);
             const uint32_t pk = tok + r >= walk.kv || odd_par(ps[k]) ? 0u : ps[k];
             const __half2 s = __high2half2(as_half2(pk)), off = __low2half2(as_half2(pk));
             uint32_t x[4];
@@ -411,10 +414,16 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
             for (int e = 0; e < 4; ++e) qw[k * 4 + e] = pack2<true>(y[e], y[e + 4]);
           }
           tmem_st_32x32b_x32(qcol + half * 32, qw);
-          const uint32_t z0 = pack2<true>(sums[0], 0.f), z1 = pack2<true>(sums[1], 0.f);
-          *reinterpret_cast<uint2*>(z + half * 8) = make_uint2(z0, z1);
-          *reinterpret_cast<uint2*>(z + 2048 + half * 8) = make_uint2(pack2<true>(sums[0] - __low2float(as_half2(z0)), 0.f),
-                                                                      pack2<true>(sums[1] - __low2float(as_half2(z1)), 0.f));
+          // a centre meets the sum, a scale half of it, each as two fp16 numbers
+          uint32_t z0[2], z1[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            z0[k] = pack2<true>(sums[k], 0.5f * sums[k]);
+            const float2 hi = __half22float2(as_half2(z0[k]));
+            z1[k] = pack2<true>(sums[k] - hi.x, 0.5f * sums[k] - hi.y);
+          }
+          *reinterpret_cast<uint2*>(z + half * 8) = make_uint2(z0[0], z0[1]);
+          *reinterpret_cast<uint2*>(z + 2048 + half * 8) = make_uint2(z1[0], z1[1]);
         }
         // (not 0, nor NaN: a masked score, -inf, stays -inf)
         mult = fmaxf(__int_as_float((127 - up) << 23) * (p.scale * 1.4426950408889634f), 1e-37f);
