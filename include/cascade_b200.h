@@ -471,7 +471,8 @@ CASCADE_API int cascade_quant_read(const void *key_cache, const void *value_cach
  * kv_len, and what only the causal mask hides, is never used, NaN included.
  * A NaN in a key that a row sees, or a score of +infinity, makes its out and
  * lse NaN; a NaN in a value at least the group's 32 values of out. A query row
- * with a NaN or an infinity that sees a token gives NaN.
+ * with a NaN or an infinity that sees a token gives NaN (a value of 2^126 / scale
+ * and more may, too).
  *   query  [num_tokens, num_heads, 128] in `dtype`, contiguous, 16-byte aligned
  * The other fields, the lengths and the block ids are as in cascade_latent_attn_t.
  * A batch of 2^30 and more is unsupported. */

@@ -99,3 +99,26 @@ def test_keys_of_small_scales(q_len, KVH, G, power, dtype):
         sums = args[0].double().unflatten(-1, (4, 32)).sum(-1).abs().amax(-1)
         want = out, lse, (size, reach + 2.0 ** 20 * scale * 16 * 2.0 ** -37 * 7.5 * sums)
     _close(Hh.ops().cascade_quant_decode(*args, q_len, scale, True), args, True, scale, want)
+
+
+@pytest.mark.parametrize("dtype,size,keys", [("bf16", 1.7e35, 1.0), ("bf16", 1e36, 1.0), ("bf16", 5e37, 2.0 ** -8),
+                                             ("bf16", 3e38, 2.0 ** -10), ("bf16", 3.3e38, 2.0 ** -14)])
+@pytest.mark.parametrize("q_len,KVH,G,lens", [(1, 2, 4, [40, 1000, 7]), (4, 1, 5, [333, 90]), (4, 2, 8, [700, 31]),
+                                              (40, 1, 4, [100, 2000])])
+def test_the_largest_queries(q_len, KVH, G, lens, dtype, size, keys):
+    """Queries up to bf16's largest number whose scores are finite."""
+    test_scores_of_any_size(q_len, KVH, G, lens, dtype, size, keys)
+
+
+@pytest.mark.parametrize("q_len,G", [(1, 4), (4, 5), (4, 8), (40, 4)])
+def test_scores_beyond_fp32_make_their_rows_nan(q_len, G):
+    """And leave the other rows as they are."""
+    import torch
+    Hh.need_cuda()
+    args = _inputs([100, 333], [q_len] * 2, 2, G, 16, seed=33)
+    clean = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, True)
+    args[0][q_len :, 1] = 3e38
+    out, lse = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, True)
+    assert bool(out[q_len:, 1].isnan().all()) and bool(lse.view(2 * q_len, -1)[q_len:, 1].isnan().all())
+    out[q_len:, 1], lse.view(2 * q_len, -1)[q_len:, 1] = clean[0][q_len:, 1], clean[1].view(2 * q_len, -1)[q_len:, 1]
+    assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])

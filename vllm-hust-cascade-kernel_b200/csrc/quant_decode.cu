@@ -11,7 +11,10 @@
 // queries stay exact down to 2^-27 of their row's largest value). One AND per two
 // codes, and a shift per eight. The term of centres and scales is one more product
 // of 16 columns: (c, s) of four groups against sum q and -7.5 sum q, each as two
-// fp16 numbers. fp32 holds every sum.
+// fp16 numbers. fp32 holds every sum. (mma.sync aligns products as if a subnormal
+// operand were 2^-14: where all of a key's centres and scales are that small, sums lose
+// bits, at 2^-24 a score 2^-18 of its sum |q k|. As tf32 products they would not:
+// 128 x 64 heads 169 us for 166, 96 x 16 rows over 4,000 tokens 180 for 172.)
 // Values are converted, (code - 7.5) s + c in one fused multiply-add, rounded to
 // fp16, as P is: fp16 holds 2^-11 of both where bf16 would hold 2^-8.
 //
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
       const float2 hi = __half22float2(as_half2(zf[n][0]));
       zf[n][1] = pack2<true>(z - hi.x, y - hi.y);
       // (not 0, nor NaN: a masked score, -inf, stays -inf)
-      const float m = fmaxf(__int_as_float((127 - up) << 23) * 0x1p24f * (p.scale * 1.4426950408889634f), 1e-37f);
+      const float m = fmaxf(__int_as_float((127 - up) << 23) * (p.scale * 1.4426950408889634f) * 0x1p14f, 1e-37f);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         int i;
@@ -360,18 +363,10 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
         const uint32_t a = ka + (u ? half_off : 0);
         const uint4 wa4 = lds128(a + off_k), wb4 = lds128(a + off_k + kNext);
         const uint4 pa4 = lds128(a + off_kp), pb4 = lds128(a + off_kp + kNext);
-        const uint32_t za = lds32(a + off_kp + 4 * t), zb = lds32(a + off_kp + kNext + 4 * t);
         wa[u][0] = wa4.x, wa[u][1] = wa4.y, wa[u][2] = wa4.z, wa[u][3] = wa4.w;
         wb[u][0] = wb4.x, wb[u][1] = wb4.y, wb[u][2] = wb4.z, wb[u][3] = wb4.w;
         pa[u][0] = pa4.x, pa[u][1] = pa4.y, pa[u][2] = pa4.z, pa[u][3] = pa4.w;
         pb[u][0] = pb4.x, pb[u][1] = pb4.y, pb[u][2] = pb4.z, pb[u][3] = pb4.w;
-        const uint32_t z[4] = {za, zb, za, zb};
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          mma_fresh(s[u][n], z, zf[n][0], zf[n][1]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s[u][n][k] *= 0x1p-10f;
-        }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -399,9 +394,26 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
             float x[4];
             mma_fresh(x, a0[u], q[0], q[1]);
             mma_16816<true>(x, a1[u], q[2], q[3]);
-            s[u][n][0] = fmaf(fa[u], x[0], s[u][n][0]), s[u][n][1] = fmaf(fa[u], x[1], s[u][n][1]);
-            s[u][n][2] = fmaf(fb[u], x[2], s[u][n][2]), s[u][n][3] = fmaf(fb[u], x[3], s[u][n][3]);
+            if (i == 0) {
+              s[u][n][0] = fa[u] * x[0], s[u][n][1] = fa[u] * x[1], s[u][n][2] = fb[u] * x[2], s[u][n][3] = fb[u] * x[3];
+            } else {
+              s[u][n][0] = fmaf(fa[u], x[0], s[u][n][0]), s[u][n][1] = fmaf(fa[u], x[1], s[u][n][1]);
+              s[u][n][2] = fmaf(fb[u], x[2], s[u][n][2]), s[u][n][3] = fmaf(fb[u], x[3], s[u][n][3]);
+            }
           }
+        }
+      }
+      // centres: products of 2^-14 where the codes' are of 2^-24; in the larger unit `mult` holds for queries of any size
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t a = ka + (u ? half_off : 0) + off_kp + 4 * t;
+        const uint32_t za = lds32(a), zb = lds32(a + kNext), z[4] = {za, zb, za, zb};
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          float x[4];
+          mma_fresh(x, z, zf[n][0], zf[n][1]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[u][n][k] = fmaf(s[u][n][k], 0x1p10f, x[k]);
         }
       }
       const uint32_t va = ka + value_off;
