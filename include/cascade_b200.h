@@ -470,7 +470,7 @@ CASCADE_API int cascade_quant_read(const void *key_cache, const void *value_cach
  * Rows that see no token give out = 0 and lse = -inf. What the pages hold past
  * kv_len, and what only the causal mask hides, is never used, NaN included.
  * A NaN in a key that a row sees, or a score of +infinity, makes its out and
- * lse NaN; a NaN in a value at least the group's 32 values of out. A query row
+ * lse NaN; a NaN in a value the group's 32 values of out, and nothing else. A query row
  * with a NaN or an infinity that sees a token gives NaN (a value of 2^126 / scale
  * and more may, too).
  *   query  [num_tokens, num_heads, 128] in `dtype`, contiguous, 16-byte aligned

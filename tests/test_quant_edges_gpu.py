@@ -122,3 +122,33 @@ def test_scores_beyond_fp32_make_their_rows_nan(q_len, G):
     assert bool(out[q_len:, 1].isnan().all()) and bool(lse.view(2 * q_len, -1)[q_len:, 1].isnan().all())
     out[q_len:, 1], lse.view(2 * q_len, -1)[q_len:, 1] = clean[0][q_len:, 1], clean[1].view(2 * q_len, -1)[q_len:, 1]
     assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
+
+
+@pytest.mark.parametrize("which", ["one", "two tokens", "last", "every group"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_len,KVH,G,lens", [(1, 2, 4, [40, 900, 33]), (1, 1, 8, [20000, 64]), (4, 2, 5, [31, 500]), (4, 1, 8, [600]),
+                                              (20, 1, 4, [50, 1000]), (100, 2, 4, [333, 90]), (64, 1, 8, [5000, 700])])
+def test_nan_values_leave_the_log_sum_exp(q_len, KVH, G, lens, causal, which):
+    """A NaN in a value makes its group's 32 values of `out` NaN for the rows that see it, wherever the token lies, and
+    nothing else: the scores do not know it."""
+    import torch
+    Hh.need_cuda()
+    args = _inputs(lens, [q_len] * len(lens), KVH, G, 16, seed=41)
+    clean, lse = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, causal)
+    want = clean.clone().view(len(lens), q_len, KVH, G, 128)
+    for b, n in enumerate(lens):
+        at = {"one": [n // 3], "two tokens": [5, n - 1 - q_len // 2], "last": [n - 1], "every group": [n // 2]}[which]
+        for i, t in enumerate(at):
+            if not 0 <= t < n:
+                continue
+            groups = range(4) if which == "every group" else [(b + 2 * i) % 4]
+            head = (b + i) % KVH
+            for g in groups:
+                args[2][int(args[3][b, t // 16]), t % 16, head, 64 + 4 * g : 68 + 4 * g] = 0xFF
+                first = max(0, t - n + q_len) if causal else 0
+                want[b, first:, head, :, 32 * g : 32 * g + 32] = float("nan")
+    want = want.view(clean.shape)
+    out, again = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, causal)
+    assert torch.equal(again, lse)
+    assert torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))

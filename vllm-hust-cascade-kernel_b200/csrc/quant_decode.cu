@@ -110,8 +110,6 @@ __device__ __forceinline__ __half2 low_code(uint32_t x, uint32_t magic) {
 __device__ __forceinline__ __half2 high_code(uint32_t x, uint32_t magic) {
   return __hfma2(as_half2(and_or(x, 0x01E001E0u, magic)), __float2half2_rn(0.03125f), __float2half2_rn(-39.5f));
 }
-// centre or scale NaN (or infinite) in either half
-__device__ __forceinline__ bool odd_par(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
 
 // d = a b, nothing added
 __device__ __forceinline__ void mma_fresh(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -148,12 +146,14 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
   __shared__ uint64_t full[kWarps][kStages], empty[kWarps][kStages];  // per group
   __shared__ uint64_t stall;
   __shared__ QuantRun found[kWarps];
+  __shared__ uint32_t odd[kWarps];  // a tile whose rows see different tokens held a NaN among its values
   const QuantDecodeLaunch& p = P.L;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem_raw + ((0u - smem_u32(smem_raw)) & 127u);
   pdl_launch_dependents();
   const int group = warp / P.heads, member = warp - group * P.heads;
   const int id = blockIdx.x * P.groups + group, head0 = id % P.head_groups * P.heads, h = head0 + member, c = id / P.head_groups;
+  if (lane == 0) odd[warp] = 0;
   if (lane < kStages && member == 0) {
     mbar_init(&full[group][lane], 1);
     mbar_init(&empty[group][lane], min(P.heads, p.kv_heads - head0));
@@ -418,22 +418,15 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
       }
       const uint32_t va = ka + value_off;
       if constexpr (masked.value) {
-        // a value that is NaN makes the scores of its token NaN, and is 0 itself (below): rows that do not see it keep
-        // their sums
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint32_t at = va + (u ? half_off : 0) + off_kp;
-          const uint4 pa = lds128(at), pb = lds128(at + kNext);
-          const bool na = odd_par(pa.x) || odd_par(pa.y) || odd_par(pa.z) || odd_par(pa.w);
-          const bool nb = odd_par(pb.x) || odd_par(pb.y) || odd_par(pb.z) || odd_par(pb.w);
-          const float nan = __int_as_float(0x7fffffff);
           const int mine = tok + u * 16 + tok_k;
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              s[u][n][k] = mine < lim[n][k] ? (na ? nan : s[u][n][k]) : -INFINITY;
-              s[u][n][2 + k] = mine + Pl::kNext < lim[n][k] ? (nb ? nan : s[u][n][2 + k]) : -INFINITY;
+              s[u][n][k] = mine < lim[n][k] ? s[u][n][k] : -INFINITY;
+              s[u][n][2 + k] = mine + Pl::kNext < lim[n][k] ? s[u][n][2 + k] : -INFINITY;
             }
           }
         }
@@ -488,8 +481,12 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int mine = tok + u * 16 + (j & 1 ? tok_v1 : tok_v0) + (j >> 1) * Pl::kNext;
-            if (mine >= most || odd_par(par[j].x)) par[j].x = 0;
-            if (mine >= most || odd_par(par[j].y)) par[j].y = 0;
+            // (a group of values that is NaN is 0 here, so that rows that do not see it keep their sums)
+            if (mine >= most) par[j].x = par[j].y = 0;
+            const bool bad_x = odd_par(par[j].x), bad_y = odd_par(par[j].y);
+            if (bad_x) par[j].x = 0;
+            if (bad_y) par[j].y = 0;
+            if (bad_x || bad_y) odd[warp] = 1;
           }
         }
 #pragma unroll
@@ -577,6 +574,31 @@ __global__ void __launch_bounds__(32 * Shape<kN>::kWarps, 1) quant_decode_kernel
             dst[0] = make_float4(y[0], y[1], y[2], y[3]);
             dst[1] = make_float4(y[4], y[5], y[6], y[7]);
           }
+        }
+      }
+    }
+    if (*const_cast<volatile uint32_t*>(&odd[warp])) {  // (rarely) which rows see which NaN: those tiles' values are looked at again
+      __syncwarp();
+      int i;
+      const int64_t row = row_of(min(lane, rows - 1), i);
+      const int seen = lane < rows ? unit.limit(walk.q, walk.kv, i) : 0, end = min(most, (walk.t0 + walk.n) * kTok);
+      uint32_t bad = 0;  // bit i: row `lane` sees a NaN in its values' group i
+      for (int tok = max(clean / kTok, walk.t0) * kTok; tok < end; tok += 32) {
+        const uint32_t its = tok + lane < end ? odd_groups(p, walk.b, tok + lane, shift, h) : 0;
+        for (uint32_t who = __ballot_sync(0xffffffffu, its != 0); who; who &= who - 1) {
+          const int l = __ffs(who) - 1;
+          const uint32_t groups = __shfl_sync(0xffffffffu, its, l);
+          if (tok + l < seen) bad |= groups;
+        }
+      }
+      for (int r = 0; r < rows; ++r) {
+        const int64_t to = __shfl_sync(0xffffffffu, row, r);
+        for (uint32_t its = __shfl_sync(0xffffffffu, bad, r); its; its &= its - 1) {
+          const int d = 32 * (__ffs(its) - 1) + lane;
+          if (whole)
+            static_cast<uint16_t*>(p.out)[to * kHeadDim + d] = 0x7fff;  // (of either type)
+          else
+            P.parts.o[(slot + r) * kHeadDim + d] = __int_as_float(0x7fffffff);
         }
       }
     }

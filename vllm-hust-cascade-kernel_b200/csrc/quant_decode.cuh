@@ -186,6 +186,17 @@ struct QuantWalk {
   }
 };
 
+// centre or scale NaN (or infinite) in either half
+__device__ __forceinline__ bool odd_par(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
+// bit i: group i of the value of token `tok` (below the request's length) is NaN
+__device__ __forceinline__ uint32_t odd_groups(const QuantDecodeLaunch& p, int b, int tok, int shift, int h) {
+  const int32_t id = p.block_table[static_cast<int64_t>(b) * p.block_cols + (tok >> shift)];
+  if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(p.num_blocks)) return 0;
+  const int64_t row = (static_cast<int64_t>(id) * p.block_size + (tok & (p.block_size - 1))) * p.kv_heads + h;
+  const uint4 par = __ldg(reinterpret_cast<const uint4*>(p.value + row * kQuantRow + kQuantCodes));
+  return odd_par(par.x) | odd_par(par.y) << 1 | odd_par(par.z) << 2 | odd_par(par.w) << 3;
+}
+
 // row_info of a unit whose first piece is run c's and whose last tile is at `last` of the axis, without its row
 __device__ __forceinline__ int32_t cut_info(const QuantRun& run, int c, int64_t last) {
   const float total = static_cast<float>(run.each * run.runs + run.rest);

@@ -58,6 +58,7 @@ constexpr int kBytes = kOffRaw + kStages * 2 * kRaw;
 struct __align__(16) Aux {
   uint64_t raw_full[kStages], raw_empty[kStages], k_full[2], k_empty[2], v_full[2], v_empty[2];  // per buffer
   uint64_t q_full[2], s_full[2], p_full[2], o_final[2], stall, drain;                                      // per tile
+  uint32_t odd;  // some group of a request's values was NaN
   uint32_t tmem_base;
   QuantRun run;
 };
@@ -77,7 +78,6 @@ using Walk = QuantWalk<kBlock, kTok, kSetup>;
 
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
-__device__ __forceinline__ bool odd_par(uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; }
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
   uint32_t y;
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       mbar_init(&aux->p_full[i], 4);
       mbar_init(&aux->o_final[i], 1);
     }
+    aux->odd = 0;
     mbar_init(&aux->stall, 1);
     mbar_init(&aux->drain, 1);
     fence_mbar_init();
@@ -219,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
         for (int i = turn; i < kTok / 8; i += kUnpackWarps) {
           const int r = i * 8 + g8;
           const uint4 word = *reinterpret_cast<const uint4*>(raw + r * kQuantRow + 16 * t);
-          uint4 par = *reinterpret_cast<const uint4*>(raw + r * kQuantRow + kQuantCodes);
+          const uint4 par = *reinterpret_cast<const uint4*>(raw + r * kQuantRow + kQuantCodes);
           const uint32_t ws[4] = {word.x, word.y, word.z, word.w}, ps[4] = {par.x, par.y, par.z, par.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -236,10 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
             *reinterpret_cast<uint4*>(dst + 2 * kPart) = make_uint4(y[0], y[1], y[2], y[3]);
           }
           if (t < 2) {
-            // the columns of centres and scales. A value that is NaN makes its token's scores NaN, and
-            // is 0 itself (below): rows that do not see it keep their sums.
-            const uint4 pv = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + kQuantCodes);
-            if (odd_par(pv.x) || odd_par(pv.y) || odd_par(pv.z) || odd_par(pv.w)) par.x = 0x7fffu;
+            // the columns of centres and scales
             *reinterpret_cast<uint4*>(smem + kOffZk + buf * 2048 + t * 1024 + r * 16) = par;
           }
         }
@@ -253,6 +251,8 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
           const uint4 word = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + 16 * t);
           const uint4 par = *reinterpret_cast<const uint4*>(raw + kRaw + r * kQuantRow + kQuantCodes);
           const uint32_t ws[4] = {word.x, word.y, word.z, word.w}, ps[4] = {par.x, par.y, par.z, par.w};
+          // (a group of values that is NaN is 0 here, so that rows that do not see it keep their sums)
+          if (tok + r < walk.kv && (odd_par(ps[0]) || odd_par(ps[1]) || odd_par(ps[2]) || odd_par(ps[3]))) aux->odd = 1;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             __half2 cd[4];
@@ -499,6 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
       }
       // ----------------------------------------------------------- output
       float inv = 0.f, lse = -INFINITY;
+      uint32_t bad = 0;  // bit i: this row sees a NaN in the values' group i
       if (mine > 0) {
         mbar_wait_warp(&aux->o_final[t], pieces++ & 1);
         tc_fence_after();
@@ -506,6 +507,18 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
           inv = 1.f / l;
           lse = fmaf(ref, mult * 0.6931471805599453f, (log2f(l) - 6.f) * 0.6931471805599453f);
           if (lse == INFINITY) inv = lse = __int_as_float(0x7fffffff);  // a score beyond fp32
+        }
+        if (*reinterpret_cast<volatile uint32_t*>(&aux->odd)) {  // (rarely) which rows see which: the piece's values are looked at again
+          const int shift = __ffs(p.block_size) - 1, end = min(walk.kv, (walk.t0 + mine) * kTok);
+          for (int tok = walk.t0 * kTok; tok < end; tok += 32) {
+            uint32_t odd = 0;
+            if (tok + lane < end) odd = odd_groups(p, walk.b, tok + lane, shift, h);
+            for (uint32_t who = __ballot_sync(0xffffffffu, odd != 0); who; who &= who - 1) {
+              const int l = __ffs(who) - 1;
+              const uint32_t its = __shfl_sync(0xffffffffu, odd, l);
+              if (tok + l - walk.t0 * kTok < lim) bad |= its;
+            }
+          }
         }
       }
       const bool whole = walk.starts && walk.ends, aborted = __any_sync(0xffffffffu, cta_aborted());
@@ -527,12 +540,13 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
 #pragma unroll 1
         for (int g = 0; g < 4; ++g) {  // 32 values
           uint32_t o[32] = {};
+          const float by = bad >> g & 1 ? __int_as_float(0x7fffffff) : inv;
           if (mine > 0) {
             tmem_ld_32x32b_x32(ocol + g * 32, o);
             tmem_wait_ld();
           }
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+          for (int e = 0; e < 32; ++e) o[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * by);
           auto y = [&](int q, int n) { return __uint_as_float(o[q * 8 + n]); };
           if (whole) {
 #pragma unroll
