@@ -152,3 +152,30 @@ def test_nan_values_leave_the_log_sum_exp(q_len, KVH, G, lens, causal, which):
     assert torch.equal(again, lse)
     assert torch.equal(out.isnan(), want.isnan())
     assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("q_lens", [[36, 200], [36, 100, 300]])
+def test_units_that_take_longer_than_a_tenth_of_a_second(q_lens):
+    """Requests of 8 million cached tokens (one page over and over) with at most 128 query rows, then one with more, in the same run of a
+    CTA: the second half of the last one's rows wait while the others are worked on. Attention over r copies of the
+    tokens is attention over the tokens, its log-sum-exp ln r more.
+
+    Tolerance: sums of 8 million terms in fp32, 16 (values) or 64 (weights) at a time, each addition off by at most 2^-23
+    (the tensor cores' may truncate) or 2^-24 of the sum: (2^23 / 16) 2^-23 + (2^23 / 64) 2^-24 = 0.0703 of sum p |v|."""
+    import torch
+    Hh.need_cuda()
+    page, KVH, cols = 512, 148, 1 << 14
+    n = len(q_lens)
+    q, kc, vc, table, qs, lens = _inputs([page] * n, q_lens, KVH, 1, page, "bf16", seed=51)
+    out, lse, (size, reach) = Q.attend(q, kc, vc, table, q_lens, [page] * n, SCALE, False)
+    table = table[:, :1].repeat(1, cols)
+    long = torch.tensor([page * cols] * (n - 1) + [page], device="cuda")
+    got, got_l = Hh.ops().cascade_quant_decode(q, kc, vc, table, qs, long, 0, SCALE, False)
+    assert Hh.capi().device_error() == 0
+    copies = torch.repeat_interleave(long // page, qs)
+    off = torch.where(copies > 1, page * cols / 16 * 2.0 ** -23 + page * cols / 64 * 2.0 ** -24, 0.0)[:, None]
+    ds = reach * 2.0 ** -20 + 2.0 ** -21
+    tol = out.abs() * 2.0 ** -8 * 1.01 + (2 * 2.0 ** -11 + 2 * ds + off)[..., None] * 1.05 * size + 2.0 ** -25
+    assert bool(((got.double() - out).abs() <= tol).all())
+    lse = lse + torch.log(copies.double())[:, None]
+    assert bool(((got_l.double().view(lse.shape) - lse).abs() <= ds + off * 1.05 + 2.0 ** -22 * lse.abs() + 2.0 ** -18 * 10).all())

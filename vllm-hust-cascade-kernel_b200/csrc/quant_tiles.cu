@@ -115,7 +115,6 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
   pdl_launch_dependents();
 
   if (tid == 0) {
-    cta_wait_init(static_cast<uint64_t>(p.wait_limit_us) * 1000);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&aux->raw_full[i], 1);
       mbar_init(&aux->raw_empty[i], kUnpackWarps);
@@ -143,7 +142,13 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
   }
   if (warp == 9) {
     const QuantRun r = find_run<kBlock, kTok, kSetup>(unit, c, P.parts.runs);
-    if (lane == 0) aux->run = r;
+    if (lane == 0) {
+      aux->run = r;
+      // The second tile waits while units without rows for it are worked on, all of the run perhaps: 1.6 us a step
+      // (measured); requests without query tokens are passed by one after the other.
+      const uint64_t us = p.wait_limit_us ? p.wait_limit_us : kWaitLimitNs / 1000 + 4 * (r.end - r.begin) + 2ull * p.batch;
+      cta_wait_init(us * 1000);
+    }
   }
   if (warp == 10 && p.q_len == 0) {  // rows of tokens that are no request's: nothing to merge
     int64_t own = 0;
