@@ -179,3 +179,40 @@ def test_units_that_take_longer_than_a_tenth_of_a_second(q_lens):
     assert bool(((got.double() - out).abs() <= tol).all())
     lse = lse + torch.log(copies.double())[:, None]
     assert bool(((got_l.double().view(lse.shape) - lse).abs() <= ds + off * 1.05 + 2.0 ** -22 * lse.abs() + 2.0 ** -18 * 10).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_len,G", [(5, 5), (4, 7), (31, 1), (4, 8), (1, 32), (25, 1)])
+@pytest.mark.parametrize("KVH", [1, 2, 3, 8])
+def test_four_blocks_of_query_rows(KVH, q_len, G, causal, dtype):
+    """25 to 32 query rows per request and kv head, in units that are whole (the short ones) and cut."""
+    import torch
+    Hh.need_cuda()
+    args = _inputs([33, 5, 3000, 700], [q_len] * 4, KVH, G, 16, dtype, seed=KVH)
+    got = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, causal)
+    _close(got, args, causal)
+    assert Hh.capi().device_error() == 0
+
+
+@pytest.mark.parametrize("KVH,q_len,G", [(5, 3, 3), (6, 2, 5), (10, 4, 4), (7, 1, 16), (18, 4, 5), (18, 3, 8), (9, 1, 32), (11, 8, 3), (70, 2, 8)])
+def test_kv_heads_that_fill_no_group(KVH, q_len, G):
+    """The last group of kv heads that share tiles is smaller than the others, with two, three and four blocks of rows."""
+    Hh.need_cuda()
+    args = _inputs([200, 1, 1500], [q_len] * 3, KVH, G, 32, seed=KVH + G)
+    got = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, True)
+    _close(got, args, True)
+    assert Hh.capi().device_error() == 0
+
+
+@pytest.mark.parametrize("KVH", [1, 3, 8])
+@pytest.mark.parametrize("q_lens", [[7, 7, 7, 6], [1, 26, 0, 1], [20, 1, 4, 1, 9, 7], [100, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1, 1]])
+def test_query_lengths_whose_mean_is_four_blocks(q_lens, KVH):
+    """Lengths on the device: 25 to 32 rows in the mean, from none to 400 in a request."""
+    Hh.need_cuda()
+    lens = [(i * 611 + 40) % 2000 for i in range(len(q_lens))]
+    args = _inputs(lens, q_lens, KVH, 4, 64, "fp16", seed=61)
+    assert 24 < sum(q_lens) * 4 / len(q_lens) <= 32
+    got = Hh.ops().cascade_quant_decode(*args, 0, SCALE, True)
+    _close(got, args, True)
+    assert Hh.capi().device_error() == 0
