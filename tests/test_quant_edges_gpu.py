@@ -216,3 +216,32 @@ def test_query_lengths_whose_mean_is_four_blocks(q_lens, KVH):
     got = Hh.ops().cascade_quant_decode(*args, 0, SCALE, True)
     _close(got, args, True)
     assert Hh.capi().device_error() == 0
+
+
+def test_write_with_every_scale():
+    """Groups of every fp16 scale up to the largest that values of +-32768 give, their values next to the borders between codes:
+    the bytes are the definition's."""
+    import torch
+    Hh.need_cuda()
+    hi = torch.arange(1, 0x7800 + 1, dtype=torch.int16).view(torch.float16)          # positive fp16 numbers up to 32768
+    low = torch.cat([hi, torch.arange(2, 0x7800 + 1, dtype=torch.int16).view(torch.float16), hi[-1:]])
+    hi = hi.repeat(2)
+    # (hi, -hi) and (hi, -the next): 2 hi / 15 and what lies between two of them
+    scale = ((hi.float() + low.float()) / np.float32(15)).half()
+    want = torch.arange(1, int(scale.max().view(torch.int16)) + 1, dtype=torch.int16).view(torch.float16)
+    assert bool(torch.isin(want.view(torch.int16), scale.view(torch.int16)).all())
+    centre = ((hi.float() - low.float()) * 0.5).half().double()
+    border = centre[:, None] + (torch.arange(15) - 7.0).double() * scale.double()[:, None]     # between codes n and n + 1
+    near = border.half()
+    step = torch.where(near.double() > border, -1, 1) * torch.where(near.double() < 0, -1, 1)   # to the border's other side
+    bits = near.view(torch.int16)
+    other = torch.where(bits & 0x7FFF == 0, bits, (bits + step.short())).view(torch.float16)
+    x = torch.cat([hi[:, None], -low[:, None], near, other], 1)
+    x = torch.minimum(torch.maximum(x, -low[:, None]), hi[:, None])
+    x = x[: x.shape[0] // 4 * 4].reshape(-1, 1, 128).contiguous().cuda()
+    x = torch.cat([x, x.flip(0)[:1]]) if x.shape[0] % 2 else x
+    T = x.shape[0]
+    kc, vc = (torch.zeros((T // 16 + 1, 16, 1, 80), dtype=torch.uint8, device="cuda") for _ in range(2))
+    Hh.ops().cascade_quant_write(x, x.flip(0), kc, vc, torch.arange(T, device="cuda"))
+    want = Q.pack(x)
+    assert torch.equal(kc.view(-1, 1, 80)[:T].cpu(), want) and torch.equal(vc.view(-1, 1, 80)[:T].cpu(), want.flip(0))

@@ -77,7 +77,8 @@ __device__ __forceinline__ float fifteenth(float x) {
   const float by = 1.f / 15.f, q = __fmul_rn(x, by);
   return __fmaf_rn(__fmaf_rn(-15.f, q, x), by, q);
 }
-// 1 / s rounded to nearest for every positive fp16 number s (compared over all of them): one Newton step.
+// 1 / s, to nearest where a code depends on it (tested with every positive fp16 scale, values next to the codes' borders): one
+// Newton step.
 __device__ __forceinline__ float reciprocal(float s) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(s));
