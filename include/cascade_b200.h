@@ -267,7 +267,8 @@ CASCADE_API int cascade_probe_hbm_read(const void *src, size_t bytes, int32_t mo
  * Neither path reads back to the host, so both can be captured in a graph.
  * A block id outside [0, num_blocks) reads as zeros and sets (word & 2) of
  * cascade_device_error(). The limit of the kernels' bounded waits is 100 ms and
- * 4 us per 64 tokens of the block table's columns. */
+ * 4 us per 64 tokens of the block table's columns. A batch of 2^30 and more is
+ * unsupported. */
 typedef struct cascade_latent_attn {
   const void *query;
   const void *cache;
@@ -475,9 +476,8 @@ CASCADE_API int cascade_quant_read(const void *key_cache, const void *value_cach
  * and more may, too).
  *   query  [num_tokens, num_heads, 128] in `dtype`, contiguous, 16-byte aligned
  * The other fields, the lengths and the block ids are as in cascade_latent_attn_t.
- * A batch of 2^30 and more is unsupported. The limit of the kernels' bounded waits
- * is 100 ms and, with many query rows, 4 us per 64 tokens that a CTA reads and 2 us
- * per request. */
+ * The limit of the kernels' bounded waits is 100 ms and, with many query rows, 4 us
+ * per 64 tokens that a CTA reads and 2 us per request. */
 typedef struct cascade_quant_attn {
   const void *query;
   const void *key_cache;

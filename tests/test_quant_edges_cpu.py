@@ -1,4 +1,4 @@
-"""CPU-only checks of sizes that the 4-bit cache's entry points have to refuse."""
+"""CPU-only checks of sizes that attention over the 4-bit and the latent cache has to refuse."""
 import ctypes
 
 import pytest
@@ -17,3 +17,14 @@ def test_decode_refuses_batches_whose_steps_wrap(batch):
     assert lib.cascade_quant_decode_workspace_size(ctypes.byref(p)) == 0
     p.batch = (1 << 30) - 1
     assert lib.cascade_quant_decode(ctypes.byref(p), None, None, None, 0, None) != C.OK and "null device pointer" in C.last_error()
+
+
+@pytest.mark.parametrize("batch", [(1 << 30), (1 << 31) - 1])
+def test_latent_decode_refuses_batches_whose_steps_wrap(batch):
+    from cascade_kernel import capi as C
+    shape = dict(num_tokens=3, num_heads=16, latent_dim=512, rope_dim=64, num_blocks=100, block_size=64, batch=batch, block_cols=0)
+    lib = C.load()
+    p = C.latent_desc(None, None, None, None, None, 0, 0.1, True, shape=shape)
+    assert lib.cascade_latent_decode(ctypes.byref(p), None, None, None, 0, None) != C.OK and "too large" in C.last_error()
+    p.batch = (1 << 30) - 1
+    assert lib.cascade_latent_decode(ctypes.byref(p), None, None, None, 0, None) != C.OK and "null device pointer" in C.last_error()

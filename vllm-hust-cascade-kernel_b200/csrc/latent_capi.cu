@@ -20,7 +20,8 @@ int check_decode(const cascade_latent_attn_t* p, const char* op) {
     return fail(CASCADE_ERR_INVALID, "%s: negative size", op);
   if (p->q_seqlen_value < 0)
     return fail(CASCADE_ERR_INVALID, "%s: q_seqlen_value must be >= 0 (0 = per request)", op);
-  if (p->batch > kI32 || p->q_seqlen_value > kI32)  // their product has to hold in 64 bits
+  // their product has to hold in 64 bits, and the kernels' steps from request to request in 32
+  if (p->batch > kI32 / 2 || p->q_seqlen_value > kI32)
     return fail(CASCADE_ERR_UNSUPPORTED, "%s: problem too large for 32-bit row indices", op);
   if (p->q_seqlen_value > 0 && p->num_tokens != p->batch * p->q_seqlen_value)
     return fail(CASCADE_ERR_INVALID, "%s: with q_seqlen_value=%lld, query.size(0) must equal batch * q_seqlen_value",
