@@ -45,7 +45,7 @@ constexpr int kThreads = 16 * 32;
 constexpr int kUnpackWarps = 7;
 constexpr int kStages = 4;                       // steps loaded ahead, less one
 constexpr int kRaw = kTok * kQuantRow;           // keys or values of a step as they lie
-constexpr int kStageOut = 32768;                 // a tile's output on its way
+constexpr int kStageOut = 4 * 4096;              // a tile's output on its way: 128 bytes of each row of a warp's
 constexpr int kPart = 8192;                      // of keys or values: 64 tokens x 64 values
 constexpr int kOffOut = 0;                       // [tile]
 constexpr int kOffK = kOffOut + 2 * kStageOut;   // [buffer][part of the scale][64 values' group][token]
