@@ -11,8 +11,11 @@
 // reach. The batches whose maximum reaches it are read again (from L2, a few more
 // than `top` of them, a lane per entry), their entries that reach it are ordered by
 // counting. A bound is a (logit, index) pair, so equal logits need no care but
-// where a thread hides very many entries: then the CTA takes one maximum after the
-// other.
+// where a thread hides very many entries, or fewer are above -inf (or a mask's lowest
+// value) than the bound asks of each warp: then the CTA takes one maximum after the
+// other (50 entries left of 128,256, 20 alternatives: 4 rows 76 us, 128 rows 656).
+// A batch with a -inf is summed twice, and a row whose token is -inf is read by single
+// logits: 128 rows without alternatives 40 to 44 us for 14.
 //
 // Bound by HBM in fp32 (1,500 rows of 128,256 without alternatives: 125 us, 6.2
 // TB/s) and by instructions in 16 bits (some ten per logit, one for the special

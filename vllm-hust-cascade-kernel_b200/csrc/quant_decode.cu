@@ -26,13 +26,13 @@
 //
 // A warp has one kv head's rows, their softmax and output, over a run of 32-token
 // tiles; the warps of up to eight heads share the tiles' ring, which the first of
-// them keeps filled by TMA. The place of a token in the MMA's rows (first_token, value_token)
+// them keeps filled by TMA. The place of a token in the MMA's rows (Places)
 // keeps every shared-memory load of 80-byte rows free of bank conflicts.
 // The running maxima move only when a score exceeds its row's by more than 2^8.
 //
-// 8 kv heads x 4 query heads: 128 requests of 1,200 to 7,800 tokens (788 MB) 165 us,
+// 8 kv heads x 8 query heads: 128 requests of 1,500 to 8,200 tokens (798 MB) 166 us,
 // 4.8 TB/s; 149 without the arithmetic, of which 8 for the start (lengths, run, page
-// ids, first tile) and 4 for the merge. One request of 900 tokens 13.9 us.
+// ids, first tile) and 4 for the merge. One request of 900 tokens 14.3 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -673,9 +673,9 @@ cudaError_t launch(const QuantDecodeLaunch& p, void* workspace, cudaStream_t str
 // Blocks of 8 query rows per warp: as a request has rows (known from the shapes: the mean, with lengths on the device).
 // Unpacking, most of a block's some 330 instructions per 16 tokens, is shared by a warp's blocks. More than four would
 // take a second walk over the tokens, and go to the 256-row blocks of quant_tiles.cu (0). Both ways, 8 kv heads: 96 requests
-// over 4,000 tokens with 32 rows 301 us here against 537, with 36 rows 537 (in two walks) against 538, with 64 rows 559
-// against 545, with 128 rows 1,035 against 562; one request over 32,768 tokens with 32 rows 54 against 60, with 36 67
-// against 57, with 128 112 against 62.
+// over 4,000 tokens with 32 rows 306 us here against 519, with 36 rows 537 (in two walks) against 519, with 64 rows 559
+// against 527, with 128 rows 1,035 against 544; one request over 32,768 tokens with 32 rows 54 against 58, with 36 67
+// against 56, with 128 112 against 62.
 int row_blocks(const QuantDecodeLaunch& p) {
   const int64_t rows = (p.num_tokens * p.group + p.batch - 1) / p.batch;
   return rows <= 32 ? static_cast<int>((rows + 7) / 8) : 0;

@@ -4,7 +4,7 @@
 // behind.
 //
 // A block of 256 query rows (token and head of the group, in that order) of one
-// request and kv head are two tiles of 128 that share the unpacked tokens, 128 at a
+// request and kv head are two tiles of 128 that share the unpacked tokens, 64 at a
 // time. Keys stay exact: with a group's centre c and scale s a value is
 // (code - 8) s + s / 2 + c, and s is split in two, s = s1 + s2, of 7 and 4 significant
 // bits, so that the whole numbers code - 8 times s1 and s2 are fp16 numbers for every s
@@ -24,11 +24,11 @@
 // A CTA takes an equal run of steps over the units (request, block) of one kv head;
 // what run boundaries cut is merged by quant_combine_kernel.
 //
-// Measured: 2,048 query tokens x 32 heads over 16,384 tokens 746 us, 691 TFLOP/s of the
-// formula's products (17 columns of 16 are issued for its 8 in the scores). The issuing
-// warp is busy throughout: a step's products alone take some 650 cycles of a tile's
-// 725. In place of this: two issuing warps 836 us, two threads per row 800,
-// a quarter of the exponentials as polynomials 775.
+// Measured: 2,048 query tokens x 32 heads over 16,384 tokens 740 us, 697 TFLOP/s of the
+// formula's products (17 columns of 16 are issued for its 8 in the scores); some 790 us
+// at the power limit. The issuing warp is busy throughout: a step's products alone take
+// some 650 cycles of a tile's 725. In place of this: two issuing warps 836 us (for 746),
+// two threads per row 800, a quarter of the exponentials as polynomials 775.
 #include <algorithm>
 #include <cstddef>
 
