@@ -245,3 +245,12 @@ def test_write_with_every_scale():
     Hh.ops().cascade_quant_write(x, x.flip(0), kc, vc, torch.arange(T, device="cuda"))
     want = Q.pack(x)
     assert torch.equal(kc.view(-1, 1, 80)[:T].cpu(), want) and torch.equal(vc.view(-1, 1, 80)[:T].cpu(), want.flip(0))
+
+
+@pytest.mark.parametrize("KVH,q_len", [(300, 1), (300, 40), (1200, 1)])
+def test_more_kv_heads_than_sms(KVH, q_len):
+    Hh.need_cuda()
+    args = _inputs([70, 5], [q_len] * 2, KVH, 1, 16, seed=71)
+    got = Hh.ops().cascade_quant_decode(*args, q_len, SCALE, True)
+    _close(got, args, True)
+    assert Hh.capi().device_error() == 0

@@ -291,6 +291,7 @@ inline size_t quant_info_bytes(const QuantDecodeLaunch& p) {
   return (static_cast<size_t>(p.num_tokens) * p.num_heads * sizeof(int32_t) + 255) / 256 * 256;
 }
 inline size_t quant_partial_bytes(const QuantDecodeLaunch& p, int runs, int block_rows) {
+  if (runs == 1) return quant_info_bytes(p);  // (no unit is cut)
   return quant_info_bytes(p) + static_cast<size_t>(runs) * 2 * p.kv_heads * block_rows * (kHeadDim + 1) * sizeof(float);
 }
 inline QuantPartials quant_partials(const QuantDecodeLaunch& p, int runs, int block_rows, void* workspace) {
