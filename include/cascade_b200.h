@@ -476,7 +476,7 @@ CASCADE_API int cascade_quant_read(const void *key_cache, const void *value_cach
  * and more may, too).
  *   query  [num_tokens, num_heads, 128] in `dtype`, contiguous, 16-byte aligned
  * The other fields, the lengths and the block ids are as in cascade_latent_attn_t.
- * The limit of the kernels' bounded waits is 100 ms and, with many query rows, 4 us
+ * The limit of the kernels' bounded waits is 100 ms and, with many query rows, 8 us
  * per 64 tokens that a CTA reads and 2 us per request. */
 typedef struct cascade_quant_attn {
   const void *query;

@@ -12,9 +12,11 @@
 // codes, and a shift per eight. The term of centres and scales is one more product
 // of 16 columns: (c, s) of four groups against sum q and -7.5 sum q, each as two
 // fp16 numbers. fp32 holds every sum. (mma.sync aligns products as if a subnormal
-// operand were 2^-14: where all of a key's centres and scales are that small, sums lose
-// bits, at 2^-24 a score 2^-18 of its sum |q k|. As tf32 products they would not:
-// 128 x 64 heads 169 us for 166, 96 x 16 rows over 4,000 tokens 180 for 172.)
+// operand were 2^-14. So the codes' sums keep some 2^-22 of sum |q k| with fp16 queries: a
+// log-sum-exp is 1.4e-7 to 1.1e-6 of its size off, 3e-8 to 2e-7 as fp32 products; with bf16
+// queries 6e-8 to 3e-7. And where all of a key's centres and scales are that small, at
+// 2^-24 a score is 2^-18 of it off. As tf32 products those would not be: 128 x 64 heads 169
+// us for 166, 96 x 16 rows over 4,000 tokens 180 for 172.)
 // Values are converted, (code - 7.5) s + c in one fused multiply-add, rounded to
 // fp16, as P is: fp16 holds 2^-11 of both where bf16 would hold 2^-8.
 //

@@ -145,8 +145,9 @@ __global__ void __launch_bounds__(kThreads, 1) quant_tiles_kernel(const __grid_c
     if (lane == 0) {
       aux->run = r;
       // The second tile waits while units without rows for it are worked on, all of the run perhaps: 1.6 us a step
-      // (measured); requests without query tokens are passed by one after the other.
-      const uint64_t us = p.wait_limit_us ? p.wait_limit_us : kWaitLimitNs / 1000 + 4 * (r.end - r.begin) + 2ull * p.batch;
+      // (measured), and as long again or twice if NaN values are looked for; requests without query tokens are passed by one after
+      // the other.
+      const uint64_t us = p.wait_limit_us ? p.wait_limit_us : kWaitLimitNs / 1000 + 8 * (r.end - r.begin) + 2ull * p.batch;
       cta_wait_init(us * 1000);
     }
   }
